@@ -166,6 +166,84 @@ long long qwa_kv_packed_bytes(int kvt, int n_pos);
 int qwa_kv_pack(const qwa_kv_layer* kv, int kvt, int n_pos, void* dst, void* stream);
 int qwa_kv_unpack(const void* src, const qwa_kv_layer* kv, int kvt, int n_pos, void* stream);
 
+/* ---- Batches of sequences over a paged cache (no counterpart in the reference, which serves one sequence) ---------- */
+
+/* A page is `page` consecutive positions of a KV layer, all 4 KV heads, K and V and their scales: page p is positions
+ * [p * page, (p + 1) * page) of a qwa_kv_layer of capacity >= n_pages * page, the pool.  One set of page tables serves
+ * the pools of every layer.  Position j of sequence s is pool position table[s * ld + j / page] * page + j % page.
+ * All arrays are device memory and are read when the call's kernels run, so a captured graph follows them.
+ * page: a power of two, 16 .. 1024.  A sequence holds the first ceil(len / page) entries of its row; entries past those
+ * are never read.  ref counts the entries that hold a page; 0 means free.  An empty set of tables has len and ref 0. */
+typedef struct {
+    int* table;  /* [n_seq][ld] */
+    int* len;    /* [n_seq] positions held */
+    int* ref;    /* [n_pages] */
+    int n_seq, ld, n_pages, page;
+} qwa_kv_pages;
+
+#define QWA_PAGES_MAXN 1024 /* requests per call of the page operators, sequences per batch call */
+#define QWA_PAGES_MAXL 32   /* layers per call */
+
+/* Bytes of the `work` buffer of the page operators on these tables (device memory, 16-byte aligned; 0: invalid tables).
+ * Calls that may run at the same time need a buffer each. */
+size_t qwa_kv_pages_work_bytes(const qwa_kv_pages* p);
+
+/* Room for add[i] more positions of sequence seqs[i] (device arrays of n entries): len grows by add[i], and the pages
+ * that its new positions reach are taken from the free ones, lowest first, request by request.  A partly filled last
+ * page that other sequences hold too is replaced by a copy first, in every layer of `layers` (host array of n_layers
+ * pools of type kvt), since the new positions would be written into it; the last of its holders keeps the page.
+ * All or nothing: *status (device) becomes 0 when done; the number of missing pages when the free pages do not suffice;
+ * -(i + 1) when request i is invalid (no such sequence, named before, add < 0, past ld * page positions).  In the last
+ * two cases nothing is changed.  The new positions hold old bytes until a prep or an append writes them. */
+int qwa_kv_pages_extend(const qwa_kv_pages* p, const int* seqs, const int* add, int n, const qwa_kv_layer* layers,
+                        int n_layers, int kvt, int* status, void* work, void* stream);
+
+/* Sequence dst[i] becomes a fork of sequence src[i], all at once (every request sees the tables as they were before the
+ * call, so beams may be permuted): it gives back its own pages and holds src[i]'s, which are shared, not copied.
+ * src[i] < 0 leaves dst[i] empty.  A request whose src or dst is no sequence is ignored; of several with the same dst
+ * the last one counts. */
+int qwa_kv_pages_fork(const qwa_kv_pages* p, const int* src, const int* dst, int n, void* work, void* stream);
+
+/* Sequence seqs[i] keeps its first lens[i] positions (lens NULL: none, which frees it) and gives back the pages past
+ * them.  A request that names no sequence, or a length outside [0, len], is ignored; of several for one sequence the
+ * last one counts. */
+int qwa_kv_pages_trim(const qwa_kv_pages* p, const int* seqs, const int* lens, int n, void* stream);
+
+/* Moves the pages in use to the front of the pool: afterwards they are pages 0 .. *n_live - 1 (n_live: device).  The
+ * pages below that bound stay; the i-th page in use above it moves to the i-th free one below it, in every layer, and
+ * every sequence's table follows. */
+int qwa_kv_pages_compact(const qwa_kv_pages* p, const qwa_kv_layer* layers, int n_layers, int kvt, int* n_live,
+                         void* work, void* stream);
+
+/* qwa_attn_prep_multi for a batch: row r = b * nq + t of qg / k / v / q_out / gate belongs to query t of batch row b,
+ * whose sequence is seqs[b] (device; NULL: b) and whose position is len - nq + t, the last nq positions that the
+ * sequence holds (after qwa_kv_pages_extend).  The rotary position is that plus rope_off[b] (device; NULL: 0).  K / V
+ * rows are appended there; a row whose position is negative, or whose page is none of the pool's, is not stored.  A
+ * sequence named by several batch rows gets the rows of the last.  n <= QWA_PAGES_MAXN, nq 1..8.  Every buffer
+ * 16-byte aligned. */
+int qwa_attn_prep_batch(const float* qg, const float* k, const float* v, const float* q_norm, const float* k_norm,
+                        const qwa_kv_pages* p, const int* seqs, int n, int nq, const int* rope_off, float theta,
+                        float eps, int kvt, const qwa_kv_layer* kv, float* q_out, float* gate, void* stream);
+
+/* Bytes of the `work` buffer of qwa_attn_decode_batch (0: invalid arguments). */
+size_t qwa_attn_batch_work_bytes(int n, int nq, int n_shared, int max_len);
+
+/* Attention of n sequences with nq (1..8) queries each over a paged cache: batch row b is sequence seqs[b] (device;
+ * NULL: b), query t of it sees positions [0, len - nq + t].  q, gate [n * nq][24][256]; out16: output * sigmoid(gate)
+ * as fp16 bits [n * nq][6144] (the input of the output projection's GEMM), optional ActQ8 rows (of the fp32 values, for
+ * the GEMV).  fp16 MFMA, fp32 accumulation and softmax.
+ * n_shared: the batch rows have their first n_shared positions in common (forks of one prompt; 0: nothing).  Their keys
+ * are read once for all rows, through the table of the longest row (the first of those); a shorter row sees as many of
+ * them as it has positions.
+ * max_len >= n_shared bounds every row's len: positions from max_len on are not seen.
+ * A row that sees no position (an empty or unknown sequence, a query before the first position) gets zeros; positions
+ * whose page is none of the pool's are not seen.  Pool bytes past a sequence's last position are never used.  n <=
+ * QWA_PAGES_MAXN; q, gate, out16, work and the pool 16-byte aligned; work of at least qwa_attn_batch_work_bytes bytes,
+ * not shared with a call that may run at the same time. */
+int qwa_attn_decode_batch(const float* q, const float* gate, const qwa_kv_layer* kv, int kvt, const qwa_kv_pages* p,
+                          const int* seqs, int n, int nq, int n_shared, int max_len, uint16_t* out16,
+                          const qwa_act_q8* oq, void* work, size_t work_bytes, void* stream);
+
 /* ---- Gated DeltaNet (the recurrent token mixer of the other layers) ---------------------------------------------- */
 
 /* New tokens per qwa_deltanet_multi call (the reference's DN_MAXN = Engine::MAX_BATCH, src/cuda/ops.cu:148). */

@@ -19,7 +19,7 @@ LIB = os.path.join(OUT_DIR, "libqwattn.so")
 ARCH = "gfx950"
 
 SOURCES = ["capi.hip", "kv_append.hip", "attn_decode.hip", "attn_decode_ilp.hip", "attn_simple.hip", "attn_prefill.hip",
-           "deltanet.hip", "deltanet_rows.hip", "gemv.hip", "gemv_mc.hip", "gemm.cpp"]
+           "attn_batch.hip", "kv_pages.hip", "deltanet.hip", "deltanet_rows.hip", "gemv.hip", "gemv_mc.hip", "gemm.cpp"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",

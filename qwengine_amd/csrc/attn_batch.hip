@@ -1,0 +1,461 @@
+// Decode attention of a batch of sequences over a paged cache, the shared prefix read once (gfx950).
+//
+// For row r = (token, head) with q_r, and its keys K_j, V_j:  out = sum_j exp(s_j - m) V_j / sum_j exp(s_j - m) *
+// sigmoid(gate), s_j = q_r . K_j / 16.  The sum splits over any partition of the keys into partial states (m, l, O), so the
+// positions that all sequences share are worked on for the rows of all sequences together, those of its own for each
+// sequence by itself, both in ranges of fixed length (batch_plan.hpp), and k_bt_combine joins a row's states in a fixed
+// order.
+//  * A workgroup has one KV head and up to BT_MAXRT 16-row tiles (row 6 * token + head of that KV head); its waves take the
+//    tiles of its key range in turn, each with its own running maximum, sum and O, and merge at the end through LDS.
+//  * Pages are multiples of 16 positions and tiles start at multiples of 16, so each 16 keys lie in one page: a tile's page
+//    numbers are wave-uniform scalar loads, one tile ahead.
+//  * S^T = K Q^T and O^T += V^T P^T on fp16 MFMA with fp32 accumulation.  A lane loads 64 dims of one key and 16 dims of the
+//    keys whose probabilities it holds straight into registers in operand order and dequantizes there (kv_operands.hpp);
+//    the next tile's K loads go out when the scores are done, its V loads when P V is.
+// Roundings below 32 bits: Q / 16, the dequantized K and V, and the probabilities are fp16 (2^-12 relative each, random in
+// sign, as in the prefill), the output is fp16.
+#include "batch_plan.hpp"
+#include "kv_operands.hpp"
+#include "launch.hpp"
+
+namespace qwa {
+
+constexpr float BT_LOG2E = 1.4426950408889634f;
+constexpr float BT_RESCALE = 8.0f;  // the running maximum moves only when a score exceeds it by this (natural-log units)
+
+size_t batch_work_bytes(int n, int nq, int n_shared, int max_len) { return batch_bytes(n, nq, n_shared, max_len); }
+
+__device__ __forceinline__ f4 bt_mfma16k16(h4 a, h4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+}
+
+// max / sum over the four lanes that hold one row (lane distances 16 and 32)
+__device__ __forceinline__ float bt_row_max(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float bt_row_sum(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+struct BatchArgs {
+    const float* q;
+    const int* seqs;
+    float* part_o;    // [slot][row][256], row = token * NH + head
+    float2* part_ml;  // [slot][row] (m, l)
+    int n, nq, n_shared, max_len;
+};
+
+// positions of batch row b, cut to max_len; 0 for an unknown sequence
+__device__ __forceinline__ int bt_seq(const BatchArgs& a, int b) { return a.seqs ? a.seqs[b] : b; }
+__device__ __forceinline__ int bt_len(const BatchArgs& a, const qwa_kv_pages& p, int b) {
+    const int s = bt_seq(a, b);
+    return s >= 0 && s < p.n_seq ? min(max(p.len[s], 0), a.max_len) : 0;
+}
+
+// the longest batch row, the first of those (wave-uniform)
+__device__ __forceinline__ int bt_longest(const BatchArgs& a, const qwa_kv_pages& p, int lane) {
+    int m = -1, b = 0;
+    for (int j = lane; j < a.n; j += 64) {
+        const int x = bt_len(a, p, j);
+        if (x > m) m = x, b = j;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int om = __shfl_xor(m, o, 64), ob = __shfl_xor(b, o, 64);
+        if (om > m || (om == m && ob < b)) m = om, b = ob;
+    }
+    return __builtin_amdgcn_readfirstlane(b);
+}
+
+template <int KVT, int RT>
+struct BtCfg {
+    static constexpr int KT = KVT == QWA_KV_F16 ? 1 : 2;  // 16-key groups of a tile
+    static constexpr int WPE = RT == 1 ? 2 : 1;           // waves per SIMD that the registers allow
+};
+
+// One workgroup: rows [row0, rows) of KV head g (rows in units 6 * token + head), keys [k0, k1) of the sequence whose table
+// row is `table`, positions below lo excluded, partial states to slot `slot`.
+template <int KVT, int RT>
+__device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64], const BatchArgs& a,
+                                        const qwa_kv_layer& kv, const qwa_kv_pages& p, const int* __restrict__ table,
+                                        int row0, int rows, int g, int k0, int k1, int lo, int slot) {
+    constexpr int KT = BtCfg<KVT, RT>::KT, VB = value_bytes(KVT), TILE = 16 * KT;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const int i16 = lane & 15, lg = lane >> 4;
+    const uint8_t* const kh = kv.k + (size_t)g * kv.capacity * VB;
+    const uint8_t* const vh = kv.v + (size_t)g * kv.capacity * VB;
+    const uint16_t* const ksh = KVT == QWA_KV_F16 ? nullptr : kv.ks + (size_t)g * kv.capacity * 8;
+    const uint16_t* const vsh = KVT == QWA_KV_F16 ? nullptr : kv.vs + (size_t)g * kv.capacity * 8;
+
+    // rows of this lane: Q / 16 as the B operand, keys below vis are seen
+    h8 qb[RT][8];
+    int vis[RT], vmin = k1;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int r = row0 + 16 * rt + i16, tok = r / GRP;
+        const bool valid = r < rows;
+        vis[rt] = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, k1) : 0;
+        if (valid) vmin = min(vmin, vis[rt]);
+        const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + 64 * lg;
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            const float4 x0 = *reinterpret_cast<const float4*>(qrow + 8 * s);
+            const float4 x1 = *reinterpret_cast<const float4*>(qrow + 8 * s + 4);
+            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                qb[rt][s][j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
+        }
+    }
+    // (uniform: the least over the 16 lanes that hold different rows)
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
+    vmin = __builtin_amdgcn_readfirstlane(vmin);
+
+    f4 o[RT][16];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // the pool position of 16 keys from kb on, or -1: past the range, or in no page of the pool
+    auto place = [&](int kb) {
+        if (kb >= k1) return -1;
+        const int pg = table[kb / p.page];
+        return (unsigned)pg < (unsigned)p.n_pages ? pg * p.page + (kb & (p.page - 1)) : -1;
+    };
+    KRaw<KVT> kr[KT];
+    VRaw<KVT> vr[4 * KT];
+    // key rows past the range re-read its last one (their probabilities are exact zeros, so what they hold must be finite:
+    // a stale row need not be), groups without a place are zeros
+    auto load_ks = [&](const int* at, int kb) {
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) {
+            const int last = k1 - 1 - (kb + 16 * kt);
+            const bool live = at[kt] >= 0;
+            const int row = min(i16, last);
+            if (live) {
+                const uint8_t* src = kh + (size_t)at[kt] * VB + (row * VB + (VB / 4) * lg);
+#pragma unroll
+                for (int i = 0; i < VB / 64; i++) {
+                    const uint4 u = ld16(src + 16 * i);
+                    kr[kt].w[4 * i] = u.x; kr[kt].w[4 * i + 1] = u.y; kr[kt].w[4 * i + 2] = u.z; kr[kt].w[4 * i + 3] = u.w;
+                }
+                if constexpr (KVT != QWA_KV_F16)
+                    kr[kt].sc = reinterpret_cast<const uint32_t*>(ksh + (size_t)at[kt] * 8)[row * 4 + lg];
+            } else {
+#pragma unroll
+                for (int i = 0; i < VB / 16; i++) kr[kt].w[i] = 0;
+                kr[kt].sc = 0;
+            }
+        }
+    };
+    auto load_vs = [&](const int* at, int kb) {
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) {
+            const int last = k1 - 1 - (kb + 16 * kt);
+            const bool live = at[kt] >= 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                VRaw<KVT>& x = vr[4 * kt + j];
+                constexpr int NW = sizeof(x.w) / 4;
+                const int row = min(4 * lg + j, last);
+                if (live) {
+                    const uint8_t* src = vh + (size_t)at[kt] * VB + (row * VB + (VB / 16) * i16);
+                    if constexpr (NW == 2) {
+                        const uint2 u = ld8(src);
+                        x.w[0] = u.x; x.w[1] = u.y;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NW / 4; i++) {
+                            const uint4 u = ld16(src + 16 * i);
+                            x.w[4 * i] = u.x; x.w[4 * i + 1] = u.y; x.w[4 * i + 2] = u.z; x.w[4 * i + 3] = u.w;
+                        }
+                    }
+                    x.sc = KVT == QWA_KV_F16 ? 0u : vsh[(size_t)at[kt] * 8 + (row * 8 + (i16 >> 1))];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NW; i++) x.w[i] = 0;
+                    x.sc = 0;
+                }
+            }
+        }
+    };
+
+    int kb = k0 + TILE * wave;
+    int at[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++) at[kt] = place(kb + 16 * kt);
+    if (kb < k1) {
+        load_ks(at, kb);
+        load_vs(at, kb);
+    }
+    for (; kb < k1; kb += TILE * BT_WAVES) {
+        const int nb = kb + TILE * BT_WAVES;
+        int nat[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) nat[kt] = place(nb + 16 * kt);
+        f4 S[RT][KT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++) S[rt][kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < 8; s++)
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++) {
+                const h8 ka = k_operand<KVT>(kr[kt], s);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) S[rt][kt] = mfma16(ka, qb[rt][s], S[rt][kt]);
+            }
+        if (nb < k1) load_ks(nat, nb);
+
+        // online softmax: a lane holds keys kb + 16 kt + 4 lg + i of row i16
+        bool masked = kb < lo || kb + TILE > vmin;
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) masked |= at[kt] < 0;
+        h8 p8[RT];
+        float cr[RT];
+        bool moved = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            if (masked) {
+#pragma unroll
+                for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int key = kb + 16 * kt + 4 * lg + i;
+                        S[rt][kt][i] = at[kt] >= 0 && key >= lo && key < vis[rt] ? S[rt][kt][i] : -INFINITY;
+                    }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, S[rt][kt][i]);
+            mx = bt_row_max(mx);
+            const float mn = mx > m[rt] + BT_RESCALE ? mx : m[rt];
+            const float msl = (mn == -INFINITY ? 0.0f : mn) * BT_LOG2E;  // a row that saw nothing keeps l = 0, O = 0
+            cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] * BT_LOG2E - msl);
+            float rs = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) p8[rt][j] = (_Float16)0.0f;
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const _Float16 e = (_Float16)fast_exp2(fmaf(S[rt][kt][i], BT_LOG2E, -msl));
+                    p8[rt][4 * kt + i] = e;
+                    rs += (float)e;  // the weights that P V applies
+                }
+            l[rt] = l[rt] * cr[rt] + rs;
+            m[rt] = mn;
+            moved |= cr[rt] != 1.0f;
+        }
+        if (__any(moved)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int dt = 0; dt < 16; dt++) o[rt][dt] *= cr[rt];
+        }
+
+        // O^T += V^T P^T: output tile dt holds dim 16 i16 + dt
+        constexpr int NW = sizeof(vr[0].w) / 4, DPW = 16 / NW;
+#pragma unroll
+        for (int wi = 0; wi < NW; wi++) {
+            uint32_t w[2 * KT][DPW];
+#pragma unroll
+            for (int h = 0; h < 2 * KT; h++)
+                v_pair_words<KVT, 1>(&vr[2 * h].w[wi], &vr[2 * h + 1].w[wi], vr[2 * h].sc, vr[2 * h + 1].sc, w[h]);
+#pragma unroll
+            for (int d = 0; d < DPW; d++)
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    f4& acc = o[rt][wi * DPW + d];
+                    if constexpr (KT == 2)
+                        acc = mfma16(make_h8(w[0][d], w[1][d], w[2][d], w[3][d]), p8[rt], acc);
+                    else
+                        acc = bt_mfma16k16(make_h4(w[0][d], w[1][d]), h4{p8[rt][0], p8[rt][1], p8[rt][2], p8[rt][3]}, acc);
+                }
+        }
+        if (nb < k1) load_vs(nat, nb);
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) at[kt] = nat[kt];
+    }
+
+    // the waves' states, joined: wave w takes output tiles 4 w .. 4 w + 3 (dims 16 (4 lg + i) + 4 w .. + 3 of the row)
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const float lt = bt_row_sum(l[rt]);
+        __syncthreads();  // the previous tile's states are read out
+#pragma unroll
+        for (int dt = 0; dt < 16; dt++) s_o[wave][dt][lane] = o[rt][dt];
+        s_ml[wave][0][lane] = m[rt];
+        s_ml[wave][1][lane] = lt;
+        __syncthreads();
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < BT_WAVES; w++) M = fmaxf(M, s_ml[w][0][lane]);
+        f4 acc[4] = {};
+#pragma unroll
+        for (int w = 0; w < BT_WAVES; w++) {
+            const float mw = s_ml[w][0][lane], lw = s_ml[w][1][lane];
+            const float f = lw == 0.0f ? 0.0f : fast_exp2((mw - M) * BT_LOG2E);  // (lw: NaN scores stay NaN)
+            L = fmaf(f, lw, L);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const f4 x = s_o[w][4 * wave + t][lane];
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[t][i] = fmaf(f, x[i], acc[t][i]);
+            }
+        }
+        const int r = row0 + 16 * rt + i16;
+        if (r < rows) {
+            const size_t rec = ((size_t)slot * a.n * a.nq + r / GRP) * NH + g * GRP + r % GRP;
+            if (wave == 0 && lg == 0) a.part_ml[rec] = make_float2(M, L);
+            float* dst = a.part_o + rec * HD + 4 * wave;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<float4*>(dst + 16 * (4 * lg + i)) = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
+        }
+    }
+}
+
+// the shared positions: workgroup = (row group, key range, KV head); slots 0 .. ns - 1
+template <int KVT, int RT>
+__global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(BtCfg<KVT, RT>::WPE)))
+k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len) {
+    __shared__ f4 s_o[BT_WAVES][16][64];
+    __shared__ float s_ml[BT_WAVES][2][64];
+    const int pairs = ns * NKV, grp = blockIdx.x / pairs, pr = blockIdx.x % pairs, g = pr % NKV, sp = pr / NKV;
+    const int b = bt_longest(a, p, threadIdx.x & 63);
+    const int k1 = min(min((sp + 1) * len, a.n_shared), bt_len(a, p, b));
+    const int seq = bt_seq(a, b);
+    const int* table = p.table + (seq >= 0 && seq < p.n_seq ? (size_t)seq * p.ld : 0);
+    bt_body<KVT, RT>(s_o, s_ml, a, kv, p, table, grp * 16 * RT, a.n * a.nq * GRP, g, sp * len, k1, 0, sp);
+}
+
+// each sequence's own positions: workgroup = (batch row, key range, KV head); slots first .. first + ns - 1
+template <int KVT, int RT>
+__global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(BtCfg<KVT, RT>::WPE)))
+k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len, int first) {
+    __shared__ f4 s_o[BT_WAVES][16][64];
+    __shared__ float s_ml[BT_WAVES][2][64];
+    const int pairs = ns * NKV, b = blockIdx.x / pairs, pr = blockIdx.x % pairs, g = pr % NKV, sp = pr / NKV;
+    const int begin = a.n_shared + sp * len, k1 = min(begin + len, bt_len(a, p, b));
+    if (begin >= k1) return;  // k_bt_combine does not read this slot
+    // (tiles start at multiples of 16; positions before `begin` are masked)
+    bt_body<KVT, RT>(s_o, s_ml, a, kv, p, p.table + (size_t)bt_seq(a, b) * p.ld, b * a.nq * GRP, (b + 1) * a.nq * GRP, g,
+                     begin & ~15, k1, begin, first + sp);
+}
+
+// Joins a row's partial states in slot order, gates, rounds: one wave per row (token * NH + head), 4 dims per lane.
+__global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p, const float* __restrict__ gate,
+                                                    int ns_shared, int ns_own, int len_own,
+                                                    uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int nrows = a.n * a.nq * NH;
+    if (row >= nrows) return;
+    const int mine = bt_len(a, p, row / NH / a.nq) - a.n_shared;  // own positions
+    const int ns = ns_shared + (mine > 0 ? min(ns_own, (mine + len_own - 1) / len_own) : 0);
+    float M = -INFINITY;
+    for (int s = lane; s < ns; s += 64) {
+        const float2 ml = a.part_ml[(size_t)s * nrows + row];
+        M = fmaxf(M, ml.y > 0.0f || ml.y != ml.y ? ml.x : -INFINITY);
+    }
+    M = wave_max(M);
+    float L = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s = 0; s < ns; s++) {
+        const float2 ml = a.part_ml[(size_t)s * nrows + row];
+        const float4 x = *reinterpret_cast<const float4*>(a.part_o + ((size_t)s * nrows + row) * HD + 4 * lane);
+        const float f = ml.y == 0.0f ? 0.0f : fast_exp2((ml.x - M) * BT_LOG2E);
+        L = fmaf(f, ml.y, L);
+        acc.x = fmaf(f, x.x, acc.x);
+        acc.y = fmaf(f, x.y, acc.y);
+        acc.z = fmaf(f, x.z, acc.z);
+        acc.w = fmaf(f, x.w, acc.w);
+    }
+    const float4 gv = *reinterpret_cast<const float4*>(gate + (size_t)row * HD + 4 * lane);
+    float v[4] = {acc.x / L * sigmoid(gv.x), acc.y / L * sigmoid(gv.y), acc.z / L * sigmoid(gv.z), acc.w / L * sigmoid(gv.w)};
+    if (L == 0.0f) v[0] = v[1] = v[2] = v[3] = 0.0f;  // no key was seen
+    *reinterpret_cast<uint2*>(out16 + (size_t)row * HD + 4 * lane) =
+        make_uint2((uint32_t)f2h_bits(v[0]) | ((uint32_t)f2h_bits(v[1]) << 16),
+                   (uint32_t)f2h_bits(v[2]) | ((uint32_t)f2h_bits(v[3]) << 16));
+    if (do_q) {
+        // ActQ8 of 32 values in 8 lanes: d = amax / 127, q = round-half-even(v / d), s = d * sum(q)
+        auto max8 = [](float x) {
+            x = fmaxf(x, row_move<0xB1>(x));
+            x = fmaxf(x, row_move<0x4E>(x));
+            return fmaxf(x, row_move<0x141>(x));
+        };
+        auto sum8 = [](float x) {
+            x += row_move<0xB1>(x);
+            x += row_move<0x4E>(x);
+            return x + row_move<0x141>(x);
+        };
+        const float d = max8(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])))) / 127.0f;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int qi = d > 0.0f ? (int)__builtin_rintf(v[j] / d) : 0;
+            oq.q[(size_t)row * HD + 4 * lane + j] = (int8_t)qi;
+            sum += (float)qi;
+        }
+        sum = sum8(sum);
+        if ((lane & 7) == 0) {
+            oq.d[(size_t)row * (HD / 32) + lane / 8] = d;
+            oq.s[(size_t)row * (HD / 32) + lane / 8] = d * sum;
+        }
+    }
+}
+
+template <int KVT>
+static void launch_ranges(const BatchArgs& a, const qwa_kv_layer& kv, const qwa_kv_pages& p, const BatchPlan& b,
+                          hipStream_t st) {
+    const dim3 block(64 * BT_WAVES);
+#define QWA_BT(K, RT, GRID, ...) hipLaunchKernelGGL((K<KVT, RT>), dim3(GRID), block, 0, st, a, kv, p, __VA_ARGS__)
+    if (b.ns_shared > 0) {
+        const int grid = b.groups * b.ns_shared * NKV;
+        if (b.rt_shared == 1) QWA_BT(k_bt_shared, 1, grid, b.ns_shared, b.len_shared);
+        else if (b.rt_shared == 2) QWA_BT(k_bt_shared, 2, grid, b.ns_shared, b.len_shared);
+        else QWA_BT(k_bt_shared, 3, grid, b.ns_shared, b.len_shared);
+    }
+    if (b.ns_own > 0) {
+        const int grid = a.n * b.ns_own * NKV;
+        if (b.rt_own == 1) QWA_BT(k_bt_own, 1, grid, b.ns_own, b.len_own, b.ns_shared);
+        else if (b.rt_own == 2) QWA_BT(k_bt_own, 2, grid, b.ns_own, b.len_own, b.ns_shared);
+        else QWA_BT(k_bt_own, 3, grid, b.ns_own, b.len_own, b.ns_shared);
+    }
+#undef QWA_BT
+}
+
+hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_layer& kv, int kvt, const qwa_kv_pages& p,
+                               const int* seqs, int n, int nq, int n_shared, int max_len, uint16_t* out16,
+                               const qwa_act_q8* oq, void* work, hipStream_t st) {
+    const BatchPlan b = batch_plan(n, nq, n_shared, max_len);
+    const size_t rows = (size_t)n * nq * NH;
+    float* o = static_cast<float*>(work);
+    const BatchArgs a{q, seqs, o, reinterpret_cast<float2*>(o + b.slots() * rows * HD), n, nq, n_shared, max_len};
+    switch (kvt) {
+        case QWA_KV_F16: launch_ranges<QWA_KV_F16>(a, kv, p, b, st); break;
+        case QWA_KV_Q8_0: launch_ranges<QWA_KV_Q8_0>(a, kv, p, b, st); break;
+        default: launch_ranges<QWA_KV_Q4_0>(a, kv, p, b, st); break;
+    }
+    const qwa_act_q8 act = oq ? *oq : qwa_act_q8{nullptr, nullptr, nullptr};
+    hipLaunchKernelGGL(k_bt_combine, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p, gate, b.ns_shared, b.ns_own,
+                       b.len_own, out16, act, oq != nullptr ? 1 : 0);
+    return hipGetLastError();
+}
+
+}  // namespace qwa

@@ -365,6 +365,151 @@ int qwa_kv_unpack(const void* src, const qwa_kv_layer* kv, int kvt, int n_pos, v
     return kv_move(kv, kvt, n_pos, static_cast<uint8_t*>(const_cast<void*>(src)), false, stream, "kv_unpack");
 }
 
+// ---- batches of sequences over a paged cache
+namespace {
+constexpr int PAGE_MIN = 16, PAGE_MAX = 1024;
+
+bool al16(const void* a) { return ((uintptr_t)a & 15) == 0; }
+
+bool pages_ok(const qwa_kv_pages* p) {
+    return p != nullptr && p->table && p->len && p->ref && p->n_seq > 0 && p->ld > 0 && p->n_pages > 0 &&
+           p->page >= PAGE_MIN && p->page <= PAGE_MAX && (p->page & (p->page - 1)) == 0;
+}
+
+int check_pages(const qwa_kv_pages* p, const char* fn) {
+    if (p == nullptr || !p->table || !p->len || !p->ref) return fail(QWA_ERR_INVALID, "%s: incomplete page tables", fn);
+    if (!pages_ok(p))
+        return fail(QWA_ERR_INVALID, "%s: page tables of %d x %d entries, %d pages of %d positions (a power of two, %d..%d)",
+                    fn, p->n_seq, p->ld, p->n_pages, p->page, PAGE_MIN, PAGE_MAX);
+    return QWA_OK;
+}
+
+int check_pool(const qwa_kv_layer* kv, int kvt, const qwa_kv_pages* p, const char* fn) {
+    int st;
+    if ((st = check_kv(kv, kvt, fn))) return st;
+    if ((long long)p->n_pages * p->page > kv->capacity)
+        return fail(QWA_ERR_RANGE, "%s: %d pages of %d positions in a layer of capacity %d", fn, p->n_pages, p->page,
+                    kv->capacity);
+    if (!al16(kv->k) || !al16(kv->v) || (kvt != QWA_KV_F16 && (!al16(kv->ks) || !al16(kv->vs))))
+        return fail(QWA_ERR_INVALID, "%s: pool not 16-byte aligned", fn);
+    return QWA_OK;
+}
+
+int check_layers(const qwa_kv_layer* layers, int n_layers, int kvt, const qwa_kv_pages* p, const char* fn) {
+    if (layers == nullptr || n_layers < 1 || n_layers > QWA_PAGES_MAXL)
+        return fail(QWA_ERR_INVALID, "%s: %d layers (1..%d)", fn, n_layers, QWA_PAGES_MAXL);
+    for (int i = 0; i < n_layers; i++)
+        if (int st = check_pool(layers + i, kvt, p, fn)) return st;
+    return QWA_OK;
+}
+
+int check_requests(int n, const char* fn) {
+    if (n < 0 || n > QWA_PAGES_MAXN) return fail(QWA_ERR_RANGE, "%s: %d requests (0..%d)", fn, n, QWA_PAGES_MAXN);
+    return QWA_OK;
+}
+
+int check_batch(const qwa_kv_pages* p, const int* seqs, int n, int nq, const char* fn) {
+    int st;
+    if ((st = check_pages(p, fn))) return st;
+    if (n < 1 || n > QWA_PAGES_MAXN) return fail(QWA_ERR_RANGE, "%s: %d sequences (1..%d)", fn, n, QWA_PAGES_MAXN);
+    if (nq < 1 || nq > qwa::MAXQ) return fail(QWA_ERR_INVALID, "%s: %d queries (1..%d)", fn, nq, qwa::MAXQ);
+    if (seqs == nullptr && n > p->n_seq)
+        return fail(QWA_ERR_RANGE, "%s: %d batch rows for %d sequences", fn, n, p->n_seq);
+    return QWA_OK;
+}
+}  // namespace
+
+size_t qwa_kv_pages_work_bytes(const qwa_kv_pages* p) { return pages_ok(p) ? qwa::pages_work_bytes(*p) : 0; }
+
+int qwa_kv_pages_extend(const qwa_kv_pages* p, const int* seqs, const int* add, int n, const qwa_kv_layer* layers,
+                        int n_layers, int kvt, int* status, void* work, void* stream) {
+    const char* fn = "kv_pages_extend";
+    int st;
+    if ((st = check_pages(p, fn)) || (st = check_requests(n, fn)) ||
+        (st = check_layers(layers, n_layers, kvt, p, fn)))
+        return st;
+    if (!status || !work || (n > 0 && (!seqs || !add))) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if (!al16(work)) return fail(QWA_ERR_INVALID, "%s: work not 16-byte aligned", fn);
+    return from_hip(qwa::launch_pages_extend(*p, seqs, add, n, layers, n_layers, kvt, status, work, as_stream(stream)), fn);
+}
+
+int qwa_kv_pages_fork(const qwa_kv_pages* p, const int* src, const int* dst, int n, void* work, void* stream) {
+    const char* fn = "kv_pages_fork";
+    int st;
+    if ((st = check_pages(p, fn)) || (st = check_requests(n, fn))) return st;
+    // (the work buffer stages a row per request)
+    if (n > p->n_seq) return fail(QWA_ERR_RANGE, "%s: %d requests for %d sequences", fn, n, p->n_seq);
+    if (n == 0) return QWA_OK;
+    if (!src || !dst || !work) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if (!al16(work)) return fail(QWA_ERR_INVALID, "%s: work not 16-byte aligned", fn);
+    return from_hip(qwa::launch_pages_fork(*p, src, dst, n, work, as_stream(stream)), fn);
+}
+
+int qwa_kv_pages_trim(const qwa_kv_pages* p, const int* seqs, const int* lens, int n, void* stream) {
+    const char* fn = "kv_pages_trim";
+    int st;
+    if ((st = check_pages(p, fn)) || (st = check_requests(n, fn))) return st;
+    if (n == 0) return QWA_OK;
+    if (!seqs) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    return from_hip(qwa::launch_pages_trim(*p, seqs, lens, n, as_stream(stream)), fn);
+}
+
+int qwa_kv_pages_compact(const qwa_kv_pages* p, const qwa_kv_layer* layers, int n_layers, int kvt, int* n_live,
+                         void* work, void* stream) {
+    const char* fn = "kv_pages_compact";
+    int st;
+    if ((st = check_pages(p, fn)) || (st = check_layers(layers, n_layers, kvt, p, fn))) return st;
+    if (!n_live || !work) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if (!al16(work)) return fail(QWA_ERR_INVALID, "%s: work not 16-byte aligned", fn);
+    return from_hip(qwa::launch_pages_compact(*p, layers, n_layers, kvt, n_live, work, as_stream(stream)), fn);
+}
+
+int qwa_attn_prep_batch(const float* qg, const float* k, const float* v, const float* q_norm, const float* k_norm,
+                        const qwa_kv_pages* p, const int* seqs, int n, int nq, const int* rope_off, float theta,
+                        float eps, int kvt, const qwa_kv_layer* kv, float* q_out, float* gate, void* stream) {
+    const char* fn = "attn_prep_batch";
+    int st;
+    if ((st = check_batch(p, seqs, n, nq, fn)) || (st = check_pool(kv, kvt, p, fn))) return st;
+    const void* const bufs[] = {qg, k, v, q_norm, k_norm, q_out, gate};
+    for (const void* b : bufs) {
+        if (!b) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+        if (!al16(b)) return fail(QWA_ERR_INVALID, "%s: buffer not 16-byte aligned", fn);
+    }
+    return from_hip(qwa::launch_prep_batch(qg, k, v, q_norm, k_norm, *p, seqs, n, nq, rope_off, theta, eps, kvt, *kv,
+                                           q_out, gate, as_stream(stream)),
+                    fn);
+}
+
+static bool batch_sizes_ok(int n, int nq, int n_shared, int max_len) {
+    return n >= 1 && n <= QWA_PAGES_MAXN && nq >= 1 && nq <= qwa::MAXQ && n_shared >= 0 && max_len >= 1 &&
+           n_shared <= max_len && max_len <= qwa::MAX_POS;
+}
+
+size_t qwa_attn_batch_work_bytes(int n, int nq, int n_shared, int max_len) {
+    return batch_sizes_ok(n, nq, n_shared, max_len) ? qwa::batch_work_bytes(n, nq, n_shared, max_len) : 0;
+}
+
+int qwa_attn_decode_batch(const float* q, const float* gate, const qwa_kv_layer* kv, int kvt, const qwa_kv_pages* p,
+                          const int* seqs, int n, int nq, int n_shared, int max_len, uint16_t* out16,
+                          const qwa_act_q8* oq, void* work, size_t work_bytes, void* stream) {
+    const char* fn = "attn_decode_batch";
+    int st;
+    if ((st = check_batch(p, seqs, n, nq, fn)) || (st = check_pool(kv, kvt, p, fn))) return st;
+    if (!batch_sizes_ok(n, nq, n_shared, max_len) || max_len > (long long)p->ld * p->page)
+        return fail(QWA_ERR_RANGE, "%s: n_shared %d, max_len %d (tables of %lld positions, at most %d)", fn, n_shared,
+                    max_len, (long long)p->ld * p->page, qwa::MAX_POS);
+    if (!q || !gate || !out16 || !work) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if (!al16(q) || !al16(gate) || !al16(out16) || !al16(work))
+        return fail(QWA_ERR_INVALID, "%s: buffer not 16-byte aligned", fn);
+    if (oq && (!oq->q || !oq->d || !oq->s)) return fail(QWA_ERR_INVALID, "%s: incomplete ActQ8 output", fn);
+    const size_t need = qwa::batch_work_bytes(n, nq, n_shared, max_len);
+    if (work_bytes < need)
+        return fail(QWA_ERR_RANGE, "%s: workspace of %zu bytes, the call needs %zu", fn, work_bytes, need);
+    return from_hip(qwa::launch_decode_batch(q, gate, *kv, kvt, *p, seqs, n, nq, n_shared, max_len, out16, oq, work,
+                                             as_stream(stream)),
+                    fn);
+}
+
 // ---- Gated DeltaNet
 namespace {
 int check_dn_params(const qwa_dn_params* p, const char* fn) {

@@ -343,6 +343,22 @@ __device__ __forceinline__ void quant_row_al(uint8_t* vals, uint16_t* scales, co
     }
 }
 
+// RMSNorm with weights wv and the rotation, for a row held by 32 lanes (lane l: elements 8 l .. 8 l + 7)
+__device__ __forceinline__ void norm_rope(float* x, const float* wv, const float* c, const float* sn, int l, float eps) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPL; j++) ss += x[j] * x[j];
+    const float rs = rsqrtf(half_sum(ss) / (float)HD + eps);
+#pragma unroll
+    for (int j = 0; j < VPL; j++) x[j] = x[j] * rs * wv[j];
+#pragma unroll
+    for (int j = 0; j < VPL; j++) {
+        const float y = xor4_low(x[j]);
+        const float lo = x[j] * c[j] - y * sn[j], hi = y * sn[j] + x[j] * c[j];
+        x[j] = l < 4 ? lo : l < 8 ? hi : x[j];
+    }
+}
+
 constexpr int PR_TASKS = NH / 2 + NKV / 2 + NKV / 2 + NH / 4;  // wave tasks per token
 template <int KVT>
 __global__ void __launch_bounds__(256) k_prep_rows_al(const float* __restrict__ qg, const float* __restrict__ k,
@@ -380,18 +396,7 @@ __global__ void __launch_bounds__(256) k_prep_rows_al(const float* __restrict__ 
             ld8(rope + (size_t)r * NROT + VPL * (l & 3), c);
             ld8(rope + (size_t)r * NROT + NROT / 2 + VPL * (l & 3), sn);
         }
-        float ss = 0.0f;
-#pragma unroll
-        for (int j = 0; j < VPL; j++) ss += x[j] * x[j];
-        const float rs = rsqrtf(half_sum(ss) / (float)HD + eps);
-#pragma unroll
-        for (int j = 0; j < VPL; j++) x[j] = x[j] * rs * wv[j];
-#pragma unroll
-        for (int j = 0; j < VPL; j++) {
-            const float y = xor4_low(x[j]);
-            const float lo = x[j] * c[j] - y * sn[j], hi = y * sn[j] + x[j] * c[j];
-            x[j] = l < 4 ? lo : l < 8 ? hi : x[j];
-        }
+        norm_rope(x, wv, c, sn, l, eps);
     }
     if (is_q) {
         float* dst = q_out + ((size_t)r * NH + h) * HD + VPL * l;
@@ -401,6 +406,75 @@ __global__ void __launch_bounds__(256) k_prep_rows_al(const float* __restrict__ 
         const size_t row = (size_t)h * kv.capacity + p0 + r;
         quant_row_al<KVT>((is_v ? kv.v : kv.k) + row * value_bytes(KVT),
                           KVT == QWA_KV_F16 ? nullptr : (is_v ? kv.vs : kv.ks) + row * 8, x, l);
+    }
+}
+
+// Batch form: the last nq positions of n sequences of a paged cache.  One workgroup per token (row b * nq + t at position
+// len - nq + t of sequence seqs[b]); the wave tasks are k_prep_rows_al's, the rotation's 32 cos / sin pairs are formed once
+// per token, in double (one lane per frequency), and shared through LDS.
+constexpr int PB_WAVES = 8;
+template <int KVT>
+__global__ void __launch_bounds__(64 * PB_WAVES) k_prep_batch(
+    const float* __restrict__ qg, const float* __restrict__ k, const float* __restrict__ v,
+    const float* __restrict__ qn_w, const float* __restrict__ kn_w, qwa_kv_pages pg, const int* __restrict__ seqs, int n,
+    int nq, const int* __restrict__ rope_off, float theta, float eps, qwa_kv_layer kv, float* __restrict__ q_out,
+    float* __restrict__ gate) {
+    __shared__ float s_cs[NROT];
+    const int r = blockIdx.x, b = r / nq, t = threadIdx.x, lane = t & 63, half = lane >> 5, l = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // the token's position, and its place in the pool (-1: not stored)
+    const int seq = seqs ? seqs[b] : b;
+    const bool known = seq >= 0 && seq < pg.n_seq;
+    const int pos = (known ? pg.len[seq] : 0) - nq + r % nq;
+    bool later = false;  // a later batch row names the same sequence
+    if (seqs)
+        for (int j = b + 1 + t; j < n; j += 64 * PB_WAVES) later |= seqs[j] == seq;
+    long long slot = -1;
+    if (known && pos >= 0 && pos / pg.page < pg.ld) {
+        const int page = pg.table[(size_t)seq * pg.ld + pos / pg.page];
+        if ((unsigned)page < (unsigned)pg.n_pages) slot = (long long)page * pg.page + pos % pg.page;
+    }
+    if (t < NROT / 2) rope_cs((double)pos + (rope_off ? rope_off[b] : 0), theta, t, &s_cs[t], &s_cs[t + NROT / 2]);
+    if (__syncthreads_or(later)) slot = -1;
+    auto ld8 = [](const float* p, float* x) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], c = reinterpret_cast<const float4*>(p)[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = c.x; x[5] = c.y; x[6] = c.z; x[7] = c.w;
+    };
+    for (int i = wave; i < PR_TASKS; i += PB_WAVES) {
+        if (i >= NH / 2 + NKV) {  // gates of 4 heads
+            const int h = 4 * (i - (NH / 2 + NKV));
+            float4 g[4];
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+                g[m] = *reinterpret_cast<const float4*>(qg + ((size_t)r * NH + h + m) * 2 * HD + HD + 4 * lane);
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+                *reinterpret_cast<float4*>(gate + ((size_t)r * NH + h + m) * HD + 4 * lane) = g[m];
+            continue;
+        }
+        float x[VPL];
+        const int h = 2 * (i < NH / 2 ? i : (i - NH / 2) % (NKV / 2)) + half;
+        const bool is_q = i < NH / 2, is_v = i >= NH / 2 + NKV / 2;
+        ld8(is_q ? qg + ((size_t)r * NH + h) * 2 * HD + VPL * l : (is_v ? v : k) + ((size_t)r * NKV + h) * HD + VPL * l, x);
+        if (!is_v) {
+            float c[VPL] = {}, sn[VPL] = {}, wv[VPL];
+            ld8((is_q ? qn_w : kn_w) + VPL * l, wv);
+            if (l < 8) {
+                ld8(s_cs + VPL * (l & 3), c);
+                ld8(s_cs + NROT / 2 + VPL * (l & 3), sn);
+            }
+            norm_rope(x, wv, c, sn, l, eps);
+        }
+        if (is_q) {
+            float* dst = q_out + ((size_t)r * NH + h) * HD + VPL * l;
+            reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else if (slot >= 0) {
+            const size_t row = (size_t)h * kv.capacity + slot;
+            quant_row_al<KVT>((is_v ? kv.v : kv.k) + row * value_bytes(KVT),
+                              KVT == QWA_KV_F16 ? nullptr : (is_v ? kv.vs : kv.ks) + row * 8, x, l);
+        }
     }
 }
 
@@ -464,6 +538,24 @@ hipError_t launch_prep_rows(const float* qg, const float* k, const float* v, con
     }
     hipLaunchKernelGGL(k_prep_rows, dim3(blocks_for((long long)B * SLOTS)), dim3(256), 0, st, qg, k, v, qn, kn, B, p0,
                        rope, eps, kvt, kv, q, gate);
+    return hipGetLastError();
+}
+
+hipError_t launch_prep_batch(const float* qg, const float* k, const float* v, const float* qn, const float* kn,
+                             const qwa_kv_pages& p, const int* seqs, int n, int nq, const int* rope_off, float theta,
+                             float eps, int kvt, const qwa_kv_layer& kv, float* q, float* gate, hipStream_t st) {
+    const dim3 grid(n * nq), block(64 * PB_WAVES);
+#define QWA_PREP_BATCH(T)                                                                                               \
+    case T:                                                                                                             \
+        hipLaunchKernelGGL(k_prep_batch<T>, grid, block, 0, st, qg, k, v, qn, kn, p, seqs, n, nq, rope_off, theta, eps, \
+                           kv, q, gate);                                                                                \
+        break
+    switch (kvt) {
+        QWA_PREP_BATCH(QWA_KV_F16);
+        QWA_PREP_BATCH(QWA_KV_Q8_0);
+        QWA_PREP_BATCH(QWA_KV_Q4_0);
+    }
+#undef QWA_PREP_BATCH
     return hipGetLastError();
 }
 

@@ -62,6 +62,25 @@ hipError_t launch_rope_table_pos(const int* pos3, int B, float theta, float* rop
 hipError_t launch_kv_append(const float* xk, const float* xv, int pos0, int n, int kvt, const qwa_kv_layer& kv,
                             hipStream_t st);
 
+hipError_t launch_prep_batch(const float* qg, const float* k, const float* v, const float* qn, const float* kn,
+                             const qwa_kv_pages& p, const int* seqs, int n, int nq, const int* rope_off, float theta,
+                             float eps, int kvt, const qwa_kv_layer& kv, float* q, float* gate, hipStream_t st);
+
+// kv_pages.hip
+size_t pages_work_bytes(const qwa_kv_pages& p);
+hipError_t launch_pages_extend(const qwa_kv_pages& p, const int* seqs, const int* add, int n, const qwa_kv_layer* layers,
+                               int n_layers, int kvt, int* status, void* work, hipStream_t st);
+hipError_t launch_pages_fork(const qwa_kv_pages& p, const int* src, const int* dst, int n, void* work, hipStream_t st);
+hipError_t launch_pages_trim(const qwa_kv_pages& p, const int* seqs, const int* lens, int n, hipStream_t st);
+hipError_t launch_pages_compact(const qwa_kv_pages& p, const qwa_kv_layer* layers, int n_layers, int kvt, int* n_live,
+                                void* work, hipStream_t st);
+
+// attn_batch.hip
+size_t batch_work_bytes(int n, int nq, int n_shared, int max_len);
+hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_layer& kv, int kvt, const qwa_kv_pages& p,
+                               const int* seqs, int n, int nq, int n_shared, int max_len, uint16_t* out16,
+                               const qwa_act_q8* oq, void* work, hipStream_t st);
+
 // split-K decode: 16-key chunks in DEC_CLASSES fixed residue classes per KV head (chunk index mod DEC_CLASSES)
 constexpr int DEC_CLASSES = 512;
 size_t dec_work_bytes(int n_pos);

@@ -43,6 +43,11 @@ class _RowSrcC(ctypes.Structure):
     _fields_ = [("dev", ctypes.c_void_p), ("host", ctypes.c_void_p), ("split", ctypes.c_int), ("host_ld", ctypes.c_int)]
 
 
+class _KVPagesC(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("len", ctypes.c_void_p), ("ref", ctypes.c_void_p), ("n_seq", ctypes.c_int),
+                ("ld", ctypes.c_int), ("n_pages", ctypes.c_int), ("page", ctypes.c_int)]
+
+
 class _DNParamsC(ctypes.Structure):
     _fields_ = [("conv_w", ctypes.c_void_p), ("dt_bias", ctypes.c_void_p), ("ssm_a", ctypes.c_void_p),
                 ("ssm_norm", ctypes.c_void_p), ("conv_state", ctypes.c_void_p), ("ssm_state", ctypes.c_void_p)]
@@ -102,6 +107,23 @@ EXPORTS = {
                                    ctypes.c_void_p]),
     "qwa_kv_unpack": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(_KVLayerC), ctypes.c_int, ctypes.c_int,
                                      ctypes.c_void_p]),
+    "qwa_kv_pages_work_bytes": (ctypes.c_size_t, [ctypes.POINTER(_KVPagesC)]),
+    "qwa_kv_pages_extend": (ctypes.c_int, [ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
+                            [ctypes.c_int, ctypes.POINTER(_KVLayerC)] + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 3),
+    "qwa_kv_pages_fork": (ctypes.c_int, [ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
+                          [ctypes.c_int] + [ctypes.c_void_p] * 2),
+    "qwa_kv_pages_trim": (ctypes.c_int, [ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
+                          [ctypes.c_int, ctypes.c_void_p]),
+    "qwa_kv_pages_compact": (ctypes.c_int, [ctypes.POINTER(_KVPagesC), ctypes.POINTER(_KVLayerC)] +
+                             [ctypes.c_int] * 2 + [ctypes.c_void_p] * 3),
+    "qwa_attn_prep_batch": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.POINTER(_KVPagesC), ctypes.c_void_p] +
+                            [ctypes.c_int] * 2 + [ctypes.c_void_p] + [ctypes.c_float] * 2 +
+                            [ctypes.c_int, ctypes.POINTER(_KVLayerC)] + [ctypes.c_void_p] * 3),
+    "qwa_attn_batch_work_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),
+    "qwa_attn_decode_batch": (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.POINTER(_KVLayerC), ctypes.c_int,
+                                                                     ctypes.POINTER(_KVPagesC), ctypes.c_void_p] +
+                              [ctypes.c_int] * 4 + [ctypes.c_void_p, ctypes.POINTER(_ActQ8C), ctypes.c_void_p,
+                                                    ctypes.c_size_t, ctypes.c_void_p]),
     "qwa_deltanet_step": (ctypes.c_int, [ctypes.POINTER(_DNParamsC)] + [ctypes.c_void_p] * 4 +
                           [ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.POINTER(_ActQ8C), ctypes.c_void_p]),
     "qwa_deltanet_multi": (ctypes.c_int, [ctypes.POINTER(_DNParamsC), ctypes.c_int, ctypes.POINTER(_DNTokensC)] +
@@ -424,6 +446,125 @@ def kv_unpack(src, kv: KVLayer, kvt, n_pos: int, stream=None) -> None:
 def kv_append(xk, xv, pos0: int, n: int, kvt, kv: KVLayer, stream=None) -> None:
     """Quantize-on-append of raw K/V rows [n, 4, 256] (the row store of src/cuda/common.cuh:54-80)."""
     _check(lib().qwa_kv_append(_ptr(xk), _ptr(xv), pos0, n, _kvt(kvt), ctypes.byref(kv.c()), _stream(stream)))
+
+
+# ---- batches of sequences over a paged cache ------------------------------------------------------------------------
+PAGES_MAXN, PAGES_MAXL = 1024, 32  # requests / sequences and layers per call
+
+
+def _dev(t, dtype=None, what="tensor"):
+    """_ptr for the batched operators: a GPU tensor of the current device, of the given type."""
+    if isinstance(t, torch.Tensor):
+        if dtype is not None and t.dtype != dtype:
+            raise QwaError(f"{what}: {dtype} wanted, got {t.dtype}")
+        if not t.is_cuda:
+            raise QwaError(f"{what}: not in GPU memory")
+        if t.device.index != torch.cuda.current_device():
+            raise QwaError(f"{what}: on {t.device}, but the current device is {torch.cuda.current_device()}")
+    return _ptr(t)
+
+
+def _count(t, n, what):
+    """An index tensor of at least n entries."""
+    if isinstance(t, torch.Tensor) and t.numel() < n:
+        raise QwaError(f"{what}: {t.numel()} entries, {n} wanted")
+    return _dev(t, torch.int32, what)
+
+
+@dataclass
+class KVPages:
+    """Page tables of a batch of sequences (qwa_kv_pages): page p is positions [p * page, (p + 1) * page) of every layer's
+    KVLayer.  table int32 [n_seq][ld], len int32 [n_seq], ref int32 [n_pages]."""
+    table: torch.Tensor
+    len: torch.Tensor
+    ref: torch.Tensor
+    page: int
+
+    @classmethod
+    def allocate(cls, n_seq: int, max_len: int, n_pages: int, page: int = 64, device="cuda") -> "KVPages":
+        i32 = {"dtype": torch.int32, "device": device}
+        return cls(torch.full((n_seq, -(-max_len // page)), -1, **i32), torch.zeros(n_seq, **i32),
+                   torch.zeros(n_pages, **i32), page)
+
+    def c(self) -> _KVPagesC:
+        n_seq, ld = self.table.shape
+        if self.len.numel() != n_seq:
+            raise QwaError(f"page tables of {n_seq} sequences with {self.len.numel()} lengths")
+        i32 = torch.int32
+        return _KVPagesC(_dev(self.table, i32, "table"), _dev(self.len, i32, "len"), _dev(self.ref, i32, "ref"), n_seq, ld,
+                         self.ref.numel(), self.page)
+
+
+def _layers(layers):
+    return (_KVLayerC * len(layers))(*(kv.c() for kv in layers)), len(layers)
+
+
+def _work(pages, work) -> int | None:
+    need = kv_pages_work_bytes(pages)
+    if isinstance(work, torch.Tensor) and work.numel() * work.element_size() < need:
+        raise QwaError(f"workspace of {work.numel() * work.element_size()} bytes, the call needs {need}")
+    return _dev(work, what="work")
+
+
+def kv_pages_work_bytes(pages: KVPages) -> int:
+    return int(lib().qwa_kv_pages_work_bytes(ctypes.byref(pages.c())))
+
+
+def kv_pages_extend(pages: KVPages, seqs, add, layers, kvt, status, work, n: int | None = None, stream=None) -> None:
+    """Room for add[i] more positions of sequence seqs[i] (int32 GPU tensors): takes free pages, and copies a partly filled
+    last page that others hold.  All or nothing; status (int32): 0 done, > 0 pages missing, -(i + 1) request i invalid."""
+    n = seqs.numel() if n is None else n
+    arr, nl = _layers(layers)
+    _check(lib().qwa_kv_pages_extend(ctypes.byref(pages.c()), _count(seqs, n, "seqs"), _count(add, n, "add"), n, arr, nl,
+                                     _kvt(kvt), _count(status, 1, "status"), _work(pages, work), _stream(stream)))
+
+
+def kv_pages_fork(pages: KVPages, src, dst, work, n: int | None = None, stream=None) -> None:
+    """Sequence dst[i] gives back its pages and shares src[i]'s (src[i] < 0: becomes empty), all requests at once."""
+    n = dst.numel() if n is None else n
+    _check(lib().qwa_kv_pages_fork(ctypes.byref(pages.c()), _count(src, n, "src"), _count(dst, n, "dst"), n,
+                                   _work(pages, work), _stream(stream)))
+
+
+def kv_pages_trim(pages: KVPages, seqs, lens=None, n: int | None = None, stream=None) -> None:
+    """Sequence seqs[i] keeps its first lens[i] positions (lens None: it is freed)."""
+    n = seqs.numel() if n is None else n
+    _check(lib().qwa_kv_pages_trim(ctypes.byref(pages.c()), _count(seqs, n, "seqs"),
+                                   None if lens is None else _count(lens, n, "lens"), n, _stream(stream)))
+
+
+def kv_pages_compact(pages: KVPages, layers, kvt, n_live, work, stream=None) -> None:
+    """Moves the pages in use to the front of every layer's pool; n_live (int32) receives their number."""
+    arr, nl = _layers(layers)
+    _check(lib().qwa_kv_pages_compact(ctypes.byref(pages.c()), arr, nl, _kvt(kvt), _count(n_live, 1, "n_live"),
+                                      _work(pages, work), _stream(stream)))
+
+
+def attn_prep_batch(qg, k, v, q_norm, k_norm, pages: KVPages, seqs, n: int, nq: int, theta: float, eps: float, kvt,
+                    kv: KVLayer, q_out, gate, rope_off=None, stream=None) -> None:
+    """attn_prep_multi for the last nq positions of n sequences (seqs int32, None: 0..n-1) of a paged cache."""
+    f32 = torch.float32
+    _check(lib().qwa_attn_prep_batch(
+        _dev(qg, f32, "qg"), _dev(k, f32, "k"), _dev(v, f32, "v"), _dev(q_norm, f32, "q_norm"), _dev(k_norm, f32, "k_norm"),
+        ctypes.byref(pages.c()), None if seqs is None else _count(seqs, n, "seqs"), n, nq,
+        None if rope_off is None else _count(rope_off, n, "rope_off"), theta, eps, _kvt(kvt), ctypes.byref(kv.c()),
+        _dev(q_out, f32, "q_out"), _dev(gate, f32, "gate"), _stream(stream)))
+
+
+def attn_batch_work_bytes(n: int, nq: int, n_shared: int, max_len: int) -> int:
+    return int(lib().qwa_attn_batch_work_bytes(n, nq, n_shared, max_len))
+
+
+def attn_decode_batch(q, gate, kv: KVLayer, kvt, pages: KVPages, seqs, n: int, nq: int, n_shared: int, max_len: int, out16,
+                      work, oq: ActQ8 | None = None, stream=None) -> None:
+    """Attention of n sequences (seqs int32, None: 0..n-1) with nq queries each over a paged cache; the first n_shared
+    positions, which all of them have in common, are read once.  out16: fp16 [n * nq, 6144]."""
+    f32 = torch.float32
+    _check(lib().qwa_attn_decode_batch(
+        _dev(q, f32, "q"), _dev(gate, f32, "gate"), ctypes.byref(kv.c()), _kvt(kvt), ctypes.byref(pages.c()),
+        None if seqs is None else _count(seqs, n, "seqs"), n, nq, n_shared, max_len,
+        _dev(out16, torch.float16, "out16"), _act(oq), _dev(work, what="work"),
+        work.numel() * work.element_size() if isinstance(work, torch.Tensor) else 1 << 62, _stream(stream)))
 
 
 # ---- Gated DeltaNet ------------------------------------------------------------------------------------------------
