@@ -54,6 +54,8 @@ FILE_FLAGS = {"attn_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attn_decode_ilp.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", *ILP_SCHED],
               "deltanet.hip": ILP_SCHED,
               "deltanet_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              # attn_batch.hip: the same (the two-tile kernels: 83 accumulation registers instead of 223)
+              "attn_batch.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               # gemv_mc.hip (IQ4_XS / IQ2_S one-column GEMV): the max-memory-clause scheduler
               "gemv_mc.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"]}
 

@@ -5,8 +5,12 @@
 // positions that all sequences share are worked on for the rows of all sequences together, those of its own for each
 // sequence by itself, both in ranges of fixed length (batch_plan.hpp), and k_bt_combine joins a row's states in a fixed
 // order.
-//  * A workgroup has one KV head and up to BT_MAXRT 16-row tiles (row 6 * token + head of that KV head); its waves take the
-//    tiles of its key range in turn, each with its own running maximum, sum and O, and merge at the end through LDS.
+//  * Register workgroups (k_bt_own, and k_bt_shared for the shared positions of few rows) have one KV head and up to
+//    BT_MAXRT 16-row tiles (row 6 * token + head of that KV head); their waves take the tiles of the key range in turn, each
+//    with its own running maximum, sum and O, and merge at the end through LDS.
+//  * Tile workgroups (k_bt_tiles, the shared positions of more rows) have PF_ROWS rows, 32 a wave: a tile's raw bytes come
+//    to LDS by direct loads, all waves dequantize them into fp16 tiles there once, and every wave multiplies its rows with
+//    them, as in the prefill's raw-tile kernels but with pages for addresses and a bound per row for the mask.
 //  * Pages are multiples of 16 positions and tiles start at multiples of 16, so each 16 keys lie in one page: a tile's page
 //    numbers are wave-uniform scalar loads, one tile ahead.
 //  * S^T = K Q^T and O^T += V^T P^T on fp16 MFMA with fp32 accumulation.  A lane loads 64 dims of one key and 16 dims of the
@@ -14,40 +18,27 @@
 //    the next tile's K loads go out when the scores are done, its V loads when P V is.
 // Roundings below 32 bits: Q / 16, the dequantized K and V, and the probabilities are fp16 (2^-12 relative each, random in
 // sign, as in the prefill), the output is fp16.
+#include "attn_tiles.hpp"
 #include "batch_plan.hpp"
-#include "kv_operands.hpp"
 #include "launch.hpp"
 
 namespace qwa {
 
-constexpr float BT_LOG2E = 1.4426950408889634f;
-constexpr float BT_RESCALE = 8.0f;  // the running maximum moves only when a score exceeds it by this (natural-log units)
-
-size_t batch_work_bytes(int n, int nq, int n_shared, int max_len) { return batch_bytes(n, nq, n_shared, max_len); }
+size_t batch_work_bytes(int n, int nq, int n_shared, int max_len) {
+    return batch_work(batch_plan(n, nq, n_shared, max_len), n, nq).bytes;
+}
 
 __device__ __forceinline__ f4 bt_mfma16k16(h4 a, h4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
 }
 
-// max / sum over the four lanes that hold one row (lane distances 16 and 32)
-__device__ __forceinline__ float bt_row_max(float x) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float bt_row_sum(float x) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 struct BatchArgs {
     const float* q;
     const int* seqs;
-    float* part_o;    // [slot][row][256], row = token * NH + head
-    float2* part_ml;  // [slot][row] (m, l)
+    PfPartO* tile_o;    // partial states (BatchWork): of the tile workgroups [range][row][256],
+    PfPartMl* tile_ml;  // [range][row]
+    float* part_o;      // of the register workgroups [slot][row][256],
+    float2* part_ml;    // [slot][row]
     int n, nq, n_shared, max_len;
 };
 
@@ -71,6 +62,13 @@ __device__ __forceinline__ int bt_longest(const BatchArgs& a, const qwa_kv_pages
         if (om > m || (om == m && ob < b)) m = om, b = ob;
     }
     return __builtin_amdgcn_readfirstlane(b);
+}
+
+// the pool position of the 16 keys from kb on (a multiple of 16), or -1: at or past the end, or in no page of the pool
+__device__ __forceinline__ int bt_place(const qwa_kv_pages& p, const int* __restrict__ table, int kb, int end) {
+    if (kb >= end) return -1;
+    const int pg = table[kb / p.page];
+    return (unsigned)pg < (unsigned)p.n_pages ? pg * p.page + (kb & (p.page - 1)) : -1;
 }
 
 template <int KVT, int RT>
@@ -128,12 +126,7 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
         for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // the pool position of 16 keys from kb on, or -1: past the range, or in no page of the pool
-    auto place = [&](int kb) {
-        if (kb >= k1) return -1;
-        const int pg = table[kb / p.page];
-        return (unsigned)pg < (unsigned)p.n_pages ? pg * p.page + (kb & (p.page - 1)) : -1;
-    };
+    auto place = [&](int kb) { return bt_place(p, table, kb, k1); };
     KRaw<KVT> kr[KT];
     VRaw<KVT> vr[4 * KT];
     // key rows past the range re-read its last one (their probabilities are exact zeros, so what they hold must be finite:
@@ -243,10 +236,10 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
             for (int kt = 0; kt < KT; kt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) mx = fmaxf(mx, S[rt][kt][i]);
-            mx = bt_row_max(mx);
-            const float mn = mx > m[rt] + BT_RESCALE ? mx : m[rt];
-            const float msl = (mn == -INFINITY ? 0.0f : mn) * BT_LOG2E;  // a row that saw nothing keeps l = 0, O = 0
-            cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] * BT_LOG2E - msl);
+            mx = rows_max(mx);
+            const float mn = mx > m[rt] + PF_RESCALE_T ? mx : m[rt];
+            const float msl = (mn == -INFINITY ? 0.0f : mn) * PF_LOG2E;  // a row that saw nothing keeps l = 0, O = 0
+            cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] * PF_LOG2E - msl);
             float rs = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) p8[rt][j] = (_Float16)0.0f;
@@ -254,7 +247,7 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
             for (int kt = 0; kt < KT; kt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const _Float16 e = (_Float16)fast_exp2(fmaf(S[rt][kt][i], BT_LOG2E, -msl));
+                    const _Float16 e = (_Float16)fast_exp2(fmaf(S[rt][kt][i], PF_LOG2E, -msl));
                     p8[rt][4 * kt + i] = e;
                     rs += (float)e;  // the weights that P V applies
                 }
@@ -296,7 +289,7 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
     // the waves' states, joined: wave w takes output tiles 4 w .. 4 w + 3 (dims 16 (4 lg + i) + 4 w .. + 3 of the row)
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const float lt = bt_row_sum(l[rt]);
+        const float lt = rows_sum(l[rt]);
         __syncthreads();  // the previous tile's states are read out
 #pragma unroll
         for (int dt = 0; dt < 16; dt++) s_o[wave][dt][lane] = o[rt][dt];
@@ -310,7 +303,7 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
 #pragma unroll
         for (int w = 0; w < BT_WAVES; w++) {
             const float mw = s_ml[w][0][lane], lw = s_ml[w][1][lane];
-            const float f = lw == 0.0f ? 0.0f : fast_exp2((mw - M) * BT_LOG2E);  // (lw: NaN scores stay NaN)
+            const float f = lw == 0.0f ? 0.0f : fast_exp2((mw - M) * PF_LOG2E);  // (lw: NaN scores stay NaN)
             L = fmaf(f, lw, L);
 #pragma unroll
             for (int t = 0; t < 4; t++) {
@@ -331,36 +324,289 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
     }
 }
 
-// the shared positions: workgroup = (row group, key range, KV head); slots 0 .. ns - 1
+// the shared positions, for the rows of one group: workgroup = (key range, KV head); slots 0 .. ns - 1
 template <int KVT, int RT>
 __global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(BtCfg<KVT, RT>::WPE)))
-k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len) {
+k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int len) {
     __shared__ f4 s_o[BT_WAVES][16][64];
     __shared__ float s_ml[BT_WAVES][2][64];
-    const int pairs = ns * NKV, grp = blockIdx.x / pairs, pr = blockIdx.x % pairs, g = pr % NKV, sp = pr / NKV;
+    const int g = blockIdx.x % NKV, sp = blockIdx.x / NKV;
     const int b = bt_longest(a, p, threadIdx.x & 63);
     const int k1 = min(min((sp + 1) * len, a.n_shared), bt_len(a, p, b));
     const int seq = bt_seq(a, b);
     const int* table = p.table + (seq >= 0 && seq < p.n_seq ? (size_t)seq * p.ld : 0);
-    bt_body<KVT, RT>(s_o, s_ml, a, kv, p, table, grp * 16 * RT, a.n * a.nq * GRP, g, sp * len, k1, 0, sp);
+    bt_body<KVT, RT>(s_o, s_ml, a, kv, p, table, 0, a.n * a.nq * GRP, g, sp * len, k1, 0, sp);
 }
 
-// each sequence's own positions: workgroup = (batch row, key range, KV head); slots first .. first + ns - 1
+// each sequence's own positions: workgroup = (batch row, key range, KV head, row group); slots first .. first + ns - 1
 template <int KVT, int RT>
 __global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(BtCfg<KVT, RT>::WPE)))
-k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len, int first) {
+k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len, int first, int groups) {
     __shared__ f4 s_o[BT_WAVES][16][64];
     __shared__ float s_ml[BT_WAVES][2][64];
-    const int pairs = ns * NKV, b = blockIdx.x / pairs, pr = blockIdx.x % pairs, g = pr % NKV, sp = pr / NKV;
+    // the groups of one (row, range, head) read the same keys: workgroups 8 apart, which one XCD runs
+    const int u = blockIdx.x / (8 * groups) * 8 + blockIdx.x % 8, grp = blockIdx.x / 8 % groups;
+    const int pairs = ns * NKV, b = u / pairs, pr = u % pairs, g = pr % NKV, sp = pr / NKV;
+    if (b >= a.n) return;
     const int begin = a.n_shared + sp * len, k1 = min(begin + len, bt_len(a, p, b));
     if (begin >= k1) return;  // k_bt_combine does not read this slot
     // (tiles start at multiples of 16; positions before `begin` are masked)
-    bt_body<KVT, RT>(s_o, s_ml, a, kv, p, p.table + (size_t)bt_seq(a, b) * p.ld, b * a.nq * GRP, (b + 1) * a.nq * GRP, g,
-                     begin & ~15, k1, begin, first + sp);
+    bt_body<KVT, RT>(s_o, s_ml, a, kv, p, p.table + (size_t)bt_seq(a, b) * p.ld, b * a.nq * GRP + grp * 16 * RT,
+                     (b + 1) * a.nq * GRP, g, begin & ~15, k1, begin, first + sp);
 }
 
-// Joins a row's partial states in slot order, gates, rounds: one wave per row (token * NH + head), 4 dims per lane.
-__global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p, const float* __restrict__ gate,
+// The shared positions for PF_ROWS rows: workgroup = (row block, tile range, KV head).  The 8 waves have 32 rows each, two a
+// SIMD: the softmax and dequantization of one issue while the other's MFMAs run.
+template <int KVT>
+__global__ void __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(PF_WAVES / 4, PF_WAVES / 4)))
+k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
+    static_assert(PF_THREADS == 512 && PF_KT == 2, "the conversion's units are the workgroup's threads");
+    using L = PfRaw<KVT>;
+    constexpr int VB = L::VB, NBUF = L::NBUF, AHEAD = L::AHEAD;
+    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NBUF][L::BYTES];
+    __shared__ __attribute__((aligned(16))) _Float16 s_k[2][PF_TILE * KS_LD];
+    __shared__ __attribute__((aligned(16))) _Float16 s_vt[2][HD * VT_LD];
+    const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // workgroups 8 apart run on one XCD: those of a (KV head, range) pair read the same tiles
+    int pair = blockIdx.x / blocks, blk = blockIdx.x % blocks;
+    if (NKV * ns % 8 == 0) {
+        pair = NKV * ns / 8 * (blockIdx.x & 7) + (blockIdx.x >> 3) / blocks;
+        blk = (blockIdx.x >> 3) % blocks;
+    }
+    const int g = pair % NKV, sp = pair / NKV;
+    const int longest = bt_longest(a, p, lane);
+    const int end = min(a.n_shared, bt_len(a, p, longest));
+    const int seq = bt_seq(a, longest);
+    const int* __restrict__ table = p.table + (seq >= 0 && seq < p.n_seq ? (size_t)seq * p.ld : 0);
+    const int all = (a.n_shared + PF_TILE - 1) / PF_TILE;
+    const int tb = (int)((long long)sp * all / ns), te = (int)((long long)(sp + 1) * all / ns);
+    const int nt = min(te, (end + PF_TILE - 1) / PF_TILE) - tb;  // (a batch shorter than its shared part: fewer, or none)
+
+    const int nrows = a.n * a.nq * GRP, wrow0 = blk * PF_ROWS + 32 * wave;
+    const size_t head = (size_t)g * kv.capacity;
+    const int nvm = L::count(wave);
+    uint32_t raw_lds[NBUF];
+#pragma unroll
+    for (int b = 0; b < NBUF; b++) raw_lds[b] = lds_addr(s_raw[b]);
+
+    // Direct-to-LDS loads of a tile, its halves of 16 keys at pool positions at0, at1 (-1: dead, position 0 is read in its
+    // place); keys at or past the end re-read the last one of their half
+    auto issue = [&](int buf, int k0, int at0, int at1) {
+        const size_t base[2] = {head + max(at0, 0), head + max(at1, 0)};
+        const int last[2] = {min(15, end - 1 - k0), min(15, end - 17 - k0)};
+#pragma unroll
+        for (int c = 0; c < (L::NKV + PF_WAVES - 1) / PF_WAVES; c++) {
+            const int ik = wave + PF_WAVES * c, iv = (wave + PF_WAVES / 2) % PF_WAVES + PF_WAVES * c;
+            auto piece = [&](int i, const uint8_t* src, uint32_t dst) {
+                const int h = i >= L::NKV / 2, q = 1024 * (i - h * (L::NKV / 2)) + 16 * lane;
+                const int row = min(q / VB, max(h ? last[1] : last[0], 0));
+                dma_sv<16>(dst + 1024 * i, src + (h ? base[1] : base[0]) * VB, (uint32_t)(row * VB + q % VB));
+            };
+            if (ik < L::NKV) piece(ik, kv.k, raw_lds[buf] + L::K);
+            if (iv < L::NKV) piece(iv, kv.v, raw_lds[buf] + L::V);
+        }
+        if constexpr (L::SC != 0) {
+            const int j = wave & 1;
+            const uint32_t off = (uint32_t)(min(lane / 4, max(j ? last[1] : last[0], 0)) * 16 + 4 * (lane & 3));
+            if (wave >= PF_WAVES - 2) dma_sv<4>(raw_lds[buf] + L::KS + 256 * j, kv.ks + (j ? base[1] : base[0]) * 8, off);
+            if (wave >= PF_WAVES / 2 - 2 && wave < PF_WAVES / 2)
+                dma_sv<4>(raw_lds[buf] + L::VS + 256 * j, kv.vs + (j ? base[1] : base[0]) * 8, off);
+        }
+    };
+    // a dead half's V is zeros: its probabilities are, and what was read in its place need not be finite
+    auto convert = [&](int raw, int dst, uint32_t dead) {
+        pf_convert<KVT>(s_raw[raw], s_k[dst], s_vt[dst], t);
+        if (dead != 0) {
+            const int cb = t & 3, dc = (t >> 2) & 63, h = t >> 8;
+            if ((dead >> h) & 1)
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+                    *reinterpret_cast<uint2*>(s_vt[dst] + (4 * dc + d) * VT_LD + 8 * cb + 4 * h) = make_uint2(0u, 0u);
+        }
+    };
+
+    int vis[2], vmin = 0x7fffffff;
+    h8 qb[2][8];
+#pragma unroll
+    for (int rt = 0; rt < 2; rt++) {
+        const int r = wrow0 + 16 * rt + i16, tok = r / GRP;
+        const bool valid = r < nrows;
+        vis[rt] = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, end) : 0;
+        if (valid) vmin = min(vmin, vis[rt]);
+        const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + 8 * lg;
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            const float4 x0 = *reinterpret_cast<const float4*>(qrow + 32 * s);
+            const float4 x1 = *reinterpret_cast<const float4*>(qrow + 32 * s + 4);
+            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                qb[rt][s][j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
+    vmin = __builtin_amdgcn_readfirstlane(vmin);
+
+    f4 o[2][16];
+    float m[2], l[2];
+#pragma unroll
+    for (int rt = 0; rt < 2; rt++) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    if (nt > 0) {
+        auto key0 = [&](int i) { return (tb + min(i, nt - 1)) * PF_TILE; };  // (past the last tile: it is re-read)
+        uint32_t dead = 0;  // two bits a tile, tile i's in bits 0, 1
+        int at0, at1;
+        auto find = [&](int i) {
+            at0 = bt_place(p, table, key0(i), end);
+            at1 = bt_place(p, table, key0(i) + 16, end);
+        };
+        wait_vmcnt<0>();  // the Q loads; from here on vmcnt counts only the tile loads
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            find(i);
+            dead |= (uint32_t)((at0 < 0) | (at1 < 0) << 1) << (2 * i);
+            issue(i, key0(i), at0, at1);
+        }
+        find(AHEAD);
+        wait_vm(nvm * (AHEAD - 1));
+        __syncthreads();
+        convert(0, 0, dead & 3);
+        if constexpr (AHEAD >= 2) wait_vm(nvm * (AHEAD - 2));
+        __syncthreads();
+
+        const bool lead = wave < PF_WAVES / 2;  // the two waves of a SIMD convert at different times
+        const bool rows_here = wrow0 < nrows;
+        for (int i = 0; i < nt; i++) {
+            const int k0 = key0(i), cur = i & 1;
+            dead |= (uint32_t)((at0 < 0) | (at1 < 0) << 1) << (2 * AHEAD);
+            issue((i + AHEAD) % NBUF, key0(i + AHEAD), at0, at1);
+            find(i + AHEAD + 1);
+            const _Float16* Ks = s_k[cur];
+            const _Float16* Vt = s_vt[cur];
+            if (AHEAD >= 2 && lead) convert((i + 1) % NBUF, cur ^ 1, (dead >> 2) & 3);
+            if (rows_here) {
+                // S^T = K Q^T: lane (row i16) gets keys k0 + 16 kt + 4 lg + j; the K fragments of a step are read while
+                // the step before multiplies
+                f4 sc[2][2];
+#pragma unroll
+                for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+                    for (int kt = 0; kt < 2; kt++) sc[rt][kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                const _Float16* krow = Ks + i16 * KS_LD + 8 * lg;
+                h8 kf[2][2] = {{lds_h8(krow), lds_h8(krow + 16 * KS_LD)}, {}};
+#pragma unroll
+                for (int s = 0; s < 8; s++) {
+                    if (s < 7)
+#pragma unroll
+                        for (int kt = 0; kt < 2; kt++) kf[(s + 1) & 1][kt] = lds_h8(krow + 16 * kt * KS_LD + 32 * (s + 1));
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                        for (int rt = 0; rt < 2; rt++) sc[rt][kt] = mfma16(kf[s & 1][kt], qb[rt][s], sc[rt][kt]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+
+                const bool masked = k0 + PF_TILE > vmin || (dead & 3) != 0;
+                float cr[2];
+                h8 pb[2];
+#pragma unroll
+                for (int rt = 0; rt < 2; rt++) {
+                    if (masked) {
+#pragma unroll
+                        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const bool seen = k0 + 16 * kt + 4 * lg + j < vis[rt] && !((dead >> kt) & 1);
+                                sc[rt][kt][j] = seen ? sc[rt][kt][j] : -INFINITY;
+                            }
+                    }
+                    float mx = max3f(max3f(-INFINITY, sc[rt][0][0], sc[rt][0][1]), sc[rt][0][2], sc[rt][0][3]);
+                    mx = rows_max(max3f(max3f(mx, sc[rt][1][0], sc[rt][1][1]), sc[rt][1][2], sc[rt][1][3]));
+                    const float mn = mx > m[rt] + PF_RESCALE_T ? mx : m[rt];
+                    cr[rt] = mn == m[rt] ? 1.0f : fast_exp2((m[rt] - mn) * PF_LOG2E);
+                    m[rt] = mn;
+                    const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        pb[rt][j] = (_Float16)fast_exp2(fmaf(sc[rt][j >> 2][j & 3], PF_LOG2E, -msl));
+                    // the sum of the rounded probabilities, the weights that P V applies
+                    const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
+                    float rs = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) rs = __builtin_amdgcn_fdot2(h2{pb[rt][j], pb[rt][j + 1]}, one2, rs, false);
+                    l[rt] = l[rt] * cr[rt] + rs;
+                }
+                if (__any(cr[0] != 1.0f || cr[1] != 1.0f)) {
+#pragma unroll
+                    for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+                        for (int dt = 0; dt < 16; dt++) o[rt][dt] *= cr[rt];
+                }
+
+                // O^T += V^T P^T, three V fragments in flight
+                const _Float16* vrow = Vt + i16 * VT_LD + 8 * lg;
+                h8 vf[3];
+#pragma unroll
+                for (int dt = 0; dt < 2; dt++) vf[dt] = lds_h8(vrow + 16 * VT_LD * dt);
+#pragma unroll
+                for (int dt = 0; dt < 16; dt++) {
+                    if (dt + 2 < 16) vf[(dt + 2) % 3] = lds_h8(vrow + 16 * VT_LD * (dt + 2));
+#pragma unroll
+                    for (int rt = 0; rt < 2; rt++) o[rt][dt] = mfma16(vf[dt % 3], pb[rt], o[rt][dt]);
+                }
+            }
+            if (AHEAD >= 2 && !lead) convert((i + 1) % NBUF, cur ^ 1, (dead >> 2) & 3);
+            if constexpr (AHEAD >= 2) {
+                wait_vm(nvm * (AHEAD - 2));  // tile i + 2 must have landed before the next iteration converts it
+                __syncthreads();
+            } else {
+                wait_vm(0);
+                __syncthreads();
+                if (i + 1 < nt) convert((i + 1) % NBUF, cur ^ 1, (dead >> 2) & 3);
+                __syncthreads();
+            }
+            dead >>= 2;
+        }
+        wait_vmcnt<0>();  // no direct-to-LDS load outlives the workgroup
+    }
+
+    // partial states: lane holds dims 16 dt + 4 lg + j of row (rt, i16)
+#pragma unroll
+    for (int rt = 0; rt < 2; rt++) {
+        const int r = wrow0 + 16 * rt + i16;
+        const float lt = rows_sum(l[rt]);
+        const float il = lt == 0.0f ? 0.0f : 1.0f / lt;  // (a row that saw nothing: l = 0 and O = 0)
+        float amax = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 16; dt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) amax = fmaxf(amax, fabsf(o[rt][dt][j]));
+        amax = rows_max(amax) * il;
+        const float qs = amax > 1e-30f ? 32767.0f / amax : 0.0f, f = il * qs;
+        if (r < nrows) {
+            const size_t rec = (size_t)sp * a.n * a.nq * NH + (size_t)(r / GRP) * NH + g * GRP + r % GRP;
+            // (a row whose O is not finite has no fixed-point form: its scale makes every value NaN)
+            const float scale = amax < INFINITY ? (qs > 0.0f ? amax * (1.0f / 32767.0f) : 0.0f) : NAN;
+            if (lg == 0) a.tile_ml[rec] = make_float4(m[rt], lt, scale, 0.0f);
+            PfPartO* dst = a.tile_o + rec * (HD / 4) + lg;
+#pragma unroll
+            for (int dt = 0; dt < 16; dt++)
+                dst[4 * dt] = pack16x4(o[rt][dt][0] * f, o[rt][dt][1] * f, o[rt][dt][2] * f, o[rt][dt][3] * f);
+        }
+    }
+}
+
+// Joins a row's partial states in a fixed order, gates, rounds: one wave per row (token * NH + head), 4 dims per lane.  The
+// weights exp(m - M) come one state a lane, 64 at a time; the states' rows are read eight at a time.
+__global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p, const float* __restrict__ gate, int nt,
                                                     int ns_shared, int ns_own, int len_own,
                                                     uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {
     const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -368,23 +614,48 @@ __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p,
     if (row >= nrows) return;
     const int mine = bt_len(a, p, row / NH / a.nq) - a.n_shared;  // own positions
     const int ns = ns_shared + (mine > 0 ? min(ns_own, (mine + len_own - 1) / len_own) : 0);
+    // (m, l, scale) of state s: the tile workgroups' states first, then the register workgroups'
+    auto state = [&](int s) {
+        if (s < nt) return a.tile_ml[(size_t)s * nrows + row];
+        if (s < nt + ns) {
+            const float2 ml = a.part_ml[(size_t)(s - nt) * nrows + row];
+            return make_float4(ml.x, ml.y, 1.0f, 0.0f);
+        }
+        return make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    };
     float M = -INFINITY;
-    for (int s = lane; s < ns; s += 64) {
-        const float2 ml = a.part_ml[(size_t)s * nrows + row];
-        M = fmaxf(M, ml.y > 0.0f || ml.y != ml.y ? ml.x : -INFINITY);
-    }
+    for (int s0 = 0; s0 < nt + ns; s0 += 64) M = fmaxf(M, state(s0 + lane).x);
     M = wave_max(M);
     float L = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s = 0; s < ns; s++) {
-        const float2 ml = a.part_ml[(size_t)s * nrows + row];
-        const float4 x = *reinterpret_cast<const float4*>(a.part_o + ((size_t)s * nrows + row) * HD + 4 * lane);
-        const float f = ml.y == 0.0f ? 0.0f : fast_exp2((ml.x - M) * BT_LOG2E);
-        L = fmaf(f, ml.y, L);
-        acc.x = fmaf(f, x.x, acc.x);
-        acc.y = fmaf(f, x.y, acc.y);
-        acc.z = fmaf(f, x.z, acc.z);
-        acc.w = fmaf(f, x.w, acc.w);
+    constexpr int U = 8;
+    for (int s0 = 0; s0 < nt + ns; s0 += 64) {
+        const PfPartMl ml = state(s0 + lane);
+        // a state that saw nothing weighs nothing; one of NaN scores (l is NaN) makes the row NaN
+        const float f = ml.y == 0.0f ? 0.0f : fast_exp2((ml.x - M) * PF_LOG2E);
+        L += wave_sum(f * ml.y);
+        // tile states hold O / l in steps of the scale, register states O
+        const float w = f * ml.z * (s0 + lane < nt ? ml.y : 1.0f);
+        const int most = min(64, nt + ns - s0);
+        for (int k = 0; k < most; k += U) {
+            float4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int s = s0 + min(k + u, most - 1);
+                if (s < nt) x[u] = unpack16x4(a.tile_o[((size_t)s * nrows + row) * (HD / 4) + lane]);
+                else x[u] = *reinterpret_cast<const float4*>(a.part_o + ((size_t)(s - nt) * nrows + row) * HD + 4 * lane);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float fu = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), min(k + u, 63)));
+                if (k + u < most) {
+                    acc.x = fmaf(fu, x[u].x, acc.x);
+                    acc.y = fmaf(fu, x[u].y, acc.y);
+                    acc.z = fmaf(fu, x[u].z, acc.z);
+                    acc.w = fmaf(fu, x[u].w, acc.w);
+                }
+            }
+        }
     }
     const float4 gv = *reinterpret_cast<const float4*>(gate + (size_t)row * HD + 4 * lane);
     float v[4] = {acc.x / L * sigmoid(gv.x), acc.y / L * sigmoid(gv.y), acc.z / L * sigmoid(gv.z), acc.w / L * sigmoid(gv.w)};
@@ -425,17 +696,16 @@ static void launch_ranges(const BatchArgs& a, const qwa_kv_layer& kv, const qwa_
                           hipStream_t st) {
     const dim3 block(64 * BT_WAVES);
 #define QWA_BT(K, RT, GRID, ...) hipLaunchKernelGGL((K<KVT, RT>), dim3(GRID), block, 0, st, a, kv, p, __VA_ARGS__)
+    if (b.nt > 0)
+        hipLaunchKernelGGL(k_bt_tiles<KVT>, dim3(b.blocks * b.nt * NKV), dim3(PF_THREADS), 0, st, a, kv, p, b.blocks, b.nt);
     if (b.ns_shared > 0) {
-        const int grid = b.groups * b.ns_shared * NKV;
-        if (b.rt_shared == 1) QWA_BT(k_bt_shared, 1, grid, b.ns_shared, b.len_shared);
-        else if (b.rt_shared == 2) QWA_BT(k_bt_shared, 2, grid, b.ns_shared, b.len_shared);
-        else QWA_BT(k_bt_shared, 3, grid, b.ns_shared, b.len_shared);
+        if (b.rt_shared == 1) QWA_BT(k_bt_shared, 1, b.ns_shared * NKV, b.len_shared);
+        else QWA_BT(k_bt_shared, 2, b.ns_shared * NKV, b.len_shared);
     }
     if (b.ns_own > 0) {
-        const int grid = a.n * b.ns_own * NKV;
-        if (b.rt_own == 1) QWA_BT(k_bt_own, 1, grid, b.ns_own, b.len_own, b.ns_shared);
-        else if (b.rt_own == 2) QWA_BT(k_bt_own, 2, grid, b.ns_own, b.len_own, b.ns_shared);
-        else QWA_BT(k_bt_own, 3, grid, b.ns_own, b.len_own, b.ns_shared);
+        const int grid = (a.n * b.ns_own * NKV + 7) / 8 * 8 * b.groups;
+        if (b.rt_own == 1) QWA_BT(k_bt_own, 1, grid, b.ns_own, b.len_own, b.ns_shared, b.groups);
+        else QWA_BT(k_bt_own, 2, grid, b.ns_own, b.len_own, b.ns_shared, b.groups);
     }
 #undef QWA_BT
 }
@@ -444,17 +714,18 @@ hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_l
                                const int* seqs, int n, int nq, int n_shared, int max_len, uint16_t* out16,
                                const qwa_act_q8* oq, void* work, hipStream_t st) {
     const BatchPlan b = batch_plan(n, nq, n_shared, max_len);
-    const size_t rows = (size_t)n * nq * NH;
-    float* o = static_cast<float*>(work);
-    const BatchArgs a{q, seqs, o, reinterpret_cast<float2*>(o + b.slots() * rows * HD), n, nq, n_shared, max_len};
+    const BatchWork w = batch_work(b, n, nq);
+    uint8_t* base = static_cast<uint8_t*>(work);
+    const BatchArgs a{q, seqs, reinterpret_cast<PfPartO*>(base + w.tile_o), reinterpret_cast<PfPartMl*>(base + w.tile_ml),
+                      reinterpret_cast<float*>(base + w.o), reinterpret_cast<float2*>(base + w.ml), n, nq, n_shared, max_len};
     switch (kvt) {
         case QWA_KV_F16: launch_ranges<QWA_KV_F16>(a, kv, p, b, st); break;
         case QWA_KV_Q8_0: launch_ranges<QWA_KV_Q8_0>(a, kv, p, b, st); break;
         default: launch_ranges<QWA_KV_Q4_0>(a, kv, p, b, st); break;
     }
     const qwa_act_q8 act = oq ? *oq : qwa_act_q8{nullptr, nullptr, nullptr};
-    hipLaunchKernelGGL(k_bt_combine, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p, gate, b.ns_shared, b.ns_own,
-                       b.len_own, out16, act, oq != nullptr ? 1 : 0);
+    hipLaunchKernelGGL(k_bt_combine, dim3((unsigned)(((size_t)n * nq * NH + 3) / 4)), dim3(256), 0, st, a, p, gate, b.nt,
+                       b.ns_shared, b.ns_own, b.len_own, out16, act, oq != nullptr ? 1 : 0);
     return hipGetLastError();
 }
 

@@ -168,15 +168,23 @@ int main() {
         for (int shared : {0, sh}) {
             if (shared > most) continue;
             const BatchPlan p = batch_plan(n, nq, shared, most);
-            CHECK(p.rt_own * 16 >= nq * GRP && p.rt_own <= BT_MAXRT, "rows of a sequence\n");
-            CHECK(p.groups * p.rt_shared * 16 >= n * nq * GRP, "rows of the batch\n");
-            CHECK((long long)p.ns_shared * p.len_shared >= shared && (shared > 0) == (p.ns_shared > 0), "shared\n");
+            const BatchWork w = batch_work(p, n, nq);
+            const long long rows = (long long)n * nq * NH;
+            CHECK(p.groups * p.rt_own * 16 >= nq * GRP && p.rt_own <= BT_MAXRT, "rows of a sequence\n");
+            CHECK(shared == 0 || (p.nt > 0) != (p.ns_shared > 0), "the shared positions: one kind of workgroup\n");
+            CHECK(p.nt == 0 || p.blocks * PF_ROWS >= n * nq * GRP, "rows of the batch\n");
+            CHECK(p.nt * (long long)PF_TILE < shared + PF_TILE, "an empty range\n");
+            CHECK(p.ns_shared == 0 || p.rt_shared * 16 >= n * nq * GRP, "rows of the batch\n");
+            CHECK(p.nt > 0 || (long long)p.ns_shared * p.len_shared >= shared, "shared\n");
             CHECK((long long)p.ns_own * p.len_own >= most - shared && (most > shared) == (p.ns_own > 0), "own\n");
             CHECK(p.ns_shared == 0 || (long long)(p.ns_shared - 1) * p.len_shared < shared, "an empty range\n");
             CHECK(p.ns_own == 0 || (long long)(p.ns_own - 1) * p.len_own < most - shared, "an empty range\n");
             CHECK(p.len_shared % 16 == 0, "a range that begins inside 16 keys\n");
-            CHECK(p.slots() >= 1, "no range\n");
-            CHECK((long long)p.groups * p.ns_shared * NKV < 1LL << 31 && (long long)n * p.ns_own * NKV < 1LL << 31, "grid\n");
+            CHECK(p.slots() + p.nt >= 1, "no range\n");
+            CHECK((long long)p.blocks * p.nt * NKV < 1LL << 31 && (long long)n * p.ns_own * NKV * p.groups < 1LL << 31,
+                  "grid\n");
+            CHECK(w.bytes >= (size_t)(rows * (p.nt * (HD * 2 + 16) + p.slots() * (HD * 4 + 8))) && w.tile_ml % 16 == 0 &&
+                  w.o % 16 == 0 && w.ml % 16 == 0, "work buffer\n");
         }
     }
     return 0;
