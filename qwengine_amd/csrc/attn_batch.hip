@@ -24,6 +24,11 @@
 
 namespace qwa {
 
+#ifndef QWA_ROWS4
+#define QWA_ROWS4 3072
+#endif
+constexpr int BT_ROWS4 = QWA_ROWS4;  // rows up to which a combine workgroup has one row
+
 size_t batch_work_bytes(int n, int nq, int n_shared, int max_len) {
     return batch_work(batch_plan(n, nq, n_shared, max_len), n, nq).bytes;
 }
@@ -37,11 +42,17 @@ struct BatchArgs {
     const int* seqs;
     PfPartO* tile_o;    // partial states (BatchWork): of the tile workgroups [range][row][256],
     PfPartMl* tile_ml;  // [range][row]
-    float* part_o;      // of the register workgroups [slot][row][256],
-    float2* part_ml;    // [slot][row]
-    int n, nq, n_shared, max_len;
+    float* part_o;      // of the register workgroups over the shared positions [range][row][256],
+    float2* part_ml;    // [range][row]
+    float* own_o;       // and over the own positions [KV head][segment][query row][256],
+    float2* own_ml;     // [KV head][segment][query row]
+    int* begin;         // first step of each batch row's own positions, and their total [n + 1]
+    int n, nq, n_shared, max_len, wgs;
 };
 
+#ifndef QWA_SB
+#define QWA_SB __builtin_amdgcn_sched_barrier(0)
+#endif
 // positions of batch row b, cut to max_len; 0 for an unknown sequence
 __device__ __forceinline__ int bt_seq(const BatchArgs& a, int b) { return a.seqs ? a.seqs[b] : b; }
 __device__ __forceinline__ int bt_len(const BatchArgs& a, const qwa_kv_pages& p, int b) {
@@ -67,22 +78,46 @@ __device__ __forceinline__ int bt_longest(const BatchArgs& a, const qwa_kv_pages
 // the pool position of the 16 keys from kb on (a multiple of 16), or -1: at or past the end, or in no page of the pool
 __device__ __forceinline__ int bt_place(const qwa_kv_pages& p, const int* __restrict__ table, int kb, int end) {
     if (kb >= end) return -1;
-    const int pg = table[kb / p.page];
+    const int pg = table[kb >> __builtin_ctz(p.page)];
     return (unsigned)pg < (unsigned)p.n_pages ? pg * p.page + (kb & (p.page - 1)) : -1;
 }
 
+#ifndef QWA_K1
+#define QWA_K1 1
+#endif
+#ifndef QWA_WPE
+#define QWA_WPE 3
+#endif
+#ifndef QWA_QL
+#define QWA_QL 0
+#endif
 template <int KVT, int RT>
 struct BtCfg {
-    static constexpr int KT = KVT == QWA_KV_F16 ? 1 : 2;  // 16-key groups of a tile
-    static constexpr int WPE = RT == 1 ? 2 : 1;           // waves per SIMD that the registers allow
+    static constexpr int KT = KVT == QWA_KV_F16 || (KVT == QWA_KV_Q8_0 && RT == 1 && QWA_K1 > 0) || (KVT == QWA_KV_Q4_0 && RT == 1 && QWA_K1 > 1) ? 1 : 2;  // 16-key groups of a tile
+    static constexpr int WPE = RT == 1 ? QWA_WPE : 2;                         // waves per SIMD that the registers allow
+    static constexpr bool QLDS = RT > QWA_QL;                  // Q fragments in LDS instead of registers
 };
 
-// One workgroup: rows [row0, rows) of KV head g (rows in units 6 * token + head), keys [k0, k1) of the sequence whose table
-// row is `table`, positions below lo excluded, partial states to slot `slot`.
 template <int KVT, int RT>
-__device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64], const BatchArgs& a,
-                                        const qwa_kv_layer& kv, const qwa_kv_pages& p, const int* __restrict__ table,
-                                        int row0, int rows, int g, int k0, int k1, int lo, int slot) {
+struct BtLds {
+    union {
+        h8 q[RT][8][64];         // while the keys are walked
+        f4 o[BT_WAVES][8][64];  // while the waves' states are joined, half of the output tiles at a time
+    };
+    float ml[BT_WAVES][2][64];
+};
+
+// One key range of a workgroup: rows [row0, rows) of KV head g (row 6 * token + head of the group), keys [k0, k1) of the
+// sequence whose table row is `table`, positions below lo excluded; the partial state of a row goes to po, pml at rstep *
+// token + head.
+template <int KVT, int RT>
+__device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a, const qwa_kv_layer& kv,
+                                        const qwa_kv_pages& p, const int* __restrict__ table, int row0, int rows, int g,
+                                        int k0, int k1, int lo, float* __restrict__ po, float2* __restrict__ pml,
+                                        int rstep) {
+    auto& s_o = lds.o;
+    auto& s_ml = lds.ml;
+    constexpr bool QLDS = BtCfg<KVT, RT>::QLDS;
     constexpr int KT = BtCfg<KVT, RT>::KT, VB = value_bytes(KVT), TILE = 16 * KT;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int i16 = lane & 15, lg = lane >> 4;
@@ -91,8 +126,96 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
     const uint16_t* const ksh = KVT == QWA_KV_F16 ? nullptr : kv.ks + (size_t)g * kv.capacity * 8;
     const uint16_t* const vsh = KVT == QWA_KV_F16 ? nullptr : kv.vs + (size_t)g * kv.capacity * 8;
 
-    // rows of this lane: Q / 16 as the B operand, keys below vis are seen
-    h8 qb[RT][8];
+    auto place = [&](int kb) { return bt_place(p, table, kb, k1); };
+    // Raw bytes of a tile.  K: 16-byte piece 4 i + lg of row i16 in words 4 i .. 4 i + 3, so that one load instruction takes
+    // 64 consecutive bytes of 16 rows and no two of them the same ones (with two pieces side by side per lane the loads of
+    // a tile met each other's cache lines in flight and stalled there: 24 sequences of up to 16384 Q4_0 positions 101 us).
+    // V: the lane's 16 dims of row 4 lg + j, F16 as two runs of 8 dims 128 apart for the same reason.  Block scales: the 16
+    // rows' 256 bytes, a dword a lane, handed out by lane permutes when they are used.
+    constexpr bool SC = KVT != QWA_KV_F16;
+    constexpr int KW = VB / 16, VW = VB / 64;  // words per lane of a K row and of a V row
+    uint32_t kr[KT][KW], vr[4 * KT][VW], ksd[KT], vsd[KT];
+    // key rows past the range re-read its last one (their probabilities are exact zeros, so what they hold must be finite:
+    // a stale row need not be), groups without a place are zeros
+    auto load_k = [&](int kt, const uint8_t* src, const uint16_t* ssc, int row, int srow) {
+#pragma unroll
+        for (int i = 0; i < KW / 4; i++) {
+            const uint4 u = ld16(src + (uint32_t)(row * VB + 16 * lg) + 64 * i);
+            kr[kt][4 * i] = u.x; kr[kt][4 * i + 1] = u.y; kr[kt][4 * i + 2] = u.z; kr[kt][4 * i + 3] = u.w;
+        }
+        if constexpr (SC) ksd[kt] = reinterpret_cast<const uint32_t*>(ssc)[(uint32_t)(4 * srow + (lane & 3))];
+    };
+    auto load_v = [&](uint32_t* w, const uint8_t* src, int row) {
+        if constexpr (VW == 2) {
+            const uint2 u = ld8(src + (uint32_t)(row * VB + 8 * i16));
+            w[0] = u.x; w[1] = u.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < VW / 4; i++) {
+                const uint4 u = ld16(src + (uint32_t)(row * VB + 16 * i16) + 256 * i);
+                w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+            }
+        }
+    };
+    auto load_ks = [&](const int* at, int kb) {
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) {
+            const int last = k1 - 1 - (kb + 16 * kt);
+            const size_t pos = (size_t)max(at[kt], 0);
+            const uint8_t* src = kh + pos * VB;
+            const uint16_t* ssc = SC ? ksh + pos * 8 : nullptr;
+            if (at[kt] >= 0 && last >= 15) {
+                load_k(kt, src, ssc, i16, lane >> 2);
+            } else if (at[kt] >= 0) {
+                load_k(kt, src, ssc, min(i16, last), min(lane >> 2, last));
+            } else {
+#pragma unroll
+                for (int i = 0; i < KW; i++) kr[kt][i] = 0;
+                ksd[kt] = 0;
+            }
+        }
+    };
+    auto load_vs = [&](const int* at, int kb) {
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) {
+            const int last = k1 - 1 - (kb + 16 * kt);
+            const size_t pos = (size_t)max(at[kt], 0);
+            const uint8_t* src = vh + pos * VB;
+            const uint32_t* ssc = SC ? reinterpret_cast<const uint32_t*>(vsh + pos * 8) : nullptr;
+            if (at[kt] >= 0 && last >= 15) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) load_v(vr[4 * kt + j], src + j * VB, 4 * lg);
+                if constexpr (SC) vsd[kt] = ssc[(uint32_t)lane];
+            } else if (at[kt] >= 0) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) load_v(vr[4 * kt + j], src, min(4 * lg + j, last));
+                if constexpr (SC) vsd[kt] = ssc[(uint32_t)(4 * min(lane >> 2, last) + (lane & 3))];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int i = 0; i < VW; i++) vr[4 * kt + j][i] = 0;
+                vsd[kt] = 0;
+            }
+        }
+    };
+    // half h (0 / 1) of lane `from`'s dword x, in both halves
+    auto scale_of = [&](uint32_t x, int from, int h) {
+        const uint32_t u = __builtin_amdgcn_ds_bpermute(4 * from, (int)x);
+        return bits_h2(__builtin_amdgcn_perm(u, u, h ? 0x03020302u : 0x01000100u));
+    };
+
+    int kb = k0 + TILE * wave;
+    int at[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; kt++) at[kt] = place(kb + 16 * kt);
+    if (kb < k1) {
+        load_ks(at, kb);
+        load_vs(at, kb);
+    }
+    // rows of this lane: Q / 16 as the B operand in the K operand's dim order, keys below vis are seen
+    constexpr int E = 4096 / VB;  // values of a 16-byte piece of a row
+    h8 qb[QLDS ? 1 : RT][8];
     int vis[RT], vmin = k1;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
@@ -100,17 +223,22 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
         const bool valid = r < rows;
         vis[rt] = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, k1) : 0;
         if (valid) vmin = min(vmin, vis[rt]);
-        const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + 64 * lg;
+        const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + E * lg;
 #pragma unroll
         for (int s = 0; s < 8; s++) {
-            const float4 x0 = *reinterpret_cast<const float4*>(qrow + 8 * s);
-            const float4 x1 = *reinterpret_cast<const float4*>(qrow + 8 * s + 4);
+            if (QLDS && s / 2 != wave) continue;  // (the waves' share)
+            const float* src = qrow + 4 * E * (8 * s / E) + 8 * s % E;
+            const float4 x0 = *reinterpret_cast<const float4*>(src);
+            const float4 x1 = *reinterpret_cast<const float4*>(src + 4);
             const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+            h8 v;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                qb[rt][s][j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
+            for (int j = 0; j < 8; j++) v[j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
+            if constexpr (QLDS) lds.q[rt][s][lane] = v;
+            else qb[rt][s] = v;
         }
     }
+    if constexpr (QLDS) __syncthreads();
     // (uniform: the least over the 16 lanes that hold different rows)
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
@@ -126,73 +254,6 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
         for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    auto place = [&](int kb) { return bt_place(p, table, kb, k1); };
-    KRaw<KVT> kr[KT];
-    VRaw<KVT> vr[4 * KT];
-    // key rows past the range re-read its last one (their probabilities are exact zeros, so what they hold must be finite:
-    // a stale row need not be), groups without a place are zeros
-    auto load_ks = [&](const int* at, int kb) {
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++) {
-            const int last = k1 - 1 - (kb + 16 * kt);
-            const bool live = at[kt] >= 0;
-            const int row = min(i16, last);
-            if (live) {
-                const uint8_t* src = kh + (size_t)at[kt] * VB + (row * VB + (VB / 4) * lg);
-#pragma unroll
-                for (int i = 0; i < VB / 64; i++) {
-                    const uint4 u = ld16(src + 16 * i);
-                    kr[kt].w[4 * i] = u.x; kr[kt].w[4 * i + 1] = u.y; kr[kt].w[4 * i + 2] = u.z; kr[kt].w[4 * i + 3] = u.w;
-                }
-                if constexpr (KVT != QWA_KV_F16)
-                    kr[kt].sc = reinterpret_cast<const uint32_t*>(ksh + (size_t)at[kt] * 8)[row * 4 + lg];
-            } else {
-#pragma unroll
-                for (int i = 0; i < VB / 16; i++) kr[kt].w[i] = 0;
-                kr[kt].sc = 0;
-            }
-        }
-    };
-    auto load_vs = [&](const int* at, int kb) {
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++) {
-            const int last = k1 - 1 - (kb + 16 * kt);
-            const bool live = at[kt] >= 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                VRaw<KVT>& x = vr[4 * kt + j];
-                constexpr int NW = sizeof(x.w) / 4;
-                const int row = min(4 * lg + j, last);
-                if (live) {
-                    const uint8_t* src = vh + (size_t)at[kt] * VB + (row * VB + (VB / 16) * i16);
-                    if constexpr (NW == 2) {
-                        const uint2 u = ld8(src);
-                        x.w[0] = u.x; x.w[1] = u.y;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < NW / 4; i++) {
-                            const uint4 u = ld16(src + 16 * i);
-                            x.w[4 * i] = u.x; x.w[4 * i + 1] = u.y; x.w[4 * i + 2] = u.z; x.w[4 * i + 3] = u.w;
-                        }
-                    }
-                    x.sc = KVT == QWA_KV_F16 ? 0u : vsh[(size_t)at[kt] * 8 + (row * 8 + (i16 >> 1))];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NW; i++) x.w[i] = 0;
-                    x.sc = 0;
-                }
-            }
-        }
-    };
-
-    int kb = k0 + TILE * wave;
-    int at[KT];
-#pragma unroll
-    for (int kt = 0; kt < KT; kt++) at[kt] = place(kb + 16 * kt);
-    if (kb < k1) {
-        load_ks(at, kb);
-        load_vs(at, kb);
-    }
     for (; kb < k1; kb += TILE * BT_WAVES) {
         const int nb = kb + TILE * BT_WAVES;
         int nat[KT];
@@ -203,14 +264,42 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int kt = 0; kt < KT; kt++) S[rt][kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        // a lane's block scales of key i16: piece 4 i + lg of 32 values (Q4_0: block 4 i + lg), or 16 (Q8_0: 2 i + lg / 2)
+        constexpr int NS = KVT == QWA_KV_Q4_0 ? 2 : 4;
+        h2 kd[KT][NS];
+        if constexpr (SC) {
 #pragma unroll
-        for (int s = 0; s < 8; s++)
+            for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                for (int i = 0; i < NS; i++)
+                    kd[kt][i] = KVT == QWA_KV_Q4_0 ? scale_of(ksd[kt], 4 * i16 + 2 * i + (lg >> 1), lg & 1)
+                                                   : scale_of(ksd[kt], 4 * i16 + i, lg >> 1);
+        }
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            h8 ka[KT];
 #pragma unroll
             for (int kt = 0; kt < KT; kt++) {
-                const h8 ka = k_operand<KVT>(kr[kt], s);
+                uint32_t w[4];
+                if constexpr (KVT == QWA_KV_F16) {
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++) S[rt][kt] = mfma16(ka, qb[rt][s], S[rt][kt]);
+                    for (int i = 0; i < 4; i++) w[i] = kr[kt][4 * s + i];
+                } else if constexpr (KVT == QWA_KV_Q8_0) {
+                    q8_word_to_h4(kr[kt][2 * s], kd[kt][s / 2], w);
+                    q8_word_to_h4(kr[kt][2 * s + 1], kd[kt][s / 2], w + 2);
+                } else {
+                    q4_word_to_h8(kr[kt][s], kd[kt][s / 4], w);
+                }
+                ka[kt] = make_h8(w[0], w[1], w[2], w[3]);
             }
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                const h8 b = QLDS ? lds.q[rt][s][lane] : qb[QLDS ? 0 : rt][s];
+#pragma unroll
+                for (int kt = 0; kt < KT; kt++) S[rt][kt] = mfma16(ka[kt], b, S[rt][kt]);
+            }
+            QWA_SB;
+        }
         if (nb < k1) load_ks(nat, nb);
 
         // online softmax: a lane holds keys kb + 16 kt + 4 lg + i of row i16
@@ -233,24 +322,19 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
             }
             float mx = -INFINITY;
 #pragma unroll
-            for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(mx, S[rt][kt][i]);
+            for (int kt = 0; kt < KT; kt++) mx = max3f(max3f(mx, S[rt][kt][0], S[rt][kt][1]), S[rt][kt][2], S[rt][kt][3]);
             mx = rows_max(mx);
             const float mn = mx > m[rt] + PF_RESCALE_T ? mx : m[rt];
-            const float msl = (mn == -INFINITY ? 0.0f : mn) * PF_LOG2E;  // a row that saw nothing keeps l = 0, O = 0
+            const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;  // a row that saw nothing keeps l = 0, O = 0
             cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] * PF_LOG2E - msl);
+            // the sum is that of the rounded probabilities, the weights that P V applies
+            const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
             float rs = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; j++) p8[rt][j] = (_Float16)0.0f;
+            for (int j = 0; j < 8; j++)
+                p8[rt][j] = j < 4 * KT ? (_Float16)fast_exp2(fmaf(S[rt][(j >> 2) % KT][j & 3], PF_LOG2E, -msl)) : (_Float16)0.0f;
 #pragma unroll
-            for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const _Float16 e = (_Float16)fast_exp2(fmaf(S[rt][kt][i], PF_LOG2E, -msl));
-                    p8[rt][4 * kt + i] = e;
-                    rs += (float)e;  // the weights that P V applies
-                }
+            for (int j = 0; j < 4 * KT; j += 2) rs = __builtin_amdgcn_fdot2(h2{p8[rt][j], p8[rt][j + 1]}, one2, rs, false);
             l[rt] = l[rt] * cr[rt] + rs;
             m[rt] = mn;
             moved |= cr[rt] != 1.0f;
@@ -262,14 +346,19 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
                 for (int dt = 0; dt < 16; dt++) o[rt][dt] *= cr[rt];
         }
 
-        // O^T += V^T P^T: output tile dt holds dim 16 i16 + dt
-        constexpr int NW = sizeof(vr[0].w) / 4, DPW = 16 / NW;
+        // O^T += V^T P^T: output tile dt holds the lane's dim dt
+        uint32_t vd[4 * KT];
 #pragma unroll
-        for (int wi = 0; wi < NW; wi++) {
+        for (int j = 0; j < 4 * KT; j++)
+            vd[j] = SC ? h2_bits(scale_of(vsd[j / 4], 4 * (4 * lg + j % 4) + (i16 >> 2), (i16 >> 1) & 1)) & 0xFFFFu : 0u;
+        constexpr int DPW = 16 / VW;
+#pragma unroll
+        for (int wi = 0; wi < VW; wi++) {
+            QWA_SB;
             uint32_t w[2 * KT][DPW];
 #pragma unroll
             for (int h = 0; h < 2 * KT; h++)
-                v_pair_words<KVT, 1>(&vr[2 * h].w[wi], &vr[2 * h + 1].w[wi], vr[2 * h].sc, vr[2 * h + 1].sc, w[h]);
+                v_pair_words<KVT, 1>(&vr[2 * h][wi], &vr[2 * h + 1][wi], vd[2 * h], vd[2 * h + 1], w[h]);
 #pragma unroll
             for (int d = 0; d < DPW; d++)
 #pragma unroll
@@ -286,73 +375,136 @@ __device__ __forceinline__ void bt_body(f4 (*s_o)[16][64], float (*s_ml)[2][64],
         for (int kt = 0; kt < KT; kt++) at[kt] = nat[kt];
     }
 
-    // the waves' states, joined: wave w takes output tiles 4 w .. 4 w + 3 (dims 16 (4 lg + i) + 4 w .. + 3 of the row)
+    // the waves' states, joined in two rounds of 8 output tiles (twice the LDS would cost a workgroup per CU): in round h
+    // wave w takes tiles 8 h + 2 w, 8 h + 2 w + 1
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const float lt = rows_sum(l[rt]);
-        __syncthreads();  // the previous tile's states are read out
-#pragma unroll
-        for (int dt = 0; dt < 16; dt++) s_o[wave][dt][lane] = o[rt][dt];
-        s_ml[wave][0][lane] = m[rt];
-        s_ml[wave][1][lane] = lt;
-        __syncthreads();
-        float M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < BT_WAVES; w++) M = fmaxf(M, s_ml[w][0][lane]);
-        f4 acc[4] = {};
-#pragma unroll
-        for (int w = 0; w < BT_WAVES; w++) {
-            const float mw = s_ml[w][0][lane], lw = s_ml[w][1][lane];
-            const float f = lw == 0.0f ? 0.0f : fast_exp2((mw - M) * PF_LOG2E);  // (lw: NaN scores stay NaN)
-            L = fmaf(f, lw, L);
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const f4 x = s_o[w][4 * wave + t][lane];
-#pragma unroll
-                for (int i = 0; i < 4; i++) acc[t][i] = fmaf(f, x[i], acc[t][i]);
-            }
-        }
         const int r = row0 + 16 * rt + i16;
-        if (r < rows) {
-            const size_t rec = ((size_t)slot * a.n * a.nq + r / GRP) * NH + g * GRP + r % GRP;
-            if (wave == 0 && lg == 0) a.part_ml[rec] = make_float2(M, L);
-            float* dst = a.part_o + rec * HD + 4 * wave;
+        // (rows of one KV head are rstep * token + head of the group apart in the states)
+        const size_t rec = (size_t)rstep * (r / GRP) + r % GRP;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                *reinterpret_cast<float4*>(dst + 16 * (4 * lg + i)) = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
+        for (int h = 0; h < 2; h++) {
+            __syncthreads();  // the previous round's states (or the last tile's Q) are read out
+#pragma unroll
+            for (int dt = 0; dt < 8; dt++) s_o[wave][dt][lane] = o[rt][8 * h + dt];
+            if (h == 0) {
+                s_ml[wave][0][lane] = m[rt];
+                s_ml[wave][1][lane] = lt;
+            }
+            __syncthreads();
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < BT_WAVES; w++) M = fmaxf(M, s_ml[w][0][lane]);
+            f4 acc[2] = {};
+#pragma unroll
+            for (int w = 0; w < BT_WAVES; w++) {
+                const float mw = s_ml[w][0][lane], lw = s_ml[w][1][lane];
+                const float f = lw == 0.0f ? 0.0f : fast_exp2((mw - M) * PF_LOG2E);  // (lw: NaN scores stay NaN)
+                L = fmaf(f, lw, L);
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const f4 x = s_o[w][2 * wave + t][lane];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[t][i] = fmaf(f, x[i], acc[t][i]);
+                }
+            }
+            if (r < rows) {
+                if (h == 0 && wave == 0 && lg == 0) pml[rec] = make_float2(M, L);
+                // (output tile dt of lane row x = 4 lg + i holds dim 16 x + dt, of F16 128 (dt / 8) + 8 x + dt % 8)
+                constexpr int STEP = KVT == QWA_KV_F16 ? 8 : 16;
+                float* dst = po + rec * HD + (KVT == QWA_KV_F16 ? 128 : 8) * h + 2 * wave;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<float2*>(dst + STEP * (4 * lg + i)) = make_float2(acc[0][i], acc[1][i]);
+            }
         }
     }
 }
 
-// the shared positions, for the rows of one group: workgroup = (key range, KV head); slots 0 .. ns - 1
+// the shared positions, for the rows of one group: workgroup = (key range, KV head, row group)
 template <int KVT, int RT>
 __global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(BtCfg<KVT, RT>::WPE)))
-k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int len) {
-    __shared__ f4 s_o[BT_WAVES][16][64];
-    __shared__ float s_ml[BT_WAVES][2][64];
-    const int g = blockIdx.x % NKV, sp = blockIdx.x / NKV;
+k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len, int groups) {
+    __shared__ BtLds<KVT, RT> lds;
+    // the groups of one (range, head) read the same keys: workgroups 8 apart, which one XCD runs
+    const int u = blockIdx.x / (8 * groups) * 8 + blockIdx.x % 8, grp = blockIdx.x / 8 % groups;
+    const int g = u % NKV, sp = u / NKV;
+    if (sp >= ns) return;
     const int b = bt_longest(a, p, threadIdx.x & 63);
     const int k1 = min(min((sp + 1) * len, a.n_shared), bt_len(a, p, b));
     const int seq = bt_seq(a, b);
     const int* table = p.table + (seq >= 0 && seq < p.n_seq ? (size_t)seq * p.ld : 0);
-    bt_body<KVT, RT>(s_o, s_ml, a, kv, p, table, 0, a.n * a.nq * GRP, g, sp * len, k1, 0, sp);
+    const size_t rec = (size_t)sp * a.n * a.nq * NH + g * GRP;
+    bt_body<KVT, RT>(lds, a, kv, p, table, grp * 16 * RT, a.n * a.nq * GRP, g, sp * len, k1, 0, a.part_o + rec * HD,
+                     a.part_ml + rec, NH);
 }
 
-// each sequence's own positions: workgroup = (batch row, key range, KV head, row group); slots first .. first + ns - 1
+// steps of batch row b's own positions (they begin at the multiple of 16 at or before n_shared)
+__device__ __forceinline__ int bt_steps(const BatchArgs& a, const qwa_kv_pages& p, int b) {
+    const int m = bt_len(a, p, b);
+    return m > a.n_shared ? (m - (a.n_shared & ~15) + BT_STEP - 1) / BT_STEP : 0;
+}
+
+// the own positions: workgroup = (slice of the steps, KV head, row group), one segment per sequence that the slice meets
 template <int KVT, int RT>
 __global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(BtCfg<KVT, RT>::WPE)))
-k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len, int first, int groups) {
-    __shared__ f4 s_o[BT_WAVES][16][64];
-    __shared__ float s_ml[BT_WAVES][2][64];
-    // the groups of one (row, range, head) read the same keys: workgroups 8 apart, which one XCD runs
+k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
+    __shared__ BtLds<KVT, RT> lds;
+    // the groups of one (slice, head) read the same keys: workgroups 8 apart, which one XCD runs
     const int u = blockIdx.x / (8 * groups) * 8 + blockIdx.x % 8, grp = blockIdx.x / 8 % groups;
-    const int pairs = ns * NKV, b = u / pairs, pr = u % pairs, g = pr % NKV, sp = pr / NKV;
-    if (b >= a.n) return;
-    const int begin = a.n_shared + sp * len, k1 = min(begin + len, bt_len(a, p, b));
-    if (begin >= k1) return;  // k_bt_combine does not read this slot
-    // (tiles start at multiples of 16; positions before `begin` are masked)
-    bt_body<KVT, RT>(s_o, s_ml, a, kv, p, p.table + (size_t)bt_seq(a, b) * p.ld, b * a.nq * GRP + grp * 16 * RT,
-                     (b + 1) * a.nq * GRP, g, begin & ~15, k1, begin, first + sp);
+    const int g = u % NKV, w = u / NKV, lane = threadIdx.x & 63;
+    if (w >= a.wgs) return;
+    // where the batch rows begin: every wave sums the steps of n / 64 rows a lane
+    const int per = (a.n + 63) / 64;
+    int mine = 0;
+    for (int j = 0; j < per; j++) mine += lane * per + j < a.n ? bt_steps(a, p, lane * per + j) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += y;
+    }
+    const int total = __builtin_amdgcn_readlane(upto, 63);
+    if (blockIdx.x == 0 && threadIdx.x < 64) {
+        int s = upto - mine;
+        for (int j = 0; j < per; j++)
+            if (lane * per + j < a.n) {
+                a.begin[lane * per + j] = s;
+                s += bt_steps(a, p, lane * per + j);
+            }
+        if (lane == 0) a.begin[a.n] = total;
+    }
+    const int slices = min(a.wgs, total);  // (none is empty)
+    if (w >= slices) return;
+    int s = (int)((long long)w * total / slices);
+    const int end = (int)((long long)(w + 1) * total / slices);
+    // the batch row that holds step s
+    const int at = __builtin_ctzll(__ballot(upto > s));
+    int b = at * per, first = __builtin_amdgcn_readlane(upto - mine, at);
+    int m = bt_steps(a, p, b);
+    while (s >= first + m) {
+        first += m;
+        m = bt_steps(a, p, ++b);
+    }
+    const int base = a.n_shared & ~15;
+    while (true) {
+        const int stop = min(end, first + m);
+        const int k0 = base + (s - first) * BT_STEP, k1 = min(base + (stop - first) * BT_STEP, bt_len(a, p, b));
+        const size_t rec = ((size_t)g * (a.wgs + a.n) + w + b) * a.nq * GRP;
+        // (row r = 6 * token + head has place r - 6 nq b of the segment)
+        float* po = a.own_o + ((ptrdiff_t)rec - (ptrdiff_t)b * a.nq * GRP) * HD;
+        float2* pml = a.own_ml + ((ptrdiff_t)rec - (ptrdiff_t)b * a.nq * GRP);
+        bt_body<KVT, RT>(lds, a, kv, p, p.table + (size_t)bt_seq(a, b) * p.ld, b * a.nq * GRP + grp * 16 * RT,
+                         (b + 1) * a.nq * GRP, g, k0, k1, a.n_shared, po, pml, GRP);
+        s = stop;
+        if (s >= end) break;
+        do {
+            first += m;
+            m = bt_steps(a, p, ++b);
+        } while (m == 0);
+        __syncthreads();  // the last segment's states are read out of LDS
+    }
 }
 
 // The shared positions for PF_ROWS rows: workgroup = (row block, tile range, KV head).  The 8 waves have 32 rows each, two a
@@ -604,57 +756,87 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
     }
 }
 
-// Joins a row's partial states in a fixed order, gates, rounds: one wave per row (token * NH + head), 4 dims per lane.  The
-// weights exp(m - M) come one state a lane, 64 at a time; the states' rows are read eight at a time.
+// Joins a row's partial states in a fixed order, gates, rounds: WPR waves per row (token * NH + head), 4 dims per lane.  The
+// weights exp(m - M) come one state a lane, 64 at a time; wave k of a row reads the states' rows k, k + WPR, ..., eight at
+// a time.
+template <int WPR>
 __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p, const float* __restrict__ gate, int nt,
-                                                    int ns_shared, int ns_own, int len_own,
-                                                    uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+                                                    int ns_shared, uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {
+    __shared__ float4 s_o[WPR > 1 ? 4 : 1][64];
+    const int wave = threadIdx.x >> 6, part = wave % WPR, lane = threadIdx.x & 63;
+    const int row = blockIdx.x * (4 / WPR) + wave / WPR;
     const int nrows = a.n * a.nq * NH;
-    if (row >= nrows) return;
-    const int mine = bt_len(a, p, row / NH / a.nq) - a.n_shared;  // own positions
-    const int ns = ns_shared + (mine > 0 ? min(ns_own, (mine + len_own - 1) / len_own) : 0);
-    // (m, l, scale) of state s: the tile workgroups' states first, then the register workgroups'
+    if (row >= nrows) return;  // (all waves of a row, and with WPR = 4 of a workgroup)
+    const int tok = row / NH, b = tok / a.nq, h = row % NH;
+    // the batch row's segments: those of the slices from its first step's to its last one's
+    int segs = 0;
+    size_t seg0 = 0;
+    if (a.wgs > 0) {
+        const long long s0 = a.begin[b], s1 = a.begin[b + 1], total = a.begin[a.n];
+        if (s1 > s0) {
+            const long long slices = min((long long)a.wgs, total);
+            const int w0 = (int)(((s0 + 1) * slices - 1) / total), w1 = (int)((s1 * slices - 1) / total);
+            segs = w1 - w0 + 1;
+            seg0 = ((size_t)(h / GRP) * (a.wgs + a.n) + w0 + b) * a.nq * GRP + (tok % a.nq) * GRP + h % GRP;
+        }
+    }
+    const int fixed = nt + ns_shared, all = fixed + segs;
+    // (m, l, scale) of state s: the tile workgroups' states, the shared ranges', the own segments'
     auto state = [&](int s) {
         if (s < nt) return a.tile_ml[(size_t)s * nrows + row];
-        if (s < nt + ns) {
-            const float2 ml = a.part_ml[(size_t)(s - nt) * nrows + row];
-            return make_float4(ml.x, ml.y, 1.0f, 0.0f);
-        }
-        return make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        if (s >= all) return make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        const float2 ml = s < fixed ? a.part_ml[(size_t)(s - nt) * nrows + row]
+                                    : a.own_ml[seg0 + (size_t)(s - fixed) * a.nq * GRP];
+        return make_float4(ml.x, ml.y, 1.0f, 0.0f);
     };
     float M = -INFINITY;
-    for (int s0 = 0; s0 < nt + ns; s0 += 64) M = fmaxf(M, state(s0 + lane).x);
+    for (int s0 = 0; s0 < all; s0 += 64) M = fmaxf(M, state(s0 + lane).x);
     M = wave_max(M);
     float L = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     constexpr int U = 8;
-    for (int s0 = 0; s0 < nt + ns; s0 += 64) {
+    for (int s0 = 0; s0 < all; s0 += 64) {
         const PfPartMl ml = state(s0 + lane);
         // a state that saw nothing weighs nothing; one of NaN scores (l is NaN) makes the row NaN
         const float f = ml.y == 0.0f ? 0.0f : fast_exp2((ml.x - M) * PF_LOG2E);
         L += wave_sum(f * ml.y);
         // tile states hold O / l in steps of the scale, register states O
-        const float w = f * ml.z * (s0 + lane < nt ? ml.y : 1.0f);
-        const int most = min(64, nt + ns - s0);
-        for (int k = 0; k < most; k += U) {
+        const float wt = f * ml.z * (s0 + lane < nt ? ml.y : 1.0f);
+        const int most = min(64, all - s0);
+        for (int k = part; k < most; k += U * WPR) {
             float4 x[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int s = s0 + min(k + u, most - 1);
+                const int s = s0 + min(k + u * WPR, most - 1);
                 if (s < nt) x[u] = unpack16x4(a.tile_o[((size_t)s * nrows + row) * (HD / 4) + lane]);
-                else x[u] = *reinterpret_cast<const float4*>(a.part_o + ((size_t)(s - nt) * nrows + row) * HD + 4 * lane);
+                else
+                    x[u] = *reinterpret_cast<const float4*>(
+                        (s < fixed ? a.part_o + ((size_t)(s - nt) * nrows + row) * HD
+                                   : a.own_o + (seg0 + (size_t)(s - fixed) * a.nq * GRP) * HD) + 4 * lane);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const float fu = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), min(k + u, 63)));
-                if (k + u < most) {
+                const float fu = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wt), min(k + u * WPR, 63)));
+                if (k + u * WPR < most) {
                     acc.x = fmaf(fu, x[u].x, acc.x);
                     acc.y = fmaf(fu, x[u].y, acc.y);
                     acc.z = fmaf(fu, x[u].z, acc.z);
                     acc.w = fmaf(fu, x[u].w, acc.w);
                 }
             }
+        }
+    }
+    if constexpr (WPR > 1) {
+        s_o[wave][lane] = acc;
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (int k = 1; k < WPR; k++) {
+            const float4 x = s_o[wave + k][lane];
+            acc.x += x.x;
+            acc.y += x.y;
+            acc.z += x.z;
+            acc.w += x.w;
         }
     }
     const float4 gv = *reinterpret_cast<const float4*>(gate + (size_t)row * HD + 4 * lane);
@@ -699,13 +881,14 @@ static void launch_ranges(const BatchArgs& a, const qwa_kv_layer& kv, const qwa_
     if (b.nt > 0)
         hipLaunchKernelGGL(k_bt_tiles<KVT>, dim3(b.blocks * b.nt * NKV), dim3(PF_THREADS), 0, st, a, kv, p, b.blocks, b.nt);
     if (b.ns_shared > 0) {
-        if (b.rt_shared == 1) QWA_BT(k_bt_shared, 1, b.ns_shared * NKV, b.len_shared);
-        else QWA_BT(k_bt_shared, 2, b.ns_shared * NKV, b.len_shared);
+        const int grid = (b.ns_shared * NKV + 7) / 8 * 8 * b.groups_shared;
+        if (b.rt_shared == 1) QWA_BT(k_bt_shared, 1, grid, b.ns_shared, b.len_shared, b.groups_shared);
+        else QWA_BT(k_bt_shared, 2, grid, b.ns_shared, b.len_shared, b.groups_shared);
     }
-    if (b.ns_own > 0) {
-        const int grid = (a.n * b.ns_own * NKV + 7) / 8 * 8 * b.groups;
-        if (b.rt_own == 1) QWA_BT(k_bt_own, 1, grid, b.ns_own, b.len_own, b.ns_shared, b.groups);
-        else QWA_BT(k_bt_own, 2, grid, b.ns_own, b.len_own, b.ns_shared, b.groups);
+    if (b.wgs > 0) {
+        const int grid = (b.wgs * NKV + 7) / 8 * 8 * b.groups;
+        if (b.rt_own == 1) QWA_BT(k_bt_own, 1, grid, b.groups);
+        else QWA_BT(k_bt_own, 2, grid, b.groups);
     }
 #undef QWA_BT
 }
@@ -717,15 +900,23 @@ hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_l
     const BatchWork w = batch_work(b, n, nq);
     uint8_t* base = static_cast<uint8_t*>(work);
     const BatchArgs a{q, seqs, reinterpret_cast<PfPartO*>(base + w.tile_o), reinterpret_cast<PfPartMl*>(base + w.tile_ml),
-                      reinterpret_cast<float*>(base + w.o), reinterpret_cast<float2*>(base + w.ml), n, nq, n_shared, max_len};
+                      reinterpret_cast<float*>(base + w.o), reinterpret_cast<float2*>(base + w.ml),
+                      reinterpret_cast<float*>(base + w.own_o), reinterpret_cast<float2*>(base + w.own_ml),
+                      reinterpret_cast<int*>(base + w.begin), n, nq, n_shared, max_len, b.wgs};
     switch (kvt) {
         case QWA_KV_F16: launch_ranges<QWA_KV_F16>(a, kv, p, b, st); break;
         case QWA_KV_Q8_0: launch_ranges<QWA_KV_Q8_0>(a, kv, p, b, st); break;
         default: launch_ranges<QWA_KV_Q4_0>(a, kv, p, b, st); break;
     }
     const qwa_act_q8 act = oq ? *oq : qwa_act_q8{nullptr, nullptr, nullptr};
-    hipLaunchKernelGGL(k_bt_combine, dim3((unsigned)(((size_t)n * nq * NH + 3) / 4)), dim3(256), 0, st, a, p, gate, b.nt,
-                       b.ns_shared, b.ns_own, b.len_own, out16, act, oq != nullptr ? 1 : 0);
+    // few rows with many states: a workgroup per row
+    const int rows = n * nq * NH;
+    if (rows <= BT_ROWS4)
+        hipLaunchKernelGGL(k_bt_combine<4>, dim3(rows), dim3(256), 0, st, a, p, gate, b.nt, b.ns_shared, out16, act,
+                           oq != nullptr ? 1 : 0);
+    else
+        hipLaunchKernelGGL(k_bt_combine<1>, dim3((rows + 3) / 4), dim3(256), 0, st, a, p, gate, b.nt, b.ns_shared, out16,
+                           act, oq != nullptr ? 1 : 0);
     return hipGetLastError();
 }
 

@@ -14,30 +14,35 @@ namespace qwa {
 
 constexpr int BT_WAVES = 4;   // waves of a register workgroup; they take the tiles of its key range in turn
 constexpr int BT_MAXRT = 2;   // 16-row MFMA tiles of such a workgroup at most
-constexpr int BT_STEP = 128;  // its key ranges are multiples of this
+#ifndef QWA_FILL
+#define QWA_FILL 768
+#endif
+constexpr int BT_STEP = 128;  // positions of a step; key ranges are whole steps
 constexpr int BT_FEW = 32;    // rows of a KV head up to which the shared positions are left to register workgroups
 
-// Key range [0, n_shared) for all rows together, and [n_shared, len) of every sequence by itself, each cut so that the
-// workgroups fill the chip.
-//  register workgroups (k_bt_shared, k_bt_own): up to BT_MAXRT row tiles, key ranges of fixed length;
-//  tile workgroups (k_bt_tiles): PF_ROWS rows, the shared PF_TILE-key tiles in nt ranges of about equal length.
+// The shared positions [0, n_shared) are worked on for all rows together, the positions of its own [n_shared, len) for every
+// sequence by itself.
+//  tile workgroups (k_bt_tiles): PF_ROWS rows, the shared PF_TILE-key tiles in nt ranges of about equal length;
+//  register workgroups over the shared positions (k_bt_shared): up to BT_MAXRT row tiles, key ranges of fixed length;
+//  register workgroups over the own positions (k_bt_own): the steps of BT_STEP positions of all sequences in a row, cut
+//  into wgs slices of equal length (the kernel knows the sequences' lengths, the plan only their bound), each worked on as
+//  one segment per sequence that it meets.
 struct BatchPlan {
-    int blocks, nt;              // row blocks and key ranges of the tile workgroups (0: none)
-    int ns_shared, len_shared;   // key ranges of register workgroups over the shared positions, and their length
-    int rt_shared;
-    int groups, rt_own;          // row groups of a sequence, and the row tiles of a group
-    int ns_own, len_own;
-    int slots() const { return ns_shared + ns_own; }  // fp32 partial states of a row
+    int blocks, nt;                // row blocks and key ranges of the tile workgroups (0: none)
+    int groups_shared, rt_shared;  // row groups of the batch, and the row tiles of a group
+    int ns_shared, len_shared;     // key ranges of register workgroups over the shared positions, and their length
+    int groups, rt_own;            // row groups of a sequence, and the row tiles of a group
+    int wgs;                       // slices of the own steps (0: no own positions)
 };
 
-inline void bt_cut(int positions, int units, int most, int* ns, int* len) {
+inline void bt_cut(int positions, int units, int fill, int most, int* ns, int* len) {
     if (positions <= 0) {
         *ns = 0;
         *len = BT_STEP;
         return;
     }
     const int steps = (positions + BT_STEP - 1) / BT_STEP;
-    const int want = std::min(std::min(most, steps), std::max(1, (512 + units - 1) / units));
+    const int want = std::min(std::min(most, steps), std::max(1, fill / units));
     *len = (steps + want - 1) / want * BT_STEP;
     *ns = (positions + *len - 1) / *len;
 }
@@ -45,7 +50,8 @@ inline void bt_cut(int positions, int units, int most, int* ns, int* len) {
 inline BatchPlan batch_plan(int n, int nq, int n_shared, int max_len) {
     BatchPlan p = {};
     const int rows = n * nq * GRP, own = nq * GRP;
-    p.rt_shared = std::min((rows + 15) / 16, BT_MAXRT);
+    p.rt_shared = rows <= 16 ? 1 : BT_MAXRT;
+    p.groups_shared = (rows + 16 * p.rt_shared - 1) / (16 * p.rt_shared);
     p.rt_own = std::min((own + 15) / 16, BT_MAXRT);
     p.groups = (own + 16 * p.rt_own - 1) / (16 * p.rt_own);
     if (rows > BT_FEW && n_shared > 0) {
@@ -54,26 +60,34 @@ inline BatchPlan batch_plan(int n, int nq, int n_shared, int max_len) {
         p.nt = std::min(tiles, std::max(1, 256 / (p.blocks * NKV)));
         p.len_shared = BT_STEP;
     } else {
-        bt_cut(n_shared, NKV, 128, &p.ns_shared, &p.len_shared);
+        bt_cut(n_shared, p.groups_shared * NKV, 512, 128, &p.ns_shared, &p.len_shared);
     }
-    bt_cut(max_len - n_shared, n * p.groups * NKV, 128, &p.ns_own, &p.len_own);
+    if (max_len > n_shared) {
+        const long long steps = (long long)n * ((max_len - (n_shared & ~15) + BT_STEP - 1) / BT_STEP);
+        p.wgs = (int)std::min<long long>(steps, std::max(1, QWA_FILL / (NKV * p.groups)));
+    }
     return p;
 }
 
-// Partial states in the work buffer, each [slot][row] with row = token * NH + head: of the tile workgroups O / l as 16-bit
-// fixed point [256] and (m, l, scale, -), of the register workgroups O as fp32 [256] and (m, l).
+// Partial states in the work buffer: of the tile workgroups O / l as 16-bit fixed point [256] and (m, l, scale, -), of the
+// register workgroups O as fp32 [256] and (m, l).  Those over the shared positions are [range][row] with row = token * NH +
+// head.  Segment (slice w, batch row b) of the own positions has number w + b (both only grow along the steps, one of them
+// with each segment): [KV head][segment][query * GRP + head of the group].  begin: the step at which each batch row begins,
+// and the total.
 struct BatchWork {
-    size_t tile_o, tile_ml, o, ml, bytes;  // byte offsets
+    size_t tile_o, tile_ml, o, ml, own_o, own_ml, begin, bytes;  // byte offsets
 };
 inline BatchWork batch_work(const BatchPlan& p, int n, int nq) {
-    const size_t rows = (size_t)n * nq * NH;
+    const size_t rows = (size_t)n * nq * NH, own = p.wgs ? (size_t)NKV * (p.wgs + n) * nq * GRP : 0;
     BatchWork w;
     w.tile_o = 0;
     w.tile_ml = w.tile_o + p.nt * rows * HD * 2;
     w.o = w.tile_ml + p.nt * rows * 16;
-    w.ml = w.o + p.slots() * rows * HD * 4;
-    w.bytes = w.ml + p.slots() * rows * 8;
-    if (w.bytes == 0) w.bytes = 16;
+    w.ml = w.o + p.ns_shared * rows * HD * 4;
+    w.own_o = w.ml + p.ns_shared * rows * 8;
+    w.own_ml = w.own_o + own * HD * 4;
+    w.begin = w.own_ml + own * 8;
+    w.bytes = w.begin + 4 * ((size_t)n + 1);
     return w;
 }
 

@@ -169,22 +169,33 @@ int main() {
             if (shared > most) continue;
             const BatchPlan p = batch_plan(n, nq, shared, most);
             const BatchWork w = batch_work(p, n, nq);
-            const long long rows = (long long)n * nq * NH;
+            const size_t rows = (size_t)n * nq * NH;
             CHECK(p.groups * p.rt_own * 16 >= nq * GRP && p.rt_own <= BT_MAXRT, "rows of a sequence\n");
             CHECK(shared == 0 || (p.nt > 0) != (p.ns_shared > 0), "the shared positions: one kind of workgroup\n");
             CHECK(p.nt == 0 || p.blocks * PF_ROWS >= n * nq * GRP, "rows of the batch\n");
             CHECK(p.nt * (long long)PF_TILE < shared + PF_TILE, "an empty range\n");
-            CHECK(p.ns_shared == 0 || p.rt_shared * 16 >= n * nq * GRP, "rows of the batch\n");
+            CHECK(p.groups_shared * p.rt_shared * 16 >= n * nq * GRP, "rows of the batch\n");
             CHECK(p.nt > 0 || (long long)p.ns_shared * p.len_shared >= shared, "shared\n");
-            CHECK((long long)p.ns_own * p.len_own >= most - shared && (most > shared) == (p.ns_own > 0), "own\n");
             CHECK(p.ns_shared == 0 || (long long)(p.ns_shared - 1) * p.len_shared < shared, "an empty range\n");
-            CHECK(p.ns_own == 0 || (long long)(p.ns_own - 1) * p.len_own < most - shared, "an empty range\n");
             CHECK(p.len_shared % 16 == 0, "a range that begins inside 16 keys\n");
-            CHECK(p.slots() + p.nt >= 1, "no range\n");
-            CHECK((long long)p.blocks * p.nt * NKV < 1LL << 31 && (long long)n * p.ns_own * NKV * p.groups < 1LL << 31,
-                  "grid\n");
-            CHECK(w.bytes >= (size_t)(rows * (p.nt * (HD * 2 + 16) + p.slots() * (HD * 4 + 8))) && w.tile_ml % 16 == 0 &&
-                  w.o % 16 == 0 && w.ml % 16 == 0, "work buffer\n");
+            CHECK((most > shared) == (p.wgs > 0), "own\n");
+            CHECK(p.wgs + p.ns_shared + p.nt >= 1, "no range\n");
+            CHECK((long long)p.blocks * p.nt * NKV < 1LL << 31 && (long long)p.wgs * NKV * p.groups < 1LL << 31 &&
+                  (long long)p.ns_shared * NKV * p.groups_shared < 1LL << 31, "grid\n");
+            const size_t own = p.wgs ? (size_t)NKV * (p.wgs + n) * nq * GRP : 0;
+            CHECK(w.bytes >= rows * (p.nt * (HD * 2 + 16) + p.ns_shared * (HD * 4 + 8)) + own * (HD * 4 + 8) + 4 * (n + 1) &&
+                  w.tile_ml % 16 == 0 && w.o % 16 == 0 && w.ml % 8 == 0 && w.own_o % 16 == 0 && w.own_ml % 8 == 0 &&
+                  w.begin % 4 == 0, "work buffer\n");
+        }
+    }
+    // slices and segments: every step lies in the slice that the combine looks for it in, segment numbers are unique
+    for (int wgs : {1, 2, 7, 192}) for (int total : {1, 2, 5, 191, 192, 193, 2048, 2097152}) {
+        const int slices = std::min(wgs, total);
+        for (int w = 0; w < slices; w++) {
+            const long long lo = (long long)w * total / slices, hi = (long long)(w + 1) * total / slices;
+            CHECK(lo < hi, "empty slice\n");
+            for (long long x : {lo, (lo + hi) / 2, hi - 1})
+                if (x < hi) CHECK(((x + 1) * slices - 1) / total == w, "step %lld of %d in slice %d\n", x, total, w);
         }
     }
     return 0;
