@@ -8,9 +8,8 @@
 //  * Register workgroups (k_bt_own, and k_bt_shared for the shared positions of few rows) have one KV head and up to
 //    BT_MAXRT 16-row tiles (row 6 * token + head of that KV head); their waves take the tiles of the key range in turn, each
 //    with its own running maximum, sum and O, and merge at the end through LDS.
-//  * Tile workgroups (k_bt_tiles, the shared positions of more rows) have PF_ROWS rows, 32 a wave: a tile's raw bytes come
-//    to LDS by direct loads, all waves dequantize them into fp16 tiles there once, and every wave multiplies its rows with
-//    them, as in the prefill's raw-tile kernels but with pages for addresses and a bound per row for the mask.
+//  * Tile workgroups (k_bt_tiles, the shared positions of more rows) have BT_TROWS rows, 16 a wave: each tile is dequantized
+//    once into LDS, by way of registers, and every wave multiplies its rows with it.
 //  * Pages are multiples of 16 positions and tiles start at multiples of 16, so each 16 keys lie in one page: a tile's page
 //    numbers are wave-uniform scalar loads, one tile ahead.
 //  * S^T = K Q^T and O^T += V^T P^T on fp16 MFMA with fp32 accumulation.  A lane loads 64 dims of one key and 16 dims of the
@@ -24,6 +23,14 @@
 
 namespace qwa {
 
+#ifndef QWA_KD
+#define QWA_KD 1
+#endif
+#ifndef QWA_VD
+#define QWA_VD 3
+#endif
+constexpr int BT_KD = QWA_KD;  // K steps read ahead of their MFMAs
+constexpr int BT_VD = QWA_VD;  // V fragments in flight
 #ifndef QWA_ROWS4
 #define QWA_ROWS4 3072
 #endif
@@ -507,19 +514,124 @@ k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
     }
 }
 
-// The shared positions for PF_ROWS rows: workgroup = (row block, tile range, KV head).  The 8 waves have 32 rows each, two a
-// SIMD: the softmax and dequantization of one issue while the other's MFMAs run.
+// What a thread converts of a tile, u = t & 255.  Waves 0 .. 3 (V): dims 8 c .. 8 c + 7 (c = u & 31) of the four keys 16 h +
+// 4 cb .. + 3 (h = (u >> 5) & 1, cb = u >> 6), which are neighbours in the P^T operand's key order.  Waves 4 .. 7 (K): the 32
+// dims of block u & 7 of key u >> 3.  The raw bytes are in registers, loaded one tile ahead.
 template <int KVT>
-__global__ void __launch_bounds__(PF_THREADS) __attribute__((amdgpu_waves_per_eu(PF_WAVES / 4, PF_WAVES / 4)))
+struct BtRaw {
+    static constexpr int VB = value_bytes(KVT);
+    uint32_t w[VB / 32];  // V: 4 rows of VB / 128 words; K: VB / 32 words of one row
+    uint32_t sc[2];       // V: the rows' block scales in halves; K: the block's scale
+};
+
+// rows past the half's last valid one (last[h]) read that one; a half without a place (at[h] < 0) reads position 0 of the
+// pool, and its V becomes zeros: its probabilities are, and what was read need not be finite
+template <int KVT>
+__device__ __forceinline__ void bt_raw_load(BtRaw<KVT>& r, const qwa_kv_layer& kv, size_t head, const int* at,
+                                            const int* last, int t, bool is_v) {
+    constexpr int VB = BtRaw<KVT>::VB, NW = VB / 32;
+    const int u = t & 255, h = is_v ? (u >> 5) & 1 : u >> 7;
+    const int place = h ? at[1] : at[0], end = h ? last[1] : last[0];
+    const size_t row0 = head + max(place, 0);
+    if (is_v) {
+        const int k0 = 4 * (u >> 6), c = u & 31;
+        uint32_t s[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const size_t row = row0 + max(min(k0 + j, end), 0);
+            const uint8_t* src = kv.v + row * VB + (VB / 32) * c;
+            if constexpr (KVT == QWA_KV_Q4_0) {
+                r.w[j] = *reinterpret_cast<const uint32_t*>(src);
+            } else if constexpr (KVT == QWA_KV_Q8_0) {
+                const uint2 x = ld8(src);
+                r.w[2 * j] = x.x; r.w[2 * j + 1] = x.y;
+            } else {
+                const uint4 x = ld16(src);
+                r.w[4 * j] = x.x; r.w[4 * j + 1] = x.y; r.w[4 * j + 2] = x.z; r.w[4 * j + 3] = x.w;
+            }
+            s[j] = KVT == QWA_KV_F16 ? 0u : kv.vs[row * 8 + (c >> 2)];
+        }
+        r.sc[0] = s[0] | s[1] << 16;
+        r.sc[1] = s[2] | s[3] << 16;
+        if (place < 0) {
+#pragma unroll
+            for (int i = 0; i < NW; i++) r.w[i] = 0;
+            r.sc[0] = r.sc[1] = 0;
+        }
+    } else {
+        const size_t row = row0 + max(min((u >> 3) & 15, end), 0);
+        const uint8_t* src = kv.k + row * VB + (VB / 8) * (u & 7);
+#pragma unroll
+        for (int i = 0; i < NW / 4; i++) {
+            const uint4 x = ld16(src + 16 * i);
+            r.w[4 * i] = x.x; r.w[4 * i + 1] = x.y; r.w[4 * i + 2] = x.z; r.w[4 * i + 3] = x.w;
+        }
+        r.sc[0] = KVT == QWA_KV_F16 ? 0u : kv.ks[row * 8 + (u & 7)];
+    }
+}
+
+// Into the fp16 tiles, in 16-byte units so ordered that the 16 lanes that the LDS serves together (0-3, 12-15, 20-23, 24-27,
+// and so on) reach distinct banks: the unit's place modulo 16 is the reading lane's i16, or that XOR a number that such lanes
+// have in common.
+//  K: unit (c, key) at 32 c + (key ^ 2 (c / 4)): dims 8 c .. 8 c + 7 in the operand's order;
+//  V^T: unit (cb, slot) at 256 cb + slot: keys 8 cb .. 8 cb + 7 in the P^T operand's order (4 cb + 16 h + j at 4 h + j) of the
+//  dim 8 (slot % 32) + slot / 32, so that the writing lanes (c = slot % 32) lie side by side, too.
+// (Rows of 528 and 80 bytes instead: half of the LDS cycles were conflicts; 128 sequences over 32768 Q4_0 positions 163 us.)
+template <int KVT>
+__device__ __forceinline__ void bt_raw_store(const BtRaw<KVT>& r, _Float16* Ks, _Float16* Vt, int t, bool is_v) {
+    constexpr int VB = BtRaw<KVT>::VB;
+    const int u = t & 255;
+    if (is_v) {
+        constexpr int VW = VB / 128, DPW = 8 / VW;  // words of a row, dims of a word
+        _Float16* dst = Vt + 8 * (256 * (u >> 6) + (u & 31)) + 4 * ((u >> 5) & 1);
+#pragma unroll
+        for (int i = 0; i < VW; i++) {
+            uint32_t lo[DPW], hi[DPW];
+            v_pair_words<KVT, 1>(&r.w[i], &r.w[VW + i], r.sc[0] & 0xFFFFu, r.sc[0] >> 16, lo);
+            v_pair_words<KVT, 1>(&r.w[2 * VW + i], &r.w[3 * VW + i], r.sc[1] & 0xFFFFu, r.sc[1] >> 16, hi);
+#pragma unroll
+            for (int d = 0; d < DPW; d++) *reinterpret_cast<uint2*>(dst + 8 * 32 * (DPW * i + d)) = make_uint2(lo[d], hi[d]);
+        }
+    } else {
+        _Float16* dst = Ks + 8 * (32 * 4 * (u & 7) + ((u >> 3) ^ (2 * (u & 7))));
+        const h2 d = scale_pair((uint16_t)r.sc[0], (uint16_t)r.sc[0]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t o[4];
+            if constexpr (KVT == QWA_KV_F16) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) o[k] = r.w[4 * i + k];
+            } else if constexpr (KVT == QWA_KV_Q8_0) {
+                q8_word_to_h4(r.w[2 * i], d, o);
+                q8_word_to_h4(r.w[2 * i + 1], d, o + 2);
+            } else {
+                q4_word_to_h8(r.w[i], d, o);
+            }
+            *reinterpret_cast<uint4*>(dst + 8 * 32 * i) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+}
+
+// The shared positions for BT_TROWS rows: workgroup = (row block, tile range, KV head).  The 12 waves have 16 rows each,
+// three a SIMD: of those one converts V at the start of an iteration, one K at its end, one nothing, so the MFMAs of one run
+// while others convert, take exponentials or wait for LDS.  (32 rows a wave, two a SIMD, read half as much LDS per row, but
+// each wave's chain of LDS reads, MFMAs and softmax steps took 3.3 us a tile.)
+template <int KVT>
+__global__ void __launch_bounds__(64 * BT_TWAVES) __attribute__((amdgpu_waves_per_eu(BT_TWAVES / 4, BT_TWAVES / 4)))
 k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
-    static_assert(PF_THREADS == 512 && PF_KT == 2, "the conversion's units are the workgroup's threads");
-    using L = PfRaw<KVT>;
-    constexpr int VB = L::VB, NBUF = L::NBUF, AHEAD = L::AHEAD;
-    __shared__ __attribute__((aligned(16))) uint8_t s_raw[NBUF][L::BYTES];
-    __shared__ __attribute__((aligned(16))) _Float16 s_k[2][PF_TILE * KS_LD];
-    __shared__ __attribute__((aligned(16))) _Float16 s_vt[2][HD * VT_LD];
+    constexpr int XCH = 16 * 64 * 8;  // bytes of a wave's exchange of its rows' state
+    __shared__ __attribute__((aligned(16))) union {
+        struct {
+            _Float16 k[2][PF_TILE * HD];
+            _Float16 vt[2][PF_TILE * HD];
+        } tile;
+        uint2 xch[BT_TWAVES][XCH / 8];
+    } lds;
+    auto& s_k = lds.tile.k;
+    auto& s_vt = lds.tile.vt;
     const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const bool is_v = wave < 4, converts = wave < 8;
     // workgroups 8 apart run on one XCD: those of a (KV head, range) pair read the same tiles
     int pair = blockIdx.x / blocks, blk = blockIdx.x % blocks;
     if (NKV * ns % 8 == 0) {
@@ -534,225 +646,174 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
     const int all = (a.n_shared + PF_TILE - 1) / PF_TILE;
     const int tb = (int)((long long)sp * all / ns), te = (int)((long long)(sp + 1) * all / ns);
     const int nt = min(te, (end + PF_TILE - 1) / PF_TILE) - tb;  // (a batch shorter than its shared part: fewer, or none)
-
-    const int nrows = a.n * a.nq * GRP, wrow0 = blk * PF_ROWS + 32 * wave;
+    const int nrows = a.n * a.nq * GRP, wrow0 = blk * BT_TROWS + 16 * wave;
     const size_t head = (size_t)g * kv.capacity;
-    const int nvm = L::count(wave);
-    uint32_t raw_lds[NBUF];
-#pragma unroll
-    for (int b = 0; b < NBUF; b++) raw_lds[b] = lds_addr(s_raw[b]);
 
-    // Direct-to-LDS loads of a tile, its halves of 16 keys at pool positions at0, at1 (-1: dead, position 0 is read in its
-    // place); keys at or past the end re-read the last one of their half
-    auto issue = [&](int buf, int k0, int at0, int at1) {
-        const size_t base[2] = {head + max(at0, 0), head + max(at1, 0)};
-        const int last[2] = {min(15, end - 1 - k0), min(15, end - 17 - k0)};
-#pragma unroll
-        for (int c = 0; c < (L::NKV + PF_WAVES - 1) / PF_WAVES; c++) {
-            const int ik = wave + PF_WAVES * c, iv = (wave + PF_WAVES / 2) % PF_WAVES + PF_WAVES * c;
-            auto piece = [&](int i, const uint8_t* src, uint32_t dst) {
-                const int h = i >= L::NKV / 2, q = 1024 * (i - h * (L::NKV / 2)) + 16 * lane;
-                const int row = min(q / VB, max(h ? last[1] : last[0], 0));
-                dma_sv<16>(dst + 1024 * i, src + (h ? base[1] : base[0]) * VB, (uint32_t)(row * VB + q % VB));
-            };
-            if (ik < L::NKV) piece(ik, kv.k, raw_lds[buf] + L::K);
-            if (iv < L::NKV) piece(iv, kv.v, raw_lds[buf] + L::V);
-        }
-        if constexpr (L::SC != 0) {
-            const int j = wave & 1;
-            const uint32_t off = (uint32_t)(min(lane / 4, max(j ? last[1] : last[0], 0)) * 16 + 4 * (lane & 3));
-            if (wave >= PF_WAVES - 2) dma_sv<4>(raw_lds[buf] + L::KS + 256 * j, kv.ks + (j ? base[1] : base[0]) * 8, off);
-            if (wave >= PF_WAVES / 2 - 2 && wave < PF_WAVES / 2)
-                dma_sv<4>(raw_lds[buf] + L::VS + 256 * j, kv.vs + (j ? base[1] : base[0]) * 8, off);
+    // tile i's raw bytes; dead: two bits a tile, tile i's in bits 0, 1
+    BtRaw<KVT> raw;
+    uint32_t dead = 0;
+    int at[2] = {-1, -1};
+    auto find = [&](int i) {
+        if (i < nt) {
+            at[0] = bt_place(p, table, (tb + i) * PF_TILE, end);
+            at[1] = bt_place(p, table, (tb + i) * PF_TILE + 16, end);
         }
     };
-    // a dead half's V is zeros: its probabilities are, and what was read in its place need not be finite
-    auto convert = [&](int raw, int dst, uint32_t dead) {
-        pf_convert<KVT>(s_raw[raw], s_k[dst], s_vt[dst], t);
-        if (dead != 0) {
-            const int cb = t & 3, dc = (t >> 2) & 63, h = t >> 8;
-            if ((dead >> h) & 1)
-#pragma unroll
-                for (int d = 0; d < 4; d++)
-                    *reinterpret_cast<uint2*>(s_vt[dst] + (4 * dc + d) * VT_LD + 8 * cb + 4 * h) = make_uint2(0u, 0u);
-        }
+    auto load = [&](int i) {
+        const int k0 = (tb + i) * PF_TILE, last[2] = {min(15, end - 1 - k0), min(15, end - 17 - k0)};
+        bt_raw_load<KVT>(raw, kv, head, at, last, t, is_v);
     };
+    auto dead_bits = [&]() { return (uint32_t)((at[0] < 0) | (at[1] < 0) << 1); };
+    if (nt > 0) {
+        find(0);
+        dead = dead_bits();
+        if (converts) load(0);
+    }
 
-    int vis[2], vmin = 0x7fffffff;
-    h8 qb[2][8];
+    // this lane's row, its bound and Q / 16 as the B operand
+    const int r = wrow0 + i16, tok = r / GRP;
+    const bool valid = r < nrows;
+    const int vis = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, end) : 0;
+    int vmin = valid ? vis : 0x7fffffff;
+    h8 qb[8];
+    const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + 8 * lg;
 #pragma unroll
-    for (int rt = 0; rt < 2; rt++) {
-        const int r = wrow0 + 16 * rt + i16, tok = r / GRP;
-        const bool valid = r < nrows;
-        vis[rt] = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, end) : 0;
-        if (valid) vmin = min(vmin, vis[rt]);
-        const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + 8 * lg;
+    for (int s = 0; s < 8; s++) {
+        const float4 x0 = *reinterpret_cast<const float4*>(qrow + 32 * s);
+        const float4 x1 = *reinterpret_cast<const float4*>(qrow + 32 * s + 4);
+        const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-        for (int s = 0; s < 8; s++) {
-            const float4 x0 = *reinterpret_cast<const float4*>(qrow + 32 * s);
-            const float4 x1 = *reinterpret_cast<const float4*>(qrow + 32 * s + 4);
-            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                qb[rt][s][j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
-        }
+        for (int j = 0; j < 8; j++) qb[s][j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
     }
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
     vmin = __builtin_amdgcn_readfirstlane(vmin);
 
-    f4 o[2][16];
-    float m[2], l[2];
+    f4 o[16];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int rt = 0; rt < 2; rt++) {
-        m[rt] = -INFINITY;
-        l[rt] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int dt = 0; dt < 16; dt++) o[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
     if (nt > 0) {
-        auto key0 = [&](int i) { return (tb + min(i, nt - 1)) * PF_TILE; };  // (past the last tile: it is re-read)
-        uint32_t dead = 0;  // two bits a tile, tile i's in bits 0, 1
-        int at0, at1;
-        auto find = [&](int i) {
-            at0 = bt_place(p, table, key0(i), end);
-            at1 = bt_place(p, table, key0(i) + 16, end);
-        };
-        wait_vmcnt<0>();  // the Q loads; from here on vmcnt counts only the tile loads
-#pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            find(i);
-            dead |= (uint32_t)((at0 < 0) | (at1 < 0) << 1) << (2 * i);
-            issue(i, key0(i), at0, at1);
+        // tile 0 converted, tile 1's bytes on their way, tile 2's pages known
+        if (converts) bt_raw_store<KVT>(raw, s_k[0], s_vt[0], t, is_v);
+        if (nt > 1) {
+            find(1);
+            dead |= dead_bits() << 2;
+            if (converts) load(1);
+            find(2);
         }
-        find(AHEAD);
-        wait_vm(nvm * (AHEAD - 1));
         __syncthreads();
-        convert(0, 0, dead & 3);
-        if constexpr (AHEAD >= 2) wait_vm(nvm * (AHEAD - 2));
-        __syncthreads();
-
-        const bool lead = wave < PF_WAVES / 2;  // the two waves of a SIMD convert at different times
         const bool rows_here = wrow0 < nrows;
+        // tile i + 1 into the other buffer (free since the last barrier), then tile i + 2's loads
+        auto convert = [&](int i) {
+            if (i + 1 < nt) bt_raw_store<KVT>(raw, s_k[(i + 1) & 1], s_vt[(i + 1) & 1], t, is_v);
+            if (i + 2 < nt) load(i + 2);
+        };
         for (int i = 0; i < nt; i++) {
-            const int k0 = key0(i), cur = i & 1;
-            dead |= (uint32_t)((at0 < 0) | (at1 < 0) << 1) << (2 * AHEAD);
-            issue((i + AHEAD) % NBUF, key0(i + AHEAD), at0, at1);
-            find(i + AHEAD + 1);
-            const _Float16* Ks = s_k[cur];
-            const _Float16* Vt = s_vt[cur];
-            if (AHEAD >= 2 && lead) convert((i + 1) % NBUF, cur ^ 1, (dead >> 2) & 3);
+            const int k0 = (tb + i) * PF_TILE;
+            const _Float16* Ks = s_k[i & 1];
+            const _Float16* Vt = s_vt[i & 1];
+            if (is_v) convert(i);
             if (rows_here) {
                 // S^T = K Q^T: lane (row i16) gets keys k0 + 16 kt + 4 lg + j; the K fragments of a step are read while
                 // the step before multiplies
-                f4 sc[2][2];
+                f4 sc[2] = {};
+                auto kfrag = [&](int s, int kt) { return lds_h8(Ks + 8 * (32 * (4 * s + lg) + 16 * kt + (i16 ^ (2 * s)))); };
+                h8 kf[BT_KD + 1][2];
 #pragma unroll
-                for (int rt = 0; rt < 2; rt++)
+                for (int s = 0; s < BT_KD; s++)
 #pragma unroll
-                    for (int kt = 0; kt < 2; kt++) sc[rt][kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-                const _Float16* krow = Ks + i16 * KS_LD + 8 * lg;
-                h8 kf[2][2] = {{lds_h8(krow), lds_h8(krow + 16 * KS_LD)}, {}};
+                    for (int kt = 0; kt < 2; kt++) kf[s][kt] = kfrag(s, kt);
 #pragma unroll
                 for (int s = 0; s < 8; s++) {
-                    if (s < 7)
+                    if (s + BT_KD < 8)
 #pragma unroll
-                        for (int kt = 0; kt < 2; kt++) kf[(s + 1) & 1][kt] = lds_h8(krow + 16 * kt * KS_LD + 32 * (s + 1));
+                        for (int kt = 0; kt < 2; kt++) kf[(s + BT_KD) % (BT_KD + 1)][kt] = kfrag(s + BT_KD, kt);
                     __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int kt = 0; kt < 2; kt++) sc[kt] = mfma16(kf[s % (BT_KD + 1)][kt], qb[s], sc[kt]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (k0 + PF_TILE > vmin || (dead & 3) != 0) {
 #pragma unroll
                     for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-                        for (int rt = 0; rt < 2; rt++) sc[rt][kt] = mfma16(kf[s & 1][kt], qb[rt][s], sc[rt][kt]);
-                    __builtin_amdgcn_sched_barrier(0);
+                        for (int j = 0; j < 4; j++)
+                            sc[kt][j] = k0 + 16 * kt + 4 * lg + j < vis && !((dead >> kt) & 1) ? sc[kt][j] : -INFINITY;
                 }
-
-                const bool masked = k0 + PF_TILE > vmin || (dead & 3) != 0;
-                float cr[2];
-                h8 pb[2];
+                float mx = max3f(max3f(-INFINITY, sc[0][0], sc[0][1]), sc[0][2], sc[0][3]);
+                mx = rows_max(max3f(max3f(mx, sc[1][0], sc[1][1]), sc[1][2], sc[1][3]));
+                const float mn = mx > m + PF_RESCALE_T ? mx : m;
+                const float cr = mn == m ? 1.0f : fast_exp2((m - mn) * PF_LOG2E);
+                const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;
+                m = mn;
+                // the V fragments' reads begin while the exponentials are taken
+                const _Float16* vrow = Vt + 8 * (256 * lg + i16);
+                h8 vf[BT_VD];
 #pragma unroll
-                for (int rt = 0; rt < 2; rt++) {
-                    if (masked) {
+                for (int dt = 0; dt < BT_VD - 1; dt++) vf[dt] = lds_h8(vrow + 8 * 16 * dt);
+                h8 pb;
 #pragma unroll
-                        for (int kt = 0; kt < 2; kt++)
+                for (int j = 0; j < 8; j++) pb[j] = (_Float16)fast_exp2(fmaf(sc[j >> 2][j & 3], PF_LOG2E, -msl));
+                // the sum of the rounded probabilities, the weights that P V applies
+                const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
+                float rs = 0.0f;
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const bool seen = k0 + 16 * kt + 4 * lg + j < vis[rt] && !((dead >> kt) & 1);
-                                sc[rt][kt][j] = seen ? sc[rt][kt][j] : -INFINITY;
-                            }
-                    }
-                    float mx = max3f(max3f(-INFINITY, sc[rt][0][0], sc[rt][0][1]), sc[rt][0][2], sc[rt][0][3]);
-                    mx = rows_max(max3f(max3f(mx, sc[rt][1][0], sc[rt][1][1]), sc[rt][1][2], sc[rt][1][3]));
-                    const float mn = mx > m[rt] + PF_RESCALE_T ? mx : m[rt];
-                    cr[rt] = mn == m[rt] ? 1.0f : fast_exp2((m[rt] - mn) * PF_LOG2E);
-                    m[rt] = mn;
-                    const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;
+                for (int j = 0; j < 8; j += 2) rs = __builtin_amdgcn_fdot2(h2{pb[j], pb[j + 1]}, one2, rs, false);
+                l = l * cr + rs;
+                if (__any(cr != 1.0f)) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        pb[rt][j] = (_Float16)fast_exp2(fmaf(sc[rt][j >> 2][j & 3], PF_LOG2E, -msl));
-                    // the sum of the rounded probabilities, the weights that P V applies
-                    const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
-                    float rs = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) rs = __builtin_amdgcn_fdot2(h2{pb[rt][j], pb[rt][j + 1]}, one2, rs, false);
-                    l[rt] = l[rt] * cr[rt] + rs;
+                    for (int dt = 0; dt < 16; dt++) o[dt] *= cr;
                 }
-                if (__any(cr[0] != 1.0f || cr[1] != 1.0f)) {
-#pragma unroll
-                    for (int rt = 0; rt < 2; rt++)
-#pragma unroll
-                        for (int dt = 0; dt < 16; dt++) o[rt][dt] *= cr[rt];
-                }
-
-                // O^T += V^T P^T, three V fragments in flight
-                const _Float16* vrow = Vt + i16 * VT_LD + 8 * lg;
-                h8 vf[3];
-#pragma unroll
-                for (int dt = 0; dt < 2; dt++) vf[dt] = lds_h8(vrow + 16 * VT_LD * dt);
+                // O^T += V^T P^T
 #pragma unroll
                 for (int dt = 0; dt < 16; dt++) {
-                    if (dt + 2 < 16) vf[(dt + 2) % 3] = lds_h8(vrow + 16 * VT_LD * (dt + 2));
-#pragma unroll
-                    for (int rt = 0; rt < 2; rt++) o[rt][dt] = mfma16(vf[dt % 3], pb[rt], o[rt][dt]);
+                    if (dt + BT_VD - 1 < 16) vf[(dt + BT_VD - 1) % BT_VD] = lds_h8(vrow + 8 * 16 * (dt + BT_VD - 1));
+                    o[dt] = mfma16(vf[dt % BT_VD], pb, o[dt]);
                 }
             }
-            if (AHEAD >= 2 && !lead) convert((i + 1) % NBUF, cur ^ 1, (dead >> 2) & 3);
-            if constexpr (AHEAD >= 2) {
-                wait_vm(nvm * (AHEAD - 2));  // tile i + 2 must have landed before the next iteration converts it
-                __syncthreads();
-            } else {
-                wait_vm(0);
-                __syncthreads();
-                if (i + 1 < nt) convert((i + 1) % NBUF, cur ^ 1, (dead >> 2) & 3);
-                __syncthreads();
-            }
+            if (converts && !is_v) convert(i);
             dead >>= 2;
+            if (i + 2 < nt) dead |= dead_bits() << 2;
+            find(i + 3);
+            __syncthreads();
         }
-        wait_vmcnt<0>();  // no direct-to-LDS load outlives the workgroup
     }
 
-    // partial states: lane holds dims 16 dt + 4 lg + j of row (rt, i16)
+    // partial state: o[2 k + e][j] is dim 8 x + k of row i16, x = 16 e + 4 lg + j; through LDS, so that a store instruction
+    // writes two whole 512-byte rows
+    uint2* const xch = lds.xch[wave];
+    __syncthreads();
+    const float lt = rows_sum(l);
+    const float il = lt == 0.0f ? 0.0f : 1.0f / lt;  // (a row that saw nothing: l = 0 and O = 0)
+    float amax = 0.0f;
 #pragma unroll
-    for (int rt = 0; rt < 2; rt++) {
-        const int r = wrow0 + 16 * rt + i16;
-        const float lt = rows_sum(l[rt]);
-        const float il = lt == 0.0f ? 0.0f : 1.0f / lt;  // (a row that saw nothing: l = 0 and O = 0)
-        float amax = 0.0f;
+    for (int dt = 0; dt < 16; dt++)
 #pragma unroll
-        for (int dt = 0; dt < 16; dt++)
+        for (int j = 0; j < 4; j++) amax = fmaxf(amax, fabsf(o[dt][j]));
+    amax = rows_max(amax) * il;
+    const float qs = amax > 1e-30f ? 32767.0f / amax : 0.0f, f = il * qs;
+    const size_t range = (size_t)sp * a.n * a.nq * NH + g * GRP;
+    // (a row whose O is not finite has no fixed-point form: its scale makes every value NaN)
+    const float scale = amax < INFINITY ? (qs > 0.0f ? amax * (1.0f / 32767.0f) : 0.0f) : NAN;
+    if (valid && lg == 0) a.tile_ml[range + (size_t)tok * NH + r % GRP] = make_float4(m, lt, scale, 0.0f);
 #pragma unroll
-            for (int j = 0; j < 4; j++) amax = fmaxf(amax, fabsf(o[rt][dt][j]));
-        amax = rows_max(amax) * il;
-        const float qs = amax > 1e-30f ? 32767.0f / amax : 0.0f, f = il * qs;
-        if (r < nrows) {
-            const size_t rec = (size_t)sp * a.n * a.nq * NH + (size_t)(r / GRP) * NH + g * GRP + r % GRP;
-            // (a row whose O is not finite has no fixed-point form: its scale makes every value NaN)
-            const float scale = amax < INFINITY ? (qs > 0.0f ? amax * (1.0f / 32767.0f) : 0.0f) : NAN;
-            if (lg == 0) a.tile_ml[rec] = make_float4(m[rt], lt, scale, 0.0f);
-            PfPartO* dst = a.tile_o + rec * (HD / 4) + lg;
+    for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int dt = 0; dt < 16; dt++)
-                dst[4 * dt] = pack16x4(o[rt][dt][0] * f, o[rt][dt][1] * f, o[rt][dt][2] * f, o[rt][dt][3] * f);
+        for (int q = 0; q < 4; q++) {
+            const int e = q & 1, k = 4 * (q >> 1);  // dims 8 x + k .. + 3: 8-byte unit 2 x + k / 4
+            xch[64 * i16 + ((2 * (16 * e + 4 * lg + j) + k / 4) ^ (4 * i16))] =
+                pack16x4(o[2 * k + e][j] * f, o[2 * k + 2 + e][j] * f, o[2 * k + 4 + e][j] * f, o[2 * k + 6 + e][j] * f);
         }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const int xr = 2 * k + (lane >> 5), ro = wrow0 + xr;
+        const uint4 w = *reinterpret_cast<const uint4*>(&xch[64 * xr + ((2 * (lane & 31)) ^ (4 * xr))]);
+        if (ro < nrows)
+            *reinterpret_cast<uint4*>(a.tile_o + (range + (size_t)(ro / GRP) * NH + ro % GRP) * (HD / 4) + 2 * (lane & 31)) = w;
     }
 }
 
@@ -879,7 +940,7 @@ static void launch_ranges(const BatchArgs& a, const qwa_kv_layer& kv, const qwa_
     const dim3 block(64 * BT_WAVES);
 #define QWA_BT(K, RT, GRID, ...) hipLaunchKernelGGL((K<KVT, RT>), dim3(GRID), block, 0, st, a, kv, p, __VA_ARGS__)
     if (b.nt > 0)
-        hipLaunchKernelGGL(k_bt_tiles<KVT>, dim3(b.blocks * b.nt * NKV), dim3(PF_THREADS), 0, st, a, kv, p, b.blocks, b.nt);
+        hipLaunchKernelGGL(k_bt_tiles<KVT>, dim3(b.blocks * b.nt * NKV), dim3(64 * BT_TWAVES), 0, st, a, kv, p, b.blocks, b.nt);
     if (b.ns_shared > 0) {
         const int grid = (b.ns_shared * NKV + 7) / 8 * 8 * b.groups_shared;
         if (b.rt_shared == 1) QWA_BT(k_bt_shared, 1, grid, b.ns_shared, b.len_shared, b.groups_shared);

@@ -17,12 +17,14 @@ constexpr int BT_MAXRT = 2;   // 16-row MFMA tiles of such a workgroup at most
 #ifndef QWA_FILL
 #define QWA_FILL 768
 #endif
+constexpr int BT_TWAVES = 12;                // waves of a tile workgroup
+constexpr int BT_TROWS = 16 * BT_TWAVES;  // its rows
 constexpr int BT_STEP = 128;  // positions of a step; key ranges are whole steps
 constexpr int BT_FEW = 32;    // rows of a KV head up to which the shared positions are left to register workgroups
 
 // The shared positions [0, n_shared) are worked on for all rows together, the positions of its own [n_shared, len) for every
 // sequence by itself.
-//  tile workgroups (k_bt_tiles): PF_ROWS rows, the shared PF_TILE-key tiles in nt ranges of about equal length;
+//  tile workgroups (k_bt_tiles): BT_TROWS rows, the shared PF_TILE-key tiles in nt ranges of about equal length;
 //  register workgroups over the shared positions (k_bt_shared): up to BT_MAXRT row tiles, key ranges of fixed length;
 //  register workgroups over the own positions (k_bt_own): the steps of BT_STEP positions of all sequences in a row, cut
 //  into wgs slices of equal length (the kernel knows the sequences' lengths, the plan only their bound), each worked on as
@@ -56,7 +58,7 @@ inline BatchPlan batch_plan(int n, int nq, int n_shared, int max_len) {
     p.groups = (own + 16 * p.rt_own - 1) / (16 * p.rt_own);
     if (rows > BT_FEW && n_shared > 0) {
         const int tiles = (n_shared + PF_TILE - 1) / PF_TILE;
-        p.blocks = (rows + PF_ROWS - 1) / PF_ROWS;
+        p.blocks = (rows + BT_TROWS - 1) / BT_TROWS;
         p.nt = std::min(tiles, std::max(1, 256 / (p.blocks * NKV)));
         p.len_shared = BT_STEP;
     } else {

@@ -172,7 +172,7 @@ int main() {
             const size_t rows = (size_t)n * nq * NH;
             CHECK(p.groups * p.rt_own * 16 >= nq * GRP && p.rt_own <= BT_MAXRT, "rows of a sequence\n");
             CHECK(shared == 0 || (p.nt > 0) != (p.ns_shared > 0), "the shared positions: one kind of workgroup\n");
-            CHECK(p.nt == 0 || p.blocks * PF_ROWS >= n * nq * GRP, "rows of the batch\n");
+            CHECK(p.nt == 0 || p.blocks * BT_TROWS >= n * nq * GRP, "rows of the batch\n");
             CHECK(p.nt * (long long)PF_TILE < shared + PF_TILE, "an empty range\n");
             CHECK(p.groups_shared * p.rt_shared * 16 >= n * nq * GRP, "rows of the batch\n");
             CHECK(p.nt > 0 || (long long)p.ns_shared * p.len_shared >= shared, "shared\n");
