@@ -829,6 +829,7 @@ __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p,
     const int nrows = a.n * a.nq * NH;
     if (row >= nrows) return;  // (all waves of a row, and with WPR = 4 of a workgroup)
     const int tok = row / NH, b = tok / a.nq, h = row % NH;
+    const float4 gv = *reinterpret_cast<const float4*>(gate + (size_t)row * HD + 4 * lane);
     // the batch row's segments: those of the slices from its first step's to its last one's
     int segs = 0;
     size_t seg0 = 0;
@@ -841,52 +842,66 @@ __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p,
             seg0 = ((size_t)(h / GRP) * (a.wgs + a.n) + w0 + b) * a.nq * GRP + (tok % a.nq) * GRP + h % GRP;
         }
     }
-    const int fixed = nt + ns_shared, all = fixed + segs;
-    // (m, l, scale) of state s: the tile workgroups' states, the shared ranges', the own segments'
-    auto state = [&](int s) {
-        if (s < nt) return a.tile_ml[(size_t)s * nrows + row];
-        if (s >= all) return make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-        const float2 ml = s < fixed ? a.part_ml[(size_t)(s - nt) * nrows + row]
-                                    : a.own_ml[seg0 + (size_t)(s - fixed) * a.nq * GRP];
-        return make_float4(ml.x, ml.y, 1.0f, 0.0f);
-    };
-    float M = -INFINITY;
-    for (int s0 = 0; s0 < all; s0 += 64) M = fmaxf(M, state(s0 + lane).x);
-    M = wave_max(M);
-    float L = 0.0f;
+    float M = -INFINITY, L = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // adds `count` states: ml(s) their (m, l, factor of the stored values), x(s) the lane's four values
     constexpr int U = 8;
-    for (int s0 = 0; s0 < all; s0 += 64) {
-        const PfPartMl ml = state(s0 + lane);
-        // a state that saw nothing weighs nothing; one of NaN scores (l is NaN) makes the row NaN
-        const float f = ml.y == 0.0f ? 0.0f : fast_exp2((ml.x - M) * PF_LOG2E);
-        L += wave_sum(f * ml.y);
-        // tile states hold O / l in steps of the scale, register states O
-        const float wt = f * ml.z * (s0 + lane < nt ? ml.y : 1.0f);
-        const int most = min(64, all - s0);
-        for (int k = part; k < most; k += U * WPR) {
+    auto add = [&](int count, auto ml_of, auto x_of) {
+        for (int s0 = 0; s0 < count; s0 += 64) {
+            const int most = min(64, count - s0);
             float4 x[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int s = s0 + min(k + u * WPR, most - 1);
-                if (s < nt) x[u] = unpack16x4(a.tile_o[((size_t)s * nrows + row) * (HD / 4) + lane]);
-                else
-                    x[u] = *reinterpret_cast<const float4*>(
-                        (s < fixed ? a.part_o + ((size_t)(s - nt) * nrows + row) * HD
-                                   : a.own_o + (seg0 + (size_t)(s - fixed) * a.nq * GRP) * HD) + 4 * lane);
-            }
+            for (int u = 0; u < U; u++) x[u] = x_of(s0 + min(part + u * WPR, most - 1));
+            const float4 ml = lane < most ? ml_of(s0 + lane) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+            const float Mn = fmaxf(M, wave_max(ml.x));
+            const float c = M == Mn ? 1.0f : fast_exp2((M - Mn) * PF_LOG2E);
+            // a state that saw nothing weighs nothing; one of NaN scores (l is NaN) makes the row NaN
+            const float f = ml.y == 0.0f ? 0.0f : fast_exp2((ml.x - Mn) * PF_LOG2E);
+            M = Mn;
+            L = fmaf(L, c, wave_sum(f * ml.y));
+            acc.x *= c;
+            acc.y *= c;
+            acc.z *= c;
+            acc.w *= c;
+            const float wt = f * ml.z;
+            for (int k = part; k < most; k += U * WPR) {
+                float4 nx[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const float fu = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wt), min(k + u * WPR, 63)));
-                if (k + u * WPR < most) {
-                    acc.x = fmaf(fu, x[u].x, acc.x);
-                    acc.y = fmaf(fu, x[u].y, acc.y);
-                    acc.z = fmaf(fu, x[u].z, acc.z);
-                    acc.w = fmaf(fu, x[u].w, acc.w);
+                for (int u = 0; u < U; u++)
+                    if (k + U * WPR < most) nx[u] = x_of(s0 + min(k + (U + u) * WPR, most - 1));
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const float fu = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wt), min(k + u * WPR, 63)));
+                    if (k + u * WPR < most) {
+                        acc.x = fmaf(fu, x[u].x, acc.x);
+                        acc.y = fmaf(fu, x[u].y, acc.y);
+                        acc.z = fmaf(fu, x[u].z, acc.z);
+                        acc.w = fmaf(fu, x[u].w, acc.w);
+                    }
+                    x[u] = nx[u];
                 }
             }
         }
-    }
+    };
+    // tile states hold O / l in steps of their scale, register states O
+    add(nt,
+        [&](int s) {
+            const float4 v = a.tile_ml[(size_t)s * nrows + row];
+            return make_float4(v.x, v.y, v.z * v.y, 0.0f);
+        },
+        [&](int s) { return unpack16x4(a.tile_o[((size_t)s * nrows + row) * (HD / 4) + lane]); });
+    add(ns_shared,
+        [&](int s) {
+            const float2 v = a.part_ml[(size_t)s * nrows + row];
+            return make_float4(v.x, v.y, 1.0f, 0.0f);
+        },
+        [&](int s) { return *reinterpret_cast<const float4*>(a.part_o + ((size_t)s * nrows + row) * HD + 4 * lane); });
+    add(segs,
+        [&](int s) {
+            const float2 v = a.own_ml[seg0 + (size_t)s * a.nq * GRP];
+            return make_float4(v.x, v.y, 1.0f, 0.0f);
+        },
+        [&](int s) { return *reinterpret_cast<const float4*>(a.own_o + (seg0 + (size_t)s * a.nq * GRP) * HD + 4 * lane); });
     if constexpr (WPR > 1) {
         s_o[wave][lane] = acc;
         __syncthreads();
@@ -900,7 +915,6 @@ __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p,
             acc.w += x.w;
         }
     }
-    const float4 gv = *reinterpret_cast<const float4*>(gate + (size_t)row * HD + 4 * lane);
     float v[4] = {acc.x / L * sigmoid(gv.x), acc.y / L * sigmoid(gv.y), acc.z / L * sigmoid(gv.z), acc.w / L * sigmoid(gv.w)};
     if (L == 0.0f) v[0] = v[1] = v[2] = v[3] = 0.0f;  // no key was seen
     *reinterpret_cast<uint2*>(out16 + (size_t)row * HD + 4 * lane) =

@@ -45,7 +45,8 @@ __device__ __forceinline__ int held(const qwa_kv_pages& p, int s) {
     return m <= 0 ? 0 : min(p.ld, pages_of(m, p.page));
 }
 
-// exclusive sum over the workgroup's PG_T threads, and the total
+// exclusive sum over the workgroup's T threads, and the total
+template <int T>
 __device__ __forceinline__ long long block_scan(long long v, long long* s_wave, long long* total) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     long long x = v;
@@ -59,7 +60,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* s_wave, 
     __syncthreads();
     long long before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < PG_T / 64; w++) {
+    for (int w = 0; w < T / 64; w++) {
         const long long y = s_wave[w];
         if (w < wave) before += y;
         all += y;
@@ -70,13 +71,15 @@ __device__ __forceinline__ long long block_scan(long long v, long long* s_wave, 
 
 constexpr int PG_PT = 4;  // counts per thread and round of the searches through ref
 
-// Room: thread i plans request i.  Requests are served in order (an exclusive sum of the pages that they need), and of the
+// Room, by a workgroup of T >= n threads: thread i plans request i.  Requests are served in order (an exclusive sum of the pages that they need), and of the
 // requests whose last, partly filled page is the same, the first ref - 1 move away to copies and the last may keep it.
-__global__ void __launch_bounds__(PG_T) k_extend(qwa_kv_pages p, const int* __restrict__ seqs,
+template <int T>
+__global__ void __launch_bounds__(T) k_extend(qwa_kv_pages p, const int* __restrict__ seqs,
                                                  const int* __restrict__ add, int n, int* __restrict__ status,
                                                  int* __restrict__ work) {
-    __shared__ long long s_wave[PG_T / 64];
-    __shared__ int s_seq[PG_T], s_tail[PG_T], s_base[PG_T + 1];
+    __shared__ long long s_wave[T / 64];
+    __shared__ int2 s_req[T];  // (sequence, last page)
+    __shared__ int s_base[T], s_have[T];
     __shared__ int s_bad;
     const int t = threadIdx.x;
     PageMove* moves = reinterpret_cast<PageMove*>(work + PG_HDR);
@@ -99,21 +102,28 @@ __global__ void __launch_bounds__(PG_T) k_extend(qwa_kv_pages p, const int* __re
             else tail = -1;
         }
     }
-    s_seq[t] = s;
-    s_tail[t] = tail;
+    s_req[t] = make_int2(s, tail);
     __syncthreads();
-    int rank = 0;
-    for (int j = 0; j < n && j < t; j++) {
-        ok = ok && !(t < n && s_seq[j] == s);
-        rank += tail >= 0 && s_tail[j] == tail;
+    int rank = 0, same = 0;
+#pragma unroll 8
+    for (int j = 0; j < min(n, t); j++) {
+        const int2 q = s_req[j];
+        same += q.x == s;
+        rank += q.y == tail;
     }
+    ok = ok && same == 0;
     if (t < n && !ok) atomicMin(&s_bad, t);
     const bool cow = tail >= 0 && rank < r - 1;
     const int have = ok ? pages_of(m, p.page) : 0;
     const int need = t < n && ok ? pages_of((long long)m + a, p.page) - have + cow : 0;
-    long long total, copies;
-    const long long base = block_scan(need, s_wave, &total);
-    const long long cbase = block_scan(cow && ok, s_wave, &copies);
+    // pages and copies in one sum (at most PG_T copies)
+    constexpr int CB = 12;
+    static_assert(PG_T < 1 << CB, "the copies' field");
+    long long total;
+    long long base = block_scan<T>(((long long)need << CB) + (cow && ok), s_wave, &total);
+    const int cbase = (int)(base & ((1 << CB) - 1)), copies = (int)(total & ((1 << CB) - 1));
+    base >>= CB;
+    total >>= CB;
     if (t == 0) work[0] = 0;
     if (s_bad < PG_T) {  // (every thread passed block_scan's barriers after the atomicMin)
         if (t == 0) *status = -(s_bad + 1);
@@ -121,7 +131,7 @@ __global__ void __launch_bounds__(PG_T) k_extend(qwa_kv_pages p, const int* __re
     }
     // the lowest free pages
     long long found = 0;
-    for (long long i0 = 0; i0 < p.n_pages && found < total; i0 += PG_T * PG_PT) {
+    for (long long i0 = 0; i0 < p.n_pages && found < total; i0 += T * PG_PT) {
         const int i = (int)i0 + PG_PT * t;
         int f[PG_PT], c = 0;
 #pragma unroll
@@ -129,7 +139,7 @@ __global__ void __launch_bounds__(PG_T) k_extend(qwa_kv_pages p, const int* __re
 #pragma unroll
         for (int k = 0; k < PG_PT; k++) c += f[k] <= 0;
         long long got;
-        long long at = found + block_scan(c, s_wave, &got);
+        long long at = found + block_scan<T>(c, s_wave, &got);
 #pragma unroll
         for (int k = 0; k < PG_PT; k++)
             if (f[k] <= 0) {
@@ -144,12 +154,10 @@ __global__ void __launch_bounds__(PG_T) k_extend(qwa_kv_pages p, const int* __re
     }
     // (total <= n_pages from here on)
     s_base[t] = (int)base;
-    if (t == 0) s_base[PG_T] = (int)total;
     // request t's plan, for the threads that carry it out
-    __shared__ int s_have[PG_T];
     s_have[t] = cow ? -have : have;  // (a copied page: have >= 1)
     __syncthreads();
-    for (int k = t; k < (int)total; k += PG_T) {
+    for (int k = t; k < (int)total; k += T) {
         // the last request whose base is at most k needs page k
         int lo = 0, hi = n;
         while (hi - lo > 1) {
@@ -159,7 +167,7 @@ __global__ void __launch_bounds__(PG_T) k_extend(qwa_kv_pages p, const int* __re
         }
         const int h = s_have[lo], first = h < 0 ? -h - 1 : h;  // first entry that gets a page
         const int pg = free_list[k];
-        p.table[(size_t)s_seq[lo] * p.ld + first + (k - s_base[lo])] = pg;
+        p.table[(size_t)s_req[lo].x * p.ld + first + (k - s_base[lo])] = pg;
         p.ref[pg] = 1;
     }
     if (t < n) {
@@ -170,7 +178,7 @@ __global__ void __launch_bounds__(PG_T) k_extend(qwa_kv_pages p, const int* __re
         p.len[s] = m + a;
     }
     if (t == 0) {
-        work[0] = (int)copies;
+        work[0] = copies;
         *status = 0;
     }
 }
@@ -184,7 +192,7 @@ __global__ void __launch_bounds__(PG_T) k_compact(qwa_kv_pages p, int* __restric
     int c = 0;
     for (long long i = t; i < p.n_pages; i += PG_T) c += p.ref[i] > 0;
     long long live;
-    block_scan(c, s_wave, &live);
+    block_scan<PG_T>(c, s_wave, &live);
     long long holes = 0, movers = 0;
     for (long long i0 = 0; i0 < p.n_pages; i0 += PG_T * PG_PT) {
         const int i = (int)i0 + PG_PT * t;
@@ -195,7 +203,7 @@ __global__ void __launch_bounds__(PG_T) k_compact(qwa_kv_pages p, int* __restric
 #pragma unroll
         for (int k = 0; k < PG_PT; k++) h += f[k] < 0 ? 0 : i + k < live ? !f[k] : (long long)f[k] << 32;
         long long got;
-        const long long at = block_scan(h, s_wave, &got);
+        const long long at = block_scan<PG_T>(h, s_wave, &got);
         long long hole = holes + (at & 0xffffffffLL), mover = movers + (at >> 32);
 #pragma unroll
         for (int k = 0; k < PG_PT; k++) {
@@ -275,69 +283,167 @@ __global__ void __launch_bounds__(256) k_move(qwa_kv_pages p, const int* __restr
     }
 }
 
-// whether an earlier or later request names sequence s too: request i gives way to the last of them
-__device__ __forceinline__ bool named_later(const int* __restrict__ seqs, int n, int i, int s) {
-    bool later = false;
-    for (int j = i + 1 + (int)threadIdx.x; j < n; j += blockDim.x) later |= seqs[j] == s;
-    return __syncthreads_or(later);
-}
+// Forks and trims: a workgroup has PG_CH requests, a thread an entry of their rows.  Neighbouring requests often hold the
+// same page there (forks of one prompt), so a thread adds up the changes of equal pages in a row and sends one atomic for
+// them.  (One request per workgroup, one atomic per request and page: 100 forks of 313 pages 11 instead of 5 us a kernel.)
+constexpr int PG_CH = 16;
+constexpr int PG_RT = 512;  // threads
 
-// Fork, first half: request i's new row is staged, and its pages counted once more, before any row changes.
-__global__ void __launch_bounds__(256) k_fork_stage(qwa_kv_pages p, const int* __restrict__ src,
-                                                    const int* __restrict__ dst, int n, int* __restrict__ work) {
-    const int i = blockIdx.x, t = threadIdx.x, s = src[i], d = dst[i];
-    const bool later = named_later(dst, n, i, d);
-    if (later || d < 0 || d >= p.n_seq || s >= p.n_seq) {
-        if (t == 0) work[2 * i] = -1;
-        return;
-    }
-    const int k = s < 0 ? 0 : held(p, s);
-    int* row = work + 2 * (size_t)n + (size_t)i * p.ld;
-    for (int e = t; e < k; e += 256) {
-        const int pg = p.table[(size_t)s * p.ld + e];
-        row[e] = pg;
-        if (page_ok(pg, p)) atomicAdd(p.ref + pg, 1);
-    }
-    if (t == 0) {
-        work[2 * i] = k;
-        work[2 * i + 1] = s < 0 ? 0 : p.len[s];
-    }
-}
-
-// Second half: the old pages are given back and the staged row put in their place.
-__global__ void __launch_bounds__(256) k_fork_commit(qwa_kv_pages p, const int* __restrict__ dst, int n,
-                                                     const int* __restrict__ work) {
-    const int i = blockIdx.x, t = threadIdx.x, k = work[2 * i];
-    if (k < 0) return;
-    const int d = dst[i], old = held(p, d);
-    const int* row = work + 2 * (size_t)n + (size_t)i * p.ld;
-    __syncthreads();  // before the length changes
-    for (int e = t; e < max(k, old); e += 256) {
-        int* at = p.table + (size_t)d * p.ld + e;
-        if (e < old) {
-            const int pg = *at;
-            if (page_ok(pg, p)) atomicSub(p.ref + pg, 1);
+struct PageSum {
+    int page = -1, count = 0;
+    __device__ __forceinline__ void add(const qwa_kv_pages& p, int pg, int by) {
+        if (pg != page) {
+            flush(p);
+            page = pg;
         }
-        *at = e < k ? row[e] : -1;
+        count += by;
     }
-    if (t == 0) p.len[d] = work[2 * i + 1];
+    __device__ __forceinline__ void flush(const qwa_kv_pages& p) {
+        if (count != 0 && page_ok(page, p)) atomicAdd(p.ref + page, count);
+        count = 0;
+    }
+};
+
+// which of the workgroup's requests [i0, i0 + PG_CH) are repeated by a later one (bit k: request i0 + k gives way)
+__device__ __forceinline__ uint32_t repeated(const int* __restrict__ seqs, int n, int i0, uint32_t* s_mask) {
+    if (threadIdx.x == 0) *s_mask = 0;
+    __syncthreads();
+    constexpr int L = PG_RT / PG_CH;  // threads per request
+    const int k = threadIdx.x / L, i = i0 + k;
+    bool later = false;
+    if (i < n) {
+        const int s = seqs[i];
+        for (int j = i + 1 + (int)(threadIdx.x % L); j < n; j += L) later |= seqs[j] == s;
+    }
+    if (later) atomicOr(s_mask, 1u << k);
+    __syncthreads();
+    return *s_mask;
 }
 
-__global__ void __launch_bounds__(256) k_trim(qwa_kv_pages p, const int* __restrict__ seqs, const int* __restrict__ lens,
-                                              int n) {
-    const int i = blockIdx.x, t = threadIdx.x, s = seqs[i];
-    if (named_later(seqs, n, i, s) || s < 0 || s >= p.n_seq) return;
-    const int m = p.len[s], keep = lens ? lens[i] : 0;
-    if (keep < 0 || keep > m) return;
-    const int old = held(p, s);
-    __syncthreads();
-    for (int e = pages_of(keep, p.page) + t; e < old; e += 256) {
-        int* at = p.table + (size_t)s * p.ld + e;
-        const int pg = *at;
-        if (page_ok(pg, p)) atomicSub(p.ref + pg, 1);
-        *at = -1;
+// Fork, first half: the requests' new rows are staged, and their pages counted once more, before any row changes.
+// work: page counts [n] (-1: ignored), lengths [n], rows [n][ld].
+__global__ void __launch_bounds__(PG_RT) k_fork_stage(qwa_kv_pages p, const int* __restrict__ src,
+                                                      const int* __restrict__ dst, int n, int* __restrict__ work) {
+    __shared__ uint32_t s_mask;
+    __shared__ int s_src[PG_CH], s_k[PG_CH];
+    const int i0 = blockIdx.x * PG_CH, t = threadIdx.x;
+    const uint32_t gone = repeated(dst, n, i0, &s_mask);
+    if (t < PG_CH) {
+        const int i = i0 + t;
+        int s = -1, k = -1, m = 0;
+        if (i < n) {
+            s = src[i];
+            const int d = dst[i];
+            if (!((gone >> t) & 1) && d >= 0 && d < p.n_seq && s < p.n_seq) {
+                k = s < 0 ? 0 : held(p, s);
+                m = s < 0 ? 0 : p.len[s];
+            }
+            work[i] = k;
+            work[n + i] = m;
+        }
+        s_src[t] = s;
+        s_k[t] = k;
     }
-    if (t == 0) p.len[s] = keep;
+    __syncthreads();
+    int most = 0;
+#pragma unroll
+    for (int k = 0; k < PG_CH; k++) most = max(most, s_k[k]);
+    for (int e = t; e < most; e += PG_RT) {
+        PageSum sum;
+        int pg[PG_CH];
+#pragma unroll
+        for (int k = 0; k < PG_CH; k++) pg[k] = e < s_k[k] ? p.table[(size_t)s_src[k] * p.ld + e] : -1;
+#pragma unroll
+        for (int k = 0; k < PG_CH; k++)
+            if (e < s_k[k]) {
+                work[2 * (size_t)n + (size_t)(i0 + k) * p.ld + e] = pg[k];
+                sum.add(p, pg[k], 1);
+            }
+        sum.flush(p);
+    }
+}
+
+// Second half: the old pages are given back and the staged rows put in their place.
+__global__ void __launch_bounds__(PG_RT) k_fork_commit(qwa_kv_pages p, const int* __restrict__ dst, int n,
+                                                       const int* __restrict__ work) {
+    __shared__ int s_dst[PG_CH], s_k[PG_CH], s_old[PG_CH];
+    const int i0 = blockIdx.x * PG_CH, t = threadIdx.x;
+    if (t < PG_CH) {
+        const int i = i0 + t, k = i < n ? work[i] : -1, d = k < 0 ? 0 : dst[i];
+        s_dst[t] = d;
+        s_k[t] = k;
+        s_old[t] = k < 0 ? -1 : held(p, d);
+        if (k >= 0) p.len[d] = work[n + i];  // (no other workgroup has this sequence)
+    }
+    __syncthreads();
+    int most = 0;
+#pragma unroll
+    for (int k = 0; k < PG_CH; k++) most = max(most, max(s_k[k], s_old[k]));
+    for (int e = t; e < most; e += PG_RT) {
+        PageSum sum;
+        int pg[PG_CH], to[PG_CH];
+#pragma unroll
+        for (int k = 0; k < PG_CH; k++) {
+            pg[k] = e < s_old[k] ? p.table[(size_t)s_dst[k] * p.ld + e] : -1;
+            to[k] = e < s_k[k] ? work[2 * (size_t)n + (size_t)(i0 + k) * p.ld + e] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < PG_CH; k++) {
+            if (e < s_old[k]) sum.add(p, pg[k], -1);
+            if (e < max(s_k[k], s_old[k])) p.table[(size_t)s_dst[k] * p.ld + e] = to[k];
+        }
+        sum.flush(p);
+    }
+}
+
+__global__ void __launch_bounds__(PG_RT) k_trim(qwa_kv_pages p, const int* __restrict__ seqs, const int* __restrict__ lens,
+                                                int n) {
+    __shared__ uint32_t s_mask;
+    __shared__ int s_seq[PG_CH], s_keep[PG_CH], s_old[PG_CH];
+    const int i0 = blockIdx.x * PG_CH, t = threadIdx.x;
+    const uint32_t gone = repeated(seqs, n, i0, &s_mask);
+    if (t < PG_CH) {
+        const int i = i0 + t;
+        int s = 0, keep = 0, old = 0;
+        if (i < n && !((gone >> t) & 1)) {
+            s = seqs[i];
+            if (s >= 0 && s < p.n_seq) {
+                const int to = lens ? lens[i] : 0;
+                if (to >= 0 && to <= p.len[s]) {
+                    keep = pages_of(to, p.page);
+                    old = held(p, s);
+                    p.len[s] = to;  // (no other workgroup has this sequence)
+                }
+            } else {
+                s = 0;
+            }
+        }
+        s_seq[t] = s;
+        s_keep[t] = keep;
+        s_old[t] = old;
+    }
+    __syncthreads();
+    int most = 0;
+#pragma unroll
+    for (int k = 0; k < PG_CH; k++) most = max(most, s_old[k]);
+    int least = most;  // (nothing to give back: no entries)
+#pragma unroll
+    for (int k = 0; k < PG_CH; k++)
+        if (s_keep[k] < s_old[k]) least = min(least, s_keep[k]);
+    for (int e = least + t; e < most; e += PG_RT) {
+        PageSum sum;
+        int pg[PG_CH];
+#pragma unroll
+        for (int k = 0; k < PG_CH; k++)
+            pg[k] = e >= s_keep[k] && e < s_old[k] ? p.table[(size_t)s_seq[k] * p.ld + e] : -1;
+#pragma unroll
+        for (int k = 0; k < PG_CH; k++)
+            if (e >= s_keep[k] && e < s_old[k]) {
+                sum.add(p, pg[k], -1);
+                p.table[(size_t)s_seq[k] * p.ld + e] = -1;
+            }
+        sum.flush(p);
+    }
 }
 
 static PageLayers page_layers(const qwa_kv_layer* layers, int n_layers) {
@@ -351,7 +457,9 @@ constexpr long long PG_MOVE_WG = 4096;  // workgroups of k_move at most
 hipError_t launch_pages_extend(const qwa_kv_pages& p, const int* seqs, const int* add, int n, const qwa_kv_layer* layers,
                                int n_layers, int kvt, int* status, void* work, hipStream_t st) {
     int* w = static_cast<int*>(work);
-    hipLaunchKernelGGL(k_extend, dim3(1), dim3(PG_T), 0, st, p, seqs, add, n, status, w);
+    // (few requests: the barriers of a small workgroup cost less; 3 requests 9.9 instead of 12.5 us)
+    if (n <= 256) hipLaunchKernelGGL(k_extend<256>, dim3(1), dim3(256), 0, st, p, seqs, add, n, status, w);
+    else hipLaunchKernelGGL(k_extend<PG_T>, dim3(1), dim3(PG_T), 0, st, p, seqs, add, n, status, w);
     const long long units = std::max(1LL, (long long)n * n_layers * NKV);
     hipLaunchKernelGGL(k_move<false>, dim3((unsigned)std::min(units, PG_MOVE_WG)), dim3(256), 0, st, p, w,
                        page_layers(layers, n_layers), n_layers, value_bytes(kvt), kvt == QWA_KV_F16 ? 0 : 16,
@@ -372,13 +480,14 @@ hipError_t launch_pages_compact(const qwa_kv_pages& p, const qwa_kv_layer* layer
 
 hipError_t launch_pages_fork(const qwa_kv_pages& p, const int* src, const int* dst, int n, void* work, hipStream_t st) {
     int* w = static_cast<int*>(work);
-    hipLaunchKernelGGL(k_fork_stage, dim3(n), dim3(256), 0, st, p, src, dst, n, w);
-    hipLaunchKernelGGL(k_fork_commit, dim3(n), dim3(256), 0, st, p, dst, n, w);
+    const dim3 grid((n + PG_CH - 1) / PG_CH), block(PG_RT);
+    hipLaunchKernelGGL(k_fork_stage, grid, block, 0, st, p, src, dst, n, w);
+    hipLaunchKernelGGL(k_fork_commit, grid, block, 0, st, p, dst, n, w);
     return hipGetLastError();
 }
 
 hipError_t launch_pages_trim(const qwa_kv_pages& p, const int* seqs, const int* lens, int n, hipStream_t st) {
-    hipLaunchKernelGGL(k_trim, dim3(n), dim3(256), 0, st, p, seqs, lens, n);
+    hipLaunchKernelGGL(k_trim, dim3((n + PG_CH - 1) / PG_CH), dim3(PG_RT), 0, st, p, seqs, lens, n);
     return hipGetLastError();
 }
 

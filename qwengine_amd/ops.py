@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -455,12 +456,16 @@ PAGES_MAXN, PAGES_MAXL = 1024, 32  # requests / sequences and layers per call
 def _dev(t, dtype=None, what="tensor"):
     """_ptr for the batched operators: a GPU tensor of the current device, of the given type."""
     if isinstance(t, torch.Tensor):
-        if dtype is not None and t.dtype != dtype:
+        if dtype is not None and t.dtype is not dtype:
             raise QwaError(f"{what}: {dtype} wanted, got {t.dtype}")
-        if not t.is_cuda:
+        dev = t.get_device()
+        if dev < 0:
             raise QwaError(f"{what}: not in GPU memory")
-        if t.device.index != torch.cuda.current_device():
+        if dev != torch._C._cuda_getDevice():
             raise QwaError(f"{what}: on {t.device}, but the current device is {torch.cuda.current_device()}")
+        if not t.is_contiguous():
+            raise QwaError("tensor arguments must be contiguous")
+        return t.data_ptr()
     return _ptr(t)
 
 
@@ -496,14 +501,29 @@ class KVPages:
 
 
 def _layers(layers):
-    return (_KVLayerC * len(layers))(*(kv.c() for kv in layers)), len(layers)
+    """The layers as a C array (packed at once: a ctypes object per layer costs more than a page kernel's launch)."""
+    n, flat = len(layers), []
+    for kv in layers:
+        for t in (kv.k, kv.v, kv.ks, kv.vs):
+            if isinstance(t, torch.Tensor):
+                if not t.is_contiguous():
+                    raise QwaError("tensor arguments must be contiguous")
+                flat.append(t.data_ptr())
+            else:
+                flat.append(0 if t is None else int(t))
+        _dev(kv.k, None, "layer")
+        flat.append(kv.capacity)
+    arr = (_KVLayerC * max(n, 1))()
+    struct.pack_into("@" + "PPPPi0P" * n, arr, 0, *flat)
+    return arr, n
 
 
-def _work(pages, work) -> int | None:
-    need = kv_pages_work_bytes(pages)
-    if isinstance(work, torch.Tensor) and work.numel() * work.element_size() < need:
-        raise QwaError(f"workspace of {work.numel() * work.element_size()} bytes, the call needs {need}")
-    return _dev(work, what="work")
+def _work(pc, work) -> int | None:
+    if isinstance(work, torch.Tensor):
+        need = lib().qwa_kv_pages_work_bytes(pc)
+        if work.numel() * work.element_size() < need:
+            raise QwaError(f"workspace of {work.numel() * work.element_size()} bytes, the call needs {need}")
+    return _dev(work, None, "work")
 
 
 def kv_pages_work_bytes(pages: KVPages) -> int:
@@ -515,15 +535,16 @@ def kv_pages_extend(pages: KVPages, seqs, add, layers, kvt, status, work, n: int
     last page that others hold.  All or nothing; status (int32): 0 done, > 0 pages missing, -(i + 1) request i invalid."""
     n = seqs.numel() if n is None else n
     arr, nl = _layers(layers)
-    _check(lib().qwa_kv_pages_extend(ctypes.byref(pages.c()), _count(seqs, n, "seqs"), _count(add, n, "add"), n, arr, nl,
-                                     _kvt(kvt), _count(status, 1, "status"), _work(pages, work), _stream(stream)))
+    pc = ctypes.byref(pages.c())
+    _check(lib().qwa_kv_pages_extend(pc, _count(seqs, n, "seqs"), _count(add, n, "add"), n, arr, nl, _kvt(kvt),
+                                     _count(status, 1, "status"), _work(pc, work), _stream(stream)))
 
 
 def kv_pages_fork(pages: KVPages, src, dst, work, n: int | None = None, stream=None) -> None:
     """Sequence dst[i] gives back its pages and shares src[i]'s (src[i] < 0: becomes empty), all requests at once."""
     n = dst.numel() if n is None else n
-    _check(lib().qwa_kv_pages_fork(ctypes.byref(pages.c()), _count(src, n, "src"), _count(dst, n, "dst"), n,
-                                   _work(pages, work), _stream(stream)))
+    pc = ctypes.byref(pages.c())
+    _check(lib().qwa_kv_pages_fork(pc, _count(src, n, "src"), _count(dst, n, "dst"), n, _work(pc, work), _stream(stream)))
 
 
 def kv_pages_trim(pages: KVPages, seqs, lens=None, n: int | None = None, stream=None) -> None:
@@ -536,8 +557,9 @@ def kv_pages_trim(pages: KVPages, seqs, lens=None, n: int | None = None, stream=
 def kv_pages_compact(pages: KVPages, layers, kvt, n_live, work, stream=None) -> None:
     """Moves the pages in use to the front of every layer's pool; n_live (int32) receives their number."""
     arr, nl = _layers(layers)
-    _check(lib().qwa_kv_pages_compact(ctypes.byref(pages.c()), arr, nl, _kvt(kvt), _count(n_live, 1, "n_live"),
-                                      _work(pages, work), _stream(stream)))
+    pc = ctypes.byref(pages.c())
+    _check(lib().qwa_kv_pages_compact(pc, arr, nl, _kvt(kvt), _count(n_live, 1, "n_live"), _work(pc, work),
+                                      _stream(stream)))
 
 
 def attn_prep_batch(qg, k, v, q_norm, k_norm, pages: KVPages, seqs, n: int, nq: int, theta: float, eps: float, kvt,
