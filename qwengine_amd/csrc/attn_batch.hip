@@ -23,19 +23,8 @@
 
 namespace qwa {
 
-#ifndef QWA_KD
-#define QWA_KD 1
-#endif
-#ifndef QWA_VD
-#define QWA_VD 3
-#endif
-constexpr int BT_KD = QWA_KD;  // K steps read ahead of their MFMAs
-constexpr int BT_VD = QWA_VD;  // V fragments in flight
-#ifndef QWA_ROWS4
-#define QWA_ROWS4 3072
-#endif
-constexpr int BT_ROWS4 = QWA_ROWS4;  // rows up to which a combine workgroup has one row
-
+constexpr int BT_KD = 1;  // K steps read ahead of their MFMAs
+constexpr int BT_VD = 3;  // V fragments in flight
 size_t batch_work_bytes(int n, int nq, int n_shared, int max_len) {
     return batch_work(batch_plan(n, nq, n_shared, max_len), n, nq).bytes;
 }
@@ -57,9 +46,6 @@ struct BatchArgs {
     int n, nq, n_shared, max_len, wgs;
 };
 
-#ifndef QWA_SB
-#define QWA_SB __builtin_amdgcn_sched_barrier(0)
-#endif
 // positions of batch row b, cut to max_len; 0 for an unknown sequence
 __device__ __forceinline__ int bt_seq(const BatchArgs& a, int b) { return a.seqs ? a.seqs[b] : b; }
 __device__ __forceinline__ int bt_len(const BatchArgs& a, const qwa_kv_pages& p, int b) {
@@ -89,26 +75,44 @@ __device__ __forceinline__ int bt_place(const qwa_kv_pages& p, const int* __rest
     return (unsigned)pg < (unsigned)p.n_pages ? pg * p.page + (kb & (p.page - 1)) : -1;
 }
 
-#ifndef QWA_K1
-#define QWA_K1 1
-#endif
-#ifndef QWA_WPE
-#define QWA_WPE 3
-#endif
-#ifndef QWA_QL
-#define QWA_QL 0
-#endif
+// Q4_0 codes with fewer shifts than q4_word_to_h8 / v_pair_words (the same values in the same order): a nibble that sits at
+// bit 4 of a half makes 64 + n there (0x5400 | n << 4), as one at bit 0 makes 1024 + n.
+__device__ __forceinline__ h2 q4_lo(uint32_t w, h2 d) {
+    const h2 bias = {(_Float16)1032.0f, (_Float16)1032.0f};
+    return (bits_h2((w & 0x000F000Fu) | 0x64006400u) - bias) * d;
+}
+__device__ __forceinline__ h2 q4_hi(uint32_t w, h2 d) {
+    const h2 bias = {(_Float16)72.0f, (_Float16)72.0f};
+    return (bits_h2((w & 0x00F000F0u) | 0x54005400u) - bias) * d;
+}
+__device__ __forceinline__ void bt_q4_k(uint32_t w, h2 d, uint32_t* out) {
+    out[0] = h2_bits(q4_lo(w, d));
+    out[1] = h2_bits(q4_hi(w, d));
+    out[2] = h2_bits(q4_lo(w >> 8, d));
+    out[3] = h2_bits(q4_hi(w >> 8, d));
+}
+// out[dim] = {V_a[dim], V_b[dim]} for the 8 (Q4_0), 4 or 2 dims of a word of keys a and b
+template <int KVT>
+__device__ __forceinline__ void bt_v_pair(uint32_t aw, uint32_t bw, uint32_t sa, uint32_t sb, uint32_t* out) {
+    if constexpr (KVT == QWA_KV_Q4_0) {
+        const h2 d = scale_pair((uint16_t)sa, (uint16_t)sb);
+        bt_q4_k(__builtin_amdgcn_perm(bw, aw, 0x05040100u), d, out);      // bytes {a0, a1, b0, b1}
+        bt_q4_k(__builtin_amdgcn_perm(bw, aw, 0x07060302u), d, out + 4);  // bytes {a2, a3, b2, b3}
+    } else {
+        v_pair_words<KVT, 1>(&aw, &bw, sa, sb, out);
+    }
+}
+
 template <int KVT, int RT>
 struct BtCfg {
-    static constexpr int KT = KVT == QWA_KV_F16 || (KVT == QWA_KV_Q8_0 && RT == 1 && QWA_K1 > 0) || (KVT == QWA_KV_Q4_0 && RT == 1 && QWA_K1 > 1) ? 1 : 2;  // 16-key groups of a tile
-    static constexpr int WPE = RT == 1 ? QWA_WPE : 2;                         // waves per SIMD that the registers allow
-    static constexpr bool QLDS = RT > QWA_QL;                  // Q fragments in LDS instead of registers
+    // 16-key groups of a tile, as two waves per SIMD leave registers for (raw bytes of 32 keys: F16 128 registers, Q8_0 66)
+    static constexpr int KT = KVT == QWA_KV_F16 || (KVT == QWA_KV_Q8_0 && RT > 1) ? 1 : 2;
 };
 
 template <int KVT, int RT>
 struct BtLds {
     union {
-        h8 q[RT][8][64];         // while the keys are walked
+        h8 q[RT][8][64];        // while the keys are walked
         f4 o[BT_WAVES][8][64];  // while the waves' states are joined, half of the output tiles at a time
     };
     float ml[BT_WAVES][2][64];
@@ -124,7 +128,6 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
                                         int rstep) {
     auto& s_o = lds.o;
     auto& s_ml = lds.ml;
-    constexpr bool QLDS = BtCfg<KVT, RT>::QLDS;
     constexpr int KT = BtCfg<KVT, RT>::KT, VB = value_bytes(KVT), TILE = 16 * KT;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int i16 = lane & 15, lg = lane >> 4;
@@ -135,10 +138,8 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
 
     auto place = [&](int kb) { return bt_place(p, table, kb, k1); };
     // Raw bytes of a tile.  K: 16-byte piece 4 i + lg of row i16 in words 4 i .. 4 i + 3, so that one load instruction takes
-    // 64 consecutive bytes of 16 rows and no two of them the same ones (with two pieces side by side per lane the loads of
-    // a tile met each other's cache lines in flight and stalled there: 24 sequences of up to 16384 Q4_0 positions 101 us).
-    // V: the lane's 16 dims of row 4 lg + j, F16 as two runs of 8 dims 128 apart for the same reason.  Block scales: the 16
-    // rows' 256 bytes, a dword a lane, handed out by lane permutes when they are used.
+    // 64 consecutive bytes of 16 rows.  V: the lane's 16 dims of row 4 lg + j, F16 as two runs of 8 dims 128 apart (whole cache
+    // lines).  Block scales: the 16 rows' 256 bytes, a dword a lane, handed out by lane permutes when they are used.
     constexpr bool SC = KVT != QWA_KV_F16;
     constexpr int KW = VB / 16, VW = VB / 64;  // words per lane of a K row and of a V row
     uint32_t kr[KT][KW], vr[4 * KT][VW], ksd[KT], vsd[KT];
@@ -222,7 +223,6 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
     }
     // rows of this lane: Q / 16 as the B operand in the K operand's dim order, keys below vis are seen
     constexpr int E = 4096 / VB;  // values of a 16-byte piece of a row
-    h8 qb[QLDS ? 1 : RT][8];
     int vis[RT], vmin = k1;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
@@ -233,7 +233,7 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
         const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + E * lg;
 #pragma unroll
         for (int s = 0; s < 8; s++) {
-            if (QLDS && s / 2 != wave) continue;  // (the waves' share)
+            if (s / 2 != wave) continue;  // (the waves' share)
             const float* src = qrow + 4 * E * (8 * s / E) + 8 * s % E;
             const float4 x0 = *reinterpret_cast<const float4*>(src);
             const float4 x1 = *reinterpret_cast<const float4*>(src + 4);
@@ -241,11 +241,10 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
             h8 v;
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
-            if constexpr (QLDS) lds.q[rt][s][lane] = v;
-            else qb[rt][s] = v;
+            lds.q[rt][s][lane] = v;
         }
     }
-    if constexpr (QLDS) __syncthreads();
+    __syncthreads();
     // (uniform: the least over the 16 lanes that hold different rows)
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
@@ -295,17 +294,17 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
                     q8_word_to_h4(kr[kt][2 * s], kd[kt][s / 2], w);
                     q8_word_to_h4(kr[kt][2 * s + 1], kd[kt][s / 2], w + 2);
                 } else {
-                    q4_word_to_h8(kr[kt][s], kd[kt][s / 4], w);
+                    bt_q4_k(kr[kt][s], kd[kt][s / 4], w);
                 }
                 ka[kt] = make_h8(w[0], w[1], w[2], w[3]);
             }
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
-                const h8 b = QLDS ? lds.q[rt][s][lane] : qb[QLDS ? 0 : rt][s];
+                const h8 b = lds.q[rt][s][lane];
 #pragma unroll
                 for (int kt = 0; kt < KT; kt++) S[rt][kt] = mfma16(ka[kt], b, S[rt][kt]);
             }
-            QWA_SB;
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (nb < k1) load_ks(nat, nb);
 
@@ -361,11 +360,11 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
         constexpr int DPW = 16 / VW;
 #pragma unroll
         for (int wi = 0; wi < VW; wi++) {
-            QWA_SB;
+            __builtin_amdgcn_sched_barrier(0);
             uint32_t w[2 * KT][DPW];
 #pragma unroll
             for (int h = 0; h < 2 * KT; h++)
-                v_pair_words<KVT, 1>(&vr[2 * h][wi], &vr[2 * h + 1][wi], vd[2 * h], vd[2 * h + 1], w[h]);
+                bt_v_pair<KVT>(vr[2 * h][wi], vr[2 * h + 1][wi], vd[2 * h], vd[2 * h + 1], w[h]);
 #pragma unroll
             for (int d = 0; d < DPW; d++)
 #pragma unroll
@@ -431,7 +430,7 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
 
 // the shared positions, for the rows of one group: workgroup = (key range, KV head, row group)
 template <int KVT, int RT>
-__global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(BtCfg<KVT, RT>::WPE)))
+__global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len, int groups) {
     __shared__ BtLds<KVT, RT> lds;
     // the groups of one (range, head) read the same keys: workgroups 8 apart, which one XCD runs
@@ -455,7 +454,7 @@ __device__ __forceinline__ int bt_steps(const BatchArgs& a, const qwa_kv_pages& 
 
 // the own positions: workgroup = (slice of the steps, KV head, row group), one segment per sequence that the slice meets
 template <int KVT, int RT>
-__global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(BtCfg<KVT, RT>::WPE)))
+__global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
     __shared__ BtLds<KVT, RT> lds;
     // the groups of one (slice, head) read the same keys: workgroups 8 apart, which one XCD runs
@@ -587,8 +586,8 @@ __device__ __forceinline__ void bt_raw_store(const BtRaw<KVT>& r, _Float16* Ks, 
 #pragma unroll
         for (int i = 0; i < VW; i++) {
             uint32_t lo[DPW], hi[DPW];
-            v_pair_words<KVT, 1>(&r.w[i], &r.w[VW + i], r.sc[0] & 0xFFFFu, r.sc[0] >> 16, lo);
-            v_pair_words<KVT, 1>(&r.w[2 * VW + i], &r.w[3 * VW + i], r.sc[1] & 0xFFFFu, r.sc[1] >> 16, hi);
+            bt_v_pair<KVT>(r.w[i], r.w[VW + i], r.sc[0] & 0xFFFFu, r.sc[0] >> 16, lo);
+            bt_v_pair<KVT>(r.w[2 * VW + i], r.w[3 * VW + i], r.sc[1] & 0xFFFFu, r.sc[1] >> 16, hi);
 #pragma unroll
             for (int d = 0; d < DPW; d++) *reinterpret_cast<uint2*>(dst + 8 * 32 * (DPW * i + d)) = make_uint2(lo[d], hi[d]);
         }
@@ -605,7 +604,7 @@ __device__ __forceinline__ void bt_raw_store(const BtRaw<KVT>& r, _Float16* Ks, 
                 q8_word_to_h4(r.w[2 * i], d, o);
                 q8_word_to_h4(r.w[2 * i + 1], d, o + 2);
             } else {
-                q4_word_to_h8(r.w[i], d, o);
+                bt_q4_k(r.w[i], d, o);
             }
             *reinterpret_cast<uint4*>(dst + 8 * 32 * i) = make_uint4(o[0], o[1], o[2], o[3]);
         }
@@ -984,9 +983,10 @@ hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_l
         default: launch_ranges<QWA_KV_Q4_0>(a, kv, p, b, st); break;
     }
     const qwa_act_q8 act = oq ? *oq : qwa_act_q8{nullptr, nullptr, nullptr};
-    // few rows with many states: a workgroup per row
-    const int rows = n * nq * NH;
-    if (rows <= BT_ROWS4)
+    // with many states a workgroup per row, else a wave (us, wave / workgroup: 768 rows of about 72 states 22.0 / 11.6, 840 of
+    // 66 12.7 / 8.8, 48 of 97 14.0 / 7.4; 576 of 10 5.2 / 5.5, 3072 of 19 11.0 / 19.2, 9600 of 2 11.6 / 29.2)
+    const int rows = n * nq * NH, states = b.nt + b.ns_shared + (b.wgs > 0 ? b.wgs / n + 1 : 0);
+    if (states > 24)
         hipLaunchKernelGGL(k_bt_combine<4>, dim3(rows), dim3(256), 0, st, a, p, gate, b.nt, b.ns_shared, out16, act,
                            oq != nullptr ? 1 : 0);
     else

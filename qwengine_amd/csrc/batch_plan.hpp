@@ -14,9 +14,7 @@ namespace qwa {
 
 constexpr int BT_WAVES = 4;   // waves of a register workgroup; they take the tiles of its key range in turn
 constexpr int BT_MAXRT = 2;   // 16-row MFMA tiles of such a workgroup at most
-#ifndef QWA_FILL
-#define QWA_FILL 768
-#endif
+constexpr int BT_FILL = 512;  // register workgroups that the chip holds, two a CU
 constexpr int BT_TWAVES = 12;                // waves of a tile workgroup
 constexpr int BT_TROWS = 16 * BT_TWAVES;  // its rows
 constexpr int BT_STEP = 128;  // positions of a step; key ranges are whole steps
@@ -62,11 +60,11 @@ inline BatchPlan batch_plan(int n, int nq, int n_shared, int max_len) {
         p.nt = std::min(tiles, std::max(1, 256 / (p.blocks * NKV)));
         p.len_shared = BT_STEP;
     } else {
-        bt_cut(n_shared, p.groups_shared * NKV, 512, 128, &p.ns_shared, &p.len_shared);
+        bt_cut(n_shared, p.groups_shared * NKV, BT_FILL, 128, &p.ns_shared, &p.len_shared);
     }
     if (max_len > n_shared) {
         const long long steps = (long long)n * ((max_len - (n_shared & ~15) + BT_STEP - 1) / BT_STEP);
-        p.wgs = (int)std::min<long long>(steps, std::max(1, QWA_FILL / (NKV * p.groups)));
+        p.wgs = (int)std::min<long long>(steps, std::max(1, BT_FILL / (NKV * p.groups)));
     }
     return p;
 }
