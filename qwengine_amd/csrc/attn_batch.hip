@@ -669,24 +669,47 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
         if (converts) load(0);
     }
 
-    // this lane's row, its bound and Q / 16 as the B operand
+    // Q / 16 as the B operand, by way of the wave's part of the exchange: a row is read as one kilobyte (fragment by fragment,
+    // 16 rows at once, the loads took 7 us), its fp16 pieces go to unit (s, lg, row ^ (4 s + lg) % 16) and come back as the
+    // lane's fragments s
     const int r = wrow0 + i16, tok = r / GRP;
     const bool valid = r < nrows;
+    h8 qb[8];
+    {
+        float4 x[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int rj = min(wrow0 + j, nrows - 1);
+            x[j] = *reinterpret_cast<const float4*>(a.q + ((size_t)(rj / GRP) * NH + g * GRP + rj % GRP) * HD + 4 * lane);
+        }
+        uint8_t* const area = reinterpret_cast<uint8_t*>(lds.xch[wave]);
+        const int c = lane >> 1, half = lane & 1;  // piece c = 4 s + lg, dims 4 half .. 4 half + 3 of it
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float f = wrow0 + j < nrows ? 0.0625f : 0.0f;
+            uint32_t w0 = h2_bits(h2{(_Float16)(x[j].x * f), (_Float16)(x[j].y * f)});
+            uint32_t w1 = h2_bits(h2{(_Float16)(x[j].z * f), (_Float16)(x[j].w * f)});
+            if constexpr (KVT == QWA_KV_Q4_0) {
+                // the operand's order [0, 4, 1, 5, 2, 6, 3, 7]: the even lane makes the first two words, the odd one the rest
+                const uint32_t mine = half ? w1 : w0, other = __builtin_amdgcn_update_dpp(0, half ? w0 : w1, 0xB1, 0xF, 0xF, true);
+                const uint32_t lo = half ? other : mine, hi = half ? mine : other;  // dims k, k + 1 and k + 4, k + 5
+                w0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+                w1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+            }
+            *reinterpret_cast<uint2*>(area + 16 * (16 * c + (j ^ (c & 15))) + 8 * half) = make_uint2(w0, w1);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int s = 0; s < 8; s++)
+            qb[s] = *reinterpret_cast<const h8*>(area + 16 * (16 * (4 * s + lg) + (i16 ^ ((4 * s + lg) & 15))));
+    }
     const int vis = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, end) : 0;
     int vmin = valid ? vis : 0x7fffffff;
-    h8 qb[8];
-    const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + 8 * lg;
-#pragma unroll
-    for (int s = 0; s < 8; s++) {
-        const float4 x0 = *reinterpret_cast<const float4*>(qrow + 32 * s);
-        const float4 x1 = *reinterpret_cast<const float4*>(qrow + 32 * s + 4);
-        const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-        for (int j = 0; j < 8; j++) qb[s][j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
-    }
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
     vmin = __builtin_amdgcn_readfirstlane(vmin);
+    __syncthreads();  // the fragments are in registers; the tiles lie in the same LDS
 
     f4 o[16];
     float m = -INFINITY, l = 0.0f;
@@ -792,18 +815,21 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
 #pragma unroll
         for (int j = 0; j < 4; j++) amax = fmaxf(amax, fabsf(o[dt][j]));
     amax = rows_max(amax) * il;
-    const float qs = amax > 1e-30f ? 32767.0f / amax : 0.0f, f = il * qs;
+    const float f = amax > 1e-30f ? il / amax : 0.0f;
     const size_t range = (size_t)sp * a.n * a.nq * NH + g * GRP;
     // (a row whose O is not finite has no fixed-point form: its scale makes every value NaN)
-    const float scale = amax < INFINITY ? (qs > 0.0f ? amax * (1.0f / 32767.0f) : 0.0f) : NAN;
+    const float scale = amax < INFINITY ? (f != 0.0f ? amax * (1.0f / 32767.0f) : 0.0f) : NAN;
     if (valid && lg == 0) a.tile_ml[range + (size_t)tok * NH + r % GRP] = make_float4(m, lt, scale, 0.0f);
+    auto pack = [&](float x, float y) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(x * f, y * f));
+    };
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const int e = q & 1, k = 4 * (q >> 1);  // dims 8 x + k .. + 3: 8-byte unit 2 x + k / 4
             xch[64 * i16 + ((2 * (16 * e + 4 * lg + j) + k / 4) ^ (4 * i16))] =
-                pack16x4(o[2 * k + e][j] * f, o[2 * k + 2 + e][j] * f, o[2 * k + 4 + e][j] * f, o[2 * k + 6 + e][j] * f);
+                make_uint2(pack(o[2 * k + e][j], o[2 * k + 2 + e][j]), pack(o[2 * k + 4 + e][j], o[2 * k + 6 + e][j]));
         }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
     __builtin_amdgcn_wave_barrier();
@@ -984,7 +1010,8 @@ hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_l
     }
     const qwa_act_q8 act = oq ? *oq : qwa_act_q8{nullptr, nullptr, nullptr};
     // with many states a workgroup per row, else a wave (us, wave / workgroup: 768 rows of about 72 states 22.0 / 11.6, 840 of
-    // 66 12.7 / 8.8, 48 of 97 14.0 / 7.4; 576 of 10 5.2 / 5.5, 3072 of 19 11.0 / 19.2, 9600 of 2 11.6 / 29.2)
+    // 66 12.7 / 8.8, 48 of 97 14.0 / 7.4; 576 of 10 5.2 / 5.5, the rows of
+    // 128 sequences of 19 states 11.0 / 19.2, 9600 of 2 11.6 / 29.2)
     const int rows = n * nq * NH, states = b.nt + b.ns_shared + (b.wgs > 0 ? b.wgs / n + 1 : 0);
     if (states > 24)
         hipLaunchKernelGGL(k_bt_combine<4>, dim3(rows), dim3(256), 0, st, a, p, gate, b.nt, b.ns_shared, out16, act,
