@@ -453,11 +453,13 @@ def kv_append(xk, xv, pos0: int, n: int, kvt, kv: KVLayer, stream=None) -> None:
 PAGES_MAXN, PAGES_MAXL = 1024, 32  # requests / sequences and layers per call
 
 
-def _dev(t, dtype=None, what="tensor"):
-    """_ptr for the batched operators: a GPU tensor of the current device, of the given type."""
+def _dev(t, dtype=None, what="tensor", least=0):
+    """_ptr for the batched operators: a GPU tensor of the current device, of the given type, with `least` entries or more."""
     if isinstance(t, torch.Tensor):
         if dtype is not None and t.dtype is not dtype:
             raise QwaError(f"{what}: {dtype} wanted, got {t.dtype}")
+        if t.numel() < least:
+            raise QwaError(f"{what}: {t.numel()} entries, {least} wanted")
         dev = t.get_device()
         if dev < 0:
             raise QwaError(f"{what}: not in GPU memory")
@@ -471,9 +473,7 @@ def _dev(t, dtype=None, what="tensor"):
 
 def _count(t, n, what):
     """An index tensor of at least n entries."""
-    if isinstance(t, torch.Tensor) and t.numel() < n:
-        raise QwaError(f"{what}: {t.numel()} entries, {n} wanted")
-    return _dev(t, torch.int32, what)
+    return _dev(t, torch.int32, what, n)
 
 
 @dataclass
@@ -500,10 +500,20 @@ class KVPages:
                          self.ref.numel(), self.page)
 
 
-def _layers(layers):
+def _pool(kv, kvt):
+    """A layer as the pool of a batched call."""
+    _dev(kv.k, None, "layer")
+    if kv.kvt != kvt:
+        raise QwaError(f"a layer of KV type {kv.kvt}, {kvt} wanted")
+    return ctypes.byref(kv.c())
+
+
+def _layers(layers, kvt):
     """The layers as a C array (packed at once: a ctypes object per layer costs more than a page kernel's launch)."""
     n, flat = len(layers), []
     for kv in layers:
+        if kv.kvt != kvt:
+            raise QwaError(f"a layer of KV type {kv.kvt}, {kvt} wanted")
         for t in (kv.k, kv.v, kv.ks, kv.vs):
             if isinstance(t, torch.Tensor):
                 if not t.is_contiguous():
@@ -533,10 +543,10 @@ def kv_pages_work_bytes(pages: KVPages) -> int:
 def kv_pages_extend(pages: KVPages, seqs, add, layers, kvt, status, work, n: int | None = None, stream=None) -> None:
     """Room for add[i] more positions of sequence seqs[i] (int32 GPU tensors): takes free pages, and copies a partly filled
     last page that others hold.  All or nothing; status (int32): 0 done, > 0 pages missing, -(i + 1) request i invalid."""
-    n = seqs.numel() if n is None else n
-    arr, nl = _layers(layers)
+    n, kvt = seqs.numel() if n is None else n, _kvt(kvt)
+    arr, nl = _layers(layers, kvt)
     pc = ctypes.byref(pages.c())
-    _check(lib().qwa_kv_pages_extend(pc, _count(seqs, n, "seqs"), _count(add, n, "add"), n, arr, nl, _kvt(kvt),
+    _check(lib().qwa_kv_pages_extend(pc, _count(seqs, n, "seqs"), _count(add, n, "add"), n, arr, nl, kvt,
                                      _count(status, 1, "status"), _work(pc, work), _stream(stream)))
 
 
@@ -556,21 +566,23 @@ def kv_pages_trim(pages: KVPages, seqs, lens=None, n: int | None = None, stream=
 
 def kv_pages_compact(pages: KVPages, layers, kvt, n_live, work, stream=None) -> None:
     """Moves the pages in use to the front of every layer's pool; n_live (int32) receives their number."""
-    arr, nl = _layers(layers)
+    kvt = _kvt(kvt)
+    arr, nl = _layers(layers, kvt)
     pc = ctypes.byref(pages.c())
-    _check(lib().qwa_kv_pages_compact(pc, arr, nl, _kvt(kvt), _count(n_live, 1, "n_live"), _work(pc, work),
+    _check(lib().qwa_kv_pages_compact(pc, arr, nl, kvt, _count(n_live, 1, "n_live"), _work(pc, work),
                                       _stream(stream)))
 
 
 def attn_prep_batch(qg, k, v, q_norm, k_norm, pages: KVPages, seqs, n: int, nq: int, theta: float, eps: float, kvt,
                     kv: KVLayer, q_out, gate, rope_off=None, stream=None) -> None:
     """attn_prep_multi for the last nq positions of n sequences (seqs int32, None: 0..n-1) of a paged cache."""
-    f32 = torch.float32
+    f32, kvt, T, HD = torch.float32, _kvt(kvt), n * nq, 256
     _check(lib().qwa_attn_prep_batch(
-        _dev(qg, f32, "qg"), _dev(k, f32, "k"), _dev(v, f32, "v"), _dev(q_norm, f32, "q_norm"), _dev(k_norm, f32, "k_norm"),
-        ctypes.byref(pages.c()), None if seqs is None else _count(seqs, n, "seqs"), n, nq,
-        None if rope_off is None else _count(rope_off, n, "rope_off"), theta, eps, _kvt(kvt), ctypes.byref(kv.c()),
-        _dev(q_out, f32, "q_out"), _dev(gate, f32, "gate"), _stream(stream)))
+        _dev(qg, f32, "qg", T * 48 * HD), _dev(k, f32, "k", T * N_KV * HD), _dev(v, f32, "v", T * N_KV * HD),
+        _dev(q_norm, f32, "q_norm", HD), _dev(k_norm, f32, "k_norm", HD), ctypes.byref(pages.c()),
+        None if seqs is None else _count(seqs, n, "seqs"), n, nq, None if rope_off is None else _count(rope_off, n, "rope_off"),
+        theta, eps, kvt, _pool(kv, kvt), _dev(q_out, f32, "q_out", T * 24 * HD), _dev(gate, f32, "gate", T * 24 * HD),
+        _stream(stream)))
 
 
 def attn_batch_work_bytes(n: int, nq: int, n_shared: int, max_len: int) -> int:
@@ -581,11 +593,14 @@ def attn_decode_batch(q, gate, kv: KVLayer, kvt, pages: KVPages, seqs, n: int, n
                       work, oq: ActQ8 | None = None, stream=None) -> None:
     """Attention of n sequences (seqs int32, None: 0..n-1) with nq queries each over a paged cache; the first n_shared
     positions, which all of them have in common, are read once.  out16: fp16 [n * nq, 6144]."""
-    f32 = torch.float32
+    f32, kvt, size = torch.float32, _kvt(kvt), n * nq * 6144
+    if oq is not None:
+        for x, dt, m, what in ((oq.q, torch.int8, size, "oq.q"), (oq.d, f32, size // 32, "oq.d"), (oq.s, f32, size // 32, "oq.s")):
+            _dev(x, dt, what, m)
     _check(lib().qwa_attn_decode_batch(
-        _dev(q, f32, "q"), _dev(gate, f32, "gate"), ctypes.byref(kv.c()), _kvt(kvt), ctypes.byref(pages.c()),
+        _dev(q, f32, "q", size), _dev(gate, f32, "gate", size), _pool(kv, kvt), kvt, ctypes.byref(pages.c()),
         None if seqs is None else _count(seqs, n, "seqs"), n, nq, n_shared, max_len,
-        _dev(out16, torch.float16, "out16"), _act(oq), _dev(work, what="work"),
+        _dev(out16, torch.float16, "out16", size), _act(oq), _dev(work, what="work"),
         work.numel() * work.element_size() if isinstance(work, torch.Tensor) else 1 << 62, _stream(stream)))
 
 

@@ -157,6 +157,34 @@ def test_tensor_arguments_are_checked():
         ops.KVPages(torch.zeros((2, 4), dtype=torch.int32), torch.zeros(3, dtype=torch.int32), i32, 64).c()
 
 
+def test_tensor_sizes_and_layer_types_are_checked():
+    """Buffers of too few rows, and layers of another type than the call's, never reach the library."""
+    f32 = lambda n: torch.zeros(n)
+    rows = 2 * 6144
+    for i in range(2):
+        bufs = [P] * 4
+        bufs[i] = f32(rows - 1)
+        with pytest.raises(ops.QwaError, match=f"{rows - 1} entries, {rows} wanted"):
+            decode(bufs=bufs)
+    with pytest.raises(ops.QwaError, match="out16: 6144 entries"):
+        decode(bufs=[P, P, torch.zeros(6144, dtype=torch.float16), P])
+    for i, want in enumerate([2 * rows, 2048, 2048, 256, 256, rows, rows]):
+        bufs = [P] * 7
+        bufs[i] = f32(want - 1)
+        with pytest.raises(ops.QwaError, match=f"{want - 1} entries, {want} wanted"):
+            prep(bufs=bufs)
+    with pytest.raises(ops.QwaError, match="oq.d"):
+        decode(oq=ops.ActQ8(P, f32(rows // 32 - 1), P))
+    with pytest.raises(ops.QwaError, match="oq.q: torch.int8 wanted"):
+        decode(oq=ops.ActQ8(f32(rows), P, P))
+    for call in (prep, decode):
+        with pytest.raises(ops.QwaError, match="layer of KV type"):
+            call(kvt="q4_0", kv=layer("q8_0"))
+    for call in (extend, compact):
+        with pytest.raises(ops.QwaError, match="layer of KV type"):
+            call(kvt="f16", layers=[layer("f16"), layer("q8_0")])
+
+
 PLAN = r'''
 #include <stdio.h>
 #include "batch_plan.hpp"
