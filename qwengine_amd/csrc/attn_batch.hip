@@ -809,12 +809,12 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
     __syncthreads();
     const float lt = rows_sum(l);
     const float il = lt == 0.0f ? 0.0f : 1.0f / lt;  // (a row that saw nothing: l = 0 and O = 0)
-    float amax = 0.0f;
+    float amax = 0.0f;  // (maximum, unlike fmaxf, keeps a NaN)
 #pragma unroll
     for (int dt = 0; dt < 16; dt++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) amax = fmaxf(amax, fabsf(o[dt][j]));
-    amax = rows_max(amax) * il;
+        for (int j = 0; j < 4; j++) amax = __builtin_elementwise_maximum(amax, fabsf(o[dt][j]));
+    amax = lt == 0.0f ? 0.0f : rows_max(amax < INFINITY ? amax : INFINITY) * il;
     const float f = amax > 1e-30f ? il / amax : 0.0f;
     const size_t range = (size_t)sp * a.n * a.nq * NH + g * GRP;
     // (a row whose O is not finite has no fixed-point form: its scale makes every value NaN)

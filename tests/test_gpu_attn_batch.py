@@ -236,6 +236,104 @@ def test_special_values(gpu):
     assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("n", [2, 9])
+@pytest.mark.parametrize("x", [float("nan"), float("inf")])
+def test_nonfinite_values_of_shared_positions(gpu, n, x):
+    """A value that is not finite shows in every row that sees it, and in no other KV head's rows (9 sequences: the partial
+    states are fixed-point numbers, which have none)."""
+    b = Batch(ops.F16, [200] * n, shared=130)
+    b.kv.v.view(torch.float16)[1, int(b.pages.table[0, 1]) * 64 + 3, 9] = x  # position 67, KV head 1, dim 9
+    _, _, out = b.run(1, 130, 200)
+    bad = ~torch.isfinite(out)
+    assert bad[:, 6:12, 9].all() and not bad[:, :6].any() and not bad[:, 12:].any()
+
+
+def test_captured_calls_share_a_work_buffer(gpu):
+    """Two captured batches with one work buffer, replayed in turn with eager calls in between, while the sequences shrink
+    and grow: every replay has the bits of the eager call."""
+    b = Batch(ops.Q4_0, [700 + 3 * i for i in range(9)], shared=512)
+    few, lens = i32([3, 8]), torch.tensor(b.lens, dtype=torch.int32)
+    new = lambda n, nq: (seeded_normal((n * nq, 24, 256), n), seeded_normal((n * nq, 24, 256), n + 1),
+                         torch.empty((n * nq, 24, 256), dtype=torch.float16, device="cuda"))
+    calls = [(*new(9, 1), None, 9, 1, 512), (*new(2, 5), few, 2, 5, 100)]
+    work = torch.empty(max(ops.attn_batch_work_bytes(n, nq, sh, 768) for *_, n, nq, sh in calls), dtype=torch.uint8,
+                       device="cuda")
+    attend = lambda q, gate, out, seqs, n, nq, sh: ops.attn_decode_batch(q, gate, b.kv, b.kvt, b.pages, seqs, n, nq, sh, 768,
+                                                                         out, work)
+    graphs = []
+    for c in calls:
+        attend(*c)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            attend(*c)
+    for cut in (0, 150, 699, 0, 40):
+        b.pages.len.copy_((lens - cut).clamp_min(0))
+        for c, graph in zip(calls, graphs):
+            attend(*c)
+            want = c[2].clone()
+            c[2].fill_(7.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(c[2], want)
+            c[0].mul_(-1)
+
+
+def test_largest_batch(gpu):
+    b = Batch(ops.Q8_0, [24 + i % 40 for i in range(1024)], shared=16, page=16)
+    b.check(8, 16, what="1024 sequences, 8 queries")
+
+
+@pytest.mark.parametrize("kvt", [ops.F16, ops.Q4_0], ids=lambda k: KV_NAMES[k])
+def test_pools_past_32_bits(gpu, kvt):
+    """Pages whose bytes lie more than 2^32 past the pool's and the KV head's beginning, in every operator."""
+    page, slots = 64, (1 << 33) // (512 if kvt == ops.F16 else 128) // 2 + 4096
+    b = Batch(kvt, [300, 280, 290, 100, 285, 270, 301], shared=256)
+    small, table, n_pages = b.kv, b.pages.table.clone(), slots // page
+    shift = n_pages - b.pages.ref.numel()
+    b.kv = ops.KVLayer.allocate(kvt, slots, zero=False)
+    for dst, src in ((b.kv.k, small.k), (b.kv.v, small.v), (b.kv.ks, small.ks), (b.kv.vs, small.vs)):
+        if dst is not None:
+            dst[:, shift * page:(shift + b.pages.ref.numel()) * page] = src[:, :b.pages.ref.numel() * page]
+    b.pages = ops.KVPages.allocate(7, 320, n_pages, page)
+    b.pages.table.copy_(torch.where(table >= 0, table + shift, table)[:, :1].expand(7, 5))
+    b.pages.table[:, :table.shape[1]] = torch.where(table >= 0, table + shift, table)
+    b.pages.len.copy_(i32(b.lens))
+    held = torch.cat([b.pages.table[i, :-(-m // page)] for i, m in enumerate(b.lens)])
+    b.pages.ref.index_add_(0, held.long(), torch.ones_like(held))
+    b.check(1, 256, what="7 sequences at the end of a large pool")
+    b.check(1, 0, seqs=[3, 0], what="two of them, nothing shared")
+    # the same pages at the pool's beginning, then again with room for one position each
+    work = torch.empty(ops.kv_pages_work_bytes(b.pages), dtype=torch.uint8, device="cuda")
+    n_live, status = i32([0]), i32([9])
+    ops.kv_pages_compact(b.pages, [b.kv], kvt, n_live, work)
+    torch.cuda.synchronize()
+    assert int(n_live) == int((b.pages.ref > 0).sum()) and int(b.pages.table.max()) == int(n_live) - 1
+    b.check(1, 256, what="moved to its beginning")
+    # a fork whose copied last page is the last of the pool
+    b.pages.ref[int(n_live):n_pages - 1] = 1
+    ops.kv_pages_trim(b.pages, i32([6]))
+    free = (b.pages.ref == 0).nonzero().flatten().tolist()
+    b.pages.ref[i32(free[:-1]).long()] = 1
+    ops.kv_pages_fork(b.pages, i32([3]), i32([6]), work)
+    ops.kv_pages_extend(b.pages, i32([6]), i32([1]), [b.kv], kvt, status, work)
+    torch.cuda.synchronize()
+    assert int(status) == 0 and int(b.pages.table[6, 1]) == n_pages - 1
+    ops.kv_pages_trim(b.pages, i32([6]), i32([100]))
+    b.lens[6], b.caches[6] = 100, b.caches[3]
+    b._rows.clear()
+    b.check(1, 0, seqs=[6, 3], what="a fork in its last page")
+    # prep stores there
+    x = lambda *s: seeded_normal(s, 91)
+    ones, q = torch.ones(256, device="cuda"), torch.empty((1, 24, 256), device="cuda")
+    k, v = x(1, 4, 256), x(1, 4, 256)
+    ops.attn_prep_batch(x(1, 24, 512), k, v, ones, ones, b.pages, i32([6]), 1, 1, THETA, EPS, kvt, b.kv, q, q.clone())
+    probe = ops.KVLayer.allocate(kvt, 1)
+    ops.kv_append(k, v, 0, 1, kvt, probe)
+    torch.cuda.synchronize()
+    assert torch.equal(b.kv.v[:, (n_pages - 1) * page + 99 - 64], probe.v[:, 0])
+
+
 # ---- prep -----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("nq", [1, 4, 8])
 @pytest.mark.parametrize("kvt", KVTS, ids=lambda k: KV_NAMES[k])
