@@ -77,13 +77,21 @@ __device__ __forceinline__ int bt_place(const qwa_kv_pages& p, const int* __rest
 
 // Q4_0 codes with fewer shifts than q4_word_to_h8 / v_pair_words (the same values in the same order): a nibble that sits at
 // bit 4 of a half makes 64 + n there (0x5400 | n << 4), as one at bit 0 makes 1024 + n.
+// (w & mask) | magic in one instruction: the mask from a scalar register, the magic from a vector register.  As two
+// instructions, which the compiler makes of two constants, 24 sequences over 16384 Q4_0 positions took 84 instead of 80 us, the
+// tiles of 128 over 32768 156 instead of 147.
+__device__ __forceinline__ uint32_t q4_bits(uint32_t w, uint32_t mask, uint32_t magic) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(magic));
+    return r;
+}
 __device__ __forceinline__ h2 q4_lo(uint32_t w, h2 d) {
     const h2 bias = {(_Float16)1032.0f, (_Float16)1032.0f};
-    return (bits_h2((w & 0x000F000Fu) | 0x64006400u) - bias) * d;
+    return (bits_h2(q4_bits(w, 0x000F000Fu, 0x64006400u)) - bias) * d;
 }
 __device__ __forceinline__ h2 q4_hi(uint32_t w, h2 d) {
     const h2 bias = {(_Float16)72.0f, (_Float16)72.0f};
-    return (bits_h2((w & 0x00F000F0u) | 0x54005400u) - bias) * d;
+    return (bits_h2(q4_bits(w, 0x00F000F0u, 0x54005400u)) - bias) * d;
 }
 __device__ __forceinline__ void bt_q4_k(uint32_t w, h2 d, uint32_t* out) {
     out[0] = h2_bits(q4_lo(w, d));
