@@ -509,22 +509,30 @@ def _pool(kv, kvt):
 
 
 def _layers(layers, kvt):
-    """The layers as a C array (packed at once: a ctypes object per layer costs more than a page kernel's launch)."""
-    n, flat = len(layers), []
+    """The layers as a C array.  Packed at once, the tensors' methods mapped over all of them: a ctypes object per layer costs
+    more than a page kernel's launch."""
+    n, bufs = len(layers), []
     for kv in layers:
         if kv.kvt != kvt:
             raise QwaError(f"a layer of KV type {kv.kvt}, {kvt} wanted")
-        for t in (kv.k, kv.v, kv.ks, kv.vs):
-            if isinstance(t, torch.Tensor):
-                if not t.is_contiguous():
-                    raise QwaError("tensor arguments must be contiguous")
-                flat.append(t.data_ptr())
-            else:
-                flat.append(0 if t is None else int(t))
-        _dev(kv.k, None, "layer")
+        bufs += (kv.k, kv.v) if kvt == F16 else (kv.k, kv.v, kv.ks, kv.vs)
+    per = 2 if kvt == F16 else 4
+    if all(map(torch.is_tensor, bufs)):
+        if not all(map(torch.Tensor.is_contiguous, bufs)):
+            raise QwaError("tensor arguments must be contiguous")
+        devs = set(map(torch.Tensor.get_device, bufs[::per]))
+        if -1 in devs:
+            raise QwaError("layer: not in GPU memory")
+        if devs and devs != {torch._C._cuda_getDevice()}:
+            raise QwaError(f"layers on devices {sorted(devs)}, but the current device is {torch.cuda.current_device()}")
+        at = list(map(torch.Tensor.data_ptr, bufs))
+    else:
+        at = [_dev(b, None, "layer") or 0 for b in bufs]
+    arr, flat = (_KVLayerC * max(n, 1))(), []
+    for i, kv in enumerate(layers):
+        flat += at[per * i:per * i + per]
         flat.append(kv.capacity)
-    arr = (_KVLayerC * max(n, 1))()
-    struct.pack_into("@" + "PPPPi0P" * n, arr, 0, *flat)
+    struct.pack_into("@" + ("PP16xi0P" if kvt == F16 else "PPPPi0P") * n, arr, 0, *flat)
     return arr, n
 
 

@@ -183,6 +183,12 @@ def test_tensor_sizes_and_layer_types_are_checked():
     for call in (extend, compact):
         with pytest.raises(ops.QwaError, match="layer of KV type"):
             call(kvt="f16", layers=[layer("f16"), layer("q8_0")])
+        with pytest.raises(ops.QwaError, match="not in GPU memory"):
+            call(layers=[ops.KVLayer.allocate("q8_0", 1024, device="cpu")])
+        sparse = ops.KVLayer.allocate("q8_0", 2048, device="cpu")
+        sparse.vs = sparse.vs[:, ::2]
+        with pytest.raises(ops.QwaError, match="contiguous"):
+            call(layers=[sparse])
 
 
 PLAN = r'''
