@@ -132,8 +132,9 @@ struct BtLds {
 template <int KVT, int RT>
 __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a, const qwa_kv_layer& kv,
                                         const qwa_kv_pages& p, const int* __restrict__ table, int row0, int rows, int g,
-                                        int k0, int k1, int lo, float* __restrict__ po, float2* __restrict__ pml,
+                                        int k0, int k1_, int lo, float* __restrict__ po, float2* __restrict__ pml,
                                         int rstep) {
+    const int k1 = __builtin_amdgcn_readfirstlane(k1_);
     auto& s_o = lds.o;
     auto& s_ml = lds.ml;
     constexpr int KT = BtCfg<KVT, RT>::KT, VB = value_bytes(KVT), TILE = 16 * KT;
@@ -144,75 +145,66 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
     const uint16_t* const ksh = KVT == QWA_KV_F16 ? nullptr : kv.ks + (size_t)g * kv.capacity * 8;
     const uint16_t* const vsh = KVT == QWA_KV_F16 ? nullptr : kv.vs + (size_t)g * kv.capacity * 8;
 
-    auto place = [&](int kb) { return bt_place(p, table, kb, k1); };
+    // The pool positions of the wave's tiles, 64 tiles ahead: lane l has those of tile l.  (Looked up a tile at a time they
+    // were a memory round trip each, and a wait for all loads on their way.)
+    constexpr int STRIDE = TILE * BT_WAVES;
+    int ahead[KT], tile = 0;
+    auto place = [&](int kb, int* at) {
+        if ((tile & 63) == 0)
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++) ahead[kt] = bt_place(p, table, kb + STRIDE * lane + 16 * kt, k1);
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++) at[kt] = __builtin_amdgcn_readlane(ahead[kt], tile & 63);
+        tile++;
+    };
     // Raw bytes of a tile.  K: 16-byte piece 4 i + lg of row i16 in words 4 i .. 4 i + 3, so that one load instruction takes
     // 64 consecutive bytes of 16 rows.  V: the lane's 16 dims of row 4 lg + j, F16 as two runs of 8 dims 128 apart (whole cache
     // lines).  Block scales: the 16 rows' 256 bytes, a dword a lane, handed out by lane permutes when they are used.
+    // Each 16 keys are a buffer that ends with the range: rows past it, and groups without a place, read as zeros.  So the
+    // loads need no branch, and the waits for K leave V's on their way and the other way round.
     constexpr bool SC = KVT != QWA_KV_F16;
     constexpr int KW = VB / 16, VW = VB / 64;  // words per lane of a K row and of a V row
     uint32_t kr[KT][KW], vr[4 * KT][VW], ksd[KT], vsd[KT];
-    // key rows past the range re-read its last one (their probabilities are exact zeros, so what they hold must be finite:
-    // a stale row need not be), groups without a place are zeros
-    auto load_k = [&](int kt, const uint8_t* src, const uint16_t* ssc, int row, int srow) {
-#pragma unroll
-        for (int i = 0; i < KW / 4; i++) {
-            const uint4 u = ld16(src + (uint32_t)(row * VB + 16 * lg) + 64 * i);
-            kr[kt][4 * i] = u.x; kr[kt][4 * i + 1] = u.y; kr[kt][4 * i + 2] = u.z; kr[kt][4 * i + 3] = u.w;
-        }
-        if constexpr (SC) ksd[kt] = reinterpret_cast<const uint32_t*>(ssc)[(uint32_t)(4 * srow + (lane & 3))];
+    auto buffer = [&](const void* base, int bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00027000);
     };
-    auto load_v = [&](uint32_t* w, const uint8_t* src, int row) {
-        if constexpr (VW == 2) {
-            const uint2 u = ld8(src + (uint32_t)(row * VB + 8 * i16));
-            w[0] = u.x; w[1] = u.y;
-        } else {
-#pragma unroll
-            for (int i = 0; i < VW / 4; i++) {
-                const uint4 u = ld16(src + (uint32_t)(row * VB + 16 * i16) + 256 * i);
-                w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
-            }
-        }
-    };
+    auto rows_of = [&](int at, int kb) { return at < 0 ? 0 : min(max(k1 - kb, 0), 16); };
     auto load_ks = [&](const int* at, int kb) {
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
-            const int last = k1 - 1 - (kb + 16 * kt);
-            const size_t pos = (size_t)max(at[kt], 0);
-            const uint8_t* src = kh + pos * VB;
-            const uint16_t* ssc = SC ? ksh + pos * 8 : nullptr;
-            if (at[kt] >= 0 && last >= 15) {
-                load_k(kt, src, ssc, i16, lane >> 2);
-            } else if (at[kt] >= 0) {
-                load_k(kt, src, ssc, min(i16, last), min(lane >> 2, last));
-            } else {
+            const size_t pos = (size_t)__builtin_amdgcn_readfirstlane(max(at[kt], 0));
+            const int n = __builtin_amdgcn_readfirstlane(rows_of(at[kt], kb + 16 * kt));
+            const auto r = buffer(kh + pos * VB, n * VB);
 #pragma unroll
-                for (int i = 0; i < KW; i++) kr[kt][i] = 0;
-                ksd[kt] = 0;
+            for (int i = 0; i < KW / 4; i++) {
+                const uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, i16 * VB + 16 * lg + 64 * i, 0, 0));
+                kr[kt][4 * i] = x.x; kr[kt][4 * i + 1] = x.y; kr[kt][4 * i + 2] = x.z; kr[kt][4 * i + 3] = x.w;
             }
+            if constexpr (SC) ksd[kt] = __builtin_amdgcn_raw_buffer_load_b32(buffer(ksh + pos * 8, n * 16), 4 * lane, 0, 0);
         }
     };
     auto load_vs = [&](const int* at, int kb) {
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
-            const int last = k1 - 1 - (kb + 16 * kt);
-            const size_t pos = (size_t)max(at[kt], 0);
-            const uint8_t* src = vh + pos * VB;
-            const uint32_t* ssc = SC ? reinterpret_cast<const uint32_t*>(vsh + pos * 8) : nullptr;
-            if (at[kt] >= 0 && last >= 15) {
+            const size_t pos = (size_t)__builtin_amdgcn_readfirstlane(max(at[kt], 0));
+            const int n = __builtin_amdgcn_readfirstlane(rows_of(at[kt], kb + 16 * kt));
+            const auto r = buffer(vh + pos * VB, n * VB);
 #pragma unroll
-                for (int j = 0; j < 4; j++) load_v(vr[4 * kt + j], src + j * VB, 4 * lg);
-                if constexpr (SC) vsd[kt] = ssc[(uint32_t)lane];
-            } else if (at[kt] >= 0) {
+            for (int j = 0; j < 4; j++) {
+                uint32_t* const w = vr[4 * kt + j];
+                if constexpr (VW == 2) {
+                    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, 4 * lg * VB + 8 * i16 + j * VB, 0, 0));
+                    w[0] = x.x; w[1] = x.y;
+                } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) load_v(vr[4 * kt + j], src, min(4 * lg + j, last));
-                if constexpr (SC) vsd[kt] = ssc[(uint32_t)(4 * min(lane >> 2, last) + (lane & 3))];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int i = 0; i < VW; i++) vr[4 * kt + j][i] = 0;
-                vsd[kt] = 0;
+                    for (int i = 0; i < VW / 4; i++) {
+                        const uint4 x = __builtin_bit_cast(
+                            uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 4 * lg * VB + 16 * i16 + j * VB + 256 * i, 0, 0));
+                        w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+                    }
+                }
             }
+            if constexpr (SC) vsd[kt] = __builtin_amdgcn_raw_buffer_load_b32(buffer(vsh + pos * 8, n * 16), 4 * lane, 0, 0);
         }
     };
     // half h (0 / 1) of lane `from`'s dword x, in both halves
@@ -221,14 +213,11 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
         return bits_h2(__builtin_amdgcn_perm(u, u, h ? 0x03020302u : 0x01000100u));
     };
 
-    int kb = k0 + TILE * wave;
+    int kb = __builtin_amdgcn_readfirstlane(k0) + TILE * wave;
     int at[KT];
-#pragma unroll
-    for (int kt = 0; kt < KT; kt++) at[kt] = place(kb + 16 * kt);
-    if (kb < k1) {
-        load_ks(at, kb);
-        load_vs(at, kb);
-    }
+    place(kb, at);
+    load_ks(at, kb);
+    load_vs(at, kb);
     // rows of this lane: Q / 16 as the B operand in the K operand's dim order, keys below vis are seen
     constexpr int E = 4096 / VB;  // values of a 16-byte piece of a row
     int vis[RT], vmin = k1;
@@ -268,11 +257,10 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
         for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    for (; kb < k1; kb += TILE * BT_WAVES) {
-        const int nb = kb + TILE * BT_WAVES;
+    for (; kb < k1; kb += STRIDE) {
+        const int nb = kb + STRIDE;
         int nat[KT];
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++) nat[kt] = place(nb + 16 * kt);
+        place(nb, nat);
         f4 S[RT][KT];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
@@ -314,7 +302,7 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (nb < k1) load_ks(nat, nb);
+        load_ks(nat, nb);
 
         // online softmax: a lane holds keys kb + 16 kt + 4 lg + i of row i16
         bool masked = kb < lo || kb + TILE > vmin;
@@ -384,7 +372,7 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
                         acc = bt_mfma16k16(make_h4(w[0][d], w[1][d]), h4{p8[rt][0], p8[rt][1], p8[rt][2], p8[rt][3]}, acc);
                 }
         }
-        if (nb < k1) load_vs(nat, nb);
+        load_vs(nat, nb);
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) at[kt] = nat[kt];
     }
