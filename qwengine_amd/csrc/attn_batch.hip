@@ -17,6 +17,8 @@
 //    the next tile's K loads go out when the scores are done, its V loads when P V is.
 // Roundings below 32 bits: Q / 16, the dequantized K and V, and the probabilities are fp16 (2^-12 relative each, random in
 // sign, as in the prefill), the output is fp16.
+#include <type_traits>
+
 #include "attn_tiles.hpp"
 #include "batch_plan.hpp"
 #include "launch.hpp"
@@ -73,6 +75,17 @@ __device__ __forceinline__ int bt_place(const qwa_kv_pages& p, const int* __rest
     if (kb >= end) return -1;
     const int pg = table[kb >> __builtin_ctz(p.page)];
     return (unsigned)pg < (unsigned)p.n_pages ? pg * p.page + (kb & (p.page - 1)) : -1;
+}
+
+// `bytes` bytes from a wave-uniform address on, in 32-bit words; what is read past them is zero
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bt_buffer(const void* base, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00027000);
+}
+__device__ __forceinline__ uint4 bt_ld16(__amdgpu_buffer_rsrc_t b, int off) {
+    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+}
+__device__ __forceinline__ uint2 bt_ld8(__amdgpu_buffer_rsrc_t b, int off) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
 }
 
 // Q4_0 codes with fewer shifts than q4_word_to_h8 / v_pair_words (the same values in the same order): a nibble that sits at
@@ -165,22 +178,19 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
     constexpr bool SC = KVT != QWA_KV_F16;
     constexpr int KW = VB / 16, VW = VB / 64;  // words per lane of a K row and of a V row
     uint32_t kr[KT][KW], vr[4 * KT][VW], ksd[KT], vsd[KT];
-    auto buffer = [&](const void* base, int bytes) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00027000);
-    };
     auto rows_of = [&](int at, int kb) { return at < 0 ? 0 : min(max(k1 - kb, 0), 16); };
     auto load_ks = [&](const int* at, int kb) {
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) {
             const size_t pos = (size_t)__builtin_amdgcn_readfirstlane(max(at[kt], 0));
             const int n = __builtin_amdgcn_readfirstlane(rows_of(at[kt], kb + 16 * kt));
-            const auto r = buffer(kh + pos * VB, n * VB);
+            const auto r = bt_buffer(kh + pos * VB, n * VB);
 #pragma unroll
             for (int i = 0; i < KW / 4; i++) {
-                const uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, i16 * VB + 16 * lg + 64 * i, 0, 0));
+                const uint4 x = bt_ld16(r, i16 * VB + 16 * lg + 64 * i);
                 kr[kt][4 * i] = x.x; kr[kt][4 * i + 1] = x.y; kr[kt][4 * i + 2] = x.z; kr[kt][4 * i + 3] = x.w;
             }
-            if constexpr (SC) ksd[kt] = __builtin_amdgcn_raw_buffer_load_b32(buffer(ksh + pos * 8, n * 16), 4 * lane, 0, 0);
+            if constexpr (SC) ksd[kt] = __builtin_amdgcn_raw_buffer_load_b32(bt_buffer(ksh + pos * 8, n * 16), 4 * lane, 0, 0);
         }
     };
     auto load_vs = [&](const int* at, int kb) {
@@ -188,23 +198,22 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
         for (int kt = 0; kt < KT; kt++) {
             const size_t pos = (size_t)__builtin_amdgcn_readfirstlane(max(at[kt], 0));
             const int n = __builtin_amdgcn_readfirstlane(rows_of(at[kt], kb + 16 * kt));
-            const auto r = buffer(vh + pos * VB, n * VB);
+            const auto r = bt_buffer(vh + pos * VB, n * VB);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 uint32_t* const w = vr[4 * kt + j];
                 if constexpr (VW == 2) {
-                    const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, 4 * lg * VB + 8 * i16 + j * VB, 0, 0));
+                    const uint2 x = bt_ld8(r, 4 * lg * VB + 8 * i16 + j * VB);
                     w[0] = x.x; w[1] = x.y;
                 } else {
 #pragma unroll
                     for (int i = 0; i < VW / 4; i++) {
-                        const uint4 x = __builtin_bit_cast(
-                            uint4, __builtin_amdgcn_raw_buffer_load_b128(r, 4 * lg * VB + 16 * i16 + j * VB + 256 * i, 0, 0));
+                        const uint4 x = bt_ld16(r, 4 * lg * VB + 16 * i16 + j * VB + 256 * i);
                         w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
                     }
                 }
             }
-            if constexpr (SC) vsd[kt] = __builtin_amdgcn_raw_buffer_load_b32(buffer(vsh + pos * 8, n * 16), 4 * lane, 0, 0);
+            if constexpr (SC) vsd[kt] = __builtin_amdgcn_raw_buffer_load_b32(bt_buffer(vsh + pos * 8, n * 16), 4 * lane, 0, 0);
         }
     };
     // half h (0 / 1) of lane `from`'s dword x, in both halves
@@ -516,53 +525,57 @@ template <int KVT>
 struct BtRaw {
     static constexpr int VB = value_bytes(KVT);
     uint32_t w[VB / 32];  // V: 4 rows of VB / 128 words; K: VB / 32 words of one row
-    uint32_t sc[2];       // V: the rows' block scales in halves; K: the block's scale
+    uint32_t sc[4];       // V: the rows' block scales; K: the block's
 };
 
-// rows past the half's last valid one (last[h]) read that one; a half without a place (at[h] < 0) reads position 0 of the
-// pool, and its V becomes zeros: its probabilities are, and what was read need not be finite
+// V of the 16 keys at positions at[h] of the pool (h: the lane's half of the tile), `rows` of each half valid: rows past the
+// last valid one re-read that one, a half without a place (at[h] < 0, rows[h] = 16) position 0 .. 15 of the pool.  Nothing here
+// looks at what was read: that would wait for it.
 template <int KVT>
-__device__ __forceinline__ void bt_raw_load(BtRaw<KVT>& r, const qwa_kv_layer& kv, size_t head, const int* at,
-                                            const int* last, int t, bool is_v) {
-    constexpr int VB = BtRaw<KVT>::VB, NW = VB / 32;
-    const int u = t & 255, h = is_v ? (u >> 5) & 1 : u >> 7;
-    const int place = h ? at[1] : at[0], end = h ? last[1] : last[0];
-    const size_t row0 = head + max(place, 0);
-    if (is_v) {
-        const int k0 = 4 * (u >> 6), c = u & 31;
-        uint32_t s[4];
+__device__ __forceinline__ void bt_load_v(BtRaw<KVT>& r, const uint8_t* v, const uint16_t* vs, const int* at,
+                                          const int* rows, int t) {
+    constexpr int VB = BtRaw<KVT>::VB;
+    const int u = t & 255, c = u & 31, k0 = 4 * (u >> 6);
+    const bool h = (u >> 5) & 1;
+    const size_t p0 = max(at[0], 0), p1 = max(at[1], 0);
+    const uint8_t* const src = (h ? v + p1 * VB : v + p0 * VB) + (VB / 32) * c;
+    const uint16_t* const ssc = (h ? vs + p1 * 8 : vs + p0 * 8) + (c >> 2);
+    int row[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const size_t row = row0 + max(min(k0 + j, end), 0);
-            const uint8_t* src = kv.v + row * VB + (VB / 32) * c;
-            if constexpr (KVT == QWA_KV_Q4_0) {
-                r.w[j] = *reinterpret_cast<const uint32_t*>(src);
-            } else if constexpr (KVT == QWA_KV_Q8_0) {
-                const uint2 x = ld8(src);
-                r.w[2 * j] = x.x; r.w[2 * j + 1] = x.y;
-            } else {
-                const uint4 x = ld16(src);
-                r.w[4 * j] = x.x; r.w[4 * j + 1] = x.y; r.w[4 * j + 2] = x.z; r.w[4 * j + 3] = x.w;
-            }
-            s[j] = KVT == QWA_KV_F16 ? 0u : kv.vs[row * 8 + (c >> 2)];
-        }
-        r.sc[0] = s[0] | s[1] << 16;
-        r.sc[1] = s[2] | s[3] << 16;
-        if (place < 0) {
+    for (int j = 0; j < 4; j++) row[j] = k0 + j;
+    if (rows[0] < 16 || rows[1] < 16)
 #pragma unroll
-            for (int i = 0; i < NW; i++) r.w[i] = 0;
-            r.sc[0] = r.sc[1] = 0;
-        }
-    } else {
-        const size_t row = row0 + max(min((u >> 3) & 15, end), 0);
-        const uint8_t* src = kv.k + row * VB + (VB / 8) * (u & 7);
+        for (int j = 0; j < 4; j++) row[j] = min(row[j], (h ? rows[1] : rows[0]) - 1);
 #pragma unroll
-        for (int i = 0; i < NW / 4; i++) {
-            const uint4 x = ld16(src + 16 * i);
-            r.w[4 * i] = x.x; r.w[4 * i + 1] = x.y; r.w[4 * i + 2] = x.z; r.w[4 * i + 3] = x.w;
+    for (int j = 0; j < 4; j++) {
+        const uint8_t* const s = src + (uint32_t)(row[j] * VB);
+        if constexpr (KVT == QWA_KV_Q4_0) {
+            r.w[j] = *reinterpret_cast<const uint32_t*>(s);
+        } else if constexpr (KVT == QWA_KV_Q8_0) {
+            const uint2 x = ld8(s);
+            r.w[2 * j] = x.x; r.w[2 * j + 1] = x.y;
+        } else {
+            const uint4 x = ld16(s);
+            r.w[4 * j] = x.x; r.w[4 * j + 1] = x.y; r.w[4 * j + 2] = x.z; r.w[4 * j + 3] = x.w;
         }
-        r.sc[0] = KVT == QWA_KV_F16 ? 0u : kv.ks[row * 8 + (u & 7)];
+        r.sc[j] = KVT == QWA_KV_F16 ? 0u : ssc[(uint32_t)(8 * row[j])];
     }
+}
+
+// K of the wave's 16 keys at position `at` of the pool: a buffer of its valid rows, the others read as zeros
+template <int KVT>
+__device__ __forceinline__ void bt_load_k(BtRaw<KVT>& r, const uint8_t* k, const uint16_t* ks, int at, int rows, int t) {
+    constexpr int VB = BtRaw<KVT>::VB;
+    const int u = t & 255, row = (u >> 3) & 15, blk = u & 7, n = __builtin_amdgcn_readfirstlane(at < 0 ? 0 : rows);
+    const size_t pos = __builtin_amdgcn_readfirstlane(max(at, 0));
+    const auto b = bt_buffer(k + pos * VB, n * VB);
+#pragma unroll
+    for (int i = 0; i < VB / 128; i++) {
+        const uint4 x = bt_ld16(b, row * VB + (VB / 8) * blk + 16 * i);
+        r.w[4 * i] = x.x; r.w[4 * i + 1] = x.y; r.w[4 * i + 2] = x.z; r.w[4 * i + 3] = x.w;
+    }
+    if constexpr (KVT != QWA_KV_F16)
+        r.sc[0] = __builtin_amdgcn_raw_buffer_load_b16(bt_buffer(ks + pos * 8, n * 16), 16 * row + 2 * blk, 0, 0);
 }
 
 // Into the fp16 tiles, in 16-byte units so ordered that the 16 lanes that the LDS serves together (0-3, 12-15, 20-23, 24-27,
@@ -573,37 +586,44 @@ __device__ __forceinline__ void bt_raw_load(BtRaw<KVT>& r, const qwa_kv_layer& k
 //  dim 8 (slot % 32) + slot / 32, so that the writing lanes (c = slot % 32) lie side by side, too.
 // (Rows of 528 and 80 bytes instead: half of the LDS cycles were conflicts; 128 sequences over 32768 Q4_0 positions 163 us.)
 template <int KVT>
-__device__ __forceinline__ void bt_raw_store(const BtRaw<KVT>& r, _Float16* Ks, _Float16* Vt, int t, bool is_v) {
-    constexpr int VB = BtRaw<KVT>::VB;
+__device__ __forceinline__ void bt_store_v(BtRaw<KVT>& r, _Float16* Vt, int t, uint32_t dead) {
+    constexpr int VB = BtRaw<KVT>::VB, VW = VB / 128, DPW = 8 / VW;  // words of a row, dims of a word
     const int u = t & 255;
-    if (is_v) {
-        constexpr int VW = VB / 128, DPW = 8 / VW;  // words of a row, dims of a word
-        _Float16* dst = Vt + 8 * (256 * (u >> 6) + (u & 31)) + 4 * ((u >> 5) & 1);
+    // (a half without a place: its probabilities are zeros, and what was read need not be finite)
+    if (dead != 0 && ((dead >> ((u >> 5) & 1)) & 1)) {
 #pragma unroll
-        for (int i = 0; i < VW; i++) {
-            uint32_t lo[DPW], hi[DPW];
-            bt_v_pair<KVT>(r.w[i], r.w[VW + i], r.sc[0] & 0xFFFFu, r.sc[0] >> 16, lo);
-            bt_v_pair<KVT>(r.w[2 * VW + i], r.w[3 * VW + i], r.sc[1] & 0xFFFFu, r.sc[1] >> 16, hi);
+        for (int i = 0; i < VB / 32; i++) r.w[i] = 0;
 #pragma unroll
-            for (int d = 0; d < DPW; d++) *reinterpret_cast<uint2*>(dst + 8 * 32 * (DPW * i + d)) = make_uint2(lo[d], hi[d]);
+        for (int j = 0; j < 4; j++) r.sc[j] = 0;
+    }
+    _Float16* dst = Vt + 8 * (256 * (u >> 6) + (u & 31)) + 4 * ((u >> 5) & 1);
+#pragma unroll
+    for (int i = 0; i < VW; i++) {
+        uint32_t lo[DPW], hi[DPW];
+        bt_v_pair<KVT>(r.w[i], r.w[VW + i], r.sc[0], r.sc[1], lo);
+        bt_v_pair<KVT>(r.w[2 * VW + i], r.w[3 * VW + i], r.sc[2], r.sc[3], hi);
+#pragma unroll
+        for (int d = 0; d < DPW; d++) *reinterpret_cast<uint2*>(dst + 8 * 32 * (DPW * i + d)) = make_uint2(lo[d], hi[d]);
+    }
+}
+template <int KVT>
+__device__ __forceinline__ void bt_store_k(const BtRaw<KVT>& r, _Float16* Ks, int t) {
+    const int u = t & 255;
+    _Float16* dst = Ks + 8 * (32 * 4 * (u & 7) + ((u >> 3) ^ (2 * (u & 7))));
+    const h2 d = scale_pair((uint16_t)r.sc[0], (uint16_t)r.sc[0]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t o[4];
+        if constexpr (KVT == QWA_KV_F16) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[k] = r.w[4 * i + k];
+        } else if constexpr (KVT == QWA_KV_Q8_0) {
+            q8_word_to_h4(r.w[2 * i], d, o);
+            q8_word_to_h4(r.w[2 * i + 1], d, o + 2);
+        } else {
+            bt_q4_k(r.w[i], d, o);
         }
-    } else {
-        _Float16* dst = Ks + 8 * (32 * 4 * (u & 7) + ((u >> 3) ^ (2 * (u & 7))));
-        const h2 d = scale_pair((uint16_t)r.sc[0], (uint16_t)r.sc[0]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            uint32_t o[4];
-            if constexpr (KVT == QWA_KV_F16) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) o[k] = r.w[4 * i + k];
-            } else if constexpr (KVT == QWA_KV_Q8_0) {
-                q8_word_to_h4(r.w[2 * i], d, o);
-                q8_word_to_h4(r.w[2 * i + 1], d, o + 2);
-            } else {
-                bt_q4_k(r.w[i], d, o);
-            }
-            *reinterpret_cast<uint4*>(dst + 8 * 32 * i) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
+        *reinterpret_cast<uint4*>(dst + 8 * 32 * i) = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 
@@ -626,7 +646,6 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
     auto& s_vt = lds.tile.vt;
     const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const bool is_v = wave < 4, converts = wave < 8;
     // workgroups 8 apart run on one XCD: those of a (KV head, range) pair read the same tiles
     int pair = blockIdx.x / blocks, blk = blockIdx.x % blocks;
     if (NKV * ns % 8 == 0) {
@@ -644,160 +663,177 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
     const int nrows = a.n * a.nq * GRP, wrow0 = blk * BT_TROWS + 16 * wave;
     const size_t head = (size_t)g * kv.capacity;
 
-    // tile i's raw bytes; dead: two bits a tile, tile i's in bits 0, 1
-    BtRaw<KVT> raw;
+    // The pool positions of the tiles' halves, 64 tiles ahead: lane l has those of tile l.  dead: which halves of tiles i, i + 1
+    // have none, two bits a tile.
+    int ahead[2], tile = 0;
     uint32_t dead = 0;
-    int at[2] = {-1, -1};
-    auto find = [&](int i) {
-        if (i < nt) {
-            at[0] = bt_place(p, table, (tb + i) * PF_TILE, end);
-            at[1] = bt_place(p, table, (tb + i) * PF_TILE + 16, end);
-        }
+    auto place = [&](int* at) {
+        if ((tile & 63) == 0)
+#pragma unroll
+            for (int h = 0; h < 2; h++) ahead[h] = bt_place(p, table, (tb + tile + lane) * PF_TILE + 16 * h, end);
+#pragma unroll
+        for (int h = 0; h < 2; h++) at[h] = __builtin_amdgcn_readlane(ahead[h], tile & 63);
+        tile++;
     };
-    auto load = [&](int i) {
-        const int k0 = (tb + i) * PF_TILE, last[2] = {min(15, end - 1 - k0), min(15, end - 17 - k0)};
-        bt_raw_load<KVT>(raw, kv, head, at, last, t, is_v);
-    };
-    auto dead_bits = [&]() { return (uint32_t)((at[0] < 0) | (at[1] < 0) << 1); };
-    if (nt > 0) {
-        find(0);
-        dead = dead_bits();
-        if (converts) load(0);
-    }
+    const uint8_t* const kh = kv.k + head * value_bytes(KVT);
+    const uint8_t* const vh = kv.v + head * value_bytes(KVT);
+    const uint16_t* const ksh = KVT == QWA_KV_F16 ? nullptr : kv.ks + head * 8;
+    const uint16_t* const vsh = KVT == QWA_KV_F16 ? nullptr : kv.vs + head * 8;
 
-    // Q / 16 as the B operand, by way of the wave's part of the exchange: a row is read as one kilobyte (fragment by fragment,
-    // 16 rows at once, the loads took 7 us), its fp16 pieces go to unit (s, lg, row ^ (4 s + lg) % 16) and come back as the
-    // lane's fragments s
-    const int r = wrow0 + i16, tok = r / GRP;
-    const bool valid = r < nrows;
     h8 qb[8];
-    {
-        float4 x[16];
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const int rj = min(wrow0 + j, nrows - 1);
-            x[j] = *reinterpret_cast<const float4*>(a.q + ((size_t)(rj / GRP) * NH + g * GRP + rj % GRP) * HD + 4 * lane);
-        }
-        uint8_t* const area = reinterpret_cast<uint8_t*>(lds.xch[wave]);
-        const int c = lane >> 1, half = lane & 1;  // piece c = 4 s + lg, dims 4 half .. 4 half + 3 of it
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const float f = wrow0 + j < nrows ? 0.0625f : 0.0f;
-            uint32_t w0 = h2_bits(h2{(_Float16)(x[j].x * f), (_Float16)(x[j].y * f)});
-            uint32_t w1 = h2_bits(h2{(_Float16)(x[j].z * f), (_Float16)(x[j].w * f)});
-            if constexpr (KVT == QWA_KV_Q4_0) {
-                // the operand's order [0, 4, 1, 5, 2, 6, 3, 7]: the even lane makes the first two words, the odd one the rest
-                const uint32_t mine = half ? w1 : w0, other = __builtin_amdgcn_update_dpp(0, half ? w0 : w1, 0xB1, 0xF, 0xF, true);
-                const uint32_t lo = half ? other : mine, hi = half ? mine : other;  // dims k, k + 1 and k + 4, k + 5
-                w0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
-                w1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-            }
-            *reinterpret_cast<uint2*>(area + 16 * (16 * c + (j ^ (c & 15))) + 8 * half) = make_uint2(w0, w1);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int s = 0; s < 8; s++)
-            qb[s] = *reinterpret_cast<const h8*>(area + 16 * (16 * (4 * s + lg) + (i16 ^ ((4 * s + lg) & 15))));
-    }
-    const int vis = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, end) : 0;
-    int vmin = valid ? vis : 0x7fffffff;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
-    vmin = __builtin_amdgcn_readfirstlane(vmin);
-    __syncthreads();  // the fragments are in registers; the tiles lie in the same LDS
-
     f4 o[16];
     float m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int dt = 0; dt < 16; dt++) o[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    if (nt > 0) {
-        // tile 0 converted, tile 1's bytes on their way, tile 2's pages known
-        if (converts) bt_raw_store<KVT>(raw, s_k[0], s_vt[0], t, is_v);
-        if (nt > 1) {
-            find(1);
-            dead |= dead_bits() << 2;
-            if (converts) load(1);
-            find(2);
-        }
-        __syncthreads();
-        const bool rows_here = wrow0 < nrows;
-        // tile i + 1 into the other buffer (free since the last barrier), then tile i + 2's loads
-        auto convert = [&](int i) {
-            if (i + 1 < nt) bt_raw_store<KVT>(raw, s_k[(i + 1) & 1], s_vt[(i + 1) & 1], t, is_v);
-            if (i + 2 < nt) load(i + 2);
+    int vis, vmin;
+    const int r = wrow0 + i16, tok = r / GRP;
+    const bool valid = r < nrows;
+    // ROLE 0: a wave that converts V, 1: K, 2: neither.  (In one loop for all three, the registers that the roles shared made
+    // a wave wait for its loads as soon as they were sent: 128 sequences over 32768 Q4_0 positions 154 instead of 129 us.)
+    auto walk = [&](auto role) __attribute__((always_inline)) {
+        constexpr int ROLE = decltype(role)::value;
+        BtRaw<KVT> raw;
+        // looks up tile i, the next one, and sends its loads
+        auto load = [&](int i) {
+            int at[2];
+            place(at);
+            const int left = end - (tb + i) * PF_TILE;
+            const int rows[2] = {at[0] < 0 ? 16 : min(left, 16), at[1] < 0 ? 16 : min(left - 16, 16)};
+            const uint32_t bits = (uint32_t)((at[0] < 0) | (at[1] < 0) << 1);
+            if constexpr (ROLE == 0) bt_load_v<KVT>(raw, vh, vsh, at, rows, t);
+            if constexpr (ROLE == 1) bt_load_k<KVT>(raw, kh, ksh, wave < 6 ? at[0] : at[1], wave < 6 ? rows[0] : rows[1], t);
+            return bits;
         };
-        for (int i = 0; i < nt; i++) {
-            const int k0 = (tb + i) * PF_TILE;
-            const _Float16* Ks = s_k[i & 1];
-            const _Float16* Vt = s_vt[i & 1];
-            if (is_v) convert(i);
-            if (rows_here) {
-                // S^T = K Q^T: lane (row i16) gets keys k0 + 16 kt + 4 lg + j; the K fragments of a step are read while
-                // the step before multiplies
-                f4 sc[2] = {};
-                auto kfrag = [&](int s, int kt) { return lds_h8(Ks + 8 * (32 * (4 * s + lg) + 16 * kt + (i16 ^ (2 * s)))); };
-                h8 kf[BT_KD + 1][2];
+        auto store = [&](int b, uint32_t bits) {
+            if constexpr (ROLE == 0) bt_store_v<KVT>(raw, s_vt[b], t, bits);
+            if constexpr (ROLE == 1) bt_store_k<KVT>(raw, s_k[b], t);
+        };
+        if (nt > 0) dead = load(0);
+
+        // Q / 16 as the B operand, by way of the wave's part of the exchange: a row is read as one kilobyte (fragment by fragment,
+        // 16 rows at once, the loads took 7 us), its fp16 pieces go to unit (s, lg, row ^ (4 s + lg) % 16) and come back as the
+        // lane's fragments s
+        {
+            float4 x[16];
 #pragma unroll
-                for (int s = 0; s < BT_KD; s++)
-#pragma unroll
-                    for (int kt = 0; kt < 2; kt++) kf[s][kt] = kfrag(s, kt);
-#pragma unroll
-                for (int s = 0; s < 8; s++) {
-                    if (s + BT_KD < 8)
-#pragma unroll
-                        for (int kt = 0; kt < 2; kt++) kf[(s + BT_KD) % (BT_KD + 1)][kt] = kfrag(s + BT_KD, kt);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int kt = 0; kt < 2; kt++) sc[kt] = mfma16(kf[s % (BT_KD + 1)][kt], qb[s], sc[kt]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                if (k0 + PF_TILE > vmin || (dead & 3) != 0) {
-#pragma unroll
-                    for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            sc[kt][j] = k0 + 16 * kt + 4 * lg + j < vis && !((dead >> kt) & 1) ? sc[kt][j] : -INFINITY;
-                }
-                float mx = max3f(max3f(-INFINITY, sc[0][0], sc[0][1]), sc[0][2], sc[0][3]);
-                mx = rows_max(max3f(max3f(mx, sc[1][0], sc[1][1]), sc[1][2], sc[1][3]));
-                const float mn = mx > m + PF_RESCALE_T ? mx : m;
-                const float cr = mn == m ? 1.0f : fast_exp2((m - mn) * PF_LOG2E);
-                const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;
-                m = mn;
-                // the V fragments' reads begin while the exponentials are taken
-                const _Float16* vrow = Vt + 8 * (256 * lg + i16);
-                h8 vf[BT_VD];
-#pragma unroll
-                for (int dt = 0; dt < BT_VD - 1; dt++) vf[dt] = lds_h8(vrow + 8 * 16 * dt);
-                h8 pb;
-#pragma unroll
-                for (int j = 0; j < 8; j++) pb[j] = (_Float16)fast_exp2(fmaf(sc[j >> 2][j & 3], PF_LOG2E, -msl));
-                // the sum of the rounded probabilities, the weights that P V applies
-                const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
-                float rs = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) rs = __builtin_amdgcn_fdot2(h2{pb[j], pb[j + 1]}, one2, rs, false);
-                l = l * cr + rs;
-                if (__any(cr != 1.0f)) {
-#pragma unroll
-                    for (int dt = 0; dt < 16; dt++) o[dt] *= cr;
-                }
-                // O^T += V^T P^T
-#pragma unroll
-                for (int dt = 0; dt < 16; dt++) {
-                    if (dt + BT_VD - 1 < 16) vf[(dt + BT_VD - 1) % BT_VD] = lds_h8(vrow + 8 * 16 * (dt + BT_VD - 1));
-                    o[dt] = mfma16(vf[dt % BT_VD], pb, o[dt]);
-                }
+            for (int j = 0; j < 16; j++) {
+                const int rj = min(wrow0 + j, nrows - 1);
+                x[j] = *reinterpret_cast<const float4*>(a.q + ((size_t)(rj / GRP) * NH + g * GRP + rj % GRP) * HD + 4 * lane);
             }
-            if (converts && !is_v) convert(i);
-            dead >>= 2;
-            if (i + 2 < nt) dead |= dead_bits() << 2;
-            find(i + 3);
-            __syncthreads();
+            uint8_t* const area = reinterpret_cast<uint8_t*>(lds.xch[wave]);
+            const int c = lane >> 1, half = lane & 1;  // piece c = 4 s + lg, dims 4 half .. 4 half + 3 of it
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float f = wrow0 + j < nrows ? 0.0625f : 0.0f;
+                uint32_t w0 = h2_bits(h2{(_Float16)(x[j].x * f), (_Float16)(x[j].y * f)});
+                uint32_t w1 = h2_bits(h2{(_Float16)(x[j].z * f), (_Float16)(x[j].w * f)});
+                if constexpr (KVT == QWA_KV_Q4_0) {
+                    // the operand's order [0, 4, 1, 5, 2, 6, 3, 7]: the even lane makes the first two words, the odd one the rest
+                    const uint32_t mine = half ? w1 : w0;
+                    const uint32_t other = __builtin_amdgcn_update_dpp(0, half ? w0 : w1, 0xB1, 0xF, 0xF, true);
+                    const uint32_t lo = half ? other : mine, hi = half ? mine : other;  // dims k, k + 1 and k + 4, k + 5
+                    w0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+                    w1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+                }
+                *reinterpret_cast<uint2*>(area + 16 * (16 * c + (j ^ (c & 15))) + 8 * half) = make_uint2(w0, w1);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int s = 0; s < 8; s++)
+                qb[s] = *reinterpret_cast<const h8*>(area + 16 * (16 * (4 * s + lg) + (i16 ^ ((4 * s + lg) & 15))));
         }
-    }
+        vis = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, end) : 0;
+        vmin = valid ? vis : 0x7fffffff;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
+        vmin = __builtin_amdgcn_readfirstlane(vmin);
+        __syncthreads();  // the fragments are in registers; the tiles lie in the same LDS
+
+#pragma unroll
+        for (int dt = 0; dt < 16; dt++) o[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+
+        if (nt > 0) {
+            // tile 0 converted, tile 1's bytes on their way
+            store(0, dead);
+            if (nt > 1) dead |= load(1) << 2;
+            __syncthreads();
+            const bool rows_here = wrow0 < nrows;
+            // tile i + 1 into the other buffer (free since the last barrier), then tile i + 2's loads
+            auto convert = [&](int i) {
+                if (i + 1 < nt) store((i + 1) & 1, (dead >> 2) & 3);
+                if (i + 2 < nt) dead |= load(i + 2) << 4;
+            };
+            for (int i = 0; i < nt; i++) {
+                const int k0 = (tb + i) * PF_TILE;
+                const _Float16* Ks = s_k[i & 1];
+                const _Float16* Vt = s_vt[i & 1];
+                if constexpr (ROLE == 0) convert(i);
+                if (rows_here) {
+                    // S^T = K Q^T: lane (row i16) gets keys k0 + 16 kt + 4 lg + j; the K fragments of a step are read while
+                    // the step before multiplies
+                    f4 sc[2] = {};
+                    auto kfrag = [&](int s, int kt) { return lds_h8(Ks + 8 * (32 * (4 * s + lg) + 16 * kt + (i16 ^ (2 * s)))); };
+                    h8 kf[BT_KD + 1][2];
+#pragma unroll
+                    for (int s = 0; s < BT_KD; s++)
+#pragma unroll
+                        for (int kt = 0; kt < 2; kt++) kf[s][kt] = kfrag(s, kt);
+#pragma unroll
+                    for (int s = 0; s < 8; s++) {
+                        if (s + BT_KD < 8)
+#pragma unroll
+                            for (int kt = 0; kt < 2; kt++) kf[(s + BT_KD) % (BT_KD + 1)][kt] = kfrag(s + BT_KD, kt);
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int kt = 0; kt < 2; kt++) sc[kt] = mfma16(kf[s % (BT_KD + 1)][kt], qb[s], sc[kt]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (k0 + PF_TILE > vmin || (dead & 3) != 0) {
+#pragma unroll
+                        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                sc[kt][j] = k0 + 16 * kt + 4 * lg + j < vis && !((dead >> kt) & 1) ? sc[kt][j] : -INFINITY;
+                    }
+                    float mx = max3f(max3f(-INFINITY, sc[0][0], sc[0][1]), sc[0][2], sc[0][3]);
+                    mx = rows_max(max3f(max3f(mx, sc[1][0], sc[1][1]), sc[1][2], sc[1][3]));
+                    const float mn = mx > m + PF_RESCALE_T ? mx : m;
+                    const float cr = mn == m ? 1.0f : fast_exp2((m - mn) * PF_LOG2E);
+                    const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;
+                    m = mn;
+                    // the V fragments' reads begin while the exponentials are taken
+                    const _Float16* vrow = Vt + 8 * (256 * lg + i16);
+                    h8 vf[BT_VD];
+#pragma unroll
+                    for (int dt = 0; dt < BT_VD - 1; dt++) vf[dt] = lds_h8(vrow + 8 * 16 * dt);
+                    h8 pb;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) pb[j] = (_Float16)fast_exp2(fmaf(sc[j >> 2][j & 3], PF_LOG2E, -msl));
+                    // the sum of the rounded probabilities, the weights that P V applies
+                    const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
+                    float rs = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) rs = __builtin_amdgcn_fdot2(h2{pb[j], pb[j + 1]}, one2, rs, false);
+                    l = l * cr + rs;
+                    if (__any(cr != 1.0f)) {
+#pragma unroll
+                        for (int dt = 0; dt < 16; dt++) o[dt] *= cr;
+                    }
+                    // O^T += V^T P^T
+#pragma unroll
+                    for (int dt = 0; dt < 16; dt++) {
+                        if (dt + BT_VD - 1 < 16) vf[(dt + BT_VD - 1) % BT_VD] = lds_h8(vrow + 8 * 16 * (dt + BT_VD - 1));
+                        o[dt] = mfma16(vf[dt % BT_VD], pb, o[dt]);
+                    }
+                }
+                if constexpr (ROLE != 0) convert(i);
+                dead >>= 2;
+                __syncthreads();
+            }
+        }
+    };
+    if (wave < 4) walk(std::integral_constant<int, 0>{});
+    else if (wave < 8) walk(std::integral_constant<int, 1>{});
+    else walk(std::integral_constant<int, 2>{});
 
     // partial state: o[2 k + e][j] is dim 8 x + k of row i16, x = 16 e + 4 lg + j; through LDS, so that a store instruction
     // writes two whole 512-byte rows
