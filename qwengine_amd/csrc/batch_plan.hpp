@@ -47,19 +47,6 @@ inline void bt_cut(int positions, int units, int fill, int most, int* ns, int* l
     *ns = (positions + *len - 1) / *len;
 }
 
-// Key ranges of the tile workgroups, of which a CU holds one: one round of the CUs, or more ranges where they fill the rounds
-// better.  More ranges cost a partial state per row each; a range takes 2.1 us a tile and 6 us, a state 0.24 ns a row.
-// (300 sequences of 8 queries over 2000 F16 positions, 300 workgroups a range: attention 412 us in one range, 386 in three; a
-// gain below 5 % is not taken, 32 sequences over 8192 Q8_0 positions 52.6 us in 64 ranges, 53.3 in the 52 of the least sum.)
-inline int bt_ranges(int units, int tiles, long long rows) {
-    auto us = [&](int r) { return (units * r + 255) / 256 * ((tiles + r - 1) / r * 2.1 + 6.0) + r * rows * 0.24e-3; };
-    int best = std::min(tiles, std::max(1, 256 / units));
-    double least = 0.95 * us(best);
-    for (int r = 1; r <= std::min(tiles, 64); r++)
-        if (us(r) < least) best = r, least = us(r);
-    return best;
-}
-
 inline BatchPlan batch_plan(int n, int nq, int n_shared, int max_len) {
     BatchPlan p = {};
     const int rows = n * nq * GRP, own = nq * GRP;
@@ -70,7 +57,7 @@ inline BatchPlan batch_plan(int n, int nq, int n_shared, int max_len) {
     if (rows > BT_FEW && n_shared > 0) {
         const int tiles = (n_shared + PF_TILE - 1) / PF_TILE;
         p.blocks = (rows + BT_TROWS - 1) / BT_TROWS;
-        p.nt = bt_ranges(p.blocks * NKV, tiles, (long long)n * nq * NH);
+        p.nt = std::min(tiles, std::max(1, 256 / (p.blocks * NKV)));
         p.len_shared = BT_STEP;
     } else {
         bt_cut(n_shared, p.groups_shared * NKV, BT_FILL, 128, &p.ns_shared, &p.len_shared);
