@@ -488,8 +488,10 @@ k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
     }
     const int slices = min(a.wgs, total);  // (none is empty)
     if (w >= slices) return;
-    int s = (int)((long long)w * total / slices);
-    const int end = (int)((long long)(w + 1) * total / slices);
+    // (BT_FILL slices of QWA_PAGES_MAXN * MAX_POS / BT_STEP steps: the products fit 32 bits, whose divisions are much shorter)
+    static_assert((long long)BT_FILL * QWA_PAGES_MAXN * (MAX_POS / BT_STEP) < 1LL << 32, "32-bit slices");
+    int s = (int)((uint32_t)w * (uint32_t)total / (uint32_t)slices);
+    const int end = (int)((uint32_t)(w + 1) * (uint32_t)total / (uint32_t)slices);
     // the batch row that holds step s
     const int at = __builtin_ctzll(__ballot(upto > s));
     int b = at * per, first = __builtin_amdgcn_readlane(upto - mine, at);
@@ -658,7 +660,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
     const int seq = bt_seq(a, longest);
     const int* __restrict__ table = p.table + (seq >= 0 && seq < p.n_seq ? (size_t)seq * p.ld : 0);
     const int all = (a.n_shared + PF_TILE - 1) / PF_TILE;
-    const int tb = (int)((long long)sp * all / ns), te = (int)((long long)(sp + 1) * all / ns);
+    const int tb = sp * all / ns, te = (sp + 1) * all / ns;
     const int nt = min(te, (end + PF_TILE - 1) / PF_TILE) - tb;  // (a batch shorter than its shared part: fewer, or none)
     const int nrows = a.n * a.nq * GRP, wrow0 = blk * BT_TROWS + 16 * wave;
     const size_t head = (size_t)g * kv.capacity;
@@ -891,9 +893,9 @@ __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p,
     int segs = 0;
     size_t seg0 = 0;
     if (a.wgs > 0) {
-        const long long s0 = a.begin[b], s1 = a.begin[b + 1], total = a.begin[a.n];
+        const uint32_t s0 = a.begin[b], s1 = a.begin[b + 1], total = a.begin[a.n];
         if (s1 > s0) {
-            const long long slices = min((long long)a.wgs, total);
+            const uint32_t slices = min((uint32_t)a.wgs, total);
             const int w0 = (int)(((s0 + 1) * slices - 1) / total), w1 = (int)((s1 * slices - 1) / total);
             segs = w1 - w0 + 1;
             seg0 = ((size_t)(h / GRP) * (a.wgs + a.n) + w0 + b) * a.nq * GRP + (tok % a.nq) * GRP + h % GRP;
