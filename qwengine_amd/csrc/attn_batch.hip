@@ -10,11 +10,12 @@
 //    with its own running maximum, sum and O, and merge at the end through LDS.
 //  * Tile workgroups (k_bt_tiles, the shared positions of more rows) have BT_TROWS rows, 16 a wave: each tile is dequantized
 //    once into LDS, by way of registers, and every wave multiplies its rows with it.
-//  * Pages are multiples of 16 positions and tiles start at multiples of 16, so each 16 keys lie in one page: a tile's page
-//    numbers are wave-uniform scalar loads, one tile ahead.
-//  * S^T = K Q^T and O^T += V^T P^T on fp16 MFMA with fp32 accumulation.  A lane loads 64 dims of one key and 16 dims of the
-//    keys whose probabilities it holds straight into registers in operand order and dequantizes there (kv_operands.hpp);
-//    the next tile's K loads go out when the scores are done, its V loads when P V is.
+//  * Pages are multiples of 16 positions and tiles start at multiples of 16, so each 16 keys lie in one page.  A wave looks
+//    the pages of its next 64 tiles up at once, a lane a tile.
+//  * S^T = K Q^T and O^T += V^T P^T on fp16 MFMA with fp32 accumulation.  In a register workgroup a lane loads 64 dims of one
+//    key and 16 dims of the keys whose probabilities it holds straight into registers in operand order and dequantizes there
+//    (kv_operands.hpp); the next tile's K loads go out when the scores are done, its V loads when P V is.
+// A batch of one call has the same bits again; another batch, or another cut, sums a row's states in another order.
 // Roundings below 32 bits: Q / 16, the dequantized K and V, and the probabilities are fp16 (2^-12 relative each, random in
 // sign, as in the prefill), the output is fp16.
 #include <type_traits>
@@ -343,7 +344,7 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
             float rs = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                p8[rt][j] = j < 4 * KT ? (_Float16)fast_exp2(fmaf(S[rt][(j >> 2) % KT][j & 3], PF_LOG2E, -msl)) : (_Float16)0.0f;
+                p8[rt][j] = (_Float16)(j < 4 * KT ? fast_exp2(fmaf(S[rt][(j >> 2) % KT][j & 3], PF_LOG2E, -msl)) : 0.0f);
 #pragma unroll
             for (int j = 0; j < 4 * KT; j += 2) rs = __builtin_amdgcn_fdot2(h2{p8[rt][j], p8[rt][j + 1]}, one2, rs, false);
             l[rt] = l[rt] * cr[rt] + rs;
@@ -457,7 +458,12 @@ __device__ __forceinline__ int bt_steps(const BatchArgs& a, const qwa_kv_pages& 
     return m > a.n_shared ? (m - (a.n_shared & ~15) + BT_STEP - 1) / BT_STEP : 0;
 }
 
-// the own positions: workgroup = (slice of the steps, KV head, row group), one segment per sequence that the slice meets
+// the own positions: workgroup = (slice of the steps, KV head, row group), one segment per sequence that the slice meets.
+// Equal slices, since a cut by sequences leaves the chip to the longest one (24 of up to 16384 positions 108 instead of 89 us).
+// About 7 us of latency (finding the slice, page numbers, first bytes, joining the waves) around a stream of the cache's bytes:
+// 24 sequences of 267 000 Q4_0 positions together 70 us (4.4 TB/s; unpacking takes half of the issue cycles), of 131 000 Q8_0
+// ones 61 us (4.7 TB/s), F16 100 us (5.3 TB/s, where a large copy reads and writes 5.15).  Not faster: a second tile on its
+// way (registers for it are there), three waves a SIMD (spills), the next segment's first tile sent before this one's merge.
 template <int KVT, int RT>
 __global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
@@ -631,8 +637,10 @@ __device__ __forceinline__ void bt_store_k(const BtRaw<KVT>& r, _Float16* Ks, in
 
 // The shared positions for BT_TROWS rows: workgroup = (row block, tile range, KV head).  The 12 waves have 16 rows each,
 // three a SIMD: of those one converts V at the start of an iteration, one K at its end, one nothing, so the MFMAs of one run
-// while others convert, take exponentials or wait for LDS.  (32 rows a wave, two a SIMD, read half as much LDS per row, but
-// each wave's chain of LDS reads, MFMAs and softmax steps took 3.3 us a tile.)
+// while others convert, take exponentials or wait for LDS.  128 sequences over 32768 Q4_0 positions: 127 us, 0.81 PFLOP/s, 1.8
+// us a tile (large products of the library reach 1.17).  The bound is LDS: 12 waves read a tile's 32 KB each, which with the
+// writes takes four fifths of the cycles.  (32 rows a wave, two a SIMD, read half as much per row, but spill 56 registers:
+// 164 us.)
 template <int KVT>
 __global__ void __launch_bounds__(64 * BT_TWAVES) __attribute__((amdgpu_waves_per_eu(BT_TWAVES / 4, BT_TWAVES / 4)))
 k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
@@ -665,8 +673,8 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
     const int nrows = a.n * a.nq * GRP, wrow0 = blk * BT_TROWS + 16 * wave;
     const size_t head = (size_t)g * kv.capacity;
 
-    // The pool positions of the tiles' halves, 64 tiles ahead: lane l has those of tile l.  dead: which halves of tiles i, i + 1
-    // have none, two bits a tile.
+    // The pool positions of the tiles' halves, 64 tiles ahead: lane l has those of tile l.  dead: which halves of tiles i,
+    // i + 1 have none, two bits a tile.
     int ahead[2], tile = 0;
     uint32_t dead = 0;
     auto place = [&](int* at) {
@@ -710,9 +718,9 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
         };
         if (nt > 0) dead = load(0);
 
-        // Q / 16 as the B operand, by way of the wave's part of the exchange: a row is read as one kilobyte (fragment by fragment,
-        // 16 rows at once, the loads took 7 us), its fp16 pieces go to unit (s, lg, row ^ (4 s + lg) % 16) and come back as the
-        // lane's fragments s
+        // Q / 16 as the B operand, by way of the wave's part of the exchange: a row is read as one kilobyte (fragment by
+        // fragment, 16 rows at once, the loads took 7 us), its fp16 pieces go to unit (s, lg, row ^ (4 s + lg) % 16) and come
+        // back as the lane's fragments s
         {
             float4 x[16];
 #pragma unroll
@@ -728,7 +736,8 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
                 uint32_t w0 = h2_bits(h2{(_Float16)(x[j].x * f), (_Float16)(x[j].y * f)});
                 uint32_t w1 = h2_bits(h2{(_Float16)(x[j].z * f), (_Float16)(x[j].w * f)});
                 if constexpr (KVT == QWA_KV_Q4_0) {
-                    // the operand's order [0, 4, 1, 5, 2, 6, 3, 7]: the even lane makes the first two words, the odd one the rest
+                    // the operand's order [0, 4, 1, 5, 2, 6, 3, 7]: the even lane makes the first two words, the odd one the
+                    // rest
                     const uint32_t mine = half ? w1 : w0;
                     const uint32_t other = __builtin_amdgcn_update_dpp(0, half ? w0 : w1, 0xB1, 0xF, 0xF, true);
                     const uint32_t lo = half ? other : mine, hi = half ? mine : other;  // dims k, k + 1 and k + 4, k + 5
@@ -773,7 +782,9 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
                     // S^T = K Q^T: lane (row i16) gets keys k0 + 16 kt + 4 lg + j; the K fragments of a step are read while
                     // the step before multiplies
                     f4 sc[2] = {};
-                    auto kfrag = [&](int s, int kt) { return lds_h8(Ks + 8 * (32 * (4 * s + lg) + 16 * kt + (i16 ^ (2 * s)))); };
+                    auto kfrag = [&](int s, int kt) {
+                        return lds_h8(Ks + 8 * (32 * (4 * s + lg) + 16 * kt + (i16 ^ (2 * s))));
+                    };
                     h8 kf[BT_KD + 1][2];
 #pragma unroll
                     for (int s = 0; s < BT_KD; s++)
@@ -879,6 +890,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
 // Joins a row's partial states in a fixed order, gates, rounds: WPR waves per row (token * NH + head), 4 dims per lane.  The
 // weights exp(m - M) come one state a lane, 64 at a time; wave k of a row reads the states' rows k, k + WPR, ..., eight at
 // a time.
+// The states' bytes and a chain of dependent loads bound it: 768 rows of 64 fixed-point and 5 fp32 states 11.4 us (31 MB).
 template <int WPR>
 __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p, const float* __restrict__ gate, int nt,
                                                     int ns_shared, uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {
@@ -1044,8 +1056,7 @@ hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_l
     }
     const qwa_act_q8 act = oq ? *oq : qwa_act_q8{nullptr, nullptr, nullptr};
     // with many states a workgroup per row, else a wave (us, wave / workgroup: 768 rows of about 72 states 22.0 / 11.6, 840 of
-    // 66 12.7 / 8.8, 48 of 97 14.0 / 7.4; 576 of 10 5.2 / 5.5, the rows of
-    // 128 sequences of 19 states 11.0 / 19.2, 9600 of 2 11.6 / 29.2)
+    // 66 12.7 / 8.8, 48 of 97 14.0 / 7.4; 576 of 10 5.2 / 5.5, those of 128 sequences of 19 11.0 / 19.2, 9600 of 2 11.6 / 29.2)
     const int rows = n * nq * NH, states = b.nt + b.ns_shared + (b.wgs > 0 ? b.wgs / n + 1 : 0);
     if (states > 24)
         hipLaunchKernelGGL(k_bt_combine<4>, dim3(rows), dim3(256), 0, st, a, p, gate, b.nt, b.ns_shared, out16, act,

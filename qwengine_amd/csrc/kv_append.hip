@@ -411,7 +411,8 @@ __global__ void __launch_bounds__(256) k_prep_rows_al(const float* __restrict__ 
 
 // Batch form: the last nq positions of n sequences of a paged cache.  One workgroup per token (row b * nq + t at position
 // len - nq + t of sequence seqs[b]); the wave tasks are k_prep_rows_al's, the rotation's 32 cos / sin pairs are formed once
-// per token, in double (one lane per frequency), and shared through LDS.
+// per token, in double (one lane per frequency), and shared through LDS.  Bytes: 800 tokens, 88 MB, 17.9 us (4.9 TB/s; a large
+// copy reaches 5.15); a few tokens 6 us of latency.
 constexpr int PB_WAVES = 8;
 template <int KVT>
 __global__ void __launch_bounds__(64 * PB_WAVES) k_prep_batch(

@@ -71,8 +71,10 @@ __device__ __forceinline__ long long block_scan(long long v, long long* s_wave, 
 
 constexpr int PG_PT = 4;  // counts per thread and round of the searches through ref
 
-// Room, by a workgroup of T >= n threads: thread i plans request i.  Requests are served in order (an exclusive sum of the pages that they need), and of the
-// requests whose last, partly filled page is the same, the first ref - 1 move away to copies and the last may keep it.
+// Room, by a workgroup of T >= n threads: thread i plans request i.  Requests are served in order (an exclusive sum of the
+// pages that they need), and of the requests whose last, partly filled page is the same, the first ref - 1 move away to
+// copies and the last may keep it.  Latency: the tables, the counts and three barriers' round trips, 4.5 us for 3 requests, 8.8
+// for 100 of which each looks at all before it.
 template <int T>
 __global__ void __launch_bounds__(T) k_extend(qwa_kv_pages p, const int* __restrict__ seqs,
                                                  const int* __restrict__ add, int n, int* __restrict__ status,
@@ -238,7 +240,9 @@ struct PageLayers {
 
 // Carries out the moves in every layer: a unit is a move of one layer and KV head (a run of K and one of V rows, and
 // their scale rows), units are strided over the workgroups.  A move's source and target are different pages, and no page
-// is both, so the order does not matter.  REMAP: the tables follow the moves (map of the pages from n_live on).
+// is both, so the order does not matter.  Bytes: compacting 1500 Q4_0 pages of 16 layers moves 876 MB in 181 us (4.8 TB/s; a
+// large copy reaches 5.15), 100 copies of 43 F16 positions in 16 layers take 59 us (282 MB written, the one source is read
+// from the caches).  REMAP: the tables follow the moves (map of the pages from n_live on).
 template <bool REMAP>
 __global__ void __launch_bounds__(256) k_move(qwa_kv_pages p, const int* __restrict__ work, PageLayers layers,
                                               int n_layers, int vb, int sb, const int* __restrict__ map,

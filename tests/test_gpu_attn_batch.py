@@ -154,6 +154,44 @@ def test_long_contexts(gpu):
     b.check(7, 20000, what="long shared verify")
 
 
+@pytest.mark.parametrize("n, nq, shared", [(5, 1, 0), (3, 8, 0), (40, 1, 262144), (40, 1, 200000)])
+@pytest.mark.parametrize("kvt", KVTS, ids=lambda k: KV_NAMES[k])
+def test_longest_sequences(gpu, kvt, n, nq, shared):
+    """The largest context: every table entry names one of 64 pages at random, so that a key counts as often as its page is
+    named.  (V is about the same all over a page and differs between pages, or everything would average out.)"""
+    page, pages, ld = 64, 64, 4096
+    K, V = seeded_normal((pages * page, 4, 256), 31), 0.1 * seeded_normal((pages * page, 4, 256), 32)
+    V += seeded_normal((pages, 4, 256), 33).repeat_interleave(page, 0)
+    kv, pg = ops.KVLayer.allocate(kvt, pages * page), ops.KVPages.allocate(n, ld * page, pages, page)
+    ops.kv_append(K, V, 0, pages * page, kvt, kv)
+    g = torch.Generator().manual_seed(34)
+    table = torch.randint(0, pages, (n, ld), generator=g, dtype=torch.int32)
+    table[:, :shared // page] = table[:1, :shared // page]
+    lens = [ld * page - 64 * (i % 3) * (shared < ld * page) for i in range(n)]
+    pg.table.copy_(table)
+    pg.len.copy_(i32(lens))
+    q, gate = seeded_normal((n * nq, 24, 256), 35), seeded_normal((n * nq, 24, 256), 36)
+    out = torch.empty((n * nq, 24, 256), dtype=torch.float16, device="cuda")
+    work = torch.empty(ops.attn_batch_work_bytes(n, nq, shared, ld * page), dtype=torch.uint8, device="cuda")
+    ops.attn_decode_batch(q, gate, kv, kvt, pg, None, n, nq, shared, ld * page, out, work)
+    torch.cuda.synchronize()
+    b = Batch.__new__(Batch)
+    b.kvt, b.caches, b._rows = kvt, [kv], {}
+    k64, v64 = b.values(0)
+    want = torch.zeros((n * nq, 24, 256), dtype=torch.float64)
+    for t in range(n * nq):
+        m = lens[t // nq] - nq + t % nq + 1
+        row = table[t // nq].long()
+        count = torch.bincount(row[:m // page], minlength=pages).double().repeat_interleave(page)
+        if m % page:
+            count[row[m // page] * page:][:m % page] += 1
+        for h in range(4):
+            s = q[t, 6 * h:6 * h + 6].double().cpu() @ k64[h].T / 16.0
+            p = torch.exp(s - s.amax(-1, keepdim=True)) * count
+            want[t, 6 * h:6 * h + 6] = (p / p.sum(-1, keepdim=True)) @ v64[h]
+    close(out, want * torch.sigmoid(gate.double().cpu()), f"{KV_NAMES[kvt]} {n} x {nq}, {shared} shared")
+
+
 def test_empty_rows(gpu):
     """Empty and unknown sequences, and queries before the first position, give zeros; the rest is as without them."""
     b = Batch(ops.Q8_0, [0, 200, 3, 0, 70])
