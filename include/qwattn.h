@@ -185,7 +185,8 @@ typedef struct {
 #define QWA_PAGES_MAXL 32   /* layers per call */
 
 /* Bytes of the `work` buffer of the page operators on these tables (device memory, 16-byte aligned; 0: invalid tables).
- * Calls that may run at the same time need a buffer each. */
+ * Calls that may run at the same time need a buffer each, as do captured graphs whose replays may overlap.  The tables
+ * themselves are one state: calls that change them, and calls that read them, have to be ordered (one stream, or events). */
 size_t qwa_kv_pages_work_bytes(const qwa_kv_pages* p);
 
 /* Room for add[i] more positions of sequence seqs[i] (device arrays of n entries): len grows by add[i], and the pages
@@ -237,9 +238,13 @@ size_t qwa_attn_batch_work_bytes(int n, int nq, int n_shared, int max_len);
  * them as it has positions.
  * max_len >= n_shared bounds every row's len: positions from max_len on are not seen.
  * A row that sees no position (an empty or unknown sequence, a query before the first position) gets zeros; positions
- * whose page is none of the pool's are not seen.  Pool bytes past a sequence's last position are never used.  n <=
- * QWA_PAGES_MAXN; q, gate, out16, work and the pool 16-byte aligned; work of at least qwa_attn_batch_work_bytes bytes,
- * not shared with a call that may run at the same time. */
+ * whose page is none of the pool's are not seen.  Pool bytes past a sequence's last position are never used.  A K or V
+ * value that is not finite shows in the rows that see it, and may show in those that do not, but share its 32 positions
+ * with one that does: a sequence's earlier queries, and a row that ends among the shared positions.
+ * A call's result has the same bits whenever it is repeated; the order of its sums depends on the batch, so a sequence
+ * need not have the bits that it has in another batch or in qwa_attn_decode_multi.
+ * n <= QWA_PAGES_MAXN; q, gate, out16, work and the pool 16-byte aligned; work of at least qwa_attn_batch_work_bytes
+ * bytes, not shared with a call that may run at the same time (nor by two captured graphs whose replays may overlap). */
 int qwa_attn_decode_batch(const float* q, const float* gate, const qwa_kv_layer* kv, int kvt, const qwa_kv_pages* p,
                           const int* seqs, int n, int nq, int n_shared, int max_len, uint16_t* out16,
                           const qwa_act_q8* oq, void* work, size_t work_bytes, void* stream);
