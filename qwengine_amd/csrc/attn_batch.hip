@@ -223,14 +223,12 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
         return bits_h2(__builtin_amdgcn_perm(u, u, h ? 0x03020302u : 0x01000100u));
     };
 
-    int kb = __builtin_amdgcn_readfirstlane(k0) + TILE * wave;
-    int at[KT];
-    place(kb, at);
-    load_ks(at, kb);
-    load_vs(at, kb);
-    // rows of this lane: Q / 16 as the B operand in the K operand's dim order, keys below vis are seen
+    // rows of this lane: keys below vis are seen; Q / 16 as the B operand in the K operand's dim order, of which a wave makes
+    // steps 2 * wave and 2 * wave + 1.  (What is read here is on its way while the pages are looked up, and is converted while
+    // the first tile is on its way.)
     constexpr int E = 4096 / VB;  // values of a 16-byte piece of a row
     int vis[RT], vmin = k1;
+    float4 qx[RT][2][2];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const int r = row0 + 16 * rt + i16, tok = r / GRP;
@@ -239,16 +237,29 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
         if (valid) vmin = min(vmin, vis[rt]);
         const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + E * lg;
 #pragma unroll
-        for (int s = 0; s < 8; s++) {
-            if (s / 2 != wave) continue;  // (the waves' share)
-            const float* src = qrow + 4 * E * (8 * s / E) + 8 * s % E;
-            const float4 x0 = *reinterpret_cast<const float4*>(src);
-            const float4 x1 = *reinterpret_cast<const float4*>(src + 4);
+        for (int i = 0; i < 2; i++) {
+            const int d = 8 * (2 * wave + i);
+            const float* src = qrow + 4 * E * (d / E) + d % E;
+            qx[rt][i][0] = *reinterpret_cast<const float4*>(src);
+            qx[rt][i][1] = *reinterpret_cast<const float4*>(src + 4);
+        }
+    }
+    int kb = __builtin_amdgcn_readfirstlane(k0) + TILE * wave;
+    int at[KT];
+    place(kb, at);
+    load_ks(at, kb);
+    load_vs(at, kb);
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const bool valid = row0 + 16 * rt + i16 < rows;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float4 x0 = qx[rt][i][0], x1 = qx[rt][i][1];
             const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
             h8 v;
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
-            lds.q[rt][s][lane] = v;
+            lds.q[rt][2 * wave + i][lane] = v;
         }
     }
     __syncthreads();
@@ -693,9 +704,13 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
     h8 qb[8];
     f4 o[16];
     float m = -INFINITY, l = 0.0f;
-    int vis, vmin;
     const int r = wrow0 + i16, tok = r / GRP;
     const bool valid = r < nrows;
+    const int vis = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, end) : 0;
+    int vmin = valid ? vis : 0x7fffffff;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
+    vmin = __builtin_amdgcn_readfirstlane(vmin);
     // ROLE 0: a wave that converts V, 1: K, 2: neither.  (In one loop for all three, the registers that the roles shared made
     // a wave wait for its loads as soon as they were sent: 128 sequences over 32768 Q4_0 positions 154 instead of 129 us.)
     auto walk = [&](auto role) __attribute__((always_inline)) {
@@ -752,11 +767,6 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
             for (int s = 0; s < 8; s++)
                 qb[s] = *reinterpret_cast<const h8*>(area + 16 * (16 * (4 * s + lg) + (i16 ^ ((4 * s + lg) & 15))));
         }
-        vis = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, end) : 0;
-        vmin = valid ? vis : 0x7fffffff;
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
-        vmin = __builtin_amdgcn_readfirstlane(vmin);
         __syncthreads();  // the fragments are in registers; the tiles lie in the same LDS
 
 #pragma unroll
