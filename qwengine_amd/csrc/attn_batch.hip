@@ -905,7 +905,7 @@ template <int WPR>
 __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p, const float* __restrict__ gate, int nt,
                                                     int ns_shared, uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {
     __shared__ float4 s_o[WPR > 1 ? 4 : 1][64];
-    const int wave = threadIdx.x >> 6, part = wave % WPR, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), part = wave % WPR, lane = threadIdx.x & 63;
     const int row = blockIdx.x * (4 / WPR) + wave / WPR;
     const int nrows = a.n * a.nq * NH;
     if (row >= nrows) return;  // (all waves of a row, and with WPR = 4 of a workgroup)
@@ -931,8 +931,15 @@ __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p,
         for (int s0 = 0; s0 < count; s0 += 64) {
             const int most = min(64, count - s0);
             float4 x[U];
+            // (with few states only those: a load of one again costs as much as the first; 57600 rows of 4 states 73 -> 54 us)
+            if (most > 4 * WPR) {
 #pragma unroll
-            for (int u = 0; u < U; u++) x[u] = x_of(s0 + min(part + u * WPR, most - 1));
+                for (int u = 0; u < U; u++) x[u] = x_of(s0 + min(part + u * WPR, most - 1));
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (part + u * WPR < most) x[u] = x_of(s0 + part + u * WPR);
+            }
             const float4 ml = lane < most ? ml_of(s0 + lane) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
             const float Mn = fmaxf(M, wave_max(ml.x));
             const float c = M == Mn ? 1.0f : fast_exp2((M - Mn) * PF_LOG2E);
