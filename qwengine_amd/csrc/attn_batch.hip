@@ -471,8 +471,8 @@ __device__ __forceinline__ int bt_steps(const BatchArgs& a, const qwa_kv_pages& 
 
 // the own positions: workgroup = (slice of the steps, KV head, row group), one segment per sequence that the slice meets.
 // Equal slices, since a cut by sequences leaves the chip to the longest one (24 of up to 16384 positions 108 instead of 89 us).
-// About 7 us of latency (finding the slice, page numbers, first bytes, joining the waves) around a stream of the cache's bytes:
-// 24 sequences of 267 000 Q4_0 positions together 70 us (4.4 TB/s; unpacking takes half of the issue cycles), of 131 000 Q8_0
+// About 6 us of latency (finding the slice, page numbers, first bytes, joining the waves) around a stream of the cache's bytes:
+// 24 sequences of 267 000 Q4_0 positions together 67 us (4.6 TB/s; unpacking takes half of the issue cycles), of 131 000 Q8_0
 // ones 61 us (4.7 TB/s), F16 100 us (5.3 TB/s, where a large copy reads and writes 5.15).  Not faster: a second tile on its
 // way (registers for it are there), three waves a SIMD (spills), the next segment's first tile sent before this one's merge.
 template <int KVT, int RT>
@@ -900,7 +900,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
 // Joins a row's partial states in a fixed order, gates, rounds: WPR waves per row (token * NH + head), 4 dims per lane.  The
 // weights exp(m - M) come one state a lane, 64 at a time; wave k of a row reads the states' rows k, k + WPR, ..., eight at
 // a time.
-// The states' bytes and a chain of dependent loads bound it: 768 rows of 64 fixed-point and 5 fp32 states 11.4 us (31 MB).
+// The states' bytes and a chain of dependent loads bound it: 768 rows of 64 fixed-point and 5 fp32 states 10.6 us (31 MB).
 template <int WPR>
 __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p, const float* __restrict__ gate, int nt,
                                                     int ns_shared, uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {
