@@ -12,13 +12,22 @@
 
 namespace qwa {
 
-constexpr int BT_WAVES = 4;   // waves of a register workgroup; they take the tiles of its key range in turn
-constexpr int BT_MAXRT = 2;   // 16-row MFMA tiles of such a workgroup at most
-constexpr int BT_FILL = 512;  // register workgroups that the chip holds, two a CU
-constexpr int BT_TWAVES = 12;                // waves of a tile workgroup
+constexpr int BT_WAVES = 4;               // waves of a register workgroup; they take the tiles of its key range in turn
+constexpr int BT_MAXRT = 2;               // 16-row MFMA tiles of such a workgroup at most
+constexpr int BT_TWAVES = 12;             // waves of a tile workgroup
 constexpr int BT_TROWS = 16 * BT_TWAVES;  // its rows
-constexpr int BT_STEP = 128;  // positions of a step; key ranges are whole steps
-constexpr int BT_FEW = 32;    // rows of a KV head up to which the shared positions are left to register workgroups
+// Register workgroups that the chip holds, two a CU (own positions of 24 sequences of up to 16384 Q4_0 positions 68 us, with
+// 1024 in two rounds 72).
+constexpr int BT_FILL = 512;
+// Positions of a step; key ranges are whole steps.  A tile for each wave (own positions, steps of 64 / 128 / 256, us: 32
+// sequences of 700 Q8_0 positions 17.9 / 15.6 / 16.7, 5 x 7 queries of 513 F16 15.2 / 11.9 / 13.4, 5 of 5000 Q4_0 17.2 / 15.2 /
+// 14.3).
+constexpr int BT_STEP = 128;
+// Rows of a KV head up to which the shared positions are left to register workgroups: one pass of them.  Register / tile
+// workgroups and the combine, us, 32768 shared positions: 18 rows Q4_0 29.3 / 35.5, Q8_0 30.4 / 34.8, F16 36.9 / 35.8; 30 rows
+// 32.6 / 35.0, 34.2 / 34.9, 41.3 / 36.5; 36 rows Q4_0 35.4 / 37.1, Q8_0 37.8 / 35.8; 60 rows Q4_0 38.5 / 37.7; 30 rows over 4096
+// Q8_0 positions 18.1 / 20.0.
+constexpr int BT_FEW = 32;
 
 // The shared positions [0, n_shared) are worked on for all rows together, the positions of its own [n_shared, len) for every
 // sequence by itself.
