@@ -202,7 +202,7 @@ int qwa_kv_pages_extend(const qwa_kv_pages* p, const int* seqs, const int* add, 
 /* Sequence dst[i] becomes a fork of sequence src[i], all at once (every request sees the tables as they were before the
  * call, so beams may be permuted): it gives back its own pages and holds src[i]'s, which are shared, not copied.
  * src[i] < 0 leaves dst[i] empty.  A request whose src or dst is no sequence is ignored; of several with the same dst
- * the last one counts. */
+ * the last one counts.  n <= n_seq. */
 int qwa_kv_pages_fork(const qwa_kv_pages* p, const int* src, const int* dst, int n, void* work, void* stream);
 
 /* Sequence seqs[i] keeps its first lens[i] positions (lens NULL: none, which frees it) and gives back the pages past

@@ -509,6 +509,29 @@ def test_decode_loop_of_forked_samples(gpu, kvt):
     assert pages.len.tolist() == [prompt + steps] * n + [0]
 
 
+@pytest.mark.parametrize("n, nq, shared", [(1, 1, 0), (3, 1, 128), (5, 1, 128), (9, 2, 128), (7, 8, 100), (33, 1, 130)])
+@pytest.mark.parametrize("kvt", KVTS, ids=lambda k: KV_NAMES[k])
+def test_nothing_past_the_ends(gpu, kvt, n, nq, shared):
+    """Output rows behind the batch, bytes behind the workspace's size and the pool stay as they were."""
+    b = Batch(kvt, [shared + 10 + 31 * (i % 7) for i in range(n)], shared=shared)
+    most = max(b.lens)
+    need = ops.attn_batch_work_bytes(n, nq, shared, most)
+    work = torch.full((need + 4096,), 0xAB, dtype=torch.uint8, device="cuda")
+    out = torch.full((n * nq + 5, 24, 256), 7.0, dtype=torch.float16, device="cuda")
+    oq = ops.ActQ8(torch.full(((n * nq + 5) * 6144,), 99, dtype=torch.int8, device="cuda"),
+                   *(torch.full(((n * nq + 5) * 192,), 55.0, device="cuda") for _ in range(2)))
+    pool = [t for t in (b.kv.k, b.kv.v, b.kv.ks, b.kv.vs) if t is not None]
+    before = [t.clone() for t in pool]
+    q, gate = seeded_normal((n * nq, 24, 256), 3), seeded_normal((n * nq, 24, 256), 4)
+    ops.attn_decode_batch(q, gate, b.kv, kvt, b.pages, None, n, nq, shared, most, out, work, oq)
+    torch.cuda.synchronize()
+    assert (work[need:] == 0xAB).all() and (out[n * nq:] == 7.0).all()
+    assert (oq.q[n * nq * 6144:] == 99).all() and (oq.d[n * nq * 192:] == 55).all() and (oq.s[n * nq * 192:] == 55).all()
+    assert all(torch.equal(x, y) for x, y in zip(pool, before))
+    want = batch_attention(q, gate, lambda t: b.values(t // nq), [b.lens[t // nq] - nq + t % nq + 1 for t in range(n * nq)])
+    close(out[:n * nq], want, "the rows themselves")
+
+
 def test_other_streams_and_work_on_them(gpu):
     """A call on a stream of its own, ordered by events, while another runs on the default stream with another work
     buffer."""

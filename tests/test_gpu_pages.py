@@ -237,3 +237,23 @@ def test_captured_step_follows_the_tables(gpu):
         b.same()
         assert int(b.n_live) == n and int(b.status) == 0
         b.extend([0], [9])                             # the program's own work between the replays
+
+
+def test_nothing_past_the_work_buffer(gpu):
+    """The operators write no byte behind kv_pages_work_bytes, at their largest number of requests and moves."""
+    n, page = 1024, 16
+    pages = ops.KVPages.allocate(n, 3 * page, 3 * n, page)
+    layers = pools(ops.Q4_0, 3 * n * page, 1, 3)
+    need = ops.kv_pages_work_bytes(pages)
+    work = torch.full((need + 4096,), 0xAB, dtype=torch.uint8, device="cuda")
+    status, n_live = i32([9]), i32([0])
+    seqs = torch.arange(n, dtype=torch.int32, device="cuda")
+    pages.table[0, 0], pages.len[0], pages.ref[0] = 0, 5, 1
+    ops.kv_pages_fork(pages, torch.zeros_like(seqs), seqs, work)          # everyone shares page 0 ...
+    ops.kv_pages_extend(pages, seqs, torch.full_like(seqs, 20), layers, ops.Q4_0, status, work)  # ... and leaves it
+    torch.cuda.synchronize()
+    assert int(status) == 0 and pages.len.tolist() == [25] * n and int((pages.ref > 0).sum()) == 2 * n
+    ops.kv_pages_trim(pages, seqs[: n // 2].contiguous())
+    ops.kv_pages_compact(pages, layers, ops.Q4_0, n_live, work)
+    torch.cuda.synchronize()
+    assert int(n_live) == n and int(pages.table.max()) == n - 1 and (work[need:] == 0xAB).all()
