@@ -55,13 +55,28 @@ __device__ __forceinline__ int bt_len(const BatchArgs& a, const qwa_kv_pages& p,
     const int s = bt_seq(a, b);
     return s >= 0 && s < p.n_seq ? min(max(p.len[s], 0), a.max_len) : 0;
 }
+// the same of rows b, b + step, ..., 0 past the batch; N loads on their way at once
+template <int N>
+__device__ __forceinline__ void bt_lens(const BatchArgs& a, const qwa_kv_pages& p, int b, int step, int* len) {
+    int s[N], m[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) s[j] = bt_seq(a, min(b + step * j, a.n - 1));
+#pragma unroll
+    for (int j = 0; j < N; j++) m[j] = p.len[min(max(s[j], 0), p.n_seq - 1)];
+#pragma unroll
+    for (int j = 0; j < N; j++) len[j] = b + step * j < a.n && s[j] >= 0 && s[j] < p.n_seq ? min(max(m[j], 0), a.max_len) : 0;
+}
+constexpr int BT_LENS = 4;
 
 // the longest batch row, the first of those (wave-uniform)
 __device__ __forceinline__ int bt_longest(const BatchArgs& a, const qwa_kv_pages& p, int lane) {
     int m = -1, b = 0;
-    for (int j = lane; j < a.n; j += 64) {
-        const int x = bt_len(a, p, j);
-        if (x > m) m = x, b = j;
+    for (int j0 = lane; j0 < a.n; j0 += 64 * BT_LENS) {
+        int x[BT_LENS];
+        bt_lens<BT_LENS>(a, p, j0, 64, x);
+#pragma unroll
+        for (int k = 0; k < BT_LENS; k++)
+            if (x[k] > m && j0 + 64 * k < a.n) m = x[k], b = j0 + 64 * k;
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -464,8 +479,7 @@ k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len, int g
 }
 
 // steps of batch row b's own positions (they begin at the multiple of 16 at or before n_shared)
-__device__ __forceinline__ int bt_steps(const BatchArgs& a, const qwa_kv_pages& p, int b) {
-    const int m = bt_len(a, p, b);
+__device__ __forceinline__ int bt_steps_of(const BatchArgs& a, int m) {
     return m > a.n_shared ? (m - (a.n_shared & ~15) + BT_STEP - 1) / BT_STEP : 0;
 }
 
@@ -485,22 +499,35 @@ k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
     if (w >= a.wgs) return;
     // where the batch rows begin: every wave sums the steps of n / 64 rows a lane
     const int per = (a.n + 63) / 64;
-    int mine = 0;
-    for (int j = 0; j < per; j++) mine += lane * per + j < a.n ? bt_steps(a, p, lane * per + j) : 0;
-    int upto = mine;
+    auto scan = [&](int x) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += y;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o, 64);
+            if (lane >= o) x += y;
+        }
+        return x;
+    };
+    int mine = 0;
+    for (int j0 = 0; j0 < per; j0 += BT_LENS) {
+        int m[BT_LENS];
+        bt_lens<BT_LENS>(a, p, lane * per + j0, 1, m);
+#pragma unroll
+        for (int k = 0; k < BT_LENS; k++) mine += j0 + k < per ? bt_steps_of(a, m[k]) : 0;
     }
+    const int upto = scan(mine);
     const int total = __builtin_amdgcn_readlane(upto, 63);
     if (blockIdx.x == 0 && threadIdx.x < 64) {
         int s = upto - mine;
-        for (int j = 0; j < per; j++)
-            if (lane * per + j < a.n) {
-                a.begin[lane * per + j] = s;
-                s += bt_steps(a, p, lane * per + j);
-            }
+        for (int j0 = 0; j0 < per; j0 += BT_LENS) {
+            int m[BT_LENS];
+            bt_lens<BT_LENS>(a, p, lane * per + j0, 1, m);
+#pragma unroll
+            for (int k = 0; k < BT_LENS; k++)
+                if (j0 + k < per && lane * per + j0 + k < a.n) {
+                    a.begin[lane * per + j0 + k] = s;
+                    s += bt_steps_of(a, m[k]);
+                }
+        }
         if (lane == 0) a.begin[a.n] = total;
     }
     const int slices = min(a.wgs, total);  // (none is empty)
@@ -509,13 +536,17 @@ k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
     static_assert((long long)BT_FILL * QWA_PAGES_MAXN * (MAX_POS / BT_STEP) < 1LL << 32, "32-bit slices");
     int s = (int)((uint32_t)w * (uint32_t)total / (uint32_t)slices);
     const int end = (int)((uint32_t)(w + 1) * (uint32_t)total / (uint32_t)slices);
-    // the batch row that holds step s
+    // the batch row that holds step s: the lane whose rows do, then one of those, a lane each
     const int at = __builtin_ctzll(__ballot(upto > s));
-    int b = at * per, first = __builtin_amdgcn_readlane(upto - mine, at);
-    int m = bt_steps(a, p, b);
-    while (s >= first + m) {
-        first += m;
-        m = bt_steps(a, p, ++b);
+    int b = at, first = __builtin_amdgcn_readlane(upto - mine, at), m = __builtin_amdgcn_readlane(mine, at);
+    if (per > 1) {
+        int x;
+        bt_lens<1>(a, p, at * per + lane, 1, &x);
+        x = lane < per ? bt_steps_of(a, x) : 0;
+        const int within = scan(x), row = __builtin_ctzll(__ballot(first + within > s));
+        b = at * per + row;
+        first += __builtin_amdgcn_readlane(within - x, row);
+        m = __builtin_amdgcn_readlane(x, row);
     }
     const int base = a.n_shared & ~15;
     while (true) {
@@ -531,7 +562,7 @@ k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
         if (s >= end) break;
         do {
             first += m;
-            m = bt_steps(a, p, ++b);
+            m = bt_steps_of(a, bt_len(a, p, ++b));
         } while (m == 0);
         __syncthreads();  // the last segment's states are read out of LDS
     }
