@@ -155,15 +155,21 @@ struct BtLds {
     float ml[BT_WAVES][2][64];
 };
 
-// One key range of a workgroup: rows [row0, rows) of KV head g (row 6 * token + head of the group), keys [k0, k1) of the
+// One key range of a workgroup: rows [row0, rows) of the KV head (row 6 * token + head of the group), keys [k0, k1) of the
 // sequence whose table row is `table`, positions below lo excluded; the partial state of a row goes to po, pml at rstep *
 // token + head.
-template <int KVT, int RT>
+struct BtSegment {
+    const int* table;
+    int row0, rows, k0, k1, lo;
+    float* po;
+    float2* pml;
+    int rstep;
+};
+
+// The segments of a workgroup, one after the other: `next` says whether there is another one, and which.
+template <int KVT, int RT, class NEXT>
 __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a, const qwa_kv_layer& kv,
-                                        const qwa_kv_pages& p, const int* __restrict__ table, int row0, int rows, int g,
-                                        int k0, int k1_, int lo, float* __restrict__ po, float2* __restrict__ pml,
-                                        int rstep) {
-    const int k1 = __builtin_amdgcn_readfirstlane(k1_);
+                                        const qwa_kv_pages& p, int g, BtSegment seg, NEXT next) {
     auto& s_o = lds.o;
     auto& s_ml = lds.ml;
     constexpr int KT = BtCfg<KVT, RT>::KT, VB = value_bytes(KVT), TILE = 16 * KT;
@@ -177,11 +183,11 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
     // The pool positions of the wave's tiles, 64 tiles ahead: lane l has those of tile l.  (Looked up a tile at a time they
     // were a memory round trip each, and a wait for all loads on their way.)
     constexpr int STRIDE = TILE * BT_WAVES;
-    int ahead[KT], tile = 0;
+    int ahead[KT], tile, kb, k1;
     auto place = [&](int kb, int* at) {
         if ((tile & 63) == 0)
 #pragma unroll
-            for (int kt = 0; kt < KT; kt++) ahead[kt] = bt_place(p, table, kb + STRIDE * lane + 16 * kt, k1);
+            for (int kt = 0; kt < KT; kt++) ahead[kt] = bt_place(p, seg.table, kb + STRIDE * lane + 16 * kt, k1);
 #pragma unroll
         for (int kt = 0; kt < KT; kt++) at[kt] = __builtin_amdgcn_readlane(ahead[kt], tile & 63);
         tile++;
@@ -239,224 +245,239 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
     };
 
     // rows of this lane: keys below vis are seen; Q / 16 as the B operand in the K operand's dim order, of which a wave makes
-    // steps 2 * wave and 2 * wave + 1.  (What is read here is on its way while the pages are looked up, and is converted while
-    // the first tile is on its way.)
+    // steps 2 * wave and 2 * wave + 1
     constexpr int E = 4096 / VB;  // values of a 16-byte piece of a row
-    int vis[RT], vmin = k1;
+    int vis[RT], vmin, at[KT];
     float4 qx[RT][2][2];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const int r = row0 + 16 * rt + i16, tok = r / GRP;
-        const bool valid = r < rows;
-        vis[rt] = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, k1) : 0;
-        if (valid) vmin = min(vmin, vis[rt]);
-        const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + E * lg;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int d = 8 * (2 * wave + i);
-            const float* src = qrow + 4 * E * (d / E) + d % E;
-            qx[rt][i][0] = *reinterpret_cast<const float4*>(src);
-            qx[rt][i][1] = *reinterpret_cast<const float4*>(src + 4);
-        }
-    }
-    int kb = __builtin_amdgcn_readfirstlane(k0) + TILE * wave;
-    int at[KT];
-    place(kb, at);
-    load_ks(at, kb);
-    load_vs(at, kb);
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const bool valid = row0 + 16 * rt + i16 < rows;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const float4 x0 = qx[rt][i][0], x1 = qx[rt][i][1];
-            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-            h8 v;
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
-            lds.q[rt][2 * wave + i][lane] = v;
-        }
-    }
-    __syncthreads();
-    // (uniform: the least over the 16 lanes that hold different rows)
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
-    vmin = __builtin_amdgcn_readfirstlane(vmin);
-
-    f4 o[RT][16];
-    float m[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        m[rt] = -INFINITY;
-        l[rt] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    for (; kb < k1; kb += STRIDE) {
-        const int nb = kb + STRIDE;
-        int nat[KT];
-        place(nb, nat);
-        f4 S[RT][KT];
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-            for (int kt = 0; kt < KT; kt++) S[rt][kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        // a lane's block scales of key i16: piece 4 i + lg of 32 values (Q4_0: block 4 i + lg), or 16 (Q8_0: 2 i + lg / 2)
-        constexpr int NS = KVT == QWA_KV_Q4_0 ? 2 : 4;
-        h2 kd[KT][NS];
-        if constexpr (SC) {
-#pragma unroll
-            for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-                for (int i = 0; i < NS; i++)
-                    kd[kt][i] = KVT == QWA_KV_Q4_0 ? scale_of(ksd[kt], 4 * i16 + 2 * i + (lg >> 1), lg & 1)
-                                                   : scale_of(ksd[kt], 4 * i16 + i, lg >> 1);
-        }
-#pragma unroll
-        for (int s = 0; s < 8; s++) {
-            h8 ka[KT];
-#pragma unroll
-            for (int kt = 0; kt < KT; kt++) {
-                uint32_t w[4];
-                if constexpr (KVT == QWA_KV_F16) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = kr[kt][4 * s + i];
-                } else if constexpr (KVT == QWA_KV_Q8_0) {
-                    q8_word_to_h4(kr[kt][2 * s], kd[kt][s / 2], w);
-                    q8_word_to_h4(kr[kt][2 * s + 1], kd[kt][s / 2], w + 2);
-                } else {
-                    bt_q4_k(kr[kt][s], kd[kt][s / 4], w);
-                }
-                ka[kt] = make_h8(w[0], w[1], w[2], w[3]);
-            }
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                const h8 b = lds.q[rt][s][lane];
-#pragma unroll
-                for (int kt = 0; kt < KT; kt++) S[rt][kt] = mfma16(ka[kt], b, S[rt][kt]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        load_ks(nat, nb);
-
-        // online softmax: a lane holds keys kb + 16 kt + 4 lg + i of row i16
-        bool masked = kb < lo || kb + TILE > vmin;
-#pragma unroll
-        for (int kt = 0; kt < KT; kt++) masked |= at[kt] < 0;
-        h8 p8[RT];
-        float cr[RT];
-        bool moved = false;
+    // A segment's first loads: what is read of Q and the lengths is on its way while the pages are looked up.
+    auto begin = [&]() {
+        k1 = __builtin_amdgcn_readfirstlane(seg.k1);
+        kb = __builtin_amdgcn_readfirstlane(seg.k0) + TILE * wave;
+        vmin = k1;
+        tile = 0;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            if (masked) {
+            const int r = seg.row0 + 16 * rt + i16, tok = r / GRP;
+            const bool valid = r < seg.rows;
+            vis[rt] = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, k1) : 0;
+            if (valid) vmin = min(vmin, vis[rt]);
+            const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + E * lg;
 #pragma unroll
-                for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int key = kb + 16 * kt + 4 * lg + i;
-                        S[rt][kt][i] = at[kt] >= 0 && key >= lo && key < vis[rt] ? S[rt][kt][i] : -INFINITY;
-                    }
+            for (int i = 0; i < 2; i++) {
+                const int d = 8 * (2 * wave + i);
+                const float* src = qrow + 4 * E * (d / E) + d % E;
+                qx[rt][i][0] = *reinterpret_cast<const float4*>(src);
+                qx[rt][i][1] = *reinterpret_cast<const float4*>(src + 4);
             }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int kt = 0; kt < KT; kt++) mx = max3f(max3f(mx, S[rt][kt][0], S[rt][kt][1]), S[rt][kt][2], S[rt][kt][3]);
-            mx = rows_max(mx);
-            const float mn = mx > m[rt] + PF_RESCALE_T ? mx : m[rt];
-            const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;  // a row that saw nothing keeps l = 0, O = 0
-            cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] * PF_LOG2E - msl);
-            // the sum is that of the rounded probabilities, the weights that P V applies
-            const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
-            float rs = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                p8[rt][j] = (_Float16)(j < 4 * KT ? fast_exp2(fmaf(S[rt][(j >> 2) % KT][j & 3], PF_LOG2E, -msl)) : 0.0f);
-#pragma unroll
-            for (int j = 0; j < 4 * KT; j += 2) rs = __builtin_amdgcn_fdot2(h2{p8[rt][j], p8[rt][j + 1]}, one2, rs, false);
-            l[rt] = l[rt] * cr[rt] + rs;
-            m[rt] = mn;
-            moved |= cr[rt] != 1.0f;
         }
-        if (__any(moved)) {
+        place(kb, at);
+        load_ks(at, kb);
+        load_vs(at, kb);
+    };
+    begin();
+    while (true) {
+        // (converted while the first tile is on its way)
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const bool valid = seg.row0 + 16 * rt + i16 < seg.rows;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float4 x0 = qx[rt][i][0], x1 = qx[rt][i][1];
+                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                h8 v;
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
+                lds.q[rt][2 * wave + i][lane] = v;
+            }
+        }
+        __syncthreads();
+        // (uniform: the least over the 16 lanes that hold different rows)
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
+        vmin = __builtin_amdgcn_readfirstlane(vmin);
+
+        f4 o[RT][16];
+        float m[RT], l[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            m[rt] = -INFINITY;
+            l[rt] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        for (; kb < k1; kb += STRIDE) {
+            const int nb = kb + STRIDE;
+            int nat[KT];
+            place(nb, nat);
+            f4 S[RT][KT];
 #pragma unroll
             for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-                for (int dt = 0; dt < 16; dt++) o[rt][dt] *= cr[rt];
-        }
-
-        // O^T += V^T P^T: output tile dt holds the lane's dim dt
-        uint32_t vd[4 * KT];
+                for (int kt = 0; kt < KT; kt++) S[rt][kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            // a lane's block scales of key i16: piece 4 i + lg of 32 values (Q4_0: block 4 i + lg), or 16 (Q8_0: 2 i + lg / 2)
+            constexpr int NS = KVT == QWA_KV_Q4_0 ? 2 : 4;
+            h2 kd[KT][NS];
+            if constexpr (SC) {
 #pragma unroll
-        for (int j = 0; j < 4 * KT; j++)
-            vd[j] = SC ? h2_bits(scale_of(vsd[j / 4], 4 * (4 * lg + j % 4) + (i16 >> 2), (i16 >> 1) & 1)) & 0xFFFFu : 0u;
-        constexpr int DPW = 16 / VW;
+                for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-        for (int wi = 0; wi < VW; wi++) {
-            __builtin_amdgcn_sched_barrier(0);
-            uint32_t w[2 * KT][DPW];
+                    for (int i = 0; i < NS; i++)
+                        kd[kt][i] = KVT == QWA_KV_Q4_0 ? scale_of(ksd[kt], 4 * i16 + 2 * i + (lg >> 1), lg & 1)
+                                                       : scale_of(ksd[kt], 4 * i16 + i, lg >> 1);
+            }
 #pragma unroll
-            for (int h = 0; h < 2 * KT; h++)
-                bt_v_pair<KVT>(vr[2 * h][wi], vr[2 * h + 1][wi], vd[2 * h], vd[2 * h + 1], w[h]);
+            for (int s = 0; s < 8; s++) {
+                h8 ka[KT];
 #pragma unroll
-            for (int d = 0; d < DPW; d++)
+                for (int kt = 0; kt < KT; kt++) {
+                    uint32_t w[4];
+                    if constexpr (KVT == QWA_KV_F16) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) w[i] = kr[kt][4 * s + i];
+                    } else if constexpr (KVT == QWA_KV_Q8_0) {
+                        q8_word_to_h4(kr[kt][2 * s], kd[kt][s / 2], w);
+                        q8_word_to_h4(kr[kt][2 * s + 1], kd[kt][s / 2], w + 2);
+                    } else {
+                        bt_q4_k(kr[kt][s], kd[kt][s / 4], w);
+                    }
+                    ka[kt] = make_h8(w[0], w[1], w[2], w[3]);
+                }
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
-                    f4& acc = o[rt][wi * DPW + d];
-                    if constexpr (KT == 2)
-                        acc = mfma16(make_h8(w[0][d], w[1][d], w[2][d], w[3][d]), p8[rt], acc);
-                    else
-                        acc = bt_mfma16k16(make_h4(w[0][d], w[1][d]), h4{p8[rt][0], p8[rt][1], p8[rt][2], p8[rt][3]}, acc);
-                }
-        }
-        load_vs(nat, nb);
+                    const h8 b = lds.q[rt][s][lane];
 #pragma unroll
-        for (int kt = 0; kt < KT; kt++) at[kt] = nat[kt];
-    }
+                    for (int kt = 0; kt < KT; kt++) S[rt][kt] = mfma16(ka[kt], b, S[rt][kt]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            load_ks(nat, nb);
 
-    // the waves' states, joined in two rounds of 8 output tiles (twice the LDS would cost a workgroup per CU): in round h
-    // wave w takes tiles 8 h + 2 w, 8 h + 2 w + 1
+            // online softmax: a lane holds keys kb + 16 kt + 4 lg + i of row i16
+            bool masked = kb < seg.lo || kb + TILE > vmin;
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const float lt = rows_sum(l[rt]);
-        const int r = row0 + 16 * rt + i16;
-        // (rows of one KV head are rstep * token + head of the group apart in the states)
-        const size_t rec = (size_t)rstep * (r / GRP) + r % GRP;
+            for (int kt = 0; kt < KT; kt++) masked |= at[kt] < 0;
+            h8 p8[RT];
+            float cr[RT];
+            bool moved = false;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            __syncthreads();  // the previous round's states (or the last tile's Q) are read out
+            for (int rt = 0; rt < RT; rt++) {
+                if (masked) {
 #pragma unroll
-            for (int dt = 0; dt < 8; dt++) s_o[wave][dt][lane] = o[rt][8 * h + dt];
-            if (h == 0) {
-                s_ml[wave][0][lane] = m[rt];
-                s_ml[wave][1][lane] = lt;
+                    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int key = kb + 16 * kt + 4 * lg + i;
+                            S[rt][kt][i] = at[kt] >= 0 && key >= seg.lo && key < vis[rt] ? S[rt][kt][i] : -INFINITY;
+                        }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < KT; kt++) mx = max3f(max3f(mx, S[rt][kt][0], S[rt][kt][1]), S[rt][kt][2], S[rt][kt][3]);
+                mx = rows_max(mx);
+                const float mn = mx > m[rt] + PF_RESCALE_T ? mx : m[rt];
+                const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;  // a row that saw nothing keeps l = 0, O = 0
+                cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] * PF_LOG2E - msl);
+                // the sum is that of the rounded probabilities, the weights that P V applies
+                const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
+                float rs = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    p8[rt][j] = (_Float16)(j < 4 * KT ? fast_exp2(fmaf(S[rt][(j >> 2) % KT][j & 3], PF_LOG2E, -msl)) : 0.0f);
+#pragma unroll
+                for (int j = 0; j < 4 * KT; j += 2) rs = __builtin_amdgcn_fdot2(h2{p8[rt][j], p8[rt][j + 1]}, one2, rs, false);
+                l[rt] = l[rt] * cr[rt] + rs;
+                m[rt] = mn;
+                moved |= cr[rt] != 1.0f;
             }
-            __syncthreads();
-            float M = -INFINITY, L = 0.0f;
+            if (__any(moved)) {
 #pragma unroll
-            for (int w = 0; w < BT_WAVES; w++) M = fmaxf(M, s_ml[w][0][lane]);
-            f4 acc[2] = {};
+                for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-            for (int w = 0; w < BT_WAVES; w++) {
-                const float mw = s_ml[w][0][lane], lw = s_ml[w][1][lane];
-                const float f = lw == 0.0f ? 0.0f : fast_exp2((mw - M) * PF_LOG2E);  // (lw: NaN scores stay NaN)
-                L = fmaf(f, lw, L);
+                    for (int dt = 0; dt < 16; dt++) o[rt][dt] *= cr[rt];
+            }
+
+            // O^T += V^T P^T: output tile dt holds the lane's dim dt
+            uint32_t vd[4 * KT];
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const f4 x = s_o[w][2 * wave + t][lane];
+            for (int j = 0; j < 4 * KT; j++)
+                vd[j] = SC ? h2_bits(scale_of(vsd[j / 4], 4 * (4 * lg + j % 4) + (i16 >> 2), (i16 >> 1) & 1)) & 0xFFFFu : 0u;
+            constexpr int DPW = 16 / VW;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[t][i] = fmaf(f, x[i], acc[t][i]);
+            for (int wi = 0; wi < VW; wi++) {
+                __builtin_amdgcn_sched_barrier(0);
+                uint32_t w[2 * KT][DPW];
+#pragma unroll
+                for (int h = 0; h < 2 * KT; h++)
+                    bt_v_pair<KVT>(vr[2 * h][wi], vr[2 * h + 1][wi], vd[2 * h], vd[2 * h + 1], w[h]);
+#pragma unroll
+                for (int d = 0; d < DPW; d++)
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        f4& acc = o[rt][wi * DPW + d];
+                        if constexpr (KT == 2)
+                            acc = mfma16(make_h8(w[0][d], w[1][d], w[2][d], w[3][d]), p8[rt], acc);
+                        else
+                            acc = bt_mfma16k16(make_h4(w[0][d], w[1][d]), h4{p8[rt][0], p8[rt][1], p8[rt][2], p8[rt][3]}, acc);
+                    }
+            }
+            load_vs(nat, nb);
+#pragma unroll
+            for (int kt = 0; kt < KT; kt++) at[kt] = nat[kt];
+        }
+
+        // the next segment's first loads, where the registers hold them beside this one's sums
+        const BtSegment cur = seg;
+        const bool more = next(seg);
+        if (RT == 1 && more) begin();
+        // the waves' states, joined in two rounds of 8 output tiles (twice the LDS would cost a workgroup per CU): in round h
+        // wave w takes tiles 8 h + 2 w, 8 h + 2 w + 1
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const float lt = rows_sum(l[rt]);
+            const int r = cur.row0 + 16 * rt + i16;
+            // (rows of one KV head are rstep * token + head of the group apart in the states)
+            const size_t rec = (size_t)cur.rstep * (r / GRP) + r % GRP;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                __syncthreads();  // the previous round's states (or the last tile's Q) are read out
+#pragma unroll
+                for (int dt = 0; dt < 8; dt++) s_o[wave][dt][lane] = o[rt][8 * h + dt];
+                if (h == 0) {
+                    s_ml[wave][0][lane] = m[rt];
+                    s_ml[wave][1][lane] = lt;
+                }
+                __syncthreads();
+                float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                for (int w = 0; w < BT_WAVES; w++) M = fmaxf(M, s_ml[w][0][lane]);
+                f4 acc[2] = {};
+#pragma unroll
+                for (int w = 0; w < BT_WAVES; w++) {
+                    const float mw = s_ml[w][0][lane], lw = s_ml[w][1][lane];
+                    const float f = lw == 0.0f ? 0.0f : fast_exp2((mw - M) * PF_LOG2E);  // (lw: NaN scores stay NaN)
+                    L = fmaf(f, lw, L);
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const f4 x = s_o[w][2 * wave + t][lane];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[t][i] = fmaf(f, x[i], acc[t][i]);
+                    }
+                }
+                if (r < cur.rows) {
+                    if (h == 0 && wave == 0 && lg == 0) cur.pml[rec] = make_float2(M, L);
+                    // (output tile dt of lane row x = 4 lg + i holds dim 16 x + dt, of F16 128 (dt / 8) + 8 x + dt % 8)
+                    constexpr int STEP = KVT == QWA_KV_F16 ? 8 : 16;
+                    float* dst = cur.po + rec * HD + (KVT == QWA_KV_F16 ? 128 : 8) * h + 2 * wave;
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        *reinterpret_cast<float2*>(dst + STEP * (4 * lg + i)) = make_float2(acc[0][i], acc[1][i]);
                 }
             }
-            if (r < rows) {
-                if (h == 0 && wave == 0 && lg == 0) pml[rec] = make_float2(M, L);
-                // (output tile dt of lane row x = 4 lg + i holds dim 16 x + dt, of F16 128 (dt / 8) + 8 x + dt % 8)
-                constexpr int STEP = KVT == QWA_KV_F16 ? 8 : 16;
-                float* dst = po + rec * HD + (KVT == QWA_KV_F16 ? 128 : 8) * h + 2 * wave;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    *reinterpret_cast<float2*>(dst + STEP * (4 * lg + i)) = make_float2(acc[0][i], acc[1][i]);
-            }
         }
+        if (!more) break;
+        if (RT > 1) begin();
+        __syncthreads();  // the states are read out of LDS
     }
 }
 
@@ -474,8 +495,9 @@ k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len, int g
     const int seq = bt_seq(a, b);
     const int* table = p.table + (seq >= 0 && seq < p.n_seq ? (size_t)seq * p.ld : 0);
     const size_t rec = (size_t)sp * a.n * a.nq * NH + g * GRP;
-    bt_body<KVT, RT>(lds, a, kv, p, table, grp * 16 * RT, a.n * a.nq * GRP, g, sp * len, k1, 0, a.part_o + rec * HD,
-                     a.part_ml + rec, NH);
+    bt_body<KVT, RT>(lds, a, kv, p, g,
+                     {table, grp * 16 * RT, a.n * a.nq * GRP, sp * len, k1, 0, a.part_o + rec * HD, a.part_ml + rec, NH},
+                     [](BtSegment&) { return false; });
 }
 
 // steps of batch row b's own positions (they begin at the multiple of 16 at or before n_shared)
@@ -486,9 +508,10 @@ __device__ __forceinline__ int bt_steps_of(const BatchArgs& a, int m) {
 // the own positions: workgroup = (slice of the steps, KV head, row group), one segment per sequence that the slice meets.
 // Equal slices, since a cut by sequences leaves the chip to the longest one (24 of up to 16384 positions 108 instead of 89 us).
 // About 6 us of latency (finding the slice, page numbers, first bytes, joining the waves) around a stream of the cache's bytes:
-// 24 sequences of 267 000 Q4_0 positions together 67 us (4.6 TB/s; unpacking takes half of the issue cycles), of 131 000 Q8_0
-// ones 61 us (4.7 TB/s), F16 100 us (5.3 TB/s, where a large copy reads and writes 5.15).  Not faster: a second tile on its
-// way (registers for it are there), three waves a SIMD (spills), the next segment's first tile sent before this one's merge.
+// 24 sequences of 267 000 Q4_0 positions together 66 us (4.7 TB/s; unpacking takes half of the issue cycles), of 131 000 Q8_0
+// ones 61 us (4.7 TB/s), F16 100 us (5.3 TB/s, where a large copy reads and writes 5.15).  The next segment's first tile is
+// sent before this one's waves are joined (24 sequences 68.2 -> 66.5 us, 1000 of 40 positions 64.7 -> 62.2).  Not faster: a
+// second tile on its way (registers for it are there), three waves a SIMD (spills).
 template <int KVT, int RT>
 __global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
@@ -548,24 +571,38 @@ k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
         first += __builtin_amdgcn_readlane(within - x, row);
         m = __builtin_amdgcn_readlane(x, row);
     }
+    // the lengths and sequences of the 64 rows from b on, a lane each (read a segment at a time they were a round trip each)
+    int row0 = b, lens, seqs;
+    auto look = [&]() {
+        row0 = b;
+        bt_lens<1>(a, p, b + lane, 1, &lens);
+        seqs = bt_seq(a, min(b + lane, a.n - 1));
+    };
+    look();
     const int base = a.n_shared & ~15;
-    while (true) {
-        const int stop = min(end, first + m);
-        const int k0 = base + (s - first) * BT_STEP, k1 = min(base + (stop - first) * BT_STEP, bt_len(a, p, b));
+    int stop = s;
+    // the segment of batch row b, from step s on
+    auto segment = [&]() {
+        stop = min(end, first + m);
+        const int k0 = base + (s - first) * BT_STEP;
+        const int k1 = min(base + (stop - first) * BT_STEP, __builtin_amdgcn_readlane(lens, b - row0));
         const size_t rec = ((size_t)g * (a.wgs + a.n) + w + b) * a.nq * GRP;
         // (row r = 6 * token + head has place r - 6 nq b of the segment)
-        float* po = a.own_o + ((ptrdiff_t)rec - (ptrdiff_t)b * a.nq * GRP) * HD;
-        float2* pml = a.own_ml + ((ptrdiff_t)rec - (ptrdiff_t)b * a.nq * GRP);
-        bt_body<KVT, RT>(lds, a, kv, p, p.table + (size_t)bt_seq(a, b) * p.ld, b * a.nq * GRP + grp * 16 * RT,
-                         (b + 1) * a.nq * GRP, g, k0, k1, a.n_shared, po, pml, GRP);
+        const ptrdiff_t place = (ptrdiff_t)rec - (ptrdiff_t)b * a.nq * GRP;
+        return BtSegment{p.table + (size_t)__builtin_amdgcn_readlane(seqs, b - row0) * p.ld, b * a.nq * GRP + grp * 16 * RT,
+                         (b + 1) * a.nq * GRP, k0, k1, a.n_shared, a.own_o + place * HD, a.own_ml + place, GRP};
+    };
+    bt_body<KVT, RT>(lds, a, kv, p, g, segment(), [&](BtSegment& seg) {
         s = stop;
-        if (s >= end) break;
+        if (s >= end) return false;
         do {
             first += m;
-            m = bt_steps_of(a, bt_len(a, p, ++b));
+            if (++b - row0 >= 64) look();
+            m = bt_steps_of(a, __builtin_amdgcn_readlane(lens, b - row0));
         } while (m == 0);
-        __syncthreads();  // the last segment's states are read out of LDS
-    }
+        seg = segment();
+        return true;
+    });
 }
 
 // What a thread converts of a tile, u = t & 255.  Waves 0 .. 3 (V): dims 8 c .. 8 c + 7 (c = u & 31) of the four keys 16 h +

@@ -317,6 +317,12 @@ def test_captured_calls_share_a_work_buffer(gpu):
             c[0].mul_(-1)
 
 
+def test_empty_sequences_inside_a_slice(gpu):
+    """The last slice of the own positions has the end of the first sequence and, 1000 empty ones on, the only other one."""
+    out = Batch(ops.Q8_0, [16384] + [0] * 999 + [50] + [0] * 23).check(1, 0, what="two of 1024")
+    assert not out[1:1000].any() and not out[1001:].any()
+
+
 def test_largest_batch(gpu):
     b = Batch(ops.Q8_0, [24 + i % 40 for i in range(1024)], shared=16, page=16)
     b.check(8, 16, what="1024 sequences, 8 queries")
