@@ -232,7 +232,8 @@ size_t qwa_attn_batch_work_bytes(int n, int nq, int n_shared, int max_len);
 /* Attention of n sequences with nq (1..8) queries each over a paged cache: batch row b is sequence seqs[b] (device;
  * NULL: b), query t of it sees positions [0, len - nq + t].  q, gate [n * nq][24][256]; out16: output * sigmoid(gate)
  * as fp16 bits [n * nq][6144] (the input of the output projection's GEMM), optional ActQ8 rows (of the fp32 values, for
- * the GEMV).  fp16 MFMA, fp32 accumulation and softmax.
+ * the GEMV).  fp16 MFMA, fp32 accumulation and softmax; scores are exact up to fp32 accumulation (K as its codes, Q in
+ * two fp16 parts), so outlier keys cost no accuracy; V as stored and the probabilities are rounded to fp16.
  * n_shared: the batch rows have their first n_shared positions in common (forks of one prompt; 0: nothing).  Their keys
  * are read once for all rows, through the table of the longest row (the first of those); a shorter row sees as many of
  * them as it has positions.

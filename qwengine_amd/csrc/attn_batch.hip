@@ -12,12 +12,16 @@
 //    once into LDS, by way of registers, and every wave multiplies its rows with it.
 //  * Pages are multiples of 16 positions and tiles start at multiples of 16, so each 16 keys lie in one page.  A wave looks
 //    the pages of its next 64 tiles up at once, a lane a tile.
-//  * S^T = K Q^T and O^T += V^T P^T on fp16 MFMA with fp32 accumulation.  In a register workgroup a lane loads 64 dims of one
-//    key and 16 dims of the keys whose probabilities it holds straight into registers in operand order and dequantizes there
-//    (kv_operands.hpp); the next tile's K loads go out when the scores are done, its V loads when P V is.
+//  * S^T = K Q^T and O^T += V^T P^T on fp16 MFMA with fp32 accumulation.  K enters as its exact codes, 32 dims (a block of the
+//    cache) an MFMA, whose fp32 product is multiplied by the key's block scale, and Q / 16 as the sum of two fp16 parts: scores
+//    are exact up to fp32 accumulation, as the one-sequence decode's are.  (With Q / 16 and d * code rounded to fp16, keys eight
+//    times as large as the others moved an output by 4e-3 to 6e-3.)  In a register workgroup a lane loads 64 dims of one key and
+//    16 dims of the keys whose probabilities it holds straight into registers and converts there; the next tile's K loads go
+//    out when the scores are done, its V loads when P V is.
 // A batch of one call has the same bits again; another batch, or another cut, sums a row's states in another order.
-// Roundings below 32 bits: Q / 16, the dequantized K and V, and the probabilities are fp16 (2^-12 relative each, random in
-// sign, as in the prefill), the output is fp16.
+// Roundings below 32 bits: the dequantized V (d * code) and the probabilities are fp16 (half a step: 2^-11 of the value, random
+// in sign, as in the prefill: P V then has one MFMA per 32 keys and 16 dims), a tile workgroup's O / l is 16-bit fixed point
+// (half a step: 2^-16 of the row's largest, attn_tiles.hpp), the output is fp16.
 #include <type_traits>
 
 #include "attn_tiles.hpp"
@@ -93,6 +97,52 @@ __device__ __forceinline__ int bt_place(const qwa_kv_pages& p, const int* __rest
     return (unsigned)pg < (unsigned)p.n_pages ? pg * p.page + (kb & (p.page - 1)) : -1;
 }
 
+// lane FROM of each row of 16 lanes, in all of them
+template <int FROM>
+__device__ __forceinline__ float row_lane(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + FROM, 0xF, 0xF, true));
+}
+// Scores of 16 keys from block S's products: a lane holds keys 4 lg + i, and lane 4 i + S / 2 of its row of 16 the scales of
+// blocks S, S ^ 1 of key 4 lg + i (even block in `even`).
+template <int S>
+__device__ __forceinline__ void add_block(f4& score, const f4& product, float even, float odd) {
+    const float d = S % 2 ? odd : even;
+    score[0] = fmaf(row_lane<S / 2>(d), product[0], score[0]);
+    score[1] = fmaf(row_lane<4 + S / 2>(d), product[1], score[1]);
+    score[2] = fmaf(row_lane<8 + S / 2>(d), product[2], score[2]);
+    score[3] = fmaf(row_lane<12 + S / 2>(d), product[3], score[3]);
+    // (the sums stay where they are: put off past the last block, they kept all scales and products, and spilled)
+    asm volatile("" : "+v"(score));
+}
+__device__ __forceinline__ void add_block(int s, f4& score, const f4& product, float even, float odd) {  // s: unrolled
+    switch (s) {
+        case 0: add_block<0>(score, product, even, odd); break;
+        case 1: add_block<1>(score, product, even, odd); break;
+        case 2: add_block<2>(score, product, even, odd); break;
+        case 3: add_block<3>(score, product, even, odd); break;
+        case 4: add_block<4>(score, product, even, odd); break;
+        case 5: add_block<5>(score, product, even, odd); break;
+        case 6: add_block<6>(score, product, even, odd); break;
+        default: add_block<7>(score, product, even, odd); break;
+    }
+}
+// Q / 16 = hi + lo, fp16 each
+__device__ __forceinline__ _Float16 q_hi(float x) { return (_Float16)x; }
+__device__ __forceinline__ _Float16 q_lo(float x) { return (_Float16)(x - (float)(_Float16)x); }
+
+// lane rows 0, 1 of b for lane rows 2, 3 of a
+__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
+    const auto x = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = x[0];
+    b = x[1];
+}
+// lane rows 0, 2 of b for lane rows 1, 3 of a
+__device__ __forceinline__ void swap_rows(uint32_t& a, uint32_t& b) {
+    const auto x = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = x[0];
+    b = x[1];
+}
+
 // `bytes` bytes from a wave-uniform address on, in 32-bit words; what is read past them is zero
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t bt_buffer(const void* base, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00027000);
@@ -114,27 +164,35 @@ __device__ __forceinline__ uint32_t q4_bits(uint32_t w, uint32_t mask, uint32_t 
     asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(magic));
     return r;
 }
-__device__ __forceinline__ h2 q4_lo(uint32_t w, h2 d) {
+__device__ __forceinline__ h2 q4_lo(uint32_t w) {
     const h2 bias = {(_Float16)1032.0f, (_Float16)1032.0f};
-    return (bits_h2(q4_bits(w, 0x000F000Fu, 0x64006400u)) - bias) * d;
+    return bits_h2(q4_bits(w, 0x000F000Fu, 0x64006400u)) - bias;
 }
-__device__ __forceinline__ h2 q4_hi(uint32_t w, h2 d) {
+__device__ __forceinline__ h2 q4_hi(uint32_t w) {
     const h2 bias = {(_Float16)72.0f, (_Float16)72.0f};
-    return (bits_h2(q4_bits(w, 0x00F000F0u, 0x54005400u)) - bias) * d;
+    return bits_h2(q4_bits(w, 0x00F000F0u, 0x54005400u)) - bias;
 }
-__device__ __forceinline__ void bt_q4_k(uint32_t w, h2 d, uint32_t* out) {
-    out[0] = h2_bits(q4_lo(w, d));
-    out[1] = h2_bits(q4_hi(w, d));
-    out[2] = h2_bits(q4_lo(w >> 8, d));
-    out[3] = h2_bits(q4_hi(w >> 8, d));
+// the codes c - 8 of a word
+__device__ __forceinline__ void bt_q4_codes(uint32_t w, uint32_t* out) {
+    out[0] = h2_bits(q4_lo(w));
+    out[1] = h2_bits(q4_hi(w));
+    out[2] = h2_bits(q4_lo(w >> 8));
+    out[3] = h2_bits(q4_hi(w >> 8));
+}
+// the same, times d (one fp16 rounding)
+__device__ __forceinline__ void bt_q4_values(uint32_t w, h2 d, uint32_t* out) {
+    out[0] = h2_bits(q4_lo(w) * d);
+    out[1] = h2_bits(q4_hi(w) * d);
+    out[2] = h2_bits(q4_lo(w >> 8) * d);
+    out[3] = h2_bits(q4_hi(w >> 8) * d);
 }
 // out[dim] = {V_a[dim], V_b[dim]} for the 8 (Q4_0), 4 or 2 dims of a word of keys a and b
 template <int KVT>
 __device__ __forceinline__ void bt_v_pair(uint32_t aw, uint32_t bw, uint32_t sa, uint32_t sb, uint32_t* out) {
     if constexpr (KVT == QWA_KV_Q4_0) {
         const h2 d = scale_pair((uint16_t)sa, (uint16_t)sb);
-        bt_q4_k(__builtin_amdgcn_perm(bw, aw, 0x05040100u), d, out);      // bytes {a0, a1, b0, b1}
-        bt_q4_k(__builtin_amdgcn_perm(bw, aw, 0x07060302u), d, out + 4);  // bytes {a2, a3, b2, b3}
+        bt_q4_values(__builtin_amdgcn_perm(bw, aw, 0x05040100u), d, out);      // bytes {a0, a1, b0, b1}
+        bt_q4_values(__builtin_amdgcn_perm(bw, aw, 0x07060302u), d, out + 4);  // bytes {a2, a3, b2, b3}
     } else {
         v_pair_words<KVT, 1>(&aw, &bw, sa, sb, out);
     }
@@ -143,13 +201,13 @@ __device__ __forceinline__ void bt_v_pair(uint32_t aw, uint32_t bw, uint32_t sa,
 template <int KVT, int RT>
 struct BtCfg {
     // 16-key groups of a tile, as two waves per SIMD leave registers for (raw bytes of 32 keys: F16 128 registers, Q8_0 66)
-    static constexpr int KT = KVT == QWA_KV_F16 || (KVT == QWA_KV_Q8_0 && RT > 1) ? 1 : 2;
+    static constexpr int KT = KVT == QWA_KV_F16 || RT > 1 ? 1 : 2;
 };
 
 template <int KVT, int RT>
 struct BtLds {
     union {
-        h8 q[RT][8][64];        // while the keys are walked
+        h8 q[RT][8][2][64];     // while the keys are walked: hi and lo part of Q / 16
         f4 o[BT_WAVES][8][64];  // while the waves' states are joined, half of the output tiles at a time
     };
     float ml[BT_WAVES][2][64];
@@ -244,9 +302,9 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
         return bits_h2(__builtin_amdgcn_perm(u, u, h ? 0x03020302u : 0x01000100u));
     };
 
-    // rows of this lane: keys below vis are seen; Q / 16 as the B operand in the K operand's dim order, of which a wave makes
-    // steps 2 * wave and 2 * wave + 1
-    constexpr int E = 4096 / VB;  // values of a 16-byte piece of a row
+    // rows of this lane: keys below vis are seen; Q / 16 as the B operand in the K operand's dim order (step s: block s, of which
+    // the lane holds 8 dims from qd on), of which a wave makes steps 2 * wave and 2 * wave + 1
+    const int qd = KVT == QWA_KV_Q8_0 ? 16 * (lg & 1) + 8 * (lg >> 1) : 8 * lg;
     int vis[RT], vmin, at[KT];
     float4 qx[RT][2][2];
     // A segment's first loads: what is read of Q and the lengths is on its way while the pages are looked up.
@@ -261,11 +319,10 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
             const bool valid = r < seg.rows;
             vis[rt] = valid ? min(bt_len(a, p, tok / a.nq) - a.nq + tok % a.nq + 1, k1) : 0;
             if (valid) vmin = min(vmin, vis[rt]);
-            const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + E * lg;
+            const float* qrow = a.q + ((size_t)(valid ? tok : 0) * NH + g * GRP + r % GRP) * HD + qd;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int d = 8 * (2 * wave + i);
-                const float* src = qrow + 4 * E * (d / E) + d % E;
+                const float* src = qrow + 32 * (2 * wave + i);
                 qx[rt][i][0] = *reinterpret_cast<const float4*>(src);
                 qx[rt][i][1] = *reinterpret_cast<const float4*>(src + 4);
             }
@@ -284,10 +341,15 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
             for (int i = 0; i < 2; i++) {
                 const float4 x0 = qx[rt][i][0], x1 = qx[rt][i][1];
                 const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-                h8 v;
+                h8 hi, lo;
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = valid ? (_Float16)(x[k_perm<KVT>(j)] * 0.0625f) : (_Float16)0.0f;
-                lds.q[rt][2 * wave + i][lane] = v;
+                for (int j = 0; j < 8; j++) {
+                    const float y = valid ? x[k_perm<KVT>(j)] * 0.0625f : 0.0f;
+                    hi[j] = q_hi(y);
+                    lo[j] = q_lo(y);
+                }
+                lds.q[rt][2 * wave + i][0][lane] = hi;
+                lds.q[rt][2 * wave + i][1][lane] = lo;
             }
         }
         __syncthreads();
@@ -315,17 +377,30 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
             for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                 for (int kt = 0; kt < KT; kt++) S[rt][kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            // a lane's block scales of key i16: piece 4 i + lg of 32 values (Q4_0: block 4 i + lg), or 16 (Q8_0: 2 i + lg / 2)
-            constexpr int NS = KVT == QWA_KV_Q4_0 ? 2 : 4;
-            h2 kd[KT][NS];
+            // The lanes' pieces become blocks, 8 dims a lane: Q4_0, where a lane has a whole block, by exchanging words and lane
+            // rows (word k of lane row r <-> word r of lane row k), Q8_0, where two lanes have one, half of that.
+            float even[KT], odd[KT];
             if constexpr (SC) {
 #pragma unroll
-                for (int kt = 0; kt < KT; kt++)
+                for (int kt = 0; kt < KT; kt++) {
 #pragma unroll
-                    for (int i = 0; i < NS; i++)
-                        kd[kt][i] = KVT == QWA_KV_Q4_0 ? scale_of(ksd[kt], 4 * i16 + 2 * i + (lg >> 1), lg & 1)
-                                                       : scale_of(ksd[kt], 4 * i16 + i, lg >> 1);
+                    for (int i = 0; i < KW; i += 4) {
+                        uint32_t* const w = kr[kt] + i;
+                        swap_halves(w[0], w[2]);
+                        swap_halves(w[1], w[3]);
+                        if constexpr (KVT == QWA_KV_Q4_0) {
+                            swap_rows(w[0], w[1]);
+                            swap_rows(w[2], w[3]);
+                        }
+                    }
+                    // (dword l of the 16 rows' scales is in lane l: rows 4 lg .. 4 lg + 3 in this lane's row of 16)
+                    even[kt] = h2f_bits((uint16_t)ksd[kt]);
+                    odd[kt] = h2f_bits((uint16_t)(ksd[kt] >> 16));
+                }
             }
+            // products of blocks s and s - LAG, where the registers allow the latter
+            constexpr int LAG = RT == 1 ? 1 : 0;
+            f4 T[1 + LAG][RT][KT];
 #pragma unroll
             for (int s = 0; s < 8; s++) {
                 h8 ka[KT];
@@ -336,20 +411,45 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
 #pragma unroll
                         for (int i = 0; i < 4; i++) w[i] = kr[kt][4 * s + i];
                     } else if constexpr (KVT == QWA_KV_Q8_0) {
-                        q8_word_to_h4(kr[kt][2 * s], kd[kt][s / 2], w);
-                        q8_word_to_h4(kr[kt][2 * s + 1], kd[kt][s / 2], w + 2);
+                        q8_word_int(kr[kt][2 * s], w);
+                        q8_word_int(kr[kt][2 * s + 1], w + 2);
                     } else {
-                        bt_q4_k(kr[kt][s], kd[kt][s / 4], w);
+                        bt_q4_codes(kr[kt][s], w);
                     }
                     ka[kt] = make_h8(w[0], w[1], w[2], w[3]);
                 }
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    const h8 b = lds.q[rt][s][lane];
+                for (int part = 1; part >= 0; part--) {
 #pragma unroll
-                    for (int kt = 0; kt < KT; kt++) S[rt][kt] = mfma16(ka[kt], b, S[rt][kt]);
+                    for (int rt = 0; rt < RT; rt++) {
+                        const h8 b = lds.q[rt][s][part][lane];
+#pragma unroll
+                        for (int kt = 0; kt < KT; kt++) {
+                            if constexpr (SC) {
+                                const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                                T[s & LAG][rt][kt] = mfma16(ka[kt], b, part ? zero : T[s & LAG][rt][kt]);
+                            } else {
+                                S[rt][kt] = mfma16(ka[kt], b, S[rt][kt]);
+                            }
+                        }
+                    }
+                    if (RT > 1) __builtin_amdgcn_sched_barrier(0);  // (registers)
+                }
+                if constexpr (SC) {
+                    if (s >= LAG)
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                            for (int kt = 0; kt < KT; kt++)
+                                add_block(s - LAG, S[rt][kt], T[(s - LAG) & LAG][rt][kt], even[kt], odd[kt]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (SC && LAG > 0) {
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int kt = 0; kt < KT; kt++) add_block(7, S[rt][kt], T[7 & LAG][rt][kt], even[kt], odd[kt]);
             }
             load_ks(nat, nb);
 
@@ -693,11 +793,15 @@ __device__ __forceinline__ void bt_store_v(BtRaw<KVT>& r, _Float16* Vt, int t, u
         for (int d = 0; d < DPW; d++) *reinterpret_cast<uint2*>(dst + 8 * 32 * (DPW * i + d)) = make_uint2(lo[d], hi[d]);
     }
 }
+// K's codes, and their scales: unit (16 keys, pair of blocks, 4 keys) of 16 bytes, [block of the pair][key of the four]
 template <int KVT>
-__device__ __forceinline__ void bt_store_k(const BtRaw<KVT>& r, _Float16* Ks, int t) {
+__device__ __forceinline__ void bt_store_k(const BtRaw<KVT>& r, _Float16* Ks, uint16_t* scales, int t) {
     const int u = t & 255;
     _Float16* dst = Ks + 8 * (32 * 4 * (u & 7) + ((u >> 3) ^ (2 * (u & 7))));
-    const h2 d = scale_pair((uint16_t)r.sc[0], (uint16_t)r.sc[0]);
+    if constexpr (KVT != QWA_KV_F16) {
+        const int key = u >> 3, b = u & 7;
+        scales[8 * (16 * (key >> 4) + 4 * (b >> 1) + ((key >> 2) & 3)) + 4 * (b & 1) + (key & 3)] = (uint16_t)r.sc[0];
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         uint32_t o[4];
@@ -705,21 +809,22 @@ __device__ __forceinline__ void bt_store_k(const BtRaw<KVT>& r, _Float16* Ks, in
 #pragma unroll
             for (int k = 0; k < 4; k++) o[k] = r.w[4 * i + k];
         } else if constexpr (KVT == QWA_KV_Q8_0) {
-            q8_word_to_h4(r.w[2 * i], d, o);
-            q8_word_to_h4(r.w[2 * i + 1], d, o + 2);
+            q8_word_int(r.w[2 * i], o);
+            q8_word_int(r.w[2 * i + 1], o + 2);
         } else {
-            bt_q4_k(r.w[i], d, o);
+            bt_q4_codes(r.w[i], o);
         }
         *reinterpret_cast<uint4*>(dst + 8 * 32 * i) = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 
-// The shared positions for BT_TROWS rows: workgroup = (row block, tile range, KV head).  The 12 waves have 16 rows each,
-// three a SIMD: of those one converts V at the start of an iteration, one K at its end, one nothing, so the MFMAs of one run
-// while others convert, take exponentials or wait for LDS.  128 sequences over 32768 Q4_0 positions: 127 us, 0.81 PFLOP/s, 1.8
-// us a tile (large products of the library reach 1.17).  The bound is LDS: 12 waves read a tile's 32 KB each, which with the
-// writes takes four fifths of the cycles.  (32 rows a wave, two a SIMD, read half as much per row, but spill 56 registers:
-// 164 us.)
+// The shared positions for BT_TROWS rows: workgroup = (row block, tile range, KV head).  The 8 waves have 16 rows each, two a
+// SIMD, of which one converts V at the start of an iteration and the other K at its end, so the MFMAs of one run while the
+// other converts, takes exponentials or waits for LDS.  128 sequences over 32768 Q4_0 positions: 196 us, 0.79 PFLOP/s with the
+// second part of Q (large products of the library reach 1.17).  Of a SIMD's cycles 44% issue VALU instructions and 30% are
+// MFMAs; LDS is busy for 43%: two waves do not cover each other's waits.  (Three a SIMD have 168 registers each, which O and
+// both parts of Q leave 40 of: 12 waves spilled 47 to 108 with the low parts in LDS.  The block scales by lane broadcasts
+// instead of from LDS: 207 us.)
 template <int KVT>
 __global__ void __launch_bounds__(64 * BT_TWAVES) __attribute__((amdgpu_waves_per_eu(BT_TWAVES / 4, BT_TWAVES / 4)))
 k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
@@ -728,6 +833,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
         struct {
             _Float16 k[2][PF_TILE * HD];
             _Float16 vt[2][PF_TILE * HD];
+            uint16_t scales[2][KVT == QWA_KV_F16 ? 8 : PF_TILE * 8];  // of K
         } tile;
         uint2 xch[BT_TWAVES][XCH / 8];
     } lds;
@@ -769,7 +875,8 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
     const uint16_t* const ksh = KVT == QWA_KV_F16 ? nullptr : kv.ks + head * 8;
     const uint16_t* const vsh = KVT == QWA_KV_F16 ? nullptr : kv.vs + head * 8;
 
-    h8 qb[8];
+    constexpr bool SC = KVT != QWA_KV_F16;
+    h8 qb[2][8];  // hi and lo part of Q / 16
     f4 o[16];
     float m = -INFINITY, l = 0.0f;
     const int r = wrow0 + i16, tok = r / GRP;
@@ -779,8 +886,8 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
     vmin = __builtin_amdgcn_readfirstlane(vmin);
-    // ROLE 0: a wave that converts V, 1: K, 2: neither.  (In one loop for all three, the registers that the roles shared made
-    // a wave wait for its loads as soon as they were sent: 128 sequences over 32768 Q4_0 positions 154 instead of 129 us.)
+    // ROLE 0: a wave that converts V, 1: K.  (In one loop for both, the registers that the roles share make a wave wait for its
+    // loads as soon as they are sent.)
     auto walk = [&](auto role) __attribute__((always_inline)) {
         constexpr int ROLE = decltype(role)::value;
         BtRaw<KVT> raw;
@@ -792,18 +899,18 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
             const int rows[2] = {at[0] < 0 ? 16 : min(left, 16), at[1] < 0 ? 16 : min(left - 16, 16)};
             const uint32_t bits = (uint32_t)((at[0] < 0) | (at[1] < 0) << 1);
             if constexpr (ROLE == 0) bt_load_v<KVT>(raw, vh, vsh, at, rows, t);
-            if constexpr (ROLE == 1) bt_load_k<KVT>(raw, kh, ksh, wave < 6 ? at[0] : at[1], wave < 6 ? rows[0] : rows[1], t);
+            else bt_load_k<KVT>(raw, kh, ksh, wave < 6 ? at[0] : at[1], wave < 6 ? rows[0] : rows[1], t);
             return bits;
         };
         auto store = [&](int b, uint32_t bits) {
             if constexpr (ROLE == 0) bt_store_v<KVT>(raw, s_vt[b], t, bits);
-            if constexpr (ROLE == 1) bt_store_k<KVT>(raw, s_k[b], t);
+            else bt_store_k<KVT>(raw, s_k[b], lds.tile.scales[b], t);
         };
         if (nt > 0) dead = load(0);
 
-        // Q / 16 as the B operand, by way of the wave's part of the exchange: a row is read as one kilobyte (fragment by
-        // fragment, 16 rows at once, the loads took 7 us), its fp16 pieces go to unit (s, lg, row ^ (4 s + lg) % 16) and come
-        // back as the lane's fragments s
+        // Q / 16 as the B operand, by way of the wave's part of the exchange, first the hi parts, then the lo parts: a row is
+        // read as one kilobyte (fragment by fragment, 16 rows at once, the loads took 7 us), its fp16 pieces go to unit (s, lg,
+        // row ^ (4 s + lg) % 16) and come back as the lane's fragments s
         {
             float4 x[16];
 #pragma unroll
@@ -814,26 +921,32 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
             uint8_t* const area = reinterpret_cast<uint8_t*>(lds.xch[wave]);
             const int c = lane >> 1, half = lane & 1;  // piece c = 4 s + lg, dims 4 half .. 4 half + 3 of it
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const float f = wrow0 + j < nrows ? 0.0625f : 0.0f;
-                uint32_t w0 = h2_bits(h2{(_Float16)(x[j].x * f), (_Float16)(x[j].y * f)});
-                uint32_t w1 = h2_bits(h2{(_Float16)(x[j].z * f), (_Float16)(x[j].w * f)});
-                if constexpr (KVT == QWA_KV_Q4_0) {
-                    // the operand's order [0, 4, 1, 5, 2, 6, 3, 7]: the even lane makes the first two words, the odd one the
-                    // rest
-                    const uint32_t mine = half ? w1 : w0;
-                    const uint32_t other = __builtin_amdgcn_update_dpp(0, half ? w0 : w1, 0xB1, 0xF, 0xF, true);
-                    const uint32_t lo = half ? other : mine, hi = half ? mine : other;  // dims k, k + 1 and k + 4, k + 5
-                    w0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
-                    w1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-                }
-                *reinterpret_cast<uint2*>(area + 16 * (16 * c + (j ^ (c & 15))) + 8 * half) = make_uint2(w0, w1);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
-            __builtin_amdgcn_wave_barrier();
+            for (int part = 0; part < 2; part++) {
+                auto piece = [&](float v, float f) { return part ? q_lo(v * f) : q_hi(v * f); };
 #pragma unroll
-            for (int s = 0; s < 8; s++)
-                qb[s] = *reinterpret_cast<const h8*>(area + 16 * (16 * (4 * s + lg) + (i16 ^ ((4 * s + lg) & 15))));
+                for (int j = 0; j < 16; j++) {
+                    const float f = wrow0 + j < nrows ? 0.0625f : 0.0f;
+                    uint32_t w0 = h2_bits(h2{piece(x[j].x, f), piece(x[j].y, f)});
+                    uint32_t w1 = h2_bits(h2{piece(x[j].z, f), piece(x[j].w, f)});
+                    if constexpr (KVT == QWA_KV_Q4_0) {
+                        // the operand's order [0, 4, 1, 5, 2, 6, 3, 7]: the even lane makes the first two words, the odd one
+                        // the rest
+                        const uint32_t mine = half ? w1 : w0;
+                        const uint32_t other = __builtin_amdgcn_update_dpp(0, half ? w0 : w1, 0xB1, 0xF, 0xF, true);
+                        const uint32_t lo = half ? other : mine, hi = half ? mine : other;  // dims k, k + 1 and k + 4, k + 5
+                        w0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+                        w1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+                    }
+                    *reinterpret_cast<uint2*>(area + 16 * (16 * c + (j ^ (c & 15))) + 8 * half) = make_uint2(w0, w1);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int s = 0; s < 8; s++)
+                    qb[part][s] = *reinterpret_cast<const h8*>(area + 16 * (16 * (4 * s + lg) + (i16 ^ ((4 * s + lg) & 15))));
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
         }
         __syncthreads();  // the fragments are in registers; the tiles lie in the same LDS
 
@@ -855,11 +968,17 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
                 const int k0 = (tb + i) * PF_TILE;
                 const _Float16* Ks = s_k[i & 1];
                 const _Float16* Vt = s_vt[i & 1];
+                const _Float16* Sc = reinterpret_cast<const _Float16*>(lds.tile.scales[i & 1]);
                 if constexpr (ROLE == 0) convert(i);
                 if (rows_here) {
                     // S^T = K Q^T: lane (row i16) gets keys k0 + 16 kt + 4 lg + j; the K fragments of a step are read while
-                    // the step before multiplies
-                    f4 sc[2] = {};
+                    // the step before multiplies, whose product is scaled while the next one is on its way
+                    f4 sc[2] = {}, T[2][2];
+                    h8 ks[2];  // scales of blocks s - 1 and s, s even, or s and s + 1
+                    auto scale = [&](int s, int kt) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) sc[kt][j] = fmaf((float)ks[kt][4 * (s & 1) + j], T[s & 1][kt][j], sc[kt][j]);
+                    };
                     auto kfrag = [&](int s, int kt) {
                         return lds_h8(Ks + 8 * (32 * (4 * s + lg) + 16 * kt + (i16 ^ (2 * s))));
                     };
@@ -875,8 +994,31 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
                             for (int kt = 0; kt < 2; kt++) kf[(s + BT_KD) % (BT_KD + 1)][kt] = kfrag(s + BT_KD, kt);
                         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int kt = 0; kt < 2; kt++) sc[kt] = mfma16(kf[s % (BT_KD + 1)][kt], qb[s], sc[kt]);
+                        for (int part = 1; part >= 0; part--)
+#pragma unroll
+                            for (int kt = 0; kt < 2; kt++) {
+                                const h8 k8 = kf[s % (BT_KD + 1)][kt];
+                                if constexpr (SC) {
+                                    const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                                    T[s & 1][kt] = mfma16(k8, qb[part][s], part ? zero : T[s & 1][kt]);
+                                } else {
+                                    sc[kt] = mfma16(k8, qb[part][s], sc[kt]);
+                                }
+                            }
+                        if constexpr (SC) {
+                            if (s > 0) {
+                                scale(s - 1, 0);
+                                scale(s - 1, 1);
+                            }
+                            if (s % 2 == 0)
+#pragma unroll
+                                for (int kt = 0; kt < 2; kt++) ks[kt] = lds_h8(Sc + 8 * (16 * kt + 2 * s + lg));
+                        }
                         __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if constexpr (SC) {
+                        scale(7, 0);
+                        scale(7, 1);
                     }
                     if (k0 + PF_TILE > vmin || (dead & 3) != 0) {
 #pragma unroll
@@ -923,8 +1065,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
         }
     };
     if (wave < 4) walk(std::integral_constant<int, 0>{});
-    else if (wave < 8) walk(std::integral_constant<int, 1>{});
-    else walk(std::integral_constant<int, 2>{});
+    else walk(std::integral_constant<int, 1>{});
 
     // partial state: o[2 k + e][j] is dim 8 x + k of row i16, x = 16 e + 4 lg + j; through LDS, so that a store instruction
     // writes two whole 512-byte rows

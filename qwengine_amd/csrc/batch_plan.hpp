@@ -14,7 +14,7 @@ namespace qwa {
 
 constexpr int BT_WAVES = 4;               // waves of a register workgroup; they take the tiles of its key range in turn
 constexpr int BT_MAXRT = 2;               // 16-row MFMA tiles of such a workgroup at most
-constexpr int BT_TWAVES = 12;             // waves of a tile workgroup
+constexpr int BT_TWAVES = 8;              // waves of a tile workgroup (four convert V, four K)
 constexpr int BT_TROWS = 16 * BT_TWAVES;  // its rows
 // Register workgroups that the chip holds, two a CU (own positions of 24 sequences of up to 16384 Q4_0 positions 68 us, with
 // 1024 in two rounds 72).
@@ -23,10 +23,10 @@ constexpr int BT_FILL = 512;
 // sequences of 700 Q8_0 positions 17.9 / 15.6 / 16.7, 5 x 7 queries of 513 F16 15.2 / 11.9 / 13.4, 5 of 5000 Q4_0 17.2 / 15.2 /
 // 14.3).
 constexpr int BT_STEP = 128;
-// Rows of a KV head up to which the shared positions are left to register workgroups: one pass of them.  Register / tile
-// workgroups and the combine, us, 32768 shared positions: 18 rows Q4_0 29.3 / 35.5, Q8_0 30.4 / 34.8, F16 36.9 / 35.8; 30 rows
-// 32.6 / 35.0, 34.2 / 34.9, 41.3 / 36.5; 36 rows Q4_0 35.4 / 37.1, Q8_0 37.8 / 35.8; 60 rows Q4_0 38.5 / 37.7; 30 rows over 4096
-// Q8_0 positions 18.1 / 20.0.
+// Rows of a KV head up to which the shared positions are left to register workgroups: one pass of them.  Whole call, us,
+// register / tile workgroups, 32768 shared positions: 18 rows Q4_0 40.5 / 47.5, Q8_0 41.7 / 47.7, F16 45.0 / 43.9; 30 rows 43.2 /
+// 47.9, 44.7 / 48.0, 49.1 / 45.4; 36 rows 47.9 / 48.0, 50.9 / 48.5, 50.5 / 45.6; 60 rows 51.2 / 49.2, 53.5 / 50.9, 54.4 / 47.8.
+// 4096: 30 rows 26.3 / 28.6, 27.6 / 28.7, 25.2 / 26.9; 60 rows 31.0 / 31.2, 31.0 / 29.9, 28.1 / 28.6.
 constexpr int BT_FEW = 32;
 
 // The shared positions [0, n_shared) are worked on for all rows together, the positions of its own [n_shared, len) for every
