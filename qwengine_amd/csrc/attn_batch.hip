@@ -20,7 +20,7 @@
 //    out when the scores are done, its V loads when P V is.
 // A batch of one call has the same bits again; another batch, or another cut, sums a row's states in another order.
 // Roundings below 32 bits: the dequantized V (d * code) and the probabilities are fp16 (half a step: 2^-11 of the value, random
-// in sign, as in the prefill: P V then has one MFMA per 32 keys and 16 dims), a tile workgroup's O / l is 16-bit fixed point
+// in sign, as in the prefill: P V then has one MFMA per 32 keys and 16 dims; for the probabilities' range see BT_RAISE), a tile workgroup's O / l is 16-bit fixed point
 // (half a step: 2^-16 of the row's largest, attn_tiles.hpp), the output is fp16.
 #include <type_traits>
 
@@ -30,6 +30,11 @@
 
 namespace qwa {
 
+// The probabilities are exp(s - m) for a reference m that is set BT_RAISE below a row's running maximum, and set again when a
+// score exceeds m by more than BT_HEAD: at most e^11 = 59874, in full fp16 precision down to 2^-14 = e^-9.7, with fewer bits
+// down to 2^-24.  Those that vanish, below 2^-25 = e^-17.3, are e^-24 to e^-28 of the largest: 2^18 of them are less than 2^-17 of
+// a row's sum.  (With m at the maximum itself they were 2^-25 of the largest, and 131071 of them moved an output by 7e-3.)
+constexpr float BT_RAISE = 7.0f, BT_HEAD = 11.0f;
 constexpr int BT_KD = 1;  // K steps read ahead of their MFMAs
 constexpr int BT_VD = 3;  // V fragments in flight
 size_t batch_work_bytes(int n, int nq, int n_shared, int max_len) {
@@ -475,7 +480,7 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
 #pragma unroll
                 for (int kt = 0; kt < KT; kt++) mx = max3f(max3f(mx, S[rt][kt][0], S[rt][kt][1]), S[rt][kt][2], S[rt][kt][3]);
                 mx = rows_max(mx);
-                const float mn = mx > m[rt] + PF_RESCALE_T ? mx : m[rt];
+                const float mn = mx > m[rt] + BT_HEAD ? mx - BT_RAISE : m[rt];
                 const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;  // a row that saw nothing keeps l = 0, O = 0
                 cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] * PF_LOG2E - msl);
                 // the sum is that of the rounded probabilities, the weights that P V applies
@@ -1029,7 +1034,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
                     }
                     float mx = max3f(max3f(-INFINITY, sc[0][0], sc[0][1]), sc[0][2], sc[0][3]);
                     mx = rows_max(max3f(max3f(mx, sc[1][0], sc[1][1]), sc[1][2], sc[1][3]));
-                    const float mn = mx > m + PF_RESCALE_T ? mx : m;
+                    const float mn = mx > m + BT_HEAD ? mx - BT_RAISE : m;
                     const float cr = mn == m ? 1.0f : fast_exp2((m - mn) * PF_LOG2E);
                     const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;
                     m = mn;

@@ -49,3 +49,41 @@ CASES = {"own positions": ([9000, 3001, 12000], 0, 1), "own positions, 8 queries
 def test_outlier_keys(gpu, kvt, case):
     lens, shared, nq = CASES[case]
     Outliers(kvt, lens, shared, page=16 if nq == 7 else 64).check(nq, shared, what=f"{KV_NAMES[kvt]} {case}")
+
+
+@pytest.mark.parametrize("n, nq, shared", [(170, 8, 131072), (128, 1, 0)])
+@pytest.mark.parametrize("kvt", KVTS, ids=lambda k: KV_NAMES[k])
+def test_many_keys_far_below_the_largest_score(gpu, kvt, n, nq, shared):
+    """One key with a score 17.4 above those of 131071 others, as the first token of a prompt may have it: each of the others
+    weighs 2.8e-8, less than half of fp16's least number, but together they move the output from -1 to -0.993.
+
+    The states that hold the first key have the whole range (prefix) or a wave's quarter of it.  Tolerance: an MFMA adds 32
+    keys in at most 4 sums, each off by half a step of 2^-24, O and l alike; the output is off by 2^-12, and the weights of
+    the others, which together are 4e-3, by 2^-9 at most (their fp16 numbers have 9 bits)."""
+    page, pages, most = 64, 64, 131072
+    kv, pg = ops.KVLayer.allocate(kvt, pages * page), ops.KVPages.allocate(n, most, pages, page)
+    K, V = torch.zeros((pages * page, 4, 256), device="cuda"), torch.ones((pages * page, 4, 256), device="cuda")
+    K[0], V[0] = 1.0875, -1.0
+    ops.kv_append(K, V, 0, pages * page, kvt, kv)
+    table = torch.randint(1, pages, (n, most // page), generator=torch.Generator().manual_seed(3), dtype=torch.int32)
+    table[:] = table[:1]
+    table[:, 0] = 0
+    pg.table.copy_(table)
+    pg.len.fill_(most)
+    q, gate = torch.ones((n * nq, 24, 256), device="cuda"), torch.full((n * nq, 24, 256), 30.0, device="cuda")
+    out = torch.empty((n * nq, 24, 256), dtype=torch.float16, device="cuda")
+    work = torch.empty(ops.attn_batch_work_bytes(n, nq, shared, most), dtype=torch.uint8, device="cuda")
+    ops.attn_decode_batch(q, gate, kv, kvt, pg, None, n, nq, shared, most, out, work)
+    torch.cuda.synchronize()
+    b = Batch.__new__(Batch)
+    b.kvt, b.caches, b._rows = kvt, [kv], {}
+    k64, v64 = b.values(0)
+    top, rest = k64[0, 0].sum() / 16, k64[0, 1].sum() / 16
+    assert 17.35 < top - rest < 17.45
+    tol = 8 * (most if shared else most // 4) / 32 * 2.0**-24 + 2.0**-12 + 4e-3 * 2.0**-9
+    for t in range(nq):
+        others = (most - nq + t) * torch.exp(rest - top)
+        want = (v64[0, 0, 0] + others * v64[0, 1, 0]) / (1 + others)
+        err = (out.view(n, nq, 24, 256)[:, t].double().cpu() - want).abs().max().item()
+        print(f"{KV_NAMES[kvt]} {n} x {nq}, query {t}: off by {err:.2e} of {tol:.2e}", flush=True)
+        assert err <= tol
