@@ -131,6 +131,11 @@ __device__ __forceinline__ void add_block(int s, f4& score, const f4& product, f
         default: add_block<7>(score, product, even, odd); break;
     }
 }
+// MFMA results before inline assembly reads them (max3f): the compiler puts the 8 wait states that they need before
+// instructions of its own, but does not look into assembly.  F16 scores are such results (they had 9 by chance); the other
+// types' have passed through their block scales.
+__device__ __forceinline__ void mfma_settle(f4& x) { asm volatile("s_nop 7" : "+v"(x)); }
+__device__ __forceinline__ void mfma_settle(f4& x, f4& y) { asm volatile("s_nop 7" : "+v"(x), "+v"(y)); }
 // Q / 16 = hi + lo, fp16 each
 __device__ __forceinline__ _Float16 q_hi(float x) { return (_Float16)x; }
 __device__ __forceinline__ _Float16 q_lo(float x) { return (_Float16)(x - (float)(_Float16)x); }
@@ -457,6 +462,11 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
                     for (int kt = 0; kt < KT; kt++) add_block(7, S[rt][kt], T[7 & LAG][rt][kt], even[kt], odd[kt]);
             }
             load_ks(nat, nb);
+            if constexpr (!SC) {
+                static_assert(SC || KT == 1, "all scores");
+                if constexpr (RT == 1) mfma_settle(S[0][0]);
+                else mfma_settle(S[0][0], S[1][0]);
+            }
 
             // online softmax: a lane holds keys kb + 16 kt + 4 lg + i of row i16
             bool masked = kb < seg.lo || kb + TILE > vmin;
@@ -1024,6 +1034,8 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
                     if constexpr (SC) {
                         scale(7, 0);
                         scale(7, 1);
+                    } else {
+                        mfma_settle(sc[0], sc[1]);
                     }
                     if (k0 + PF_TILE > vmin || (dead & 3) != 0) {
 #pragma unroll
