@@ -194,20 +194,20 @@ size_t qwa_kv_pages_work_bytes(const qwa_kv_pages* p);
  * page that other sequences hold too is replaced by a copy first, in every layer of `layers` (host array of n_layers
  * pools of type kvt), since the new positions would be written into it; the last of its holders keeps the page.
  * All or nothing: *status (device) becomes 0 when done; the number of missing pages when the free pages do not suffice;
- * -(i + 1) when request i is invalid (no such sequence, named before, add < 0, past ld * page positions).  In the last
- * two cases nothing is changed.  The new positions hold old bytes until a prep or an append writes them. */
+ * -(i + 1) when request i is invalid (no such sequence, named before, add < 0, past ld * page positions; or a broken
+ * table: len < 0, or the partly filled last page is none of the pool's).  In the last two cases nothing is changed.  The new positions hold old bytes until a prep or an append writes them. */
 int qwa_kv_pages_extend(const qwa_kv_pages* p, const int* seqs, const int* add, int n, const qwa_kv_layer* layers,
                         int n_layers, int kvt, int* status, void* work, void* stream);
 
 /* Sequence dst[i] becomes a fork of sequence src[i], all at once (every request sees the tables as they were before the
  * call, so beams may be permuted): it gives back its own pages and holds src[i]'s, which are shared, not copied.
- * src[i] < 0 leaves dst[i] empty.  A request whose src or dst is no sequence is ignored; of several with the same dst
- * the last one counts.  n <= n_seq. */
+ * src[i] < 0 leaves dst[i] empty.  A request whose src or dst is no sequence is ignored; of several others with the same
+ * dst the last one counts.  n <= n_seq. */
 int qwa_kv_pages_fork(const qwa_kv_pages* p, const int* src, const int* dst, int n, void* work, void* stream);
 
 /* Sequence seqs[i] keeps its first lens[i] positions (lens NULL: none, which frees it) and gives back the pages past
- * them.  A request that names no sequence, or a length outside [0, len], is ignored; of several for one sequence the
- * last one counts. */
+ * them.  A request that names no sequence, or a length outside [0, len], is ignored; of several others for one
+ * sequence the last one counts. */
 int qwa_kv_pages_trim(const qwa_kv_pages* p, const int* seqs, const int* lens, int n, void* stream);
 
 /* Moves the pages in use to the front of the pool: afterwards they are pages 0 .. *n_live - 1 (n_live: device).  The

@@ -308,8 +308,9 @@ struct PageSum {
     }
 };
 
-// which of the workgroup's requests [i0, i0 + PG_CH) are repeated by a later one (bit k: request i0 + k gives way)
-__device__ __forceinline__ uint32_t repeated(const int* __restrict__ seqs, int n, int i0, uint32_t* s_mask) {
+// which of the workgroup's requests [i0, i0 + PG_CH) are repeated by a later one that counts (bit k: request i0 + k gives way)
+template <class COUNTS>
+__device__ __forceinline__ uint32_t repeated(const int* __restrict__ seqs, int n, int i0, uint32_t* s_mask, COUNTS counts) {
     if (threadIdx.x == 0) *s_mask = 0;
     __syncthreads();
     constexpr int L = PG_RT / PG_CH;  // threads per request
@@ -317,7 +318,7 @@ __device__ __forceinline__ uint32_t repeated(const int* __restrict__ seqs, int n
     bool later = false;
     if (i < n) {
         const int s = seqs[i];
-        for (int j = i + 1 + (int)(threadIdx.x % L); j < n; j += L) later |= seqs[j] == s;
+        for (int j = i + 1 + (int)(threadIdx.x % L); j < n; j += L) later |= seqs[j] == s && counts(j);
     }
     if (later) atomicOr(s_mask, 1u << k);
     __syncthreads();
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(PG_RT) k_fork_stage(qwa_kv_pages p, const int*
     __shared__ uint32_t s_mask;
     __shared__ int s_src[PG_CH], s_k[PG_CH];
     const int i0 = blockIdx.x * PG_CH, t = threadIdx.x;
-    const uint32_t gone = repeated(dst, n, i0, &s_mask);
+    const uint32_t gone = repeated(dst, n, i0, &s_mask, [&](int j) { return src[j] < p.n_seq; });
     if (t < PG_CH) {
         const int i = i0 + t;
         int s = -1, k = -1, m = 0;
@@ -405,7 +406,12 @@ __global__ void __launch_bounds__(PG_RT) k_trim(qwa_kv_pages p, const int* __res
     __shared__ uint32_t s_mask;
     __shared__ int s_seq[PG_CH], s_keep[PG_CH], s_old[PG_CH];
     const int i0 = blockIdx.x * PG_CH, t = threadIdx.x;
-    const uint32_t gone = repeated(seqs, n, i0, &s_mask);
+    // (Another workgroup may be cutting len[s] meanwhile, to the length of the last request that counts.  That one counts
+    // before and after; those behind it, longer than the sequence or negative, do not; those before it give way to it.)
+    const uint32_t gone = repeated(seqs, n, i0, &s_mask, [&](int j) {
+        const int s = seqs[j], to = lens ? lens[j] : 0;
+        return s >= 0 && s < p.n_seq && to >= 0 && to <= p.len[s];
+    });
     if (t < PG_CH) {
         const int i = i0 + t;
         int s = 0, keep = 0, old = 0;
