@@ -186,7 +186,8 @@ typedef struct {
 
 /* Bytes of the `work` buffer of the page operators on these tables (device memory, 16-byte aligned; 0: invalid tables).
  * Calls that may run at the same time need a buffer each, as do captured graphs whose replays may overlap.  The tables
- * themselves are one state: calls that change them, and calls that read them, have to be ordered (one stream, or events). */
+ * themselves are one state: calls that change them, and calls that read them, have to be ordered (one stream, or events).
+ * A call whose work_bytes is smaller than this is refused. */
 size_t qwa_kv_pages_work_bytes(const qwa_kv_pages* p);
 
 /* Room for add[i] more positions of sequence seqs[i] (device arrays of n entries): len grows by add[i], and the pages
@@ -197,13 +198,14 @@ size_t qwa_kv_pages_work_bytes(const qwa_kv_pages* p);
  * -(i + 1) when request i is invalid (no such sequence, named before, add < 0, past ld * page positions; or a broken
  * table: len < 0, or the partly filled last page is none of the pool's).  In the last two cases nothing is changed.  The new positions hold old bytes until a prep or an append writes them. */
 int qwa_kv_pages_extend(const qwa_kv_pages* p, const int* seqs, const int* add, int n, const qwa_kv_layer* layers,
-                        int n_layers, int kvt, int* status, void* work, void* stream);
+                        int n_layers, int kvt, int* status, void* work, size_t work_bytes, void* stream);
 
 /* Sequence dst[i] becomes a fork of sequence src[i], all at once (every request sees the tables as they were before the
  * call, so beams may be permuted): it gives back its own pages and holds src[i]'s, which are shared, not copied.
  * src[i] < 0 leaves dst[i] empty.  A request whose src or dst is no sequence is ignored; of several others with the same
  * dst the last one counts.  n <= n_seq. */
-int qwa_kv_pages_fork(const qwa_kv_pages* p, const int* src, const int* dst, int n, void* work, void* stream);
+int qwa_kv_pages_fork(const qwa_kv_pages* p, const int* src, const int* dst, int n, void* work, size_t work_bytes,
+                      void* stream);
 
 /* Sequence seqs[i] keeps its first lens[i] positions (lens NULL: none, which frees it) and gives back the pages past
  * them.  A request that names no sequence, or a length outside [0, len], is ignored; of several others for one
@@ -214,7 +216,7 @@ int qwa_kv_pages_trim(const qwa_kv_pages* p, const int* seqs, const int* lens, i
  * pages below that bound stay; the i-th page in use above it moves to the i-th free one below it, in every layer, and
  * every sequence's table follows. */
 int qwa_kv_pages_compact(const qwa_kv_pages* p, const qwa_kv_layer* layers, int n_layers, int kvt, int* n_live,
-                         void* work, void* stream);
+                         void* work, size_t work_bytes, void* stream);
 
 /* qwa_attn_prep_multi for a batch: row r = b * nq + t of qg / k / v / q_out / gate belongs to query t of batch row b,
  * whose sequence is seqs[b] (device; NULL: b) and whose position is len - nq + t, the last nq positions that the

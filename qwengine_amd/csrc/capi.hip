@@ -403,6 +403,15 @@ int check_layers(const qwa_kv_layer* layers, int n_layers, int kvt, const qwa_kv
     return QWA_OK;
 }
 
+int check_pages_work(const qwa_kv_pages* p, const void* work, size_t work_bytes, const char* fn) {
+    if (!work) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if (!al16(work)) return fail(QWA_ERR_INVALID, "%s: work not 16-byte aligned", fn);
+    const size_t need = qwa::pages_work_bytes(*p);
+    if (work_bytes < need)
+        return fail(QWA_ERR_RANGE, "%s: workspace of %zu bytes, the call needs %zu", fn, work_bytes, need);
+    return QWA_OK;
+}
+
 int check_requests(int n, const char* fn) {
     if (n < 0 || n > QWA_PAGES_MAXN) return fail(QWA_ERR_RANGE, "%s: %d requests (0..%d)", fn, n, QWA_PAGES_MAXN);
     return QWA_OK;
@@ -422,26 +431,27 @@ int check_batch(const qwa_kv_pages* p, const int* seqs, int n, int nq, const cha
 size_t qwa_kv_pages_work_bytes(const qwa_kv_pages* p) { return pages_ok(p) ? qwa::pages_work_bytes(*p) : 0; }
 
 int qwa_kv_pages_extend(const qwa_kv_pages* p, const int* seqs, const int* add, int n, const qwa_kv_layer* layers,
-                        int n_layers, int kvt, int* status, void* work, void* stream) {
+                        int n_layers, int kvt, int* status, void* work, size_t work_bytes, void* stream) {
     const char* fn = "kv_pages_extend";
     int st;
     if ((st = check_pages(p, fn)) || (st = check_requests(n, fn)) ||
         (st = check_layers(layers, n_layers, kvt, p, fn)))
         return st;
-    if (!status || !work || (n > 0 && (!seqs || !add))) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
-    if (!al16(work)) return fail(QWA_ERR_INVALID, "%s: work not 16-byte aligned", fn);
+    if (!status || (n > 0 && (!seqs || !add))) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if ((st = check_pages_work(p, work, work_bytes, fn))) return st;
     return from_hip(qwa::launch_pages_extend(*p, seqs, add, n, layers, n_layers, kvt, status, work, as_stream(stream)), fn);
 }
 
-int qwa_kv_pages_fork(const qwa_kv_pages* p, const int* src, const int* dst, int n, void* work, void* stream) {
+int qwa_kv_pages_fork(const qwa_kv_pages* p, const int* src, const int* dst, int n, void* work, size_t work_bytes,
+                      void* stream) {
     const char* fn = "kv_pages_fork";
     int st;
     if ((st = check_pages(p, fn)) || (st = check_requests(n, fn))) return st;
     // (the work buffer stages a row per request)
     if (n > p->n_seq) return fail(QWA_ERR_RANGE, "%s: %d requests for %d sequences", fn, n, p->n_seq);
     if (n == 0) return QWA_OK;
-    if (!src || !dst || !work) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
-    if (!al16(work)) return fail(QWA_ERR_INVALID, "%s: work not 16-byte aligned", fn);
+    if (!src || !dst) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if ((st = check_pages_work(p, work, work_bytes, fn))) return st;
     return from_hip(qwa::launch_pages_fork(*p, src, dst, n, work, as_stream(stream)), fn);
 }
 
@@ -455,12 +465,12 @@ int qwa_kv_pages_trim(const qwa_kv_pages* p, const int* seqs, const int* lens, i
 }
 
 int qwa_kv_pages_compact(const qwa_kv_pages* p, const qwa_kv_layer* layers, int n_layers, int kvt, int* n_live,
-                         void* work, void* stream) {
+                         void* work, size_t work_bytes, void* stream) {
     const char* fn = "kv_pages_compact";
     int st;
     if ((st = check_pages(p, fn)) || (st = check_layers(layers, n_layers, kvt, p, fn))) return st;
-    if (!n_live || !work) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
-    if (!al16(work)) return fail(QWA_ERR_INVALID, "%s: work not 16-byte aligned", fn);
+    if (!n_live) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if ((st = check_pages_work(p, work, work_bytes, fn))) return st;
     return from_hip(qwa::launch_pages_compact(*p, layers, n_layers, kvt, n_live, work, as_stream(stream)), fn);
 }
 

@@ -110,13 +110,14 @@ EXPORTS = {
                                      ctypes.c_void_p]),
     "qwa_kv_pages_work_bytes": (ctypes.c_size_t, [ctypes.POINTER(_KVPagesC)]),
     "qwa_kv_pages_extend": (ctypes.c_int, [ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
-                            [ctypes.c_int, ctypes.POINTER(_KVLayerC)] + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 3),
+                            [ctypes.c_int, ctypes.POINTER(_KVLayerC)] + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 2 +
+                            [ctypes.c_size_t, ctypes.c_void_p]),
     "qwa_kv_pages_fork": (ctypes.c_int, [ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
-                          [ctypes.c_int] + [ctypes.c_void_p] * 2),
+                          [ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "qwa_kv_pages_trim": (ctypes.c_int, [ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
                           [ctypes.c_int, ctypes.c_void_p]),
     "qwa_kv_pages_compact": (ctypes.c_int, [ctypes.POINTER(_KVPagesC), ctypes.POINTER(_KVLayerC)] +
-                             [ctypes.c_int] * 2 + [ctypes.c_void_p] * 3),
+                             [ctypes.c_int] * 2 + [ctypes.c_void_p] * 2 + [ctypes.c_size_t, ctypes.c_void_p]),
     "qwa_attn_prep_batch": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.POINTER(_KVPagesC), ctypes.c_void_p] +
                             [ctypes.c_int] * 2 + [ctypes.c_void_p] + [ctypes.c_float] * 2 +
                             [ctypes.c_int, ctypes.POINTER(_KVLayerC)] + [ctypes.c_void_p] * 3),
@@ -536,12 +537,9 @@ def _layers(layers, kvt):
     return arr, n
 
 
-def _work(pc, work) -> int | None:
-    if isinstance(work, torch.Tensor):
-        need = lib().qwa_kv_pages_work_bytes(pc)
-        if work.numel() * work.element_size() < need:
-            raise QwaError(f"workspace of {work.numel() * work.element_size()} bytes, the call needs {need}")
-    return _dev(work, None, "work")
+def _work(work) -> tuple:
+    """A workspace and its size (a raw pointer's is the caller's word)."""
+    return _dev(work, None, "work"), work.numel() * work.element_size() if isinstance(work, torch.Tensor) else 1 << 62
 
 
 def kv_pages_work_bytes(pages: KVPages) -> int:
@@ -555,14 +553,14 @@ def kv_pages_extend(pages: KVPages, seqs, add, layers, kvt, status, work, n: int
     arr, nl = _layers(layers, kvt)
     pc = ctypes.byref(pages.c())
     _check(lib().qwa_kv_pages_extend(pc, _count(seqs, n, "seqs"), _count(add, n, "add"), n, arr, nl, kvt,
-                                     _count(status, 1, "status"), _work(pc, work), _stream(stream)))
+                                     _count(status, 1, "status"), *_work(work), _stream(stream)))
 
 
 def kv_pages_fork(pages: KVPages, src, dst, work, n: int | None = None, stream=None) -> None:
     """Sequence dst[i] gives back its pages and shares src[i]'s (src[i] < 0: becomes empty), all requests at once."""
     n = dst.numel() if n is None else n
     pc = ctypes.byref(pages.c())
-    _check(lib().qwa_kv_pages_fork(pc, _count(src, n, "src"), _count(dst, n, "dst"), n, _work(pc, work), _stream(stream)))
+    _check(lib().qwa_kv_pages_fork(pc, _count(src, n, "src"), _count(dst, n, "dst"), n, *_work(work), _stream(stream)))
 
 
 def kv_pages_trim(pages: KVPages, seqs, lens=None, n: int | None = None, stream=None) -> None:
@@ -577,8 +575,7 @@ def kv_pages_compact(pages: KVPages, layers, kvt, n_live, work, stream=None) -> 
     kvt = _kvt(kvt)
     arr, nl = _layers(layers, kvt)
     pc = ctypes.byref(pages.c())
-    _check(lib().qwa_kv_pages_compact(pc, arr, nl, kvt, _count(n_live, 1, "n_live"), _work(pc, work),
-                                      _stream(stream)))
+    _check(lib().qwa_kv_pages_compact(pc, arr, nl, kvt, _count(n_live, 1, "n_live"), *_work(work), _stream(stream)))
 
 
 def attn_prep_batch(qg, k, v, q_norm, k_norm, pages: KVPages, seqs, n: int, nq: int, theta: float, eps: float, kvt,
@@ -608,8 +605,7 @@ def attn_decode_batch(q, gate, kv: KVLayer, kvt, pages: KVPages, seqs, n: int, n
     _check(lib().qwa_attn_decode_batch(
         _dev(q, f32, "q", size), _dev(gate, f32, "gate", size), _pool(kv, kvt), kvt, ctypes.byref(pages.c()),
         None if seqs is None else _count(seqs, n, "seqs"), n, nq, n_shared, max_len,
-        _dev(out16, torch.float16, "out16", size), _act(oq), _dev(work, what="work"),
-        work.numel() * work.element_size() if isinstance(work, torch.Tensor) else 1 << 62, _stream(stream)))
+        _dev(out16, torch.float16, "out16", size), _act(oq), *_work(work), _stream(stream)))
 
 
 # ---- Gated DeltaNet ------------------------------------------------------------------------------------------------
