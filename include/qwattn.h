@@ -239,7 +239,9 @@ size_t qwa_attn_batch_work_bytes(int n, int nq, int n_shared, int max_len);
  * n_shared: the batch rows have their first n_shared positions in common (forks of one prompt; 0: nothing).  Their keys
  * are read once for all rows, through the table of the longest row (the first of those); a shorter row sees as many of
  * them as it has positions.
- * max_len >= n_shared bounds every row's len: positions from max_len on are not seen.
+ * max_len >= n_shared is a bound of the rows' lens.  A sequence that is longer counts as one of max_len positions, as if
+ * qwa_kv_pages_trim had cut it: query t sees [0, max_len - nq + t].  (Its last nq positions, which prep stored, are then not
+ * those of the queries: a captured call needs a max_len that its sequences do not outgrow.)
  * A row that sees no position (an empty or unknown sequence, a query before the first position) gets zeros; positions
  * whose page is none of the pool's are not seen.  Pool bytes past a sequence's last position are never used.  A K or V
  * value that is not finite shows in the rows that see it, and may show in those that do not, but share its 32 positions

@@ -58,7 +58,8 @@ struct BatchArgs {
     int n, nq, n_shared, max_len, wgs;
 };
 
-// positions of batch row b, cut to max_len; 0 for an unknown sequence
+// positions of batch row b, 0 for an unknown sequence.  A longer sequence counts as one of max_len positions, for its queries'
+// limits as for the key ranges.
 __device__ __forceinline__ int bt_seq(const BatchArgs& a, int b) { return a.seqs ? a.seqs[b] : b; }
 __device__ __forceinline__ int bt_len(const BatchArgs& a, const qwa_kv_pages& p, int b) {
     const int s = bt_seq(a, b);

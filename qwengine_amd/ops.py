@@ -597,7 +597,8 @@ def attn_batch_work_bytes(n: int, nq: int, n_shared: int, max_len: int) -> int:
 def attn_decode_batch(q, gate, kv: KVLayer, kvt, pages: KVPages, seqs, n: int, nq: int, n_shared: int, max_len: int, out16,
                       work, oq: ActQ8 | None = None, stream=None) -> None:
     """Attention of n sequences (seqs int32, None: 0..n-1) with nq queries each over a paged cache; the first n_shared
-    positions, which all of them have in common, are read once.  out16: fp16 [n * nq, 6144]."""
+    positions, which all of them have in common, are read once.  max_len bounds the lengths: a longer sequence counts as one
+    of max_len positions.  out16: fp16 [n * nq, 6144]."""
     f32, kvt, size = torch.float32, _kvt(kvt), n * nq * 6144
     if oq is not None:
         for x, dt, m, what in ((oq.q, torch.int8, size, "oq.q"), (oq.d, f32, size // 32, "oq.d"), (oq.s, f32, size // 32, "oq.s")):
