@@ -2,9 +2,9 @@
 //
 // For row r = (token, head) with q_r, and its keys K_j, V_j:  out = sum_j exp(s_j - m) V_j / sum_j exp(s_j - m) *
 // sigmoid(gate), s_j = q_r . K_j / 16.  The sum splits over any partition of the keys into partial states (m, l, O), so the
-// positions that all sequences share are worked on for the rows of all sequences together, those of its own for each
-// sequence by itself, both in ranges of fixed length (batch_plan.hpp), and k_bt_combine joins a row's states in a fixed
-// order.
+// positions that all sequences share are worked on for the rows of all sequences together, in ranges of fixed length, those
+// of its own for each sequence by itself, in equal slices of all sequences' positions (batch_plan.hpp), and k_bt_combine joins a
+// row's states in a fixed order.
 //  * Register workgroups (k_bt_own, and k_bt_shared for the shared positions of few rows) have one KV head and up to
 //    BT_MAXRT 16-row tiles (row 6 * token + head of that KV head); their waves take the tiles of the key range in turn, each
 //    with its own running maximum, sum and O, and merge at the end through LDS.
@@ -597,22 +597,19 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
     }
 }
 
-// the shared positions, for the rows of one group: workgroup = (key range, KV head, row group)
+// the shared positions, for up to BT_FEW rows of a KV head: workgroup = (key range, KV head)
 template <int KVT, int RT>
 __global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
-k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int ns, int len, int groups) {
+k_bt_shared(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int len) {
     __shared__ BtLds<KVT, RT> lds;
-    // the groups of one (range, head) read the same keys: workgroups 8 apart, which one XCD runs
-    const int u = blockIdx.x / (8 * groups) * 8 + blockIdx.x % 8, grp = blockIdx.x / 8 % groups;
-    const int g = u % NKV, sp = u / NKV;
-    if (sp >= ns) return;
+    const int g = blockIdx.x % NKV, sp = blockIdx.x / NKV;
     const int b = bt_longest(a, p, threadIdx.x & 63);
     const int k1 = min(min((sp + 1) * len, a.n_shared), bt_len(a, p, b));
     const int seq = bt_seq(a, b);
     const int* table = p.table + (seq >= 0 && seq < p.n_seq ? (size_t)seq * p.ld : 0);
     const size_t rec = (size_t)sp * a.n * a.nq * NH + g * GRP;
     bt_body<KVT, RT>(lds, a, kv, p, g,
-                     {table, grp * 16 * RT, a.n * a.nq * GRP, sp * len, k1, 0, a.part_o + rec * HD, a.part_ml + rec, NH},
+                     {table, 0, a.n * a.nq * GRP, sp * len, k1, 0, a.part_o + rec * HD, a.part_ml + rec, NH},
                      [](BtSegment&) { return false; });
 }
 
@@ -1129,8 +1126,8 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
 // a time.
 // The states' bytes and a chain of dependent loads bound it: 768 rows of 64 fixed-point and 5 fp32 states 10.6 us (31 MB).
 template <int WPR>
-__global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, qwa_kv_pages p, const float* __restrict__ gate, int nt,
-                                                    int ns_shared, uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {
+__global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, const float* __restrict__ gate, int nt, int ns_shared,
+                                                    uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {
     __shared__ float4 s_o[WPR > 1 ? 4 : 1][64];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), part = wave % WPR, lane = threadIdx.x & 63;
     const int row = blockIdx.x * (4 / WPR) + wave / WPR;
@@ -1271,9 +1268,8 @@ static void launch_ranges(const BatchArgs& a, const qwa_kv_layer& kv, const qwa_
     if (b.nt > 0)
         hipLaunchKernelGGL(k_bt_tiles<KVT>, dim3(b.blocks * b.nt * NKV), dim3(64 * BT_TWAVES), 0, st, a, kv, p, b.blocks, b.nt);
     if (b.ns_shared > 0) {
-        const int grid = (b.ns_shared * NKV + 7) / 8 * 8 * b.groups_shared;
-        if (b.rt_shared == 1) QWA_BT(k_bt_shared, 1, grid, b.ns_shared, b.len_shared, b.groups_shared);
-        else QWA_BT(k_bt_shared, 2, grid, b.ns_shared, b.len_shared, b.groups_shared);
+        if (b.rt_shared == 1) QWA_BT(k_bt_shared, 1, b.ns_shared * NKV, b.len_shared);
+        else QWA_BT(k_bt_shared, 2, b.ns_shared * NKV, b.len_shared);
     }
     if (b.wgs > 0) {
         const int grid = (b.wgs * NKV + 7) / 8 * 8 * b.groups;
@@ -1303,10 +1299,10 @@ hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_l
     // 66 12.7 / 8.8, 48 of 97 14.0 / 7.4; 576 of 10 5.2 / 5.5, those of 128 sequences of 19 11.0 / 19.2, 9600 of 2 11.6 / 29.2)
     const int rows = n * nq * NH, states = b.nt + b.ns_shared + (b.wgs > 0 ? b.wgs / n + 1 : 0);
     if (states > 24)
-        hipLaunchKernelGGL(k_bt_combine<4>, dim3(rows), dim3(256), 0, st, a, p, gate, b.nt, b.ns_shared, out16, act,
+        hipLaunchKernelGGL(k_bt_combine<4>, dim3(rows), dim3(256), 0, st, a, gate, b.nt, b.ns_shared, out16, act,
                            oq != nullptr ? 1 : 0);
     else
-        hipLaunchKernelGGL(k_bt_combine<1>, dim3((rows + 3) / 4), dim3(256), 0, st, a, p, gate, b.nt, b.ns_shared, out16,
+        hipLaunchKernelGGL(k_bt_combine<1>, dim3((rows + 3) / 4), dim3(256), 0, st, a, gate, b.nt, b.ns_shared, out16,
                            act, oq != nullptr ? 1 : 0);
     return hipGetLastError();
 }

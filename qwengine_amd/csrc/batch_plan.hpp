@@ -38,23 +38,11 @@ constexpr int BT_FEW = 32;
 //  one segment per sequence that it meets.
 struct BatchPlan {
     int blocks, nt;                // row blocks and key ranges of the tile workgroups (0: none)
-    int groups_shared, rt_shared;  // row groups of the batch, and the row tiles of a group
+    int groups_shared, rt_shared;  // passes of register workgroups that the batch's rows would take (where they run: 1), their row tiles
     int ns_shared, len_shared;     // key ranges of register workgroups over the shared positions, and their length
     int groups, rt_own;            // row groups of a sequence, and the row tiles of a group
     int wgs;                       // slices of the own steps (0: no own positions)
 };
-
-inline void bt_cut(int positions, int units, int fill, int most, int* ns, int* len) {
-    if (positions <= 0) {
-        *ns = 0;
-        *len = BT_STEP;
-        return;
-    }
-    const int steps = (positions + BT_STEP - 1) / BT_STEP;
-    const int want = std::min(std::min(most, steps), std::max(1, fill / units));
-    *len = (steps + want - 1) / want * BT_STEP;
-    *ns = (positions + *len - 1) / *len;
-}
 
 inline BatchPlan batch_plan(int n, int nq, int n_shared, int max_len) {
     BatchPlan p = {};
@@ -67,9 +55,11 @@ inline BatchPlan batch_plan(int n, int nq, int n_shared, int max_len) {
         const int tiles = (n_shared + PF_TILE - 1) / PF_TILE;
         p.blocks = (rows + BT_TROWS - 1) / BT_TROWS;
         p.nt = std::min(tiles, std::max(1, 256 / (p.blocks * NKV)));
-        p.len_shared = BT_STEP;
-    } else {
-        bt_cut(n_shared, p.groups_shared * NKV, BT_FILL, 128, &p.ns_shared, &p.len_shared);
+    } else if (n_shared > 0) {
+        static_assert(BT_FEW <= 16 * BT_MAXRT, "one pass");
+        const int steps = (n_shared + BT_STEP - 1) / BT_STEP, most = std::min(steps, BT_FILL / NKV);
+        p.len_shared = (steps + most - 1) / most * BT_STEP;
+        p.ns_shared = (n_shared + p.len_shared - 1) / p.len_shared;
     }
     if (max_len > n_shared) {
         const long long steps = (long long)n * ((max_len - (n_shared & ~15) + BT_STEP - 1) / BT_STEP);
