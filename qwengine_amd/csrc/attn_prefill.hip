@@ -32,7 +32,11 @@ namespace qwa {
 #ifndef QWA_PF_XCD
 #define QWA_PF_XCD 1
 #endif
+constexpr int PF_THREADS = PF_WAVES * 64;
 constexpr int PF_WPE = PF_WAVES / 4;             // waves per SIMD
+constexpr int PF_KT = PF_TILE / 16;              // 16-key MFMA tiles per tile
+constexpr int KS_LD = HD + 8;                    // K tile row stride (halves)
+constexpr int VT_LD = PF_TILE + 8;               // V^T tile row stride (halves)
 #ifndef QWA_PF_VD
 #define QWA_PF_VD 3
 #endif
@@ -45,12 +49,33 @@ constexpr int PF_KPF = QWA_PF_KPF;               // score steps of K fragments r
 #define QWA_PF_GROUP_BIT 4
 #endif
 constexpr int PF_GROUP_BIT = QWA_PF_GROUP_BIT;   // wave bit that tells the two waves of a SIMD apart
+constexpr float PF_RESCALE_T = 8.0f;  // lazy-rescale threshold on the running maximum (natural-log units)
 
 // Partial softmax states of one pass live in the caller's workspace: per split and output row
 // (row = token * NH + head, ps rows per split) O / l as 16-bit fixed point [split][row][HD] against the row's largest
 // |O / l| (pack16x4; absolute error <= that maximum * 2^-16) and (m, l, scale) as fp32 [split][row]; the combine
 // reweights them by l * exp(m - M).  (fp16 partials would add a third fp16 rounding, up to 2^-12 |O|, on top of the
 // fp16 P and output of the reference's own MMA kernel: measured above the tolerance.)
+
+// raw bytes of one tile in LDS, in the cache's own layout: K rows, V rows, K scales, V scales (8 fp16 per row)
+template <int KVT> struct PfRaw {
+    static constexpr int VB = value_bytes(KVT);
+    static constexpr int K = 0, V = PF_TILE * VB;
+    static constexpr int SC = KVT == QWA_KV_F16 ? 0 : PF_TILE * 16;
+    static constexpr int KS = 2 * PF_TILE * VB, VS = KS + SC;
+    static constexpr int BYTES = 2 * PF_TILE * VB + 2 * SC;
+    static constexpr int NKV = PF_TILE * VB / 1024;          // 1 KB load instructions for K (and for V)
+    static constexpr int NBUF = KVT == QWA_KV_F16 ? 2 : 3;   // raw tiles in flight (F16 tiles are 32 KB)
+    static constexpr int AHEAD = NBUF - 1;                    // tiles loaded ahead of the one being computed
+    // load instructions of wave w per tile: K instruction i on wave i % W, V instruction i on wave (i + W / 2) % W,
+    // K scales (two 256-byte instructions) on waves W - 2, W - 1, V scales on waves W / 2 - 2, W / 2 - 1
+    __device__ static constexpr int count(int w) {
+        int n = 0;
+        for (int i = 0; i < NKV; i++) n += (i % PF_WAVES == w) + ((i + PF_WAVES / 2) % PF_WAVES == w);
+        if (SC) n += (w >= PF_WAVES - 2) + (w >= PF_WAVES / 2 - 2 && w < PF_WAVES / 2);
+        return n;
+    }
+};
 
 // Issues this wave's direct-to-LDS loads of the tile starting at key k0: K instructions wave, wave + 8, ..., V
 // instructions (wave + 4) % 8, + 8, ..., scales on waves 2, 3 (V) and 6, 7 (K).  Keys past kmax re-read row kmax
@@ -82,6 +107,123 @@ __device__ __forceinline__ void pf_issue(uint32_t raw, const qwa_kv_layer& kv, s
         if (wave >= PF_WAVES - 2) dma_sv<4>(raw + L::KS + 256 * j, kv.ks + (rowbase + k0) * 8, off);
         if (wave >= PF_WAVES / 2 - 2 && wave < PF_WAVES / 2)
             dma_sv<4>(raw + L::VS + 256 * j, kv.vs + (rowbase + k0) * 8, off);
+    }
+}
+
+// waits until at most n of this wave's direct-to-LDS loads are outstanding (n is wave-uniform)
+__device__ __forceinline__ void wait_vm(int n) {
+    switch (n) {
+        case 0: wait_vmcnt<0>(); break;
+        case 1: wait_vmcnt<1>(); break;
+        case 2: wait_vmcnt<2>(); break;
+        case 3: wait_vmcnt<3>(); break;
+        case 4: wait_vmcnt<4>(); break;
+        case 5: wait_vmcnt<5>(); break;
+        case 6: wait_vmcnt<6>(); break;
+        case 7: wait_vmcnt<7>(); break;
+        case 8: wait_vmcnt<8>(); break;
+        case 9: wait_vmcnt<9>(); break;
+        case 10: wait_vmcnt<10>(); break;
+        case 11: wait_vmcnt<11>(); break;
+        case 12: wait_vmcnt<12>(); break;
+        default: wait_vmcnt<0>(); break;
+    }
+}
+
+// 4 dims of one V key as two half2 {d0, d1}, {d2, d3}, scaled by the key's block scale (one fp16 rounding)
+template <int KVT>
+__device__ __forceinline__ void pf_v4(const uint8_t* vrow, int dc, uint32_t sc, uint32_t* out) {
+    if constexpr (KVT == QWA_KV_F16) {
+        const uint2 u = *reinterpret_cast<const uint2*>(vrow + 8 * dc);
+        out[0] = u.x;
+        out[1] = u.y;
+    } else if constexpr (KVT == QWA_KV_Q8_0) {
+        const h2 d = scale_pair((uint16_t)sc, (uint16_t)sc);
+        q8_word_to_h4(*reinterpret_cast<const uint32_t*>(vrow + 4 * dc), d, out);
+    } else {
+        const h2 d = scale_pair((uint16_t)sc, (uint16_t)sc);
+        const h2 bias = {(_Float16)1032.0f, (_Float16)1032.0f};
+        const uint32_t x = *reinterpret_cast<const uint16_t*>(vrow + 2 * dc);
+        // byte 0 -> dims 0 (low nibble), 1 (high nibble); byte 1 -> dims 2, 3
+        const uint32_t p01 = ((x & 0x0Fu) | ((x & 0xF0u) << 12)) | 0x64006400u;
+        const uint32_t p23 = (((x >> 8) & 0x0Fu) | (((x >> 8) & 0xF0u) << 12)) | 0x64006400u;
+        out[0] = h2_bits((bits_h2(p01) - bias) * d);
+        out[1] = h2_bits((bits_h2(p23) - bias) * d);
+    }
+}
+
+// Dequantises one raw tile into the fp16 tiles (thread t of 512).  K: LDS position 32 s + 8 g + j of a row holds dim
+// 32 s + 8 g + perm(j) (the Q operand is loaded with the same permutation).  V^T: row d, position 8 cb + j holds key
+// 16 (j / 4) + 4 cb + j % 4, the key order of the P^T operand (lane group g of a 16-key MFMA tile holds keys
+// 4 g .. 4 g + 3).
+template <int KVT>
+__device__ __forceinline__ void pf_convert_kv(const uint8_t* raw, _Float16* Ks, _Float16* Vt, int t, bool do_k,
+                                              bool do_v) {
+    using L = PfRaw<KVT>;
+    constexpr int VB = L::VB;
+    const uint16_t* kss = reinterpret_cast<const uint16_t*>(raw + L::KS);
+    const uint16_t* vss = reinterpret_cast<const uint16_t*>(raw + L::VS);
+    if (!do_k) {
+    } else if constexpr (KVT == QWA_KV_F16) {
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int idx = t + 512 * c, key = idx >> 5, pc = idx & 31;
+            *reinterpret_cast<uint4*>(Ks + key * KS_LD + 8 * pc) =
+                *reinterpret_cast<const uint4*>(raw + L::K + key * VB + 16 * pc);
+        }
+    } else if constexpr (KVT == QWA_KV_Q8_0) {
+        const int key = t >> 4, pc = t & 15;
+        const uint4 u = *reinterpret_cast<const uint4*>(raw + L::K + key * VB + 16 * pc);
+        const uint16_t sc = kss[key * 8 + (pc >> 1)];
+        const h2 d = scale_pair(sc, sc);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) q8_word_to_h4(w[i], d, o + 2 * i);
+        *reinterpret_cast<uint4*>(Ks + key * KS_LD + 16 * pc) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(Ks + key * KS_LD + 16 * pc + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+    } else {
+        if (t < PF_TILE * 8) {
+            const int key = t >> 3, pc = t & 7;
+            const uint4 u = *reinterpret_cast<const uint4*>(raw + L::K + key * VB + 16 * pc);
+            const uint16_t sc = kss[key * 8 + pc];
+            const h2 d = scale_pair(sc, sc);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t o[4];
+                q4_word_to_h8(w[i], d, o);
+                *reinterpret_cast<uint4*>(Ks + key * KS_LD + 32 * pc + 8 * i) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+    }
+    if (!do_v) return;
+    // V^T: thread (cb, dc, h) converts keys 16 h + 4 cb + jj (jj < 4), dims 4 dc .. 4 dc + 3
+    const int cb = t & 3, dc = (t >> 2) & 63, h = t >> 8;
+    uint32_t hv[4][2];
+#pragma unroll
+    for (int jj = 0; jj < 4; jj++) {
+        const int key = 16 * h + 4 * cb + jj;
+        const uint32_t sc = KVT == QWA_KV_F16 ? 0u : (uint32_t)vss[key * 8 + (dc >> 3)];
+        pf_v4<KVT>(raw + L::V + key * VB, dc, sc, hv[jj]);
+    }
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+        const uint32_t sel = (d & 1) ? 0x07060302u : 0x05040100u;  // high / low half of both words
+        const uint32_t w0 = __builtin_amdgcn_perm(hv[1][d >> 1], hv[0][d >> 1], sel);
+        const uint32_t w1 = __builtin_amdgcn_perm(hv[3][d >> 1], hv[2][d >> 1], sel);
+        *reinterpret_cast<uint2*>(Vt + (4 * dc + d) * VT_LD + 8 * cb + 4 * h) = make_uint2(w0, w1);
+    }
+}
+
+// The conversion is cut into 512 K units and 512 V units, spread over the workgroup's threads
+template <int KVT>
+__device__ __forceinline__ void pf_convert(const uint8_t* raw, _Float16* Ks, _Float16* Vt, int t) {
+    if constexpr (PF_THREADS == 512) {
+        pf_convert_kv<KVT>(raw, Ks, Vt, t, true, true);
+    } else {
+#pragma unroll
+        for (int u = t; u < 1024; u += PF_THREADS) pf_convert_kv<KVT>(raw, Ks, Vt, u & 511, u < 512, u >= 512);
     }
 }
 
@@ -130,7 +272,6 @@ __device__ __forceinline__ void pf_issue_img(uint32_t lds, const uint8_t* src, i
         dma_sv<16>(lds + 1024 * i, src, (uint32_t)(1024 * i + 16 * lane));
     }
 }
-
 
 // One split of one row block: grid (row blocks, NKV, NS splits).  Tokens 0 .. B-1 of this pass sit at cache positions
 // p0 .. p0 + B - 1.
