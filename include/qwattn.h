@@ -244,8 +244,8 @@ size_t qwa_attn_batch_work_bytes(int n, int nq, int n_shared, int max_len);
  * those of the queries: a captured call needs a max_len that its sequences do not outgrow.)
  * A row that sees no position (an empty or unknown sequence, a query before the first position) gets zeros; positions
  * whose page is none of the pool's are not seen.  Pool bytes past a sequence's last position are never used.  A K or V
- * value that is not finite shows in the rows that see it, and may show in those that do not, but share its 32 positions
- * with one that does: a sequence's earlier queries, and a row that ends among the shared positions.
+ * value that is not finite shows in the rows that see it (V: at least in its dim, as NaN or infinity; K: as NaN, or not at
+ * all where its score is -infinity) and changes no other row.
  * A call's result has the same bits whenever it is repeated; the order of its sums depends on the batch, so a sequence
  * need not have the bits that it has in another batch or in qwa_attn_decode_multi.
  * n <= QWA_PAGES_MAXN; q, gate, out16, work and the pool 16-byte aligned; work of at least qwa_attn_batch_work_bytes

@@ -209,6 +209,26 @@ __device__ __forceinline__ void bt_v_pair(uint32_t aw, uint32_t bw, uint32_t sa,
     }
 }
 
+// ---- V that is not finite.  A key that a row does not see has probability 0, but 0 * NaN is NaN.  So in tiles of which some
+// row does not see some key, such values enter P V as zeros, and a dim of O becomes NaN in the rows that see one.
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+// largest magnitude (as bits) of fp16 numbers, two at a time, and whether it reaches `least`
+__device__ __forceinline__ us2 max_bits(us2 m, uint32_t w) {
+    return __builtin_elementwise_max(m, __builtin_bit_cast(us2, w & 0x7FFF7FFFu));
+}
+__device__ __forceinline__ bool reaches(us2 m, uint16_t least) { return m[0] >= least || m[1] >= least; }
+// (of a quantized type a block's values are finite as long as the largest code's is: 8 * 8188, 127 * 515.5)
+template <int KVT>
+constexpr uint16_t ODD_FROM = KVT == QWA_KV_Q4_0 ? 0x7000 /* 8192 */ : KVT == QWA_KV_Q8_0 ? 0x6008 /* 516 */ : 0x7C00;
+// all bits of the halves that are not finite
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
+    return ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u);
+}
+__device__ __forceinline__ void nan_where(f4& o, f4 count) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = count[i] > 0.0f ? NAN : o[i];
+}
+
 template <int KVT, int RT>
 struct BtCfg {
     // 16-key groups of a tile, as two waves per SIMD leave registers for (raw bytes of 32 keys: F16 128 registers, Q8_0 66)
@@ -519,6 +539,68 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
             for (int j = 0; j < 4 * KT; j++)
                 vd[j] = SC ? h2_bits(scale_of(vsd[j / 4], 4 * (4 * lg + j % 4) + (i16 >> 2), (i16 >> 1) & 1)) & 0xFFFFu : 0u;
             constexpr int DPW = 16 / VW;
+            if (masked) {
+                us2 top = {0, 0};
+#pragma unroll
+                for (int j = 0; j < 4 * KT; j++) {
+                    if constexpr (SC) {
+                        top = max_bits(top, vd[j]);
+                    } else {
+#pragma unroll
+                        for (int wi = 0; wi < VW; wi++) top = max_bits(top, vr[j][wi]);
+                    }
+                }
+                if (__any(reaches(top, ODD_FROM<KVT>))) {
+                    // which rows see how many such values: the product of ones in their place with ones for the seen keys
+                    const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                    h4 seen[RT][KT];
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const int key = kb + 16 * kt + 4 * lg + j;
+                                seen[rt][kt][j] = at[kt] >= 0 && key >= seg.lo && key < vis[rt] ? (_Float16)1.0f : (_Float16)0.0f;
+                            }
+                    if constexpr (SC) {  // (a block as a whole; the lane's 16 dims lie in one)
+                        h4 ones[KT];
+#pragma unroll
+                        for (int j = 0; j < 4 * KT; j++) {
+                            const bool odd = (vd[j] & 0x7FFFu) >= ODD_FROM<KVT>;
+                            ones[j / 4][j % 4] = odd ? (_Float16)1.0f : (_Float16)0.0f;
+                            vd[j] = odd ? 0u : vd[j];
+                        }
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++) {
+                            f4 count = zero;
+#pragma unroll
+                            for (int kt = 0; kt < KT; kt++) count = bt_mfma16k16(ones[kt], seen[rt][kt], count);
+#pragma unroll
+                            for (int dt = 0; dt < 16; dt++) nan_where(o[rt][dt], count);
+                        }
+                    } else {
+#pragma unroll
+                        for (int wi = 0; wi < VW; wi++) {
+                            uint32_t ones[4], lo[DPW], hi[DPW];
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const uint32_t odd = odd_halves(vr[j][wi]);
+                                ones[j] = odd & 0x3C003C00u;
+                                vr[j][wi] &= ~odd;
+                            }
+                            bt_v_pair<KVT>(ones[0], ones[1], 0, 0, lo);
+                            bt_v_pair<KVT>(ones[2], ones[3], 0, 0, hi);
+#pragma unroll
+                            for (int d = 0; d < DPW; d++)
+#pragma unroll
+                                for (int rt = 0; rt < RT; rt++)
+                                    nan_where(o[rt][wi * DPW + d], bt_mfma16k16(make_h4(lo[d], hi[d]), seen[rt][0], zero));
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                }
+            }
 #pragma unroll
             for (int wi = 0; wi < VW; wi++) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -785,8 +867,14 @@ __device__ __forceinline__ void bt_load_k(BtRaw<KVT>& r, const uint8_t* k, const
 //  V^T: unit (cb, slot) at 256 cb + slot: keys 8 cb .. 8 cb + 7 in the P^T operand's order (4 cb + 16 h + j at 4 h + j) of the
 //  dim 8 (slot % 32) + slot / 32, so that the writing lanes (c = slot % 32) lie side by side, too.
 // (Rows of 528 and 80 bytes instead: half of the LDS cycles were conflicts; 128 sequences over 32768 Q4_0 positions 163 us.)
+// Values that are not finite become zeros; a wave that has one notes the tile, and which: of dim d and its keys 16 h + 4 cb .. + 3
+// the bits of byte 8 d + 2 cb + h.
+struct alignas(16) BtOdd {
+    uint8_t keys[8 * HD];
+    int tile[4];  // by wave (cb)
+};
 template <int KVT>
-__device__ __forceinline__ void bt_store_v(BtRaw<KVT>& r, _Float16* Vt, int t, uint32_t dead) {
+__device__ __forceinline__ void bt_store_v(BtRaw<KVT>& r, _Float16* Vt, BtOdd& odd, int t, uint32_t dead, int tile) {
     constexpr int VB = BtRaw<KVT>::VB, VW = VB / 128, DPW = 8 / VW;  // words of a row, dims of a word
     const int u = t & 255;
     // (a half without a place: its probabilities are zeros, and what was read need not be finite)
@@ -796,12 +884,32 @@ __device__ __forceinline__ void bt_store_v(BtRaw<KVT>& r, _Float16* Vt, int t, u
 #pragma unroll
         for (int j = 0; j < 4; j++) r.sc[j] = 0;
     }
+    us2 top = {0, 0};
+    if constexpr (KVT == QWA_KV_F16) {
+#pragma unroll
+        for (int i = 0; i < VB / 32; i++) top = max_bits(top, r.w[i]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = max_bits(top, r.sc[j]);
+    }
+    const bool any_odd = __any(reaches(top, ODD_FROM<KVT>));
+    if (any_odd && (u & 63) == 0) odd.tile[u >> 6] = tile;
     _Float16* dst = Vt + 8 * (256 * (u >> 6) + (u & 31)) + 4 * ((u >> 5) & 1);
 #pragma unroll
     for (int i = 0; i < VW; i++) {
         uint32_t lo[DPW], hi[DPW];
         bt_v_pair<KVT>(r.w[i], r.w[VW + i], r.sc[0], r.sc[1], lo);
         bt_v_pair<KVT>(r.w[2 * VW + i], r.w[3 * VW + i], r.sc[2], r.sc[3], hi);
+        if (any_odd) {
+#pragma unroll
+            for (int d = 0; d < DPW; d++) {
+                const uint32_t a = odd_halves(lo[d]), b = odd_halves(hi[d]);
+                odd.keys[8 * (8 * (u & 31) + DPW * i + d) + 2 * (u >> 6) + ((u >> 5) & 1)] =
+                    (uint8_t)((a & 1) | (a >> 31) << 1 | (b & 1) << 2 | (b >> 31) << 3);
+                lo[d] &= ~a;
+                hi[d] &= ~b;
+            }
+        }
 #pragma unroll
         for (int d = 0; d < DPW; d++) *reinterpret_cast<uint2*>(dst + 8 * 32 * (DPW * i + d)) = make_uint2(lo[d], hi[d]);
     }
@@ -847,9 +955,11 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
             _Float16 k[2][PF_TILE * HD];
             _Float16 vt[2][PF_TILE * HD];
             uint16_t scales[2][KVT == QWA_KV_F16 ? 8 : PF_TILE * 8];  // of K
+            BtOdd odd[2];
         } tile;
         uint2 xch[BT_TWAVES][XCH / 8];
     } lds;
+    static_assert(sizeof(lds.xch) <= sizeof(lds.tile.k) + sizeof(lds.tile.vt), "the exchange ends before what lies behind the tiles");
     auto& s_k = lds.tile.k;
     auto& s_vt = lds.tile.vt;
     const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, lg = lane >> 4;
@@ -915,11 +1025,13 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
             else bt_load_k<KVT>(raw, kh, ksh, wave < 6 ? at[0] : at[1], wave < 6 ? rows[0] : rows[1], t);
             return bits;
         };
-        auto store = [&](int b, uint32_t bits) {
-            if constexpr (ROLE == 0) bt_store_v<KVT>(raw, s_vt[b], t, bits);
+        auto store = [&](int i, uint32_t bits) {
+            const int b = i & 1;
+            if constexpr (ROLE == 0) bt_store_v<KVT>(raw, s_vt[b], lds.tile.odd[b], t, bits, i);
             else bt_store_k<KVT>(raw, s_k[b], lds.tile.scales[b], t);
         };
         if (nt > 0) dead = load(0);
+        if (t < 8) lds.tile.odd[t >> 2].tile[t & 3] = -1;  // (behind the part of LDS that the exchange uses)
 
         // Q / 16 as the B operand, by way of the wave's part of the exchange, first the hi parts, then the lo parts: a row is
         // read as one kilobyte (fragment by fragment, 16 rows at once, the loads took 7 us), its fp16 pieces go to unit (s, lg,
@@ -974,7 +1086,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
             const bool rows_here = wrow0 < nrows;
             // tile i + 1 into the other buffer (free since the last barrier), then tile i + 2's loads
             auto convert = [&](int i) {
-                if (i + 1 < nt) store((i + 1) & 1, (dead >> 2) & 3);
+                if (i + 1 < nt) store(i + 1, (dead >> 2) & 3);
                 if (i + 2 < nt) dead |= load(i + 2) << 4;
             };
             for (int i = 0; i < nt; i++) {
@@ -1071,6 +1183,27 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
                     for (int dt = 0; dt < 16; dt++) {
                         if (dt + BT_VD - 1 < 16) vf[(dt + BT_VD - 1) % BT_VD] = lds_h8(vrow + 8 * 16 * (dt + BT_VD - 1));
                         o[dt] = mfma16(vf[dt % BT_VD], pb, o[dt]);
+                    }
+                    // a dim is NaN in the rows that see a value of it that is not finite
+                    const int4 w = *reinterpret_cast<const int4*>(lds.tile.odd[i & 1].tile);
+                    if (__builtin_amdgcn_readfirstlane(w.x == i || w.y == i || w.z == i || w.w == i)) {
+                        const int of[4] = {w.x, w.y, w.z, w.w};
+                        uint32_t seen[2] = {0, 0};
+#pragma unroll
+                        for (int k = 0; k < PF_TILE; k++) {
+                            const int cb = k / 4 % 4, h = k / 16;
+                            if (of[cb] == i && k0 + k < vis && !((dead >> h) & 1)) seen[cb / 2] |= 1u << (8 * (2 * (cb & 1) + h) + k % 4);
+                        }
+#pragma unroll
+                        for (int dt = 0; dt < 16; dt++) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const int dim = 8 * (16 * (dt & 1) + 4 * lg + j) + (dt >> 1);
+                                const uint2 keys = *reinterpret_cast<const uint2*>(&lds.tile.odd[i & 1].keys[8 * dim]);
+                                o[dt][j] = ((keys.x & seen[0]) | (keys.y & seen[1])) != 0 ? NAN : o[dt][j];
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
                 }
                 if constexpr (ROLE != 0) convert(i);

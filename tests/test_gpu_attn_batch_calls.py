@@ -72,3 +72,46 @@ def test_calls_in_flight_on_two_streams(gpu):
     for s in range(2):
         for rep in range(4):
             assert all(torch.equal(a, w) for a, w in zip(outs[s][rep], want[s]))
+
+
+@pytest.mark.parametrize("x", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("lens, shared, nq, s, at", [
+    ([70, 300], 0, 8, 1, 299),                                    # own positions: the last of eight queries sees it
+    ([70, 300, 13], 0, 5, 1, 296),
+    ([300, 64, 65], 0, 1, 0, 17),                                 # every row of its sequence
+    ([100, 300], 256, 1, 1, 250),                                 # a prefix of which one row has only a part
+    ([250, 251, 90, 300, 0], 256, 1, 3, 250),
+    ([0, 3, 40, 100, 250, 251, 252, 300, 301, 256, 255, 17], 256, 1, 7, 250),
+    ([0, 3, 40, 100, 250, 251, 252, 300, 301, 256, 255, 17], 256, 1, 7, 0),
+    ([256] * 6 + [255], 256, 8, 0, 255),                          # everything shared, eight queries
+    ([600 - 50 * i for i in range(12)], 590, 3, 0, 333)])
+@pytest.mark.parametrize("kvt", KVTS, ids=lambda k: KV_NAMES[k])
+def test_values_that_are_not_finite_stay_in_the_rows_that_see_them(gpu, kvt, lens, shared, nq, s, at, x):
+    """A V value, then a K value (of a quantized type: a block's scale) at position `at` of sequence s that is not finite: the
+    rows that see it are not finite there (for an infinite K where its score is infinity; with a score of -infinity the key
+    weighs nothing), all others have the bits that they have with a finite one."""
+    page, kvh, dim = 32, 2, 41
+    b = Batch(kvt, lens, shared=shared, page=page)
+    most = max(lens)
+    _, _, clean = b.run(nq, shared, most)
+    slot = int(b.pages.table[s, at // page]) * page + at % page
+    # the position is every row's whose sequence holds that page there
+    same = b.pages.table[:, at // page] == b.pages.table[s, at // page]
+    sees = torch.tensor([bool(same[i]) and at < m - nq + t + 1 for i, m in enumerate(lens) for t in range(nq)], device="cuda")
+    assert sees.any() and not sees.all()
+    heads = torch.zeros(24, dtype=torch.bool, device="cuda")
+    heads[6 * kvh:6 * kvh + 6] = True
+    hit = sees[:, None] & heads
+    for which in ("v", "k"):
+        buf, col = (getattr(b.kv, which), dim) if kvt == ops.F16 else (getattr(b.kv, which + "s"), dim // 32)
+        buf = buf.view(torch.float16)
+        old = buf[kvh, slot, col].clone()
+        buf[kvh, slot, col] = x
+        _, _, out = b.run(nq, shared, most)
+        buf[kvh, slot, col] = old
+        seen = out[hit]
+        if which == "v":
+            assert not torch.isfinite(seen[:, dim]).any()
+        elif x != x:
+            assert torch.isnan(seen).all()
+        assert torch.equal(out[~hit], clean[~hit])
