@@ -30,11 +30,13 @@
 
 namespace qwa {
 
-// The probabilities are exp(s - m) for a reference m that is set BT_RAISE below a row's running maximum, and set again when a
-// score exceeds m by more than BT_HEAD: at most e^11 = 59874, in full fp16 precision down to 2^-14 = e^-9.7, with fewer bits
-// down to 2^-24.  Those that vanish, below 2^-25 = e^-17.3, are e^-24 to e^-28 of the largest: 2^18 of them are less than 2^-17 of
-// a row's sum.  (With m at the maximum itself they were 2^-25 of the largest, and 131071 of them moved an output by 7e-3.)
-constexpr float BT_RAISE = 7.0f, BT_HEAD = 11.0f;
+// The probabilities are 2^(s log2(e) - m) for a reference m that is set BT_RAISE below a row's running maximum, and set again
+// when a score exceeds m by more than BT_HEAD: at most 2^15, in full fp16 precision down to 2^-14, with fewer bits down to
+// 2^-24.  Those that vanish, below 2^-25, are 2^-35 to 2^-40 of the largest: 2^18 of them are less than 2^-17 of a row's sum.
+// (With m at the maximum itself they were 2^-25 of the largest, and 131071 of them moved an output by 7e-3.)
+// m is kept in powers of two, as it enters the exponent: a reference in units of s, multiplied when it is used, would be another
+// one by the product's rounding, 0.1 at scores of a million, and the states of a row would not weigh the same.
+constexpr float BT_RAISE = 10.0f, BT_HEAD = 15.0f;
 constexpr int BT_KD = 1;  // K steps read ahead of their MFMAs
 constexpr int BT_VD = 3;  // V fragments in flight
 size_t batch_work_bytes(int n, int nq, int n_shared, int max_len) {
@@ -511,15 +513,15 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
 #pragma unroll
                 for (int kt = 0; kt < KT; kt++) mx = max3f(max3f(mx, S[rt][kt][0], S[rt][kt][1]), S[rt][kt][2], S[rt][kt][3]);
                 mx = rows_max(mx);
-                const float mn = mx > m[rt] + BT_HEAD ? mx - BT_RAISE : m[rt];
-                const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;  // a row that saw nothing keeps l = 0, O = 0
-                cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] * PF_LOG2E - msl);
+                const float mx2 = mx * PF_LOG2E, mn = mx2 > m[rt] + BT_HEAD ? mx2 - BT_RAISE : m[rt];
+                const float ref = mn == -INFINITY ? 0.0f : mn;  // a row that saw nothing keeps l = 0, O = 0
+                cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] - mn);
                 // the sum is that of the rounded probabilities, the weights that P V applies
                 const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
                 float rs = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    p8[rt][j] = (_Float16)(j < 4 * KT ? fast_exp2(fmaf(S[rt][(j >> 2) % KT][j & 3], PF_LOG2E, -msl)) : 0.0f);
+                    p8[rt][j] = (_Float16)(j < 4 * KT ? fast_exp2(fmaf(S[rt][(j >> 2) % KT][j & 3], PF_LOG2E, -ref)) : 0.0f);
 #pragma unroll
                 for (int j = 0; j < 4 * KT; j += 2) rs = __builtin_amdgcn_fdot2(h2{p8[rt][j], p8[rt][j + 1]}, one2, rs, false);
                 l[rt] = l[rt] * cr[rt] + rs;
@@ -653,7 +655,7 @@ __device__ __forceinline__ void bt_body(BtLds<KVT, RT>& lds, const BatchArgs& a,
 #pragma unroll
                 for (int w = 0; w < BT_WAVES; w++) {
                     const float mw = s_ml[w][0][lane], lw = s_ml[w][1][lane];
-                    const float f = lw == 0.0f ? 0.0f : fast_exp2((mw - M) * PF_LOG2E);  // (lw: NaN scores stay NaN)
+                    const float f = lw == 0.0f ? 0.0f : fast_exp2(mw - M);  // (lw: NaN scores stay NaN)
                     L = fmaf(f, lw, L);
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
@@ -1156,9 +1158,9 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
                     }
                     float mx = max3f(max3f(-INFINITY, sc[0][0], sc[0][1]), sc[0][2], sc[0][3]);
                     mx = rows_max(max3f(max3f(mx, sc[1][0], sc[1][1]), sc[1][2], sc[1][3]));
-                    const float mn = mx > m + BT_HEAD ? mx - BT_RAISE : m;
-                    const float cr = mn == m ? 1.0f : fast_exp2((m - mn) * PF_LOG2E);
-                    const float msl = mn == -INFINITY ? 0.0f : mn * PF_LOG2E;
+                    const float mx2 = mx * PF_LOG2E, mn = mx2 > m + BT_HEAD ? mx2 - BT_RAISE : m;
+                    const float cr = mn == m ? 1.0f : fast_exp2(m - mn);
+                    const float ref = mn == -INFINITY ? 0.0f : mn;
                     m = mn;
                     // the V fragments' reads begin while the exponentials are taken
                     const _Float16* vrow = Vt + 8 * (256 * lg + i16);
@@ -1167,7 +1169,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
                     for (int dt = 0; dt < BT_VD - 1; dt++) vf[dt] = lds_h8(vrow + 8 * 16 * dt);
                     h8 pb;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) pb[j] = (_Float16)fast_exp2(fmaf(sc[j >> 2][j & 3], PF_LOG2E, -msl));
+                    for (int j = 0; j < 8; j++) pb[j] = (_Float16)fast_exp2(fmaf(sc[j >> 2][j & 3], PF_LOG2E, -ref));
                     // the sum of the rounded probabilities, the weights that P V applies
                     const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
                     float rs = 0.0f;
@@ -1255,7 +1257,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
 }
 
 // Joins a row's partial states in a fixed order, gates, rounds: WPR waves per row (token * NH + head), 4 dims per lane.  The
-// weights exp(m - M) come one state a lane, 64 at a time; wave k of a row reads the states' rows k, k + WPR, ..., eight at
+// weights 2^(m - M) come one state a lane, 64 at a time; wave k of a row reads the states' rows k, k + WPR, ..., eight at
 // a time.
 // The states' bytes and a chain of dependent loads bound it: 768 rows of 64 fixed-point and 5 fp32 states 10.6 us (31 MB).
 template <int WPR>
@@ -1299,9 +1301,9 @@ __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, const float* __
             }
             const float4 ml = lane < most ? ml_of(s0 + lane) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
             const float Mn = fmaxf(M, wave_max(ml.x));
-            const float c = M == Mn ? 1.0f : fast_exp2((M - Mn) * PF_LOG2E);
+            const float c = M == Mn ? 1.0f : fast_exp2(M - Mn);
             // a state that saw nothing weighs nothing; one of NaN scores (l is NaN) makes the row NaN
-            const float f = ml.y == 0.0f ? 0.0f : fast_exp2((ml.x - Mn) * PF_LOG2E);
+            const float f = ml.y == 0.0f ? 0.0f : fast_exp2(ml.x - Mn);
             M = Mn;
             L = fmaf(L, c, wave_sum(f * ml.y));
             acc.x *= c;

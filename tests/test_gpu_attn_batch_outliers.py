@@ -12,7 +12,8 @@ import torch
 
 import qwengine_amd.ops as ops
 from kvutil import KVTS, KV_NAMES, seeded_normal
-from test_gpu_attn_batch import Batch
+from pageref import batch_attention
+from test_gpu_attn_batch import Batch, close
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +88,33 @@ def test_many_keys_far_below_the_largest_score(gpu, kvt, n, nq, shared):
         err = (out.view(n, nq, 24, 256)[:, t].double().cpu() - want).abs().max().item()
         print(f"{KV_NAMES[kvt]} {n} x {nq}, query {t}: off by {err:.2e} of {tol:.2e}", flush=True)
         assert err <= tol
+
+
+@pytest.mark.parametrize("base", [60000, 59968, 52544, 33024])
+@pytest.mark.parametrize("lens, shared, nq", [([3000, 200], 0, 1), ([700], 0, 8), ([2900, 2800], 2700, 1),
+                                              ([2900 - 10 * i for i in range(9)], 2700, 1)])
+def test_scores_of_a_million(gpu, lens, shared, nq, base):
+    """Scores of 1.0 to 1.9 million that differ by 0 to 10, all of them whole numbers that fp32 holds: a state's reference times
+    log2(e) is off by up to 0.1 there, and the states of a row, each with its own, have to weigh the same all the same.
+    F16 keys of 255 equal numbers and a small one; half of the queries look the other way (scores below minus a million)."""
+    b = Batch(ops.F16, lens, shared=shared)
+    n = len(lens)
+    for i, m in enumerate(lens):
+        g = torch.Generator(device="cuda").manual_seed(900 + i)
+        g0 = torch.Generator(device="cuda").manual_seed(899)
+        own = torch.randint(0, 11, (m, 4), generator=g, device="cuda")
+        own[:min(shared, m)] = torch.randint(0, 11, (max(shared, 1), 4), generator=g0, device="cuda")[:min(shared, m)]
+        K = torch.full((m, 4, 256), float(base), device="cuda")
+        K[..., 255] = 8.0 * own
+        ops.kv_append(K, None, 0, m, ops.F16, b.caches[i])
+        at = torch.arange(m, device="cuda")
+        b.kv.k[:, b.pages.table[i].long()[at // b.page] * b.page + at % b.page] = b.caches[i].k[:, :m]
+    q, gate = torch.full((n * nq, 24, 256), 2.0, device="cuda"), seeded_normal((n * nq, 24, 256), 4)
+    q[:, ::2] = -2.0
+    q[..., 255] = 2.0
+    out = torch.empty((n * nq, 24, 256), dtype=torch.float16, device="cuda")
+    work = torch.empty(ops.attn_batch_work_bytes(n, nq, shared, max(lens)), dtype=torch.uint8, device="cuda")
+    ops.attn_decode_batch(q, gate, b.kv, b.kvt, b.pages, None, n, nq, shared, max(lens), out, work)
+    torch.cuda.synchronize()
+    want = batch_attention(q, gate, lambda t: b.values(t // nq), [lens[t // nq] - nq + t % nq + 1 for t in range(n * nq)])
+    close(out, want, f"{lens} shared {shared}, {base}")
