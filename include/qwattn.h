@@ -196,7 +196,8 @@ size_t qwa_kv_pages_work_bytes(const qwa_kv_pages* p);
  * pools of type kvt), since the new positions would be written into it; the last of its holders keeps the page.
  * All or nothing: *status (device) becomes 0 when done; the number of missing pages when the free pages do not suffice;
  * -(i + 1) when request i is invalid (no such sequence, named before, add < 0, past ld * page positions; or a broken
- * table: len < 0, or the partly filled last page is none of the pool's).  In the last two cases nothing is changed.  The new positions hold old bytes until a prep or an append writes them. */
+ * table: len < 0, or the partly filled last page is none of the pool's).  In the last two cases nothing is changed.  The
+ * new positions hold old bytes until a prep or an append writes them. */
 int qwa_kv_pages_extend(const qwa_kv_pages* p, const int* seqs, const int* add, int n, const qwa_kv_layer* layers,
                         int n_layers, int kvt, int* status, void* work, size_t work_bytes, void* stream);
 

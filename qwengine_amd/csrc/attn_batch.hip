@@ -20,8 +20,8 @@
 //    out when the scores are done, its V loads when P V is.
 // A batch of one call has the same bits again; another batch, or another cut, sums a row's states in another order.
 // Roundings below 32 bits: the dequantized V (d * code) and the probabilities are fp16 (half a step: 2^-11 of the value, random
-// in sign, as in the prefill: P V then has one MFMA per 32 keys and 16 dims; for the probabilities' range see BT_RAISE), a tile workgroup's O / l is 16-bit fixed point
-// (half a step: 2^-16 of the row's largest, attn_tiles.hpp), the output is fp16.
+// in sign, as in the prefill: P V then has one MFMA per 32 keys and 16 dims; for the probabilities' range see BT_RAISE), a tile
+// workgroup's O / l is 16-bit fixed point (half a step: 2^-16 of the row's largest, attn_tiles.hpp), the output is fp16.
 #include <type_traits>
 
 #include "attn_tiles.hpp"
@@ -961,7 +961,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
         } tile;
         uint2 xch[BT_TWAVES][XCH / 8];
     } lds;
-    static_assert(sizeof(lds.xch) <= sizeof(lds.tile.k) + sizeof(lds.tile.vt), "the exchange ends before what lies behind the tiles");
+    static_assert(sizeof(lds.xch) <= sizeof(lds.tile.k) + sizeof(lds.tile.vt), "what lies behind the tiles is not exchanged");
     auto& s_k = lds.tile.k;
     auto& s_vt = lds.tile.vt;
     const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, lg = lane >> 4;
@@ -1194,7 +1194,8 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
 #pragma unroll
                         for (int k = 0; k < PF_TILE; k++) {
                             const int cb = k / 4 % 4, h = k / 16;
-                            if (of[cb] == i && k0 + k < vis && !((dead >> h) & 1)) seen[cb / 2] |= 1u << (8 * (2 * (cb & 1) + h) + k % 4);
+                            if (of[cb] == i && k0 + k < vis && !((dead >> h) & 1))
+                                seen[cb / 2] |= 1u << (8 * (2 * (cb & 1) + h) + k % 4);
                         }
 #pragma unroll
                         for (int dt = 0; dt < 16; dt++) {

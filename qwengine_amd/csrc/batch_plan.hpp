@@ -38,7 +38,7 @@ constexpr int BT_FEW = 32;
 //  one segment per sequence that it meets.
 struct BatchPlan {
     int blocks, nt;                // row blocks and key ranges of the tile workgroups (0: none)
-    int groups_shared, rt_shared;  // passes of register workgroups that the batch's rows would take (where they run: 1), their row tiles
+    int groups_shared, rt_shared;  // passes of register workgroups over the batch's rows (1 where they run), their row tiles
     int ns_shared, len_shared;     // key ranges of register workgroups over the shared positions, and their length
     int groups, rt_own;            // row groups of a sequence, and the row tiles of a group
     int wgs;                       // slices of the own steps (0: no own positions)

@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(64 * PB_WAVES) k_prep_batch(
     const float* __restrict__ qn_w, const float* __restrict__ kn_w, qwa_kv_pages pg, const int* __restrict__ seqs, int n,
     int nq, const int* __restrict__ rope_off, float theta, float eps, qwa_kv_layer kv, float* __restrict__ q_out,
     float* __restrict__ gate) {
-    __shared__ float s_cs[NROT];
+    __shared__ __attribute__((aligned(16))) float s_cs[NROT];  // (read 16 bytes at a time)
     const int r = blockIdx.x, b = r / nq, t = threadIdx.x, lane = t & 63, half = lane >> 5, l = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     // the token's position, and its place in the pool (-1: not stored)
