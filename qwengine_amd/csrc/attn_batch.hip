@@ -170,8 +170,8 @@ __device__ __forceinline__ uint2 bt_ld8(__amdgpu_buffer_rsrc_t b, int off) {
 // Q4_0 codes with fewer shifts than q4_word_to_h8 / v_pair_words (the same values in the same order): a nibble that sits at
 // bit 4 of a half makes 64 + n there (0x5400 | n << 4), as one at bit 0 makes 1024 + n.
 // (w & mask) | magic in one instruction: the mask from a scalar register, the magic from a vector register.  As two
-// instructions, which the compiler makes of two constants, 24 sequences over 16384 Q4_0 positions took 84 instead of 80 us, the
-// tiles of 128 over 32768 156 instead of 147.
+// instructions, which the compiler makes of two constants, 24 sequences over 16384 Q4_0 positions take 78 instead of 71 us, the
+// tiles of 128 over 32768 214 instead of 209.
 __device__ __forceinline__ uint32_t q4_bits(uint32_t w, uint32_t mask, uint32_t magic) {
     uint32_t r;
     asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(magic));
@@ -703,12 +703,14 @@ __device__ __forceinline__ int bt_steps_of(const BatchArgs& a, int m) {
 }
 
 // the own positions: workgroup = (slice of the steps, KV head, row group), one segment per sequence that the slice meets.
-// Equal slices, since a cut by sequences leaves the chip to the longest one (24 of up to 16384 positions 108 instead of 89 us).
-// About 6 us of latency (finding the slice, page numbers, first bytes, joining the waves) around a stream of the cache's bytes:
-// 24 sequences of 267 000 Q4_0 positions together 66 us (4.7 TB/s; unpacking takes half of the issue cycles), of 131 000 Q8_0
-// ones 61 us (4.7 TB/s), F16 100 us (5.3 TB/s, where a large copy reads and writes 5.15).  The next segment's first tile is
-// sent before this one's waves are joined (24 sequences 68.2 -> 66.5 us, 1000 of 40 positions 64.7 -> 62.2).  Not faster: a
-// second tile on its way (registers for it are there), three waves a SIMD (spills).
+// Equal slices, since a cut by sequences leaves the chip to the longest one (24 of up to 16384 positions: 108 instead of 89 us,
+// in an early form).  About 6 us of latency (finding the slice, page numbers, first bytes, joining the waves) around a stream of the
+// cache's bytes: 24 sequences of 267 000 Q4_0 positions together 71 us (4.3 TB/s; VALU instructions, most of them unpacking,
+// take 56% of the issue cycles), of 131 000 Q8_0 ones 60 us (4.7 TB/s), F16 99 us (5.4 TB/s, where a large copy reads and writes
+// 5.15).  The next segment's first tile is sent before this one's waves are joined (2 to 3 us of 65).  Not faster: a second tile
+// on its way (registers for it are there), three waves a SIMD (spills).  Of several row tiles (more than two queries) a tile
+// has 16 keys, since 32 spill: 8 x 8 queries over 12000 own Q4_0 positions 63 us.  <F16, 2> keeps 17 registers in scratch, none of
+// them in the loop over tiles.
 template <int KVT, int RT>
 __global__ void __launch_bounds__(64 * BT_WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 k_bt_own(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int groups) {
@@ -943,11 +945,13 @@ __device__ __forceinline__ void bt_store_k(const BtRaw<KVT>& r, _Float16* Ks, ui
 
 // The shared positions for BT_TROWS rows: workgroup = (row block, tile range, KV head).  The 8 waves have 16 rows each, two a
 // SIMD, of which one converts V at the start of an iteration and the other K at its end, so the MFMAs of one run while the
-// other converts, takes exponentials or waits for LDS.  128 sequences over 32768 Q4_0 positions: 196 us, 0.79 PFLOP/s with the
-// second part of Q (large products of the library reach 1.17).  Of a SIMD's cycles 44% issue VALU instructions and 30% are
-// MFMAs; LDS is busy for 43%: two waves do not cover each other's waits.  (Three a SIMD have 168 registers each, which O and
-// both parts of Q leave 40 of: 12 waves spilled 47 to 108 with the low parts in LDS.  The block scales by lane broadcasts
-// instead of from LDS: 207 us.)
+// other converts, takes exponentials or waits for LDS.  128 sequences over 32768 positions: Q4_0 209 us, 0.74 PFLOP/s with the
+// second part of Q (large products of the library reach 1.17), Q8_0 218, F16 202; 2.0 us a tile.  No unit bounds it: of a
+// SIMD's cycles 45% issue VALU instructions and 30% are MFMAs, LDS is busy for 37% and 5% of conflicts.  Two waves do not
+// cover each other's waits, and three a SIMD have 168 registers each, of which O and both parts of Q leave 40.  (12 waves with
+// the low parts of Q in LDS spill 18 to 89 of them; whole call, 12 / 8 waves: Q4_0 240 to 256 / 245 us, Q8_0 256 to 265 / 229, F16
+// 226 to 239 / 215, 32 sequences over 8192 Q8_0 58 / 52.5.  Block scales by lane broadcasts instead of from LDS: 12 us more.
+// K and V fragments read further ahead: no difference.)
 template <int KVT>
 __global__ void __launch_bounds__(64 * BT_TWAVES) __attribute__((amdgpu_waves_per_eu(BT_TWAVES / 4, BT_TWAVES / 4)))
 k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
@@ -1260,7 +1264,7 @@ k_bt_tiles(BatchArgs a, qwa_kv_layer kv, qwa_kv_pages p, int blocks, int ns) {
 // Joins a row's partial states in a fixed order, gates, rounds: WPR waves per row (token * NH + head), 4 dims per lane.  The
 // weights 2^(m - M) come one state a lane, 64 at a time; wave k of a row reads the states' rows k, k + WPR, ..., eight at
 // a time.
-// The states' bytes and a chain of dependent loads bound it: 768 rows of 64 fixed-point and 5 fp32 states 10.6 us (31 MB).
+// The states' bytes and a chain of dependent loads bound it: 768 rows of 32 fixed-point and 5 fp32 states 7.1 us (17 MB).
 template <int WPR>
 __global__ void __launch_bounds__(256) k_bt_combine(BatchArgs a, const float* __restrict__ gate, int nt, int ns_shared,
                                                     uint16_t* __restrict__ out16, qwa_act_q8 oq, int do_q) {

@@ -16,12 +16,12 @@ constexpr int BT_WAVES = 4;               // waves of a register workgroup; they
 constexpr int BT_MAXRT = 2;               // 16-row MFMA tiles of such a workgroup at most
 constexpr int BT_TWAVES = 8;              // waves of a tile workgroup (four convert V, four K)
 constexpr int BT_TROWS = 16 * BT_TWAVES;  // its rows
-// Register workgroups that the chip holds, two a CU (own positions of 24 sequences of up to 16384 Q4_0 positions 68 us, with
-// 1024 in two rounds 72).
+// Register workgroups that the chip holds, two a CU.  Own positions of 24 sequences, us, 256 / 512 / 1024 workgroups (one a CU,
+// two, two rounds): up to 16384 Q4_0 positions 81 / 71 / 83, 8000 Q8_0 59 / 60 / 63, 8000 F16 97 / 99 / 103.
 constexpr int BT_FILL = 512;
 // Positions of a step; key ranges are whole steps.  A tile for each wave (own positions, steps of 64 / 128 / 256, us: 32
-// sequences of 700 Q8_0 positions 17.9 / 15.6 / 16.7, 5 x 7 queries of 513 F16 15.2 / 11.9 / 13.4, 5 of 5000 Q4_0 17.2 / 15.2 /
-// 14.3).
+// sequences of up to 700 Q8_0 positions 19.6 / 17.7 / 17.8, 5 x 7 queries of 513 F16 15.7 / 15.2 / 17.6, 5 of 5000 Q4_0 18.2 / 16.1
+// / 16.1).
 constexpr int BT_STEP = 128;
 // Rows of a KV head up to which the shared positions are left to register workgroups: one pass of them.  Whole call, us,
 // register / tile workgroups, 32768 shared positions: 18 rows Q4_0 40.5 / 47.5, Q8_0 41.7 / 47.7, F16 45.0 / 43.9; 30 rows 43.2 /
