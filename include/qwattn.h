@@ -255,6 +255,42 @@ int qwa_attn_decode_batch(const float* q, const float* gate, const qwa_kv_layer*
                           const int* seqs, int n, int nq, int n_shared, int max_len, uint16_t* out16,
                           const qwa_act_q8* oq, void* work, size_t work_bytes, void* stream);
 
+/* Chunks: any number of new tokens for each of n sequences.  The tokens of all are rows of one buffer: batch row b has rows
+ * off[b] .. off[b + 1] - 1 (off: device, n + 1 entries), a chunk of off[b + 1] - off[b] tokens, which are the last positions
+ * that its sequence seqs[b] (device; NULL: b) holds.  `rows` is the size of the buffers: rows that no chunk has (behind the
+ * last one, between two) are neither read nor written.  A chunk of no tokens takes no part; one that begins before an earlier
+ * one's end, or has rows outside [0, rows], counts as empty.  A captured graph follows the device's numbers. */
+#define QWA_CHUNK_MAXROWS 65536 /* rows per call */
+
+/* qwa_attn_prep_batch for chunks: row r of qg / k / v / q_out / gate belongs to the chunk that has it, token t of a chunk of c
+ * tokens has position len - c + t of its sequence, and the rotary position is that plus rope_off[b] (device; NULL: 0).  K / V
+ * rows are appended there; a row whose position is negative, or whose page is none of the pool's, is not stored.  Of
+ * several chunks of one sequence the last one is stored.  n <= QWA_PAGES_MAXN.  Every buffer 16-byte aligned. */
+int qwa_attn_prep_rows_batch(const float* qg, const float* k, const float* v, const float* q_norm, const float* k_norm,
+                             const qwa_kv_pages* p, const int* seqs, const int* off, int n, int rows, const int* rope_off,
+                             float theta, float eps, int kvt, const qwa_kv_layer* kv, float* q_out, float* gate,
+                             void* stream);
+
+/* Bytes of the `work` buffer of qwa_attn_prefill_batch (0: invalid arguments). */
+size_t qwa_attn_prefill_batch_work_bytes(int n, int rows, int max_len);
+
+/* Attention of chunks over a paged cache: token t of batch row b's chunk of c tokens sees positions [0, len - c + t].
+ * q, gate [rows][24][256]; out16: output * sigmoid(gate) as fp16 bits [rows][6144]; lse (optional) [rows][24]: the log of the
+ * sum of exp(score) over the positions that a row sees, as qwa_attn_weights_batch takes it.  Chunks of one token and of
+ * thousands may go together: the work is cut evenly over the chip.  fp16 MFMA, fp32 accumulation and softmax; scores are
+ * exact up to fp32 accumulation (K as its codes, Q in two fp16 parts); V as stored and the probabilities are rounded to fp16.
+ * max_len is a bound of the sequences' lens.  A sequence that is longer counts as one of max_len positions, as if
+ * qwa_kv_pages_trim had cut it.
+ * A row that sees no position (of an empty or unknown sequence, or before the first position) gets zeros, and -infinity in
+ * lse; positions whose page is none of the pool's are not seen.  Pool bytes past a sequence's last position are never used.
+ * A K or V value that is not finite shows in the rows that see it, as in qwa_attn_decode_batch, and changes no other row.
+ * A call's result has the same bits whenever it is repeated; the order of its sums depends on the batch.
+ * n <= QWA_PAGES_MAXN; q, gate, out16, work and the pool 16-byte aligned; work of at least qwa_attn_prefill_batch_work_bytes
+ * bytes, not shared with a call that may run at the same time (nor by two captured graphs whose replays may overlap). */
+int qwa_attn_prefill_batch(const float* q, const float* gate, const qwa_kv_layer* kv, int kvt, const qwa_kv_pages* p,
+                           const int* seqs, const int* off, int n, int rows, int max_len, uint16_t* out16, float* lse,
+                           void* work, size_t work_bytes, void* stream);
+
 /* ---- Gated DeltaNet (the recurrent token mixer of the other layers) ---------------------------------------------- */
 
 /* New tokens per qwa_deltanet_multi call (the reference's DN_MAXN = Engine::MAX_BATCH, src/cuda/ops.cu:148). */

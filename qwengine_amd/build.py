@@ -19,7 +19,8 @@ LIB = os.path.join(OUT_DIR, "libqwattn.so")
 ARCH = "gfx950"
 
 SOURCES = ["capi.hip", "kv_append.hip", "attn_decode.hip", "attn_decode_ilp.hip", "attn_simple.hip", "attn_prefill.hip",
-           "attn_batch.hip", "kv_pages.hip", "deltanet.hip", "deltanet_rows.hip", "gemv.hip", "gemv_mc.hip", "gemm.cpp"]
+           "attn_batch.hip", "attn_chunks.hip", "kv_pages.hip", "deltanet.hip", "deltanet_rows.hip", "gemv.hip", "gemv_mc.hip",
+           "gemm.cpp"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -56,6 +57,7 @@ FILE_FLAGS = {"attn_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "deltanet_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               # attn_batch.hip: the same (the two-tile kernels: 83 accumulation registers instead of 223)
               "attn_batch.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "attn_chunks.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               # gemv_mc.hip (IQ4_XS / IQ2_S one-column GEMV): the max-memory-clause scheduler
               "gemv_mc.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"]}
 

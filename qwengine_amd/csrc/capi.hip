@@ -520,6 +520,72 @@ int qwa_attn_decode_batch(const float* q, const float* gate, const qwa_kv_layer*
                     fn);
 }
 
+namespace {
+bool chunk_sizes_ok(int n, int rows, int max_len) {
+    return n >= 1 && n <= QWA_PAGES_MAXN && rows >= 1 && rows <= QWA_CHUNK_MAXROWS && max_len >= 1 &&
+           max_len <= qwa::MAX_POS;
+}
+
+// what the operators on chunks have in common (max_len < 0: none)
+int check_chunks(const qwa_kv_pages* p, const qwa_kv_layer* kv, int kvt, const int* seqs, const int* off, int n, int rows,
+                 int max_len, const char* fn) {
+    int st;
+    if ((st = check_batch(p, seqs, n, 1, fn)) || (st = check_pool(kv, kvt, p, fn))) return st;
+    if (!off) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if (rows < 1 || rows > QWA_CHUNK_MAXROWS)
+        return fail(QWA_ERR_RANGE, "%s: %d rows (1..%d)", fn, rows, QWA_CHUNK_MAXROWS);
+    if (max_len >= 0 && (!chunk_sizes_ok(n, rows, max_len) || max_len > (long long)p->ld * p->page))
+        return fail(QWA_ERR_RANGE, "%s: max_len %d (tables of %lld positions, at most %d)", fn, max_len,
+                    (long long)p->ld * p->page, qwa::MAX_POS);
+    return QWA_OK;
+}
+
+int check_buffers(const void* const* bufs, int n, const char* fn) {
+    for (int i = 0; i < n; i++) {
+        if (!bufs[i]) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+        if (!al16(bufs[i])) return fail(QWA_ERR_INVALID, "%s: buffer not 16-byte aligned", fn);
+    }
+    return QWA_OK;
+}
+
+int check_size(size_t have, size_t need, const char* fn) {
+    if (have < need) return fail(QWA_ERR_RANGE, "%s: workspace of %zu bytes, the call needs %zu", fn, have, need);
+    return QWA_OK;
+}
+}  // namespace
+
+int qwa_attn_prep_rows_batch(const float* qg, const float* k, const float* v, const float* q_norm, const float* k_norm,
+                             const qwa_kv_pages* p, const int* seqs, const int* off, int n, int rows, const int* rope_off,
+                             float theta, float eps, int kvt, const qwa_kv_layer* kv, float* q_out, float* gate,
+                             void* stream) {
+    const char* fn = "attn_prep_rows_batch";
+    const void* const bufs[] = {qg, k, v, q_norm, k_norm, q_out, gate};
+    int st;
+    if ((st = check_chunks(p, kv, kvt, seqs, off, n, rows, -1, fn)) || (st = check_buffers(bufs, 7, fn))) return st;
+    return from_hip(qwa::launch_prep_rows_batch(qg, k, v, q_norm, k_norm, *p, seqs, off, n, rows, rope_off, theta, eps, kvt,
+                                                *kv, q_out, gate, as_stream(stream)),
+                    fn);
+}
+
+size_t qwa_attn_prefill_batch_work_bytes(int n, int rows, int max_len) {
+    return chunk_sizes_ok(n, rows, max_len) ? qwa::prefill_batch_work_bytes(n, rows, max_len) : 0;
+}
+
+int qwa_attn_prefill_batch(const float* q, const float* gate, const qwa_kv_layer* kv, int kvt, const qwa_kv_pages* p,
+                           const int* seqs, const int* off, int n, int rows, int max_len, uint16_t* out16, float* lse,
+                           void* work, size_t work_bytes, void* stream) {
+    const char* fn = "attn_prefill_batch";
+    const void* const bufs[] = {q, gate, out16, work};
+    int st;
+    if (max_len < 0) max_len = 0;
+    if ((st = check_chunks(p, kv, kvt, seqs, off, n, rows, max_len, fn)) || (st = check_buffers(bufs, 4, fn)) ||
+        (st = check_size(work_bytes, qwa::prefill_batch_work_bytes(n, rows, max_len), fn)))
+        return st;
+    return from_hip(qwa::launch_prefill_batch(q, gate, *kv, kvt, *p, seqs, off, n, rows, max_len, out16, lse, work,
+                                              as_stream(stream)),
+                    fn);
+}
+
 // ---- Gated DeltaNet
 namespace {
 int check_dn_params(const qwa_dn_params* p, const char* fn) {

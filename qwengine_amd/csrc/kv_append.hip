@@ -409,34 +409,16 @@ __global__ void __launch_bounds__(256) k_prep_rows_al(const float* __restrict__ 
     }
 }
 
-// Batch form: the last nq positions of n sequences of a paged cache.  One workgroup per token (row b * nq + t at position
-// len - nq + t of sequence seqs[b]); the wave tasks are k_prep_rows_al's, the rotation's 32 cos / sin pairs are formed once
-// per token, in double (one lane per frequency), and shared through LDS.  Bytes: 800 tokens, 88 MB, 17.9 us (4.9 TB/s; a large
-// copy reaches 5.15); a few tokens 6 us of latency.
+// A token's wave tasks (k_prep_rows_al's) by a workgroup of a paged cache's batch: row r of the inputs and outputs, K and V to
+// position slot of the pool (-1: not stored), the rotation's cos / sin pairs in s_cs.
 constexpr int PB_WAVES = 8;
 template <int KVT>
-__global__ void __launch_bounds__(64 * PB_WAVES) k_prep_batch(
-    const float* __restrict__ qg, const float* __restrict__ k, const float* __restrict__ v,
-    const float* __restrict__ qn_w, const float* __restrict__ kn_w, qwa_kv_pages pg, const int* __restrict__ seqs, int n,
-    int nq, const int* __restrict__ rope_off, float theta, float eps, qwa_kv_layer kv, float* __restrict__ q_out,
-    float* __restrict__ gate) {
-    __shared__ __attribute__((aligned(16))) float s_cs[NROT];  // (read 16 bytes at a time)
-    const int r = blockIdx.x, b = r / nq, t = threadIdx.x, lane = t & 63, half = lane >> 5, l = lane & 31;
+__device__ __forceinline__ void prep_token(const float* __restrict__ qg, const float* __restrict__ k,
+                                           const float* __restrict__ v, const float* __restrict__ qn_w,
+                                           const float* __restrict__ kn_w, int r, long long slot, const float* s_cs, float eps,
+                                           const qwa_kv_layer& kv, float* __restrict__ q_out, float* __restrict__ gate) {
+    const int t = threadIdx.x, lane = t & 63, half = lane >> 5, l = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    // the token's position, and its place in the pool (-1: not stored)
-    const int seq = seqs ? seqs[b] : b;
-    const bool known = seq >= 0 && seq < pg.n_seq;
-    const int pos = (known ? pg.len[seq] : 0) - nq + r % nq;
-    bool later = false;  // a later batch row names the same sequence
-    if (seqs)
-        for (int j = b + 1 + t; j < n; j += 64 * PB_WAVES) later |= seqs[j] == seq;
-    long long slot = -1;
-    if (known && pos >= 0 && pos / pg.page < pg.ld) {
-        const int page = pg.table[(size_t)seq * pg.ld + pos / pg.page];
-        if ((unsigned)page < (unsigned)pg.n_pages) slot = (long long)page * pg.page + pos % pg.page;
-    }
-    if (t < NROT / 2) rope_cs((double)pos + (rope_off ? rope_off[b] : 0), theta, t, &s_cs[t], &s_cs[t + NROT / 2]);
-    if (__syncthreads_or(later)) slot = -1;
     auto ld8 = [](const float* p, float* x) {
         const float4 a = reinterpret_cast<const float4*>(p)[0], c = reinterpret_cast<const float4*>(p)[1];
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
@@ -477,6 +459,83 @@ __global__ void __launch_bounds__(64 * PB_WAVES) k_prep_batch(
                               KVT == QWA_KV_F16 ? nullptr : (is_v ? kv.vs : kv.ks) + row * 8, x, l);
         }
     }
+}
+
+// Batch form: the last nq positions of n sequences of a paged cache.  One workgroup per token (row b * nq + t at position
+// len - nq + t of sequence seqs[b]); the wave tasks are k_prep_rows_al's, the rotation's 32 cos / sin pairs are formed once
+// per token, in double (one lane per frequency), and shared through LDS.  Bytes: 800 tokens, 88 MB, 17.9 us (4.9 TB/s; a large
+// copy reaches 5.15); a few tokens 6 us of latency.
+template <int KVT>
+__global__ void __launch_bounds__(64 * PB_WAVES) k_prep_batch(
+    const float* __restrict__ qg, const float* __restrict__ k, const float* __restrict__ v,
+    const float* __restrict__ qn_w, const float* __restrict__ kn_w, qwa_kv_pages pg, const int* __restrict__ seqs, int n,
+    int nq, const int* __restrict__ rope_off, float theta, float eps, qwa_kv_layer kv, float* __restrict__ q_out,
+    float* __restrict__ gate) {
+    __shared__ __attribute__((aligned(16))) float s_cs[NROT];  // (read 16 bytes at a time)
+    const int r = blockIdx.x, b = r / nq, t = threadIdx.x;
+    // the token's position, and its place in the pool (-1: not stored)
+    const int seq = seqs ? seqs[b] : b;
+    const bool known = seq >= 0 && seq < pg.n_seq;
+    const int pos = (known ? pg.len[seq] : 0) - nq + r % nq;
+    bool later = false;  // a later batch row names the same sequence
+    if (seqs)
+        for (int j = b + 1 + t; j < n; j += 64 * PB_WAVES) later |= seqs[j] == seq;
+    long long slot = -1;
+    if (known && pos >= 0 && pos / pg.page < pg.ld) {
+        const int page = pg.table[(size_t)seq * pg.ld + pos / pg.page];
+        if ((unsigned)page < (unsigned)pg.n_pages) slot = (long long)page * pg.page + pos % pg.page;
+    }
+    if (t < NROT / 2) rope_cs((double)pos + (rope_off ? rope_off[b] : 0), theta, t, &s_cs[t], &s_cs[t + NROT / 2]);
+    if (__syncthreads_or(later)) slot = -1;
+    prep_token<KVT>(qg, k, v, qn_w, kn_w, r, slot, s_cs, eps, kv, q_out, gate);
+}
+
+// The same for chunks of any number of tokens: batch row b has rows off[b] .. off[b + 1] - 1, the last positions of its
+// sequence.  The workgroup's threads look for its row in `off` a chunk each (a binary search would be ten round trips).
+template <int KVT>
+__global__ void __launch_bounds__(64 * PB_WAVES) k_prep_rows_batch(
+    const float* __restrict__ qg, const float* __restrict__ k, const float* __restrict__ v,
+    const float* __restrict__ qn_w, const float* __restrict__ kn_w, qwa_kv_pages pg, const int* __restrict__ seqs,
+    const int* __restrict__ off, int n, int rows, const int* __restrict__ rope_off, float theta, float eps, qwa_kv_layer kv,
+    float* __restrict__ q_out, float* __restrict__ gate) {
+    constexpr int PER = (QWA_PAGES_MAXN + 64 * PB_WAVES - 1) / (64 * PB_WAVES);  // chunks a thread
+    __shared__ __attribute__((aligned(16))) float s_cs[NROT];  // (read 16 bytes at a time)
+    __shared__ int s_b;
+    const int r = blockIdx.x, t = threadIdx.x;
+    if (t == 0) s_b = n;
+    __syncthreads();
+    int first[PER], end[PER];  // (an invalid chunk has none)
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int c = t + 64 * PB_WAVES * j;
+        first[j] = c < n ? off[c] : 0;
+        end[j] = c < n ? off[c + 1] : 0;
+        if (first[j] < 0 || end[j] > rows) end[j] = first[j];
+        if (r >= first[j] && r < end[j]) atomicMin(&s_b, c);
+    }
+    __syncthreads();
+    const int b = s_b;
+    if (b >= n) return;  // nobody's row: left as it is
+    const int r0 = off[b], count = off[b + 1] - r0;
+    const int seq = seqs ? seqs[b] : b;
+    const bool known = seq >= 0 && seq < pg.n_seq;
+    const int pos = (known ? max(pg.len[seq], 0) : 0) - count + (r - r0);
+    bool overlaps = false, later = false;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int c = t + 64 * PB_WAVES * j;
+        overlaps |= c < b && end[j] > first[j] && end[j] > r0;              // it begins before an earlier one's end
+        later |= seqs && c > b && end[j] > first[j] && seqs[c] == seq;      // a later chunk is the same sequence's
+    }
+    long long slot = -1;
+    if (known && pos >= 0 && pos / pg.page < pg.ld) {
+        const int page = pg.table[(size_t)seq * pg.ld + pos / pg.page];
+        if ((unsigned)page < (unsigned)pg.n_pages) slot = (long long)page * pg.page + pos % pg.page;
+    }
+    if (t < NROT / 2) rope_cs((double)pos + (rope_off ? rope_off[b] : 0), theta, t, &s_cs[t], &s_cs[t + NROT / 2]);
+    if (__syncthreads_or(overlaps)) return;
+    if (__syncthreads_or(later)) slot = -1;
+    prep_token<KVT>(qg, k, v, qn_w, kn_w, r, slot, s_cs, eps, kv, q_out, gate);
 }
 
 // one thread per (token, frequency); pos3 != nullptr selects M-RoPE, where frequency i turns with component i % 3
@@ -557,6 +616,25 @@ hipError_t launch_prep_batch(const float* qg, const float* k, const float* v, co
         QWA_PREP_BATCH(QWA_KV_Q4_0);
     }
 #undef QWA_PREP_BATCH
+    return hipGetLastError();
+}
+
+hipError_t launch_prep_rows_batch(const float* qg, const float* k, const float* v, const float* qn, const float* kn,
+                                  const qwa_kv_pages& p, const int* seqs, const int* off, int n, int rows,
+                                  const int* rope_off, float theta, float eps, int kvt, const qwa_kv_layer& kv, float* q,
+                                  float* gate, hipStream_t st) {
+    const dim3 grid(rows), block(64 * PB_WAVES);
+#define QWA_PREP_ROWS_BATCH(T)                                                                                            \
+    case T:                                                                                                               \
+        hipLaunchKernelGGL(k_prep_rows_batch<T>, grid, block, 0, st, qg, k, v, qn, kn, p, seqs, off, n, rows, rope_off,   \
+                           theta, eps, kv, q, gate);                                                                      \
+        break
+    switch (kvt) {
+        QWA_PREP_ROWS_BATCH(QWA_KV_F16);
+        QWA_PREP_ROWS_BATCH(QWA_KV_Q8_0);
+        QWA_PREP_ROWS_BATCH(QWA_KV_Q4_0);
+    }
+#undef QWA_PREP_ROWS_BATCH
     return hipGetLastError();
 }
 

@@ -66,6 +66,11 @@ hipError_t launch_prep_batch(const float* qg, const float* k, const float* v, co
                              const qwa_kv_pages& p, const int* seqs, int n, int nq, const int* rope_off, float theta,
                              float eps, int kvt, const qwa_kv_layer& kv, float* q, float* gate, hipStream_t st);
 
+hipError_t launch_prep_rows_batch(const float* qg, const float* k, const float* v, const float* qn, const float* kn,
+                                  const qwa_kv_pages& p, const int* seqs, const int* off, int n, int rows,
+                                  const int* rope_off, float theta, float eps, int kvt, const qwa_kv_layer& kv, float* q,
+                                  float* gate, hipStream_t st);
+
 // kv_pages.hip
 size_t pages_work_bytes(const qwa_kv_pages& p);
 hipError_t launch_pages_extend(const qwa_kv_pages& p, const int* seqs, const int* add, int n, const qwa_kv_layer* layers,
@@ -80,6 +85,12 @@ size_t batch_work_bytes(int n, int nq, int n_shared, int max_len);
 hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_layer& kv, int kvt, const qwa_kv_pages& p,
                                const int* seqs, int n, int nq, int n_shared, int max_len, uint16_t* out16,
                                const qwa_act_q8* oq, void* work, hipStream_t st);
+
+// attn_chunks.hip
+size_t prefill_batch_work_bytes(int n, int rows, int max_len);
+hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_layer& kv, int kvt, const qwa_kv_pages& p,
+                                const int* seqs, const int* off, int n, int rows, int max_len, uint16_t* out16, float* lse,
+                                void* work, hipStream_t st);
 
 // split-K decode: 16-key chunks in DEC_CLASSES fixed residue classes per KV head (chunk index mod DEC_CLASSES)
 constexpr int DEC_CLASSES = 512;

@@ -126,6 +126,13 @@ EXPORTS = {
                                                                      ctypes.POINTER(_KVPagesC), ctypes.c_void_p] +
                               [ctypes.c_int] * 4 + [ctypes.c_void_p, ctypes.POINTER(_ActQ8C), ctypes.c_void_p,
                                                     ctypes.c_size_t, ctypes.c_void_p]),
+    "qwa_attn_prep_rows_batch": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
+                                 [ctypes.c_int] * 2 + [ctypes.c_void_p] + [ctypes.c_float] * 2 +
+                                 [ctypes.c_int, ctypes.POINTER(_KVLayerC)] + [ctypes.c_void_p] * 3),
+    "qwa_attn_prefill_batch_work_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
+    "qwa_attn_prefill_batch": (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.POINTER(_KVLayerC), ctypes.c_int,
+                                                                      ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
+                               [ctypes.c_int] * 3 + [ctypes.c_void_p] * 3 + [ctypes.c_size_t, ctypes.c_void_p]),
     "qwa_deltanet_step": (ctypes.c_int, [ctypes.POINTER(_DNParamsC)] + [ctypes.c_void_p] * 4 +
                           [ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.POINTER(_ActQ8C), ctypes.c_void_p]),
     "qwa_deltanet_multi": (ctypes.c_int, [ctypes.POINTER(_DNParamsC), ctypes.c_int, ctypes.POINTER(_DNTokensC)] +
@@ -607,6 +614,39 @@ def attn_decode_batch(q, gate, kv: KVLayer, kvt, pages: KVPages, seqs, n: int, n
         _dev(q, f32, "q", size), _dev(gate, f32, "gate", size), _pool(kv, kvt), kvt, ctypes.byref(pages.c()),
         None if seqs is None else _count(seqs, n, "seqs"), n, nq, n_shared, max_len,
         _dev(out16, torch.float16, "out16", size), _act(oq), *_work(work), _stream(stream)))
+
+
+CHUNK_MAXROWS = 65536  # rows of a call on chunks
+
+
+def attn_prep_rows_batch(qg, k, v, q_norm, k_norm, pages: KVPages, seqs, off, n: int, rows: int, theta: float, eps: float, kvt,
+                         kv: KVLayer, q_out, gate, rope_off=None, stream=None) -> None:
+    """attn_prep_rows for chunks over a paged cache: batch row b (sequence seqs[b], int32, None: b) has rows off[b] ..
+    off[b + 1] - 1 (int32, n + 1 entries) of buffers of `rows` rows, the last positions of its sequence."""
+    f32, kvt, HD = torch.float32, _kvt(kvt), 256
+    _check(lib().qwa_attn_prep_rows_batch(
+        _dev(qg, f32, "qg", rows * 48 * HD), _dev(k, f32, "k", rows * N_KV * HD), _dev(v, f32, "v", rows * N_KV * HD),
+        _dev(q_norm, f32, "q_norm", HD), _dev(k_norm, f32, "k_norm", HD), ctypes.byref(pages.c()),
+        None if seqs is None else _count(seqs, n, "seqs"), _count(off, n + 1, "off"), n, rows,
+        None if rope_off is None else _count(rope_off, n, "rope_off"), theta, eps, kvt, _pool(kv, kvt),
+        _dev(q_out, f32, "q_out", rows * 24 * HD), _dev(gate, f32, "gate", rows * 24 * HD), _stream(stream)))
+
+
+def attn_prefill_batch_work_bytes(n: int, rows: int, max_len: int) -> int:
+    return int(lib().qwa_attn_prefill_batch_work_bytes(n, rows, max_len))
+
+
+def attn_prefill_batch(q, gate, kv: KVLayer, kvt, pages: KVPages, seqs, off, n: int, rows: int, max_len: int, out16, work,
+                       lse=None, stream=None) -> None:
+    """Causal attention of chunks (attn_prep_rows_batch) over a paged cache; max_len bounds the lengths: a longer sequence counts
+    as one of max_len positions.  out16: fp16 [rows, 6144]; lse (float32 [rows, 24]): the log of each row's sum of exponentials,
+    for attn_weights_batch."""
+    f32, kvt, size = torch.float32, _kvt(kvt), rows * 6144
+    _check(lib().qwa_attn_prefill_batch(
+        _dev(q, f32, "q", size), _dev(gate, f32, "gate", size), _pool(kv, kvt), kvt, ctypes.byref(pages.c()),
+        None if seqs is None else _count(seqs, n, "seqs"), _count(off, n + 1, "off"), n, rows, max_len,
+        _dev(out16, torch.float16, "out16", size), None if lse is None else _dev(lse, f32, "lse", rows * N_HEAD),
+        *_work(work), _stream(stream)))
 
 
 # ---- Gated DeltaNet ------------------------------------------------------------------------------------------------
