@@ -7,15 +7,18 @@
 //    of all blocks in a row are cut into equal slices, a workgroup each: a long sequence's decoded token and a prompt of
 //    a thousand load the chip alike.  A block that lies in several slices leaves partial states, which k_ch_join joins in the
 //    slices' order; the others are finished where they are.
-//  * A workgroup has two waves a SIMD, with a role each.  The score waves keep Q (32 rows: hi and lo part, 128 registers), take
-//    S^T = K Q^T of tile i, the exponentials, and leave P in LDS.  The value waves keep O (32 rows, 128 registers), add V^T P^T of
-//    tile i - 1, and bring the next tiles from the cache into LDS.  So each fragment of K and V that is read from LDS meets 32
-//    rows, which one wave with both Q and O has no registers for, and the exponentials of one wave run beside the other's MFMAs.
+//  * A workgroup has two waves a SIMD, with a role each.  The score waves keep Q (32 rows: hi and lo part, 128 registers), bring K
+//    into LDS and leave S^T = K Q^T of tile i there.  The value waves keep O (32 rows, 128 registers), bring V into LDS, take the
+//    exponentials of tile i - 1 and add V^T P^T.  So each fragment of K and V that is read from LDS meets 32 rows, which one wave
+//    with both Q and O has no registers for, and one wave's arithmetic runs beside the other's MFMAs.
+//  * Chunks of many blocks would convert each tile once a block: k_ch_image does it for them once, and the waves copy the images into
+//    LDS, two tiles ahead.
 //  * Scores are exact up to fp32 accumulation (K as its codes, Q / 16 as the sum of two fp16 parts), as the batched decode's are;
 //    the arithmetic of a tile, of V that is not finite and of the probabilities' range is paged_tiles.hpp's.
 // Roundings below 32 bits: the dequantized V (d * code) and the probabilities are fp16, half a step 2^-11 of the value; the sum of a
 // row's probabilities is that of the rounded ones, which P V applies, but the log of the sum is taken of the unrounded.  The
 // output is fp16.
+#include <algorithm>
 #include <type_traits>
 
 #include "chunk_plan.hpp"
@@ -25,10 +28,11 @@
 namespace qwa {
 
 // a block: its chunk's first row and number of tokens, the sequence's length and number (< 0: unknown, len 0), the block's number in
-// the chunk, its first tile in the row of all tiles, its tiles
+// the chunk, its first tile in the row of all tiles, its tiles, the positions that its last row sees, the chunk's first image (-1: none)
 struct alignas(16) ChunkBlock {
     int row0, count, len, seq;
-    int blk, begin, tiles, end;  // end: positions that its last row sees
+    int blk, begin, tiles, end;
+    int img, pad[3];
 };
 static_assert(sizeof(ChunkBlock) == CH_BLOCK_BYTES, "work buffer");
 
@@ -38,7 +42,9 @@ struct ChunkArgs {
     uint16_t* out16;
     float* lse;              // [rows][24] or none
     const ChunkBlock* blocks;
-    const int* head;         // number of blocks, number of tiles
+    const int4* list;        // chunks with images: sequence, length, first image, images
+    const int* head;         // numbers of blocks, their tiles, chunks with images, images
+    ChunkImage* images;      // [tile][KV head]
     float* part_o;           // [KV head][slice][2][rows][256]
     float4* part_ml;         // [KV head][slice][2][rows]
     int slices, prows;
@@ -74,10 +80,11 @@ __device__ __forceinline__ int ch_scan(int v, int* s_wave, int* total) {
 // earlier one's end, has none.
 constexpr int CH_PT = QWA_PAGES_MAXN;
 __global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __restrict__ seqs, const int* __restrict__ off, int n,
-                                                   int rows, int max_len, int most, ChunkBlock* __restrict__ blocks,
+                                                   int rows, int max_len, int most, int most_images, int img_tiles,
+                                                   ChunkBlock* __restrict__ blocks, int4* __restrict__ list,
                                                    int* __restrict__ head) {
     __shared__ int s_wave[CH_PT / 64];
-    __shared__ int s_end[CH_PT], s_first[CH_PT], s_count[CH_PT], s_len[CH_PT], s_seq[CH_PT], s_blk[CH_PT + 1];
+    __shared__ int s_end[CH_PT], s_first[CH_PT], s_count[CH_PT], s_len[CH_PT], s_seq[CH_PT], s_blk[CH_PT], s_img[CH_PT];
     const int t = threadIdx.x, lane = t & 63;
     int first = 0, end = 0;
     if (t < n) {
@@ -106,9 +113,17 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __
     int nb;
     const int mine = (GRP * count + CH_ROWS - 1) / CH_ROWS;
     s_blk[t] = ch_scan<CH_PT>(mine, s_wave, &nb);
-    if (t == CH_PT - 1) s_blk[CH_PT] = nb;
-    __syncthreads();
     nb = min(nb, most);  // (never more: the chunks' rows are disjoint)
+    // images, as long as there is room for them
+    const int want = mine >= CH_IMG_BLOCKS ? (s_len[t] + PF_TILE - 1) / PF_TILE : 0;
+    int all_want, images, img_used;
+    const int img = ch_scan<CH_PT>(min(want, img_tiles + 1), s_wave, &all_want);
+    const bool has = want > 0 && img + want <= img_tiles;
+    const int place = ch_scan<CH_PT>(has, s_wave, &images);
+    ch_scan<CH_PT>(has ? want : 0, s_wave, &img_used);
+    s_img[t] = has && place < most_images ? img : -1;
+    if (s_img[t] >= 0) list[place] = make_int4(s_seq[t], s_len[t], img, want);
+    __syncthreads();
     int tiles = 0;
     for (int j0 = 0; j0 < nb; j0 += CH_PT) {
         const int j = j0 + t;
@@ -128,6 +143,7 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __
             const int last = min((x.blk + 1) * CH_ROWS, GRP * x.count) - 1;
             x.end = max(0, x.len - x.count + last / GRP + 1);
             x.tiles = max(1, (x.end + PF_TILE - 1) / PF_TILE);  // (rows that see nothing are written too)
+            x.img = s_img[lo];
         }
         int all;
         x.begin = tiles + ch_scan<CH_PT>(x.tiles, s_wave, &all);
@@ -137,6 +153,8 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __
     if (t == 0) {
         head[0] = nb;
         head[1] = tiles;
+        head[2] = min(images, most_images);
+        head[3] = img_used;
     }
 }
 
@@ -154,33 +172,512 @@ __device__ __forceinline__ int ch_find(const ChunkArgs& a, int nb, int s, int* s
     return __builtin_amdgcn_readfirstlane(*s_found);
 }
 
-constexpr int CH_VD = 3;  // V fragments in flight
+// The images: a workgroup of 512 threads converts a tile of one KV head, half of them K, half V, from registers to memory.
+constexpr int CH_IMG_WGS = 2048;
+template <int KVT>
+__global__ void __launch_bounds__(512) k_ch_image(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
+    constexpr int VB = value_bytes(KVT);
+    const int t = threadIdx.x, n = a.head[2], units = a.head[3] * NKV;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const int tile = unit / NKV, g = unit % NKV;
+        int lo = 0, hi = n;  // the last chunk whose first image is at most this
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.list[mid].z <= tile) lo = mid;
+            else hi = mid;
+        }
+        const int4 c = a.list[lo];
+        const int k0 = (tile - c.z) * PF_TILE, end = c.y;
+        const int* __restrict__ table = p.table + (size_t)max(c.x, 0) * p.ld;
+        int at[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) at[h] = __builtin_amdgcn_readfirstlane(bt_place(p, table, k0 + 16 * h, end));
+        const size_t head = (size_t)g * kv.capacity;
+        ChunkImage& img = a.images[(size_t)tile * NKV + g];
+        const int dead = (at[0] < 0) | (at[1] < 0) << 1, left = end - k0;
+        BtRaw<KVT> raw;
+        if (wave < 4) {
+            const int rows[2] = {at[0] < 0 ? 16 : min(left, 16), at[1] < 0 ? 16 : min(left - 16, 16)};
+            bt_load_v<KVT>(raw, kv.v + head * VB, KVT == QWA_KV_F16 ? nullptr : kv.vs + head * 8, at, rows, t);
+            static_assert(offsetof(ChunkImage, odd) - offsetof(ChunkImage, odd_keys) == offsetof(BtOdd, tile), "BtOdd");
+            BtOdd& odd = *reinterpret_cast<BtOdd*>(img.odd_keys);
+            if ((t & 63) == 0) odd.tile[wave] = 0;  // (the wave's own, before it may be set)
+            if (t == 0) img.dead = dead;
+            bt_store_v<KVT>(raw, reinterpret_cast<_Float16*>(img.vt), odd, t, (uint32_t)dead, 1);
+        } else {
+            const int h = (wave >> 1) & 1;
+            bt_load_k<KVT>(raw, kv.k + head * VB, KVT == QWA_KV_F16 ? nullptr : kv.ks + head * 8, at[h],
+                           min(max(left - 16 * h, 0), 16), t);
+            bt_store_k<KVT>(raw, reinterpret_cast<_Float16*>(img.k), img.scales, t);
+        }
+    }
+}
+
+constexpr int CH_VD = 3;    // V fragments in flight
+constexpr int CH_RING = 3;  // tiles in LDS: the one read, and two on their way
 
 template <int KVT>
 struct ChunkLds {
-    _Float16 k[2][PF_TILE * HD];
-    _Float16 vt[2][PF_TILE * HD];
-    uint16_t scales[2][KVT == QWA_KV_F16 ? 8 : PF_TILE * 8];  // of K
-    BtOdd odd[2];                                             // of V
-    int dead[4];                                              // by tile: halves without a place
-    h8 p[2][CH_PAIRS][2][64];                                 // P^T of a tile, as operands
-    float cr[2][CH_PAIRS][2][16];                             // what O is multiplied by before it, where it is
-    int moved[2][CH_PAIRS];                                   // ... anything but 1
-    float4 ml[CH_PAIRS][2][16];                               // of a finished segment: m, l, the log's sum
+    _Float16 k[CH_RING][PF_TILE * HD];
+    _Float16 vt[CH_RING][PF_TILE * HD];
+    uint16_t scales[CH_RING][PF_TILE * 8];  // of K
+    BtOdd odd[2];                           // of V that was not an image
+    int flags[CH_RING][64];                 // of an image: its odd, dead
     union {
-        uint2 q[CH_PAIRS][16 * HD / 4];                       // a row tile's Q, one part, on its way into operands
-        float4 x[CH_PAIRS][16 * HD / 8];                      // half of a row tile's O on its way out
-    };
+        f4 s[2][2][2][64];                  // S^T of a tile: [tile & 1][row tile][half of the keys][lane]
+        float4 x[16 * HD / 8];              // half of a row tile's O on its way out
+    } pair[CH_PAIRS];
+    uint2 q[CH_PAIRS][16 * HD / 8];         // half of a row tile's Q, one part, on its way into operands
     int found;
 };
+
+// A segment: the tiles [tb, tb + nt) of a block that a workgroup walks.
+struct ChunkSegment {
+    ChunkBlock c;
+    int tb, nt, nrows, wrow0;  // rows of the chunk; the wave's first
+    int base;                  // tiles that the workgroup has walked before: tile i has place (base + i) of the rings in LDS
+};
+
+// Q / 16 of a wave's 32 rows as the B operand, hi and lo part: rows are read in runs of 512 bytes, their fp16 pieces go to unit
+// (4 s + lg, row ^ (4 s + lg) % 16) of the wave's part of LDS and come back as the lane's fragments s.
+template <int KVT>
+__device__ __forceinline__ void ch_load_q(h8 (&qb)[2][2][8], const ChunkArgs& a, const ChunkSegment& sg, int g, uint2* lds_q,
+                                          int lane) {
+    const int i16 = lane & 15, lg = lane >> 4, l5 = lane & 31, half = l5 & 1, u = l5 >> 1;
+    uint8_t* const area = reinterpret_cast<uint8_t*>(lds_q);
+    float4 x[2][8];
+    auto load = [&](int r) {  // round r = 2 * row tile + half of the dims
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int row = min(sg.wrow0 + 16 * (r >> 1) + 2 * k + (lane >> 5), sg.nrows - 1);
+            x[r & 1][k] = *reinterpret_cast<const float4*>(
+                a.q + ((size_t)(sg.c.row0 + row / GRP) * NH + g * GRP + row % GRP) * HD + 128 * (r & 1) + 4 * l5);
+        }
+    };
+    load(0);
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int rt = r >> 1;
+        if (r < 3) load(r + 1);
+        __builtin_amdgcn_sched_barrier(0);  // (registers: one round ahead)
+#pragma unroll
+        for (int part = 0; part < 2; part++) {
+            auto piece = [&](float v, float f) { return part ? q_lo(v * f) : q_hi(v * f); };
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int row = 2 * k + (lane >> 5);
+                const float f = sg.wrow0 + 16 * rt + row < sg.nrows ? 0.0625f : 0.0f;
+                uint32_t w0 = h2_bits(h2{piece(x[r & 1][k].x, f), piece(x[r & 1][k].y, f)});
+                uint32_t w1 = h2_bits(h2{piece(x[r & 1][k].z, f), piece(x[r & 1][k].w, f)});
+                if constexpr (KVT == QWA_KV_Q4_0) {
+                    // the operand's order [0, 4, 1, 5, 2, 6, 3, 7]: the even lane makes the first two words, the odd one the rest
+                    const uint32_t mine = half ? w1 : w0;
+                    const uint32_t other = __builtin_amdgcn_update_dpp(0, half ? w0 : w1, 0xB1, 0xF, 0xF, true);
+                    const uint32_t lo = half ? other : mine, hi = half ? mine : other;
+                    w0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+                    w1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+                }
+                *reinterpret_cast<uint2*>(area + 16 * (16 * u + (row ^ u)) + 8 * half) = make_uint2(w0, w1);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+                qb[rt][part][4 * (r & 1) + s] =
+                    *reinterpret_cast<const h8*>(area + 16 * (16 * (4 * s + lg) + (i16 ^ (4 * s + lg))));
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// S^T = K Q^T of a tile: lane (row i16 of row tile rt) gets keys 16 kt + 4 lg + e.  The K fragments of a step are read while the
+// step before multiplies; a row tile's products are scaled while the other's are on their way.
+template <int KVT>
+__device__ __forceinline__ void ch_scores(f4 (&sc)[2][2], const h8 (&qb)[2][2][8], const _Float16* Ks, const _Float16* Sc, int i16,
+                                          int lg) {
+    constexpr bool SC = KVT != QWA_KV_F16;
+    f4 T[2][2];
+    h4 ks[2][2];
+    h8 kf[2][2];
+    auto scale = [&](int st, int rt) {
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) sc[rt][kt][e] = fmaf((float)ks[st & 1][kt][e], T[rt][kt][e], sc[rt][kt][e]);
+            // (the sums stay where they are: put off past the last block, they kept all products, and spilled)
+            asm volatile("" : "+v"(sc[rt][kt]));
+        }
+    };
+    auto read = [&](int st) {
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) kf[st & 1][kt] = lds_h8(Ks + 8 * (32 * (4 * st + lg) + 16 * kt + (i16 ^ (2 * st))));
+        if constexpr (SC)
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+                ks[st & 1][kt] = *reinterpret_cast<const h4*>(Sc + 8 * (16 * kt + 4 * (st >> 1) + lg) + 4 * (st & 1));
+    };
+    auto multiply = [&](int st, int rt) {
+#pragma unroll
+        for (int part = 1; part >= 0; part--)
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (SC) T[rt][kt] = mfma16(kf[st & 1][kt], qb[rt][part][st], part ? zero : T[rt][kt]);
+                else sc[rt][kt] = mfma16(kf[st & 1][kt], qb[rt][part][st], sc[rt][kt]);
+            }
+    };
+#pragma unroll
+    for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) sc[rt][kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    read(0);
+#pragma unroll
+    for (int st = 0; st < 8; st++) {
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(st, 0);
+        if (SC && st > 0) scale(st - 1, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (st + 1 < 8) read(st + 1);
+        multiply(st, 1);
+        if (SC) scale(st, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (SC) scale(7, 1);
+}
+
+// The pool positions of a tile's halves, 64 tiles ahead: lane l has those of tile l.
+struct ChunkPlaces {
+    int ahead[2], tile = 0;
+    __device__ __forceinline__ void next(int (&at)[2], const qwa_kv_pages& p, const int* __restrict__ table, int tb, int end,
+                                         int lane) {
+        if ((tile & 63) == 0)
+#pragma unroll
+            for (int h = 0; h < 2; h++) ahead[h] = bt_place(p, table, (tb + tile + lane) * PF_TILE + 16 * h, end);
+#pragma unroll
+        for (int h = 0; h < 2; h++) at[h] = __builtin_amdgcn_readlane(ahead[h], tile & 63);
+        tile++;
+    }
+};
+
+// a wave's part of 16 KB on their way into LDS, without registers
+__device__ __forceinline__ void ch_copy(const void* lds, const void* src, int wave, int lane) {
+#pragma unroll
+    for (int c = 0; c < 16 / CH_PAIRS; c++) {
+        const int i = wave + CH_PAIRS * c;
+        dma_sv<16>(lds_addr(lds) + 1024 * i, src, (uint32_t)(1024 * i + 16 * lane));
+    }
+}
+
+// The score waves' segment.  Between barriers i and i + 1: K of tile i + 1 from registers (or tile i + 2 of the images) into LDS,
+// scores of tile i.
+template <int KVT, bool IMG>
+__device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArgs& a, const qwa_kv_layer& kv,
+                                              const qwa_kv_pages& p, const ChunkSegment& sg, int g, int pair, int t) {
+    constexpr bool SC = KVT != QWA_KV_F16;
+    const int lane = t & 63;
+    const int* __restrict__ table = p.table + (size_t)max(sg.c.seq, 0) * p.ld;
+    const size_t head = (size_t)g * kv.capacity;
+    const uint8_t* const kh = kv.k + head * value_bytes(KVT);
+    const uint16_t* const ksh = SC ? kv.ks + head * 8 : nullptr;
+    const ChunkImage* const img = a.images + (size_t)(max(sg.c.img, 0) + sg.tb) * NKV + g;
+    BtRaw<KVT> rk;
+    ChunkPlaces places;
+    auto load = [&](int i) {
+        int at[2];
+        places.next(at, p, table, sg.tb, sg.c.end, lane);
+        const int h = pair >> 1, left = sg.c.end - (sg.tb + i) * PF_TILE - 16 * h;
+        bt_load_k<KVT>(rk, kh, ksh, h ? at[1] : at[0], min(max(left, 0), 16), t);
+    };
+    auto slot = [&](int i) { return (sg.base + i) % CH_RING; };
+    auto copy = [&](int i) {
+        const ChunkImage& x = img[(size_t)i * NKV];
+        ch_copy(lds.k[slot(i)], x.k, pair, lane);
+        if (SC && pair < 2) dma_sv<4>(lds_addr(lds.scales[slot(i)]) + 256 * pair, x.scales, (uint32_t)(256 * pair + 4 * lane));
+    };
+    auto landed = [&](bool last) {  // all copies (but the last one, if there is another on its way)
+        if (last) wait_vmcnt<0>();
+        else if (SC && pair < 2) wait_vmcnt<16 / CH_PAIRS + 1>();
+        else wait_vmcnt<16 / CH_PAIRS>();
+    };
+    if constexpr (!IMG) load(0);
+    h8 qb[2][2][8];
+    ch_load_q<KVT>(qb, a, sg, g, lds.q[pair], lane);
+    if constexpr (IMG) {
+        wait_vmcnt<0>();  // from here on vmcnt counts only the copies
+        copy(0);
+        if (sg.nt > 1) copy(1);
+        landed(sg.nt <= 1);
+    } else {
+        bt_store_k<KVT>(rk, lds.k[slot(0)], lds.scales[slot(0)], t);
+        if (sg.nt > 1) load(1);
+    }
+    __syncthreads();
+    for (int i = 0; i < sg.nt; i++) {
+        if constexpr (IMG) {
+            if (i + 2 < sg.nt) copy(i + 2);
+        } else {
+            if (i + 1 < sg.nt) bt_store_k<KVT>(rk, lds.k[slot(i + 1)], lds.scales[slot(i + 1)], t);
+            if (i + 2 < sg.nt) load(i + 2);
+        }
+        if (sg.wrow0 < sg.nrows) {
+            // (an opaque copy of the lane: the LDS addresses, kept across the tiles, spilled)
+            int ol = lane;
+            asm volatile("" : "+v"(ol));
+            f4 sc[2][2];
+            ch_scores<KVT>(sc, qb, lds.k[slot(i)], reinterpret_cast<const _Float16*>(lds.scales[slot(i)]), ol & 15, ol >> 4);
+#pragma unroll
+            for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) lds.pair[pair].s[i & 1][rt][kt][ol] = sc[rt][kt];
+        }
+        if constexpr (IMG) landed(i + 2 >= sg.nt);
+        __syncthreads();
+    }
+}
+
+// The value waves' segment.  Between barriers i and i + 1: V of tile i from registers (or tile i + 1 of the images) into LDS,
+// exponentials and P V of tile i - 1; behind the last barrier the last tile's, and the rows' results.
+template <int KVT, bool IMG, bool LSE>
+__device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArgs& a, const qwa_kv_layer& kv,
+                                              const qwa_kv_pages& p, const ChunkSegment& sg, int g, int pair, size_t part, int t) {
+    constexpr bool SC = KVT != QWA_KV_F16;
+    const int lane = t & 63, i16 = lane & 15, lg = lane >> 4;
+    const int* __restrict__ table = p.table + (size_t)max(sg.c.seq, 0) * p.ld;
+    const size_t head = (size_t)g * kv.capacity;
+    const uint8_t* const vh = kv.v + head * value_bytes(KVT);
+    const uint16_t* const vsh = SC ? kv.vs + head * 8 : nullptr;
+    const ChunkImage* const img = a.images + (size_t)(max(sg.c.img, 0) + sg.tb) * NKV + g;
+    const bool rows_here = sg.wrow0 < sg.nrows;
+    int vis[2], vmin = 0x7fffffff;  // positions that this lane's rows see, the fewest that one of the wave's does
+#pragma unroll
+    for (int rt = 0; rt < 2; rt++) {
+        const int r = sg.wrow0 + 16 * rt + i16;
+        vis[rt] = r < sg.nrows ? sg.c.len - sg.c.count + r / GRP + 1 : 0;
+        if (r < sg.nrows) vmin = min(vmin, vis[rt]);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
+    vmin = __builtin_amdgcn_readfirstlane(vmin);
+    BtRaw<KVT> rv;
+    ChunkPlaces places;
+    uint32_t dead = 0;  // halves without a place, two bits a tile: tile i - 1, tile i, ...
+    auto load = [&](int i) {
+        int at[2];
+        places.next(at, p, table, sg.tb, sg.c.end, lane);
+        const int left = sg.c.end - (sg.tb + i) * PF_TILE;
+        const int rows[2] = {at[0] < 0 ? 16 : min(left, 16), at[1] < 0 ? 16 : min(left - 16, 16)};
+        bt_load_v<KVT>(rv, vh, vsh, at, rows, t);
+        return (uint32_t)((at[0] < 0) | (at[1] < 0) << 1);
+    };
+    auto slot = [&](int i) { return (sg.base + i) % CH_RING; };
+    auto copy = [&](int i) {
+        const ChunkImage& x = img[(size_t)i * NKV];
+        ch_copy(lds.vt[slot(i)], x.vt, pair, lane);
+        if (pair == 0) dma_sv<4>(lds_addr(lds.flags[slot(i)]), x.odd, (uint32_t)(4 * lane));
+    };
+    auto landed = [&](bool last) {
+        if (last) wait_vmcnt<0>();
+        else if (pair == 0) wait_vmcnt<16 / CH_PAIRS + 1>();
+        else wait_vmcnt<16 / CH_PAIRS>();
+    };
+    f4 o[2][16];
+    float m[2], l[2], lx[2];
+#pragma unroll
+    for (int rt = 0; rt < 2; rt++) {
+        m[rt] = -INFINITY;
+        l[rt] = lx[rt] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if constexpr (IMG) {
+        wait_vmcnt<0>();  // from here on vmcnt counts only the copies
+        copy(0);
+    } else {
+        dead = load(0) << 2;
+    }
+    __syncthreads();
+    for (int i = 0; i <= sg.nt; i++) {
+        // (opaque copies: LDS addresses kept across the tiles took the registers of O)
+        int ol = lane;
+        asm volatile("" : "+v"(ol));
+        const int oi = ol & 15, og = ol >> 4;
+        if constexpr (IMG) {
+            if (i + 1 < sg.nt) copy(i + 1);
+        } else {
+            if (i < sg.nt)
+                bt_store_v<KVT>(rv, lds.vt[slot(i)], lds.odd[(sg.base + i) & 1], 64 * pair + ol, (dead >> 2) & 3, sg.base + i);
+            if (i + 1 < sg.nt) dead |= load(i + 1) << 4;
+        }
+        if (i > 0 && rows_here) {
+            const int b = (i - 1) & 1, k0 = (sg.tb + i - 1) * PF_TILE;
+            int gone = (int)(dead & 3);
+            const int4 odd = *reinterpret_cast<const int4*>(IMG ? lds.flags[slot(i - 1)] : lds.odd[(sg.base + i - 1) & 1].tile);
+            if constexpr (IMG) gone = __builtin_amdgcn_readfirstlane(lds.flags[slot(i - 1)][4]);
+            f4 sc[2][2];
+#pragma unroll
+            for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) sc[rt][kt] = lds.pair[pair].s[b][rt][kt][ol];
+            if (k0 + PF_TILE > vmin || gone != 0) {
+#pragma unroll
+                for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+                    for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            sc[rt][kt][e] =
+                                k0 + 16 * kt + 4 * og + e < vis[rt] && !((gone >> kt) & 1) ? sc[rt][kt][e] : -INFINITY;
+            }
+            float cr[2], ref[2];
+#pragma unroll
+            for (int rt = 0; rt < 2; rt++) {
+                float mx = max3f(max3f(-INFINITY, sc[rt][0][0], sc[rt][0][1]), sc[rt][0][2], sc[rt][0][3]);
+                mx = rows_max(max3f(max3f(mx, sc[rt][1][0], sc[rt][1][1]), sc[rt][1][2], sc[rt][1][3]));
+                const float mx2 = mx * PF_LOG2E, mn = mx2 > m[rt] + BT_HEAD ? mx2 - BT_RAISE : m[rt];
+                cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] - mn);
+                ref[rt] = mn == -INFINITY ? 0.0f : mn;  // a row that saw nothing keeps l = 0, O = 0
+                m[rt] = mn;
+            }
+            // the V fragments' reads begin while the exponentials are taken
+            const _Float16* vrow = lds.vt[slot(i - 1)] + 8 * (256 * og + oi);
+            h8 vf[CH_VD];
+#pragma unroll
+            for (int dt = 0; dt < CH_VD - 1; dt++) vf[dt] = lds_h8(vrow + 8 * 16 * dt);
+            h8 pb[2];
+#pragma unroll
+            for (int rt = 0; rt < 2; rt++) {
+                float rx = 0.0f, rs = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float x = fast_exp2(fmaf(sc[rt][e >> 2][e & 3], PF_LOG2E, -ref[rt]));
+                    pb[rt][e] = (_Float16)x;
+                    if (LSE) rx += x;
+                }
+                // the sum of the rounded probabilities, the weights that P V applies
+                const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) rs = __builtin_amdgcn_fdot2(h2{pb[rt][e], pb[rt][e + 1]}, one2, rs, false);
+                l[rt] = l[rt] * cr[rt] + rs;
+                if (LSE) lx[rt] = lx[rt] * cr[rt] + rx;
+            }
+            if (__any(cr[0] != 1.0f || cr[1] != 1.0f)) {
+#pragma unroll
+                for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+                    for (int dt = 0; dt < 16; dt++) o[rt][dt] *= cr[rt];
+            }
+            // O^T += V^T P^T
+#pragma unroll
+            for (int dt = 0; dt < 16; dt++) {
+                if (dt + CH_VD - 1 < 16) vf[(dt + CH_VD - 1) % CH_VD] = lds_h8(vrow + 8 * 16 * (dt + CH_VD - 1));
+#pragma unroll
+                for (int rt = 0; rt < 2; rt++) o[rt][dt] = mfma16(vf[dt % CH_VD], pb[rt], o[rt][dt]);
+            }
+            // a dim is NaN in the rows that see a value of it that is not finite
+            const int mark = IMG ? 1 : sg.base + i - 1;
+            if (__builtin_amdgcn_readfirstlane(odd.x == mark || odd.y == mark || odd.z == mark || odd.w == mark)) {
+                const int of[4] = {odd.x, odd.y, odd.z, odd.w};
+                const uint8_t* const keys_of = IMG ? img[(size_t)(i - 1) * NKV].odd_keys : lds.odd[(sg.base + i - 1) & 1].keys;
+                uint32_t seen[2][2] = {};
+#pragma unroll
+                for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+                    for (int k = 0; k < PF_TILE; k++) {
+                        const int cb = k / 4 % 4, h = k / 16;
+                        if (of[cb] == mark && k0 + k < vis[rt] && !((gone >> h) & 1))
+                            seen[rt][cb / 2] |= 1u << (8 * (2 * (cb & 1) + h) + k % 4);
+                    }
+#pragma unroll
+                for (int dt = 0; dt < 16; dt++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int dim = 8 * (16 * (dt & 1) + 4 * og + e) + (dt >> 1);
+                        const uint2 keys = *reinterpret_cast<const uint2*>(keys_of + 8 * dim);
+#pragma unroll
+                        for (int rt = 0; rt < 2; rt++)
+                            o[rt][dt][e] = ((keys.x & seen[rt][0]) | (keys.y & seen[rt][1])) != 0 ? NAN : o[rt][dt][e];
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if constexpr (IMG) wait_vmcnt<0>();
+            }
+        }
+        dead >>= 2;
+        if (i < sg.nt) {
+            // (V of tile i, sent before that of tile i + 1)
+            if constexpr (IMG) landed(i + 1 >= sg.nt);
+            __syncthreads();
+        }
+    }
+    if (!rows_here) return;
+    // O by way of LDS, half of a row tile's dims at a time, so that rows are written as they lie in memory
+    const bool whole = sg.nt == sg.c.tiles;
+    float4* const area = lds.pair[pair].x;
+    const int u = lane & 31;
+    float4 gv[2][8];
+    auto place = [&](int r, int k) {  // output row k of round r = 2 * row tile + half of the dims
+        const int row = min(sg.wrow0 + 16 * (r >> 1) + 2 * k + (lane >> 5), sg.nrows - 1);
+        return ((size_t)(sg.c.row0 + row / GRP) * NH + g * GRP + row % GRP) * HD + 128 * (r & 1) + 4 * u;
+    };
+    auto gates = [&](int r) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) gv[r & 1][k] = *reinterpret_cast<const float4*>(a.gate + place(r, k));
+    };
+    if (whole) gates(0);
+#pragma unroll
+    for (int rt = 0; rt < 2; rt++) {
+        const float lt = rows_sum(l[rt]), lxt = LSE ? rows_sum(lx[rt]) : 0.0f;
+        const float il = whole ? (lt == 0.0f ? 0.0f : 1.0f / lt) : 1.0f;
+        const int r0 = sg.wrow0 + 16 * rt + i16;
+        if (lg == 0 && r0 < sg.nrows) {
+            if (!whole) a.part_ml[part + r0 - CH_ROWS * sg.c.blk] = make_float4(m[rt], lt, lxt, 0.0f);
+            else if (LSE)
+                a.lse[(size_t)(sg.c.row0 + r0 / GRP) * NH + g * GRP + r0 % GRP] =
+                    lxt == 0.0f ? -INFINITY : (m[rt] + __log2f(lxt)) * 0.6931471805599453f;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int r = 2 * rt + e;
+            if (whole && r < 3) gates(r + 1);
+            // o[rt][2 k + e][j] is dim 8 x + k, x = 16 e + 4 lg + j: unit 2 (4 lg + j) + k / 4 of the half
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    area[32 * i16 + ((2 * (4 * lg + j) + h) ^ (i16 & 7))] =
+                        make_float4(o[rt][8 * h + e][j] * il, o[rt][8 * h + 2 + e][j] * il, o[rt][8 * h + 4 + e][j] * il,
+                                    o[rt][8 * h + 6 + e][j] * il);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int xr = 2 * k + (lane >> 5), row = sg.wrow0 + 16 * rt + xr;
+                const float4 v = area[32 * xr + (u ^ (xr & 7))];
+                if (whole) {
+                    const float4 gt = gv[r & 1][k];
+                    const uint2 w = make_uint2(
+                        (uint32_t)f2h_bits(v.x * sigmoid(gt.x)) | ((uint32_t)f2h_bits(v.y * sigmoid(gt.y)) << 16),
+                        (uint32_t)f2h_bits(v.z * sigmoid(gt.z)) | ((uint32_t)f2h_bits(v.w * sigmoid(gt.w)) << 16));
+                    if (row < sg.nrows) *reinterpret_cast<uint2*>(a.out16 + place(r, k)) = w;
+                } else if (row < sg.nrows) {
+                    *reinterpret_cast<float4*>(a.part_o + (part + row - CH_ROWS * sg.c.blk) * HD + 128 * e + 4 * u) = v;
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
 
 template <int KVT, bool LSE>
 __global__ void __launch_bounds__(128 * CH_PAIRS) __attribute__((amdgpu_waves_per_eu(2, 2)))
 k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     __shared__ __attribute__((aligned(16))) ChunkLds<KVT> lds;
-    constexpr bool SC = KVT != QWA_KV_F16;
-    const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, lg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int pair = wave & (CH_PAIRS - 1);
     // workgroups 8 apart run on one XCD: each has consecutive slices of one head, whose tiles its L2 then holds
     int unit = blockIdx.x;
@@ -191,375 +688,36 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     if (w >= slices) return;
     int s = ch_cut(w, tiles, slices);
     const int s_begin = s, s_end = ch_cut(w + 1, tiles, slices);
+    if (threadIdx.x < 8) lds.odd[threadIdx.x >> 2].tile[threadIdx.x & 3] = -1;
     int j = ch_find(a, nb, s, &lds.found);
-    const size_t head = (size_t)g * kv.capacity;
-    const uint8_t* const kh = kv.k + head * value_bytes(KVT);
-    const uint8_t* const vh = kv.v + head * value_bytes(KVT);
-    const uint16_t* const ksh = SC ? kv.ks + head * 8 : nullptr;
-    const uint16_t* const vsh = SC ? kv.vs + head * 8 : nullptr;
-
-    auto walk = [&](auto role) __attribute__((always_inline)) {
-        constexpr bool VALUES = decltype(role)::value;
-        while (s < s_end) {
-            const ChunkBlock c = a.blocks[j];
-            const int tb = s - c.begin, nt = min(s_end, c.begin + c.tiles) - s;
-            const int end = __builtin_amdgcn_readfirstlane(c.end), nrows = __builtin_amdgcn_readfirstlane(GRP * c.count);
-            const int wrow0 = __builtin_amdgcn_readfirstlane(CH_ROWS * c.blk) + 32 * pair;
-            const bool rows_here = wrow0 < nrows;
-            int vis[2];  // positions that this lane's rows see
-#pragma unroll
-            for (int rt = 0; rt < 2; rt++) {
-                const int r = wrow0 + 16 * rt + i16;
-                vis[rt] = r < nrows ? c.len - c.count + r / GRP + 1 : 0;
-            }
-            if constexpr (VALUES) {
-                const int* __restrict__ table = p.table + (size_t)max(c.seq, 0) * p.ld;
-                BtRaw<KVT> rk, rv;
-                // the pool positions of the tiles' halves, 64 tiles ahead: lane l has those of tile l
-                int ahead[2], at[2], tile = 0;
-                auto place = [&]() {
-                    if ((tile & 63) == 0)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) ahead[h] = bt_place(p, table, (tb + tile + lane) * PF_TILE + 16 * h, end);
-#pragma unroll
-                    for (int h = 0; h < 2; h++) at[h] = __builtin_amdgcn_readlane(ahead[h], tile & 63);
-                    tile++;
-                };
-                auto bits = [&]() { return (uint32_t)((at[0] < 0) | (at[1] < 0) << 1); };
-                auto load_k = [&](int i) {
-                    const int h = pair >> 1, left = end - (tb + i) * PF_TILE - 16 * h;
-                    bt_load_k<KVT>(rk, kh, ksh, h ? at[1] : at[0], min(max(left, 0), 16), t);
-                };
-                auto load_v = [&](int i) {
-                    const int left = end - (tb + i) * PF_TILE;
-                    const int rows[2] = {at[0] < 0 ? 16 : min(left, 16), at[1] < 0 ? 16 : min(left - 16, 16)};
-                    bt_load_v<KVT>(rv, vh, vsh, at, rows, t);
-                };
-                auto store_k = [&](int i, uint32_t dead) {
-                    bt_store_k<KVT>(rk, lds.k[i & 1], lds.scales[i & 1], t);
-                    if (wave == CH_PAIRS && lane == 0) lds.dead[i & 3] = (int)dead;
-                };
-                f4 o[2][16];
-#pragma unroll
-                for (int rt = 0; rt < 2; rt++)
-#pragma unroll
-                    for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-                place();
-                load_k(0);
-                load_v(0);
-                uint32_t dead_v = bits(), dead_k = dead_v;
-                if (wave == CH_PAIRS && lane < 8) lds.odd[lane >> 2].tile[lane & 3] = -1;
-                store_k(0, dead_k);
-                if (nt > 1) {
-                    place();
-                    load_k(1);
-                    dead_k = bits();
-                }
-                __syncthreads();
-                for (int i = 0; i <= nt; i++) {
-                    // K of tile i + 1 and V of tile i into LDS, then their successors' loads
-                    if (i + 1 < nt) store_k(i + 1, dead_k);
-                    if (i < nt) bt_store_v<KVT>(rv, lds.vt[i & 1], lds.odd[i & 1], t, dead_v, i);
-                    if (i + 1 < nt) {
-                        load_v(i + 1);
-                        dead_v = dead_k;
-                    }
-                    if (i + 2 < nt) {
-                        place();
-                        load_k(i + 2);
-                        dead_k = bits();
-                    }
-                    if (i > 0 && rows_here) {
-                        const int b = (i - 1) & 1;
-                        if (__builtin_amdgcn_readfirstlane(lds.moved[b][pair])) {
-#pragma unroll
-                            for (int rt = 0; rt < 2; rt++) {
-                                const float f = lds.cr[b][pair][rt][i16];
-#pragma unroll
-                                for (int dt = 0; dt < 16; dt++) o[rt][dt] *= f;
-                            }
-                        }
-                        h8 pb[2];
-#pragma unroll
-                        for (int rt = 0; rt < 2; rt++) pb[rt] = lds.p[b][pair][rt][lane];
-                        // O^T += V^T P^T
-                        const _Float16* vrow = lds.vt[b] + 8 * (256 * lg + i16);
-                        h8 vf[CH_VD];
-#pragma unroll
-                        for (int dt = 0; dt < CH_VD - 1; dt++) vf[dt] = lds_h8(vrow + 8 * 16 * dt);
-#pragma unroll
-                        for (int dt = 0; dt < 16; dt++) {
-                            if (dt + CH_VD - 1 < 16) vf[(dt + CH_VD - 1) % CH_VD] = lds_h8(vrow + 8 * 16 * (dt + CH_VD - 1));
-#pragma unroll
-                            for (int rt = 0; rt < 2; rt++) o[rt][dt] = mfma16(vf[dt % CH_VD], pb[rt], o[rt][dt]);
-                        }
-                        // a dim is NaN in the rows that see a value of it that is not finite
-                        const int4 of4 = *reinterpret_cast<const int4*>(lds.odd[b].tile);
-                        if (__builtin_amdgcn_readfirstlane(of4.x == i - 1 || of4.y == i - 1 || of4.z == i - 1 || of4.w == i - 1)) {
-                            const int of[4] = {of4.x, of4.y, of4.z, of4.w};
-                            const int k0 = (tb + i - 1) * PF_TILE, dead = lds.dead[(i - 1) & 3];
-                            uint32_t seen[2][2] = {};
-#pragma unroll
-                            for (int rt = 0; rt < 2; rt++)
-#pragma unroll
-                                for (int k = 0; k < PF_TILE; k++) {
-                                    const int cb = k / 4 % 4, h = k / 16;
-                                    if (of[cb] == i - 1 && k0 + k < vis[rt] && !((dead >> h) & 1))
-                                        seen[rt][cb / 2] |= 1u << (8 * (2 * (cb & 1) + h) + k % 4);
-                                }
-#pragma unroll
-                            for (int dt = 0; dt < 16; dt++) {
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const int dim = 8 * (16 * (dt & 1) + 4 * lg + e) + (dt >> 1);
-                                    const uint2 keys = *reinterpret_cast<const uint2*>(&lds.odd[b].keys[8 * dim]);
-#pragma unroll
-                                    for (int rt = 0; rt < 2; rt++)
-                                        o[rt][dt][e] =
-                                            ((keys.x & seen[rt][0]) | (keys.y & seen[rt][1])) != 0 ? NAN : o[rt][dt][e];
-                                }
-                                __builtin_amdgcn_sched_barrier(0);
-                            }
-                        }
-                    }
-                    if (i < nt) __syncthreads();
-                }
-                // O by way of LDS, half of the dims at a time, so that rows are written as they lie in memory
-                const bool whole = nt == c.tiles;
-                const size_t part = (((size_t)g * a.slices + w) * 2 + (s == s_begin ? 0 : 1)) * a.prows;
-                if (rows_here) {
-                    float4* const area = lds.x[pair];
-#pragma unroll
-                    for (int rt = 0; rt < 2; rt++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            // o[rt][2 k + e][j] is dim 8 x + k, x = 16 e + 4 lg + j: unit 2 (4 lg + j) + k / 4 of the half
-#pragma unroll
-                            for (int jj = 0; jj < 4; jj++)
-#pragma unroll
-                                for (int h = 0; h < 2; h++)
-                                    area[32 * i16 + ((2 * (4 * lg + jj) + h) ^ (i16 & 7))] =
-                                        make_float4(o[rt][8 * h + e][jj], o[rt][8 * h + 2 + e][jj], o[rt][8 * h + 4 + e][jj],
-                                                    o[rt][8 * h + 6 + e][jj]);
-                            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
-                            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                            for (int k = 0; k < 8; k++) {
-                                const int xr = 2 * k + (lane >> 5), u = lane & 31, r = wrow0 + 16 * rt + xr;
-                                const float4 v = area[32 * xr + (u ^ (xr & 7))];
-                                if (r < nrows) {
-                                    const int dim = 128 * e + 4 * u;
-                                    if (whole) {
-                                        const size_t at0 = ((size_t)(c.row0 + r / GRP) * NH + g * GRP + r % GRP) * HD + dim;
-                                        const float l = lds.ml[pair][rt][xr].y, il = l == 0.0f ? 0.0f : 1.0f / l;
-                                        const float4 gv = *reinterpret_cast<const float4*>(a.gate + at0);
-                                        *reinterpret_cast<uint2*>(a.out16 + at0) =
-                                            make_uint2((uint32_t)f2h_bits(v.x * il * sigmoid(gv.x)) |
-                                                           ((uint32_t)f2h_bits(v.y * il * sigmoid(gv.y)) << 16),
-                                                       (uint32_t)f2h_bits(v.z * il * sigmoid(gv.z)) |
-                                                           ((uint32_t)f2h_bits(v.w * il * sigmoid(gv.w)) << 16));
-                                    } else {
-                                        *reinterpret_cast<float4*>(a.part_o + (part + r - CH_ROWS * c.blk) * HD + dim) = v;
-                                    }
-                                }
-                            }
-                            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                            __builtin_amdgcn_wave_barrier();
-                        }
-#pragma unroll
-                    for (int rt = 0; rt < 2; rt++) {
-                        const int r = wrow0 + 16 * rt + i16;
-                        if (lg == 0 && r < nrows) {
-                            const float4 ml = lds.ml[pair][rt][i16];
-                            if (!whole) a.part_ml[part + r - CH_ROWS * c.blk] = ml;
-                            else if (LSE)
-                                a.lse[(size_t)(c.row0 + r / GRP) * NH + g * GRP + r % GRP] =
-                                    ml.z == 0.0f ? -INFINITY : (ml.x + __log2f(ml.z)) * 0.6931471805599453f;
-                        }
-                    }
-                }
-                __syncthreads();
-            } else {
-                // Q / 16 as the B operand, hi and lo part: a row is read as one kilobyte, its fp16 pieces go to unit (s, lg,
-                // row ^ (4 s + lg) % 16) of the wave's part of LDS and come back as the lane's fragments s
-                h8 qb[2][2][8];
-#pragma unroll
-                for (int rt = 0; rt < 2; rt++) {
-                    float4 x[16];
-#pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        const int rk = min(wrow0 + 16 * rt + k, nrows - 1);
-                        x[k] = *reinterpret_cast<const float4*>(
-                            a.q + ((size_t)(c.row0 + rk / GRP) * NH + g * GRP + rk % GRP) * HD + 4 * lane);
-                    }
-                    uint8_t* const area = reinterpret_cast<uint8_t*>(lds.q[pair]);
-                    const int u = lane >> 1, half = lane & 1;  // piece u = 4 s + lg, dims 4 half .. 4 half + 3 of it
-#pragma unroll
-                    for (int part = 0; part < 2; part++) {
-                        auto piece = [&](float v, float f) { return part ? q_lo(v * f) : q_hi(v * f); };
-#pragma unroll
-                        for (int k = 0; k < 16; k++) {
-                            const float f = wrow0 + 16 * rt + k < nrows ? 0.0625f : 0.0f;
-                            uint32_t w0 = h2_bits(h2{piece(x[k].x, f), piece(x[k].y, f)});
-                            uint32_t w1 = h2_bits(h2{piece(x[k].z, f), piece(x[k].w, f)});
-                            if constexpr (KVT == QWA_KV_Q4_0) {
-                                // the operand's order [0, 4, 1, 5, 2, 6, 3, 7]: the even lane makes the first two words, the odd
-                                // one the rest
-                                const uint32_t mine = half ? w1 : w0;
-                                const uint32_t other = __builtin_amdgcn_update_dpp(0, half ? w0 : w1, 0xB1, 0xF, 0xF, true);
-                                const uint32_t lo = half ? other : mine, hi = half ? mine : other;
-                                w0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
-                                w1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-                            }
-                            *reinterpret_cast<uint2*>(area + 16 * (16 * u + (k ^ (u & 15))) + 8 * half) = make_uint2(w0, w1);
-                        }
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
-                        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            qb[rt][part][k] =
-                                *reinterpret_cast<const h8*>(area + 16 * (16 * (4 * k + lg) + (i16 ^ ((4 * k + lg) & 15))));
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                        __builtin_amdgcn_wave_barrier();
-                    }
-                }
-                int vmin = 0x7fffffff;
-#pragma unroll
-                for (int rt = 0; rt < 2; rt++)
-                    if (wrow0 + 16 * rt + i16 < nrows) vmin = min(vmin, vis[rt]);
-#pragma unroll
-                for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
-                vmin = __builtin_amdgcn_readfirstlane(vmin);
-                float m[2], l[2], lx[2];
-#pragma unroll
-                for (int rt = 0; rt < 2; rt++) {
-                    m[rt] = -INFINITY;
-                    l[rt] = lx[rt] = 0.0f;
-                }
-                __syncthreads();
-                for (int i = 0; i < nt; i++) {
-                    if (rows_here) {
-                        const int k0 = (tb + i) * PF_TILE, b = i & 1;
-                        const _Float16* Ks = lds.k[b];
-                        const _Float16* Sc = reinterpret_cast<const _Float16*>(lds.scales[b]);
-                        // S^T = K Q^T: lane (row i16 of row tile rt) gets keys k0 + 16 kt + 4 lg + e; the K fragments of a step
-                        // are read while the step before multiplies, whose product is scaled while the next one is on its way
-                        f4 sc[2][2] = {}, T[2][2][2];
-                        h8 ks[2];  // scales of blocks s - 1 and s, s even, or s and s + 1
-                        auto scale = [&](int st, int rt, int kt) {
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                sc[rt][kt][e] = fmaf((float)ks[kt][4 * (st & 1) + e], T[st & 1][rt][kt][e], sc[rt][kt][e]);
-                        };
-                        auto kfrag = [&](int st, int kt) {
-                            return lds_h8(Ks + 8 * (32 * (4 * st + lg) + 16 * kt + (i16 ^ (2 * st))));
-                        };
-                        h8 kf[2][2];
-#pragma unroll
-                        for (int kt = 0; kt < 2; kt++) kf[0][kt] = kfrag(0, kt);
-#pragma unroll
-                        for (int st = 0; st < 8; st++) {
-                            if (st + 1 < 8)
-#pragma unroll
-                                for (int kt = 0; kt < 2; kt++) kf[(st + 1) & 1][kt] = kfrag(st + 1, kt);
-                            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                            for (int part = 1; part >= 0; part--)
-#pragma unroll
-                                for (int rt = 0; rt < 2; rt++)
-#pragma unroll
-                                    for (int kt = 0; kt < 2; kt++) {
-                                        const h8 k8 = kf[st & 1][kt];
-                                        if constexpr (SC) {
-                                            const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                                            T[st & 1][rt][kt] = mfma16(k8, qb[rt][part][st], part ? zero : T[st & 1][rt][kt]);
-                                        } else {
-                                            sc[rt][kt] = mfma16(k8, qb[rt][part][st], sc[rt][kt]);
-                                        }
-                                    }
-                            if constexpr (SC) {
-                                if (st > 0)
-#pragma unroll
-                                    for (int rt = 0; rt < 2; rt++) {
-                                        scale(st - 1, rt, 0);
-                                        scale(st - 1, rt, 1);
-                                    }
-                                if (st % 2 == 0)
-#pragma unroll
-                                    for (int kt = 0; kt < 2; kt++) ks[kt] = lds_h8(Sc + 8 * (16 * kt + 2 * st + lg));
-                            }
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                        if constexpr (SC) {
-#pragma unroll
-                            for (int rt = 0; rt < 2; rt++) {
-                                scale(7, rt, 0);
-                                scale(7, rt, 1);
-                            }
-                        } else {
-                            mfma_settle(sc[0][0], sc[0][1]);
-                            mfma_settle(sc[1][0], sc[1][1]);
-                        }
-                        const int dead = __builtin_amdgcn_readfirstlane(lds.dead[i & 3]);
-                        bool moved = false;
-                        float cr[2];
-#pragma unroll
-                        for (int rt = 0; rt < 2; rt++) {
-                            if (k0 + PF_TILE > vmin || dead != 0) {
-#pragma unroll
-                                for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                                    for (int e = 0; e < 4; e++)
-                                        sc[rt][kt][e] = k0 + 16 * kt + 4 * lg + e < vis[rt] && !((dead >> kt) & 1)
-                                                            ? sc[rt][kt][e] : -INFINITY;
-                            }
-                            float mx = max3f(max3f(-INFINITY, sc[rt][0][0], sc[rt][0][1]), sc[rt][0][2], sc[rt][0][3]);
-                            mx = rows_max(max3f(max3f(mx, sc[rt][1][0], sc[rt][1][1]), sc[rt][1][2], sc[rt][1][3]));
-                            const float mx2 = mx * PF_LOG2E, mn = mx2 > m[rt] + BT_HEAD ? mx2 - BT_RAISE : m[rt];
-                            cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] - mn);
-                            const float ref = mn == -INFINITY ? 0.0f : mn;  // a row that saw nothing keeps l = 0, O = 0
-                            m[rt] = mn;
-                            moved |= cr[rt] != 1.0f;
-                            h8 pb;
-                            float rx = 0.0f;
-#pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                const float x = fast_exp2(fmaf(sc[rt][e >> 2][e & 3], PF_LOG2E, -ref));
-                                pb[e] = (_Float16)x;
-                                if (LSE) rx += x;
-                            }
-                            lds.p[b][pair][rt][lane] = pb;
-                            // the sum of the rounded probabilities, the weights that P V applies
-                            const h2 one2 = {(_Float16)1.0f, (_Float16)1.0f};
-                            float rs = 0.0f;
-#pragma unroll
-                            for (int e = 0; e < 8; e += 2) rs = __builtin_amdgcn_fdot2(h2{pb[e], pb[e + 1]}, one2, rs, false);
-                            l[rt] = l[rt] * cr[rt] + rs;
-                            if (LSE) lx[rt] = lx[rt] * cr[rt] + rx;
-                        }
-                        const bool any = __any(moved);
-                        if (any)
-#pragma unroll
-                            for (int rt = 0; rt < 2; rt++) lds.cr[b][pair][rt][i16] = cr[rt];
-                        if (lane == 0) lds.moved[b][pair] = any;
-                        if (i + 1 == nt) {
-#pragma unroll
-                            for (int rt = 0; rt < 2; rt++) {
-                                const float4 ml = make_float4(m[rt], rows_sum(l[rt]), LSE ? rows_sum(lx[rt]) : 0.0f, 0.0f);
-                                if (lg == 0) lds.ml[pair][rt][i16] = ml;
-                            }
-                        }
-                    }
-                    __syncthreads();
-                }
-                __syncthreads();
-            }
-            s += nt;
-            j++;
+    // The segments; the roles meet at a segment's barriers, one and one a tile.  Behind the last one the score waves go on to the
+    // next segment's Q and K while the value waves finish: what these still read there (V and flags of the last tile, its
+    // scores, which the pair's own O follows) is written by nobody before the next barrier.
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    while (s < s_end) {
+        // (an opaque copy of the thread: addresses kept across the segments took registers of the loop over tiles)
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));
+        ChunkSegment sg;
+        const ChunkBlock c = a.blocks[j];
+        sg.c = ChunkBlock{uni(c.row0), uni(c.count), uni(c.len), uni(c.seq), uni(c.blk), uni(c.begin), uni(c.tiles), uni(c.end),
+                          uni(c.img)};
+        sg.base = s - s_begin;
+        sg.tb = s - sg.c.begin;
+        sg.nt = min(s_end, sg.c.begin + sg.c.tiles) - s;
+        sg.nrows = GRP * sg.c.count;
+        sg.wrow0 = CH_ROWS * sg.c.blk + 32 * pair;
+        const size_t part = (((size_t)g * a.slices + w) * 2 + (s == s_begin ? 0 : 1)) * a.prows;
+        if (wave < CH_PAIRS) {
+            if (sg.c.img >= 0) ch_score_walk<KVT, true>(lds, a, kv, p, sg, g, pair, t);
+            else ch_score_walk<KVT, false>(lds, a, kv, p, sg, g, pair, t);
+        } else {
+            if (sg.c.img >= 0) ch_value_walk<KVT, true, LSE>(lds, a, kv, p, sg, g, pair, part, t);
+            else ch_value_walk<KVT, false, LSE>(lds, a, kv, p, sg, g, pair, part, t);
         }
-    };
-    if (wave < CH_PAIRS) walk(std::false_type{});
-    else walk(std::true_type{});
+        s += sg.nt;
+        j++;
+    }
 }
 
 // Joins the states of the blocks that lie in several slices, in the slices' order: workgroup (cut between two slices, KV head,
@@ -630,9 +788,19 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
     uint8_t* base = static_cast<uint8_t*>(work);
     ChunkBlock* blocks = reinterpret_cast<ChunkBlock*>(base + w.blocks);
     int* head = reinterpret_cast<int*>(base + w.head);
-    const ChunkArgs a{q, gate, out16, lse, blocks, head, reinterpret_cast<float*>(base + w.o),
-                      reinterpret_cast<float4*>(base + w.ml), pl.slices, pl.rows};
-    hipLaunchKernelGGL(k_ch_plan, dim3(1), dim3(CH_PT), 0, st, p, seqs, off, n, rows, max_len, pl.blocks, blocks, head);
+    int4* list = reinterpret_cast<int4*>(base + w.list);
+    const ChunkArgs a{q, gate, out16, lse, blocks, list, head, reinterpret_cast<ChunkImage*>(base + w.images),
+                      reinterpret_cast<float*>(base + w.o), reinterpret_cast<float4*>(base + w.ml), pl.slices, pl.rows};
+    hipLaunchKernelGGL(k_ch_plan, dim3(1), dim3(CH_PT), 0, st, p, seqs, off, n, rows, max_len, pl.blocks, pl.images, pl.tiles,
+                       blocks, list, head);
+    if (pl.tiles > 0) {
+        const dim3 ig((unsigned)std::min(pl.tiles * NKV, CH_IMG_WGS));
+        switch (kvt) {
+            case QWA_KV_F16: hipLaunchKernelGGL(k_ch_image<QWA_KV_F16>, ig, dim3(512), 0, st, a, kv, p); break;
+            case QWA_KV_Q8_0: hipLaunchKernelGGL(k_ch_image<QWA_KV_Q8_0>, ig, dim3(512), 0, st, a, kv, p); break;
+            default: hipLaunchKernelGGL(k_ch_image<QWA_KV_Q4_0>, ig, dim3(512), 0, st, a, kv, p); break;
+        }
+    }
     const dim3 grid(pl.slices * NKV), block(128 * CH_PAIRS);
 #define QWA_CH(T)                                                                              \
     case T:                                                                                    \

@@ -16,36 +16,58 @@ constexpr int CH_PAIRS = 4;                 // pairs of waves of a workgroup: on
 constexpr int CH_ROWS = 32 * CH_PAIRS;      // rows (token, head of the group) of a workgroup
 constexpr int CH_SLICES = 256 / NKV;        // workgroups of a KV head: one round of the chip's 256 CUs
 
+// Chunks of at least CH_IMG_BLOCKS blocks read their keys as images: tiles that k_ch_image has brought into the form of LDS once,
+// instead of every block by itself.  Images take 4 times the bytes of a Q8_0 cache, so there is room for CH_IMG_TILES tiles (of
+// each KV head) or one sequence, whichever is more, and chunks that find none left do without.
+constexpr int CH_IMG_BLOCKS = 4;
+constexpr int CH_IMG_TILES = 4096;
+struct ChunkImage {
+    uint16_t k[PF_TILE * HD];
+    uint16_t scales[PF_TILE * 8];
+    uint16_t vt[PF_TILE * HD];
+    uint8_t odd_keys[8 * HD];  // of V values that are not finite
+    int odd[4];                // which quarters of them hold any (1)
+    int dead;                  // halves without a place
+    int pad[59];               // (these 256 bytes are copied as one)
+};
+
 // A chunk's rows are cut into blocks of CH_ROWS; a block walks the PF_TILE-key tiles from the first to the last that one of its
 // rows sees.  The tiles of all blocks in a row, cut into `slices` equal parts, are the workgroups of a KV head.
-// blocks, slices: bounds of what the device finds, which knows the chunks; rows: of a block that are stored.
+// blocks, slices, images (chunks that read images), tiles (of images): bounds of what the device finds, which knows the chunks;
+// rows: of a block that are stored.
 struct ChunkPlan {
-    int blocks, slices, rows;
+    int blocks, slices, rows, images, tiles;
 };
 
 inline ChunkPlan chunk_plan(int n, int rows, int max_len) {
     ChunkPlan p;
+    const int most = (max_len + PF_TILE - 1) / PF_TILE;
     // (a chunk has one partly filled block)
     p.blocks = (int)std::min<long long>((long long)GRP * rows, (long long)GRP * rows / CH_ROWS + n);
-    p.slices = (int)std::min<long long>(CH_SLICES, (long long)p.blocks * ((max_len + PF_TILE - 1) / PF_TILE));
+    p.slices = (int)std::min<long long>(CH_SLICES, (long long)p.blocks * most);
     p.rows = std::min(CH_ROWS, GRP * rows);
+    // (a chunk of CH_IMG_BLOCKS blocks has more than CH_IMG_BLOCKS - 1 full ones)
+    p.images = std::min(n, (int)((long long)GRP * rows / (CH_ROWS * (CH_IMG_BLOCKS - 1))));
+    p.tiles = (int)std::min<long long>((long long)p.images * most, std::max(most, CH_IMG_TILES));
     return p;
 }
 
-// Work buffer: the blocks' descriptions, their number and that of their tiles; the partial states of the blocks that lie in
-// several slices, two places a slice (its first block, if it began in an earlier one, and its last one): O as fp32 [256] and
-// (m, l, sum for the log) a row.
+// Work buffer: the blocks' descriptions, the list of chunks with images, the numbers of blocks, their tiles, chunks with images
+// and those tiles; the images; the partial states of the blocks that lie in several slices, two places a slice (its first block,
+// if it began in an earlier one, and its last one): O as fp32 [256] and (m, l, sum for the log) a row.
 struct ChunkWork {
-    size_t blocks, head, o, ml, bytes;  // byte offsets
+    size_t images, o, ml, blocks, list, head, bytes;  // byte offsets
 };
-constexpr size_t CH_BLOCK_BYTES = 32;
+constexpr size_t CH_BLOCK_BYTES = 48;
 inline ChunkWork chunk_work(const ChunkPlan& p) {
     const size_t parts = (size_t)NKV * p.slices * 2 * p.rows;
     ChunkWork w;
-    w.o = 0;
+    w.images = 0;
+    w.o = w.images + (size_t)NKV * p.tiles * sizeof(ChunkImage);
     w.ml = w.o + parts * HD * 4;
     w.blocks = w.ml + parts * 16;
-    w.head = w.blocks + p.blocks * CH_BLOCK_BYTES;
+    w.list = w.blocks + p.blocks * CH_BLOCK_BYTES;
+    w.head = w.list + p.images * 16;
     w.bytes = w.head + 16;
     return w;
 }
