@@ -214,7 +214,14 @@ __global__ void __launch_bounds__(512) k_ch_image(ChunkArgs a, qwa_kv_layer kv, 
     }
 }
 
-constexpr int CH_VD = 3;    // V fragments in flight
+#ifndef QWA_CH_VD
+#define QWA_CH_VD 6
+#endif
+#ifndef QWA_CH_KD
+#define QWA_CH_KD 2
+#endif
+constexpr int CH_KD = QWA_CH_KD;    // K steps read ahead of their MFMAs
+constexpr int CH_VD = QWA_CH_VD;    // V fragments in flight
 constexpr int CH_RING = 3;  // tiles in LDS: the one read, and two on their way
 
 template <int KVT>
@@ -300,24 +307,24 @@ __device__ __forceinline__ void ch_scores(f4 (&sc)[2][2], const h8 (&qb)[2][2][8
                                           int lg) {
     constexpr bool SC = KVT != QWA_KV_F16;
     f4 T[2][2];
-    h4 ks[2][2];
-    h8 kf[2][2];
+    h4 ks[CH_KD + 1][2];
+    h8 kf[CH_KD + 1][2];
     auto scale = [&](int st, int rt) {
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) sc[rt][kt][e] = fmaf((float)ks[st & 1][kt][e], T[rt][kt][e], sc[rt][kt][e]);
+            for (int e = 0; e < 4; e++) sc[rt][kt][e] = fmaf((float)ks[st % (CH_KD + 1)][kt][e], T[rt][kt][e], sc[rt][kt][e]);
             // (the sums stay where they are: put off past the last block, they kept all products, and spilled)
             asm volatile("" : "+v"(sc[rt][kt]));
         }
     };
     auto read = [&](int st) {
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) kf[st & 1][kt] = lds_h8(Ks + 8 * (32 * (4 * st + lg) + 16 * kt + (i16 ^ (2 * st))));
+        for (int kt = 0; kt < 2; kt++) kf[st % (CH_KD + 1)][kt] = lds_h8(Ks + 8 * (32 * (4 * st + lg) + 16 * kt + (i16 ^ (2 * st))));
         if constexpr (SC)
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
-                ks[st & 1][kt] = *reinterpret_cast<const h4*>(Sc + 8 * (16 * kt + 4 * (st >> 1) + lg) + 4 * (st & 1));
+                ks[st % (CH_KD + 1)][kt] = *reinterpret_cast<const h4*>(Sc + 8 * (16 * kt + 4 * (st >> 1) + lg) + 4 * (st & 1));
     };
     auto multiply = [&](int st, int rt) {
 #pragma unroll
@@ -325,22 +332,23 @@ __device__ __forceinline__ void ch_scores(f4 (&sc)[2][2], const h8 (&qb)[2][2][8
 #pragma unroll
             for (int kt = 0; kt < 2; kt++) {
                 const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (SC) T[rt][kt] = mfma16(kf[st & 1][kt], qb[rt][part][st], part ? zero : T[rt][kt]);
-                else sc[rt][kt] = mfma16(kf[st & 1][kt], qb[rt][part][st], sc[rt][kt]);
+                if constexpr (SC) T[rt][kt] = mfma16(kf[st % (CH_KD + 1)][kt], qb[rt][part][st], part ? zero : T[rt][kt]);
+                else sc[rt][kt] = mfma16(kf[st % (CH_KD + 1)][kt], qb[rt][part][st], sc[rt][kt]);
             }
     };
 #pragma unroll
     for (int rt = 0; rt < 2; rt++)
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) sc[rt][kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    read(0);
+#pragma unroll
+    for (int st = 0; st < CH_KD; st++) read(st);
 #pragma unroll
     for (int st = 0; st < 8; st++) {
         __builtin_amdgcn_sched_barrier(0);
         multiply(st, 0);
         if (SC && st > 0) scale(st - 1, 1);
         __builtin_amdgcn_sched_barrier(0);
-        if (st + 1 < 8) read(st + 1);
+        if (st + CH_KD < 8) read(st + CH_KD);
         multiply(st, 1);
         if (SC) scale(st, 0);
     }

@@ -19,7 +19,10 @@ constexpr int CH_SLICES = 256 / NKV;        // workgroups of a KV head: one roun
 // Chunks of at least CH_IMG_BLOCKS blocks read their keys as images: tiles that k_ch_image has brought into the form of LDS once,
 // instead of every block by itself.  Images take 4 times the bytes of a Q8_0 cache, so there is room for CH_IMG_TILES tiles (of
 // each KV head) or one sequence, whichever is more, and chunks that find none left do without.
-constexpr int CH_IMG_BLOCKS = 4;
+#ifndef QWA_CH_IMG_BLOCKS
+#define QWA_CH_IMG_BLOCKS 4
+#endif
+constexpr int CH_IMG_BLOCKS = QWA_CH_IMG_BLOCKS;
 constexpr int CH_IMG_TILES = 4096;
 struct ChunkImage {
     uint16_t k[PF_TILE * HD];
