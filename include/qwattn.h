@@ -291,6 +291,22 @@ int qwa_attn_prefill_batch(const float* q, const float* gate, const qwa_kv_layer
                            const int* seqs, const int* off, int n, int rows, int max_len, uint16_t* out16, float* lse,
                            void* work, size_t work_bytes, void* stream);
 
+/* Bytes of the `work` buffer of qwa_attn_weights_batch (0: invalid arguments). */
+size_t qwa_attn_weights_batch_work_bytes(int n, int rows, int max_len);
+
+/* The attention weight that positions gather: for each KV head of one layer and each position j that a chunk's tokens see, the
+ * sum over these tokens and the head's 6 query heads of exp(score - lse) is added to mass[seq][head][j] (fp32, device,
+ * [n_seq][4][ld * page]); the chunk's own positions, which are new, begin with it.  Chunks of one token do for decoded
+ * tokens.  q, lse: those of the qwa_attn_prefill_batch call of the same chunks (of all its tokens, or with other offsets of its
+ * last ones, the positions that the sequences hold then ending with them).  Rows that see no position add nothing; entries of
+ * positions past a sequence's last one, and of positions that no token sees, are left as they are.  Scores are exact up to
+ * fp32 accumulation, all sums fp32 in a fixed order.  Of several chunks of one sequence the last one counts.
+ * n <= QWA_PAGES_MAXN; max_len as for qwa_attn_prefill_batch; q, work and the pool 16-byte aligned; work of at least
+ * qwa_attn_weights_batch_work_bytes bytes, not shared with a call that may run at the same time. */
+int qwa_attn_weights_batch(const float* q, const float* lse, const qwa_kv_layer* kv, int kvt, const qwa_kv_pages* p,
+                           const int* seqs, const int* off, int n, int rows, int max_len, float* mass, void* work,
+                           size_t work_bytes, void* stream);
+
 /* ---- Gated DeltaNet (the recurrent token mixer of the other layers) ---------------------------------------------- */
 
 /* New tokens per qwa_deltanet_multi call (the reference's DN_MAXN = Engine::MAX_BATCH, src/cuda/ops.cu:148). */

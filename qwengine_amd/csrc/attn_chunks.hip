@@ -28,11 +28,12 @@
 namespace qwa {
 
 // a block: its chunk's first row and number of tokens, the sequence's length and number (< 0: unknown, len 0), the block's number in
-// the chunk, its first tile in the row of all tiles, its tiles, the positions that its last row sees, the chunk's first image (-1: none)
+// the chunk, its first tile in the row of all tiles, its tiles, the positions that its last row sees, the chunk's first image, or the
+// block's place for its sums (-1: none)
 struct alignas(16) ChunkBlock {
     int row0, count, len, seq;
     int blk, begin, tiles, end;
-    int img, pad[3];
+    int place, pad[3];
 };
 static_assert(sizeof(ChunkBlock) == CH_BLOCK_BYTES, "work buffer");
 
@@ -77,14 +78,18 @@ __device__ __forceinline__ int ch_scan(int v, int* s_wave, int* total) {
 }
 
 // The blocks of all chunks, by one workgroup: thread b has chunk b.  A chunk of rows outside [0, rows], or that begins before an
-// earlier one's end, has none.
+// earlier one's end, has none.  For the weights (other sizes of blocks and tiles) only the last chunk of a sequence counts, and
+// chunks of several blocks get places for their sums (list: sequence, length, tokens, first place) instead of images (sequence,
+// length, first image, images).
 constexpr int CH_PT = QWA_PAGES_MAXN;
+template <bool WEIGHTS>
 __global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __restrict__ seqs, const int* __restrict__ off, int n,
-                                                   int rows, int max_len, int most, int most_images, int img_tiles,
+                                                   int rows, int max_len, int most, int most_list, int room,
                                                    ChunkBlock* __restrict__ blocks, int4* __restrict__ list,
                                                    int* __restrict__ head) {
+    constexpr int ROWS = WEIGHTS ? CW_ROWS : CH_ROWS, TILE = WEIGHTS ? CW_TILE : PF_TILE;
     __shared__ int s_wave[CH_PT / 64];
-    __shared__ int s_end[CH_PT], s_first[CH_PT], s_count[CH_PT], s_len[CH_PT], s_seq[CH_PT], s_blk[CH_PT], s_img[CH_PT];
+    __shared__ int s_end[CH_PT], s_first[CH_PT], s_count[CH_PT], s_len[CH_PT], s_seq[CH_PT], s_blk[CH_PT], s_place[CH_PT];
     const int t = threadIdx.x, lane = t & 63;
     int first = 0, end = 0;
     if (t < n) {
@@ -103,26 +108,34 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __
     __syncthreads();
     int before = lane > 0 ? s_end[t - 1] : 0;
     for (int w = 0; w < t >> 6; w++) before = max(before, s_end[64 * w + 63]);
-    const int count = end > first && before <= first ? end - first : 0;
+    int count = end > first && before <= first ? end - first : 0;
     const int seq = t < n ? (seqs ? seqs[t] : t) : -1;
     const bool known = seq >= 0 && seq < p.n_seq;
     s_first[t] = first;
-    s_count[t] = count;
     s_len[t] = known && count > 0 ? min(max(p.len[seq], 0), max_len) : 0;
     s_seq[t] = known ? seq : -1;
-    int nb;
-    const int mine = (GRP * count + CH_ROWS - 1) / CH_ROWS;
+    s_count[t] = count;
+    if (WEIGHTS) {
+        __syncthreads();
+        if (!known) count = 0;
+        if (seqs && count > 0)
+            for (int j = t + 1; j < n; j++)
+                if (s_seq[j] == seq && s_count[j] > 0) count = 0;
+        __syncthreads();
+        s_count[t] = count;
+    }
+    const int mine = (GRP * count + ROWS - 1) / ROWS;
+    int nb, all, listed, used;
     s_blk[t] = ch_scan<CH_PT>(mine, s_wave, &nb);
     nb = min(nb, most);  // (never more: the chunks' rows are disjoint)
-    // images, as long as there is room for them
-    const int want = mine >= CH_IMG_BLOCKS ? (s_len[t] + PF_TILE - 1) / PF_TILE : 0;
-    int all_want, images, img_used;
-    const int img = ch_scan<CH_PT>(min(want, img_tiles + 1), s_wave, &all_want);
-    const bool has = want > 0 && img + want <= img_tiles;
-    const int place = ch_scan<CH_PT>(has, s_wave, &images);
-    ch_scan<CH_PT>(has ? want : 0, s_wave, &img_used);
-    s_img[t] = has && place < most_images ? img : -1;
-    if (s_img[t] >= 0) list[place] = make_int4(s_seq[t], s_len[t], img, want);
+    // images, or places, as long as there is room for them (of places there always is)
+    const int want = WEIGHTS ? (mine > 1 ? mine : 0) : mine >= CH_IMG_BLOCKS ? (s_len[t] + PF_TILE - 1) / PF_TILE : 0;
+    const int place = ch_scan<CH_PT>(min(want, room + 1), s_wave, &all);
+    const bool has = want > 0 && place + want <= room;
+    const int entry = ch_scan<CH_PT>(has, s_wave, &listed);
+    ch_scan<CH_PT>(has ? want : 0, s_wave, &used);
+    s_place[t] = has && entry < most_list ? place : -1;
+    if (s_place[t] >= 0) list[entry] = WEIGHTS ? make_int4(s_seq[t], s_len[t], count, place) : make_int4(s_seq[t], s_len[t], place, want);
     __syncthreads();
     int tiles = 0;
     for (int j0 = 0; j0 < nb; j0 += CH_PT) {
@@ -140,12 +153,11 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __
             x.len = s_len[lo];
             x.seq = s_seq[lo];
             x.blk = j - s_blk[lo];
-            const int last = min((x.blk + 1) * CH_ROWS, GRP * x.count) - 1;
+            const int last = min((x.blk + 1) * ROWS, GRP * x.count) - 1;
             x.end = max(0, x.len - x.count + last / GRP + 1);
-            x.tiles = max(1, (x.end + PF_TILE - 1) / PF_TILE);  // (rows that see nothing are written too)
-            x.img = s_img[lo];
+            x.tiles = max(1, (x.end + TILE - 1) / TILE);  // (rows that see nothing are written too)
+            x.place = s_place[lo] < 0 ? -1 : s_place[lo] + (WEIGHTS ? x.blk : 0);
         }
-        int all;
         x.begin = tiles + ch_scan<CH_PT>(x.tiles, s_wave, &all);
         tiles += all;
         if (j < nb) blocks[j] = x;
@@ -153,23 +165,30 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __
     if (t == 0) {
         head[0] = nb;
         head[1] = tiles;
-        head[2] = min(images, most_images);
-        head[3] = img_used;
+        head[2] = min(listed, most_list);
+        head[3] = used;
     }
 }
 
 // slices that hold tiles: the same number for every workgroup of a call
-__device__ __forceinline__ int ch_slices(const ChunkArgs& a, int tiles) { return min(a.slices, tiles); }
+__device__ __forceinline__ int ch_slices(int slices, int tiles) { return min(slices, tiles); }
 __device__ __forceinline__ int ch_cut(int w, int tiles, int slices) { return (int)((long long)w * tiles / slices); }
 
 // the block that holds tile s, found by the whole workgroup
-__device__ __forceinline__ int ch_find(const ChunkArgs& a, int nb, int s, int* s_found) {
+__device__ __forceinline__ int ch_find(const ChunkBlock* blocks, int nb, int s, int* s_found) {
     for (int j = threadIdx.x; j < nb; j += blockDim.x) {
-        const int begin = a.blocks[j].begin;
-        if (begin <= s && s < begin + a.blocks[j].tiles) *s_found = j;
+        const int begin = blocks[j].begin;
+        if (begin <= s && s < begin + blocks[j].tiles) *s_found = j;
     }
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(*s_found);
+}
+
+// a block's description in scalar registers
+__device__ __forceinline__ ChunkBlock ch_block(const ChunkBlock& c) {
+    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    return ChunkBlock{uni(c.row0), uni(c.count), uni(c.len), uni(c.seq), uni(c.blk), uni(c.begin), uni(c.tiles), uni(c.end),
+                      uni(c.place)};
 }
 
 // The images: a workgroup of 512 threads converts a tile of one KV head, half of them K, half V, from registers to memory.
@@ -249,17 +268,17 @@ struct ChunkSegment {
 // Q / 16 of a wave's 32 rows as the B operand, hi and lo part: rows are read in runs of 512 bytes, their fp16 pieces go to unit
 // (4 s + lg, row ^ (4 s + lg) % 16) of the wave's part of LDS and come back as the lane's fragments s.
 template <int KVT>
-__device__ __forceinline__ void ch_load_q(h8 (&qb)[2][2][8], const ChunkArgs& a, const ChunkSegment& sg, int g, uint2* lds_q,
-                                          int lane) {
+__device__ __forceinline__ void ch_load_q(h8 (&qb)[2][2][8], const float* __restrict__ q, const ChunkBlock& c, int wrow0,
+                                          int nrows, int g, uint2* lds_q, int lane) {
     const int i16 = lane & 15, lg = lane >> 4, l5 = lane & 31, half = l5 & 1, u = l5 >> 1;
     uint8_t* const area = reinterpret_cast<uint8_t*>(lds_q);
     float4 x[2][8];
     auto load = [&](int r) {  // round r = 2 * row tile + half of the dims
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const int row = min(sg.wrow0 + 16 * (r >> 1) + 2 * k + (lane >> 5), sg.nrows - 1);
+            const int row = min(wrow0 + 16 * (r >> 1) + 2 * k + (lane >> 5), nrows - 1);
             x[r & 1][k] = *reinterpret_cast<const float4*>(
-                a.q + ((size_t)(sg.c.row0 + row / GRP) * NH + g * GRP + row % GRP) * HD + 128 * (r & 1) + 4 * l5);
+                q + ((size_t)(c.row0 + row / GRP) * NH + g * GRP + row % GRP) * HD + 128 * (r & 1) + 4 * l5);
         }
     };
     load(0);
@@ -274,7 +293,7 @@ __device__ __forceinline__ void ch_load_q(h8 (&qb)[2][2][8], const ChunkArgs& a,
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const int row = 2 * k + (lane >> 5);
-                const float f = sg.wrow0 + 16 * rt + row < sg.nrows ? 0.0625f : 0.0f;
+                const float f = wrow0 + 16 * rt + row < nrows ? 0.0625f : 0.0f;
                 uint32_t w0 = h2_bits(h2{piece(x[r & 1][k].x, f), piece(x[r & 1][k].y, f)});
                 uint32_t w1 = h2_bits(h2{piece(x[r & 1][k].z, f), piece(x[r & 1][k].w, f)});
                 if constexpr (KVT == QWA_KV_Q4_0) {
@@ -356,16 +375,17 @@ __device__ __forceinline__ void ch_scores(f4 (&sc)[2][2], const h8 (&qb)[2][2][8
     if constexpr (SC) scale(7, 1);
 }
 
-// The pool positions of a tile's halves, 64 tiles ahead: lane l has those of tile l.
+// The pool positions of a tile's groups of 16 keys, 64 tiles ahead: lane l has those of tile l.
+template <int G>
 struct ChunkPlaces {
-    int ahead[2], tile = 0;
-    __device__ __forceinline__ void next(int (&at)[2], const qwa_kv_pages& p, const int* __restrict__ table, int tb, int end,
+    int ahead[G], tile = 0;
+    __device__ __forceinline__ void next(int (&at)[G], const qwa_kv_pages& p, const int* __restrict__ table, int tb, int end,
                                          int lane) {
         if ((tile & 63) == 0)
 #pragma unroll
-            for (int h = 0; h < 2; h++) ahead[h] = bt_place(p, table, (tb + tile + lane) * PF_TILE + 16 * h, end);
+            for (int h = 0; h < G; h++) ahead[h] = bt_place(p, table, 16 * (G * (tb + tile + lane) + h), end);
 #pragma unroll
-        for (int h = 0; h < 2; h++) at[h] = __builtin_amdgcn_readlane(ahead[h], tile & 63);
+        for (int h = 0; h < G; h++) at[h] = __builtin_amdgcn_readlane(ahead[h], tile & 63);
         tile++;
     }
 };
@@ -390,9 +410,9 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
     const size_t head = (size_t)g * kv.capacity;
     const uint8_t* const kh = kv.k + head * value_bytes(KVT);
     const uint16_t* const ksh = SC ? kv.ks + head * 8 : nullptr;
-    const ChunkImage* const img = a.images + (size_t)(max(sg.c.img, 0) + sg.tb) * NKV + g;
+    const ChunkImage* const img = a.images + (size_t)(max(sg.c.place, 0) + sg.tb) * NKV + g;
     BtRaw<KVT> rk;
-    ChunkPlaces places;
+    ChunkPlaces<2> places;
     auto load = [&](int i) {
         int at[2];
         places.next(at, p, table, sg.tb, sg.c.end, lane);
@@ -412,7 +432,7 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
     };
     if constexpr (!IMG) load(0);
     h8 qb[2][2][8];
-    ch_load_q<KVT>(qb, a, sg, g, lds.q[pair], lane);
+    ch_load_q<KVT>(qb, a.q, sg.c, sg.wrow0, sg.nrows, g, lds.q[pair], lane);
     if constexpr (IMG) {
         wait_vmcnt<0>();  // from here on vmcnt counts only the copies
         copy(0);
@@ -457,7 +477,7 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
     const size_t head = (size_t)g * kv.capacity;
     const uint8_t* const vh = kv.v + head * value_bytes(KVT);
     const uint16_t* const vsh = SC ? kv.vs + head * 8 : nullptr;
-    const ChunkImage* const img = a.images + (size_t)(max(sg.c.img, 0) + sg.tb) * NKV + g;
+    const ChunkImage* const img = a.images + (size_t)(max(sg.c.place, 0) + sg.tb) * NKV + g;
     const bool rows_here = sg.wrow0 < sg.nrows;
     int vis[2], vmin = 0x7fffffff;  // positions that this lane's rows see, the fewest that one of the wave's does
 #pragma unroll
@@ -470,7 +490,7 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
     for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
     vmin = __builtin_amdgcn_readfirstlane(vmin);
     BtRaw<KVT> rv;
-    ChunkPlaces places;
+    ChunkPlaces<2> places;
     uint32_t dead = 0;  // halves without a place, two bits a tile: tile i - 1, tile i, ...
     auto load = [&](int i) {
         int at[2];
@@ -692,24 +712,21 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     if (gridDim.x % 8 == 0) unit = (int)(gridDim.x / 8) * (blockIdx.x & 7) + (blockIdx.x >> 3);
     const int g = unit / a.slices, w = unit % a.slices;
     const int nb = a.head[0], tiles = a.head[1];
-    const int slices = ch_slices(a, tiles);
+    const int slices = ch_slices(a.slices, tiles);
     if (w >= slices) return;
     int s = ch_cut(w, tiles, slices);
     const int s_begin = s, s_end = ch_cut(w + 1, tiles, slices);
     if (threadIdx.x < 8) lds.odd[threadIdx.x >> 2].tile[threadIdx.x & 3] = -1;
-    int j = ch_find(a, nb, s, &lds.found);
+    int j = ch_find(a.blocks, nb, s, &lds.found);
     // The segments; the roles meet at a segment's barriers, one and one a tile.  Behind the last one the score waves go on to the
     // next segment's Q and K while the value waves finish: what these still read there (V and flags of the last tile, its
     // scores, which the pair's own O follows) is written by nobody before the next barrier.
-    auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
     while (s < s_end) {
         // (an opaque copy of the thread: addresses kept across the segments took registers of the loop over tiles)
         int t = threadIdx.x;
         asm volatile("" : "+v"(t));
         ChunkSegment sg;
-        const ChunkBlock c = a.blocks[j];
-        sg.c = ChunkBlock{uni(c.row0), uni(c.count), uni(c.len), uni(c.seq), uni(c.blk), uni(c.begin), uni(c.tiles), uni(c.end),
-                          uni(c.img)};
+        sg.c = ch_block(a.blocks[j]);
         sg.base = s - s_begin;
         sg.tb = s - sg.c.begin;
         sg.nt = min(s_end, sg.c.begin + sg.c.tiles) - s;
@@ -717,10 +734,10 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         sg.wrow0 = CH_ROWS * sg.c.blk + 32 * pair;
         const size_t part = (((size_t)g * a.slices + w) * 2 + (s == s_begin ? 0 : 1)) * a.prows;
         if (wave < CH_PAIRS) {
-            if (sg.c.img >= 0) ch_score_walk<KVT, true>(lds, a, kv, p, sg, g, pair, t);
+            if (sg.c.place >= 0) ch_score_walk<KVT, true>(lds, a, kv, p, sg, g, pair, t);
             else ch_score_walk<KVT, false>(lds, a, kv, p, sg, g, pair, t);
         } else {
-            if (sg.c.img >= 0) ch_value_walk<KVT, true, LSE>(lds, a, kv, p, sg, g, pair, part, t);
+            if (sg.c.place >= 0) ch_value_walk<KVT, true, LSE>(lds, a, kv, p, sg, g, pair, part, t);
             else ch_value_walk<KVT, false, LSE>(lds, a, kv, p, sg, g, pair, part, t);
         }
         s += sg.nt;
@@ -734,11 +751,11 @@ constexpr int CH_JR = 16;  // rows of a workgroup
 template <bool LSE>
 __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a) {
     __shared__ int found;
-    const int tiles = a.head[1], slices = ch_slices(a, tiles);
+    const int tiles = a.head[1], slices = ch_slices(a.slices, tiles);
     const int g = blockIdx.y, cut = blockIdx.x + 1;
     if (cut >= slices) return;
     const int s = ch_cut(cut, tiles, slices), s_before = ch_cut(cut - 1, tiles, slices);
-    const int j = ch_find(a, a.head[0], s, &found);
+    const int j = ch_find(a.blocks, a.head[0], s, &found);
     const ChunkBlock c = a.blocks[j];
     if (c.begin == s || c.begin < s_before) return;  // the cut lies between two blocks, or an earlier one lies in this
     // its slices: cut - 1 up to the one that holds its last tile
@@ -799,7 +816,7 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
     int4* list = reinterpret_cast<int4*>(base + w.list);
     const ChunkArgs a{q, gate, out16, lse, blocks, list, head, reinterpret_cast<ChunkImage*>(base + w.images),
                       reinterpret_cast<float*>(base + w.o), reinterpret_cast<float4*>(base + w.ml), pl.slices, pl.rows};
-    hipLaunchKernelGGL(k_ch_plan, dim3(1), dim3(CH_PT), 0, st, p, seqs, off, n, rows, max_len, pl.blocks, pl.images, pl.tiles,
+    hipLaunchKernelGGL(k_ch_plan<false>, dim3(1), dim3(CH_PT), 0, st, p, seqs, off, n, rows, max_len, pl.blocks, pl.images, pl.tiles,
                        blocks, list, head);
     if (pl.tiles > 0) {
         const dim3 ig((unsigned)std::min(pl.tiles * NKV, CH_IMG_WGS));
@@ -825,6 +842,210 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
         const dim3 jg(pl.slices - 1, NKV, (pl.rows + CH_JR - 1) / CH_JR);
         if (lse) hipLaunchKernelGGL(k_ch_join<true>, jg, dim3(256), 0, st, a);
         else hipLaunchKernelGGL(k_ch_join<false>, jg, dim3(256), 0, st, a);
+    }
+    return hipGetLastError();
+}
+
+// ---- the weights: for position j of a sequence and KV head g, the sum over the chunk's rows (token, head of g) that see it of
+// exp(s_j - lse), added to what it had (the chunk's own positions begin with it).
+struct WeightsArgs {
+    const float* q;
+    const float* lse;          // [rows][24]
+    float* mass;               // [sequence][KV head][ld * page]
+    const ChunkBlock* blocks;
+    const int4* list;          // chunks of several blocks: sequence, length, tokens, first place
+    const int* head;           // numbers of blocks, their tiles, such chunks, places
+    float* parts;              // [place][KV head][max_len]
+    int slices, max_len;
+};
+
+size_t weights_batch_work_bytes(int n, int rows, int max_len) {
+    return weights_work(weights_plan(n, rows, max_len), max_len).bytes;
+}
+
+constexpr int CW_WAVES = CW_ROWS / 32;
+template <int KVT>
+struct WeightsLds {
+    _Float16 k[2][CW_TILE * HD];
+    uint16_t scales[2][CW_TILE * 8];
+    int dead[2];                       // of the tile, groups of 16 keys without a place
+    float sum[2][CW_WAVES][CW_TILE];   // of the waves' rows, by key
+    uint2 q[CW_WAVES][16 * HD / 8];
+    int found;
+};
+
+// A workgroup walks the 64-key tiles of a slice as k_ch_tiles does, with K alone: all waves convert it, then each takes the scores
+// of its 32 rows, and the sums over them; the workgroup's sum of a tile is written while the next one is multiplied.
+template <int KVT>
+__global__ void __launch_bounds__(64 * CW_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
+k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
+    __shared__ __attribute__((aligned(16))) WeightsLds<KVT> lds;
+    constexpr bool SC = KVT != QWA_KV_F16;
+    constexpr int G = CW_TILE / 16;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    int unit = blockIdx.x;
+    if (gridDim.x % 8 == 0) unit = (int)(gridDim.x / 8) * (blockIdx.x & 7) + (blockIdx.x >> 3);
+    const int g = unit / a.slices, w = unit % a.slices;
+    const int nb = a.head[0], tiles = a.head[1];
+    const int slices = ch_slices(a.slices, tiles);
+    if (w >= slices) return;
+    int s = ch_cut(w, tiles, slices);
+    const int s_end = ch_cut(w + 1, tiles, slices);
+    int j = ch_find(a.blocks, nb, s, &lds.found);
+    const size_t head = (size_t)g * kv.capacity;
+    const uint8_t* const kh = kv.k + head * value_bytes(KVT);
+    const uint16_t* const ksh = SC ? kv.ks + head * 8 : nullptr;
+    while (s < s_end) {
+        // (an opaque copy of the thread: addresses kept across the segments took registers of the loop over tiles)
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));
+        const int lane = t & 63, i16 = lane & 15;
+        const ChunkBlock c = ch_block(a.blocks[j]);
+        const int tb = s - c.begin, nt = min(s_end, c.begin + c.tiles) - s;
+        const int nrows = GRP * c.count, wrow0 = CW_ROWS * c.blk + 32 * wave;
+        const bool rows_here = wrow0 < nrows;
+        const int* __restrict__ table = p.table + (size_t)max(c.seq, 0) * p.ld;
+        int vis[2], vmin = 0x7fffffff;  // (0 with a row that there is not: what it has is left out like a hidden position)
+        float lse[2];
+#pragma unroll
+        for (int rt = 0; rt < 2; rt++) {
+            const int r = wrow0 + 16 * rt + i16;
+            vis[rt] = r < nrows ? c.len - c.count + r / GRP + 1 : 0;
+            vmin = min(vmin, vis[rt]);
+            lse[rt] = r < nrows ? a.lse[(size_t)(c.row0 + r / GRP) * NH + g * GRP + r % GRP] : 0.0f;
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
+        vmin = __builtin_amdgcn_readfirstlane(vmin);
+        BtRaw<KVT> rk;
+        ChunkPlaces<G> places;
+        int dead_next = 0;
+        const int grp = __builtin_amdgcn_readfirstlane(t >> 7);  // the thread's group of 16 keys
+        auto load = [&](int i) {
+            int at[G];
+            places.next(at, p, table, tb, c.end, lane);
+            const int mine = grp == 0 ? at[0] : grp == 1 ? at[1] : grp == 2 ? at[2] : at[3];
+            dead_next = (at[0] < 0) | (at[1] < 0) << 1 | (at[2] < 0) << 2 | (at[3] < 0) << 3;
+            bt_load_k<KVT>(rk, kh, ksh, mine, min(max(c.end - (tb + i) * CW_TILE - 16 * grp, 0), 16), t);
+        };
+        auto store = [&](int i) {
+            const int b = i & 1, h = t >> 8;
+            bt_store_k<KVT>(rk, lds.k[b] + PF_TILE * HD * h, lds.scales[b] + PF_TILE * 8 * h, t);
+            if (t == 0) lds.dead[b] = dead_next;
+        };
+        // the sums of tile i: to the sequence's weights, or to the block's place
+        auto write = [&](int i) {
+            if (t >= CW_TILE) return;
+            const int key = (tb + i) * CW_TILE + t;
+            if (key >= c.end) return;
+            float v = 0.0f;
+#pragma unroll
+            for (int k = 0; k < CW_WAVES; k++) v += lds.sum[i & 1][k][t];
+            if (c.place >= 0) {
+                a.parts[((size_t)c.place * NKV + g) * a.max_len + key] = v;
+            } else {
+                float* const m = a.mass + ((size_t)c.seq * NKV + g) * ((size_t)p.ld * p.page) + key;
+                *m = key < c.len - c.count ? *m + v : v;
+            }
+        };
+        load(0);
+        h8 qb[2][2][8];
+        ch_load_q<KVT>(qb, a.q, c, wrow0, nrows, g, lds.q[wave], lane);
+        store(0);
+        if (nt > 1) load(1);
+        __syncthreads();
+        for (int i = 0; i < nt; i++) {
+            const int k0 = (tb + i) * CW_TILE, b = i & 1;
+            if (i > 0) write(i - 1);
+            if (i + 1 < nt) store(i + 1);
+            if (i + 2 < nt) load(i + 2);
+            int ol = lane;  // (opaque: LDS addresses kept across the tiles)
+            asm volatile("" : "+v"(ol));
+            const int oi = ol & 15, og = ol >> 4;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                f4 sum[2] = {};
+                if (rows_here) {
+                    f4 sc[2][2];
+                    ch_scores<KVT>(sc, qb, lds.k[b] + PF_TILE * HD * h,
+                                   reinterpret_cast<const _Float16*>(lds.scales[b] + PF_TILE * 8 * h), oi, og);
+                    const int dead = __builtin_amdgcn_readfirstlane(lds.dead[b]) >> (2 * h);
+                    const bool masked = k0 + CW_TILE > vmin || dead != 0;
+#pragma unroll
+                    for (int rt = 0; rt < 2; rt++)
+#pragma unroll
+                        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                float x = (sc[rt][kt][e] - lse[rt]) * PF_LOG2E;
+                                if (masked)
+                                    x = k0 + 32 * h + 16 * kt + 4 * og + e < vis[rt] && !((dead >> kt) & 1) ? x : -INFINITY;
+                                sum[kt][e] += fast_exp2(x);
+                            }
+                }
+                // over the 16 rows of the lanes
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float x = sum[kt][e];
+                        x += row_move<0xB1>(x);
+                        x += row_move<0x4E>(x);
+                        x += row_move<0x141>(x);
+                        x += row_move<0x140>(x);
+                        sum[kt][e] = x;
+                    }
+                    if (oi == 0)
+                        *reinterpret_cast<f4*>(&lds.sum[b][wave][32 * h + 16 * kt + 4 * og]) = sum[kt];
+                }
+            }
+            __syncthreads();
+        }
+        write(nt - 1);
+        // (the next segment's first sums are written behind its first barrier)
+        s += nt;
+        j++;
+    }
+}
+
+// The weights of chunks of several blocks: the blocks' sums in order.
+__global__ void __launch_bounds__(256) k_cw_join(WeightsArgs a, size_t ld_pos) {
+    const int g = blockIdx.y;
+    for (int k = blockIdx.z; k < a.head[2]; k += gridDim.z) {
+        const int4 c = a.list[k];
+        const int nb = (GRP * c.z + CW_ROWS - 1) / CW_ROWS;
+        for (int key = blockIdx.x * 256 + threadIdx.x; key < c.y; key += gridDim.x * 256) {
+            // the first block that sees the position: the first whose last row does
+            const int r = GRP * max(0, key - (c.y - c.z)), b0 = r / CW_ROWS;
+            float v = 0.0f;
+            for (int b = b0; b < nb; b++) v += a.parts[((size_t)(c.w + b) * NKV + g) * a.max_len + key];
+            float* const m = a.mass + ((size_t)c.x * NKV + g) * ld_pos + key;
+            *m = key < c.y - c.z ? *m + v : v;
+        }
+    }
+}
+
+hipError_t launch_weights_batch(const float* q, const float* lse, const qwa_kv_layer& kv, int kvt, const qwa_kv_pages& p,
+                                const int* seqs, const int* off, int n, int rows, int max_len, float* mass, void* work,
+                                hipStream_t st) {
+    const WeightsPlan pl = weights_plan(n, rows, max_len);
+    const WeightsWork w = weights_work(pl, max_len);
+    uint8_t* base = static_cast<uint8_t*>(work);
+    ChunkBlock* blocks = reinterpret_cast<ChunkBlock*>(base + w.blocks);
+    int4* list = reinterpret_cast<int4*>(base + w.list);
+    int* head = reinterpret_cast<int*>(base + w.head);
+    const WeightsArgs a{q, lse, mass, blocks, list, head, reinterpret_cast<float*>(base + w.parts), pl.slices, max_len};
+    hipLaunchKernelGGL(k_ch_plan<true>, dim3(1), dim3(CH_PT), 0, st, p, seqs, off, n, rows, max_len, pl.blocks, pl.parts / 2,
+                       pl.parts, blocks, list, head);
+    const dim3 grid(pl.slices * NKV), block(64 * CW_WAVES);
+    switch (kvt) {
+        case QWA_KV_F16: hipLaunchKernelGGL(k_cw_tiles<QWA_KV_F16>, grid, block, 0, st, a, kv, p); break;
+        case QWA_KV_Q8_0: hipLaunchKernelGGL(k_cw_tiles<QWA_KV_Q8_0>, grid, block, 0, st, a, kv, p); break;
+        default: hipLaunchKernelGGL(k_cw_tiles<QWA_KV_Q4_0>, grid, block, 0, st, a, kv, p); break;
+    }
+    if (pl.parts > 0) {
+        const dim3 jg((unsigned)std::min(64, (max_len + 255) / 256), NKV, (unsigned)std::min(pl.parts / 2, 16));
+        hipLaunchKernelGGL(k_cw_join, jg, dim3(256), 0, st, a, (size_t)p.ld * p.page);
     }
     return hipGetLastError();
 }

@@ -586,6 +586,26 @@ int qwa_attn_prefill_batch(const float* q, const float* gate, const qwa_kv_layer
                     fn);
 }
 
+size_t qwa_attn_weights_batch_work_bytes(int n, int rows, int max_len) {
+    return chunk_sizes_ok(n, rows, max_len) ? qwa::weights_batch_work_bytes(n, rows, max_len) : 0;
+}
+
+int qwa_attn_weights_batch(const float* q, const float* lse, const qwa_kv_layer* kv, int kvt, const qwa_kv_pages* p,
+                           const int* seqs, const int* off, int n, int rows, int max_len, float* mass, void* work,
+                           size_t work_bytes, void* stream) {
+    const char* fn = "attn_weights_batch";
+    const void* const bufs[] = {q, work};
+    int st;
+    if (max_len < 0) max_len = 0;
+    if ((st = check_chunks(p, kv, kvt, seqs, off, n, rows, max_len, fn)) || (st = check_buffers(bufs, 2, fn)) ||
+        (st = check_size(work_bytes, qwa::weights_batch_work_bytes(n, rows, max_len), fn)))
+        return st;
+    if (!lse || !mass) return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    return from_hip(qwa::launch_weights_batch(q, lse, *kv, kvt, *p, seqs, off, n, rows, max_len, mass, work,
+                                              as_stream(stream)),
+                    fn);
+}
+
 // ---- Gated DeltaNet
 namespace {
 int check_dn_params(const qwa_dn_params* p, const char* fn) {

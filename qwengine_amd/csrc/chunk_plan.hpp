@@ -75,4 +75,32 @@ inline ChunkWork chunk_work(const ChunkPlan& p) {
     return w;
 }
 
+// The weights: blocks of CW_ROWS rows, tiles of CW_TILE keys.  A block's sums go to its sequence's weights if it is its
+// chunk's only one, else to a place [KV head][max_len] of the work buffer, from which they are added up in order.
+// parts: places (a chunk of several blocks has at most twice as many as it has full ones).
+constexpr int CW_ROWS = 256, CW_TILE = 64;
+struct WeightsPlan {
+    int blocks, slices, parts;
+};
+inline WeightsPlan weights_plan(int n, int rows, int max_len) {
+    WeightsPlan p;
+    const long long full = (long long)GRP * rows / CW_ROWS;
+    p.blocks = (int)std::min<long long>((long long)GRP * rows, full + n);
+    p.slices = (int)std::min<long long>(CH_SLICES, (long long)p.blocks * ((max_len + CW_TILE - 1) / CW_TILE));
+    p.parts = (int)std::min<long long>(p.blocks, 2 * full);
+    return p;
+}
+struct WeightsWork {
+    size_t parts, blocks, list, head, bytes;  // byte offsets
+};
+inline WeightsWork weights_work(const WeightsPlan& p, int max_len) {
+    WeightsWork w;
+    w.parts = 0;
+    w.blocks = w.parts + ((size_t)p.parts * NKV * max_len * 4 + 15) / 16 * 16;
+    w.list = w.blocks + p.blocks * CH_BLOCK_BYTES;
+    w.head = w.list + (size_t)(p.parts / 2) * 16;
+    w.bytes = w.head + 16;
+    return w;
+}
+
 }  // namespace qwa

@@ -92,6 +92,11 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
                                 const int* seqs, const int* off, int n, int rows, int max_len, uint16_t* out16, float* lse,
                                 void* work, hipStream_t st);
 
+size_t weights_batch_work_bytes(int n, int rows, int max_len);
+hipError_t launch_weights_batch(const float* q, const float* lse, const qwa_kv_layer& kv, int kvt, const qwa_kv_pages& p,
+                                const int* seqs, const int* off, int n, int rows, int max_len, float* mass, void* work,
+                                hipStream_t st);
+
 // split-K decode: 16-key chunks in DEC_CLASSES fixed residue classes per KV head (chunk index mod DEC_CLASSES)
 constexpr int DEC_CLASSES = 512;
 size_t dec_work_bytes(int n_pos);

@@ -133,6 +133,10 @@ EXPORTS = {
     "qwa_attn_prefill_batch": (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.POINTER(_KVLayerC), ctypes.c_int,
                                                                       ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
                                [ctypes.c_int] * 3 + [ctypes.c_void_p] * 3 + [ctypes.c_size_t, ctypes.c_void_p]),
+    "qwa_attn_weights_batch_work_bytes": (ctypes.c_size_t, [ctypes.c_int] * 3),
+    "qwa_attn_weights_batch": (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.POINTER(_KVLayerC), ctypes.c_int,
+                                                                      ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
+                               [ctypes.c_int] * 3 + [ctypes.c_void_p] * 2 + [ctypes.c_size_t, ctypes.c_void_p]),
     "qwa_deltanet_step": (ctypes.c_int, [ctypes.POINTER(_DNParamsC)] + [ctypes.c_void_p] * 4 +
                           [ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.POINTER(_ActQ8C), ctypes.c_void_p]),
     "qwa_deltanet_multi": (ctypes.c_int, [ctypes.POINTER(_DNParamsC), ctypes.c_int, ctypes.POINTER(_DNTokensC)] +
@@ -647,6 +651,22 @@ def attn_prefill_batch(q, gate, kv: KVLayer, kvt, pages: KVPages, seqs, off, n: 
         None if seqs is None else _count(seqs, n, "seqs"), _count(off, n + 1, "off"), n, rows, max_len,
         _dev(out16, torch.float16, "out16", size), None if lse is None else _dev(lse, f32, "lse", rows * N_HEAD),
         *_work(work), _stream(stream)))
+
+
+def attn_weights_batch_work_bytes(n: int, rows: int, max_len: int) -> int:
+    return int(lib().qwa_attn_weights_batch_work_bytes(n, rows, max_len))
+
+
+def attn_weights_batch(q, lse, kv: KVLayer, kvt, pages: KVPages, seqs, off, n: int, rows: int, max_len: int, mass, work,
+                       stream=None) -> None:
+    """Adds the attention weight that a layer's positions gather from the chunks' tokens (summed over the 6 query heads of each KV
+    head) to mass (float32 [n_seq, 4, ld * page]); a chunk's own positions begin with it.  q and lse are those of the chunks'
+    attn_prefill_batch call."""
+    f32, kvt, pc = torch.float32, _kvt(kvt), pages.c()
+    _check(lib().qwa_attn_weights_batch(
+        _dev(q, f32, "q", rows * 6144), _dev(lse, f32, "lse", rows * N_HEAD), _pool(kv, kvt), kvt, ctypes.byref(pc),
+        None if seqs is None else _count(seqs, n, "seqs"), _count(off, n + 1, "off"), n, rows, max_len,
+        _dev(mass, f32, "mass", pc.n_seq * N_KV * pc.ld * pc.page), *_work(work), _stream(stream)))
 
 
 # ---- Gated DeltaNet ------------------------------------------------------------------------------------------------
