@@ -307,6 +307,25 @@ int qwa_attn_weights_batch(const float* q, const float* lse, const qwa_kv_layer*
                            const int* seqs, const int* off, int n, int rows, int max_len, float* mass, void* work,
                            size_t work_bytes, void* stream);
 
+/* Bytes of the `work` buffer of qwa_kv_pages_evict (device memory, 16-byte aligned; 0: invalid arguments). */
+size_t qwa_kv_pages_evict_work_bytes(const qwa_kv_pages* p, int n, int n_layers, int max_keep);
+
+/* Cuts sequence seqs[i] (device arrays of n entries) to keep[i] <= max_keep positions, if it has more: each KV head of each layer
+ * keeps its last min(recent, keep[i]) positions and, of the others, those of the largest weight in mass (fp32, device, 16-byte
+ * aligned, [n_layers][n_seq][4][ld * page], as qwa_attn_weights_batch gathers it), the lower position of equal ones, NaN last.
+ * The kept positions move to the front in their order, in every layer of `layers` and in mass; heads and layers keep
+ * different positions.  The sequence's length becomes keep[i]; the pages past that are given back.  Pages of the kept part that
+ * other sequences hold too are left to them and replaced by free ones, lowest first, request by request.  dropped[i] (device)
+ * becomes the number of positions that went: keys carry their rotary position with them, so for the sequence's next tokens
+ * the preps' rope_off grows by it.  All or nothing: *status (device) becomes 0 when done; the number of missing pages when
+ * the free ones do not suffice; -(i + 1) when request i is invalid (no such sequence, named before, keep outside
+ * [0, max_keep]; or a broken table: a length outside [0, ld * page], a page that is none of the pool's).  In the last two cases
+ * nothing is changed, and dropped is 0.
+ * work: at least qwa_kv_pages_evict_work_bytes bytes, one for each call or captured graph that may run at the same time. */
+int qwa_kv_pages_evict(const qwa_kv_pages* p, const int* seqs, const int* keep, int n, int recent, int max_keep,
+                       const qwa_kv_layer* layers, int n_layers, int kvt, float* mass, int* dropped, int* status, void* work,
+                       size_t work_bytes, void* stream);
+
 /* ---- Gated DeltaNet (the recurrent token mixer of the other layers) ---------------------------------------------- */
 
 /* New tokens per qwa_deltanet_multi call (the reference's DN_MAXN = Engine::MAX_BATCH, src/cuda/ops.cu:148). */

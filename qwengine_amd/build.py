@@ -19,8 +19,8 @@ LIB = os.path.join(OUT_DIR, "libqwattn.so")
 ARCH = "gfx950"
 
 SOURCES = ["capi.hip", "kv_append.hip", "attn_decode.hip", "attn_decode_ilp.hip", "attn_simple.hip", "attn_prefill.hip",
-           "attn_batch.hip", "attn_chunks.hip", "kv_pages.hip", "deltanet.hip", "deltanet_rows.hip", "gemv.hip", "gemv_mc.hip",
-           "gemm.cpp"]
+           "attn_batch.hip", "attn_chunks.hip", "kv_pages.hip", "kv_evict.hip", "deltanet.hip", "deltanet_rows.hip", "gemv.hip",
+           "gemv_mc.hip", "gemm.cpp"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",

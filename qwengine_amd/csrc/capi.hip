@@ -606,6 +606,34 @@ int qwa_attn_weights_batch(const float* q, const float* lse, const qwa_kv_layer*
                     fn);
 }
 
+static bool evict_sizes_ok(int n, int n_layers, int max_keep) {
+    return n >= 0 && n <= QWA_PAGES_MAXN && n_layers >= 1 && n_layers <= QWA_PAGES_MAXL && max_keep >= 0 &&
+           max_keep <= qwa::MAX_POS;
+}
+
+size_t qwa_kv_pages_evict_work_bytes(const qwa_kv_pages* p, int n, int n_layers, int max_keep) {
+    return pages_ok(p) && evict_sizes_ok(n, n_layers, max_keep) ? qwa::evict_work_bytes(*p, n, n_layers, max_keep) : 0;
+}
+
+int qwa_kv_pages_evict(const qwa_kv_pages* p, const int* seqs, const int* keep, int n, int recent, int max_keep,
+                       const qwa_kv_layer* layers, int n_layers, int kvt, float* mass, int* dropped, int* status, void* work,
+                       size_t work_bytes, void* stream) {
+    const char* fn = "kv_pages_evict";
+    int st;
+    if ((st = check_pages(p, fn)) || (st = check_requests(n, fn)) || (st = check_layers(layers, n_layers, kvt, p, fn)))
+        return st;
+    if (!evict_sizes_ok(n, n_layers, max_keep))
+        return fail(QWA_ERR_RANGE, "%s: max_keep %d (0..%d)", fn, max_keep, qwa::MAX_POS);
+    if (recent < 0) return fail(QWA_ERR_INVALID, "%s: recent = %d", fn, recent);
+    if (!status || !work || (n > 0 && (!seqs || !keep || !mass || !dropped)))
+        return fail(QWA_ERR_INVALID, "%s: null pointer", fn);
+    if (!al16(work) || !al16(mass)) return fail(QWA_ERR_INVALID, "%s: buffer not 16-byte aligned", fn);
+    if ((st = check_size(work_bytes, qwa::evict_work_bytes(*p, n, n_layers, max_keep), fn))) return st;
+    return from_hip(qwa::launch_pages_evict(*p, seqs, keep, n, recent, max_keep, layers, n_layers, kvt, mass, dropped, status,
+                                            work, as_stream(stream)),
+                    fn);
+}
+
 // ---- Gated DeltaNet
 namespace {
 int check_dn_params(const qwa_dn_params* p, const char* fn) {

@@ -80,6 +80,12 @@ hipError_t launch_pages_trim(const qwa_kv_pages& p, const int* seqs, const int* 
 hipError_t launch_pages_compact(const qwa_kv_pages& p, const qwa_kv_layer* layers, int n_layers, int kvt, int* n_live,
                                 void* work, hipStream_t st);
 
+// kv_evict.hip
+size_t evict_work_bytes(const qwa_kv_pages& p, int n, int n_layers, int max_keep);
+hipError_t launch_pages_evict(const qwa_kv_pages& p, const int* seqs, const int* keep, int n, int recent, int max_keep,
+                              const qwa_kv_layer* layers, int n_layers, int kvt, float* mass, int* dropped, int* status,
+                              void* work, hipStream_t st);
+
 // attn_batch.hip
 size_t batch_work_bytes(int n, int nq, int n_shared, int max_len);
 hipError_t launch_decode_batch(const float* q, const float* gate, const qwa_kv_layer& kv, int kvt, const qwa_kv_pages& p,

@@ -137,6 +137,10 @@ EXPORTS = {
     "qwa_attn_weights_batch": (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.POINTER(_KVLayerC), ctypes.c_int,
                                                                       ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 +
                                [ctypes.c_int] * 3 + [ctypes.c_void_p] * 2 + [ctypes.c_size_t, ctypes.c_void_p]),
+    "qwa_kv_pages_evict_work_bytes": (ctypes.c_size_t, [ctypes.POINTER(_KVPagesC)] + [ctypes.c_int] * 3),
+    "qwa_kv_pages_evict": (ctypes.c_int, [ctypes.POINTER(_KVPagesC)] + [ctypes.c_void_p] * 2 + [ctypes.c_int] * 3 +
+                           [ctypes.POINTER(_KVLayerC)] + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 4 +
+                           [ctypes.c_size_t, ctypes.c_void_p]),
     "qwa_deltanet_step": (ctypes.c_int, [ctypes.POINTER(_DNParamsC)] + [ctypes.c_void_p] * 4 +
                           [ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.POINTER(_ActQ8C), ctypes.c_void_p]),
     "qwa_deltanet_multi": (ctypes.c_int, [ctypes.POINTER(_DNParamsC), ctypes.c_int, ctypes.POINTER(_DNTokensC)] +
@@ -667,6 +671,25 @@ def attn_weights_batch(q, lse, kv: KVLayer, kvt, pages: KVPages, seqs, off, n: i
         _dev(q, f32, "q", rows * 6144), _dev(lse, f32, "lse", rows * N_HEAD), _pool(kv, kvt), kvt, ctypes.byref(pc),
         None if seqs is None else _count(seqs, n, "seqs"), _count(off, n + 1, "off"), n, rows, max_len,
         _dev(mass, f32, "mass", pc.n_seq * N_KV * pc.ld * pc.page), *_work(work), _stream(stream)))
+
+
+def kv_pages_evict_work_bytes(pages: KVPages, n: int, n_layers: int, max_keep: int) -> int:
+    return int(lib().qwa_kv_pages_evict_work_bytes(ctypes.byref(pages.c()), n, n_layers, max_keep))
+
+
+def kv_pages_evict(pages: KVPages, seqs, keep, recent: int, max_keep: int, layers, kvt, mass, dropped, status, work,
+                   n: int | None = None, stream=None) -> None:
+    """Cuts sequence seqs[i] to keep[i] <= max_keep positions (int32 GPU tensors): each layer's KV heads keep their last `recent`
+    positions and those of the largest weight in mass (float32 [layers, n_seq, 4, ld * page], attn_weights_batch), which
+    move to the front.  dropped (int32): how many positions went, by which the next tokens' rope_off grows.  All or nothing;
+    status (int32): 0 done, > 0 pages missing (for kept pages that others hold), -(i + 1) request i invalid."""
+    n, kvt = seqs.numel() if n is None else n, _kvt(kvt)
+    arr, nl = _layers(layers, kvt)
+    pc = pages.c()
+    _check(lib().qwa_kv_pages_evict(
+        ctypes.byref(pc), _count(seqs, n, "seqs"), _count(keep, n, "keep"), n, recent, max_keep, arr, nl, kvt,
+        _dev(mass, torch.float32, "mass", nl * pc.n_seq * N_KV * pc.ld * pc.page), _count(dropped, n, "dropped"),
+        _count(status, 1, "status"), *_work(work), _stream(stream)))
 
 
 # ---- Gated DeltaNet ------------------------------------------------------------------------------------------------
