@@ -37,7 +37,17 @@ struct alignas(16) ChunkBlock {
 };
 static_assert(sizeof(ChunkBlock) == CH_BLOCK_BYTES, "work buffer");
 
+// what the plan is made from
+struct ChunkSource {
+    qwa_kv_pages p;
+    const int* seqs;
+    const int* off;
+    int n, rows, max_len;
+};
+
 struct ChunkArgs {
+    ChunkSource src;
+    bool own;                // every workgroup makes the plan itself
     const float* q;
     const float* gate;
     uint16_t* out16;
@@ -83,11 +93,14 @@ __device__ __forceinline__ int ch_scan(int v, int* s_wave, int* total) {
 // length, first image, images).
 constexpr int CH_PT = QWA_PAGES_MAXN;
 template <bool WEIGHTS>
-__global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __restrict__ seqs, const int* __restrict__ off, int n,
-                                                   int rows, int max_len, int most, int most_list, int room,
+__global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, int most_list, int room,
                                                    ChunkBlock* __restrict__ blocks, int4* __restrict__ list,
                                                    int* __restrict__ head) {
     constexpr int ROWS = WEIGHTS ? CW_ROWS : CH_ROWS, TILE = WEIGHTS ? CW_TILE : PF_TILE;
+    const qwa_kv_pages& p = src.p;
+    const int* __restrict__ seqs = src.seqs;
+    const int* __restrict__ off = src.off;
+    const int n = src.n, rows = src.rows, max_len = src.max_len;
     __shared__ int s_wave[CH_PT / 64];
     __shared__ int s_end[CH_PT], s_first[CH_PT], s_count[CH_PT], s_len[CH_PT], s_seq[CH_PT], s_blk[CH_PT], s_place[CH_PT];
     const int t = threadIdx.x, lane = t & 63;
@@ -170,6 +183,84 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(qwa_kv_pages p, const int* __
     }
 }
 
+// The same of up to CH_OWN chunks and blocks, by one wave, in LDS; places without a bound.
+struct OwnPlan {
+    ChunkBlock blocks[CH_OWN];
+    int4 list[CH_OWN];
+    int head[4];
+};
+template <bool WEIGHTS>
+__device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& src) {
+    static_assert(CH_OWN == 64, "a lane a chunk, a lane a block");
+    constexpr int ROWS = WEIGHTS ? CW_ROWS : CH_ROWS, TILE = WEIGHTS ? CW_TILE : PF_TILE;
+    if (threadIdx.x < 64) {
+        const int t = threadIdx.x;
+        auto before = [&](int x) {  // sum over the lanes before
+            int y = x;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int z = __shfl_up(y, o, 64);
+                if (t >= o) y += z;
+            }
+            return y - x;
+        };
+        int first = t < src.n ? src.off[t] : 0, end = t < src.n ? src.off[t + 1] : 0;
+        int seq = t < src.n ? (src.seqs ? src.seqs[t] : t) : -1;
+        const bool known = seq >= 0 && seq < src.p.n_seq;
+        const int all = src.p.len[known ? seq : 0];
+        if (first < 0 || end > src.rows || end < first) end = first = 0;
+        int far = end;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(far, o, 64);
+            if (t >= o) far = max(far, y);
+        }
+        far = __shfl_up(far, 1, 64);
+        int count = end > first && (t == 0 || far <= first) ? end - first : 0;
+        if (!known) seq = -1;
+        if (WEIGHTS) {
+            if (!known) count = 0;
+            if (src.seqs) {
+                const int had = count;
+                for (int j = 1; j < src.n; j++) {
+                    const int oc = __builtin_amdgcn_readlane(had, j), os = __builtin_amdgcn_readlane(seq, j);
+                    if (j > t && oc > 0 && os == seq) count = 0;
+                }
+            }
+        }
+        const int len = known && count > 0 ? min(max(all, 0), src.max_len) : 0;
+        const int mine = (GRP * count + ROWS - 1) / ROWS, blk0 = before(mine);
+        const int want = WEIGHTS && mine > 1 ? mine : 0, place = before(want), entry = before(want > 0);
+        if (want > 0) plan.list[entry] = make_int4(seq, len, count, place);
+        const int nb = min(__builtin_amdgcn_readlane(blk0 + mine, 63), CH_OWN);
+        int lo = 0;  // block t's chunk
+        for (int j = 0; j < src.n; j++) {
+            const int b0 = __builtin_amdgcn_readlane(blk0, j);
+            if (t >= b0 && t < b0 + __builtin_amdgcn_readlane(mine, j)) lo = j;
+        }
+        ChunkBlock x = {};
+        x.row0 = __shfl(first, lo, 64);
+        x.count = __shfl(count, lo, 64);
+        x.len = __shfl(len, lo, 64);
+        x.seq = __shfl(seq, lo, 64);
+        x.blk = t - __shfl(blk0, lo, 64);
+        const int last = min((x.blk + 1) * ROWS, GRP * x.count) - 1;
+        x.end = max(0, x.len - x.count + last / GRP + 1);
+        x.tiles = t < nb ? max(1, (x.end + TILE - 1) / TILE) : 0;
+        const int pl = __shfl(place, lo, 64), many = __shfl(want, lo, 64);
+        x.place = many > 0 ? pl + x.blk : -1;
+        x.begin = before(x.tiles);
+        if (t < nb) plan.blocks[t] = x;
+        if (t == 63) {
+            plan.head[0] = nb;
+            plan.head[1] = x.begin + x.tiles;
+            plan.head[2] = entry + (want > 0);
+            plan.head[3] = 0;
+        }
+    }
+    __syncthreads();
+}
+
 // slices that hold tiles: the same number for every workgroup of a call
 __device__ __forceinline__ int ch_slices(int slices, int tiles) { return min(slices, tiles); }
 __device__ __forceinline__ int ch_cut(int w, int tiles, int slices) { return (int)((long long)w * tiles / slices); }
@@ -241,6 +332,14 @@ __global__ void __launch_bounds__(512) k_ch_image(ChunkArgs a, qwa_kv_layer kv, 
 #endif
 constexpr int CH_KD = QWA_CH_KD;    // K steps read ahead of their MFMAs
 constexpr int CH_VD = QWA_CH_VD;    // V fragments in flight
+
+// sigmoid by the reciprocal instruction (1 ulp; the output is rounded to fp16): the division's steps are a third of what the rows'
+// ends took
+__device__ __forceinline__ float ch_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + fast_exp2(-PF_LOG2E * x)); }
+__device__ __forceinline__ uint2 ch_gated(float4 v, float4 g) {
+    return make_uint2((uint32_t)f2h_bits(v.x * ch_sigmoid(g.x)) | ((uint32_t)f2h_bits(v.y * ch_sigmoid(g.y)) << 16),
+                      (uint32_t)f2h_bits(v.z * ch_sigmoid(g.z)) | ((uint32_t)f2h_bits(v.w * ch_sigmoid(g.w)) << 16));
+}
 constexpr int CH_RING = 3;  // tiles in LDS: the one read, and two on their way
 
 template <int KVT>
@@ -256,6 +355,7 @@ struct ChunkLds {
     } pair[CH_PAIRS];
     uint2 q[CH_PAIRS][16 * HD / 8];         // half of a row tile's Q, one part, on its way into operands
     int found;
+    OwnPlan plan;
 };
 
 // A segment: the tiles [tb, tb + nt) of a block that a workgroup walks.
@@ -363,13 +463,24 @@ __device__ __forceinline__ void ch_scores(f4 (&sc)[2][2], const h8 (&qb)[2][2][8
     for (int st = 0; st < CH_KD; st++) read(st);
 #pragma unroll
     for (int st = 0; st < 8; st++) {
+        // (two of the eight multiplications by scales behind each MFMA: they run while it does)
+        auto mix = [&](bool scales) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (scales) __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+            }
+        };
         __builtin_amdgcn_sched_barrier(0);
         multiply(st, 0);
         if (SC && st > 0) scale(st - 1, 1);
+        mix(SC && st > 0);
         __builtin_amdgcn_sched_barrier(0);
-        if (st + CH_KD < 8) read(st + CH_KD);
+        if (st + CH_KD < 8) read(st + CH_KD);  // (into the places of step st - 1)
+        __builtin_amdgcn_sched_barrier(0);
         multiply(st, 1);
         if (SC) scale(st, 0);
+        mix(SC);
     }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (SC) scale(7, 1);
@@ -411,9 +522,9 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
     const uint8_t* const kh = kv.k + head * value_bytes(KVT);
     const uint16_t* const ksh = SC ? kv.ks + head * 8 : nullptr;
     const ChunkImage* const img = a.images + (size_t)(max(sg.c.place, 0) + sg.tb) * NKV + g;
-    BtRaw<KVT> rk;
+    BtRaw<KVT> rk[2];
     ChunkPlaces<2> places;
-    auto load = [&](int i) {
+    auto load = [&](BtRaw<KVT>& rk, int i) {
         int at[2];
         places.next(at, p, table, sg.tb, sg.c.end, lane);
         const int h = pair >> 1, left = sg.c.end - (sg.tb + i) * PF_TILE - 16 * h;
@@ -430,7 +541,10 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
         else if (SC && pair < 2) wait_vmcnt<16 / CH_PAIRS + 1>();
         else wait_vmcnt<16 / CH_PAIRS>();
     };
-    if constexpr (!IMG) load(0);
+    if constexpr (!IMG) {
+        load(rk[0], 0);
+        if (sg.nt > 1) load(rk[1], 1);
+    }
     h8 qb[2][2][8];
     ch_load_q<KVT>(qb, a.q, sg.c, sg.wrow0, sg.nrows, g, lds.q[pair], lane);
     if constexpr (IMG) {
@@ -439,16 +553,16 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
         if (sg.nt > 1) copy(1);
         landed(sg.nt <= 1);
     } else {
-        bt_store_k<KVT>(rk, lds.k[slot(0)], lds.scales[slot(0)], t);
-        if (sg.nt > 1) load(1);
+        bt_store_k<KVT>(rk[0], lds.k[slot(0)], lds.scales[slot(0)], t);
+        if (sg.nt > 2) load(rk[0], 2);
     }
     __syncthreads();
-    for (int i = 0; i < sg.nt; i++) {
+    auto step = [&](int i, BtRaw<KVT>& rk) __attribute__((always_inline)) {
         if constexpr (IMG) {
             if (i + 2 < sg.nt) copy(i + 2);
         } else {
             if (i + 1 < sg.nt) bt_store_k<KVT>(rk, lds.k[slot(i + 1)], lds.scales[slot(i + 1)], t);
-            if (i + 2 < sg.nt) load(i + 2);
+            if (i + 3 < sg.nt) load(rk, i + 3);
         }
         if (sg.wrow0 < sg.nrows) {
             // (an opaque copy of the lane: the LDS addresses, kept across the tiles, spilled)
@@ -463,6 +577,14 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
         }
         if constexpr (IMG) landed(i + 2 >= sg.nt);
         __syncthreads();
+    };
+    if constexpr (IMG) {
+        for (int i = 0; i < sg.nt; i++) step(i, rk[0]);
+    } else {  // (the bytes of two tiles on their way: those of one were waited for where a workgroup is alone with its rows)
+        for (int i = 0; i < sg.nt; i += 2) {
+            step(i, rk[1]);
+            if (i + 1 < sg.nt) step(i + 1, rk[0]);
+        }
     }
 }
 
@@ -489,10 +611,10 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
     vmin = __builtin_amdgcn_readfirstlane(vmin);
-    BtRaw<KVT> rv;
+    BtRaw<KVT> rv[2];
     ChunkPlaces<2> places;
     uint32_t dead = 0;  // halves without a place, two bits a tile: tile i - 1, tile i, ...
-    auto load = [&](int i) {
+    auto load = [&](BtRaw<KVT>& rv, int i) {
         int at[2];
         places.next(at, p, table, sg.tb, sg.c.end, lane);
         const int left = sg.c.end - (sg.tb + i) * PF_TILE;
@@ -524,10 +646,11 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
         wait_vmcnt<0>();  // from here on vmcnt counts only the copies
         copy(0);
     } else {
-        dead = load(0) << 2;
+        dead = load(rv[0], 0) << 2;
+        if (sg.nt > 1) dead |= load(rv[1], 1) << 4;
     }
     __syncthreads();
-    for (int i = 0; i <= sg.nt; i++) {
+    auto step = [&](int i, BtRaw<KVT>& rv) __attribute__((always_inline)) {
         // (opaque copies: LDS addresses kept across the tiles took the registers of O)
         int ol = lane;
         asm volatile("" : "+v"(ol));
@@ -537,7 +660,7 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
         } else {
             if (i < sg.nt)
                 bt_store_v<KVT>(rv, lds.vt[slot(i)], lds.odd[(sg.base + i) & 1], 64 * pair + ol, (dead >> 2) & 3, sg.base + i);
-            if (i + 1 < sg.nt) dead |= load(i + 1) << 4;
+            if (i + 2 < sg.nt) dead |= load(rv, i + 2) << 6;
         }
         if (i > 0 && rows_here) {
             const int b = (i - 1) & 1, k0 = (sg.tb + i - 1) * PF_TILE;
@@ -639,6 +762,14 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
             if constexpr (IMG) landed(i + 1 >= sg.nt);
             __syncthreads();
         }
+    };
+    if constexpr (IMG) {
+        for (int i = 0; i <= sg.nt; i++) step(i, rv[0]);
+    } else {
+        for (int i = 0; i <= sg.nt; i += 2) {
+            step(i, rv[0]);
+            if (i < sg.nt) step(i + 1, rv[1]);
+        }
     }
     if (!rows_here) return;
     // O by way of LDS, half of a row tile's dims at a time, so that rows are written as they lie in memory
@@ -680,19 +811,24 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
                                     o[rt][8 * h + 6 + e][j] * il);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the area is the wave's own)
             __builtin_amdgcn_wave_barrier();
+            float4 v[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const int xr = 2 * k + (lane >> 5), row = sg.wrow0 + 16 * rt + xr;
-                const float4 v = area[32 * xr + (u ^ (xr & 7))];
-                if (whole) {
-                    const float4 gt = gv[r & 1][k];
-                    const uint2 w = make_uint2(
-                        (uint32_t)f2h_bits(v.x * sigmoid(gt.x)) | ((uint32_t)f2h_bits(v.y * sigmoid(gt.y)) << 16),
-                        (uint32_t)f2h_bits(v.z * sigmoid(gt.z)) | ((uint32_t)f2h_bits(v.w * sigmoid(gt.w)) << 16));
-                    if (row < sg.nrows) *reinterpret_cast<uint2*>(a.out16 + place(r, k)) = w;
-                } else if (row < sg.nrows) {
-                    *reinterpret_cast<float4*>(a.part_o + (part + row - CH_ROWS * sg.c.blk) * HD + 128 * e + 4 * u) = v;
+                const int xr = 2 * k + (lane >> 5);
+                v[k] = area[32 * xr + (u ^ (xr & 7))];
+            }
+            const int row0 = sg.wrow0 + 16 * rt + (lane >> 5);
+            if (whole) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const uint2 w = ch_gated(v[k], gv[r & 1][k]);
+                    if (row0 + 2 * k < sg.nrows) *reinterpret_cast<uint2*>(a.out16 + place(r, k)) = w;
                 }
+            } else {
+                float* const dst = a.part_o + (part + row0 - CH_ROWS * sg.c.blk) * HD + 128 * e + 4 * u;
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (row0 + 2 * k < sg.nrows) *reinterpret_cast<float4*>(dst + 2 * k * HD) = v[k];
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -710,14 +846,32 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     // workgroups 8 apart run on one XCD: each has consecutive slices of one head, whose tiles its L2 then holds
     int unit = blockIdx.x;
     if (gridDim.x % 8 == 0) unit = (int)(gridDim.x / 8) * (blockIdx.x & 7) + (blockIdx.x >> 3);
-    const int g = unit / a.slices, w = unit % a.slices;
-    const int nb = a.head[0], tiles = a.head[1];
-    const int slices = ch_slices(a.slices, tiles);
-    if (w >= slices) return;
-    int s = ch_cut(w, tiles, slices);
-    const int s_begin = s, s_end = ch_cut(w + 1, tiles, slices);
+    const ChunkBlock* blocks = a.blocks;
+    const int* head = a.head;
+    if (a.own) {
+        ch_own_plan<false>(lds.plan, a.src);
+        blocks = lds.plan.blocks;
+        head = lds.plan.head;
+    }
+    const int nb = __builtin_amdgcn_readfirstlane(head[0]), tiles = __builtin_amdgcn_readfirstlane(head[1]);
+    // a slice, or a block as a whole
+    const int per = a.slices > 0 ? a.slices : (int)gridDim.x / NKV, g = unit / per, w = unit % per;
+    int s, s_end, j;
     if (threadIdx.x < 8) lds.odd[threadIdx.x >> 2].tile[threadIdx.x & 3] = -1;
-    int j = ch_find(a.blocks, nb, s, &lds.found);
+    if (a.slices > 0) {
+        const int slices = ch_slices(a.slices, tiles);
+        if (w >= slices) return;
+        s = ch_cut(w, tiles, slices);
+        s_end = ch_cut(w + 1, tiles, slices);
+        j = ch_find(blocks, nb, s, &lds.found);
+    } else {
+        if (w >= nb) return;
+        j = w;
+        s = __builtin_amdgcn_readfirstlane(blocks[j].begin);
+        s_end = s + __builtin_amdgcn_readfirstlane(blocks[j].tiles);
+        __syncthreads();
+    }
+    const int s_begin = s;
     // The segments; the roles meet at a segment's barriers, one and one a tile.  Behind the last one the score waves go on to the
     // next segment's Q and K while the value waves finish: what these still read there (V and flags of the last tile, its
     // scores, which the pair's own O follows) is written by nobody before the next barrier.
@@ -726,7 +880,7 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         int t = threadIdx.x;
         asm volatile("" : "+v"(t));
         ChunkSegment sg;
-        sg.c = ch_block(a.blocks[j]);
+        sg.c = ch_block(blocks[j]);
         sg.base = s - s_begin;
         sg.tb = s - sg.c.begin;
         sg.nt = min(s_end, sg.c.begin + sg.c.tiles) - s;
@@ -751,12 +905,20 @@ constexpr int CH_JR = 16;  // rows of a workgroup
 template <bool LSE>
 __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a) {
     __shared__ int found;
-    const int tiles = a.head[1], slices = ch_slices(a.slices, tiles);
+    __shared__ OwnPlan plan;
+    const ChunkBlock* blocks = a.blocks;
+    const int* head = a.head;
+    if (a.own) {
+        ch_own_plan<false>(plan, a.src);
+        blocks = plan.blocks;
+        head = plan.head;
+    }
+    const int tiles = head[1], slices = ch_slices(a.slices, tiles);
     const int g = blockIdx.y, cut = blockIdx.x + 1;
     if (cut >= slices) return;
     const int s = ch_cut(cut, tiles, slices), s_before = ch_cut(cut - 1, tiles, slices);
-    const int j = ch_find(a.blocks, a.head[0], s, &found);
-    const ChunkBlock c = a.blocks[j];
+    const int j = ch_find(blocks, head[0], s, &found);
+    const ChunkBlock c = blocks[j];
     if (c.begin == s || c.begin < s_before) return;  // the cut lies between two blocks, or an earlier one lies in this
     // its slices: cut - 1 up to the one that holds its last tile
     const int last = c.begin + c.tiles - 1;
@@ -799,8 +961,7 @@ __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a) {
         }
         const float il = L == 0.0f ? 0.0f : 1.0f / L;
         *reinterpret_cast<uint2*>(a.out16 + out * HD + 4 * lane) =
-            make_uint2((uint32_t)f2h_bits(acc.x * il * sigmoid(gv.x)) | ((uint32_t)f2h_bits(acc.y * il * sigmoid(gv.y)) << 16),
-                       (uint32_t)f2h_bits(acc.z * il * sigmoid(gv.z)) | ((uint32_t)f2h_bits(acc.w * il * sigmoid(gv.w)) << 16));
+            ch_gated(make_float4(acc.x * il, acc.y * il, acc.z * il, acc.w * il), gv);
         if (LSE && lane == 0) a.lse[out] = X == 0.0f ? -INFINITY : (M + __log2f(X)) * 0.6931471805599453f;
     }
 }
@@ -814,10 +975,11 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
     ChunkBlock* blocks = reinterpret_cast<ChunkBlock*>(base + w.blocks);
     int* head = reinterpret_cast<int*>(base + w.head);
     int4* list = reinterpret_cast<int4*>(base + w.list);
-    const ChunkArgs a{q, gate, out16, lse, blocks, list, head, reinterpret_cast<ChunkImage*>(base + w.images),
+    const ChunkSource src{p, seqs, off, n, rows, max_len};
+    const ChunkArgs a{src, pl.own, q, gate, out16, lse, blocks, list, head, reinterpret_cast<ChunkImage*>(base + w.images),
                       reinterpret_cast<float*>(base + w.o), reinterpret_cast<float4*>(base + w.ml), pl.slices, pl.rows};
-    hipLaunchKernelGGL(k_ch_plan<false>, dim3(1), dim3(CH_PT), 0, st, p, seqs, off, n, rows, max_len, pl.blocks, pl.images, pl.tiles,
-                       blocks, list, head);
+    if (!pl.own)
+        hipLaunchKernelGGL(k_ch_plan<false>, dim3(1), dim3(CH_PT), 0, st, src, pl.blocks, pl.images, pl.tiles, blocks, list, head);
     if (pl.tiles > 0) {
         const dim3 ig((unsigned)std::min(pl.tiles * NKV, CH_IMG_WGS));
         switch (kvt) {
@@ -826,7 +988,7 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
             default: hipLaunchKernelGGL(k_ch_image<QWA_KV_Q4_0>, ig, dim3(512), 0, st, a, kv, p); break;
         }
     }
-    const dim3 grid(pl.slices * NKV), block(128 * CH_PAIRS);
+    const dim3 grid((pl.whole ? pl.blocks : pl.slices) * NKV), block(128 * CH_PAIRS);
 #define QWA_CH(T)                                                                              \
     case T:                                                                                    \
         if (lse) hipLaunchKernelGGL((k_ch_tiles<T, true>), grid, block, 0, st, a, kv, p);      \
@@ -849,6 +1011,8 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
 // ---- the weights: for position j of a sequence and KV head g, the sum over the chunk's rows (token, head of g) that see it of
 // exp(s_j - lse), added to what it had (the chunk's own positions begin with it).
 struct WeightsArgs {
+    ChunkSource src;
+    bool own;                  // every workgroup makes the plan itself
     const float* q;
     const float* lse;          // [rows][24]
     float* mass;               // [sequence][KV head][ld * page]
@@ -872,6 +1036,7 @@ struct WeightsLds {
     float sum[2][CW_WAVES][CW_TILE];   // of the waves' rows, by key
     uint2 q[CW_WAVES][16 * HD / 8];
     int found;
+    OwnPlan plan;
 };
 
 // A workgroup walks the 64-key tiles of a slice as k_ch_tiles does, with K alone: all waves convert it, then each takes the scores
@@ -886,12 +1051,19 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     int unit = blockIdx.x;
     if (gridDim.x % 8 == 0) unit = (int)(gridDim.x / 8) * (blockIdx.x & 7) + (blockIdx.x >> 3);
     const int g = unit / a.slices, w = unit % a.slices;
-    const int nb = a.head[0], tiles = a.head[1];
+    const ChunkBlock* blocks = a.blocks;
+    const int* head_of = a.head;
+    if (a.own) {
+        ch_own_plan<true>(lds.plan, a.src);
+        blocks = lds.plan.blocks;
+        head_of = lds.plan.head;
+    }
+    const int nb = __builtin_amdgcn_readfirstlane(head_of[0]), tiles = __builtin_amdgcn_readfirstlane(head_of[1]);
     const int slices = ch_slices(a.slices, tiles);
     if (w >= slices) return;
     int s = ch_cut(w, tiles, slices);
     const int s_end = ch_cut(w + 1, tiles, slices);
-    int j = ch_find(a.blocks, nb, s, &lds.found);
+    int j = ch_find(blocks, nb, s, &lds.found);
     const size_t head = (size_t)g * kv.capacity;
     const uint8_t* const kh = kv.k + head * value_bytes(KVT);
     const uint16_t* const ksh = SC ? kv.ks + head * 8 : nullptr;
@@ -900,7 +1072,7 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         int t = threadIdx.x;
         asm volatile("" : "+v"(t));
         const int lane = t & 63, i16 = lane & 15;
-        const ChunkBlock c = ch_block(a.blocks[j]);
+        const ChunkBlock c = ch_block(blocks[j]);
         const int tb = s - c.begin, nt = min(s_end, c.begin + c.tiles) - s;
         const int nrows = GRP * c.count, wrow0 = CW_ROWS * c.blk + 32 * wave;
         const bool rows_here = wrow0 < nrows;
@@ -917,48 +1089,54 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
         vmin = __builtin_amdgcn_readfirstlane(vmin);
-        BtRaw<KVT> rk;
+        BtRaw<KVT> rk[2];
         ChunkPlaces<G> places;
-        int dead_next = 0;
+        int dead_next = 0;  // groups without a place, four bits a tile, of the next tile to be stored first
         const int grp = __builtin_amdgcn_readfirstlane(t >> 7);  // the thread's group of 16 keys
-        auto load = [&](int i) {
+        auto load = [&](BtRaw<KVT>& rk, int i, int ahead) {
             int at[G];
             places.next(at, p, table, tb, c.end, lane);
             const int mine = grp == 0 ? at[0] : grp == 1 ? at[1] : grp == 2 ? at[2] : at[3];
-            dead_next = (at[0] < 0) | (at[1] < 0) << 1 | (at[2] < 0) << 2 | (at[3] < 0) << 3;
+            dead_next |= ((at[0] < 0) | (at[1] < 0) << 1 | (at[2] < 0) << 2 | (at[3] < 0) << 3) << (G * ahead);
             bt_load_k<KVT>(rk, kh, ksh, mine, min(max(c.end - (tb + i) * CW_TILE - 16 * grp, 0), 16), t);
         };
-        auto store = [&](int i) {
+        auto store = [&](BtRaw<KVT>& rk, int i) {
             const int b = i & 1, h = t >> 8;
             bt_store_k<KVT>(rk, lds.k[b] + PF_TILE * HD * h, lds.scales[b] + PF_TILE * 8 * h, t);
-            if (t == 0) lds.dead[b] = dead_next;
+            if (t == 0) lds.dead[b] = dead_next & ((1 << G) - 1);
+            dead_next >>= G;
         };
-        // the sums of tile i: to the sequence's weights, or to the block's place
+        // The sums of tile i: to the block's place, or to the sequence's weights, whose old values are read a tile ahead.  The
+        // last wave does it: of chunks of few tokens it is one that has no rows.
+        const bool writes = wave == CW_WAVES - 1;
+        float* const mass = a.mass + ((size_t)max(c.seq, 0) * NKV + g) * ((size_t)p.ld * p.page);
+        float old = 0.0f;
+        auto fetch = [&](int i) {
+            const int key = (tb + i) * CW_TILE + lane;
+            if (writes && c.place < 0) old = key < c.len - c.count ? mass[key] : 0.0f;
+        };
         auto write = [&](int i) {
-            if (t >= CW_TILE) return;
-            const int key = (tb + i) * CW_TILE + t;
-            if (key >= c.end) return;
+            const int key = (tb + i) * CW_TILE + lane;
+            if (!writes || key >= c.end) return;
             float v = 0.0f;
 #pragma unroll
-            for (int k = 0; k < CW_WAVES; k++) v += lds.sum[i & 1][k][t];
-            if (c.place >= 0) {
-                a.parts[((size_t)c.place * NKV + g) * a.max_len + key] = v;
-            } else {
-                float* const m = a.mass + ((size_t)c.seq * NKV + g) * ((size_t)p.ld * p.page) + key;
-                *m = key < c.len - c.count ? *m + v : v;
-            }
+            for (int k = 0; k < CW_WAVES; k++) v += lds.sum[i & 1][k][lane];
+            if (c.place >= 0) a.parts[((size_t)c.place * NKV + g) * a.max_len + key] = v;
+            else mass[key] = old + v;
         };
-        load(0);
+        load(rk[0], 0, 0);
+        if (nt > 1) load(rk[1], 1, 1);
         h8 qb[2][2][8];
         ch_load_q<KVT>(qb, a.q, c, wrow0, nrows, g, lds.q[wave], lane);
-        store(0);
-        if (nt > 1) load(1);
+        store(rk[0], 0);
+        if (nt > 2) load(rk[0], 2, 1);
         __syncthreads();
-        for (int i = 0; i < nt; i++) {
+        auto step = [&](int i, BtRaw<KVT>& rk) __attribute__((always_inline)) {
             const int k0 = (tb + i) * CW_TILE, b = i & 1;
             if (i > 0) write(i - 1);
-            if (i + 1 < nt) store(i + 1);
-            if (i + 2 < nt) load(i + 2);
+            fetch(i);
+            if (i + 1 < nt) store(rk, i + 1);
+            if (i + 3 < nt) load(rk, i + 3, 1);
             int ol = lane;  // (opaque: LDS addresses kept across the tiles)
             asm volatile("" : "+v"(ol));
             const int oi = ol & 15, og = ol >> 4;
@@ -1000,6 +1178,10 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
                 }
             }
             __syncthreads();
+        };
+        for (int i = 0; i < nt; i += 2) {
+            step(i, rk[1]);
+            if (i + 1 < nt) step(i + 1, rk[0]);
         }
         write(nt - 1);
         // (the next segment's first sums are written behind its first barrier)
@@ -1010,9 +1192,11 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
 
 // The weights of chunks of several blocks: the blocks' sums in order.
 __global__ void __launch_bounds__(256) k_cw_join(WeightsArgs a, size_t ld_pos) {
-    const int g = blockIdx.y;
-    for (int k = blockIdx.z; k < a.head[2]; k += gridDim.z) {
-        const int4 c = a.list[k];
+    __shared__ OwnPlan plan;
+    if (a.own) ch_own_plan<true>(plan, a.src);
+    const int g = blockIdx.y, n = a.own ? plan.head[2] : a.head[2];
+    for (int k = blockIdx.z; k < n; k += gridDim.z) {
+        const int4 c = a.own ? plan.list[k] : a.list[k];
         const int nb = (GRP * c.z + CW_ROWS - 1) / CW_ROWS;
         for (int key = blockIdx.x * 256 + threadIdx.x; key < c.y; key += gridDim.x * 256) {
             // the first block that sees the position: the first whose last row does
@@ -1034,9 +1218,10 @@ hipError_t launch_weights_batch(const float* q, const float* lse, const qwa_kv_l
     ChunkBlock* blocks = reinterpret_cast<ChunkBlock*>(base + w.blocks);
     int4* list = reinterpret_cast<int4*>(base + w.list);
     int* head = reinterpret_cast<int*>(base + w.head);
-    const WeightsArgs a{q, lse, mass, blocks, list, head, reinterpret_cast<float*>(base + w.parts), pl.slices, max_len};
-    hipLaunchKernelGGL(k_ch_plan<true>, dim3(1), dim3(CH_PT), 0, st, p, seqs, off, n, rows, max_len, pl.blocks, pl.parts / 2,
-                       pl.parts, blocks, list, head);
+    const ChunkSource src{p, seqs, off, n, rows, max_len};
+    const WeightsArgs a{src, pl.own, q, lse, mass, blocks, list, head, reinterpret_cast<float*>(base + w.parts), pl.slices, max_len};
+    if (!pl.own)
+        hipLaunchKernelGGL(k_ch_plan<true>, dim3(1), dim3(CH_PT), 0, st, src, pl.blocks, pl.parts / 2, pl.parts, blocks, list, head);
     const dim3 grid(pl.slices * NKV), block(64 * CW_WAVES);
     switch (kvt) {
         case QWA_KV_F16: hipLaunchKernelGGL(k_cw_tiles<QWA_KV_F16>, grid, block, 0, st, a, kv, p); break;

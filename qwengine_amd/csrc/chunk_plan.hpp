@@ -36,10 +36,19 @@ struct ChunkImage {
 
 // A chunk's rows are cut into blocks of CH_ROWS; a block walks the PF_TILE-key tiles from the first to the last that one of its
 // rows sees.  The tiles of all blocks in a row, cut into `slices` equal parts, are the workgroups of a KV head.
-// blocks, slices, images (chunks that read images), tiles (of images): bounds of what the device finds, which knows the chunks;
+// blocks, slices (0: every block as a whole), images (chunks that read images), tiles (of images): bounds of what the device finds, which knows the chunks;
 // rows: of a block that are stored.
+// Calls of few chunks and blocks, without images, need no plan from a kernel of its own: a wave of every workgroup makes it, a
+// lane a chunk, a lane a block.
+constexpr int CH_OWN = 64;
+// Short sequences are not cut into slices: a workgroup has a block as a whole, and no states are joined.
+#ifndef QWA_CH_WHOLE
+#define QWA_CH_WHOLE 512
+#endif
+constexpr int CH_WHOLE = QWA_CH_WHOLE;
 struct ChunkPlan {
     int blocks, slices, rows, images, tiles;
+    bool whole, own;
 };
 
 inline ChunkPlan chunk_plan(int n, int rows, int max_len) {
@@ -47,11 +56,13 @@ inline ChunkPlan chunk_plan(int n, int rows, int max_len) {
     const int most = (max_len + PF_TILE - 1) / PF_TILE;
     // (a chunk has one partly filled block)
     p.blocks = (int)std::min<long long>((long long)GRP * rows, (long long)GRP * rows / CH_ROWS + n);
-    p.slices = (int)std::min<long long>(CH_SLICES, (long long)p.blocks * most);
+    p.whole = max_len <= CH_WHOLE;
+    p.slices = p.whole ? 0 : (int)std::min<long long>(CH_SLICES, (long long)p.blocks * most);
     p.rows = std::min(CH_ROWS, GRP * rows);
     // (a chunk of CH_IMG_BLOCKS blocks has more than CH_IMG_BLOCKS - 1 full ones)
     p.images = std::min(n, (int)((long long)GRP * rows / (CH_ROWS * (CH_IMG_BLOCKS - 1))));
     p.tiles = (int)std::min<long long>((long long)p.images * most, std::max(most, CH_IMG_TILES));
+    p.own = n <= CH_OWN && p.blocks <= CH_OWN && p.images == 0;
     return p;
 }
 
@@ -81,6 +92,7 @@ inline ChunkWork chunk_work(const ChunkPlan& p) {
 constexpr int CW_ROWS = 256, CW_TILE = 64;
 struct WeightsPlan {
     int blocks, slices, parts;
+    bool own;
 };
 inline WeightsPlan weights_plan(int n, int rows, int max_len) {
     WeightsPlan p;
@@ -88,6 +100,7 @@ inline WeightsPlan weights_plan(int n, int rows, int max_len) {
     p.blocks = (int)std::min<long long>((long long)GRP * rows, full + n);
     p.slices = (int)std::min<long long>(CH_SLICES, (long long)p.blocks * ((max_len + CW_TILE - 1) / CW_TILE));
     p.parts = (int)std::min<long long>(p.blocks, 2 * full);
+    p.own = n <= CH_OWN && p.blocks <= CH_OWN;
     return p;
 }
 struct WeightsWork {

@@ -4,7 +4,7 @@
 // others, those of the largest weight w_j, the lower position of equals, in their order.  With r_0 < r_1 < ... the positions
 // kept, row r_i of K, V, scales and weights moves to position i; the layers and heads keep different positions, but as many, so
 // one length and one table row serve them all.
-//  * k_evict_select (a workgroup per request, layer and head) finds the smallest weight kept by its bits, 11 at a time (a histogram
+//  * k_evict_select (a workgroup per request, layer and head, and one per request for its pages) finds the smallest weight kept by its bits, 11 at a time (a histogram
 //    in LDS of those that agree in the bits before), and lists the kept positions' places in the pool.  Nothing changes yet.
 //  * k_evict_plan (one workgroup) checks all requests, takes pages for those of the first `keep` positions that other sequences
 //    hold too, and changes the tables.
@@ -20,6 +20,8 @@ namespace qwa {
 constexpr int EV_T = 1024;       // threads of the selecting and the planning workgroups
 constexpr int EV_E = 32;         // most weights a thread holds
 constexpr int EV_BINS = 2048;
+constexpr int EV_LANE = 16;      // weights a lane holds where one wave does
+static_assert(64 * EV_LANE < 1 << 15 && EV_LANE % 16 == 0, "counts of both kinds in a word, a page a 16 positions");
 static_assert(EV_T >= QWA_PAGES_MAXN, "one thread per request");
 
 // work buffer (ints): whether the plan holds, then per request its number of shared pages (-1: invalid, -2: nothing to do), the
@@ -60,7 +62,7 @@ __device__ __forceinline__ uint32_t ev_key(float x) {
 }
 
 __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
-    __shared__ int s_hist[EV_BINS];
+    __shared__ __attribute__((aligned(16))) int s_hist[EV_BINS];
     __shared__ long long s_wave[EV_T / 64];
     __shared__ int s_bin, s_above;
     const int t = threadIdx.x, i = blockIdx.y, lh = blockIdx.x;
@@ -70,8 +72,7 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
     if (seq >= 0 && seq < a.p.n_seq && keep >= 0 && keep <= a.max_keep) m = a.p.len[seq];
     const bool valid = m >= 0 && m <= (long long)a.p.ld * a.p.page;
     const int* __restrict__ table = a.p.table + (size_t)max(seq, 0) * a.p.ld;
-    if (lh == 0) {
-        // the request's pages
+    if (lh == a.n_layers * NKV) {  // the request's pages, by a workgroup of its own
         int bad = !valid, shared = 0;
         if (valid && m > keep) {
             const int kept = pages_of(keep, a.p.page), per = pages_of(a.max_keep, a.p.page);
@@ -88,6 +89,7 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
         long long all;
         block_scan<EV_T>(((long long)bad << 32) + shared, s_wave, &all);
         if (t == 0) a.work[w.count + i] = (all >> 32) ? -1 : m > keep ? (int)(all & 0xffffffffLL) : -2;
+        return;
     }
     if (!valid || m <= keep || keep == 0) return;
 
@@ -114,6 +116,65 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
             }
     };
     if (runs == 1) load(0);
+    const size_t at = ((size_t)i * a.n_layers * NKV + lh) * a.max_keep;
+    int* const rows = a.work + w.rows + at;
+    float* const out = reinterpret_cast<float*>(a.work + w.mass) + at;
+    const int sh = __builtin_ctz(a.p.page);
+    if (m <= 64 * EV_LANE) {
+        // Few positions: one wave, EV_LANE neighbouring ones a lane, without LDS or barriers.  The key, the largest that at least
+        // `want` candidates reach, bit by bit.  (By the histograms below 600 positions take 19 us, this way FEW_US.)
+        if (t >= 64) return;
+        float x[EV_LANE];
+        uint32_t k[EV_LANE];
+        const int j0 = EV_LANE * t;
+        int pg[EV_LANE / 16];
+#pragma unroll
+        for (int e = 0; e < EV_LANE; e++) x[e] = j0 + e < m ? mass[j0 + e] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < EV_LANE / 16; e++) pg[e] = table[min(j0 + 16 * e, m - 1) >> sh];  // (a foreign page's request changes nothing)
+#pragma unroll
+        for (int e = 0; e < EV_LANE; e++) k[e] = j0 + e < c ? ev_key(x[e]) : 0u;
+        uint32_t key = 0;
+        if (want > 0) {
+            for (int bit = 31; bit >= 0; bit--) {
+                const uint32_t up = key | 1u << bit;
+                int reach = 0;
+#pragma unroll
+                for (int e = 0; e < EV_LANE; e++) reach += __popcll(__ballot(k[e] >= up));
+                if (reach >= want) key = up;
+            }
+            int above = 0;
+#pragma unroll
+            for (int e = 0; e < EV_LANE; e++) above += __popcll(__ballot(k[e] > key));
+            want -= above;  // of those that equal it
+        }
+        int more = 0, same = 0;
+#pragma unroll
+        for (int e = 0; e < EV_LANE; e++) {
+            const bool last = j0 + e >= c && j0 + e < m, cand = j0 + e < c && keep > near;
+            more += last || (cand && k[e] > key);
+            same += cand && k[e] == key;
+        }
+        int sum = more | same << 16;  // (at most 64 * EV_LANE of both)
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(sum, o, 64);
+            if (t >= o) sum += y;
+        }
+        sum -= more | same << 16;
+        int before = sum >> 16, place = (sum & 0xffff) + min(before, want);
+#pragma unroll
+        for (int e = 0; e < EV_LANE; e++) {
+            const bool cand = j0 + e < c && keep > near;
+            bool stays = (j0 + e >= c && j0 + e < m) || (cand && k[e] > key);
+            if (cand && k[e] == key) stays = before++ < want;
+            if (stays && place < keep) {
+                rows[place] = (pg[e / 16] << sh) + ((j0 + e) & (a.p.page - 1));
+                out[place++] = x[e];
+            }
+        }
+        return;
+    }
     // the smallest key that stays, by its highest 11 bits, the next 11 and the last 10
     uint32_t key = 0;
     if (want > 0) {
@@ -153,14 +214,15 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
         }
     }
     // kept: the last ones, those above the key, and the first `want` that equal it
-    const size_t at = ((size_t)i * a.n_layers * NKV + lh) * a.max_keep;
-    int* const rows = a.work + w.rows + at;
-    float* const out = reinterpret_cast<float*>(a.work + w.mass) + at;
     const int all_want = keep - near;
     long long done = 0;  // kept so far, and (upper half) equals so far
     for (int r = 0; r < runs; r++) {
         if (runs > 1) load(r);
         const int j0 = r * run + t * per;
+        // the pages of the thread's positions (of 16 positions at least: three for 32), on their way meanwhile
+        int pg[3];
+#pragma unroll
+        for (int k = 0; k < 3; k++) pg[k] = table[min((j0 >> sh) + k, (m - 1) >> sh)];
         int more = 0, same = 0;
 #pragma unroll
         for (int e = 0; e < EV_E; e++)
@@ -184,8 +246,9 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
                     bool stays = last || (all_want > 0 && k > key);
                     if (!last && all_want > 0 && k == key) stays = before++ < want;
                     if (stays && place < keep) {
-                        const int pg = table[(j0 + e) / a.p.page];  // (a foreign page's request changes nothing)
-                        rows[place] = pg * a.p.page + (j0 + e) % a.p.page;
+                        const int k = ((j0 + e) >> sh) - (j0 >> sh);
+                        const int base = k == 0 ? pg[0] : k == 1 ? pg[1] : pg[2];
+                        rows[place] = (base << sh) + ((j0 + e) & (a.p.page - 1));  // (a foreign page's request changes nothing)
                         out[place++] = x[e];
                     }
                 }
@@ -280,91 +343,126 @@ __global__ void __launch_bounds__(EV_T) k_evict_plan(EvictArgs a, int* __restric
     }
 }
 
-// The rows of a request, layer and head, of K or V.
+// The rows of a request, layer and head, of K or V: PARTS workgroups, each with a part of the columns (the order of the rows binds
+// a workgroup; their columns do not depend on each other).  While a run is written, the next one is on its way, and the places
+// of that after it.
 constexpr int EV_MT = 512;  // threads
-template <int KVT>
+template <int KVT, int PARTS>
 __global__ void __launch_bounds__(EV_MT) k_evict_move(EvictArgs a, PageLayers layers) {
-    constexpr int VB = value_bytes(KVT), UNITS = VB / 16;  // 16-byte units of a row
-    constexpr int U = 8, ROWS = EV_MT * U / UNITS;         // units a thread moves of a run, rows of it
-    static_assert(ROWS <= EV_MT, "a thread a row for the scales");
+    constexpr int VB = value_bytes(KVT), UNITS = VB / 16 / PARTS;  // 16-byte units of a row's part
+    constexpr int U = PARTS == 1 ? 8 : 4;                          // units a thread moves of a run
+    constexpr int ROWS = EV_MT * U / UNITS;                        // rows of it
+    constexpr int SU = KVT == QWA_KV_F16 ? 0 : (ROWS + EV_MT - 1) / EV_MT;  // rows whose scales it moves
     const int t = threadIdx.x;
     const EvictWork w = evict_work(a.p, a.n, a.n_layers, a.max_keep);
-    const int which = blockIdx.x & 1, lh = blockIdx.x >> 1, i = blockIdx.y, l = lh / NKV, h = lh % NKV;
+    // (parts of the same rows 8 workgroups apart: one XCD, whose L2 then holds their lines)
+    const int part = blockIdx.x / 8 % PARTS, unit = blockIdx.x / (8 * PARTS) * 8 + blockIdx.x % 8;
+    const int which = unit & 1, lh = unit >> 1, i = blockIdx.y;
+    const int l = lh / NKV, h = lh % NKV;
     if (a.work[0] == 0 || a.work[w.count + i] < 0) return;
-    const int seq = a.seqs[i], keep = a.keep[i];
+    const int seq = a.seqs[i], keep = a.keep[i], sh = __builtin_ctz(a.p.page);
     const int* __restrict__ table = a.p.table + (size_t)seq * a.p.ld;
     const size_t at = ((size_t)i * a.n_layers * NKV + lh) * a.max_keep;
     const int* __restrict__ rows = a.work + w.rows + at;
     const qwa_kv_layer& kv = layers.l[l];
     const size_t head = (size_t)h * kv.capacity;
-    uint8_t* const vals = (which ? kv.v : kv.k) + head * VB;
+    uint8_t* const vals = (which ? kv.v : kv.k) + head * VB + (VB / PARTS) * part;
     uint16_t* const scales = KVT == QWA_KV_F16 ? nullptr : (which ? kv.vs : kv.ks) + head * 8;
-    if (which == 0) {
+    const bool do_scales = SU > 0 && part == 0;
+    if (which == 0 && part == PARTS - 1) {
         float* const mass = a.mass + (((size_t)l * a.p.n_seq + seq) * NKV + h) * ((size_t)a.p.ld * a.p.page);
         const float* const src = reinterpret_cast<const float*>(a.work + w.mass) + at;
         for (int r = t; r < keep; r += EV_MT) mass[r] = src[r];
     }
-    auto place = [&](int r) { return table[r / a.p.page] * a.p.page + r % a.p.page; };
-    struct Run {
-        uint4 x[U], sc;
-        int from[U], to[U], sfrom, sto;
+    struct Places {
+        int from[U], to[U], sfrom[SU > 0 ? SU : 1], sto[SU > 0 ? SU : 1];
     };
-    auto load = [&](Run& b, int r0) {
+    struct Values {
+        uint4 x[U], sc[SU > 0 ? SU : 1];
+    };
+    auto look = [&](Places& b, int r0) {  // (equal ones: nothing to move)
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int r = r0 + (t + EV_MT * u) / UNITS;
-            b.from[u] = r < keep ? rows[r] : 0;
-            b.to[u] = r < keep ? place(r) : 0;  // (equal: nothing to move)
+            const int r = min(r0 + (t + EV_MT * u) / UNITS, keep - 1);
+            b.from[u] = rows[r];
+            b.to[u] = (table[r >> sh] << sh) + (r & (a.p.page - 1));
         }
-        if constexpr (KVT != QWA_KV_F16) {
-            b.sfrom = t < ROWS && r0 + t < keep ? rows[r0 + t] : 0;
-            b.sto = t < ROWS && r0 + t < keep ? place(r0 + t) : 0;
-        }
+        if (do_scales)
+#pragma unroll
+            for (int u = 0; u < SU; u++) {
+                const int r = min(r0 + t + EV_MT * u, keep - 1);
+                b.sfrom[u] = rows[r];
+                b.sto[u] = (table[r >> sh] << sh) + (r & (a.p.page - 1));
+            }
+    };
+    // which of the places are the run's
+    auto live = [&](int r0, int u) { return r0 + (t + EV_MT * u) / UNITS < keep; };
+    auto slive = [&](int r0, int u) { return do_scales && t + EV_MT * u < ROWS && r0 + t + EV_MT * u < keep; };
+    auto load = [&](Values& v, const Places& b, int r0) {
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (b.from[u] != b.to[u])
-                b.x[u] = *reinterpret_cast<const uint4*>(vals + (size_t)b.from[u] * VB + 16 * ((t + EV_MT * u) % UNITS));
-        if constexpr (KVT != QWA_KV_F16)
-            if (b.sfrom != b.sto) b.sc = *reinterpret_cast<const uint4*>(scales + (size_t)b.sfrom * 8);
+            if (live(r0, u) && b.from[u] != b.to[u])
+                v.x[u] = *reinterpret_cast<const uint4*>(vals + (size_t)b.from[u] * VB + 16 * ((t + EV_MT * u) % UNITS));
+        if constexpr (SU > 0)
+#pragma unroll
+            for (int u = 0; u < SU; u++)
+                if (slive(r0, u) && b.sfrom[u] != b.sto[u])
+                    v.sc[u] = *reinterpret_cast<const uint4*>(scales + (size_t)b.sfrom[u] * 8);
     };
-    auto store = [&](Run& b) {
+    auto store = [&](Values& v, const Places& b, int r0) {
         // everything of the run is in registers before any of it is written
 #pragma unroll
-        for (int u = 0; u < U; u++) asm volatile("" : "+v"(b.x[u].x), "+v"(b.x[u].y), "+v"(b.x[u].z), "+v"(b.x[u].w));
-        if constexpr (KVT != QWA_KV_F16) asm volatile("" : "+v"(b.sc.x), "+v"(b.sc.y), "+v"(b.sc.z), "+v"(b.sc.w));
+        for (int u = 0; u < U; u++) asm volatile("" : "+v"(v.x[u].x), "+v"(v.x[u].y), "+v"(v.x[u].z), "+v"(v.x[u].w));
+        if constexpr (SU > 0)
+#pragma unroll
+            for (int u = 0; u < SU; u++) asm volatile("" : "+v"(v.sc[u].x), "+v"(v.sc[u].y), "+v"(v.sc[u].z), "+v"(v.sc[u].w));
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (b.from[u] != b.to[u])
-                *reinterpret_cast<uint4*>(vals + (size_t)b.to[u] * VB + 16 * ((t + EV_MT * u) % UNITS)) = b.x[u];
-        if constexpr (KVT != QWA_KV_F16)
-            if (b.sfrom != b.sto) *reinterpret_cast<uint4*>(scales + (size_t)b.sto * 8) = b.sc;
+            if (live(r0, u) && b.from[u] != b.to[u])
+                *reinterpret_cast<uint4*>(vals + (size_t)b.to[u] * VB + 16 * ((t + EV_MT * u) % UNITS)) = v.x[u];
+        if constexpr (SU > 0)
+#pragma unroll
+            for (int u = 0; u < SU; u++)
+                if (slive(r0, u) && b.sfrom[u] != b.sto[u]) *reinterpret_cast<uint4*>(scales + (size_t)b.sto[u] * 8) = v.sc[u];
     };
-    // the next run is read while this one is written: it lies behind all places of this one
-    Run b[2] = {};
-    load(b[0], 0);
+    if (keep == 0) return;
+    // a run is read behind all places of those before it that are still to be written
+    Places p0, p1, p2;
+    Values v0 = {}, v1 = {};
+    look(p0, 0);
+    look(p1, ROWS);
+    load(v0, p0, 0);
     for (int r0 = 0; r0 < keep; r0 += 2 * ROWS) {
-        load(b[1], r0 + ROWS);
-        store(b[0]);
-        load(b[0], r0 + 2 * ROWS);
-        store(b[1]);
+        look(p2, r0 + 2 * ROWS);
+        load(v1, p1, r0 + ROWS);
+        store(v0, p0, r0);
+        p0 = p2;
+        look(p2, r0 + 3 * ROWS);
+        load(v0, p0, r0 + 2 * ROWS);
+        store(v1, p1, r0 + ROWS);
+        p1 = p2;
     }
 }
 
+constexpr int EV_FEW = 256;  // workgroups of whole rows up to which they are cut into parts
 hipError_t launch_pages_evict(const qwa_kv_pages& p, const int* seqs, const int* keep, int n, int recent, int max_keep,
                               const qwa_kv_layer* layers, int n_layers, int kvt, float* mass, int* dropped, int* status,
                               void* work, hipStream_t st) {
     const EvictArgs a{p, seqs, keep, n, n_layers, recent, max_keep, mass, static_cast<int*>(work)};
-    if (n > 0) hipLaunchKernelGGL(k_evict_select, dim3(n_layers * NKV, n), dim3(EV_T), 0, st, a);
+    if (n > 0) hipLaunchKernelGGL(k_evict_select, dim3(n_layers * NKV + 1, n), dim3(EV_T), 0, st, a);
     hipLaunchKernelGGL(k_evict_plan, dim3(1), dim3(EV_T), 0, st, a, dropped, status);
     if (n == 0) return hipGetLastError();
-    const dim3 grid(2 * n_layers * NKV, n);
     const PageLayers pl = page_layers(layers, n_layers);
+    const bool few = n * n_layers * NKV * 2 <= EV_FEW;
+#define QWA_EV(T, P) \
+    hipLaunchKernelGGL((k_evict_move<T, P>), dim3(2 * n_layers * NKV * P, n), dim3(EV_MT), 0, st, a, pl)
     switch (kvt) {
-        case QWA_KV_F16: hipLaunchKernelGGL(k_evict_move<QWA_KV_F16>, grid, dim3(EV_MT), 0, st, a, pl); break;
-        case QWA_KV_Q8_0: hipLaunchKernelGGL(k_evict_move<QWA_KV_Q8_0>, grid, dim3(EV_MT), 0, st, a, pl); break;
-        default: hipLaunchKernelGGL(k_evict_move<QWA_KV_Q4_0>, grid, dim3(EV_MT), 0, st, a, pl); break;
+        case QWA_KV_F16: if (few) QWA_EV(QWA_KV_F16, 4); else QWA_EV(QWA_KV_F16, 1); break;
+        case QWA_KV_Q8_0: if (few) QWA_EV(QWA_KV_Q8_0, 4); else QWA_EV(QWA_KV_Q8_0, 1); break;
+        default: if (few) QWA_EV(QWA_KV_Q4_0, 4); else QWA_EV(QWA_KV_Q4_0, 1); break;
     }
+#undef QWA_EV
     return hipGetLastError();
 }
 

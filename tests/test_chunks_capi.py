@@ -162,7 +162,7 @@ def test_sizes_of_invalid_calls():
         for args in ((0, 9, 100), (1025, 9, 100), (2, 0, 100), (2, 65537, 100), (2, 9, 0), (2, 9, 262145)):
             assert size(*args) == 0
         # a larger call's buffer does for a smaller one
-        assert size(1, 1, 1) <= size(2, 9, 100) <= size(3, 1000, 100) <= size(3, 1000, 5000) <= size(1024, 65536, 262144)
+        assert 0 < size(1, 1, 1) <= size(2, 9, 100) <= size(3, 1000, 5000) <= size(1024, 65536, 262144)
     for args in ((-1, 1, 20), (1025, 1, 20), (2, 0, 20), (2, 33, 20), (2, 1, -1), (2, 1, 262145)):
         assert ops.kv_pages_evict_work_bytes(FakePages(), *args) == 0
 
@@ -200,7 +200,7 @@ int main() {
         CHECK(blocks <= p.blocks && images <= p.images, "%lld blocks, %lld with images: %d, %d\n", blocks, images, p.blocks, p.images);
         CHECK(wblocks <= q.blocks && parts <= q.parts && multi <= q.parts / 2, "weights: %lld blocks, %lld places\n", wblocks, parts);
         CHECK(p.images == 0 || p.tiles >= (most + PF_TILE - 1) / PF_TILE, "room for one sequence\n");
-        CHECK(p.slices >= 1 && p.slices <= CH_SLICES && q.slices >= 1 && q.slices <= CH_SLICES, "slices\n");
+        CHECK(p.whole == (p.slices == 0) && p.slices <= CH_SLICES && q.slices >= 1 && q.slices <= CH_SLICES, "slices\n");
         // tiles fit 32 bits
         CHECK((long long)p.blocks * ((MAX_POS + PF_TILE - 1) / PF_TILE) < 1LL << 31, "tiles\n");
         CHECK(w.o % 16 == 0 && w.ml % 16 == 0 && w.blocks % 16 == 0 && w.list % 16 == 0 && w.head % 16 == 0, "alignment\n");
