@@ -8,8 +8,8 @@
 //    a thousand load the chip alike.  A block that lies in several slices leaves partial states, which k_ch_join joins in the
 //    slices' order; the others are finished where they are.
 //  * A workgroup has two waves a SIMD, with a role each.  The score waves keep Q (32 rows: hi and lo part, 128 registers), bring K
-//    into LDS and leave S^T = K Q^T of tile i there.  The value waves keep O (32 rows, 128 registers), bring V into LDS, take the
-//    exponentials of tile i - 1 and add V^T P^T.  So each fragment of K and V that is read from LDS meets 32 rows, which one wave
+//    into LDS and leave tile i's exponents there: S^T = K Q^T against the rows' references.  The value waves keep O (32 rows, 128
+//    registers), bring V into LDS, take the exponentials of tile i - 1 and add V^T P^T.  So each fragment of K and V that is read from LDS meets 32 rows, which one wave
 //    with both Q and O has no registers for, and one wave's arithmetic runs beside the other's MFMAs.
 //  * Chunks of many blocks would convert each tile once a block: k_ch_image does it for them once, and the waves copy the images into
 //    LDS, two tiles ahead.
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(512) k_ch_image(ChunkArgs a, qwa_kv_layer kv, 
             static_assert(offsetof(ChunkImage, odd) - offsetof(ChunkImage, odd_keys) == offsetof(BtOdd, tile), "BtOdd");
             BtOdd& odd = *reinterpret_cast<BtOdd*>(img.odd_keys);
             if ((t & 63) == 0) odd.tile[wave] = 0;  // (the wave's own, before it may be set)
-            if (t == 0) img.dead = dead;
+            if (t == 0) img.k_dead = dead;
             bt_store_v<KVT>(raw, reinterpret_cast<_Float16*>(img.vt), odd, t, (uint32_t)dead, 1);
         } else {
             const int h = (wave >> 1) & 1;
@@ -348,9 +348,13 @@ struct ChunkLds {
     _Float16 vt[CH_RING][PF_TILE * HD];
     uint16_t scales[CH_RING][PF_TILE * 8];  // of K
     BtOdd odd[2];                           // of V that was not an image
-    int flags[CH_RING][64];                 // of an image: its odd, dead
+    int odd_flags[CH_RING][64];             // of an image: its odd
+    int k_flags[CH_RING][64];               // and k_dead
+    float cr[2][CH_PAIRS][2][16];           // what O is multiplied by before a tile's P V
+    int moved[2][CH_PAIRS];                 // ... if any of it is not 1
+    float m[CH_PAIRS][2][16];               // a finished segment's references
     union {
-        f4 s[2][2][2][64];                  // S^T of a tile: [tile & 1][row tile][half of the keys][lane]
+        f4 s[2][2][2][64];                  // a tile's exponents: [tile & 1][row tile][half of the keys][lane]
         float4 x[16 * HD / 8];              // half of a row tile's O on its way out
     } pair[CH_PAIRS];
     uint2 q[CH_PAIRS][16 * HD / 8];         // half of a row tile's Q, one part, on its way into operands
@@ -522,11 +526,25 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
     const uint8_t* const kh = kv.k + head * value_bytes(KVT);
     const uint16_t* const ksh = SC ? kv.ks + head * 8 : nullptr;
     const ChunkImage* const img = a.images + (size_t)(max(sg.c.place, 0) + sg.tb) * NKV + g;
+    // positions that this lane's rows see, the fewest that one of the wave's does
+    int vis[2], vmin = 0x7fffffff;
+#pragma unroll
+    for (int rt = 0; rt < 2; rt++) {
+        const int r = sg.wrow0 + 16 * rt + (lane & 15);
+        vis[rt] = r < sg.nrows ? sg.c.len - sg.c.count + r / GRP + 1 : 0;
+        if (r < sg.nrows) vmin = min(vmin, vis[rt]);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
+    vmin = __builtin_amdgcn_readfirstlane(vmin);
+    float m[2] = {-INFINITY, -INFINITY};  // the rows' references
+    uint32_t dead = 0;  // halves without a place, two bits a tile from tile i on
     BtRaw<KVT> rk[2];
     ChunkPlaces<2> places;
-    auto load = [&](BtRaw<KVT>& rk, int i) {
+    auto load = [&](BtRaw<KVT>& rk, int i, int ahead) {
         int at[2];
         places.next(at, p, table, sg.tb, sg.c.end, lane);
+        dead |= (uint32_t)((at[0] < 0) | (at[1] < 0) << 1) << (2 * ahead);
         const int h = pair >> 1, left = sg.c.end - (sg.tb + i) * PF_TILE - 16 * h;
         bt_load_k<KVT>(rk, kh, ksh, h ? at[1] : at[0], min(max(left, 0), 16), t);
     };
@@ -535,15 +553,16 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
         const ChunkImage& x = img[(size_t)i * NKV];
         ch_copy(lds.k[slot(i)], x.k, pair, lane);
         if (SC && pair < 2) dma_sv<4>(lds_addr(lds.scales[slot(i)]) + 256 * pair, x.scales, (uint32_t)(256 * pair + 4 * lane));
+        if (pair == 2) dma_sv<4>(lds_addr(lds.k_flags[slot(i)]), &x.k_dead, (uint32_t)(4 * lane));
     };
     auto landed = [&](bool last) {  // all copies (but the last one, if there is another on its way)
         if (last) wait_vmcnt<0>();
-        else if (SC && pair < 2) wait_vmcnt<16 / CH_PAIRS + 1>();
+        else if ((SC && pair < 2) || pair == 2) wait_vmcnt<16 / CH_PAIRS + 1>();
         else wait_vmcnt<16 / CH_PAIRS>();
     };
     if constexpr (!IMG) {
-        load(rk[0], 0);
-        if (sg.nt > 1) load(rk[1], 1);
+        load(rk[0], 0, 0);
+        if (sg.nt > 1) load(rk[1], 1, 1);
     }
     h8 qb[2][2][8];
     ch_load_q<KVT>(qb, a.q, sg.c, sg.wrow0, sg.nrows, g, lds.q[pair], lane);
@@ -554,7 +573,7 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
         landed(sg.nt <= 1);
     } else {
         bt_store_k<KVT>(rk[0], lds.k[slot(0)], lds.scales[slot(0)], t);
-        if (sg.nt > 2) load(rk[0], 2);
+        if (sg.nt > 2) load(rk[0], 2, 2);
     }
     __syncthreads();
     auto step = [&](int i, BtRaw<KVT>& rk) __attribute__((always_inline)) {
@@ -562,7 +581,7 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
             if (i + 2 < sg.nt) copy(i + 2);
         } else {
             if (i + 1 < sg.nt) bt_store_k<KVT>(rk, lds.k[slot(i + 1)], lds.scales[slot(i + 1)], t);
-            if (i + 3 < sg.nt) load(rk, i + 3);
+            if (i + 3 < sg.nt) load(rk, i + 3, 3);
         }
         if (sg.wrow0 < sg.nrows) {
             // (an opaque copy of the lane: the LDS addresses, kept across the tiles, spilled)
@@ -570,11 +589,49 @@ __device__ __forceinline__ void ch_score_walk(ChunkLds<KVT>& lds, const ChunkArg
             asm volatile("" : "+v"(ol));
             f4 sc[2][2];
             ch_scores<KVT>(sc, qb, lds.k[slot(i)], reinterpret_cast<const _Float16*>(lds.scales[slot(i)]), ol & 15, ol >> 4);
+            if constexpr (!SC) {
+                mfma_settle(sc[0][0], sc[0][1]);
+                mfma_settle(sc[1][0], sc[1][1]);
+            }
+            const int k0 = (sg.tb + i) * PF_TILE, b = i & 1;
+            const int gone = IMG ? __builtin_amdgcn_readfirstlane(lds.k_flags[slot(i)][0]) : (int)(dead & 3);
+            if (k0 + PF_TILE > vmin || gone != 0) {
 #pragma unroll
-            for (int rt = 0; rt < 2; rt++)
+                for (int rt = 0; rt < 2; rt++)
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++) lds.pair[pair].s[i & 1][rt][kt][ol] = sc[rt][kt];
+                    for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            sc[rt][kt][e] = k0 + 16 * kt + 4 * (ol >> 4) + e < vis[rt] && !((gone >> kt) & 1) ? sc[rt][kt][e]
+                                                                                                              : -INFINITY;
+            }
+            float cr[2];
+#pragma unroll
+            for (int rt = 0; rt < 2; rt++) {
+                float mx = max3f(max3f(-INFINITY, sc[rt][0][0], sc[rt][0][1]), sc[rt][0][2], sc[rt][0][3]);
+                mx = rows_max(max3f(max3f(mx, sc[rt][1][0], sc[rt][1][1]), sc[rt][1][2], sc[rt][1][3]));
+                const float mx2 = mx * PF_LOG2E, mn = mx2 > m[rt] + BT_HEAD ? mx2 - BT_RAISE : m[rt];
+                cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] - mn);
+                const float ref = mn == -INFINITY ? 0.0f : mn;  // a row that saw nothing keeps l = 0, O = 0
+                m[rt] = mn;
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) {
+                    f4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = fmaf(sc[rt][kt][e], PF_LOG2E, -ref);
+                    lds.pair[pair].s[b][rt][kt][ol] = x;
+                }
+            }
+            const bool any = __any(cr[0] != 1.0f || cr[1] != 1.0f);
+            if (any)
+#pragma unroll
+                for (int rt = 0; rt < 2; rt++) lds.cr[b][pair][rt][ol & 15] = cr[rt];
+            if (ol == 0) lds.moved[b][pair] = any;
+            if (i + 1 == sg.nt)
+#pragma unroll
+                for (int rt = 0; rt < 2; rt++) lds.m[pair][rt][ol & 15] = m[rt];
         }
+        dead >>= 2;
         if constexpr (IMG) landed(i + 2 >= sg.nt);
         __syncthreads();
     };
@@ -601,16 +658,12 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
     const uint16_t* const vsh = SC ? kv.vs + head * 8 : nullptr;
     const ChunkImage* const img = a.images + (size_t)(max(sg.c.place, 0) + sg.tb) * NKV + g;
     const bool rows_here = sg.wrow0 < sg.nrows;
-    int vis[2], vmin = 0x7fffffff;  // positions that this lane's rows see, the fewest that one of the wave's does
+    int vis[2];  // positions that this lane's rows see
 #pragma unroll
     for (int rt = 0; rt < 2; rt++) {
         const int r = sg.wrow0 + 16 * rt + i16;
         vis[rt] = r < sg.nrows ? sg.c.len - sg.c.count + r / GRP + 1 : 0;
-        if (r < sg.nrows) vmin = min(vmin, vis[rt]);
     }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) vmin = min(vmin, __shfl_xor(vmin, o, 64));
-    vmin = __builtin_amdgcn_readfirstlane(vmin);
     BtRaw<KVT> rv[2];
     ChunkPlaces<2> places;
     uint32_t dead = 0;  // halves without a place, two bits a tile: tile i - 1, tile i, ...
@@ -626,7 +679,7 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
     auto copy = [&](int i) {
         const ChunkImage& x = img[(size_t)i * NKV];
         ch_copy(lds.vt[slot(i)], x.vt, pair, lane);
-        if (pair == 0) dma_sv<4>(lds_addr(lds.flags[slot(i)]), x.odd, (uint32_t)(4 * lane));
+        if (pair == 0) dma_sv<4>(lds_addr(lds.odd_flags[slot(i)]), x.odd, (uint32_t)(4 * lane));
     };
     auto landed = [&](bool last) {
         if (last) wait_vmcnt<0>();
@@ -634,10 +687,9 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
         else wait_vmcnt<16 / CH_PAIRS>();
     };
     f4 o[2][16];
-    float m[2], l[2], lx[2];
+    float l[2], lx[2];
 #pragma unroll
     for (int rt = 0; rt < 2; rt++) {
-        m[rt] = -INFINITY;
         l[rt] = lx[rt] = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < 16; dt++) o[rt][dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -664,34 +716,18 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
         }
         if (i > 0 && rows_here) {
             const int b = (i - 1) & 1, k0 = (sg.tb + i - 1) * PF_TILE;
-            int gone = (int)(dead & 3);
-            const int4 odd = *reinterpret_cast<const int4*>(IMG ? lds.flags[slot(i - 1)] : lds.odd[(sg.base + i - 1) & 1].tile);
-            if constexpr (IMG) gone = __builtin_amdgcn_readfirstlane(lds.flags[slot(i - 1)][4]);
             f4 sc[2][2];
 #pragma unroll
             for (int rt = 0; rt < 2; rt++)
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++) sc[rt][kt] = lds.pair[pair].s[b][rt][kt][ol];
-            if (k0 + PF_TILE > vmin || gone != 0) {
+            const int4 odd =
+                *reinterpret_cast<const int4*>(IMG ? lds.odd_flags[slot(i - 1)] : lds.odd[(sg.base + i - 1) & 1].tile);
+            const bool moved = __builtin_amdgcn_readfirstlane(lds.moved[b][pair]) != 0;
+            float cr[2] = {1.0f, 1.0f};
+            if (moved)
 #pragma unroll
-                for (int rt = 0; rt < 2; rt++)
-#pragma unroll
-                    for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            sc[rt][kt][e] =
-                                k0 + 16 * kt + 4 * og + e < vis[rt] && !((gone >> kt) & 1) ? sc[rt][kt][e] : -INFINITY;
-            }
-            float cr[2], ref[2];
-#pragma unroll
-            for (int rt = 0; rt < 2; rt++) {
-                float mx = max3f(max3f(-INFINITY, sc[rt][0][0], sc[rt][0][1]), sc[rt][0][2], sc[rt][0][3]);
-                mx = rows_max(max3f(max3f(mx, sc[rt][1][0], sc[rt][1][1]), sc[rt][1][2], sc[rt][1][3]));
-                const float mx2 = mx * PF_LOG2E, mn = mx2 > m[rt] + BT_HEAD ? mx2 - BT_RAISE : m[rt];
-                cr[rt] = mn == m[rt] ? 1.0f : fast_exp2(m[rt] - mn);
-                ref[rt] = mn == -INFINITY ? 0.0f : mn;  // a row that saw nothing keeps l = 0, O = 0
-                m[rt] = mn;
-            }
+                for (int rt = 0; rt < 2; rt++) cr[rt] = lds.cr[b][pair][rt][oi];
             // the V fragments' reads begin while the exponentials are taken
             const _Float16* vrow = lds.vt[slot(i - 1)] + 8 * (256 * og + oi);
             h8 vf[CH_VD];
@@ -703,7 +739,7 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
                 float rx = 0.0f, rs = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float x = fast_exp2(fmaf(sc[rt][e >> 2][e & 3], PF_LOG2E, -ref[rt]));
+                    const float x = fast_exp2(sc[rt][e >> 2][e & 3]);
                     pb[rt][e] = (_Float16)x;
                     if (LSE) rx += x;
                 }
@@ -714,7 +750,7 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
                 l[rt] = l[rt] * cr[rt] + rs;
                 if (LSE) lx[rt] = lx[rt] * cr[rt] + rx;
             }
-            if (__any(cr[0] != 1.0f || cr[1] != 1.0f)) {
+            if (moved) {
 #pragma unroll
                 for (int rt = 0; rt < 2; rt++)
 #pragma unroll
@@ -738,7 +774,7 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
 #pragma unroll
                     for (int k = 0; k < PF_TILE; k++) {
                         const int cb = k / 4 % 4, h = k / 16;
-                        if (of[cb] == mark && k0 + k < vis[rt] && !((gone >> h) & 1))
+                        if (of[cb] == mark && k0 + k < vis[rt])  // (halves without a place are zeros)
                             seen[rt][cb / 2] |= 1u << (8 * (2 * (cb & 1) + h) + k % 4);
                     }
 #pragma unroll
@@ -788,14 +824,14 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
     if (whole) gates(0);
 #pragma unroll
     for (int rt = 0; rt < 2; rt++) {
-        const float lt = rows_sum(l[rt]), lxt = LSE ? rows_sum(lx[rt]) : 0.0f;
+        const float lt = rows_sum(l[rt]), lxt = LSE ? rows_sum(lx[rt]) : 0.0f, m = lds.m[pair][rt][i16];
         const float il = whole ? (lt == 0.0f ? 0.0f : 1.0f / lt) : 1.0f;
         const int r0 = sg.wrow0 + 16 * rt + i16;
         if (lg == 0 && r0 < sg.nrows) {
-            if (!whole) a.part_ml[part + r0 - CH_ROWS * sg.c.blk] = make_float4(m[rt], lt, lxt, 0.0f);
+            if (!whole) a.part_ml[part + r0 - CH_ROWS * sg.c.blk] = make_float4(m, lt, lxt, 0.0f);
             else if (LSE)
                 a.lse[(size_t)(sg.c.row0 + r0 / GRP) * NH + g * GRP + r0 % GRP] =
-                    lxt == 0.0f ? -INFINITY : (m[rt] + __log2f(lxt)) * 0.6931471805599453f;
+                    lxt == 0.0f ? -INFINITY : (m + __log2f(lxt)) * 0.6931471805599453f;
         }
 #pragma unroll
         for (int e = 0; e < 2; e++) {

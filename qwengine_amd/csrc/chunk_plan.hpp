@@ -27,11 +27,12 @@ constexpr int CH_IMG_TILES = 4096;
 struct ChunkImage {
     uint16_t k[PF_TILE * HD];
     uint16_t scales[PF_TILE * 8];
+    int k_dead;                // halves without a place
+    int k_pad[63];             // (these 256 bytes are copied as one)
     uint16_t vt[PF_TILE * HD];
     uint8_t odd_keys[8 * HD];  // of V values that are not finite
     int odd[4];                // which quarters of them hold any (1)
-    int dead;                  // halves without a place
-    int pad[59];               // (these 256 bytes are copied as one)
+    int pad[60];               // (as are these)
 };
 
 // A chunk's rows are cut into blocks of CH_ROWS; a block walks the PF_TILE-key tiles from the first to the last that one of its
