@@ -11,6 +11,8 @@
 //    into LDS and leave tile i's exponents there: S^T = K Q^T against the rows' references.  The value waves keep O (32 rows, 128
 //    registers), bring V into LDS, take the exponentials of tile i - 1 and add V^T P^T.  So each fragment of K and V that is read from LDS meets 32 rows, which one wave
 //    with both Q and O has no registers for, and one wave's arithmetic runs beside the other's MFMAs.
+//  * Chunks of one or two tokens leave most of a block empty.  Where sequences are cut, they are worked on behind the tiles: a wave
+//    a tile, its bytes straight into registers (paged_walk.hpp).
 //  * Chunks of many blocks would convert each tile once a block: k_ch_image does it for them once, and the waves copy the images into
 //    LDS, two tiles ahead.
 //  * Scores are exact up to fp32 accumulation (K as its codes, Q / 16 as the sum of two fp16 parts), as the batched decode's are;
@@ -23,7 +25,7 @@
 
 #include "chunk_plan.hpp"
 #include "launch.hpp"
-#include "paged_tiles.hpp"
+#include "paged_walk.hpp"
 
 namespace qwa {
 
@@ -43,6 +45,7 @@ struct ChunkSource {
     const int* seqs;
     const int* off;
     int n, rows, max_len;
+    int few;  // chunks of up to so many rows are listed by themselves
 };
 
 struct ChunkArgs {
@@ -54,11 +57,13 @@ struct ChunkArgs {
     float* lse;              // [rows][24] or none
     const ChunkBlock* blocks;
     const int4* list;        // chunks with images: sequence, length, first image, images
-    const int* head;         // numbers of blocks, their tiles, chunks with images, images
+    const int* head;         // numbers of blocks, their tiles, chunks with images, images, chunks of few rows, their steps
     ChunkImage* images;      // [tile][KV head]
     float* part_o;           // [KV head][slice][2][rows][256]
     float4* part_ml;         // [KV head][slice][2][rows]
-    int slices, prows;
+    float* few_o;            // [KV head][slice + chunk of few rows][CH_FEW_ROWS][256]
+    float4* few_ml;
+    int slices, prows, few;
 };
 
 size_t prefill_batch_work_bytes(int n, int rows, int max_len) { return chunk_work(chunk_plan(n, rows, max_len)).bytes; }
@@ -90,7 +95,7 @@ __device__ __forceinline__ int ch_scan(int v, int* s_wave, int* total) {
 // The blocks of all chunks, by one workgroup: thread b has chunk b.  A chunk of rows outside [0, rows], or that begins before an
 // earlier one's end, has none.  For the weights (other sizes of blocks and tiles) only the last chunk of a sequence counts, and
 // chunks of several blocks get places for their sums (list: sequence, length, tokens, first place) instead of images (sequence,
-// length, first image, images).
+// length, first image, images).  The chunks of few rows follow the blocks: their `begin` and `tiles` count steps.
 constexpr int CH_PT = QWA_PAGES_MAXN;
 template <bool WEIGHTS>
 __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, int most_list, int room,
@@ -137,7 +142,8 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
         __syncthreads();
         s_count[t] = count;
     }
-    const int mine = (GRP * count + ROWS - 1) / ROWS;
+    const bool few = !WEIGHTS && count > 0 && GRP * count <= src.few;
+    const int mine = few ? 0 : (GRP * count + ROWS - 1) / ROWS;
     int nb, all, listed, used;
     s_blk[t] = ch_scan<CH_PT>(mine, s_wave, &nb);
     nb = min(nb, most);  // (never more: the chunks' rows are disjoint)
@@ -175,11 +181,26 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
         tiles += all;
         if (j < nb) blocks[j] = x;
     }
+    int n_few = 0, steps = 0;
+    if (!WEIGHTS && src.few > 0) {
+        const int j = ch_scan<CH_PT>(few, s_wave, &n_few);
+        ChunkBlock x = {};
+        x.row0 = first;
+        x.count = count;
+        x.len = x.end = s_len[t];
+        x.seq = s_seq[t];
+        x.tiles = few ? max(1, (x.len + CH_STEP - 1) / CH_STEP) : 0;
+        x.place = -1;
+        x.begin = ch_scan<CH_PT>(x.tiles, s_wave, &steps);
+        if (few && nb + j < most) blocks[nb + j] = x;  // (always)
+    }
     if (t == 0) {
         head[0] = nb;
         head[1] = tiles;
         head[2] = min(listed, most_list);
         head[3] = used;
+        head[4] = n_few;
+        head[5] = steps;
     }
 }
 
@@ -187,7 +208,7 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
 struct OwnPlan {
     ChunkBlock blocks[CH_OWN];
     int4 list[CH_OWN];
-    int head[4];
+    int head[6];
 };
 template <bool WEIGHTS>
 __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& src) {
@@ -229,7 +250,8 @@ __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& sr
             }
         }
         const int len = known && count > 0 ? min(max(all, 0), src.max_len) : 0;
-        const int mine = (GRP * count + ROWS - 1) / ROWS, blk0 = before(mine);
+        const bool few = !WEIGHTS && count > 0 && GRP * count <= src.few;
+        const int mine = few ? 0 : (GRP * count + ROWS - 1) / ROWS, blk0 = before(mine);
         const int want = WEIGHTS && mine > 1 ? mine : 0, place = before(want), entry = before(want > 0);
         if (want > 0) plan.list[entry] = make_int4(seq, len, count, place);
         const int nb = min(__builtin_amdgcn_readlane(blk0 + mine, 63), CH_OWN);
@@ -251,11 +273,28 @@ __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& sr
         x.place = many > 0 ? pl + x.blk : -1;
         x.begin = before(x.tiles);
         if (t < nb) plan.blocks[t] = x;
+        int n_few = 0, steps = 0;
+        if (!WEIGHTS && src.few > 0) {
+            const int j = before(few);
+            ChunkBlock y = {};
+            y.row0 = first;
+            y.count = count;
+            y.len = y.end = len;
+            y.seq = seq;
+            y.tiles = few ? max(1, (len + CH_STEP - 1) / CH_STEP) : 0;
+            y.place = -1;
+            y.begin = before(y.tiles);
+            if (few && nb + j < CH_OWN) plan.blocks[nb + j] = y;  // (always)
+            n_few = j + few;
+            steps = y.begin + y.tiles;
+        }
         if (t == 63) {
             plan.head[0] = nb;
             plan.head[1] = x.begin + x.tiles;
             plan.head[2] = entry + (want > 0);
             plan.head[3] = 0;
+            plan.head[4] = n_few;
+            plan.head[5] = steps;
         }
     }
     __syncthreads();
@@ -358,8 +397,6 @@ struct ChunkLds {
         float4 x[16 * HD / 8];              // half of a row tile's O on its way out
     } pair[CH_PAIRS];
     uint2 q[CH_PAIRS][16 * HD / 8];         // half of a row tile's Q, one part, on its way into operands
-    int found;
-    OwnPlan plan;
 };
 
 // A segment: the tiles [tb, tb + nt) of a block that a workgroup walks.
@@ -873,10 +910,41 @@ __device__ __forceinline__ void ch_value_walk(ChunkLds<KVT>& lds, const ChunkArg
     }
 }
 
+// a chunk of few rows, for bt_walk: its state goes to place `rec` on
+struct FewSegment : BtRange {
+    int first, count, len;
+    size_t rec;
+};
+template <bool LSE>
+struct FewRows {
+    static constexpr int WAVES = 2 * CH_PAIRS;
+    static constexpr bool SUM = LSE;
+    using SEGMENT = FewSegment;
+    const ChunkArgs& a;
+    __device__ __forceinline__ int seen(const SEGMENT& s, int tok) const { return s.len - s.count + tok + 1; }
+    __device__ __forceinline__ const float* q(const SEGMENT& s, int tok) const { return a.q + (size_t)(s.first + tok) * NH * HD; }
+    __device__ __forceinline__ size_t place(const SEGMENT& s, int r) const { return s.rec + r; }
+    __device__ __forceinline__ void sums(const SEGMENT&, size_t place, float m, float l, float x) const {
+        a.few_ml[place] = make_float4(m, l, x, 0.0f);
+    }
+    __device__ __forceinline__ float* o(const SEGMENT&, size_t place) const { return a.few_o + place * HD; }
+};
+
+template <int KVT, bool LSE>
+struct ChunkShared {
+    union {
+        ChunkLds<KVT> tiles;
+        BtLds<KVT, 1, FewRows<LSE>::WAVES, LSE> walk;
+    };
+    int found;
+    OwnPlan plan;
+};
+
 template <int KVT, bool LSE>
 __global__ void __launch_bounds__(128 * CH_PAIRS) __attribute__((amdgpu_waves_per_eu(2, 2)))
 k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
-    __shared__ __attribute__((aligned(16))) ChunkLds<KVT> lds;
+    __shared__ __attribute__((aligned(16))) ChunkShared<KVT, LSE> shared;
+    ChunkLds<KVT>& lds = shared.tiles;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int pair = wave & (CH_PAIRS - 1);
     // workgroups 8 apart run on one XCD: each has consecutive slices of one head, whose tiles its L2 then holds
@@ -885,27 +953,24 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     const ChunkBlock* blocks = a.blocks;
     const int* head = a.head;
     if (a.own) {
-        ch_own_plan<false>(lds.plan, a.src);
-        blocks = lds.plan.blocks;
-        head = lds.plan.head;
+        ch_own_plan<false>(shared.plan, a.src);
+        blocks = shared.plan.blocks;
+        head = shared.plan.head;
     }
     const int nb = __builtin_amdgcn_readfirstlane(head[0]), tiles = __builtin_amdgcn_readfirstlane(head[1]);
     // a slice, or a block as a whole
     const int per = a.slices > 0 ? a.slices : (int)gridDim.x / NKV, g = unit / per, w = unit % per;
-    int s, s_end, j;
+    int s = 0, s_end = 0, j = w;
     if (threadIdx.x < 8) lds.odd[threadIdx.x >> 2].tile[threadIdx.x & 3] = -1;
-    if (a.slices > 0) {
-        const int slices = ch_slices(a.slices, tiles);
-        if (w >= slices) return;
-        s = ch_cut(w, tiles, slices);
-        s_end = ch_cut(w + 1, tiles, slices);
-        j = ch_find(blocks, nb, s, &lds.found);
-    } else {
+    if (a.slices == 0) {
         if (w >= nb) return;
-        j = w;
         s = __builtin_amdgcn_readfirstlane(blocks[j].begin);
         s_end = s + __builtin_amdgcn_readfirstlane(blocks[j].tiles);
         __syncthreads();
+    } else if (const int slices = ch_slices(a.slices, tiles); w < slices) {
+        s = ch_cut(w, tiles, slices);
+        s_end = ch_cut(w + 1, tiles, slices);
+        j = ch_find(blocks, nb, s, &shared.found);
     }
     const int s_begin = s;
     // The segments; the roles meet at a segment's barriers, one and one a tile.  Behind the last one the score waves go on to the
@@ -933,13 +998,74 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         s += sg.nt;
         j++;
     }
+    const int n_few = a.few > 0 ? __builtin_amdgcn_readfirstlane(head[4]) : 0;
+    if (n_few == 0) return;
+    // the chunks of few rows
+    const int steps = __builtin_amdgcn_readfirstlane(head[5]), slices = ch_slices(a.slices, steps);
+    if (w >= slices) return;
+    s = ch_cut(w, steps, slices);
+    s_end = ch_cut(w + 1, steps, slices);
+    __syncthreads();  // (of the tiles' LDS nothing is read any more)
+    j = ch_find(blocks + nb, n_few, s, &shared.found);
+    auto segment = [&] {
+        const ChunkBlock c = ch_block(blocks[nb + j]);
+        const int k0 = (s - c.begin) * CH_STEP, stop = min(s_end, c.begin + c.tiles);
+        const FewSegment x = {{p.table + (size_t)max(c.seq, 0) * p.ld, 0, GRP * c.count, k0, min((stop - c.begin) * CH_STEP, c.end), 0},
+                              c.row0, c.count, c.len, ((size_t)g * (a.slices + a.few) + w + j) * CH_FEW_ROWS};
+        s = stop;
+        return x;
+    };
+    bt_walk<KVT, 1>(shared.walk, FewRows<LSE>{a}, kv, p, g, segment(), [&](FewSegment& seg) {
+        if (s >= s_end) return false;
+        j++;
+        seg = segment();
+        return true;
+    });
 }
 
-// Joins the states of the blocks that lie in several slices, in the slices' order: workgroup (cut between two slices, KV head,
-// part of the rows) has the block that the cut lies in, if it is the first cut in it; a wave a row, 4 dims a lane.
+// A row's output from its states of slices w0 .. w1, in that order: 4 dims a lane.
+template <bool LSE, class PLACE>
+__device__ __forceinline__ void ch_join_row(const ChunkArgs& a, const float* o, const float4* sums, size_t out, int w0, int w1,
+                                            int lane, PLACE place) {
+    const float4 gv = *reinterpret_cast<const float4*>(a.gate + out * HD + 4 * lane);
+    float M = -INFINITY, L = 0.0f, X = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int w = w0; w <= w1; w += 4) {
+        float4 ml[4], x[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const size_t at = place(min(w + u, w1));
+            ml[u] = sums[at];
+            x[u] = *reinterpret_cast<const float4*>(o + at * HD + 4 * lane);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (w + u > w1) break;
+            const float Mn = fmaxf(M, ml[u].x);
+            const float f0 = M == Mn ? 1.0f : fast_exp2(M - Mn);
+            // a state that saw nothing weighs nothing; one of NaN scores (l is NaN) makes the row NaN
+            const float f = ml[u].y == 0.0f ? 0.0f : fast_exp2(ml[u].x - Mn);
+            M = Mn;
+            L = fmaf(L, f0, f * ml[u].y);
+            if (LSE) X = fmaf(X, f0, f * ml[u].z);
+            acc.x = fmaf(acc.x, f0, f * x[u].x);
+            acc.y = fmaf(acc.y, f0, f * x[u].y);
+            acc.z = fmaf(acc.z, f0, f * x[u].z);
+            acc.w = fmaf(acc.w, f0, f * x[u].w);
+        }
+    }
+    const float il = L == 0.0f ? 0.0f : 1.0f / L;
+    *reinterpret_cast<uint2*>(a.out16 + out * HD + 4 * lane) =
+        ch_gated(make_float4(acc.x * il, acc.y * il, acc.z * il, acc.w * il), gv);
+    if (LSE && lane == 0) a.lse[out] = X == 0.0f ? -INFINITY : (M + __log2f(X)) * 0.6931471805599453f;
+}
+
+// Joins the states of the blocks that lie in several slices, in the slices' order: workgroup (cut between two slices, part of the
+// rows; KV head) has the block that the cut lies in, if it is the first cut in it; a wave a row.  The workgroups behind those have
+// a chunk of few rows each.
 constexpr int CH_JR = 16;  // rows of a workgroup
 template <bool LSE>
-__global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a) {
+__global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a, int parts) {
     __shared__ int found;
     __shared__ OwnPlan plan;
     const ChunkBlock* blocks = a.blocks;
@@ -949,56 +1075,37 @@ __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a) {
         blocks = plan.blocks;
         head = plan.head;
     }
+    const int g = blockIdx.y, cut = blockIdx.x / parts + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (cut >= a.slices) {
+        const int j = (int)blockIdx.x - (a.slices - 1) * parts;
+        if (j >= head[4]) return;
+        const ChunkBlock c = blocks[head[0] + j];
+        const int steps = head[5], slices = ch_slices(a.slices, steps);
+        auto slice = [&](int s) { return (int)(((long long)(s + 1) * slices - 1) / steps); };  // that holds step s
+        const int w0 = slice(c.begin), w1 = slice(c.begin + c.tiles - 1);
+        const size_t rec = (size_t)g * (a.slices + a.few) + j;
+        for (int r = wave; r < GRP * c.count; r += 4)
+            ch_join_row<LSE>(a, a.few_o, a.few_ml, (size_t)(c.row0 + r / GRP) * NH + g * GRP + r % GRP, w0, w1, lane,
+                             [&](int w) { return (rec + w) * CH_FEW_ROWS + r; });
+        return;
+    }
     const int tiles = head[1], slices = ch_slices(a.slices, tiles);
-    const int g = blockIdx.y, cut = blockIdx.x + 1;
     if (cut >= slices) return;
     const int s = ch_cut(cut, tiles, slices), s_before = ch_cut(cut - 1, tiles, slices);
     const int j = ch_find(blocks, head[0], s, &found);
     const ChunkBlock c = blocks[j];
     if (c.begin == s || c.begin < s_before) return;  // the cut lies between two blocks, or an earlier one lies in this
     // its slices: cut - 1 up to the one that holds its last tile
-    const int last = c.begin + c.tiles - 1;
+    const int last = c.begin + c.tiles - 1, part = blockIdx.x % parts;
     int w1 = cut;
     while (w1 + 1 < slices && ch_cut(w1 + 1, tiles, slices) <= last) w1++;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    auto place = [&](int w) {
-        return (((size_t)g * a.slices + w) * 2 + (w == cut - 1 && c.begin != s_before ? 1 : 0)) * a.prows;
-    };
-    for (int r = CH_JR * blockIdx.z + wave; r < CH_JR * ((int)blockIdx.z + 1); r += 4) {
+    for (int r = CH_JR * part + wave; r < CH_JR * (part + 1); r += 4) {
         const int row = CH_ROWS * c.blk + r;
         if (row >= GRP * c.count) return;
-        const size_t out = (size_t)(c.row0 + row / GRP) * NH + g * GRP + row % GRP;
-        const float4 gv = *reinterpret_cast<const float4*>(a.gate + out * HD + 4 * lane);
-        float M = -INFINITY, L = 0.0f, X = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int w0 = cut - 1; w0 <= w1; w0 += 4) {
-            float4 ml[4], x[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const size_t at = place(min(w0 + u, w1)) + r;
-                ml[u] = a.part_ml[at];
-                x[u] = *reinterpret_cast<const float4*>(a.part_o + at * HD + 4 * lane);
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                if (w0 + u > w1) break;
-                const float Mn = fmaxf(M, ml[u].x);
-                const float f0 = M == Mn ? 1.0f : fast_exp2(M - Mn);
-                // a state that saw nothing weighs nothing; one of NaN scores (l is NaN) makes the row NaN
-                const float f = ml[u].y == 0.0f ? 0.0f : fast_exp2(ml[u].x - Mn);
-                M = Mn;
-                L = fmaf(L, f0, f * ml[u].y);
-                if (LSE) X = fmaf(X, f0, f * ml[u].z);
-                acc.x = fmaf(acc.x, f0, f * x[u].x);
-                acc.y = fmaf(acc.y, f0, f * x[u].y);
-                acc.z = fmaf(acc.z, f0, f * x[u].z);
-                acc.w = fmaf(acc.w, f0, f * x[u].w);
-            }
-        }
-        const float il = L == 0.0f ? 0.0f : 1.0f / L;
-        *reinterpret_cast<uint2*>(a.out16 + out * HD + 4 * lane) =
-            ch_gated(make_float4(acc.x * il, acc.y * il, acc.z * il, acc.w * il), gv);
-        if (LSE && lane == 0) a.lse[out] = X == 0.0f ? -INFINITY : (M + __log2f(X)) * 0.6931471805599453f;
+        ch_join_row<LSE>(a, a.part_o, a.part_ml, (size_t)(c.row0 + row / GRP) * NH + g * GRP + row % GRP, cut - 1, w1, lane,
+                         [&](int w) {
+                             return (((size_t)g * a.slices + w) * 2 + (w == cut - 1 && c.begin != s_before ? 1 : 0)) * a.prows + r;
+                         });
     }
 }
 
@@ -1011,9 +1118,11 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
     ChunkBlock* blocks = reinterpret_cast<ChunkBlock*>(base + w.blocks);
     int* head = reinterpret_cast<int*>(base + w.head);
     int4* list = reinterpret_cast<int4*>(base + w.list);
-    const ChunkSource src{p, seqs, off, n, rows, max_len};
+    const ChunkSource src{p, seqs, off, n, rows, max_len, pl.few > 0 ? CH_FEW : 0};
     const ChunkArgs a{src, pl.own, q, gate, out16, lse, blocks, list, head, reinterpret_cast<ChunkImage*>(base + w.images),
-                      reinterpret_cast<float*>(base + w.o), reinterpret_cast<float4*>(base + w.ml), pl.slices, pl.rows};
+                      reinterpret_cast<float*>(base + w.o), reinterpret_cast<float4*>(base + w.ml),
+                      reinterpret_cast<float*>(base + w.few_o), reinterpret_cast<float4*>(base + w.few_ml), pl.slices, pl.rows,
+                      pl.few};
     if (!pl.own)
         hipLaunchKernelGGL(k_ch_plan<false>, dim3(1), dim3(CH_PT), 0, st, src, pl.blocks, pl.images, pl.tiles, blocks, list, head);
     if (pl.tiles > 0) {
@@ -1036,10 +1145,11 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
         default: QWA_CH(QWA_KV_Q4_0);
     }
 #undef QWA_CH
-    if (pl.slices > 1) {
-        const dim3 jg(pl.slices - 1, NKV, (pl.rows + CH_JR - 1) / CH_JR);
-        if (lse) hipLaunchKernelGGL(k_ch_join<true>, jg, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(k_ch_join<false>, jg, dim3(256), 0, st, a);
+    if (pl.slices > 1 || pl.few > 0) {
+        const int parts = (pl.rows + CH_JR - 1) / CH_JR;
+        const dim3 jg((pl.slices - 1) * parts + pl.few, NKV);
+        if (lse) hipLaunchKernelGGL(k_ch_join<true>, jg, dim3(256), 0, st, a, parts);
+        else hipLaunchKernelGGL(k_ch_join<false>, jg, dim3(256), 0, st, a, parts);
     }
     return hipGetLastError();
 }
@@ -1254,7 +1364,7 @@ hipError_t launch_weights_batch(const float* q, const float* lse, const qwa_kv_l
     ChunkBlock* blocks = reinterpret_cast<ChunkBlock*>(base + w.blocks);
     int4* list = reinterpret_cast<int4*>(base + w.list);
     int* head = reinterpret_cast<int*>(base + w.head);
-    const ChunkSource src{p, seqs, off, n, rows, max_len};
+    const ChunkSource src{p, seqs, off, n, rows, max_len, 0};
     const WeightsArgs a{src, pl.own, q, lse, mass, blocks, list, head, reinterpret_cast<float*>(base + w.parts), pl.slices, max_len};
     if (!pl.own)
         hipLaunchKernelGGL(k_ch_plan<true>, dim3(1), dim3(CH_PT), 0, st, src, pl.blocks, pl.parts / 2, pl.parts, blocks, list, head);

@@ -47,8 +47,12 @@ constexpr int CH_OWN = 64;
 #define QWA_CH_WHOLE 512
 #endif
 constexpr int CH_WHOLE = QWA_CH_WHOLE;
+// Chunks of up to CH_FEW rows (one or two tokens) are no blocks where slices are cut: their keys' steps of CH_STEP positions in a
+// row, cut into as many equal slices, follow a workgroup's tiles, and are walked by its waves a tile each (paged_walk.hpp): 499
+// tokens and 23 decoded ones over 8192 Q4_0 positions 230 us, as blocks 317, of which a decoded token filled a twentieth.
+constexpr int CH_FEW = 16, CH_FEW_ROWS = CH_FEW / GRP * GRP, CH_STEP = 256;
 struct ChunkPlan {
-    int blocks, slices, rows, images, tiles;
+    int blocks, slices, rows, images, tiles, few;  // few: chunks that may be of so few rows
     bool whole, own;
 };
 
@@ -63,15 +67,17 @@ inline ChunkPlan chunk_plan(int n, int rows, int max_len) {
     // (a chunk of CH_IMG_BLOCKS blocks has more than CH_IMG_BLOCKS - 1 full ones)
     p.images = std::min(n, (int)((long long)GRP * rows / (CH_ROWS * (CH_IMG_BLOCKS - 1))));
     p.tiles = (int)std::min<long long>((long long)p.images * most, std::max(most, CH_IMG_TILES));
+    p.few = p.whole || CH_FEW_ROWS == 0 ? 0 : std::min(n, rows);
     p.own = n <= CH_OWN && p.blocks <= CH_OWN && p.images == 0;
     return p;
 }
 
 // Work buffer: the blocks' descriptions, the list of chunks with images, the numbers of blocks, their tiles, chunks with images
 // and those tiles; the images; the partial states of the blocks that lie in several slices, two places a slice (its first block,
-// if it began in an earlier one, and its last one): O as fp32 [256] and (m, l, sum for the log) a row.
+// if it began in an earlier one, and its last one): O as fp32 [256] and (m, l, sum for the log) a row; the same of the chunks of few
+// rows, a place for each pair of a slice and a chunk that meet (slice + number of the chunk).
 struct ChunkWork {
-    size_t images, o, ml, blocks, list, head, bytes;  // byte offsets
+    size_t images, o, ml, few_o, few_ml, blocks, list, head, bytes;  // byte offsets
 };
 constexpr size_t CH_BLOCK_BYTES = 48;
 inline ChunkWork chunk_work(const ChunkPlan& p) {
@@ -80,10 +86,13 @@ inline ChunkWork chunk_work(const ChunkPlan& p) {
     w.images = 0;
     w.o = w.images + (size_t)NKV * p.tiles * sizeof(ChunkImage);
     w.ml = w.o + parts * HD * 4;
-    w.blocks = w.ml + parts * 16;
+    w.few_o = w.ml + parts * 16;
+    const size_t few = p.few > 0 ? (size_t)NKV * (p.slices + p.few) * CH_FEW_ROWS : 0;
+    w.few_ml = w.few_o + few * HD * 4;
+    w.blocks = w.few_ml + few * 16;
     w.list = w.blocks + p.blocks * CH_BLOCK_BYTES;
     w.head = w.list + p.images * 16;
-    w.bytes = w.head + 16;
+    w.bytes = w.head + 32;
     return w;
 }
 
@@ -113,7 +122,7 @@ inline WeightsWork weights_work(const WeightsPlan& p, int max_len) {
     w.blocks = w.parts + ((size_t)p.parts * NKV * max_len * 4 + 15) / 16 * 16;
     w.list = w.blocks + p.blocks * CH_BLOCK_BYTES;
     w.head = w.list + (size_t)(p.parts / 2) * 16;
-    w.bytes = w.head + 16;
+    w.bytes = w.head + 32;
     return w;
 }
 
