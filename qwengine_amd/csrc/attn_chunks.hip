@@ -30,7 +30,7 @@
 namespace qwa {
 
 // a block: its chunk's first row and number of tokens, the sequence's length and number (< 0: unknown, len 0), the block's number in
-// the chunk, its first tile in the row of all tiles, its tiles, the positions that its last row sees, the chunk's first image, or the
+// the chunk, its place in the row of all tiles (for the attention CH_EXTRA before its first tile), its tiles, the positions that its last row sees, the chunk's first image, or the
 // block's place for its sums (-1: none)
 struct alignas(16) ChunkBlock {
     int row0, count, len, seq;
@@ -177,7 +177,8 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
             x.tiles = max(1, (x.end + TILE - 1) / TILE);  // (rows that see nothing are written too)
             x.place = s_place[lo] < 0 ? -1 : s_place[lo] + (WEIGHTS ? x.blk : 0);
         }
-        x.begin = tiles + ch_scan<CH_PT>(x.tiles, s_wave, &all);
+        const int takes = WEIGHTS || j >= nb ? x.tiles : x.tiles + CH_EXTRA;
+        x.begin = tiles + ch_scan<CH_PT>(takes, s_wave, &all);
         tiles += all;
         if (j < nb) blocks[j] = x;
     }
@@ -271,7 +272,8 @@ __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& sr
         x.tiles = t < nb ? max(1, (x.end + TILE - 1) / TILE) : 0;
         const int pl = __shfl(place, lo, 64), many = __shfl(want, lo, 64);
         x.place = many > 0 ? pl + x.blk : -1;
-        x.begin = before(x.tiles);
+        const int takes = WEIGHTS || t >= nb ? x.tiles : x.tiles + CH_EXTRA;
+        x.begin = before(takes);
         if (t < nb) plan.blocks[t] = x;
         int n_few = 0, steps = 0;
         if (!WEIGHTS && src.few > 0) {
@@ -290,7 +292,7 @@ __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& sr
         }
         if (t == 63) {
             plan.head[0] = nb;
-            plan.head[1] = x.begin + x.tiles;
+            plan.head[1] = x.begin + takes;
             plan.head[2] = entry + (want > 0);
             plan.head[3] = 0;
             plan.head[4] = n_few;
@@ -304,11 +306,12 @@ __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& sr
 __device__ __forceinline__ int ch_slices(int slices, int tiles) { return min(slices, tiles); }
 __device__ __forceinline__ int ch_cut(int w, int tiles, int slices) { return (int)((long long)w * tiles / slices); }
 
-// the block that holds tile s, found by the whole workgroup
+// the block that holds place s, found by the whole workgroup
+template <int EXTRA>
 __device__ __forceinline__ int ch_find(const ChunkBlock* blocks, int nb, int s, int* s_found) {
     for (int j = threadIdx.x; j < nb; j += blockDim.x) {
         const int begin = blocks[j].begin;
-        if (begin <= s && s < begin + blocks[j].tiles) *s_found = j;
+        if (begin <= s && s < begin + EXTRA + blocks[j].tiles) *s_found = j;
     }
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(*s_found);
@@ -965,14 +968,15 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     if (a.slices == 0) {
         if (w >= nb) return;
         s = __builtin_amdgcn_readfirstlane(blocks[j].begin);
-        s_end = s + __builtin_amdgcn_readfirstlane(blocks[j].tiles);
+        s_end = s + CH_EXTRA + __builtin_amdgcn_readfirstlane(blocks[j].tiles);
         __syncthreads();
     } else if (const int slices = ch_slices(a.slices, tiles); w < slices) {
         s = ch_cut(w, tiles, slices);
         s_end = ch_cut(w + 1, tiles, slices);
-        j = ch_find(blocks, nb, s, &shared.found);
+        j = ch_find<CH_EXTRA>(blocks, nb, s, &shared.found);
     }
     const int s_begin = s;
+    int walked = 0;
     // The segments; the roles meet at a segment's barriers, one and one a tile.  Behind the last one the score waves go on to the
     // next segment's Q and K while the value waves finish: what these still read there (V and flags of the last tile, its
     // scores, which the pair's own O follows) is written by nobody before the next barrier.
@@ -982,12 +986,17 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         asm volatile("" : "+v"(t));
         ChunkSegment sg;
         sg.c = ch_block(blocks[j]);
-        sg.base = s - s_begin;
-        sg.tb = s - sg.c.begin;
-        sg.nt = min(s_end, sg.c.begin + sg.c.tiles) - s;
+        const int first = sg.c.begin + CH_EXTRA, stop = min(s_end, first + sg.c.tiles), from = s;
+        s = stop;
+        j++;
+        sg.base = walked;
+        sg.tb = max(from - first, 0);
+        sg.nt = stop - first - sg.tb;
+        if (sg.nt <= 0) continue;  // (the slice ends before the block's first tile)
+        walked += sg.nt;
         sg.nrows = GRP * sg.c.count;
         sg.wrow0 = CH_ROWS * sg.c.blk + 32 * pair;
-        const size_t part = (((size_t)g * a.slices + w) * 2 + (s == s_begin ? 0 : 1)) * a.prows;
+        const size_t part = (((size_t)g * a.slices + w) * 2 + (from == s_begin ? 0 : 1)) * a.prows;
         if (wave < CH_PAIRS) {
             if (sg.c.place >= 0) ch_score_walk<KVT, true>(lds, a, kv, p, sg, g, pair, t);
             else ch_score_walk<KVT, false>(lds, a, kv, p, sg, g, pair, t);
@@ -995,8 +1004,6 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
             if (sg.c.place >= 0) ch_value_walk<KVT, true, LSE>(lds, a, kv, p, sg, g, pair, part, t);
             else ch_value_walk<KVT, false, LSE>(lds, a, kv, p, sg, g, pair, part, t);
         }
-        s += sg.nt;
-        j++;
     }
     const int n_few = a.few > 0 ? __builtin_amdgcn_readfirstlane(head[4]) : 0;
     if (n_few == 0) return;
@@ -1006,7 +1013,7 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     s = ch_cut(w, steps, slices);
     s_end = ch_cut(w + 1, steps, slices);
     __syncthreads();  // (of the tiles' LDS nothing is read any more)
-    j = ch_find(blocks + nb, n_few, s, &shared.found);
+    j = ch_find<0>(blocks + nb, n_few, s, &shared.found);
     auto segment = [&] {
         const ChunkBlock c = ch_block(blocks[nb + j]);
         const int k0 = (s - c.begin) * CH_STEP, stop = min(s_end, c.begin + c.tiles);
@@ -1092,11 +1099,13 @@ __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a, int parts) {
     const int tiles = head[1], slices = ch_slices(a.slices, tiles);
     if (cut >= slices) return;
     const int s = ch_cut(cut, tiles, slices), s_before = ch_cut(cut - 1, tiles, slices);
-    const int j = ch_find(blocks, head[0], s, &found);
+    const int j = ch_find<CH_EXTRA>(blocks, head[0], s, &found);
     const ChunkBlock c = blocks[j];
-    if (c.begin == s || c.begin < s_before) return;  // the cut lies between two blocks, or an earlier one lies in this
+    // the cut lies before the block's first tile, or an earlier one lies behind that
+    const int first = c.begin + CH_EXTRA;
+    if (s <= first || s_before > first) return;
     // its slices: cut - 1 up to the one that holds its last tile
-    const int last = c.begin + c.tiles - 1, part = blockIdx.x % parts;
+    const int last = first + c.tiles - 1, part = blockIdx.x % parts;
     int w1 = cut;
     while (w1 + 1 < slices && ch_cut(w1 + 1, tiles, slices) <= last) w1++;
     for (int r = CH_JR * part + wave; r < CH_JR * (part + 1); r += 4) {
@@ -1104,7 +1113,7 @@ __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a, int parts) {
         if (row >= GRP * c.count) return;
         ch_join_row<LSE>(a, a.part_o, a.part_ml, (size_t)(c.row0 + row / GRP) * NH + g * GRP + row % GRP, cut - 1, w1, lane,
                          [&](int w) {
-                             return (((size_t)g * a.slices + w) * 2 + (w == cut - 1 && c.begin != s_before ? 1 : 0)) * a.prows + r;
+                             return (((size_t)g * a.slices + w) * 2 + (w == cut - 1 && c.begin > s_before ? 1 : 0)) * a.prows + r;
                          });
     }
 }
@@ -1209,7 +1218,7 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     if (w >= slices) return;
     int s = ch_cut(w, tiles, slices);
     const int s_end = ch_cut(w + 1, tiles, slices);
-    int j = ch_find(blocks, nb, s, &lds.found);
+    int j = ch_find<0>(blocks, nb, s, &lds.found);
     const size_t head = (size_t)g * kv.capacity;
     const uint8_t* const kh = kv.k + head * value_bytes(KVT);
     const uint16_t* const ksh = SC ? kv.ks + head * 8 : nullptr;

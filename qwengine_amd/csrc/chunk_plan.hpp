@@ -51,6 +51,11 @@ constexpr int CH_WHOLE = QWA_CH_WHOLE;
 // row, cut into as many equal slices, follow a workgroup's tiles, and are walked by its waves a tile each (paged_walk.hpp): 499
 // tokens and 23 decoded ones over 8192 Q4_0 positions 230 us, as blocks 317, of which a decoded token filled a twentieth.
 constexpr int CH_FEW = 16, CH_FEW_ROWS = CH_FEW / GRP * GRP, CH_STEP = 256;
+// What a block takes besides its tiles (Q's way into registers, O's way out), in tiles: the slices are cut from rows of both.
+#ifndef QWA_CH_EXTRA
+#define QWA_CH_EXTRA 8
+#endif
+constexpr int CH_EXTRA = QWA_CH_EXTRA;
 struct ChunkPlan {
     int blocks, slices, rows, images, tiles, few;  // few: chunks that may be of so few rows
     bool whole, own;
@@ -62,7 +67,7 @@ inline ChunkPlan chunk_plan(int n, int rows, int max_len) {
     // (a chunk has one partly filled block)
     p.blocks = (int)std::min<long long>((long long)GRP * rows, (long long)GRP * rows / CH_ROWS + n);
     p.whole = max_len <= CH_WHOLE;
-    p.slices = p.whole ? 0 : (int)std::min<long long>(CH_SLICES, (long long)p.blocks * most);
+    p.slices = p.whole ? 0 : (int)std::min<long long>(CH_SLICES, (long long)p.blocks * (most + CH_EXTRA));
     p.rows = std::min(CH_ROWS, GRP * rows);
     // (a chunk of CH_IMG_BLOCKS blocks has more than CH_IMG_BLOCKS - 1 full ones)
     p.images = std::min(n, (int)((long long)GRP * rows / (CH_ROWS * (CH_IMG_BLOCKS - 1))));
