@@ -30,7 +30,7 @@
 namespace qwa {
 
 // a block: its chunk's first row and number of tokens, the sequence's length and number (< 0: unknown, len 0), the block's number in
-// the chunk, its place in the row of all tiles (for the attention CH_EXTRA before its first tile), its tiles, the positions that its last row sees, the chunk's first image, or the
+// the chunk, its first tile in the row of all tiles, its tiles, the positions that its last row sees, the chunk's first image, or the
 // block's place for its sums (-1: none)
 struct alignas(16) ChunkBlock {
     int row0, count, len, seq;
@@ -55,9 +55,9 @@ struct ChunkArgs {
     const float* gate;
     uint16_t* out16;
     float* lse;              // [rows][24] or none
-    const ChunkBlock* blocks;
+    ChunkBlock* blocks;
     const int4* list;        // chunks with images: sequence, length, first image, images
-    const int* head;         // numbers of blocks, their tiles, chunks with images, images, chunks of few rows, their steps
+    int* head;               // numbers of blocks, their tiles, chunks with images, images, chunks of few rows, their steps, the longest block
     ChunkImage* images;      // [tile][KV head]
     float* part_o;           // [KV head][slice][2][rows][256]
     float4* part_ml;         // [KV head][slice][2][rows]
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
     s_place[t] = has && entry < most_list ? place : -1;
     if (s_place[t] >= 0) list[entry] = WEIGHTS ? make_int4(s_seq[t], s_len[t], count, place) : make_int4(s_seq[t], s_len[t], place, want);
     __syncthreads();
-    int tiles = 0;
+    int tiles = 0, longest = 0;
     for (int j0 = 0; j0 < nb; j0 += CH_PT) {
         const int j = j0 + t;
         ChunkBlock x = {};
@@ -177,10 +177,20 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
             x.tiles = max(1, (x.end + TILE - 1) / TILE);  // (rows that see nothing are written too)
             x.place = s_place[lo] < 0 ? -1 : s_place[lo] + (WEIGHTS ? x.blk : 0);
         }
-        const int takes = WEIGHTS || j >= nb ? x.tiles : x.tiles + CH_EXTRA;
-        x.begin = tiles + ch_scan<CH_PT>(takes, s_wave, &all);
+        x.begin = tiles + ch_scan<CH_PT>(x.tiles, s_wave, &all);
         tiles += all;
-        if (j < nb) blocks[j] = x;
+        if (j < nb) {
+            blocks[j] = x;
+            longest = max(longest, x.tiles);
+        }
+    }
+    if (!WEIGHTS) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) longest = max(longest, __shfl_xor(longest, o, 64));
+        __syncthreads();
+        if (lane == 0) s_wave[t >> 6] = longest;
+        __syncthreads();
+        for (int w = 0; w < CH_PT / 64; w++) longest = max(longest, s_wave[w]);
     }
     int n_few = 0, steps = 0;
     if (!WEIGHTS && src.few > 0) {
@@ -202,6 +212,7 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
         head[3] = used;
         head[4] = n_few;
         head[5] = steps;
+        head[6] = longest;
     }
 }
 
@@ -209,7 +220,7 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
 struct OwnPlan {
     ChunkBlock blocks[CH_OWN];
     int4 list[CH_OWN];
-    int head[6];
+    int head[7];
 };
 template <bool WEIGHTS>
 __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& src) {
@@ -272,9 +283,11 @@ __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& sr
         x.tiles = t < nb ? max(1, (x.end + TILE - 1) / TILE) : 0;
         const int pl = __shfl(place, lo, 64), many = __shfl(want, lo, 64);
         x.place = many > 0 ? pl + x.blk : -1;
-        const int takes = WEIGHTS || t >= nb ? x.tiles : x.tiles + CH_EXTRA;
-        x.begin = before(takes);
+        x.begin = before(x.tiles);
         if (t < nb) plan.blocks[t] = x;
+        int longest = x.tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) longest = max(longest, __shfl_xor(longest, o, 64));
         int n_few = 0, steps = 0;
         if (!WEIGHTS && src.few > 0) {
             const int j = before(few);
@@ -292,26 +305,62 @@ __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& sr
         }
         if (t == 63) {
             plan.head[0] = nb;
-            plan.head[1] = x.begin + takes;
+            plan.head[1] = x.begin + x.tiles;
             plan.head[2] = entry + (want > 0);
             plan.head[3] = 0;
             plan.head[4] = n_few;
             plan.head[5] = steps;
+            plan.head[6] = longest;
         }
     }
     __syncthreads();
 }
 
-// slices that hold tiles: the same number for every workgroup of a call
-__device__ __forceinline__ int ch_slices(int slices, int tiles) { return min(slices, tiles); }
-__device__ __forceinline__ int ch_cut(int w, int tiles, int slices) { return (int)((long long)w * tiles / slices); }
+// How the tiles are cut: the same for every workgroup of a call.  Where that keeps the longest slice about as short (few blocks),
+// each block by itself, into parts of up to `part` tiles: a workgroup has one part.  Otherwise the row of all tiles, of which a
+// block has the places extra * (j + 1) + its tiles' numbers, and `extra` before those, into slices of the same length.
+struct ChunkCuts {
+    int extra, row, slices, part;  // part: 0 if the row is cut
+    __device__ __forceinline__ int cut(int w) const { return (int)((long long)w * row / slices); }
+    // the block of slice w, and its parts before that: a lane a block (wave-uniform; -1: none)
+    __device__ __forceinline__ int block(const ChunkBlock* blocks, int nb, int w, int* before) const {
+        const int lane = threadIdx.x & 63, parts = lane < nb ? (blocks[lane].tiles + part - 1) / part : 0;
+        int upto = parts;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += y;
+        }
+        const unsigned long long has = __ballot(lane < nb && upto - parts <= w && w < upto);
+        const int j = has ? __builtin_ctzll(has) : -1;
+        *before = __builtin_amdgcn_readlane(upto - parts, j < 0 ? 0 : j);
+        return j;
+    }
+};
+__device__ __forceinline__ ChunkCuts ch_cuts(int slices, int nb, int tiles, int longest) {
+    ChunkCuts c = {0, tiles, min(slices, tiles), 0};
+    if (tiles == 0) return c;
+    if (nb <= slices) {
+        static_assert(CH_SLICES <= 64, "a lane a block");
+        const int spare = slices - nb;  // (sum of the parts <= nb + tiles / part <= slices)
+        const int part = spare > 0 ? min(longest, max(CH_LEAST, (tiles + spare - 1) / spare)) : longest;
+        if (part <= tiles / slices + CH_EXTRA) c.part = part;
+    }
+    if (c.part == 0) {
+        c.extra = CH_EXTRA;
+        c.row = tiles + CH_EXTRA * nb;
+        c.slices = slices;
+    }
+    return c;
+}
+// steps, or tiles of the weights
+__device__ __forceinline__ ChunkCuts ch_cuts(int slices, int tiles) { return ChunkCuts{0, tiles, min(slices, tiles), 0}; }
 
 // the block that holds place s, found by the whole workgroup
-template <int EXTRA>
-__device__ __forceinline__ int ch_find(const ChunkBlock* blocks, int nb, int s, int* s_found) {
+__device__ __forceinline__ int ch_find(const ChunkBlock* blocks, int nb, int extra, int s, int* s_found) {
     for (int j = threadIdx.x; j < nb; j += blockDim.x) {
-        const int begin = blocks[j].begin;
-        if (begin <= s && s < begin + EXTRA + blocks[j].tiles) *s_found = j;
+        const int begin = blocks[j].begin + extra * j;
+        if (begin <= s && s < begin + extra + blocks[j].tiles) *s_found = j;
     }
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(*s_found);
@@ -959,21 +1008,32 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         ch_own_plan<false>(shared.plan, a.src);
         blocks = shared.plan.blocks;
         head = shared.plan.head;
+        if (blockIdx.x == 0) {  // for the join
+            const int words = (head[0] + head[4]) * (int)(sizeof(ChunkBlock) / 4);
+            for (int i = threadIdx.x; i < words; i += blockDim.x)
+                reinterpret_cast<int*>(a.blocks)[i] = reinterpret_cast<const int*>(blocks)[i];
+            if (threadIdx.x < 7) a.head[threadIdx.x] = head[threadIdx.x];
+        }
     }
     const int nb = __builtin_amdgcn_readfirstlane(head[0]), tiles = __builtin_amdgcn_readfirstlane(head[1]);
-    // a slice, or a block as a whole
-    const int per = a.slices > 0 ? a.slices : (int)gridDim.x / NKV, g = unit / per, w = unit % per;
-    int s = 0, s_end = 0, j = w;
+    const int g = unit / a.slices, w = unit % a.slices;
+    int s = 0, s_end = 0, j = 0;
     if (threadIdx.x < 8) lds.odd[threadIdx.x >> 2].tile[threadIdx.x & 3] = -1;
-    if (a.slices == 0) {
-        if (w >= nb) return;
-        s = __builtin_amdgcn_readfirstlane(blocks[j].begin);
-        s_end = s + CH_EXTRA + __builtin_amdgcn_readfirstlane(blocks[j].tiles);
+    const ChunkCuts tile_cuts = ch_cuts(a.slices, nb, tiles, __builtin_amdgcn_readfirstlane(head[6]));
+    if (tile_cuts.part > 0) {
+        int before;
+        j = tile_cuts.block(blocks, nb, w, &before);
+        if (j >= 0) {
+            const ChunkBlock c = ch_block(blocks[j]);
+            const int parts = (c.tiles + tile_cuts.part - 1) / tile_cuts.part;
+            s = c.begin + (w - before) * c.tiles / parts;
+            s_end = c.begin + (w - before + 1) * c.tiles / parts;
+        }
         __syncthreads();
-    } else if (const int slices = ch_slices(a.slices, tiles); w < slices) {
-        s = ch_cut(w, tiles, slices);
-        s_end = ch_cut(w + 1, tiles, slices);
-        j = ch_find<CH_EXTRA>(blocks, nb, s, &shared.found);
+    } else if (w < tile_cuts.slices) {
+        s = tile_cuts.cut(w);
+        s_end = tile_cuts.cut(w + 1);
+        j = ch_find(blocks, nb, tile_cuts.extra, s, &shared.found);
     }
     const int s_begin = s;
     int walked = 0;
@@ -986,7 +1046,7 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         asm volatile("" : "+v"(t));
         ChunkSegment sg;
         sg.c = ch_block(blocks[j]);
-        const int first = sg.c.begin + CH_EXTRA, stop = min(s_end, first + sg.c.tiles), from = s;
+        const int first = sg.c.begin + tile_cuts.extra * (j + 1), stop = min(s_end, first + sg.c.tiles), from = s;
         s = stop;
         j++;
         sg.base = walked;
@@ -1008,12 +1068,13 @@ k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     const int n_few = a.few > 0 ? __builtin_amdgcn_readfirstlane(head[4]) : 0;
     if (n_few == 0) return;
     // the chunks of few rows
-    const int steps = __builtin_amdgcn_readfirstlane(head[5]), slices = ch_slices(a.slices, steps);
-    if (w >= slices) return;
-    s = ch_cut(w, steps, slices);
-    s_end = ch_cut(w + 1, steps, slices);
+    const int steps = __builtin_amdgcn_readfirstlane(head[5]);
+    const ChunkCuts cuts = ch_cuts(a.slices, steps);
+    if (w >= cuts.slices) return;
+    s = cuts.cut(w);
+    s_end = cuts.cut(w + 1);
     __syncthreads();  // (of the tiles' LDS nothing is read any more)
-    j = ch_find<0>(blocks + nb, n_few, s, &shared.found);
+    j = ch_find(blocks + nb, n_few, 0, s, &shared.found);
     auto segment = [&] {
         const ChunkBlock c = ch_block(blocks[nb + j]);
         const int k0 = (s - c.begin) * CH_STEP, stop = min(s_end, c.begin + c.tiles);
@@ -1037,16 +1098,16 @@ __device__ __forceinline__ void ch_join_row(const ChunkArgs& a, const float* o, 
     const float4 gv = *reinterpret_cast<const float4*>(a.gate + out * HD + 4 * lane);
     float M = -INFINITY, L = 0.0f, X = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int w = w0; w <= w1; w += 4) {
-        float4 ml[4], x[4];
+    for (int w = w0; w <= w1; w += 8) {
+        float4 ml[8], x[8];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < 8; u++) {
             const size_t at = place(min(w + u, w1));
             ml[u] = sums[at];
             x[u] = *reinterpret_cast<const float4*>(o + at * HD + 4 * lane);
         }
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < 8; u++) {
             if (w + u > w1) break;
             const float Mn = fmaxf(M, ml[u].x);
             const float f0 = M == Mn ? 1.0f : fast_exp2(M - Mn);
@@ -1074,20 +1135,14 @@ constexpr int CH_JR = 16;  // rows of a workgroup
 template <bool LSE>
 __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a, int parts) {
     __shared__ int found;
-    __shared__ OwnPlan plan;
-    const ChunkBlock* blocks = a.blocks;
-    const int* head = a.head;
-    if (a.own) {
-        ch_own_plan<false>(plan, a.src);
-        blocks = plan.blocks;
-        head = plan.head;
-    }
+    const ChunkBlock* const blocks = a.blocks;
+    const int* const head = a.head;
     const int g = blockIdx.y, cut = blockIdx.x / parts + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (cut >= a.slices) {
         const int j = (int)blockIdx.x - (a.slices - 1) * parts;
         if (j >= head[4]) return;
         const ChunkBlock c = blocks[head[0] + j];
-        const int steps = head[5], slices = ch_slices(a.slices, steps);
+        const int steps = head[5], slices = ch_cuts(a.slices, steps).slices;
         auto slice = [&](int s) { return (int)(((long long)(s + 1) * slices - 1) / steps); };  // that holds step s
         const int w0 = slice(c.begin), w1 = slice(c.begin + c.tiles - 1);
         const size_t rec = (size_t)g * (a.slices + a.few) + j;
@@ -1096,26 +1151,42 @@ __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a, int parts) {
                              [&](int w) { return (rec + w) * CH_FEW_ROWS + r; });
         return;
     }
-    const int tiles = head[1], slices = ch_slices(a.slices, tiles);
-    if (cut >= slices) return;
-    const int s = ch_cut(cut, tiles, slices), s_before = ch_cut(cut - 1, tiles, slices);
-    const int j = ch_find<CH_EXTRA>(blocks, head[0], s, &found);
+    const ChunkCuts cuts = ch_cuts(a.slices, head[0], head[1], head[6]);
+    const int part = blockIdx.x % parts;
+    auto rows = [&](const ChunkBlock& c, int w0, int w1, auto place) {
+        for (int r = CH_JR * part + wave; r < CH_JR * (part + 1); r += 4) {
+            const int row = CH_ROWS * c.blk + r;
+            if (row >= GRP * c.count) return;
+            ch_join_row<LSE>(a, a.part_o, a.part_ml, (size_t)(c.row0 + row / GRP) * NH + g * GRP + row % GRP, w0, w1, lane,
+                             [&](int w) { return (((size_t)g * a.slices + w) * 2 + place(w)) * a.prows + r; });
+        }
+    };
+    if (cuts.part > 0) {  // (a block by itself, in slices of its own; all blocks but one at most where any is cut)
+        const int j = cut - 1;
+        if (j >= head[0]) return;
+        const ChunkBlock c = blocks[j];
+        const int n = (c.tiles + cuts.part - 1) / cuts.part;
+        if (n == 1) return;
+        int w0 = 0;  // the parts of the blocks before it
+        for (int i = lane; i < j; i += 64) w0 += (blocks[i].tiles + cuts.part - 1) / cuts.part;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) w0 += __shfl_xor(w0, o, 64);
+        w0 = __builtin_amdgcn_readfirstlane(w0);
+        rows(c, w0, w0 + n - 1, [](int) { return 0; });
+        return;
+    }
+    if (cut >= cuts.slices) return;
+    const int s = cuts.cut(cut), s_before = cuts.cut(cut - 1);
+    const int j = ch_find(blocks, head[0], cuts.extra, s, &found);
     const ChunkBlock c = blocks[j];
     // the cut lies before the block's first tile, or an earlier one lies behind that
-    const int first = c.begin + CH_EXTRA;
+    const int begin = c.begin + cuts.extra * j, first = begin + cuts.extra;
     if (s <= first || s_before > first) return;
     // its slices: cut - 1 up to the one that holds its last tile
-    const int last = first + c.tiles - 1, part = blockIdx.x % parts;
+    const int last = first + c.tiles - 1;
     int w1 = cut;
-    while (w1 + 1 < slices && ch_cut(w1 + 1, tiles, slices) <= last) w1++;
-    for (int r = CH_JR * part + wave; r < CH_JR * (part + 1); r += 4) {
-        const int row = CH_ROWS * c.blk + r;
-        if (row >= GRP * c.count) return;
-        ch_join_row<LSE>(a, a.part_o, a.part_ml, (size_t)(c.row0 + row / GRP) * NH + g * GRP + row % GRP, cut - 1, w1, lane,
-                         [&](int w) {
-                             return (((size_t)g * a.slices + w) * 2 + (w == cut - 1 && c.begin > s_before ? 1 : 0)) * a.prows + r;
-                         });
-    }
+    while (w1 + 1 < cuts.slices && cuts.cut(w1 + 1) <= last) w1++;
+    rows(c, cut - 1, w1, [&](int w) { return w == cut - 1 && begin > s_before ? 1 : 0; });
 }
 
 hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_layer& kv, int kvt, const qwa_kv_pages& p,
@@ -1142,7 +1213,7 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
             default: hipLaunchKernelGGL(k_ch_image<QWA_KV_Q4_0>, ig, dim3(512), 0, st, a, kv, p); break;
         }
     }
-    const dim3 grid((pl.whole ? pl.blocks : pl.slices) * NKV), block(128 * CH_PAIRS);
+    const dim3 grid(pl.slices * NKV), block(128 * CH_PAIRS);
 #define QWA_CH(T)                                                                              \
     case T:                                                                                    \
         if (lse) hipLaunchKernelGGL((k_ch_tiles<T, true>), grid, block, 0, st, a, kv, p);      \
@@ -1154,7 +1225,7 @@ hipError_t launch_prefill_batch(const float* q, const float* gate, const qwa_kv_
         default: QWA_CH(QWA_KV_Q4_0);
     }
 #undef QWA_CH
-    if (pl.slices > 1 || pl.few > 0) {
+    if (pl.join) {
         const int parts = (pl.rows + CH_JR - 1) / CH_JR;
         const dim3 jg((pl.slices - 1) * parts + pl.few, NKV);
         if (lse) hipLaunchKernelGGL(k_ch_join<true>, jg, dim3(256), 0, st, a, parts);
@@ -1214,11 +1285,11 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         head_of = lds.plan.head;
     }
     const int nb = __builtin_amdgcn_readfirstlane(head_of[0]), tiles = __builtin_amdgcn_readfirstlane(head_of[1]);
-    const int slices = ch_slices(a.slices, tiles);
-    if (w >= slices) return;
-    int s = ch_cut(w, tiles, slices);
-    const int s_end = ch_cut(w + 1, tiles, slices);
-    int j = ch_find<0>(blocks, nb, s, &lds.found);
+    const ChunkCuts cuts = ch_cuts(a.slices, tiles);
+    if (w >= cuts.slices) return;
+    int s = cuts.cut(w);
+    const int s_end = cuts.cut(w + 1);
+    int j = ch_find(blocks, nb, 0, s, &lds.found);
     const size_t head = (size_t)g * kv.capacity;
     const uint8_t* const kh = kv.k + head * value_bytes(KVT);
     const uint16_t* const ksh = SC ? kv.ks + head * 8 : nullptr;

@@ -37,17 +37,12 @@ struct ChunkImage {
 
 // A chunk's rows are cut into blocks of CH_ROWS; a block walks the PF_TILE-key tiles from the first to the last that one of its
 // rows sees.  The tiles of all blocks in a row, cut into `slices` equal parts, are the workgroups of a KV head.
-// blocks, slices (0: every block as a whole), images (chunks that read images), tiles (of images): bounds of what the device finds, which knows the chunks;
+// blocks, slices, images (chunks that read images), tiles (of images): bounds of what the device finds, which knows the chunks;
 // rows: of a block that are stored.
 // Calls of few chunks and blocks, without images, need no plan from a kernel of its own: a wave of every workgroup makes it, a
 // lane a chunk, a lane a block.
 constexpr int CH_OWN = 64;
-// Short sequences are not cut into slices: a workgroup has a block as a whole, and no states are joined.
-#ifndef QWA_CH_WHOLE
-#define QWA_CH_WHOLE 512
-#endif
-constexpr int CH_WHOLE = QWA_CH_WHOLE;
-// Chunks of up to CH_FEW rows (one or two tokens) are no blocks where slices are cut: their keys' steps of CH_STEP positions in a
+// Chunks of up to CH_FEW rows (one or two tokens) are no blocks where blocks are cut: their keys' steps of CH_STEP positions in a
 // row, cut into as many equal slices, follow a workgroup's tiles, and are walked by its waves a tile each (paged_walk.hpp): 499
 // tokens and 23 decoded ones over 8192 Q4_0 positions 230 us, as blocks 317, of which a decoded token filled a twentieth.
 constexpr int CH_FEW = 16, CH_FEW_ROWS = CH_FEW / GRP * GRP, CH_STEP = 256;
@@ -56,9 +51,14 @@ constexpr int CH_FEW = 16, CH_FEW_ROWS = CH_FEW / GRP * GRP, CH_STEP = 256;
 #define QWA_CH_EXTRA 8
 #endif
 constexpr int CH_EXTRA = QWA_CH_EXTRA;
+// Tiles of the parts that a block is cut into at least.
+#ifndef QWA_CH_LEAST
+#define QWA_CH_LEAST 4
+#endif
+constexpr int CH_LEAST = QWA_CH_LEAST;
 struct ChunkPlan {
     int blocks, slices, rows, images, tiles, few;  // few: chunks that may be of so few rows
-    bool whole, own;
+    bool own, join;
 };
 
 inline ChunkPlan chunk_plan(int n, int rows, int max_len) {
@@ -66,13 +66,13 @@ inline ChunkPlan chunk_plan(int n, int rows, int max_len) {
     const int most = (max_len + PF_TILE - 1) / PF_TILE;
     // (a chunk has one partly filled block)
     p.blocks = (int)std::min<long long>((long long)GRP * rows, (long long)GRP * rows / CH_ROWS + n);
-    p.whole = max_len <= CH_WHOLE;
-    p.slices = p.whole ? 0 : (int)std::min<long long>(CH_SLICES, (long long)p.blocks * (most + CH_EXTRA));
+    p.slices = (int)std::min<long long>(CH_SLICES, (long long)p.blocks * most);
+    p.join = p.blocks > p.slices || most > CH_LEAST;  // (else every block stays whole)
     p.rows = std::min(CH_ROWS, GRP * rows);
     // (a chunk of CH_IMG_BLOCKS blocks has more than CH_IMG_BLOCKS - 1 full ones)
     p.images = std::min(n, (int)((long long)GRP * rows / (CH_ROWS * (CH_IMG_BLOCKS - 1))));
     p.tiles = (int)std::min<long long>((long long)p.images * most, std::max(most, CH_IMG_TILES));
-    p.few = p.whole || CH_FEW_ROWS == 0 ? 0 : std::min(n, rows);
+    p.few = p.join ? std::min(n, rows) : 0;
     p.own = n <= CH_OWN && p.blocks <= CH_OWN && p.images == 0;
     return p;
 }

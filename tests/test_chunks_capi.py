@@ -200,7 +200,7 @@ int main() {
         CHECK(blocks <= p.blocks && images <= p.images, "%lld blocks, %lld with images: %d, %d\n", blocks, images, p.blocks, p.images);
         CHECK(wblocks <= q.blocks && parts <= q.parts && multi <= q.parts / 2, "weights: %lld blocks, %lld places\n", wblocks, parts);
         CHECK(p.images == 0 || p.tiles >= (most + PF_TILE - 1) / PF_TILE, "room for one sequence\n");
-        CHECK(p.whole == (p.slices == 0) && p.slices <= CH_SLICES && q.slices >= 1 && q.slices <= CH_SLICES, "slices\n");
+        CHECK(p.slices >= 1 && p.slices <= CH_SLICES && q.slices >= 1 && q.slices <= CH_SLICES, "slices\n");
         // tiles fit 32 bits
         CHECK((long long)p.blocks * ((MAX_POS + PF_TILE - 1) / PF_TILE) < 1LL << 31, "tiles\n");
         CHECK(w.o % 16 == 0 && w.ml % 16 == 0 && w.blocks % 16 == 0 && w.list % 16 == 0 && w.head % 16 == 0, "alignment\n");
