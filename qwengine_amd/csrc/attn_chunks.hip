@@ -415,14 +415,8 @@ __global__ void __launch_bounds__(512) k_ch_image(ChunkArgs a, qwa_kv_layer kv, 
     }
 }
 
-#ifndef QWA_CH_VD
-#define QWA_CH_VD 6
-#endif
-#ifndef QWA_CH_KD
-#define QWA_CH_KD 2
-#endif
-constexpr int CH_KD = QWA_CH_KD;    // K steps read ahead of their MFMAs
-constexpr int CH_VD = QWA_CH_VD;    // V fragments in flight
+constexpr int CH_KD = 2;    // K steps read ahead of their MFMAs
+constexpr int CH_VD = 6;    // V fragments in flight
 
 // sigmoid by the reciprocal instruction (1 ulp; the output is rounded to fp16): the division's steps are a third of what the rows'
 // ends took

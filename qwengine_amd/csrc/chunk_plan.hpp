@@ -18,11 +18,10 @@ constexpr int CH_SLICES = 256 / NKV;        // workgroups of a KV head: one roun
 
 // Chunks of at least CH_IMG_BLOCKS blocks read their keys as images: tiles that k_ch_image has brought into the form of LDS once,
 // instead of every block by itself.  Images take 4 times the bytes of a Q8_0 cache, so there is room for CH_IMG_TILES tiles (of
-// each KV head) or one sequence, whichever is more, and chunks that find none left do without.
-#ifndef QWA_CH_IMG_BLOCKS
-#define QWA_CH_IMG_BLOCKS 4
-#endif
-constexpr int CH_IMG_BLOCKS = QWA_CH_IMG_BLOCKS;
+// each KV head) or one sequence, whichever is more, and chunks that find none left do without.  Chunks at 8000 positions, us, with /
+// without images: 100 tokens (5 blocks) F16 83 / 69, Q8_0 84 / 76, Q4_0 84 / 76; 4 of 200 (10 blocks) 271 / 249, 284 / 299, 287 /
+// 298; 1000 tokens (47) 259 / 275, 279 / 331, 280 / 330.
+constexpr int CH_IMG_BLOCKS = 12;
 constexpr int CH_IMG_TILES = 4096;
 struct ChunkImage {
     uint16_t k[PF_TILE * HD];
@@ -47,15 +46,12 @@ constexpr int CH_OWN = 64;
 // tokens and 23 decoded ones over 8192 Q4_0 positions 230 us, as blocks 317, of which a decoded token filled a twentieth.
 constexpr int CH_FEW = 16, CH_FEW_ROWS = CH_FEW / GRP * GRP, CH_STEP = 256;
 // What a block takes besides its tiles (Q's way into registers, O's way out), in tiles: the slices are cut from rows of both.
-#ifndef QWA_CH_EXTRA
-#define QWA_CH_EXTRA 8
-#endif
-constexpr int CH_EXTRA = QWA_CH_EXTRA;
-// Tiles of the parts that a block is cut into at least.
-#ifndef QWA_CH_LEAST
-#define QWA_CH_LEAST 4
-#endif
-constexpr int CH_LEAST = QWA_CH_LEAST;
+// (Six prompts of up to 1021 F16 tokens, of whose blocks some have 1 tile and some 32, the kernel: 0 / 4 / 6 / 8 / 11: 208 / 166 / 158
+// / 148 / 149 us; a chunk of 1024 tokens at 32768 the same with each.)
+constexpr int CH_EXTRA = 8;
+// Tiles of the parts that a block is cut into at least.  Whole call, us, 2 / 3 / 4 / 5: two chunks of 20 tokens at 512 Q8_0 positions
+// 35 / 32 / 31 / 31, at 320 28 with each, 100 tokens of 100 35 / 37 / 30 / 30.
+constexpr int CH_LEAST = 4;
 struct ChunkPlan {
     int blocks, slices, rows, images, tiles, few;  // few: chunks that may be of so few rows
     bool own, join;

@@ -241,6 +241,42 @@ def test_pages_outside_the_pool(gpu, kvt):
     assert (lse[:50].double().cpu() - want_lse).abs().max() <= LSE
 
 
+@pytest.mark.parametrize("kvt", KVTS, ids=lambda k: KV_NAMES[k])
+def test_images_of_odd_keys(gpu, kvt):
+    """Both of the above for a chunk of many blocks, whose keys are brought into LDS's form once."""
+    b, n = Batch(kvt, [700], page=32), 300
+    q, gate, clean, _ = prefill(b, [0, n], 1, n, 700)
+    bad = 600  # tokens from 200 on see it
+    slot = int(b.pages.table[0, bad // b.page]) * b.page + bad % b.page
+    keep = [None if x is None else x[1, slot].clone() for x in (b.kv.v, b.kv.vs, b.kv.k, b.kv.ks)]
+    mark = torch.zeros((n, 24, 256), dtype=torch.bool, device="cuda")
+    for values, scales, what in ((b.kv.v, b.kv.vs, "v"), (b.kv.k, b.kv.ks, "k")):
+        if kvt == ops.F16:
+            values[1, slot].view(torch.int16)[5] = 0x7E00
+            dims = [5]
+        else:
+            scales[1, slot, 2] = 0x7E00
+            dims = list(range(64, 96))
+        _, _, out, lse = prefill(b, [0, n], 1, n, 700, q=q, gate=gate)
+        mark[:] = False
+        mark[200:, 6:12, dims if what == "v" else slice(None)] = True
+        assert torch.isnan(out[mark]).all() and torch.equal(out[~mark], clean[~mark])
+        assert torch.isnan(lse[200:, 6:12]).all() == (what == "k") and torch.isfinite(lse[:200]).all()
+        for x, y in zip((b.kv.v, b.kv.vs, b.kv.k, b.kv.ks), keep):
+            if x is not None:
+                x[1, slot] = y
+    for e, none in ((2, -1), (7, 1 << 30), (21, b.pages.ref.numel())):
+        b.pages.table[0, e] = none
+    _, _, out, lse = prefill(b, [0, n], 1, n, 700, q=q, gate=gate)
+    gone = torch.zeros(700, dtype=torch.bool)
+    gone[64:96] = gone[224:256] = gone[672:] = True
+    K, V = b.values(0)
+    K, V, kept = K[:, ~gone], V[:, ~gone], (~gone).cumsum(0)
+    want, want_lse = attention(q, gate, lambda t: (K, V), [int(kept[400 + t]) for t in range(n)])
+    close(out, want, "holes")
+    assert (lse.double().cpu() - want_lse).abs().max() <= LSE
+
+
 def test_repeated_calls_streams_and_graphs(gpu):
     """The same bits again, on another stream beside it, and from a captured graph that follows the device's numbers."""
     kvt, n, rows = ops.Q8_0, 3, 200
