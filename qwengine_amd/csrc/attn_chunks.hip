@@ -3,22 +3,23 @@
 // Batch row b has the tokens off[b] .. off[b + 1] - 1, the last c = off[b + 1] - off[b] positions of its sequence; token t of it
 // sees positions [0, len - c + t].  For row r = (token, head):  out = sum_j p_j V_j / sum_j p_j * sigmoid(gate),
 // p_j = exp(s_j), s_j = q_r . K_j / 16, and log sum_j p_j for who asks for it.
-//  * A block is CH_ROWS consecutive rows (6 * token + head of the group) of a chunk; its keys are walked in 32-key tiles.  The tiles
-//    of all blocks in a row are cut into equal slices, a workgroup each: a long sequence's decoded token and a prompt of
-//    a thousand load the chip alike.  A block that lies in several slices leaves partial states, which k_ch_join joins in the
+//  * A block is CH_ROWS consecutive rows (6 * token + head of the group) of a chunk; its keys are walked in 32-key tiles.  The
+//    tiles of all blocks are cut into slices of about the same time, a workgroup each: a long sequence's tokens and a prompt of a
+//    thousand load the chip alike.  A block that lies in several slices leaves partial states, which k_ch_join joins in the
 //    slices' order; the others are finished where they are.
 //  * A workgroup has two waves a SIMD, with a role each.  The score waves keep Q (32 rows: hi and lo part, 128 registers), bring K
 //    into LDS and leave tile i's exponents there: S^T = K Q^T against the rows' references.  The value waves keep O (32 rows, 128
-//    registers), bring V into LDS, take the exponentials of tile i - 1 and add V^T P^T.  So each fragment of K and V that is read from LDS meets 32 rows, which one wave
-//    with both Q and O has no registers for, and one wave's arithmetic runs beside the other's MFMAs.
+//    registers), bring V into LDS, take the exponentials of tile i - 1 and add V^T P^T.  So each fragment of K and V that is read
+//    from LDS meets 32 rows, which one wave with both Q and O has no registers for, and one wave's arithmetic runs beside the
+//    other's MFMAs.
 //  * Chunks of one or two tokens leave most of a block empty.  Where sequences are cut, they are worked on behind the tiles: a wave
 //    a tile, its bytes straight into registers (paged_walk.hpp).
-//  * Chunks of many blocks would convert each tile once a block: k_ch_image does it for them once, and the waves copy the images into
-//    LDS, two tiles ahead.
+//  * Chunks of many blocks would convert each tile once a block: k_ch_image does it for them once, and the waves copy the images
+//    into LDS, two tiles ahead.
 //  * Scores are exact up to fp32 accumulation (K as its codes, Q / 16 as the sum of two fp16 parts), as the batched decode's are;
 //    the arithmetic of a tile, of V that is not finite and of the probabilities' range is paged_tiles.hpp's.
-// Roundings below 32 bits: the dequantized V (d * code) and the probabilities are fp16, half a step 2^-11 of the value; the sum of a
-// row's probabilities is that of the rounded ones, which P V applies, but the log of the sum is taken of the unrounded.  The
+// Roundings below 32 bits: the dequantized V (d * code) and the probabilities are fp16, half a step 2^-11 of the value; the sum of
+// a row's probabilities is that of the rounded ones, which P V applies, but the log of the sum is taken of the unrounded.  The
 // output is fp16.
 #include <algorithm>
 #include <type_traits>
@@ -29,9 +30,9 @@
 
 namespace qwa {
 
-// a block: its chunk's first row and number of tokens, the sequence's length and number (< 0: unknown, len 0), the block's number in
-// the chunk, its first tile in the row of all tiles, its tiles, the positions that its last row sees, the chunk's first image, or the
-// block's place for its sums (-1: none)
+// a block: its chunk's first row and number of tokens, the sequence's length and number (< 0: unknown, len 0), the block's number
+// in the chunk, its first tile in the row of all tiles, its tiles, the positions that its last row sees, the chunk's first image,
+// or the block's place for its sums (-1: none)
 struct alignas(16) ChunkBlock {
     int row0, count, len, seq;
     int blk, begin, tiles, end;
@@ -57,7 +58,8 @@ struct ChunkArgs {
     float* lse;              // [rows][24] or none
     ChunkBlock* blocks;
     const int4* list;        // chunks with images: sequence, length, first image, images
-    int* head;               // numbers of blocks, their tiles, chunks with images, images, chunks of few rows, their steps, the longest block
+    int* head;               // numbers of blocks, their tiles, chunks with images, images, chunks of few rows, their steps, and
+                             // the longest block's tiles
     ChunkImage* images;      // [tile][KV head]
     float* part_o;           // [KV head][slice][2][rows][256]
     float4* part_ml;         // [KV head][slice][2][rows]
@@ -154,7 +156,8 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
     const int entry = ch_scan<CH_PT>(has, s_wave, &listed);
     ch_scan<CH_PT>(has ? want : 0, s_wave, &used);
     s_place[t] = has && entry < most_list ? place : -1;
-    if (s_place[t] >= 0) list[entry] = WEIGHTS ? make_int4(s_seq[t], s_len[t], count, place) : make_int4(s_seq[t], s_len[t], place, want);
+    if (s_place[t] >= 0)
+        list[entry] = WEIGHTS ? make_int4(s_seq[t], s_len[t], count, place) : make_int4(s_seq[t], s_len[t], place, want);
     __syncthreads();
     int tiles = 0, longest = 0;
     for (int j0 = 0; j0 < nb; j0 += CH_PT) {
@@ -373,7 +376,8 @@ __device__ __forceinline__ ChunkBlock ch_block(const ChunkBlock& c) {
                       uni(c.place)};
 }
 
-// The images: a workgroup of 512 threads converts a tile of one KV head, half of them K, half V, from registers to memory.
+// The images: a workgroup of 512 threads converts a tile of one KV head, half of them K, half V, from registers to memory.  What it
+// writes bounds it: 33792 Q8_0 positions (144 MB of images) 37 us.
 constexpr int CH_IMG_WGS = 2048;
 template <int KVT>
 __global__ void __launch_bounds__(512) k_ch_image(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
@@ -986,6 +990,13 @@ struct ChunkShared {
     OwnPlan plan;
 };
 
+// 1024 tokens over 32768 Q8_0 positions 1200 to 1260 us, 0.70 PFLOP/s, 1.05 with the second part of Q (large products of the
+// library 1.21); 1.65 us a tile.  Of a SIMD's cycles 49% are MFMAs and 39% issue VALU instructions, LDS is busy for 31% and without
+// conflicts; the value waves are the longer chain: copies' issue and exponents 1200 cycles, exponentials 900, P V 750 and 500
+// between them, of 3400 to 3800 a tile.  Without the images' copies a tile took 1.4 us, the copies alone 1.2 (7.3 TB/s of images,
+// which the L2s miss: a head's workgroups are spread over the positions).  A segment costs about 8 tiles besides: Q's way in and, longer, O's
+// way out, where a SIMD has one wave that takes sigmoids and stores.  Measured and not kept: Q three loads ahead and the next
+// block's description in LDS (no difference), the raw tiles for long chunks (1450).
 template <int KVT, bool LSE>
 __global__ void __launch_bounds__(128 * CH_PAIRS) __attribute__((amdgpu_waves_per_eu(2, 2)))
 k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
@@ -1124,7 +1135,7 @@ __device__ __forceinline__ void ch_join_row(const ChunkArgs& a, const float* o, 
 
 // Joins the states of the blocks that lie in several slices, in the slices' order: workgroup (cut between two slices, part of the
 // rows; KV head) has the block that the cut lies in, if it is the first cut in it; a wave a row.  The workgroups behind those have
-// a chunk of few rows each.
+// a chunk of few rows each.  The states' bytes bound it: 64 MB 18 to 21 us; two blocks of three parts 7.4.
 constexpr int CH_JR = 16;  // rows of a workgroup
 template <bool LSE>
 __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a, int parts) {
@@ -1260,7 +1271,11 @@ struct WeightsLds {
 };
 
 // A workgroup walks the 64-key tiles of a slice as k_ch_tiles does, with K alone: all waves convert it, then each takes the scores
-// of its 32 rows, and the sums over them; the workgroup's sum of a tile is written while the next one is multiplied.
+// of its 32 rows, and the sums over them; the workgroup's sum of a tile is written while the next one is multiplied.  1000 tokens
+// over 16384 Q4_0 positions 460 to 490 us, 0.43 PFLOP/s, 0.85 with both parts of Q: of a SIMD's cycles 39% are MFMAs and 54% issue
+// VALU instructions (a block scale's product for each score and 32 dims, exponentials, sums over rows), which its two waves rarely
+// overlap; <Q8_0> keeps 16 registers in scratch, <Q4_0> 7.  16 tokens over 16000 F16 positions 109 us:
+// their keys' bytes at 4.8 TB/s.
 template <int KVT>
 __global__ void __launch_bounds__(64 * CW_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
 k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
@@ -1414,7 +1429,7 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     }
 }
 
-// The weights of chunks of several blocks: the blocks' sums in order.
+// The weights of chunks of several blocks: the blocks' sums in order (24 blocks of 17384 positions, 40 MB, 16 us).
 __global__ void __launch_bounds__(256) k_cw_join(WeightsArgs a, size_t ld_pos) {
     __shared__ OwnPlan plan;
     if (a.own) ch_own_plan<true>(plan, a.src);

@@ -35,11 +35,11 @@ struct ChunkImage {
 };
 
 // A chunk's rows are cut into blocks of CH_ROWS; a block walks the PF_TILE-key tiles from the first to the last that one of its
-// rows sees.  The tiles of all blocks in a row, cut into `slices` equal parts, are the workgroups of a KV head.
-// blocks, slices, images (chunks that read images), tiles (of images): bounds of what the device finds, which knows the chunks;
-// rows: of a block that are stored.
-// Calls of few chunks and blocks, without images, need no plan from a kernel of its own: a wave of every workgroup makes it, a
-// lane a chunk, a lane a block.
+// rows sees.  What a KV head's workgroups walk are `slices` parts of the blocks' tiles (ch_cuts in attn_chunks.hip).
+// blocks, slices, images (chunks that read images), tiles (of images), few: bounds of what the device finds, which knows the
+// chunks; rows: of a block that are stored; join: whether any block may lie in several slices.
+// Calls of few chunks and blocks, without images, need no plan from a kernel of its own (7 to 10 us): a wave of every workgroup
+// makes it in 2, a lane a chunk, a lane a block.
 constexpr int CH_OWN = 64;
 // Chunks of up to CH_FEW rows (one or two tokens) are no blocks where blocks are cut: their keys' steps of CH_STEP positions in a
 // row, cut into as many equal slices, follow a workgroup's tiles, and are walked by its waves a tile each (paged_walk.hpp): 499

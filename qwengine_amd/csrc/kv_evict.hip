@@ -4,11 +4,12 @@
 // others, those of the largest weight w_j, the lower position of equals, in their order.  With r_0 < r_1 < ... the positions
 // kept, row r_i of K, V, scales and weights moves to position i; the layers and heads keep different positions, but as many, so
 // one length and one table row serve them all.
-//  * k_evict_select (a workgroup per request, layer and head, and one per request for its pages) finds the smallest weight kept by its bits, 11 at a time (a histogram
-//    in LDS of those that agree in the bits before), and lists the kept positions' places in the pool.  Nothing changes yet.
+//  * k_evict_select (a workgroup per request, layer and head, and one per request for its pages) finds the smallest weight kept by
+//    its bits, 11 at a time (a histogram in LDS of those that agree in the bits before), and lists the kept positions' places in
+//    the pool.  Nothing changes yet.
 //  * k_evict_plan (one workgroup) checks all requests, takes pages for those of the first `keep` positions that other sequences
 //    hold too, and changes the tables.
-//  * k_evict_move (a workgroup per request, layer, head, and K or V) moves the rows in order, a run at a time: position i <= r_i,
+//  * k_evict_move (one or four workgroups per request, layer, head, and K or V) moves the rows in order, a run at a time: position i <= r_i,
 //    so a run is written where no later run reads, and after all of it has been read.
 #include <algorithm>
 
@@ -61,6 +62,10 @@ __device__ __forceinline__ uint32_t ev_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// A workgroup reads its weights once, into registers, and is then bound by its own instructions and barriers: of 36 us for 32768
+// positions (64 workgroups) the weights and the first histogram take 7, a histogram's search and the next one 4 to 5 each, counting
+// what stays 7, writing it 7.  Measured and as fast: neighbouring positions over a wave's lanes instead of in a thread's
+// registers (and places by ballots); slower (42): the first 11 bits by counting bit by bit.
 __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
     __shared__ __attribute__((aligned(16))) int s_hist[EV_BINS];
     __shared__ long long s_wave[EV_T / 64];
@@ -131,7 +136,8 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
 #pragma unroll
         for (int e = 0; e < EV_LANE; e++) x[e] = j0 + e < m ? mass[j0 + e] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < EV_LANE / 16; e++) pg[e] = table[min(j0 + 16 * e, m - 1) >> sh];  // (a foreign page's request changes nothing)
+        for (int e = 0; e < EV_LANE / 16; e++)
+            pg[e] = table[min(j0 + 16 * e, m - 1) >> sh];  // (a foreign page's request changes nothing)
 #pragma unroll
         for (int e = 0; e < EV_LANE; e++) k[e] = j0 + e < c ? ev_key(x[e]) : 0u;
         uint32_t key = 0;
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
     }
 }
 
-// The requests together: all of them, or none.
+// The requests together: all of them, or none.  One workgroup's latency: 4 to 9 us.
 __global__ void __launch_bounds__(EV_T) k_evict_plan(EvictArgs a, int* __restrict__ dropped, int* __restrict__ status) {
     __shared__ long long s_wave[EV_T / 64];
     __shared__ int s_seq[EV_T], s_count[EV_T], s_base[EV_T], s_bad;
@@ -343,12 +349,17 @@ __global__ void __launch_bounds__(EV_T) k_evict_plan(EvictArgs a, int* __restric
     }
 }
 
-// The rows of a request, layer and head, of K or V: PARTS workgroups, each with a part of the columns (the order of the rows binds
-// a workgroup; their columns do not depend on each other).  While a run is written, the next one is on its way, and the places
-// of that after it.
+// The rows of a request, layer and head, of K or V.  While a run is written, the next one is on its way, and the places of that after
+// it.  The order of the rows binds a workgroup, but their columns do not depend on each other: of F16 each of four workgroups has
+// 128 bytes of a row (6 sequences of 8000 cut to 2000 in 16 layers, 1.57 GB: 310 us, 5.1 TB/s, the copy rate; whole rows 349).
+// Rows of the quantized types, of 256 and 128 bytes, stay whole (one Q4_0 document of 32768 cut to 4096 in 16 layers, 151 MB: 51 us by
+// 128 workgroups, which wait for their rows; in four parts 52; two Q8_0 of 600 to 256 10, in parts 12).
 constexpr int EV_MT = 512;  // threads
-template <int KVT, int PARTS>
+template <int KVT>
+constexpr int EV_PARTS = KVT == QWA_KV_F16 ? 4 : 1;
+template <int KVT>
 __global__ void __launch_bounds__(EV_MT) k_evict_move(EvictArgs a, PageLayers layers) {
+    constexpr int PARTS = EV_PARTS<KVT>;
     constexpr int VB = value_bytes(KVT), UNITS = VB / 16 / PARTS;  // 16-byte units of a row's part
     constexpr int U = PARTS == 1 ? 8 : 4;                          // units a thread moves of a run
     constexpr int ROWS = EV_MT * U / UNITS;                        // rows of it
@@ -445,7 +456,6 @@ __global__ void __launch_bounds__(EV_MT) k_evict_move(EvictArgs a, PageLayers la
     }
 }
 
-constexpr int EV_FEW = 256;  // workgroups of whole rows up to which they are cut into parts
 hipError_t launch_pages_evict(const qwa_kv_pages& p, const int* seqs, const int* keep, int n, int recent, int max_keep,
                               const qwa_kv_layer* layers, int n_layers, int kvt, float* mass, int* dropped, int* status,
                               void* work, hipStream_t st) {
@@ -454,13 +464,12 @@ hipError_t launch_pages_evict(const qwa_kv_pages& p, const int* seqs, const int*
     hipLaunchKernelGGL(k_evict_plan, dim3(1), dim3(EV_T), 0, st, a, dropped, status);
     if (n == 0) return hipGetLastError();
     const PageLayers pl = page_layers(layers, n_layers);
-    const bool few = n * n_layers * NKV * 2 <= EV_FEW;
-#define QWA_EV(T, P) \
-    hipLaunchKernelGGL((k_evict_move<T, P>), dim3(2 * n_layers * NKV * P, n), dim3(EV_MT), 0, st, a, pl)
+#define QWA_EV(T) \
+    hipLaunchKernelGGL(k_evict_move<T>, dim3(2 * n_layers * NKV * EV_PARTS<T>, n), dim3(EV_MT), 0, st, a, pl)
     switch (kvt) {
-        case QWA_KV_F16: if (few) QWA_EV(QWA_KV_F16, 4); else QWA_EV(QWA_KV_F16, 1); break;
-        case QWA_KV_Q8_0: if (few) QWA_EV(QWA_KV_Q8_0, 4); else QWA_EV(QWA_KV_Q8_0, 1); break;
-        default: if (few) QWA_EV(QWA_KV_Q4_0, 4); else QWA_EV(QWA_KV_Q4_0, 1); break;
+        case QWA_KV_F16: QWA_EV(QWA_KV_F16); break;
+        case QWA_KV_Q8_0: QWA_EV(QWA_KV_Q8_0); break;
+        default: QWA_EV(QWA_KV_Q4_0); break;
     }
 #undef QWA_EV
     return hipGetLastError();
