@@ -994,9 +994,10 @@ struct ChunkShared {
 // library 1.21); 1.65 us a tile.  Of a SIMD's cycles 49% are MFMAs and 39% issue VALU instructions, LDS is busy for 31% and without
 // conflicts; the value waves are the longer chain: copies' issue and exponents 1200 cycles, exponentials 900, P V 750 and 500
 // between them, of 3400 to 3800 a tile.  Without the images' copies a tile took 1.4 us, the copies alone 1.2 (7.3 TB/s of images,
-// which the L2s miss: a head's workgroups are spread over the positions).  A segment costs about 8 tiles besides: Q's way in and, longer, O's
-// way out, where a SIMD has one wave that takes sigmoids and stores.  Measured and not kept: Q three loads ahead and the next
-// block's description in LDS (no difference), the raw tiles for long chunks (1450).
+// which the L2s miss: a head's workgroups are spread over the positions).  A segment costs about 8 tiles besides: Q's way in and,
+// longer, O's way out with the gates.  Six prompts of up to 1021 F16 tokens, 136 to 152 us, move 0.5 GB of Q, gates, outputs and
+// states meanwhile.  Measured and not kept, none with a difference: Q three loads ahead, the next block's description in LDS, rows'
+// addresses without divisions, the exponents' reads before the copies; slower: raw tiles for long chunks (1450).
 template <int KVT, bool LSE>
 __global__ void __launch_bounds__(128 * CH_PAIRS) __attribute__((amdgpu_waves_per_eu(2, 2)))
 k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
@@ -1166,7 +1167,7 @@ __global__ void __launch_bounds__(256) k_ch_join(ChunkArgs a, int parts) {
                              [&](int w) { return (((size_t)g * a.slices + w) * 2 + place(w)) * a.prows + r; });
         }
     };
-    if (cuts.part > 0) {  // (a block by itself, in slices of its own; all blocks but one at most where any is cut)
+    if (cuts.part > 0) {  // blocks in slices of their own (where one is cut there are fewer blocks than slices)
         const int j = cut - 1;
         if (j >= head[0]) return;
         const ChunkBlock c = blocks[j];

@@ -352,8 +352,8 @@ __global__ void __launch_bounds__(EV_T) k_evict_plan(EvictArgs a, int* __restric
 // The rows of a request, layer and head, of K or V.  While a run is written, the next one is on its way, and the places of that after
 // it.  The order of the rows binds a workgroup, but their columns do not depend on each other: of F16 each of four workgroups has
 // 128 bytes of a row (6 sequences of 8000 cut to 2000 in 16 layers, 1.57 GB: 310 us, 5.1 TB/s, the copy rate; whole rows 349).
-// Rows of the quantized types, of 256 and 128 bytes, stay whole (one Q4_0 document of 32768 cut to 4096 in 16 layers, 151 MB: 51 us by
-// 128 workgroups, which wait for their rows; in four parts 52; two Q8_0 of 600 to 256 10, in parts 12).
+// Rows of the quantized types, of 256 and 128 bytes, stay whole (one Q4_0 document of 32768 cut to 4096 in 16 layers: 51 us, in four
+// parts 52; 151 MB, but a row's 16 bytes of scales are read as a line of 128, 0.21 GB; two Q8_0 of 600 to 256 10, in parts 12).
 constexpr int EV_MT = 512;  // threads
 template <int KVT>
 constexpr int EV_PARTS = KVT == QWA_KV_F16 ? 4 : 1;
