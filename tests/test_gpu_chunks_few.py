@@ -132,3 +132,46 @@ def test_streams_and_graphs(gpu):
         torch.cuda.synchronize()
         assert torch.equal(second[0], third[0]) and torch.equal(second[1], third[1])
         assert bool(third[0].abs().sum() > 0)
+
+
+@pytest.mark.parametrize("n", [64, 65, 128, 129])
+def test_numbers_of_chunks(gpu, n):
+    """Where plans are made by a wave, by two and by a workgroup of 1024: chunks of none to 30 tokens, one of 300."""
+    counts = [(i * 11) % 31 if i % 3 == 0 else i % 3 for i in range(n)]
+    counts[n // 2] = 300
+    b = Batch(ops.Q8_0, [max(c, (i * 53) % 640) for i, c in enumerate(counts)])
+    check(b, counts, pad=2)
+
+
+def test_offsets_past_32_bits(gpu):
+    """A pool whose rows lie past 4 GiB of their head's, and heads past 8 GiB: two tokens, and a chunk that is read through images."""
+    kvt, page = ops.F16, 1024
+    small = Batch(kvt, [3000], page=page)
+    n_pages = 8400
+    kv = ops.KVLayer.allocate(kvt, n_pages * page)
+    pages = ops.KVPages.allocate(1, 3 * page, n_pages, page)
+    last = [n_pages - 1, n_pages - 3, n_pages - 2]
+    pages.table[0, :3] = i32(last)
+    pages.len.fill_(3000)
+    for e, pg in enumerate(last):
+        old = int(small.pages.table[0, e])
+        for dst, src in ((kv.k, small.kv.k), (kv.v, small.kv.v)):
+            dst[:, pg * page:(pg + 1) * page] = src[:, old * page:(old + 1) * page]
+    want = [prefill(small, [0, c], 1, c, 3000)[2:] for c in (2, 300)]
+    small.kv, small.pages = kv, pages
+    for c, (out, lse) in zip((2, 300), want):
+        got = prefill(small, [0, c], 1, c, 3000)[2:]
+        assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+
+
+def test_images_without_room(gpu):
+    """Three long chunks, of which the scratch has room for one's images: each as in a call of its own, both within the tolerance."""
+    counts, lens = [300, 310, 290], [70000, 66000, 68000]
+    b, rows = Batch(ops.Q4_0, lens, page=1024), sum(counts)
+    off = offsets(counts)
+    q, gate, out, lse = prefill(b, off, 3, rows, max(lens))
+    for i, c in enumerate(counts):
+        at = slice(off[i], off[i + 1])
+        _, _, alone, alone_lse = prefill(b, [0, c], 1, c, max(lens), seqs=[i], q=q[at].contiguous(), gate=gate[at].contiguous())
+        close(out[at], alone, f"chunk {i}", max_abs=4e-3, rel_l2=1e-3)
+        assert (lse[at] - alone_lse).abs().max().item() <= 2 * LSE
