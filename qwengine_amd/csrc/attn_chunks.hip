@@ -1009,7 +1009,8 @@ struct ChunkShared {
 // which the L2s miss: a head's workgroups are spread over the positions).  A segment costs about 8 tiles besides: Q's way in and,
 // longer, O's way out with the gates.  Six prompts of up to 1021 F16 tokens, 136 to 152 us, move 0.5 GB of Q, gates, outputs and
 // states meanwhile.  Measured and not kept, none with a difference: Q three loads ahead, the next block's description in LDS, rows'
-// addresses without divisions, the exponents' reads before the copies; slower: raw tiles for long chunks (1450).
+// addresses without divisions, the exponents' reads before the copies, the score waves at a higher priority; slower: raw tiles for
+// long chunks (1450), the value waves at a higher priority (1365).
 template <int KVT, bool LSE>
 __global__ void __launch_bounds__(128 * CH_PAIRS) __attribute__((amdgpu_waves_per_eu(2, 2)))
 k_ch_tiles(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
