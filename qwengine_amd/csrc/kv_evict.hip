@@ -9,8 +9,8 @@
 //    the pool.  Nothing changes yet.
 //  * k_evict_plan (one workgroup) checks all requests, takes pages for those of the first `keep` positions that other sequences
 //    hold too, and changes the tables.
-//  * k_evict_move (one or four workgroups per request, layer, head, and K or V) moves the rows in order, a run at a time: position i <= r_i,
-//    so a run is written where no later run reads, and after all of it has been read.
+//  * k_evict_move (one or four workgroups per request, layer, head, and K or V) moves the rows in order, a run at a time: position
+//    i <= r_i, so a run is written where no later run reads, and after all of it has been read.
 #include <algorithm>
 
 #include "launch.hpp"
