@@ -265,7 +265,7 @@ int qwa_attn_decode_batch(const float* q, const float* gate, const qwa_kv_layer*
 /* qwa_attn_prep_batch for chunks: row r of qg / k / v / q_out / gate belongs to the chunk that has it, token t of a chunk of c
  * tokens has position len - c + t of its sequence, and the rotary position is that plus rope_off[b] (device; NULL: 0).  K / V
  * rows are appended there; a row whose position is negative, or whose page is none of the pool's, is not stored.  Of
- * several chunks of one sequence the last one is stored.  n <= QWA_PAGES_MAXN.  Every buffer 16-byte aligned. */
+ * several chunks of one sequence the last one that has tokens is stored.  n <= QWA_PAGES_MAXN.  Every buffer 16-byte aligned. */
 int qwa_attn_prep_rows_batch(const float* qg, const float* k, const float* v, const float* q_norm, const float* k_norm,
                              const qwa_kv_pages* p, const int* seqs, const int* off, int n, int rows, const int* rope_off,
                              float theta, float eps, int kvt, const qwa_kv_layer* kv, float* q_out, float* gate,

@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(64 * PB_WAVES) k_prep_rows_batch(
     float* __restrict__ q_out, float* __restrict__ gate) {
     constexpr int PER = (QWA_PAGES_MAXN + 64 * PB_WAVES - 1) / (64 * PB_WAVES);  // chunks a thread
     __shared__ __attribute__((aligned(16))) float s_cs[NROT];  // (read 16 bytes at a time)
-    __shared__ int s_b;
+    __shared__ int s_b, s_far[PB_WAVES];
     const int r = blockIdx.x, t = threadIdx.x;
     if (t == 0) s_b = n;
     __syncthreads();
@@ -522,12 +522,13 @@ __global__ void __launch_bounds__(64 * PB_WAVES) k_prep_rows_batch(
     const int seq = seqs ? seqs[b] : b;
     const bool known = seq >= 0 && seq < pg.n_seq;
     const int pos = (known ? max(pg.len[seq], 0) : 0) - count + (r - r0);
-    bool overlaps = false, later = false;
+    bool overlaps = false, later = false, named[PER];
 #pragma unroll
     for (int j = 0; j < PER; j++) {
         const int c = t + 64 * PB_WAVES * j;
         overlaps |= c < b && end[j] > first[j] && end[j] > r0;              // it begins before an earlier one's end
-        later |= seqs && c > b && end[j] > first[j] && seqs[c] == seq;      // a later chunk is the same sequence's
+        named[j] = seqs && c > b && end[j] > first[j] && seqs[c] == seq;    // a later one of the same sequence
+        later |= named[j];
     }
     long long slot = -1;
     if (known && pos >= 0 && pos / pg.page < pg.ld) {
@@ -536,7 +537,30 @@ __global__ void __launch_bounds__(64 * PB_WAVES) k_prep_rows_batch(
     }
     if (t < NROT / 2) rope_cs((double)pos + (rope_off ? rope_off[b] : 0), theta, t, &s_cs[t], &s_cs[t + NROT / 2]);
     if (__syncthreads_or(overlaps)) return;
-    if (__syncthreads_or(later)) slot = -1;
+    if (__syncthreads_or(later)) {
+        // Only a later one that counts takes this one's place: it must not begin before the furthest end ahead of it.
+        const int lane = t & 63, wave = t >> 6;
+        bool counts = false;
+        int far = 0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            int upto = end[j] > first[j] ? end[j] : 0;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(upto, o, 64);
+                if (lane >= o) upto = max(upto, x);
+            }
+            __syncthreads();  // s_far may still be read
+            if (lane == 63) s_far[wave] = upto;
+            const int prev = __shfl_up(upto, 1, 64);
+            __syncthreads();
+            int before = lane > 0 ? max(far, prev) : far;
+            for (int w = 0; w < wave; w++) before = max(before, s_far[w]);
+            counts |= named[j] && before <= first[j];
+            for (int w = 0; w < PB_WAVES; w++) far = max(far, s_far[w]);
+        }
+        if (__syncthreads_or(counts)) slot = -1;
+    }
     prep_token<KVT>(qg, k, v, qn_w, kn_w, r, slot, s_cs, eps, kv, q_out, gate);
 }
 
