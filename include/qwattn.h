@@ -258,8 +258,9 @@ int qwa_attn_decode_batch(const float* q, const float* gate, const qwa_kv_layer*
 /* Chunks: any number of new tokens for each of n sequences.  The tokens of all are rows of one buffer: batch row b has rows
  * off[b] .. off[b + 1] - 1 (off: device, n + 1 entries), a chunk of off[b + 1] - off[b] tokens, which are the last positions
  * that its sequence seqs[b] (device; NULL: b) holds.  `rows` is the size of the buffers: rows that no chunk has (behind the
- * last one, between two) are neither read nor written.  A chunk of no tokens takes no part; one that begins before an earlier
- * one's end, or has rows outside [0, rows], counts as empty.  A captured graph follows the device's numbers. */
+ * last one, between two) are neither read nor written.  A chunk of no tokens takes no part, wherever it stands; one with
+ * rows outside [0, rows] counts as empty; so does one that begins before the furthest end of the others ahead of it, of which each
+ * may count or not.  A captured graph follows the device's numbers. */
 #define QWA_CHUNK_MAXROWS 65536 /* rows per call */
 
 /* qwa_attn_prep_batch for chunks: row r of qg / k / v / q_out / gate belongs to the chunk that has it, token t of a chunk of c

@@ -257,7 +257,7 @@ __device__ __forceinline__ void ch_own_plan(OwnPlan& plan, const ChunkSource& sr
         const bool known = seq >= 0 && seq < src.p.n_seq;
         const int all = src.p.len[known ? seq : 0];
         if (first < 0 || end > src.rows || end < first) end = first = 0;
-        int far = end;
+        int far = end > first ? end : 0;  // (an empty chunk has no end)
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int y = __shfl_up(far, o, 64);

@@ -7,9 +7,10 @@ import pytest
 import torch
 
 import qwengine_amd.ops as ops
-from kvutil import KVTS, KV_NAMES
-from test_gpu_attn_batch import EPS, THETA, i32
-from test_gpu_chunks import prep_inputs, tables
+from kvutil import KVTS, KV_NAMES, seeded_normal
+from test_gpu_attn_batch import EPS, THETA, Batch, i32
+from test_gpu_chunks import LSE, attention, close, prefill, prep_inputs, tables
+from test_gpu_weights import log_sums, near, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +95,66 @@ def test_prep_of_many(gpu, n):
     for seed in range(3):
         seqs = [rng.randint(0, n // 3) for _ in range(n)]
         check_prep(ops.Q8_0, some_offsets(n, 3 * n, seed), seqs, 3 * n, [3 + (i * 5) % 40 for i in range(n // 3 + 1)])
+
+
+def check_attention(b, off, seqs, rows, max_len):
+    n, chunks = len(seqs), live(off, rows)
+    q, gate, out, lse = prefill(b, off, n, rows, max_len, seqs)
+    src, seen, at = [], [], []
+    for i, a, e in chunks:
+        m = min(b.lens[seqs[i]], max_len)
+        src += [b.values(seqs[i])] * (e - a)
+        seen += [m - (e - a) + t + 1 for t in range(e - a)]
+        at += list(range(a, e))
+    want, want_lse = attention(q[at], gate[at], lambda t: src[t], seen)
+    close(out[at], want, f"{KV_NAMES[b.kvt]} {n} chunks, {len(chunks)} count")
+    none = torch.isinf(want_lse)
+    got = lse[at].double().cpu()
+    assert torch.equal(torch.isinf(got), none) and (got[~none] - want_lse[~none]).abs().max().item() <= LSE
+    rest = [r for r in range(rows) if r not in set(at)]
+    assert (out[rest] == 7.0).all() and (lse[rest] == 7.0).all(), off
+
+
+def check_weights(b, off, seqs, rows, max_len):
+    n, chunks = len(seqs), live(off, rows)
+    q = seeded_normal((rows, 24, 256), 5)
+    lse = torch.full((rows, 24), float("nan"), device="cuda")
+    before = seeded_normal((len(b.lens), 4, b.pages.table.shape[1] * b.page), 9).abs()
+    want = before.double().cpu()
+    for i, a, e in chunks:
+        x, sums = log_sums(b, q[a:e], [seqs[i]], [e - a], max_len)
+        lse[a:e] = x.float().cuda()
+        if (i, a, e) in last_of(chunks, seqs):
+            m = min(b.lens[seqs[i]], max_len)
+            want[seqs[i], :, max(0, m - (e - a)):m] = 0.0
+            want[seqs[i], :, :m] += sums[0]
+    mass = before.clone()
+    weights(b, q, lse, off, n, rows, max_len, mass, seqs)
+    near(mass, want, f"{KV_NAMES[b.kvt]} {n} chunks, {len(chunks)} count")
+
+
+@pytest.mark.parametrize("n", [0, 64, 65, 130, 1024])
+@pytest.mark.parametrize("off, seqs", ODD, ids=str)
+def test_odd_offsets(gpu, off, seqs, n):
+    """Attention and weights, with as many empty chunks behind as make the wave's plan one of a workgroup; the prep's chunks
+    (test_prep_of_odd_offsets) are the same."""
+    b = Batch(ops.Q8_0, [40, 33, 70])
+    more = max(0, n - len(seqs))
+    off, seqs = off + [off[-1]] * more, seqs + [i % 3 for i in range(more)]
+    check_attention(b, off, seqs, 32, 70)
+    check_weights(b, off, seqs, 32, 70)
+
+
+@pytest.mark.parametrize("kvt", KVTS, ids=lambda k: KV_NAMES[k])
+def test_odd_offsets_of_many(gpu, kvt):
+    """The same of up to 64 chunks, and more, of which those of one or two tokens are walked by themselves."""
+    for n in (40, 64, 65, 130, 513):
+        rng, rows = random.Random(n), 3 * n
+        b = Batch(kvt, [3 + (i * 5) % 40 for i in range(n // 3 + 1)], page=16, ld=64)
+        seqs = [rng.randint(0, n // 3) for _ in range(n)]
+        off = some_offsets(n, rows, n)
+        check_attention(b, off, seqs, rows, (1024, 40)[n % 2])
+        check_weights(b, off, seqs, rows, 1024)
+        off[:4] = [rows, rows, 0, 3]  # an empty chunk at the end of the buffers first
+        check_attention(b, off, seqs, rows, 1024)
+        check_weights(b, off, seqs, rows, 1024)
