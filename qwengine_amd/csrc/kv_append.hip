@@ -536,8 +536,8 @@ __global__ void __launch_bounds__(64 * PB_WAVES) k_prep_rows_batch(
         if ((unsigned)page < (unsigned)pg.n_pages) slot = (long long)page * pg.page + pos % pg.page;
     }
     if (t < NROT / 2) rope_cs((double)pos + (rope_off ? rope_off[b] : 0), theta, t, &s_cs[t], &s_cs[t + NROT / 2]);
-    if (__syncthreads_or(overlaps)) return;
-    if (__syncthreads_or(later)) {
+    if (__syncthreads_or(overlaps || later)) {
+        if (__syncthreads_or(overlaps)) return;
         // Only a later one that counts takes this one's place: it must not begin before the furthest end ahead of it.
         const int lane = t & 63, wave = t >> 6;
         bool counts = false;
