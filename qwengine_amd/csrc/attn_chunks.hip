@@ -1288,7 +1288,7 @@ struct WeightsLds {
 // of its 32 rows, and the sums over them; the workgroup's sum of a tile is written while the next one is multiplied.  1000 tokens
 // over 16384 Q4_0 positions 460 to 490 us, 0.43 PFLOP/s, 0.85 with both parts of Q: of a SIMD's cycles 39% are MFMAs and 54% issue
 // VALU instructions (a block scale's product for each score and 32 dims, exponentials, sums over rows), which its two waves rarely
-// overlap; <Q8_0> keeps 16 registers in scratch, <Q4_0> 7.  16 tokens over 16000 F16 positions 109 us:
+// overlap; <Q8_0> keeps 15 registers in scratch, <Q4_0> 8.  16 tokens over 16000 F16 positions 109 us:
 // their keys' bytes at 4.8 TB/s.
 template <int KVT>
 __global__ void __launch_bounds__(64 * CW_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -1363,14 +1363,18 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         // last wave does it: of chunks of few tokens it is one that has no rows.
         const bool writes = wave == CW_WAVES - 1;
         float* const mass = a.mass + ((size_t)max(c.seq, 0) * NKV + g) * ((size_t)p.ld * p.page);
+        // (What no token sees is left as it is, a position without a place too; k_cw_join looks at the pages itself.)
         float old = 0.0f;
+        bool unseen = false;
         auto fetch = [&](int i) {
             const int key = (tb + i) * CW_TILE + lane;
-            if (writes && c.place < 0) old = key < c.len - c.count ? mass[key] : 0.0f;
+            if (!writes || c.place >= 0) return;
+            old = key < c.len - c.count ? mass[key] : 0.0f;
+            unseen = (lds.dead[i & 1] >> (lane >> 4)) & 1;
         };
         auto write = [&](int i) {
             const int key = (tb + i) * CW_TILE + lane;
-            if (!writes || key >= c.end) return;
+            if (!writes || key >= c.end || unseen) return;
             float v = 0.0f;
 #pragma unroll
             for (int k = 0; k < CW_WAVES; k++) v += lds.sum[i & 1][k][lane];
@@ -1457,7 +1461,8 @@ __global__ void __launch_bounds__(256) k_cw_join(WeightsArgs a, size_t ld_pos) {
             float v = 0.0f;
             for (int b = b0; b < nb; b++) v += a.parts[((size_t)(c.w + b) * NKV + g) * a.max_len + key];
             float* const m = a.mass + ((size_t)c.x * NKV + g) * ld_pos + key;
-            *m = key < c.y - c.z ? *m + v : v;
+            if (bt_place(a.src.p, a.src.p.table + (size_t)c.x * a.src.p.ld, key & ~15, c.y) >= 0)
+                *m = key < c.y - c.z ? *m + v : v;
         }
     }
 }
