@@ -1,5 +1,7 @@
 """The weights where their plan is made by a workgroup, and what they leave as it is.  Definition and tolerances as in
 test_gpu_weights."""
+import random
+
 import pytest
 import torch
 
@@ -7,7 +9,7 @@ import qwengine_amd.ops as ops
 from kvutil import KVTS, KV_NAMES, seeded_normal
 from test_gpu_attn_batch import Batch
 from test_gpu_chunks import offsets
-from test_gpu_weights import near, weights
+from test_gpu_weights import check, near, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +44,26 @@ def test_own_positions_without_a_place(gpu, kvt, tokens, n):
         left[s, :, :m] = gone[s]
     assert torch.equal(mass.cpu()[left].view(torch.int32), before.cpu()[left].view(torch.int32))
     near(mass, want, f"{KV_NAMES[kvt]} {tokens} tokens")
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 128, 129, 700])
+@pytest.mark.parametrize("kvt", KVTS, ids=lambda k: KV_NAMES[k])
+def test_numbers_of_chunks(gpu, kvt, n):
+    """Up to 64 chunks by a wave, 128 by two, more by a workgroup of 1024: chunks of none to 30 tokens, and between them some of
+    several blocks (43 tokens and up), whose sums are joined; sequences named twice, of which the last chunk with tokens counts."""
+    rng = random.Random(n)
+    counts = [rng.choice((0, 1, 2, rng.randint(3, 30))) for _ in range(n)]
+    for i, c in zip(rng.sample(range(n), 6), (42, 43, 85, 86, 130, 200)):
+        counts[i] = c
+    lens = [max(1, (i * 53) % 640) for i in range(n - n // 8)]
+    seqs = list(range(len(lens))) + rng.sample(range(len(lens)), n // 8)
+    rng.shuffle(seqs)
+    last = {s: i for i, s in enumerate(seqs) if counts[i] > 0}
+    check(Batch(kvt, lens, page=32), counts, seqs=seqs, pad=2, counted=set(last.values()))
+
+
+@pytest.mark.parametrize("kvt", KVTS, ids=lambda k: KV_NAMES[k])
+def test_few_chunks_of_many_blocks(gpu, kvt):
+    """More than 64 blocks of a few chunks, one of which is longer than its sequence, and one of one block."""
+    check(Batch(kvt, [1200, 700, 900, 333]), [1000, 800, 900, 40], pad=1)
+    check(Batch(kvt, [1200, 700, 900, 333]), [1000, 800, 900, 40], seqs=[0, 1, 0, 3], counted=[1, 2, 3])
