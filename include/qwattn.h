@@ -300,8 +300,12 @@ size_t qwa_attn_weights_batch_work_bytes(int n, int rows, int max_len);
  * [n_seq][4][ld * page]); the chunk's own positions, which are new, begin with it.  Chunks of one token do for decoded
  * tokens.  q, lse: those of the qwa_attn_prefill_batch call of the same chunks (of all its tokens, or with other offsets of its
  * last ones, the positions that the sequences hold then ending with them).  Rows that see no position add nothing; entries of
- * positions past a sequence's last one, and of positions that no token sees, are left as they are.  Scores are exact up to
- * fp32 accumulation, all sums fp32 in a fixed order.  Of several chunks of one sequence the last one counts.
+ * positions past a sequence's last one, and of positions that no token sees, are left as they are.
+ * Every other position that a token sees has what it had added to, also one that is new but none of the chunk's: before a window
+ * of a chunk's last tokens, or of tokens whose weights were not taken.  The caller clears those: trims and evictions leave the
+ * entries past a sequence's end as they were, and forks do not copy any.
+ * Scores are exact up to fp32 accumulation, all sums fp32 in a fixed order.  Of several chunks of one sequence the last one that
+ * has tokens counts.
  * n <= QWA_PAGES_MAXN; max_len as for qwa_attn_prefill_batch; q, work and the pool 16-byte aligned; work of at least
  * qwa_attn_weights_batch_work_bytes bytes, not shared with a call that may run at the same time. */
 int qwa_attn_weights_batch(const float* q, const float* lse, const qwa_kv_layer* kv, int kvt, const qwa_kv_pages* p,
@@ -314,8 +318,8 @@ size_t qwa_kv_pages_evict_work_bytes(const qwa_kv_pages* p, int n, int n_layers,
 /* Cuts sequence seqs[i] (device arrays of n entries) to keep[i] <= max_keep positions, if it has more: each KV head of each layer
  * keeps its last min(recent, keep[i]) positions and, of the others, those of the largest weight in mass (fp32, device, 16-byte
  * aligned, [n_layers][n_seq][4][ld * page], as qwa_attn_weights_batch gathers it), the lower position of equal ones, NaN last.
- * The kept positions move to the front in their order, in every layer of `layers` and in mass; heads and layers keep
- * different positions.  The sequence's length becomes keep[i]; the pages past that are given back.  Pages of the kept part that
+ * The kept positions move to the front in their order, in every layer of `layers` and in mass, whose entries from keep[i] on stay
+ * as they are; heads and layers keep different positions.  The sequence's length becomes keep[i]; the pages past that are given back.  Pages of the kept part that
  * other sequences hold too are left to them and replaced by free ones, lowest first, request by request.  dropped[i] (device)
  * becomes the number of positions that went: keys carry their rotary position with them, so for the sequence's next tokens
  * the preps' rope_off grows by it.  All or nothing: *status (device) becomes 0 when done; the number of missing pages when
