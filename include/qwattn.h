@@ -324,8 +324,8 @@ size_t qwa_kv_pages_evict_work_bytes(const qwa_kv_pages* p, int n, int n_layers,
  * becomes the number of positions that went: keys carry their rotary position with them, so for the sequence's next tokens
  * the preps' rope_off grows by it.  All or nothing: *status (device) becomes 0 when done; the number of missing pages when
  * the free ones do not suffice; -(i + 1) when request i is invalid (no such sequence, named before, keep outside
- * [0, max_keep]; or a broken table: a length outside [0, ld * page], a page that is none of the pool's).  In the last two cases
- * nothing is changed, and dropped is 0.
+ * [0, max_keep]; or a broken table: a length outside [0, ld * page], or, of one that is cut, a page that is none of the
+ * pool's).  In the last two cases nothing is changed, and dropped is 0.
  * work: at least qwa_kv_pages_evict_work_bytes bytes, one for each call or captured graph that may run at the same time. */
 int qwa_kv_pages_evict(const qwa_kv_pages* p, const int* seqs, const int* keep, int n, int recent, int max_keep,
                        const qwa_kv_layer* layers, int n_layers, int kvt, float* mass, int* dropped, int* status, void* work,

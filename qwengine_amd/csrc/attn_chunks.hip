@@ -18,9 +18,11 @@
 //    into LDS, two tiles ahead.
 //  * Scores are exact up to fp32 accumulation (K as its codes, Q / 16 as the sum of two fp16 parts), as the batched decode's are;
 //    the arithmetic of a tile, of V that is not finite and of the probabilities' range is paged_tiles.hpp's.
-// Roundings below 32 bits: the dequantized V (d * code) and the probabilities are fp16, half a step 2^-11 of the value; the sum of
-// a row's probabilities is that of the rounded ones, which P V applies, but the log of the sum is taken of the unrounded.  The
-// output is fp16.
+// Roundings below 32 bits: the dequantized V (d * code) and the probabilities are fp16, half a step 2^-11 of the value, because the
+// matrix instructions take fp16.  Exact ones would need a second product for the low parts, or, of V, one with P * d for each
+// block of 32 dims; as they are, errors against 64 bits are 2.1e-4 of the norm over F16, which is the output's own rounding, and
+// 2.6e-4 to 3.1e-4 over the quantized types.  The sum of a row's probabilities is that of the rounded ones, which P V applies, but
+// the log of the sum is taken of the unrounded.  The output is fp16.
 #include <algorithm>
 #include <type_traits>
 
@@ -218,7 +220,9 @@ __global__ void __launch_bounds__(CH_PT) k_ch_plan(ChunkSource src, int most, in
     }
 }
 
-// (a thread a chunk; fewer waves wait less at its barriers: 24 chunks 7.0 us with 128 threads, 9.4 with 1024)
+// (a thread a chunk; fewer waves wait less at its barriers: 24 chunks 7.0 us with 128 threads, 9.4 with 1024.  With many blocks it
+// goes through more rounds, 25 instead of 4 for 128 chunks of 512 tokens, which is 8 us of a call of 1770; 128 chunks of 8 tokens
+// 54.4 / 56.6, of 64 170.9 / 170.6)
 constexpr int CH_PLAN_FEW = 128;
 template <bool WEIGHTS>
 void launch_plan(const ChunkSource& src, int most, int most_list, int room, ChunkBlock* blocks, int4* list, int* head,
@@ -389,7 +393,7 @@ __device__ __forceinline__ ChunkBlock ch_block(const ChunkBlock& c) {
 }
 
 // The images: a workgroup of 512 threads converts a tile of one KV head, half of them K, half V, from registers to memory.  What it
-// writes bounds it: 33792 Q8_0 positions (144 MB of images) 37 us.
+// writes bounds it: 33792 Q8_0 positions (151 MB of images) 37 us.
 constexpr int CH_IMG_WGS = 2048;
 template <int KVT>
 __global__ void __launch_bounds__(512) k_ch_image(ChunkArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
@@ -1007,7 +1011,7 @@ struct ChunkShared {
 // conflicts; the value waves are the longer chain: copies' issue and exponents 1200 cycles, exponentials 900, P V 750 and 500
 // between them, of 3400 to 3800 a tile.  Without the images' copies a tile took 1.4 us, the copies alone 1.2 (7.3 TB/s of images,
 // which the L2s miss: a head's workgroups are spread over the positions).  A segment costs about 8 tiles besides: Q's way in and,
-// longer, O's way out with the gates.  Six prompts of up to 1021 F16 tokens, 136 to 152 us, move 0.5 GB of Q, gates, outputs and
+// longer, O's way out with the gates.  Six prompts of up to 1021 F16 tokens, 136 to 152 us, move 0.36 GB of Q, gates, outputs and
 // states meanwhile.  Measured and not kept, none with a difference: Q three loads ahead, the next block's description in LDS, rows'
 // addresses without divisions, the exponents' reads before the copies, the score waves at a higher priority; slower: raw tiles for
 // long chunks (1450), the value waves at a higher priority (1365).
@@ -1286,10 +1290,11 @@ struct WeightsLds {
 
 // A workgroup walks the 64-key tiles of a slice as k_ch_tiles does, with K alone: all waves convert it, then each takes the scores
 // of its 32 rows, and the sums over them; the workgroup's sum of a tile is written while the next one is multiplied.  1000 tokens
-// over 16384 Q4_0 positions 460 to 490 us, 0.43 PFLOP/s, 0.85 with both parts of Q: of a SIMD's cycles 39% are MFMAs and 54% issue
-// VALU instructions (a block scale's product for each score and 32 dims, exponentials, sums over rows), which its two waves rarely
-// overlap; <Q8_0> keeps 15 registers in scratch, <Q4_0> 8.  16 tokens over 16000 F16 positions 109 us:
-// their keys' bytes at 4.8 TB/s.
+// over 16384 Q4_0 positions 460 to 520 us, 0.43 PFLOP/s, 0.85 with both parts of Q: of a SIMD's cycles 39% are MFMAs and 54% issue
+// VALU instructions (a block scale's product for each score and 32 dims, exponentials, sums over rows, and K's conversion, which
+// each of its 24 blocks does for itself), which its two waves, at the same step of a tile, rarely overlap; <Q8_0> keeps 15 registers
+// in scratch, <Q4_0> 8.  A token in each of 16 sequences of 6000 to 16000 positions: F16 108 us, 367 MB at 3.4 TB/s, Q8_0 117,
+// Q4_0 109.  What the three types have in common there is a tile's chain: conversion, a barrier, scores by two of eight waves.
 template <int KVT>
 __global__ void __launch_bounds__(64 * CW_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
 k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
@@ -1324,8 +1329,8 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
         const ChunkBlock c = ch_block(blocks[j]);
         const int tb = s - c.begin, nt = min(s_end, c.begin + c.tiles) - s;
         const int nrows = GRP * c.count;
-        // (a block of one wave's rows: two waves have them, and half of the keys each; 16 tokens over 16000 F16 positions 109 us
-        // instead of 136)
+        // (a block of one wave's rows: two waves have them, and half of the keys each; 16 tokens over 6000 to 16000 F16 positions
+        // 109 us instead of 136)
         const bool few = nrows <= 32;
         const int wrow0 = few ? 0 : CW_ROWS * c.blk + 32 * wave;
         const bool rows_here = few ? wave < 2 : wrow0 < nrows;
@@ -1447,7 +1452,7 @@ k_cw_tiles(WeightsArgs a, qwa_kv_layer kv, qwa_kv_pages p) {
     }
 }
 
-// The weights of chunks of several blocks: the blocks' sums in order (24 blocks of 17384 positions, 40 MB, 16 us).
+// The weights of chunks of several blocks: the blocks' sums in order (24 blocks of 17384 positions, 6.7 MB, 16 us).
 __global__ void __launch_bounds__(256) k_cw_join(WeightsArgs a, size_t ld_pos) {
     __shared__ OwnPlan plan;
     if (a.own) ch_own_plan<true>(plan, a.src);

@@ -17,10 +17,16 @@ constexpr int CH_ROWS = 32 * CH_PAIRS;      // rows (token, head of the group) o
 constexpr int CH_SLICES = 256 / NKV;        // workgroups of a KV head: one round of the chip's 256 CUs
 
 // Chunks of at least CH_IMG_BLOCKS blocks read their keys as images: tiles that k_ch_image has brought into the form of LDS once,
-// instead of every block by itself.  Images take 4 times the bytes of a Q8_0 cache, so there is room for CH_IMG_TILES tiles (of
-// each KV head) or one sequence, whichever is more, and chunks that find none left do without.  Chunks at 8000 positions, us, with /
-// without images: 100 tokens (5 blocks) F16 83 / 69, Q8_0 84 / 76, Q4_0 84 / 76; 4 of 200 (10 blocks) 271 / 249, 284 / 299, 287 /
-// 298; 1000 tokens (47) 259 / 275, 279 / 331, 280 / 330.
+// instead of every block by itself.  An image is 35840 bytes, 1.1 times what its tile takes in an F16 cache, 2.1 times Q8_0, 3.9 times
+// Q4_0.  There is room for CH_IMG_TILES tiles (of each KV head: 587 MB) or one sequence, whichever is more, as far as the rows
+// allow, and chunks that find none left do without.  The bound is one for all types, about where the quantized ones break even;
+// of F16, which has nothing to convert, chunks of 12 to 23 blocks lose up to a tenth by it.  One chunk at 8000 positions, whole
+// call, us, with / without images:
+//   blocks      6            8            10             12             16             24
+//   F16     85.2 / 74.2  92.6 / 84.1  100.2 / 91.3   115.1 / 105.5  129.1 / 124.4  170.0 / 169.3
+//   Q8_0    85.8 / 80.4  97.1 / 94.4  103.6 / 102.9  116.3 / 116.2  132.0 / 140.0  175.0 / 191.9
+//   Q4_0    86.3 / 82.1  96.2 / 95.5  102.0 / 103.7  113.5 / 116.4  130.9 / 138.7  171.2 / 190.1
+// Four chunks of 12 blocks 332 / 320, 343 / 358, 339 / 356; of 24 blocks 589 / 629, 629 / 711, 603 / 692.
 constexpr int CH_IMG_BLOCKS = 12;
 constexpr int CH_IMG_TILES = 4096;
 struct ChunkImage {

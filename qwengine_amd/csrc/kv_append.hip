@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(64 * PB_WAVES) k_prep_batch(
 
 // The same for chunks of any number of tokens: batch row b has rows off[b] .. off[b + 1] - 1, the last positions of its
 // sequence.  The workgroup's threads look for its row in `off` a chunk each (a binary search would be ten round trips).  A stream
-// of its rows: 3540 tokens, 306 MB read and written, 56 us (5.5 TB/s, where a large copy has 5.1); 40 tokens 6.7 us, a chain of
+// of its rows: 2840 tokens, 306 MB read and written, 56 us (5.5 TB/s, where a large copy has 5.1); 40 tokens 6.7 us, a chain of
 // round trips (offsets, length, page).
 template <int KVT>
 __global__ void __launch_bounds__(64 * PB_WAVES) k_prep_rows_batch(

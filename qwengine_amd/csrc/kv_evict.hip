@@ -62,10 +62,11 @@ __device__ __forceinline__ uint32_t ev_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// A workgroup reads its weights once, into registers, and is then bound by its own instructions and barriers: of 36 us for 32768
-// positions (64 workgroups) the weights and the first histogram take 7, a histogram's search and the next one 4 to 5 each, counting
-// what stays 7, writing it 7.  Measured and as fast: neighbouring positions over a wave's lanes instead of in a thread's
-// registers (and places by ballots); slower (42): the first 11 bits by counting bit by bit.
+// A workgroup reads up to EV_T * EV_E weights once, into registers (more of them once for each histogram and once for what stays), and
+// is then bound by its own instructions and barriers: of 36 us for 32768 positions (64 workgroups) the weights and the first
+// histogram take 7, a histogram's search and the next one 4 to 5 each, counting what stays 7, writing it 7.  Measured and as fast:
+// neighbouring positions over a wave's lanes instead of in a thread's registers (and places by ballots); slower (42): the first 11
+// bits by counting bit by bit.
 __global__ void __launch_bounds__(EV_T) k_evict_select(EvictArgs a) {
     __shared__ __attribute__((aligned(16))) int s_hist[EV_BINS];
     __shared__ long long s_wave[EV_T / 64];
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(EV_T) k_evict_plan(EvictArgs a, int* __restric
 
 // The rows of a request, layer and head, of K or V.  While a run is written, the next one is on its way, and the places of that after
 // it.  The order of the rows binds a workgroup, but their columns do not depend on each other: of F16 each of four workgroups has
-// 128 bytes of a row (6 sequences of 8000 cut to 2000 in 16 layers, 1.57 GB: 310 us, 5.1 TB/s, the copy rate; whole rows 349).
+// 128 bytes of a row (6 sequences of up to 8000 cut to 2000 or less in 16 layers, 1.41 GB: 310 us, 4.5 TB/s; whole rows 349).
 // Rows of the quantized types, of 256 and 128 bytes, stay whole (one Q4_0 document of 32768 cut to 4096 in 16 layers: 51 us, in four
 // parts 52; 151 MB, but a row's 16 bytes of scales are read as a line of 128, 0.21 GB; two Q8_0 of 600 to 256 10, in parts 12).
 constexpr int EV_MT = 512;  // threads
