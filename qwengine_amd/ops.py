@@ -666,7 +666,8 @@ def attn_weights_batch(q, lse, kv: KVLayer, kvt, pages: KVPages, seqs, off, n: i
     """Adds the attention weight that a layer's positions gather from the chunks' tokens (summed over the 6 query heads of each KV
     head) to mass (float32 [n_seq, 4, ld * page]); a chunk's own positions begin with it.  q and lse are those of the chunks'
     attn_prefill_batch call.  Where new positions are not all of them a chunk's (a window of a step's last tokens), clear what
-    is past the lengths before the step: mass.masked_fill_(torch.arange(ld * page) >= pages.len[:, None, None], 0.0)."""
+    is past the lengths before the step:
+    mass.masked_fill_(torch.arange(mass.shape[-1], device=mass.device) >= pages.len[:, None, None], 0.0)."""
     f32, kvt, pc = torch.float32, _kvt(kvt), pages.c()
     _check(lib().qwa_attn_weights_batch(
         _dev(q, f32, "q", rows * 6144), _dev(lse, f32, "lse", rows * N_HEAD), _pool(kv, kvt), kvt, ctypes.byref(pc),
